@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define SGL_ABI_VERSION 23
+#define SGL_ABI_VERSION 24
 
 #define SGL_OK 0
 #define SGL_ERR_INVALID 1   /* bad argument (host-checked) */
@@ -851,6 +851,118 @@ int sgl_plan_run(const sgl_op *ops, int32_t n_front, int32_t n_back,
                  hipStream_t front, hipStream_t back, uint32_t *sync,
                  uint32_t seq, uint32_t need_back, int32_t timed_op,
                  hipEvent_t t_start, hipEvent_t t_end);
+
+/* ---------------------------------------------------------------------------
+ * History operators: a sequence encoder over windows of events (no reference
+ * counterpart; models.py:77-137 attends with one query row over the window).
+ * Element types of the tensors given as void *:
+ * ------------------------------------------------------------------------- */
+#define SGL_FP32 0
+#define SGL_BF16 1
+#define SGL_FP16 2
+
+/* Gated linear recurrence over N sequences of up to L events of D channels:
+ *   a = s(gate) exp(-decay gaps),  h_t = a_t h_{t-1} + (1 - a_t) value_t
+ * (without gaps and decay a = s(gate)), s the logistic function. gate and
+ * value: element (n, t, d) at n * gate_n + t * gate_t + d (strides in
+ * elements), h [N, L, D]. lens int32 [N] (clamped to [0, L]; NULL: all L):
+ * events past a sequence's length are not read and their h is 0. state fp32
+ * [N, D] (NULL: 0), last fp32 [N, D] (may be NULL): the state after each
+ * sequence's last event. gaps fp32 at n * gaps_n + t * gaps_t, decay fp32 [D].
+ * keep (may be NULL): sgl_gated_scan_keep_elems floats that the backward
+ * reads. Nothing is launched for N = 0 or L = 0. `last` may be `state` itself
+ * when L = 1. */
+int64_t sgl_gated_scan_keep_elems(int64_t N, int64_t L, int32_t D);
+size_t sgl_gated_scan_workspace_bytes(int32_t dtype, int64_t N, int64_t L,
+                                      int32_t D, int32_t backward,
+                                      int32_t decay);
+int sgl_gated_scan_forward(int32_t dtype, int64_t N, int64_t L, int32_t D,
+                           const void *gate, int64_t gate_n, int64_t gate_t,
+                           const void *value, int64_t value_n, int64_t value_t,
+                           const int32_t *lens, const float *state,
+                           const float *gaps, int64_t gaps_n, int64_t gaps_t,
+                           const float *decay, void *h, float *last,
+                           float *keep, void *workspace,
+                           size_t workspace_bytes, hipStream_t stream);
+/* gh [N, L, D] (NULL: 0), glast fp32 [N, D] (NULL: 0) -> dgate, dvalue
+ * [N, L, D] (0 past a length), dstate fp32 [N, D] (may be NULL), ddecay fp32
+ * [D] (with decay). */
+int sgl_gated_scan_backward(int32_t dtype, int64_t N, int64_t L, int32_t D,
+                            const void *gate, int64_t gate_n, int64_t gate_t,
+                            const void *value, int64_t value_n,
+                            int64_t value_t, const int32_t *lens,
+                            const float *state, const float *gaps,
+                            int64_t gaps_n, int64_t gaps_t, const float *decay,
+                            const float *keep, const void *gh,
+                            const float *glast, void *dgate, void *dvalue,
+                            float *dstate, float *ddecay, void *workspace,
+                            size_t workspace_bytes, hipStream_t stream);
+
+/* Attention of the rows of n sequences of up to lq query events over up to lk
+ * key events, heads_q query heads sharing heads_kv key heads, each of
+ * head_dim <= 128 elements, with a bias table over time distances. Tensors are
+ * addressed by strides in elements, the last dimension contiguous. q_lens,
+ * k_lens: int32 [n] (clamped; NULL: all). key_mask: bytes, 0 a dead key.
+ * bias: fp32 [heads_q][buckets, or 2 buckets if two_sided] (at most 64
+ * columns; NULL: none), with 2^resolution (0 to 4) buckets an octave of
+ * |q_pos - k_pos|; the second half is for q_pos < k_pos, which a one-sided
+ * table counts as distance 0. Distances from 2^32 on count as 2^32 - 1. */
+typedef struct sgl_attention {
+  int32_t dtype, heads_q, heads_kv, head_dim;
+  int64_t n, lq, lk;
+  int64_t q_n, q_t, q_h, k_n, k_t, k_h, v_n, v_t, v_h;
+  const void *q, *k, *v;
+  const int32_t *q_lens, *k_lens;
+  const uint8_t *key_mask;
+  int64_t mask_n, mask_t;
+  const float *bias;
+  int32_t buckets, resolution, two_sided;
+  float scale;
+  const int64_t *q_pos, *k_pos;
+  int64_t qpos_n, qpos_t, kpos_n, kpos_t;
+} sgl_attention;
+
+/* o [n, lq, heads_q, head_dim]; lse fp32 [n, heads_kv, lq * heads_q /
+ * heads_kv] (what the backward reads). Rows past a query length and rows
+ * without a live key are 0. The problem struct is HOST memory. */
+size_t sgl_cross_attention_workspace_bytes(const sgl_attention *problem,
+                                           int32_t backward);
+int sgl_cross_attention_forward(const sgl_attention *problem, void *o,
+                                float *lse, void *workspace,
+                                size_t workspace_bytes, hipStream_t stream);
+/* go like o -> dq like o, dk and dv [n, lk, heads_kv, head_dim], dbias fp32
+ * like the table (NULL: not computed). */
+int sgl_cross_attention_backward(const sgl_attention *problem, const void *o,
+                                 const float *lse, const void *go, void *dq,
+                                 void *dk, void *dv, float *dbias,
+                                 void *workspace, size_t workspace_bytes,
+                                 hipStream_t stream);
+
+/* y = x + scale * s(gate) * Norm(z; post), n = Norm(y; pre) over rows of D <=
+ * 8192 values: Norm(t) = (t - mean) / sqrt(var + eps) * w + b, with rms != 0
+ * t / sqrt(mean(t^2) + eps) * w + b. x, z and gate rows sx, sz, sg elements
+ * apart; y, n and all gradients contiguous; scale fp32 [D]; the norms' weights
+ * and biases fp32 [D] (NULL: 1 and 0). */
+int sgl_gated_norm_forward(int32_t dtype, int64_t rows, int32_t D,
+                           const void *x, int64_t sx, const void *z,
+                           int64_t sz, const void *gate, int64_t sg,
+                           const float *scale, const float *post_w,
+                           const float *post_b, const float *pre_w,
+                           const float *pre_b, float eps, int32_t rms, void *y,
+                           void *n, hipStream_t stream);
+size_t sgl_gated_norm_workspace_bytes(int64_t rows, int32_t D);
+/* gy, gn (either may be NULL: 0) -> dx, dz, dgate and dparams fp32 [nsum][D]:
+ * the gradients of scale, post_w, pre_w (nsum 3) and post_b, pre_b (nsum 5). */
+int sgl_gated_norm_backward(int32_t dtype, int64_t rows, int32_t D,
+                            const void *x, int64_t sx, const void *z,
+                            int64_t sz, const void *gate, int64_t sg,
+                            const float *scale, const float *post_w,
+                            const float *post_b, const float *pre_w,
+                            const float *pre_b, float eps, int32_t rms,
+                            const void *gy, const void *gn, void *dx, void *dz,
+                            void *dgate, float *dparams, int32_t nsum,
+                            void *workspace, size_t workspace_bytes,
+                            hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -17,7 +17,7 @@ import torch  # loads the HIP runtime first, so the library binds to the same on
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libstarrygl_mi355x.so"
 LIB_PATH = os.path.join(_HERE, LIB_NAME)
-ABI_VERSION = 23
+ABI_VERSION = 24
 
 SGL_DERR_NODE_RANGE = 1
 SGL_DERR_EID_RANGE = 2
@@ -27,6 +27,7 @@ SGL_DONE_WORDS = 1088   # int32 words of sgl_predictor's completion counter
 SGL_DONE_RANGE_WORD = 32   # its word that flags a value outside the fixed-point range
 SGL_COMPACT_NOALLOC_MAX_QUERIES = 1 << 24   # sgl_recent_compact_noalloc's limit
 SGL_LINK_METRICS_MAX_SCORES = 8192   # sgl_link_metrics' limit on positive + negative scores
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # SGL_FP32, SGL_BF16, SGL_FP16
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -36,6 +37,11 @@ _sz = ctypes.c_size_t
 # the attention's dropout arguments: p_att, p_out, seed, rng_step, pass, sv_sdrop
 _DROP = [ctypes.c_float, ctypes.c_float, ctypes.c_uint64, _vp, _i32, _vp]
 _DROPS = [*_DROP[:-1], _i32, _DROP[-1]]   # the several-pass calls: npass after pass
+
+# the gated scan's inputs: gate, value, lens, state, gaps, decay with their strides
+_SCAN = [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp]
+# the gated norm's: x, z, gate with their row strides, the weights, eps, rms
+_NORM = [_vp, _i64] * 3 + [_vp] * 5 + [ctypes.c_float, _i32]
 
 # name -> (restype, argtypes); mirrors include/starrygl_mi355x.h
 SIGNATURES: dict[str, tuple] = {
@@ -98,6 +104,16 @@ SIGNATURES: dict[str, tuple] = {
                       + [_vp, _vp]),
     "sgl_grad_shadows": (ctypes.c_int, [_vp, _vp, _i32, _vp, _vp, _vp]),
     "sgl_adam_coef": (ctypes.c_int, [_i32] + [_vp] * 3 + [ctypes.c_float] * 3 + [_vp] * 3),
+    "sgl_gated_scan_keep_elems": (_i64, [_i64, _i64, _i32]),
+    "sgl_gated_scan_workspace_bytes": (_sz, [_i32, _i64, _i64, _i32, _i32, _i32]),
+    "sgl_gated_scan_forward": (ctypes.c_int, [_i32, _i64, _i64, _i32] + _SCAN + [_vp] * 4 + [_sz, _vp]),
+    "sgl_gated_scan_backward": (ctypes.c_int, [_i32, _i64, _i64, _i32] + _SCAN + [_vp] * 8 + [_sz, _vp]),
+    "sgl_cross_attention_workspace_bytes": (_sz, [_vp, _i32]),
+    "sgl_cross_attention_forward": (ctypes.c_int, [_vp] * 4 + [_sz, _vp]),
+    "sgl_cross_attention_backward": (ctypes.c_int, [_vp] * 9 + [_sz, _vp]),
+    "sgl_gated_norm_workspace_bytes": (_sz, [_i64, _i32]),
+    "sgl_gated_norm_forward": (ctypes.c_int, [_i32, _i64, _i32] + _NORM + [_vp] * 3),
+    "sgl_gated_norm_backward": (ctypes.c_int, [_i32, _i64, _i32] + _NORM + [_vp] * 6 + [_i32, _vp, _sz, _vp]),
 }
 
 _lock = threading.Lock()
@@ -205,6 +221,16 @@ class Bf16Weights(ctypes.Structure):
     """struct sgl_bf16_weights of include/starrygl_mi355x.h."""
     _fields_ = [(n, _vp) for n in ("wq", "wk", "wv", "wout", "wkt", "wvt", "wot", "ws", "wd", "wst", "wdt")] + \
                [(n, _i32) for n in ("ld_q", "ld_c", "ld_o", "ld_h", "hp", "ld_d")]
+
+
+class Attention(ctypes.Structure):
+    """struct sgl_attention of include/starrygl_mi355x.h."""
+    _fields_ = [(n, _i32) for n in ("dtype", "heads_q", "heads_kv", "head_dim")] + \
+               [(n, _i64) for n in ("n", "lq", "lk", "q_n", "q_t", "q_h", "k_n", "k_t", "k_h", "v_n", "v_t", "v_h")] + \
+               [(n, _vp) for n in ("q", "k", "v", "q_lens", "k_lens", "key_mask")] + \
+               [("mask_n", _i64), ("mask_t", _i64), ("bias", _vp)] + \
+               [(n, _i32) for n in ("buckets", "resolution", "two_sided")] + [("scale", ctypes.c_float)] + \
+               [("q_pos", _vp), ("k_pos", _vp)] + [(n, _i64) for n in ("qpos_n", "qpos_t", "kpos_n", "kpos_t")]
 
 
 SGL_OP_MAX_ARGS = 64
