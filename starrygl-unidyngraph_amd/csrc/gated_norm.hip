@@ -60,8 +60,8 @@ __device__ __forceinline__ float row_sum(float v, float *s_red, int &slot) {
 template <typename T, int V, int NV, int LPR>
 struct Row {
   static constexpr int E = V * NV;
-  static constexpr int RPB = LPR >= 256 ? 1 : 256 / LPR;   // rows of a workgroup at a time
-  static constexpr int BLOCK = LPR >= 256 ? LPR : 256;
+  static constexpr int RPB = LPR > kWave ? 1 : 256 / LPR;   // rows of a workgroup at a time
+  static constexpr int BLOCK = LPR > kWave ? LPR : 256;
 
   static __device__ __forceinline__ void load(float (&r)[E], const T *p, int lane, int D) {
 #pragma unroll
@@ -146,37 +146,28 @@ __global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK)) void k_norm_fwd(NormAr
   int slot = 0;
   const int lane = threadIdx.x % LPR;
   const float inv = 1.f / float(a.D);
+  float al[E], pw[E], pb[E], nw[E], nb[E];
+  R::weight(al, a.scale, 0.f, lane, a.D);
+  R::weight(pw, a.post_w, 1.f, lane, a.D);
+  R::weight(pb, a.post_b, 0.f, lane, a.D);
+  R::weight(nw, a.pre_w, 1.f, lane, a.D);
+  R::weight(nb, a.pre_b, 0.f, lane, a.D);
   for (int64_t r = int64_t(blockIdx.x) * R::RPB + threadIdx.x / LPR; r < a.rows; r += int64_t(gridDim.x) * R::RPB) {
-    float x[E], z[E], g[E], w[E];
-    R::load(x, static_cast<const T *>(a.x) + r * a.sx, lane, a.D);
+    float x[E], z[E], g[E];
     R::load(z, static_cast<const T *>(a.z) + r * a.sz, lane, a.D);
+    R::load(x, static_cast<const T *>(a.x) + r * a.sx, lane, a.D);
     R::load(g, static_cast<const T *>(a.gate) + r * a.sg, lane, a.D);
     R::standard(z, lane, a.D, inv, a.eps, a.rms, s_red, slot);
-    R::weight(w, a.post_w, 1.f, lane, a.D);
-#pragma unroll
-    for (int e = 0; e < E; ++e) z[e] *= w[e];
-    if (a.post_b != nullptr) {
-      R::weight(w, a.post_b, 0.f, lane, a.D);
-#pragma unroll
-      for (int e = 0; e < E; ++e) z[e] += w[e];
-    }
-    R::weight(w, a.scale, 0.f, lane, a.D);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       float s, sn;
       sgl::sigmoid_pair(g[e], s, sn);
-      x[e] += w[e] * s * z[e];
+      x[e] += al[e] * s * (z[e] * pw[e] + pb[e]);
     }
     R::store(y + r * a.D, x, lane, a.D);
     R::standard(x, lane, a.D, inv, a.eps, a.rms, s_red, slot);
-    R::weight(w, a.pre_w, 1.f, lane, a.D);
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] *= w[e];
-    if (a.pre_b != nullptr) {
-      R::weight(w, a.pre_b, 0.f, lane, a.D);
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] += w[e];
-    }
+    for (int e = 0; e < E; ++e) x[e] = x[e] * nw[e] + nb[e];
     R::store(n + r * a.D, x, lane, a.D);
   }
 }
@@ -195,13 +186,18 @@ __global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK)) void k_norm_bwd(NormAr
   int slot = 0;
   const int lane = threadIdx.x % LPR;
   const float inv = 1.f / float(a.D);
+  float al[E], pw[E], pb[E], nw[E];
+  R::weight(al, a.scale, 0.f, lane, a.D);
+  R::weight(pw, a.post_w, 1.f, lane, a.D);
+  R::weight(pb, a.post_b, 0.f, lane, a.D);
+  R::weight(nw, a.pre_w, 1.f, lane, a.D);
   float sums[5][E];
 #pragma unroll
   for (int k = 0; k < 5; ++k)
 #pragma unroll
     for (int e = 0; e < E; ++e) sums[k][e] = 0.f;
   for (int64_t r = int64_t(blockIdx.x) * R::RPB + threadIdx.x / LPR; r < a.rows; r += int64_t(gridDim.x) * R::RPB) {
-    float x[E], z[E], g[E], q[E], u[E], w[E];
+    float x[E], z[E], g[E], q[E], u[E];
     R::load(x, static_cast<const T *>(a.x) + r * a.sx, lane, a.D);
     R::load(z, static_cast<const T *>(a.z) + r * a.sz, lane, a.D);
     R::load(g, static_cast<const T *>(a.gate) + r * a.sg, lane, a.D);
@@ -219,10 +215,6 @@ __global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK)) void k_norm_bwd(NormAr
     }
     // y again
     const float zr = R::standard(z, lane, a.D, inv, a.eps, a.rms, s_red, slot);
-    float pw[E], pb[E], al[E];
-    R::weight(pw, a.post_w, 1.f, lane, a.D);
-    R::weight(pb, a.post_b, 0.f, lane, a.D);
-    R::weight(al, a.scale, 0.f, lane, a.D);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       float s, sn;
@@ -231,12 +223,11 @@ __global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK)) void k_norm_bwd(NormAr
     }
     const float yr = R::standard(x, lane, a.D, inv, a.eps, a.rms, s_red, slot);
     // the pre norm
-    R::weight(w, a.pre_w, 1.f, lane, a.D);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       sums[2][e] += u[e] * x[e];
       sums[4][e] += u[e];
-      u[e] *= w[e];
+      u[e] *= nw[e];
     }
     R::through(u, x, yr, inv, a.rms, s_red, slot);
     // the residual, the gate and the scale
@@ -261,7 +252,7 @@ __global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK)) void k_norm_bwd(NormAr
   }
   // the workgroup's rows (RPB of them at a time) into one row of sums
   if constexpr (R::RPB > 1) {
-    __shared__ float s_sum[LPR * E * (256 / LPR)];
+    __shared__ float s_sum[R::RPB * LPR * E];
 #pragma unroll
     for (int k = 0; k < 5; ++k) {
       if (k >= nsum) break;
@@ -292,7 +283,7 @@ __global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK)) void k_norm_bwd(NormAr
   }
 }
 
-constexpr unsigned kFwdGrid = 2048, kBwdGrid = 1024;
+constexpr unsigned kFwdGrid = 1536, kBwdGrid = 1024;
 
 unsigned norm_grid(int64_t rows, int rpb, unsigned most) {
   return unsigned(std::max<int64_t>(1, std::min<int64_t>((rows + rpb - 1) / rpb, most)));
@@ -314,8 +305,7 @@ int run_norm(const NormArgs &a, const void *gy, const void *gn, void *o1, void *
   return int(grid);
 }
 
-// Lanes a row: as few as hold it in one vector each up to a wave, then a
-// wave with two, then workgroups.
+// Lanes a row: as few as hold it in one vector each.
 template <typename T, int V>
 int pick_norm(const NormArgs &a, const void *gy, const void *gn, void *o1, void *o2, void *o3, float *part, int nsum,
               bool back, hipStream_t s) {
@@ -323,7 +313,7 @@ int pick_norm(const NormArgs &a, const void *gy, const void *gn, void *o1, void 
   if (u <= 16) return run_norm<T, V, 1, 16>(a, gy, gn, o1, o2, o3, part, nsum, back, s);
   if (u <= 32) return run_norm<T, V, 1, 32>(a, gy, gn, o1, o2, o3, part, nsum, back, s);
   if (u <= 64) return run_norm<T, V, 1, 64>(a, gy, gn, o1, o2, o3, part, nsum, back, s);
-  if (u <= 128) return run_norm<T, V, 2, 64>(a, gy, gn, o1, o2, o3, part, nsum, back, s);
+  if (u <= 128) return run_norm<T, V, 1, 128>(a, gy, gn, o1, o2, o3, part, nsum, back, s);
   if (u <= 256) return run_norm<T, V, 1, 256>(a, gy, gn, o1, o2, o3, part, nsum, back, s);
   if (u <= 1024) return run_norm<T, V, 1, 1024>(a, gy, gn, o1, o2, o3, part, nsum, back, s);
   if (V > 1 || u <= 2048) return run_norm<T, V, 2, 1024>(a, gy, gn, o1, o2, o3, part, nsum, back, s);

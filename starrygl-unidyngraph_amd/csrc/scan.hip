@@ -14,13 +14,15 @@
 // written). A thread owns V neighbouring channels of one sequence, and the
 // threads of a wave neighbouring channels, so each step is one contiguous
 // access. States stay in fp32 registers. Both directions are chains in t, so
-// a sequence is cut into chunks where there are too few channels to fill the
-// GPU: a first kernel gives each chunk's composition (A, B) of h -> A h + B, and
-// the second forms each chunk's starting state from those before it and
-// walks its chunk. The forward keeps the state in fp32 at every kKeep-th
-// step; the backward walks blocks of kKeep steps last to first, computing a
-// block's states again in registers from the kept one, so it neither reads
-// the (rounded) outputs nor differentiates through their rounding.
+// where the channels alone are too few to fill the GPU a sequence is cut into
+// up to kMaxSupers * kSubs pieces: a first kernel forms each piece's
+// composition (A, B) of h -> A h + B and, in LDS, those of the pieces before
+// it in its workgroup; the second kernel forms a piece's starting state from
+// the workgroups' compositions and its own prefix, and walks its piece.
+// The forward keeps the state in fp32 at every kKeep-th step; the backward
+// walks blocks of kKeep steps last to first, computing a block's states again
+// in registers from the kept one, so it neither reads the (rounded) outputs
+// nor differentiates through their rounding.
 #include <climits>
 
 #include "history.h"
@@ -28,10 +30,12 @@
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kKeep = 16;            // steps between kept states
+constexpr int kKeep = 8;             // steps between kept states
 constexpr int64_t kFill = 1 << 18;   // threads that fill the GPU: 16 waves a CU
-constexpr int kMaxChunks = 64;
-constexpr int kMinChunk = 64;        // steps (a multiple of kKeep)
+constexpr int kSubs = 8;             // pieces a workgroup of the cut form: kLanes channel groups each
+constexpr int kLanes = kBlock / kSubs;
+constexpr int kMaxSupers = 32;
+constexpr int kMinPiece = 32;        // steps (a multiple of kKeep)
 
 struct ScanArgs {
   const void *gate, *value;
@@ -42,8 +46,10 @@ struct ScanArgs {
   int64_t gaps_n, gaps_t;
   const float *decay;   // [D]
   int64_t N, L;
-  int D, chunks;
-  int64_t clen;         // steps a chunk (a multiple of kKeep)
+  int D;
+  int supers;           // workgroups along a sequence (0: sequences whole, channels side by side)
+  int64_t piece;        // steps a piece (a multiple of kKeep)
+  float2 *sup, *sub;    // compositions: [N][supers][D], [N][supers][kSubs][D] (those before it in its workgroup)
 };
 
 // a and 1 - a of one step
@@ -69,91 +75,143 @@ __device__ __forceinline__ int64_t seq_len(const ScanArgs &a, int64_t n) {
   return min(max(int64_t(a.lens[n]), int64_t(0)), a.L);
 }
 
-// Units: (sequence, channel group, chunk), the channel group fastest, so that
-// a wave's accesses are contiguous; chunks before sequences.
+// What a thread walks: V channels from d of sequence n, steps [t0, t1) of it.
 struct Unit {
-  int64_t n;
-  int d, chunk;
+  int64_t n, t0, t1;
+  int d, super, sub;
+  bool ok;
 };
 template <int V>
-__device__ __forceinline__ Unit unit_of(const ScanArgs &a, int64_t i) {
+__device__ __forceinline__ Unit unit_of(const ScanArgs &a) {
   const int dv = (a.D + V - 1) / V;
   Unit u;
-  const int64_t q = i / dv;
-  u.d = int(i - q * dv) * V;
-  u.n = q / a.chunks;
-  u.chunk = int(q - u.n * a.chunks);
+  if (a.supers == 0) {   // whole sequences: (n, d) side by side
+    const int64_t i = int64_t(blockIdx.x) * kBlock + threadIdx.x;
+    u.n = i / dv;
+    u.d = int(i - u.n * dv) * V;
+    u.super = u.sub = 0;
+    u.t0 = 0;
+    u.t1 = a.L;
+    u.ok = u.n < a.N;
+  } else {   // a workgroup: kLanes channel groups x kSubs pieces
+    const int blocks = (dv + kLanes - 1) / kLanes;
+    int64_t i = blockIdx.x;
+    const int cb = int(i % blocks);
+    i /= blocks;
+    u.super = int(i % a.supers);
+    u.n = i / a.supers;
+    u.sub = threadIdx.x / kLanes;
+    u.d = (cb * kLanes + threadIdx.x % kLanes) * V;
+    u.t0 = min((int64_t(u.super) * kSubs + u.sub) * a.piece, a.L);
+    u.t1 = min(u.t0 + a.piece, a.L);
+    u.ok = u.d < a.D;
+  }
   return u;
 }
+template <int V>
+__device__ __forceinline__ int64_t comp_at(const ScanArgs &a, const Unit &u, int super) {
+  return (u.n * a.supers + super) * a.D + u.d;
+}
+// s -> A s + B
+template <int V>
+__device__ __forceinline__ void compose(float (&s)[V], const float2 *__restrict__ p) {
+  float2 c[V];
+  __builtin_memcpy(c, p, sizeof(c));
+#pragma unroll
+  for (int j = 0; j < V; ++j) s[j] = c[j].x * s[j] + c[j].y;
+}
 
-// The compositions of each chunk: forward (A = prod a, B = the state it ends
-// in from 0), or backward (B = a_0 lam_0 of the chunk from nothing after it).
+// The compositions of the pieces: forward (A = prod a, B = the state a piece
+// ends in from 0), or backward (B = a_0 lam_0 of the piece from nothing after
+// it), combined over the pieces before it (forward) or after it (backward) in
+// the workgroup; the workgroup's own into sup.
 template <typename T, int V, bool DECAY, bool BACK>
-__global__ __launch_bounds__(kBlock) void k_scan_chunks(ScanArgs a, const T *__restrict__ gh, float *__restrict__ comp) {
-  const int64_t units = a.N * a.chunks * ((a.D + V - 1) / V);
-  const int64_t i = int64_t(blockIdx.x) * kBlock + threadIdx.x;
-  if (i >= units) return;
-  const Unit u = unit_of<V>(a, i);
-  const int64_t len = seq_len(a, u.n);
-  const int64_t t0 = u.chunk * a.clen, t1 = min(t0 + a.clen, len);
-  const T *gate = static_cast<const T *>(a.gate) + u.n * a.gate_n + u.d;
-  const T *src = BACK ? gh + u.n * a.L * a.D + u.d : static_cast<const T *>(a.value) + u.n * a.value_n + u.d;
-  const int64_t src_t = BACK ? a.D : a.value_t;
+__global__ __launch_bounds__(kBlock) void k_scan_pieces(ScanArgs a, const T *__restrict__ gh) {
+  __shared__ float2 comp[kSubs][kLanes * V];
+  const Unit u = unit_of<V>(a);
   float A[V], B[V], dec[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     A[j] = 1.f;
     B[j] = 0.f;
-    dec[j] = DECAY ? a.decay[u.d + j] : 0.f;
+    dec[j] = DECAY && u.ok ? a.decay[u.d + j] : 0.f;
   }
-  constexpr int U = 8;
-  for (int64_t t = t0; t < t1; t += U) {
-    T f[U][V], x[U][V];
-    float gap[U];
-    const int m = int(min(int64_t(U), t1 - t));
+  if (u.ok) {
+    const int64_t t0 = u.t0, t1 = min(u.t1, seq_len(a, u.n));
+    const T *gate = static_cast<const T *>(a.gate) + u.n * a.gate_n + u.d;
+    const T *src = BACK ? gh + u.n * a.L * a.D + u.d : static_cast<const T *>(a.value) + u.n * a.value_n + u.d;
+    const int64_t src_t = BACK ? a.D : a.value_t;
+    constexpr int U = 8;
+    for (int64_t t = t0; t < t1; t += U) {
+      T f[U][V], x[U][V];
+      float gap[U];
+      const int m = int(min(int64_t(U), t1 - t));
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int64_t at = BACK ? t1 - 1 - (t - t0) - min(k, m - 1) : t + min(k, m - 1);
-      sgl::load_n(f[k], gate + at * a.gate_t);
-      if (BACK && gh == nullptr) {
+      for (int k = 0; k < U; ++k) {
+        const int64_t at = BACK ? t1 - 1 - (t - t0) - min(k, m - 1) : t + min(k, m - 1);
+        sgl::load_n(f[k], gate + at * a.gate_t);
+        if (BACK && gh == nullptr) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[k][j] = T(0.f);
-      } else {
-        sgl::load_n(x[k], src + at * src_t);
+          for (int j = 0; j < V; ++j) x[k][j] = T(0.f);
+        } else {
+          sgl::load_n(x[k], src + at * src_t);
+        }
+        gap[k] = DECAY ? a.gaps[u.n * a.gaps_n + at * a.gaps_t] : 0.f;
       }
-      gap[k] = DECAY ? a.gaps[u.n * a.gaps_n + at * a.gaps_t] : 0.f;
-    }
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (k < m) {
+      for (int k = 0; k < U; ++k) {
+        if (k < m) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float ga, gb, sn;
-          step_gate<DECAY>(float(f[k][j]), dec[j] * gap[k], ga, gb, sn);
-          A[j] *= ga;
-          B[j] = BACK ? ga * (float(x[k][j]) + B[j]) : ga * B[j] + gb * float(x[k][j]);
+          for (int j = 0; j < V; ++j) {
+            float ga, gb, sn;
+            step_gate<DECAY>(float(f[k][j]), dec[j] * gap[k], ga, gb, sn);
+            A[j] *= ga;
+            B[j] = BACK ? ga * (float(x[k][j]) + B[j]) : ga * B[j] + gb * float(x[k][j]);
+          }
         }
       }
     }
   }
+  const int l = (threadIdx.x % kLanes) * V;
+#pragma unroll
+  for (int j = 0; j < V; ++j) comp[u.sub][l + j] = make_float2(A[j], B[j]);
+  __syncthreads();
+  if (!u.ok) return;
+  float pa[V], pb[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    float2 c = make_float2(A[j], B[j]);
-    *reinterpret_cast<float2 *>(comp + 2 * ((u.n * a.chunks + u.chunk) * a.D + u.d + j)) = c;
+    pa[j] = 1.f;
+    pb[j] = 0.f;
+  }
+  for (int i = 0; i < (BACK ? kSubs - 1 - u.sub : u.sub); ++i) {
+    const int from = BACK ? kSubs - 1 - i : i;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float2 c = comp[from][l + j];
+      pa[j] *= c.x;
+      pb[j] = c.x * pb[j] + c.y;
+    }
+  }
+  float2 o[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) o[j] = make_float2(pa[j], pb[j]);
+  sgl::store_n(a.sub + ((u.n * a.supers + u.super) * kSubs + u.sub) * a.D + u.d, o);
+  if (u.sub == (BACK ? 0 : kSubs - 1)) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = make_float2(A[j] * pa[j], A[j] * pb[j] + B[j]);
+    sgl::store_n(a.sup + comp_at<V>(a, u, u.super), o);
   }
 }
 
 // Forward: h (all L steps; zero past the length), the last state, and the
 // kept states (keep may be NULL).
 template <typename T, int V, bool DECAY>
-__global__ __launch_bounds__(kBlock) void k_scan_fwd(ScanArgs a, const float *__restrict__ comp, T *__restrict__ h,
-                                                     float *__restrict__ last, float *__restrict__ keep) {
-  const int64_t units = a.N * a.chunks * ((a.D + V - 1) / V);
-  const int64_t i = int64_t(blockIdx.x) * kBlock + threadIdx.x;
-  if (i >= units) return;
-  const Unit u = unit_of<V>(a, i);
+__global__ __launch_bounds__(kBlock) void k_scan_fwd(ScanArgs a, T *__restrict__ h, float *__restrict__ last,
+                                                     float *__restrict__ keep) {
+  const Unit u = unit_of<V>(a);
+  if (!u.ok) return;
   const int64_t len = seq_len(a, u.n);
-  const int64_t t0 = u.chunk * a.clen, t1 = min(t0 + a.clen, a.L), live = min(t1, len);
+  const int64_t t0 = u.t0, t1 = u.t1, live = min(t1, len);
   const T *gate = static_cast<const T *>(a.gate) + u.n * a.gate_n + u.d;
   const T *value = static_cast<const T *>(a.value) + u.n * a.value_n + u.d;
   T *out = h + u.n * a.L * a.D + u.d;
@@ -164,12 +222,9 @@ __global__ __launch_bounds__(kBlock) void k_scan_fwd(ScanArgs a, const float *__
     s[j] = a.state != nullptr ? a.state[u.n * a.D + u.d + j] : 0.f;
     dec[j] = DECAY ? a.decay[u.d + j] : 0.f;
   }
-  for (int c = 0; c < u.chunk; ++c) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float2 p = *reinterpret_cast<const float2 *>(comp + 2 * ((u.n * a.chunks + c) * a.D + u.d + j));
-      s[j] = p.x * s[j] + p.y;
-    }
+  if (a.supers > 0) {
+    for (int c = 0; c < u.super; ++c) compose(s, a.sup + comp_at<V>(a, u, c));
+    compose(s, a.sub + ((u.n * a.supers + u.super) * kSubs + u.sub) * a.D + u.d);
   }
   constexpr int U = 8;
   static_assert(kKeep % U == 0, "kept states fall on the first step of a group");
@@ -209,165 +264,188 @@ __global__ __launch_bounds__(kBlock) void k_scan_fwd(ScanArgs a, const float *__
         if (t + k < t1) sgl::store_n(out + (t + k) * a.D, o);
     }
   }
-  // the chunk that holds the last event (the first one of an empty sequence)
-  if (last != nullptr && (len > t0 ? len <= t0 + a.clen : len == 0 && u.chunk == 0))
-    sgl::store_n(last + u.n * a.D + u.d, s);
+  // the piece that holds the last event (the first one of an empty sequence)
+  if (last != nullptr && (len > 0 ? len > t0 && len <= t1 : t0 == 0)) sgl::store_n(last + u.n * a.D + u.d, s);
 }
 
-// Backward: thread g of `groups` walks the sequences g, g + groups, ... of its
-// channels (all its chunks' work units), so that decay's gradient is one row
-// of partial sums a group.
+// One piece's adjoint, from c = a_{t+1} lam_{t+1} after it; c becomes a_0 lam_0 of
+// its first step, dsum gathers decay's gradient.
 template <typename T, int V, bool DECAY>
-__global__ __launch_bounds__(kBlock) void k_scan_bwd(ScanArgs a, const float *__restrict__ comp,
-                                                     const float *__restrict__ keep, const T *__restrict__ gh,
-                                                     const float *__restrict__ glast, T *__restrict__ dgate,
-                                                     T *__restrict__ dvalue, float *__restrict__ dstate,
-                                                     float *__restrict__ part, int64_t groups) {
-  const int dv = (a.D + V - 1) / V;
-  const int64_t i = int64_t(blockIdx.x) * kBlock + threadIdx.x;
-  if (i >= groups * dv) return;
-  const int64_t g = i / dv;
-  const int d = int(i - g * dv) * V;
+__device__ __forceinline__ void walk_back(const ScanArgs &a, const Unit &u, int64_t len, const float (&dec)[V],
+                                          const float *__restrict__ keep, const T *__restrict__ gh,
+                                          T *__restrict__ dgate, T *__restrict__ dvalue, float (&c)[V],
+                                          float (&dsum)[V]) {
+  const int64_t t0 = u.t0, t1 = u.t1, live = min(t1, len);
   const int64_t keeps = (a.L + kKeep - 1) / kKeep;
-  float dec[V], dsum[V];
+  const T *gate = static_cast<const T *>(a.gate) + u.n * a.gate_n + u.d;
+  const T *value = static_cast<const T *>(a.value) + u.n * a.value_n + u.d;
+  const int64_t row0 = u.n * a.L * a.D + u.d;
+  T zero[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    dec[j] = DECAY ? a.decay[d + j] : 0.f;
-    dsum[j] = 0.f;
+  for (int j = 0; j < V; ++j) zero[j] = T(0.f);
+  for (int64_t t = max(t0, live); t < t1; ++t) {
+    sgl::store_n(dgate + row0 + t * a.D, zero);
+    sgl::store_n(dvalue + row0 + t * a.D, zero);
   }
-  for (int64_t w = g; w < a.N * a.chunks; w += groups) {
-    const int64_t n = w / a.chunks;
-    const int chunk = int(w - n * a.chunks);
-    const int64_t len = seq_len(a, n);
-    const int64_t t0 = chunk * a.clen, t1 = min(t0 + a.clen, a.L), live = min(t1, len);
-    const T *gate = static_cast<const T *>(a.gate) + n * a.gate_n + d;
-    const T *value = static_cast<const T *>(a.value) + n * a.value_n + d;
-    const int64_t row0 = n * a.L * a.D + d;
-    float c[V];   // a_{t+1} lam_{t+1}
+  if (live <= t0) return;
+  for (int64_t b = (live - 1) / kKeep * kKeep; b >= t0; b -= kKeep) {
+    T f[kKeep][V], x[kKeep][V], gr[kKeep][V];
+    float gap[kKeep], s[V];
+    const int m = int(min(int64_t(kKeep), live - b));
+    sgl::load_n(s, keep + (u.n * keeps + b / kKeep) * a.D + u.d);
 #pragma unroll
-    for (int j = 0; j < V; ++j) c[j] = glast != nullptr ? glast[n * a.D + d + j] : 0.f;
-    for (int k = a.chunks - 1; k > chunk; --k) {
-      if (k * a.clen >= len) continue;
+    for (int k = 0; k < kKeep; ++k) {
+      const int64_t at = b + min(k, m - 1);
+      sgl::load_n(f[k], gate + at * a.gate_t);
+      sgl::load_n(x[k], value + at * a.value_t);
+      if (gh != nullptr) {
+        sgl::load_n(gr[k], gh + row0 + at * a.D);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) gr[k][j] = zero[j];
+      }
+      gap[k] = DECAY ? a.gaps[u.n * a.gaps_n + at * a.gaps_t] : 0.f;
+    }
+    // forward through the block: a, 1 - a, and the factors lam meets
+    float ga[kKeep][V], gb[kKeep][V], wl[kKeep][V], wg[kKeep][V];
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float2 p = *reinterpret_cast<const float2 *>(comp + 2 * ((n * a.chunks + k) * a.D + d + j));
-        c[j] = p.x * c[j] + p.y;
+        float sn;
+        step_gate<DECAY>(float(f[k][j]), dec[j] * gap[k], ga[k][j], gb[k][j], sn);
+        const float xv = float(x[k][j]);
+        wl[k][j] = (s[j] - xv) * ga[k][j];   // d log a
+        wg[k][j] = wl[k][j] * sn;            // d gate
+        s[j] = ga[k][j] * s[j] + gb[k][j] * xv;
+      }
+#pragma unroll
+    for (int k = kKeep - 1; k >= 0; --k) {
+      if (k < m) {
+        T og[V], ov[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float lam = float(gr[k][j]) + c[j];
+          c[j] = ga[k][j] * lam;
+          og[j] = T(lam * wg[k][j]);
+          ov[j] = T(lam * gb[k][j]);
+          if (DECAY) dsum[j] -= lam * wl[k][j] * gap[k];
+        }
+        sgl::store_n(dgate + row0 + (b + k) * a.D, og);
+        sgl::store_n(dvalue + row0 + (b + k) * a.D, ov);
       }
     }
-    T zero[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) zero[j] = T(0.f);
-    for (int64_t t = max(t0, live); t < t1; ++t) {
-      sgl::store_n(dgate + row0 + t * a.D, zero);
-      sgl::store_n(dvalue + row0 + t * a.D, zero);
-    }
-    if (live > t0) {
-      for (int64_t b = (live - 1) / kKeep * kKeep; b >= t0; b -= kKeep) {
-        T f[kKeep][V], x[kKeep][V], gr[kKeep][V];
-        float gap[kKeep], s[V];
-        const int m = int(min(int64_t(kKeep), live - b));
-        sgl::load_n(s, keep + (n * keeps + b / kKeep) * a.D + d);
-#pragma unroll
-        for (int k = 0; k < kKeep; ++k) {
-          const int64_t at = b + min(k, m - 1);
-          sgl::load_n(f[k], gate + at * a.gate_t);
-          sgl::load_n(x[k], value + at * a.value_t);
-          if (gh != nullptr) {
-            sgl::load_n(gr[k], gh + row0 + at * a.D);
-          } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) gr[k][j] = T(0.f);
-          }
-          gap[k] = DECAY ? a.gaps[n * a.gaps_n + at * a.gaps_t] : 0.f;
-        }
-        float before[kKeep][V];   // the state each step meets
-#pragma unroll
-        for (int k = 0; k < kKeep; ++k)
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            before[k][j] = s[j];
-            float ga, gb, sn;
-            step_gate<DECAY>(float(f[k][j]), dec[j] * gap[k], ga, gb, sn);
-            s[j] = ga * s[j] + gb * float(x[k][j]);
-          }
-#pragma unroll
-        for (int k = kKeep - 1; k >= 0; --k) {
-          if (k < m) {
-            T og[V], ov[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              float ga, gb, sn;
-              step_gate<DECAY>(float(f[k][j]), dec[j] * gap[k], ga, gb, sn);
-              const float lam = float(gr[k][j]) + c[j];
-              const float dlog = lam * (before[k][j] - float(x[k][j])) * ga;
-              c[j] = ga * lam;
-              og[j] = T(dlog * sn);
-              ov[j] = T(gb * lam);
-              if (DECAY) dsum[j] -= dlog * gap[k];
-            }
-            sgl::store_n(dgate + row0 + (b + k) * a.D, og);
-            sgl::store_n(dvalue + row0 + (b + k) * a.D, ov);
-          }
-        }
-      }
-    }
-    if (dstate != nullptr && chunk == 0) sgl::store_n(dstate + n * a.D + d, c);
   }
-  if (DECAY) sgl::store_n(part + g * a.D + d, dsum);
 }
 
-// Chunks a sequence: one where the channels alone fill the GPU, else as many
-// as do, of at least kMinChunk steps each.
-int scan_chunks(int64_t N, int64_t L, int64_t dv) {
-  const int64_t want = (kFill + N * dv - 1) / (N * dv);
-  return int(std::max<int64_t>(1, std::min<int64_t>({want, L / kMinChunk, int64_t(kMaxChunks)})));
+// Backward. Whole sequences: thread group g of `groups` walks the sequences g,
+// g + groups, ... of its channels, so that decay's gradient is one row of
+// partial sums a group. Cut: a workgroup's pieces, one row a workgroup.
+template <typename T, int V, bool DECAY>
+__global__ __launch_bounds__(kBlock) void k_scan_bwd(ScanArgs a, const float *__restrict__ keep,
+                                                     const T *__restrict__ gh, const float *__restrict__ glast,
+                                                     T *__restrict__ dgate, T *__restrict__ dvalue,
+                                                     float *__restrict__ dstate, float *__restrict__ part,
+                                                     int64_t groups) {
+  Unit u = unit_of<V>(a);
+  float dec[V], dsum[V], c[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    dec[j] = DECAY && u.ok ? a.decay[u.d + j] : 0.f;
+    dsum[j] = 0.f;
+  }
+  if (a.supers == 0) {
+    const int64_t g = u.n;
+    if (g >= groups) return;
+    for (u.n = g; u.n < a.N; u.n += groups) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) c[j] = glast != nullptr ? glast[u.n * a.D + u.d + j] : 0.f;
+      walk_back<T, V, DECAY>(a, u, seq_len(a, u.n), dec, keep, gh, dgate, dvalue, c, dsum);
+      if (dstate != nullptr) sgl::store_n(dstate + u.n * a.D + u.d, c);
+    }
+    if (DECAY) sgl::store_n(part + g * a.D + u.d, dsum);
+    return;
+  }
+  if (u.ok) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) c[j] = glast != nullptr ? glast[u.n * a.D + u.d + j] : 0.f;
+    for (int k = a.supers - 1; k > u.super; --k) compose(c, a.sup + comp_at<V>(a, u, k));
+    compose(c, a.sub + ((u.n * a.supers + u.super) * kSubs + u.sub) * a.D + u.d);
+    walk_back<T, V, DECAY>(a, u, seq_len(a, u.n), dec, keep, gh, dgate, dvalue, c, dsum);
+    if (dstate != nullptr && u.t0 == 0 && u.super == 0 && u.sub == 0) sgl::store_n(dstate + u.n * a.D + u.d, c);
+  }
+  if (DECAY) {
+    __shared__ float sums[kSubs][kLanes * V];
+    const int l = (threadIdx.x % kLanes) * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) sums[u.sub][l + j] = dsum[j];
+    __syncthreads();
+    if (u.sub == 0 && u.ok) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        for (int i = 1; i < kSubs; ++i) dsum[j] += sums[i][l + j];
+      sgl::store_n(part + comp_at<V>(a, u, u.super), dsum);
+    }
+  }
 }
-int64_t chunk_len(int64_t L, int chunks) {
-  const int64_t c = (L + chunks - 1) / chunks;
-  return (c + kKeep - 1) / kKeep * kKeep;
-}
+
 int scan_vec(int32_t dtype, int32_t D) { return dtype != SGL_FP32 && D % 2 == 0 ? 2 : 1; }
 
-int64_t bwd_groups(int64_t N, int chunks, int64_t dv) {
-  return std::max<int64_t>(1, std::min<int64_t>(N * chunks, (kFill + dv - 1) / dv));
-}
-
+// Sequences whole where their channels fill half the GPU or a piece would be
+// shorter than kMinPiece; else cut so that the pieces fill it twice.
 struct ScanPlan {
-  int vec, chunks;
-  int64_t clen, comp, groups;   // comp: floats of the compositions
+  int vec, supers;
+  int64_t piece, groups;       // groups: rows of decay's partial sums
+  size_t sup, sub, part;       // bytes of the workspace's parts
 };
 ScanPlan scan_plan(int32_t dtype, int64_t N, int64_t L, int32_t D) {
   ScanPlan p;
   p.vec = scan_vec(dtype, D);
-  const int64_t dv = (D + p.vec - 1) / p.vec;
-  p.chunks = scan_chunks(N, L, dv);
-  p.clen = chunk_len(L, p.chunks);
-  p.chunks = int((L + p.clen - 1) / p.clen);
-  p.comp = p.chunks > 1 ? 2 * N * p.chunks * D : 0;
-  p.groups = bwd_groups(N, p.chunks, dv);
+  const int64_t dv = (D + p.vec - 1) / p.vec, threads = N * dv;
+  int64_t supers = 0;
+  if (2 * threads < kFill) {
+    const int64_t want = (2 * kFill + threads * kSubs - 1) / (threads * kSubs);
+    supers = std::min<int64_t>({want, L / (kMinPiece * kSubs), int64_t(kMaxSupers)});
+  }
+  p.supers = 0;
+  p.piece = L;
+  if (supers > 0) {
+    p.piece = (L + supers * kSubs - 1) / (supers * kSubs);
+    p.piece = (p.piece + kKeep - 1) / kKeep * kKeep;
+    p.supers = int((L + p.piece * kSubs - 1) / (p.piece * kSubs));
+    p.groups = N * p.supers;
+  } else {   // as many as fill the GPU twice, each with as many sequences
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(N, 2 * kFill / dv)), each = (N + most - 1) / most;
+    p.groups = (N + each - 1) / each;
+  }
+  p.sup = sgl::align_up(sizeof(float2) * size_t(N * p.supers * D));
+  p.sub = sgl::align_up(sizeof(float2) * size_t(N * p.supers * kSubs * D));
+  p.part = sizeof(float) * size_t(p.groups) * size_t(D);
   return p;
 }
 
-template <typename T, int V, bool DECAY>
-void scan_fwd(const ScanArgs &a, float *comp, void *h, float *last, float *keep, hipStream_t s) {
-  const int64_t units = a.N * a.chunks * ((a.D + V - 1) / V);
-  const dim3 grid(unsigned((units + kBlock - 1) / kBlock));
-  if (a.chunks > 1)
-    sgl::launch(&k_scan_chunks<T, V, DECAY, false>, grid, dim3(kBlock), 0, s, a, static_cast<const T *>(nullptr), comp);
-  sgl::launch(&k_scan_fwd<T, V, DECAY>, grid, dim3(kBlock), 0, s, a, static_cast<const float *>(comp),
-              static_cast<T *>(h), last, keep);
+unsigned scan_grid(const ScanArgs &a, int64_t rows, int V) {
+  const int64_t dv = (a.D + V - 1) / V;
+  if (a.supers > 0) return unsigned(a.N * a.supers * ((dv + kLanes - 1) / kLanes));
+  return unsigned((rows * dv + kBlock - 1) / kBlock);
 }
 
 template <typename T, int V, bool DECAY>
-void scan_bwd(const ScanArgs &a, float *comp, const float *keep, const void *gh, const float *glast, void *dgate,
-              void *dvalue, float *dstate, float *ddecay, float *part, int64_t groups, hipStream_t s) {
-  const int64_t dv = (a.D + V - 1) / V, units = a.N * a.chunks * dv;
-  if (a.chunks > 1)
-    sgl::launch(&k_scan_chunks<T, V, DECAY, true>, dim3(unsigned((units + kBlock - 1) / kBlock)), dim3(kBlock), 0, s,
-                a, static_cast<const T *>(gh), comp);
-  sgl::launch(&k_scan_bwd<T, V, DECAY>, dim3(unsigned((groups * dv + kBlock - 1) / kBlock)), dim3(kBlock), 0, s, a,
-              static_cast<const float *>(comp), keep, static_cast<const T *>(gh), glast, static_cast<T *>(dgate),
-              static_cast<T *>(dvalue), dstate, part, groups);
+void scan_fwd(const ScanArgs &a, void *h, float *last, float *keep, hipStream_t s) {
+  const dim3 grid(scan_grid(a, a.N, V));
+  if (a.supers > 0)
+    sgl::launch(&k_scan_pieces<T, V, DECAY, false>, grid, dim3(kBlock), 0, s, a, static_cast<const T *>(nullptr));
+  sgl::launch(&k_scan_fwd<T, V, DECAY>, grid, dim3(kBlock), 0, s, a, static_cast<T *>(h), last, keep);
+}
+
+template <typename T, int V, bool DECAY>
+void scan_bwd(const ScanArgs &a, const float *keep, const void *gh, const float *glast, void *dgate, void *dvalue,
+              float *dstate, float *ddecay, float *part, int64_t groups, hipStream_t s) {
+  const dim3 grid(scan_grid(a, groups, V));
+  if (a.supers > 0)
+    sgl::launch(&k_scan_pieces<T, V, DECAY, true>, grid, dim3(kBlock), 0, s, a, static_cast<const T *>(gh));
+  sgl::launch(&k_scan_bwd<T, V, DECAY>, grid, dim3(kBlock), 0, s, a, keep, static_cast<const T *>(gh), glast,
+              static_cast<T *>(dgate), static_cast<T *>(dvalue), dstate, part, groups);
   if (DECAY) sgl::sum_rows(part, groups, a.D, ddecay, s);
 }
 
@@ -384,6 +462,16 @@ void by_type(int32_t dtype, int vec, bool decay, F f) {
   else if (dtype == SGL_BF16) go(sgl::bf16_t{}, I1{});
   else if (vec == 2) go(sgl::fp16_t{}, I2{});
   else go(sgl::fp16_t{}, I1{});
+}
+
+// The workspace's parts; returns decay's partial sums.
+float *place_work(ScanArgs &a, const ScanPlan &p, void *workspace) {
+  char *w = static_cast<char *>(workspace);
+  a.supers = p.supers;
+  a.piece = p.piece;
+  a.sup = reinterpret_cast<float2 *>(w);
+  a.sub = reinterpret_cast<float2 *>(w + p.sup);
+  return reinterpret_cast<float *>(w + p.sup + p.sub);
 }
 
 int check_scan(int32_t dtype, int64_t N, int64_t L, int32_t D, const ScanArgs &a) {
@@ -406,9 +494,7 @@ extern "C" size_t sgl_gated_scan_workspace_bytes(int32_t dtype, int64_t N, int64
                                                  int32_t decay) {
   if (N <= 0 || L <= 0 || D <= 0) return 0;
   const ScanPlan p = scan_plan(dtype, N, L, D);
-  size_t b = sgl::align_up(sizeof(float) * size_t(p.comp));
-  if (backward && decay) b += sizeof(float) * size_t(p.groups) * size_t(D);
-  return b;
+  return p.sup + p.sub + (backward && decay ? p.part : 0);
 }
 
 extern "C" int sgl_gated_scan_forward(int32_t dtype, int64_t N, int64_t L, int32_t D, const void *gate,
@@ -416,7 +502,8 @@ extern "C" int sgl_gated_scan_forward(int32_t dtype, int64_t N, int64_t L, int32
                                       int64_t value_t, const int32_t *lens, const float *state, const float *gaps,
                                       int64_t gaps_n, int64_t gaps_t, const float *decay, void *h, float *last,
                                       float *keep, void *workspace, size_t workspace_bytes, hipStream_t stream) {
-  ScanArgs a{gate, value, gate_n, gate_t, value_n, value_t, lens, state, gaps, gaps_n, gaps_t, decay, N, L, D, 1, L};
+  ScanArgs a{gate, value, gate_n, gate_t, value_n, value_t, lens, state, gaps, gaps_n, gaps_t, decay, N, L, D,
+             0, L, nullptr, nullptr};
   if (const int rc = check_scan(dtype, N, L, D, a)) return rc;
   if (N == 0 || L == 0) return SGL_OK;
   SGL_REQUIRE(h != nullptr, "gated_scan: NULL array");
@@ -426,11 +513,9 @@ extern "C" int sgl_gated_scan_forward(int32_t dtype, int64_t N, int64_t L, int32
     sgl::set_error("gated_scan: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     return SGL_ERR_WORKSPACE;
   }
-  a.chunks = p.chunks;
-  a.clen = p.clen;
+  place_work(a, p, workspace);
   by_type(dtype, p.vec, decay != nullptr, [&](auto t, auto v, auto dec) {
-    scan_fwd<decltype(t), decltype(v)::value, decltype(dec)::value>(a, static_cast<float *>(workspace), h, last, keep,
-                                                                    stream);
+    scan_fwd<decltype(t), decltype(v)::value, decltype(dec)::value>(a, h, last, keep, stream);
   });
   SGL_CHECK_LAUNCH();
   return SGL_OK;
@@ -442,7 +527,8 @@ extern "C" int sgl_gated_scan_backward(int32_t dtype, int64_t N, int64_t L, int3
                                        int64_t gaps_n, int64_t gaps_t, const float *decay, const float *keep,
                                        const void *gh, const float *glast, void *dgate, void *dvalue, float *dstate,
                                        float *ddecay, void *workspace, size_t workspace_bytes, hipStream_t stream) {
-  ScanArgs a{gate, value, gate_n, gate_t, value_n, value_t, lens, state, gaps, gaps_n, gaps_t, decay, N, L, D, 1, L};
+  ScanArgs a{gate, value, gate_n, gate_t, value_n, value_t, lens, state, gaps, gaps_n, gaps_t, decay, N, L, D,
+             0, L, nullptr, nullptr};
   if (const int rc = check_scan(dtype, N, L, D, a)) return rc;
   if (N == 0 || L == 0) return SGL_OK;
   SGL_REQUIRE(keep && dgate && dvalue && (decay == nullptr || ddecay != nullptr), "gated_scan_backward: NULL array");
@@ -452,13 +538,10 @@ extern "C" int sgl_gated_scan_backward(int32_t dtype, int64_t N, int64_t L, int3
     sgl::set_error("gated_scan_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     return SGL_ERR_WORKSPACE;
   }
-  a.chunks = p.chunks;
-  a.clen = p.clen;
-  float *comp = static_cast<float *>(workspace);
-  float *part = reinterpret_cast<float *>(static_cast<char *>(workspace) + sgl::align_up(sizeof(float) * size_t(p.comp)));
+  float *part = place_work(a, p, workspace);
   by_type(dtype, p.vec, decay != nullptr, [&](auto t, auto v, auto dec) {
-    scan_bwd<decltype(t), decltype(v)::value, decltype(dec)::value>(a, comp, keep, gh, glast, dgate, dvalue, dstate,
-                                                                    ddecay, part, p.groups, stream);
+    scan_bwd<decltype(t), decltype(v)::value, decltype(dec)::value>(a, keep, gh, glast, dgate, dvalue, dstate, ddecay,
+                                                                    part, p.groups, stream);
   });
   SGL_CHECK_LAUNCH();
   return SGL_OK;
