@@ -922,21 +922,24 @@ typedef struct sgl_attention {
   int64_t qpos_n, qpos_t, kpos_n, kpos_t;
 } sgl_attention;
 
-/* o [n, lq, heads_q, head_dim]; lse fp32 [n, heads_kv, lq * heads_q /
- * heads_kv] (what the backward reads). Rows past a query length and rows
- * without a live key are 0. The problem struct is HOST memory. */
+/* o [n, lq, heads_q, head_dim]; rows past a query length and rows without a
+ * live key are 0. What the backward reads of the forward, by the bits of
+ * sgl_cross_attention_saves: 1: o and lse (fp32 [n, heads_kv, lq * heads_q /
+ * heads_kv]), 2: rest (like o: what rounding o left). lse and rest may be NULL
+ * where they are not needed. The problem struct is HOST memory. */
+int32_t sgl_cross_attention_saves(const sgl_attention *problem);
 size_t sgl_cross_attention_workspace_bytes(const sgl_attention *problem,
                                            int32_t backward);
 int sgl_cross_attention_forward(const sgl_attention *problem, void *o,
-                                float *lse, void *workspace,
+                                void *rest, float *lse, void *workspace,
                                 size_t workspace_bytes, hipStream_t stream);
 /* go like o -> dq like o, dk and dv [n, lk, heads_kv, head_dim], dbias fp32
  * like the table (NULL: not computed). */
 int sgl_cross_attention_backward(const sgl_attention *problem, const void *o,
-                                 const float *lse, const void *go, void *dq,
-                                 void *dk, void *dv, float *dbias,
-                                 void *workspace, size_t workspace_bytes,
-                                 hipStream_t stream);
+                                 const void *rest, const float *lse,
+                                 const void *go, void *dq, void *dk, void *dv,
+                                 float *dbias, void *workspace,
+                                 size_t workspace_bytes, hipStream_t stream);
 
 /* y = x + scale * s(gate) * Norm(z; post), n = Norm(y; pre) over rows of D <=
  * 8192 values: Norm(t) = (t - mean) / sqrt(var + eps) * w + b, with rms != 0

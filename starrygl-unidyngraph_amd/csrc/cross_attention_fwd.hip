@@ -1,0 +1,581 @@
+// Forward kernels of the cross attention.
+#include "cross_attention.h"
+
+namespace sgl {
+namespace attn {
+namespace {
+
+// ------------------------------------------------------------------ many rows
+// A workgroup takes 4 x NQ blocks of 16 rows of a (sequence, key head), NQ a
+// wave, and walks the keys 64 at a time with the running maximum and sum of
+// the softmax (base 2). The next tile's keys and values are in flight while
+// the current one is worked on. The products are computed as (keys x rows) and
+// (head size x rows): a lane keeps one row a block, so its maximum, sum and
+// rescale are its own, joined over four lanes only. The accumulators are
+// rescaled only when the maximum has grown by more than 2^6: p stays below
+// 2^6, and the sum and the products carry the same factor.
+constexpr float kSlack = 6.f;
+
+template <typename T, int DP>
+struct FwdLds {
+  T k[kKeys * Tile<T, DP>::LD], v[kKeys * Tile<T, DP>::LD];
+  PosTile<kKeys> pos;
+};
+
+template <typename T, int DP, int NQ, bool SHARE>
+__global__ __launch_bounds__(kBlock) void k_attn_fwd(Args a, int64_t tiles, T *__restrict__ o, T *__restrict__ rest,
+                                                     float *__restrict__ lse) {
+  using M = Mma<T>;
+  using L = Tile<T, DP>;
+  constexpr int ST = DP / M::KS, DB = DP / 16, KB = kKeys / 16;
+  constexpr int NP = SHARE ? 1 : NQ;   // positions a lane holds
+  extern __shared__ __align__(16) char smem[];
+  FwdLds<T, DP> &s = *reinterpret_cast<FwdLds<T, DP> *>(smem);
+  float *table = reinterpret_cast<float *>(smem + sizeof(s));
+  const sgl_attention &p = a.p;
+  const int dh = p.head_dim;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
+  int64_t id = blockIdx.x;
+  const int64_t rt = id % tiles;
+  id /= tiles;
+  const int hk = int(id % p.heads_kv);
+  const int64_t n = id / p.heads_kv;
+  const Seq<T> q = seq_of<T>(p, n, hk, a.G);
+  const bool biased = p.bias != nullptr;
+  const Buckets bk = buckets_of(p);
+  // the workgroup's first query; nothing to do past the length
+  const int64_t t0 = rt * (SHARE ? 64 : 64 * NQ);
+  const int64_t i0 = row_at<SHARE>(t0, 0, a.G).i;
+  const bool any = i0 < q.qlen;
+  if (biased) stage_bias(table, a, hk, threadIdx.x, kBlock);
+  RowAt row[NQ];
+  bool in[NQ], ok[NQ];
+  FragOf<T> qf[NQ][ST];
+  int64_t qpos[NP];
+  int qrel[NP];
+  const int64_t base = biased && any ? q.qpos[i0 * p.qpos_t] : 0;
+  bool qnear = true;
+#pragma unroll
+  for (int b = 0; b < NQ; ++b) {
+    const int64_t t = SHARE ? t0 + w * 16 + cl : t0 + (w * NQ + b) * 16 + cl;
+    row[b] = row_at<SHARE>(t, b, a.G);
+    in[b] = row[b].i < p.lq;
+    ok[b] = row[b].i < q.qlen;
+#pragma unroll
+    for (int st = 0; st < ST; ++st)
+      qf[b][st] = load_row<T>(q.q + row[b].i * p.q_t + row[b].h * p.q_h, ok[b], st * M::KS + g * M::E, dh);
+    if (b < NP) {
+      qpos[b] = biased && ok[b] ? q.qpos[row[b].i * p.qpos_t] : base;
+      qnear = qnear && is_near(qpos[b] - base);
+      qrel[b] = int(qpos[b] - base);
+    }
+  }
+  qnear = __all(qnear);
+  const float c = p.scale * kLog2e;
+  float m[NQ], l[NQ];
+  f32x4 acc[NQ][DB];
+#pragma unroll
+  for (int b = 0; b < NQ; ++b) {
+    m[b] = -INFINITY;
+    l[b] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // a tile in flight: one key a lane for liveness and position, the rows by units
+  constexpr int PER = kKeys * L::UPR / kBlock;
+  FragOf<T> kr[PER], vr[PER];
+  uint64_t live = 0;
+  bool near_ = true;
+  int64_t kp = 0;
+  auto load_tile = [&](int64_t j0) {
+    const bool on = key_live(q, p, j0 + lane);
+    live = __ballot(on);
+    if (biased) {
+      kp = on ? q.kpos[(j0 + lane) * p.kpos_t] : base;
+      near_ = qnear && __all(is_near(kp - base));
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = threadIdx.x + i * kBlock, r = u / L::UPR, d = (u % L::UPR) * M::E;
+      const bool on_r = (live >> r) & 1;
+      kr[i] = load_raw<T>(q.k + (j0 + r) * p.k_t, on_r, d, dh);
+      vr[i] = load_raw<T>(q.v + (j0 + r) * p.v_t, on_r, d, dh);
+    }
+  };
+  if (any && q.klen > 0) load_tile(0);
+  for (int64_t j0 = 0; any && j0 < q.klen; j0 += kKeys) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = threadIdx.x + i * kBlock, r = u / L::UPR, d = (u % L::UPR) * M::E;
+      *reinterpret_cast<FragOf<T> *>(s.k + r * L::LD + d) = fix<T>(kr[i], d, dh);
+      *reinterpret_cast<FragOf<T> *>(s.v + r * L::LD + d) = fix<T>(vr[i], d, dh);
+    }
+    if (biased && w == 0) {
+      s.pos.pos[lane] = kp;
+      s.pos.rel[lane] = int(kp - base);
+    }
+    const uint64_t on = live;
+    const bool near_now = near_;
+    __syncthreads();
+    if (j0 + kKeys < q.klen) load_tile(j0 + kKeys);
+    float x[NQ][KB][4], mx[NQ];
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) mx[b] = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      FragOf<T> kf[ST];
+#pragma unroll
+      for (int st = 0; st < ST; ++st) kf[st] = L::frag(s.k, kb * 16, st * M::KS);
+      int col[4];
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) {
+        f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < ST; ++st) sc = M::mma(kf[st], qf[b][st], sc);
+        if (biased) {
+          if (b < NP) columns4(col, s.pos, kb * 16 + 4 * g, qrel[b < NP ? b : 0], qpos[b < NP ? b : 0], near_now, 1, bk);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) x[b][kb][v] = sc[v] * c + table[row[b].h * a.cols + col[v]];
+        } else {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) x[b][kb][v] = sc[v] * c;
+        }
+      }
+    }
+    if (on != ~0ull) {   // uniform
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const bool dead = !((on >> (kb * 16 + 4 * g + v)) & 1);
+#pragma unroll
+          for (int b = 0; b < NQ; ++b) x[b][kb][v] = dead ? -INFINITY : x[b][kb][v];
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) mx[b] = fmaxf(mx[b], x[b][kb][v]);
+      mx[b] = groups_max(mx[b]);
+      if (__any(mx[b] > m[b] + kSlack)) {   // (uniform over the wave; also the first live tile)
+        const float mn = fmaxf(m[b], mx[b]);
+        const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[b] - mn);
+        l[b] *= alpha;
+        m[b] = mn;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[b][d] *= alpha;
+      }
+      const float at = m[b] == -INFINITY ? 0.f : m[b];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          x[b][kb][v] = __builtin_amdgcn_exp2f(x[b][kb][v] - at);
+          l[b] += x[b][kb][v];
+        }
+    }
+#pragma unroll
+    for (int st = 0; st < kKeys / M::KS; ++st) {
+      FragOf<T> pf[NQ];
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) pf[b] = frag_of<T>(x[b], st);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const FragOf<T> vf = L::template frag_t<kKeys>(s.v, d * 16, st * M::KS);
+#pragma unroll
+        for (int b = 0; b < NQ; ++b) acc[b][d] = M::mma(vf, pf[b], acc[b][d]);
+      }
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < NQ; ++b) {
+    const float sum = groups_sum(l[b]);
+    if (!in[b]) continue;
+    const float inv = ok[b] && sum > 0.f ? 1.f / sum : 0.f;
+    const int64_t at = out_row(a, n, hk, row[b].i, row[b].h);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const f32x4 v = acc[b][d] * inv;
+      store4(o + at, d * 16 + 4 * g, dh, v);
+      if (rest != nullptr) {   // what rounding o left, for the backward's D
+        f32x4 e;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = v[i] - float(T(v[i]));
+        store4(rest + at, d * 16 + 4 * g, dh, e);
+      }
+    }
+    // log2 of the sum of 2^x; +inf where no key is live, so that p is 0 there
+    if (lse != nullptr && g == 0)
+      lse[(n * p.heads_kv + hk) * a.rows + row[b].i * a.G + row[b].h] =
+          ok[b] && sum > 0.f ? m[b] + __log2f(sum) : INFINITY;
+  }
+}
+
+// ------------------------------------------------------------------ few rows
+// Up to 16 NQ rows a (sequence, key head): there is no reuse of a key beyond a
+// wave, so the waves work apart: keys go from memory straight into fragments,
+// values through the wave's own LDS tile for the transposed read, 32 keys at
+// a time, the next ones in flight. One wave takes a short sequence (`parts` 0);
+// long ones are split over the four waves of `parts` workgroups, whose
+// (maximum, sum, products) are joined in LDS and, with several workgroups, by
+// a second kernel.
+constexpr int kStep = 32;
+
+template <typename T, int DP, int NQ>
+struct FewLds {
+  T v[kStep * Tile<T, DP>::LD];
+  PosTile<kStep> pos;
+};
+
+template <typename T, int DP, int NQ>
+__global__ __launch_bounds__(kBlock) void k_attn_few(Args a, int parts, int64_t part_keys, T *__restrict__ o,
+                                                     T *__restrict__ rest, float *__restrict__ lse,
+                                                     float *__restrict__ pacc, float2 *__restrict__ pml) {
+  using M = Mma<T>;
+  using L = Tile<T, DP>;
+  constexpr int ST = DP / M::KS, DB = DP / 16, KB = kStep / 16;
+  extern __shared__ __align__(16) char smem[];
+  const sgl_attention &p = a.p;
+  const int dh = p.head_dim;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
+  using Lds = FewLds<T, DP, NQ>;
+  const size_t per = align_bytes(sizeof(Lds) + sizeof(float) * size_t(a.G) * a.cols);
+  Lds &s = *reinterpret_cast<Lds *>(smem + w * per);
+  float *table = reinterpret_cast<float *>(smem + w * per + sizeof(Lds));
+  const int64_t items = p.n * p.heads_kv;
+  int64_t item = parts == 0 ? int64_t(blockIdx.x) * kWaves + w : blockIdx.x / parts;
+  const int part = parts == 0 ? 0 : int(blockIdx.x - item * parts);
+  const bool work = item < items;
+  if (parts == 0 && !work) return;   // (whole waves; no barrier follows in this form)
+  const int hk = int(item % p.heads_kv);
+  const int64_t n = item / p.heads_kv;
+  const Seq<T> q = seq_of<T>(p, n, hk, a.G);
+  const bool biased = p.bias != nullptr;
+  const Buckets bk = buckets_of(p);
+  if (biased) {
+    stage_bias(table, a, hk, lane, kWave);
+    wave_sync();
+  }
+  RowAt row[NQ];
+  bool in[NQ], ok[NQ];
+  FragOf<T> qf[NQ][ST];
+  int64_t qpos[NQ];
+  int qrel[NQ];
+  const int64_t base = biased && q.qlen > 0 ? q.qpos[0] : 0;
+  bool qnear = true;
+#pragma unroll
+  for (int b = 0; b < NQ; ++b) {
+    row[b] = row_at<false>(b * 16 + cl, b, a.G);
+    in[b] = row[b].i < p.lq;
+    ok[b] = row[b].i < q.qlen;
+#pragma unroll
+    for (int st = 0; st < ST; ++st)
+      qf[b][st] = load_row<T>(q.q + row[b].i * p.q_t + row[b].h * p.q_h, ok[b], st * M::KS + g * M::E, dh);
+    qpos[b] = biased && ok[b] ? q.qpos[row[b].i * p.qpos_t] : base;
+    qnear = qnear && is_near(qpos[b] - base);
+    qrel[b] = int(qpos[b] - base);
+  }
+  qnear = __all(qnear);
+  const float c = p.scale * kLog2e;
+  float m[NQ], l[NQ];
+  f32x4 acc[NQ][DB];
+#pragma unroll
+  for (int b = 0; b < NQ; ++b) {
+    m[b] = -INFINITY;
+    l[b] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int64_t stride = parts == 0 ? kStep : kStep * kWaves;
+  const int64_t end = q.qlen > 0 ? (parts == 0 ? q.klen : min(q.klen, (part + 1) * part_keys)) : 0;
+  int64_t j0 = parts == 0 ? 0 : part * part_keys + w * kStep;
+  constexpr int PER = kStep * L::UPR / kWave;
+  FragOf<T> kr[KB][ST], vr[PER];
+  uint64_t live = 0;
+  bool near_ = true;
+  int64_t kp = 0;
+  auto load_tile = [&](int64_t j) {
+    const bool on = lane < kStep && key_live(q, p, j + lane);
+    live = __ballot(on);
+    if (biased) {
+      kp = on ? q.kpos[(j + lane) * p.kpos_t] : base;
+      near_ = qnear && __all(is_near(kp - base));
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int st = 0; st < ST; ++st)
+        kr[kb][st] = load_raw<T>(q.k + (j + kb * 16 + cl) * p.k_t, (live >> (kb * 16 + cl)) & 1, st * M::KS + g * M::E,
+                                 dh);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = lane + i * kWave, r = u / L::UPR, d = (u % L::UPR) * M::E;
+      vr[i] = load_raw<T>(q.v + (j + r) * p.v_t, (live >> r) & 1, d, dh);
+    }
+  };
+  if (j0 < end) load_tile(j0);
+  for (; j0 < end; j0 += stride) {
+    const uint64_t on = live;
+    const bool near_now = near_;
+    FragOf<T> kf[KB][ST];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int st = 0; st < ST; ++st) kf[kb][st] = fix<T>(kr[kb][st], st * M::KS + g * M::E, dh);
+    wave_sync();   // the reads of the tile before are done
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = lane + i * kWave, r = u / L::UPR, d = (u % L::UPR) * M::E;
+      *reinterpret_cast<FragOf<T> *>(s.v + r * L::LD + d) = fix<T>(vr[i], d, dh);
+    }
+    if (biased && lane < kStep) {
+      s.pos.pos[lane] = kp;
+      s.pos.rel[lane] = int(kp - base);
+    }
+    wave_sync();
+    if (j0 + stride < end) load_tile(j0 + stride);
+    float x[NQ][KB][4];
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < ST; ++st) sc = M::mma(kf[kb][st], qf[b][st], sc);
+        int col[4];
+        if (biased) columns4(col, s.pos, kb * 16 + 4 * g, qrel[b], qpos[b], near_now, 1, bk);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          float t = sc[v] * c;
+          if (biased) t += table[row[b].h * a.cols + col[v]];
+          x[b][kb][v] = (on >> (kb * 16 + 4 * g + v)) & 1 ? t : -INFINITY;
+          mx = fmaxf(mx, x[b][kb][v]);
+        }
+      }
+      mx = groups_max(mx);
+      if (__any(mx > m[b] + kSlack)) {
+        const float mn = fmaxf(m[b], mx);
+        const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[b] - mn);
+        l[b] *= alpha;
+        m[b] = mn;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[b][d] *= alpha;
+      }
+      const float at = m[b] == -INFINITY ? 0.f : m[b];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          x[b][kb][v] = __builtin_amdgcn_exp2f(x[b][kb][v] - at);
+          l[b] += x[b][kb][v];
+        }
+    }
+#pragma unroll
+    for (int st = 0; st < kStep / M::KS; ++st) {
+      FragOf<T> pf[NQ];
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) pf[b] = frag_of<T>(x[b], st);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const FragOf<T> vf = L::template frag_t<kStep>(s.v, d * 16, st * M::KS);
+#pragma unroll
+        for (int b = 0; b < NQ; ++b) acc[b][d] = M::mma(vf, pf[b], acc[b][d]);
+      }
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < NQ; ++b) l[b] = groups_sum(l[b]);
+  if (parts != 0) {
+    // the four waves' parts into wave 0's terms: [wave][block][d][row] products, [wave][block][row] (m, l)
+    float2 *ml = reinterpret_cast<float2 *>(smem);
+    float *pr = reinterpret_cast<float *>(smem + sizeof(float2) * kWaves * NQ * 16);
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NQ; ++b)
+      if (g == 0) ml[(w * NQ + b) * 16 + cl] = make_float2(m[b], l[b]);
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) top = fmaxf(top, ml[(i * NQ + b) * 16 + cl].x);
+      const float at = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) {
+        const float2 e = ml[(i * NQ + b) * 16 + cl];
+        sum += e.y * __builtin_amdgcn_exp2f(e.x - at);
+      }
+      const float f = __builtin_amdgcn_exp2f(m[b] - at);
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          pr[((w * NQ + b) * DP + d * 16 + 4 * g + v) * 16 + cl] = acc[b][d][v] * f;
+      m[b] = top;
+      l[b] = sum;
+    }
+    __syncthreads();
+    if (w != 0) return;
+#pragma unroll
+    for (int b = 0; b < NQ; ++b)
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          float t = 0.f;
+#pragma unroll
+          for (int i = 0; i < kWaves; ++i) t += pr[((i * NQ + b) * DP + d * 16 + 4 * g + v) * 16 + cl];
+          acc[b][d][v] = t;
+        }
+  }
+#pragma unroll
+  for (int b = 0; b < NQ; ++b) {
+    if (!in[b]) continue;
+    if (parts > 1) {
+      const int64_t r = (item * parts + part) * a.rows + row[b].i * a.G + row[b].h;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) store4(pacc + r * dh, d * 16 + 4 * g, dh, acc[b][d]);
+      if (g == 0) pml[r] = make_float2(m[b], l[b]);
+      continue;
+    }
+    const float inv = ok[b] && l[b] > 0.f ? 1.f / l[b] : 0.f;
+    const int64_t at = out_row(a, n, hk, row[b].i, row[b].h);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const f32x4 v = acc[b][d] * inv;
+      store4(o + at, d * 16 + 4 * g, dh, v);
+      if (rest != nullptr) {
+        f32x4 e;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = v[i] - float(T(v[i]));
+        store4(rest + at, d * 16 + 4 * g, dh, e);
+      }
+    }
+    if (lse != nullptr && g == 0)
+      lse[item * a.rows + row[b].i * a.G + row[b].h] = ok[b] && l[b] > 0.f ? m[b] + __log2f(l[b]) : INFINITY;
+  }
+}
+
+// The parts of a row joined: one wave a row, a lane two neighbouring values.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void k_attn_join(Args a, int parts, const float *__restrict__ pacc,
+                                                      const float2 *__restrict__ pml, T *__restrict__ o,
+                                                      T *__restrict__ rest, float *__restrict__ lse) {
+  const sgl_attention &p = a.p;
+  const int lane = threadIdx.x & 63, dh = p.head_dim;
+  const int64_t x = int64_t(blockIdx.x) * kWaves + (threadIdx.x >> 6);   // (item, row)
+  if (x >= p.n * p.heads_kv * a.rows) return;
+  const int64_t item = x / a.rows, r = x - item * a.rows;
+  const int64_t n = item / p.heads_kv, i = r / a.G;
+  const int hk = int(item - n * p.heads_kv), h = int(r - i * a.G);
+  const bool ok = p.q_lens == nullptr || i < p.q_lens[n];
+  float top = -INFINITY;
+  for (int k = lane; k < parts; k += kWave) top = fmaxf(top, pml[(item * parts + k) * a.rows + r].x);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
+  const float at = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, v0 = 0.f, v1 = 0.f;
+  const int d = 2 * lane;
+  for (int k = 0; k < parts; ++k) {
+    const int64_t row = (item * parts + k) * a.rows + r;
+    const float2 e = pml[row];
+    const float f = __builtin_amdgcn_exp2f(e.x - at);
+    sum += e.y * f;
+    if (d < dh) v0 += f * pacc[row * dh + d];
+    if (d + 1 < dh) v1 += f * pacc[row * dh + d + 1];
+  }
+  const float inv = ok && sum > 0.f ? 1.f / sum : 0.f;
+  const int64_t to = out_row(a, n, hk, i, h);
+  v0 *= inv;
+  v1 *= inv;
+  if (d < dh) o[to + d] = T(v0);
+  if (d + 1 < dh) o[to + d + 1] = T(v1);
+  if (rest != nullptr) {
+    if (d < dh) rest[to + d] = T(v0 - float(T(v0)));
+    if (d + 1 < dh) rest[to + d + 1] = T(v1 - float(T(v1)));
+  }
+  if (lse != nullptr && lane == 0) lse[x] = ok && sum > 0.f ? top + __log2f(sum) : INFINITY;
+}
+
+// ------------------------------------------------------------------ host
+constexpr int kFewRows = 32;
+
+// Workgroups a (sequence, key head) whose rows are few: 0 (a wave alone) up to
+// 4 steps of keys, else as many as bring 1,024 workgroups, of at least 4 steps
+// a wave each.
+int few_parts(const Args &a) {
+  if (a.p.lk <= 4 * kStep) return 0;
+  const int64_t items = a.p.n * a.p.heads_kv, most = (a.p.lk + 4 * kStep * kWaves - 1) / (4 * kStep * kWaves);
+  return int(std::max<int64_t>(1, std::min<int64_t>({(1024 + items - 1) / items, most, int64_t(256)})));
+}
+int64_t few_keys(const Args &a, int parts) {
+  const int64_t k = (a.p.lk + parts - 1) / parts;
+  return (k + kStep * kWaves - 1) / (kStep * kWaves) * (kStep * kWaves);
+}
+size_t ml_bytes(const Args &a, int parts) {
+  return align_up(sizeof(float2) * size_t(a.p.n * a.p.heads_kv) * size_t(parts) * size_t(a.rows));
+}
+
+template <typename T, int DP, int NQ>
+int launch_few(const Args &a, T *o, T *rest, float *lse, void *ws, hipStream_t s) {
+  const int parts = few_parts(a);
+  const int64_t items = a.p.n * a.p.heads_kv, keys = parts > 0 ? few_keys(a, parts) : 0;
+  const size_t per = align_bytes(sizeof(FewLds<T, DP, NQ>) + sizeof(float) * size_t(a.G) * a.cols);
+  size_t lds = per * kWaves;
+  if (parts > 0)
+    lds = std::max(lds, sizeof(float2) * kWaves * NQ * 16 + sizeof(float) * kWaves * NQ * 16 * size_t(DP));
+  float2 *ml = static_cast<float2 *>(ws);
+  float *acc = reinterpret_cast<float *>(static_cast<char *>(ws) + (parts > 1 ? ml_bytes(a, parts) : 0));
+  SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_few<T, DP, NQ>), lds));
+  const int64_t grid = parts == 0 ? (items + kWaves - 1) / kWaves : items * parts;
+  launch(&k_attn_few<T, DP, NQ>, dim3(unsigned(grid)), dim3(kBlock), lds, s, a, parts, keys, o, rest, lse, acc, ml);
+  if (parts > 1)
+    launch(&k_attn_join<T>, dim3(unsigned((items * a.rows + kWaves - 1) / kWaves)), dim3(kBlock), 0, s, a, parts,
+           static_cast<const float *>(acc), static_cast<const float2 *>(ml), o, rest, lse);
+  SGL_CHECK_LAUNCH();
+  return SGL_OK;
+}
+
+template <typename T, int DP, int NQ, bool SHARE>
+int launch_fwd(const Args &a, T *o, T *rest, float *lse, hipStream_t s) {
+  const int64_t count = SHARE ? a.rows / 2 : a.rows, per = SHARE ? 64 : 64 * NQ, tiles = (count + per - 1) / per;
+  const size_t lds = sizeof(FwdLds<T, DP>) + sizeof(float) * size_t(a.G) * a.cols;
+  SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_fwd<T, DP, NQ, SHARE>), lds));
+  launch(&k_attn_fwd<T, DP, NQ, SHARE>, dim3(unsigned(a.p.n * a.p.heads_kv * tiles)), dim3(kBlock), lds, s, a, tiles,
+         o, rest, lse);
+  SGL_CHECK_LAUNCH();
+  return SGL_OK;
+}
+
+}  // namespace
+
+size_t forward_bytes(const Args &a) {
+  if (a.rows > kFewRows) return 0;
+  const int parts = few_parts(a);
+  if (parts <= 1) return 0;
+  return ml_bytes(a, parts) +
+         sizeof(float) * size_t(a.p.n * a.p.heads_kv) * size_t(parts) * size_t(a.rows) * size_t(a.p.head_dim);
+}
+
+int run_forward(const Args &a, void *o, void *rest, float *lse, void *ws, hipStream_t s) {
+  return by_instance(a.p, [&](auto t, auto dp) {
+    using T = decltype(t);
+    constexpr int DP = decltype(dp)::value;
+    T *to = static_cast<T *>(o), *tr = static_cast<T *>(rest);
+    if (a.rows <= 16) return launch_few<T, DP, 1>(a, to, tr, lse, ws, s);
+    if (a.rows <= kFewRows) return launch_few<T, DP, 2>(a, to, tr, lse, ws, s);
+    // two blocks a wave where that still fills the GPU: each key fragment read
+    // from LDS, and with an even G each column, then serves two
+    const int64_t groups = a.p.n * a.p.heads_kv * ((a.rows + 127) / 128);
+    if (groups < 256) return launch_fwd<T, DP, 1, false>(a, to, tr, lse, s);
+    if (a.G % 2 == 0) return launch_fwd<T, DP, 2, true>(a, to, tr, lse, s);
+    return launch_fwd<T, DP, 2, false>(a, to, tr, lse, s);
+  });
+}
+
+}  // namespace attn
+}  // namespace sgl

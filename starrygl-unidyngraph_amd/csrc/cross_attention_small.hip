@@ -1,0 +1,337 @@
+// The cross attention's backward for windows: up to 32 rows (queries x heads
+// of a key head) and 64 keys, one wave a (sequence, key head) and no barriers.
+//
+// Everything of an item is on chip at once, so the softmax is formed again
+// with its own maximum and sum, D is the sum of p dp, and nothing of the
+// forward is read but its inputs. q, k, v and do are read once, straight into
+// fragments; k, do and q pass through the wave's LDS for the products down
+// their columns, p and ds to be read with the rows as the reduction index. A
+// wave walks items of one key head, so that the bias' gradient is one row of
+// partial sums a wave.
+#include "cross_attention.h"
+
+namespace sgl {
+namespace attn {
+namespace {
+
+template <typename T, int DP, int NQ, int NK>
+struct SmallLds {
+  static constexpr int R = 16 * NQ, K = 16 * NK;
+  static constexpr int kKeyTile = K * Tile<T, DP>::LD, kProbTile = R * Tile<T, K>::LD;
+  // k, then p and ds in its place; do, then q in its place
+  T a[kKeyTile > 2 * kProbTile ? kKeyTile : 2 * kProbTile];
+  T b[R * Tile<T, DP>::LD];
+  PosTile<K> pos;
+};
+
+template <typename T, int DP, int NQ, int NK>
+__global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each, const T *__restrict__ go,
+                                                           T *__restrict__ dq, T *__restrict__ dk,
+                                                           T *__restrict__ dv, float *__restrict__ part) {
+  using M = Mma<T>;
+  using L = Tile<T, DP>;
+  using Lds = SmallLds<T, DP, NQ, NK>;
+  using P = Tile<T, Lds::K>;
+  constexpr int ST = DP / M::KS, DB = DP / 16, R = Lds::R, K = Lds::K;
+  extern __shared__ __align__(16) char smem[];
+  const sgl_attention &p = a.p;
+  const int dh = p.head_dim;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
+  const size_t per = align_bytes(sizeof(Lds) + sizeof(float) * (size_t(a.G) * a.cols +
+                                                                (part != nullptr ? size_t(NQ) * 16 * a.cols : 0)));
+  Lds &s = *reinterpret_cast<Lds *>(smem + w * per);
+  float *table = reinterpret_cast<float *>(smem + w * per + sizeof(Lds));
+  float *cells = table + a.G * a.cols;
+  const int64_t gw = int64_t(blockIdx.x) * (blockDim.x / kWave) + w;
+  const int hk = int(gw % p.heads_kv);
+  const int64_t first = gw / p.heads_kv;
+  if (first >= each) return;   // (whole waves; there are no barriers)
+  const bool biased = p.bias != nullptr;
+  const Buckets bk = buckets_of(p);
+  if (biased) stage_bias(table, a, hk, lane, kWave);
+  if (part != nullptr) clear_cells(cells, NQ * 16 * a.cols);
+  wave_sync();
+  RowAt row[NQ];
+#pragma unroll
+  for (int b = 0; b < NQ; ++b) row[b] = row_at<false>(b * 16 + cl, b, a.G);
+  const float c = p.scale * kLog2e;
+  for (int64_t n = first; n < p.n; n += each) {
+    const Seq<T> q = seq_of<T>(p, n, hk, a.G);
+    const int64_t base = biased && q.qlen > 0 ? q.qpos[0] : 0;
+    const bool on_key = lane < K && q.qlen > 0 && key_live(q, p, lane);
+    const uint64_t live = __ballot(on_key);
+    int64_t kp = base;
+    if (biased && on_key) kp = q.kpos[lane * p.kpos_t];
+    FragOf<T> qf[NQ][ST], gf[NQ][ST];
+    int64_t qpos[NQ];
+    int qrel[NQ];
+    bool near_ = is_near(kp - base), ok[NQ];
+    float most = 0.f;
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+      ok[b] = row[b].i < q.qlen;
+      const int64_t at = out_row(a, n, hk, row[b].i, row[b].h);
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const int d = st * M::KS + g * M::E;
+        qf[b][st] = load_raw<T>(q.q + row[b].i * p.q_t + row[b].h * p.q_h, ok[b], d, dh);
+        gf[b][st] = load_raw<T>(go + at, ok[b], d, dh);
+      }
+      qpos[b] = biased && ok[b] ? q.qpos[row[b].i * p.qpos_t] : base;
+      near_ = near_ && is_near(qpos[b] - base);
+      qrel[b] = int(qpos[b] - base);
+    }
+    near_ = __all(near_);
+    wave_sync();   // the item before is done with the LDS
+    if (biased && lane < K) {
+      s.pos.pos[lane] = kp;
+      s.pos.rel[lane] = int(kp - base);
+    }
+    wave_sync();
+#pragma unroll
+    for (int b = 0; b < NQ; ++b)
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const int d = st * M::KS + g * M::E;
+        qf[b][st] = fix<T>(qf[b][st], d, dh);
+        gf[b][st] = fix<T>(gf[b][st], d, dh);
+        if constexpr (std::is_same_v<T, fp16_t>) {
+#pragma unroll
+          for (int e = 0; e < M::E; ++e) most = fmaxf(most, fabsf(float(gf[b][st][e])));
+        }
+        *reinterpret_cast<FragOf<T> *>(s.b + (b * 16 + cl) * L::LD + d) = gf[b][st];
+      }
+    float gs = 1.f;
+    if constexpr (std::is_same_v<T, fp16_t>) {
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, kWave));
+      gs = grad_scale<T>(most);
+    }
+    // scores and dp, (keys x rows)
+    float x[NQ][NK][4], y[NQ][NK][4];
+    int col[NQ][NK][4];
+#pragma unroll
+    for (int kb = 0; kb < NK; ++kb) {
+      FragOf<T> kf[ST], vf[ST];
+      const bool on_r = (live >> (kb * 16 + cl)) & 1;
+      const int64_t j = kb * 16 + cl;
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const int d = st * M::KS + g * M::E;
+        kf[st] = load_raw<T>(q.k + j * p.k_t, on_r, d, dh);
+        vf[st] = load_raw<T>(q.v + j * p.v_t, on_r, d, dh);
+      }
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const int d = st * M::KS + g * M::E;
+        kf[st] = fix<T>(kf[st], d, dh);
+        vf[st] = fix<T>(vf[st], d, dh);
+        *reinterpret_cast<FragOf<T> *>(s.a + (kb * 16 + cl) * L::LD + d) = kf[st];
+      }
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) {
+        f32x4 sc = {0.f, 0.f, 0.f, 0.f}, dp = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < ST; ++st) {
+          sc = M::mma(kf[st], qf[b][st], sc);
+          dp = M::mma(vf[st], gf[b][st], dp);
+        }
+        if (biased) columns4(col[b][kb], s.pos, kb * 16 + 4 * g, qrel[b], qpos[b], near_, 1, bk);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          float t = sc[v] * c;
+          if (biased) t += table[row[b].h * a.cols + col[b][kb][v]];
+          x[b][kb][v] = (live >> (kb * 16 + 4 * g + v)) & 1 ? t : -INFINITY;
+          y[b][kb][v] = dp[v];
+        }
+      }
+    }
+    // p, D and ds
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+      float mx = -INFINITY, sum = 0.f, de = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) mx = fmaxf(mx, x[b][kb][v]);
+      mx = groups_max(mx);
+      const float at = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+      for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          x[b][kb][v] = __builtin_amdgcn_exp2f(x[b][kb][v] - at);
+          sum += x[b][kb][v];
+        }
+      sum = groups_sum(sum);
+      const float inv = ok[b] && sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+      for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          x[b][kb][v] *= inv;
+          de += x[b][kb][v] * y[b][kb][v];
+        }
+      de = groups_sum(de);
+#pragma unroll
+      for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) y[b][kb][v] = x[b][kb][v] * (y[b][kb][v] - de);
+      if (part != nullptr) add_cells(cells + b * 16 * a.cols, col[b], y[b]);
+      if constexpr (std::is_same_v<T, fp16_t>) {
+#pragma unroll
+        for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            y[b][kb][v] *= gs;
+            x[b][kb][v] *= kProbUp<T>;
+          }
+      }
+    }
+    const float fk = p.scale / gs;
+    // dq (head size x rows)
+    wave_sync();
+    {
+      f32x4 acc[NQ][DB];
+#pragma unroll
+      for (int b = 0; b < NQ; ++b)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int st = 0; st < K / M::KS; ++st) {
+        FragOf<T> df[NQ];
+#pragma unroll
+        for (int b = 0; b < NQ; ++b) df[b] = frag_of<T>(y[b], st);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const FragOf<T> kt = L::template frag_t<K>(s.a, d * 16, st * M::KS);
+#pragma unroll
+          for (int b = 0; b < NQ; ++b) acc[b][d] = M::mma(kt, df[b], acc[b][d]);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) {
+        if (row[b].i < p.lq) {
+          const int64_t at = out_row(a, n, hk, row[b].i, row[b].h);
+#pragma unroll
+          for (int d = 0; d < DB; ++d) store4(dq + at, d * 16 + 4 * g, dh, acc[b][d] * fk);
+        }
+      }
+    }
+    // p and ds as [row][key], over k
+    T *ps = s.a, *ds = s.a + R * P::LD;
+    wave_sync();
+#pragma unroll
+    for (int b = 0; b < NQ; ++b)
+#pragma unroll
+      for (int kb = 0; kb < NK; ++kb) {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 pv, dvv;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          pv[v] = T(x[b][kb][v]);
+          dvv[v] = T(y[b][kb][v]);
+        }
+        const int at = (b * 16 + cl) * P::LD + kb * 16 + 4 * g;
+        *reinterpret_cast<T4 *>(ps + at) = pv;
+        *reinterpret_cast<T4 *>(ds + at) = dvv;
+      }
+    wave_sync();
+    // dv, then dk (head size x keys), do and then q in s.b
+    constexpr int RS = (R + M::KS - 1) / M::KS;   // steps over the rows
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      if (which == 1) {
+        wave_sync();
+#pragma unroll
+        for (int b = 0; b < NQ; ++b)
+#pragma unroll
+          for (int st = 0; st < ST; ++st)
+            *reinterpret_cast<FragOf<T> *>(s.b + (b * 16 + cl) * L::LD + st * M::KS + g * M::E) = qf[b][st];
+        wave_sync();
+      }
+      T *out = which == 0 ? dv : dk;
+      const T *src = which == 0 ? ps : ds;
+      const float f = which == 0 ? 1.f / kProbUp<T> : fk;
+#pragma unroll
+      for (int kb = 0; kb < NK; ++kb) {
+        FragOf<T> pf[RS];
+#pragma unroll
+        for (int st = 0; st < RS; ++st) pf[st] = P::template frag_t<R>(src, kb * 16, st * M::KS);
+        const int64_t j = kb * 16 + cl;
+        const int64_t at = ((n * p.lk + j) * p.heads_kv + hk) * dh;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int st = 0; st < RS; ++st)
+            acc = M::mma(L::template frag_t<R>(s.b, d * 16, st * M::KS), pf[st], acc);
+          if (j < p.lk) store4(out + at, d * 16 + 4 * g, dh, acc * f);
+        }
+      }
+    }
+  }
+  if (part != nullptr) {
+    wave_sync();
+    float *out = part + (first * p.heads_kv + hk) * a.G * a.cols;
+    for (int x = lane; x < a.G * a.cols; x += kWave) {
+      const int h = x / a.cols, cidx = x - h * a.cols;
+      float t = 0.f;
+      for (int r = 0; r < R; ++r) {
+        const int e = (r & ~15) | ((r + cidx) & 15);
+        if (e % a.G == h) t += cells[((e >> 4) * a.cols + cidx) * 16 + (e & 15)];
+      }
+      out[x] = t;
+    }
+  }
+}
+
+// Waves a key head: enough to fill the GPU four waves a SIMD deep, the
+// sequences in equal numbers.
+int64_t small_each(const Args &a) {
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(a.p.n, 4096 / a.p.heads_kv));
+  const int64_t per = (a.p.n + most - 1) / most;
+  return (a.p.n + per - 1) / per;
+}
+
+template <typename T, int DP, int NQ, int NK>
+int launch_small(const Args &a, const void *go, void *dq, void *dk, void *dv, float *part, hipStream_t s) {
+  const size_t per =
+      align_bytes(sizeof(SmallLds<T, DP, NQ, NK>) +
+                  sizeof(float) * (size_t(a.G) * a.cols + (part != nullptr ? size_t(NQ) * 16 * a.cols : 0)));
+  const int64_t wpb = std::min<int64_t>(kWaves, 160 * 1024 / int64_t(per));   // waves a workgroup
+  SGL_REQUIRE(wpb > 0, "cross_attention_backward: %zu bytes of LDS", per);
+  const size_t lds = per * size_t(wpb);
+  SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_small_bwd<T, DP, NQ, NK>), lds));
+  const int64_t each = small_each(a), waves = each * a.p.heads_kv;
+  launch(&k_attn_small_bwd<T, DP, NQ, NK>, dim3(unsigned((waves + wpb - 1) / wpb)), dim3(unsigned(wpb) * kWave), lds, s, a, each,
+         static_cast<const T *>(go), static_cast<T *>(dq), static_cast<T *>(dk), static_cast<T *>(dv), part);
+  SGL_CHECK_LAUNCH();
+  return SGL_OK;
+}
+
+}  // namespace
+
+size_t small_backward_bytes(const Args &a) { return sizeof(float) * size_t(small_each(a)) * a.p.heads_q * a.cols; }
+
+int run_small_backward(const Args &a, const void *go, void *dq, void *dk, void *dv, float *dbias, void *ws,
+                       hipStream_t s) {
+  float *part = dbias != nullptr ? static_cast<float *>(ws) : nullptr;
+  const int rc = by_instance(a.p, [&](auto t, auto dp) {
+    using T = decltype(t);
+    constexpr int DP = decltype(dp)::value;
+    if (a.rows <= 16) {
+      if (a.p.lk <= 32) return launch_small<T, DP, 1, 2>(a, go, dq, dk, dv, part, s);
+      return launch_small<T, DP, 1, 4>(a, go, dq, dk, dv, part, s);
+    }
+    if (a.p.lk <= 32) return launch_small<T, DP, 2, 2>(a, go, dq, dk, dv, part, s);
+    return launch_small<T, DP, 2, 4>(a, go, dq, dk, dv, part, s);
+  });
+  if (rc != SGL_OK) return rc;
+  if (dbias != nullptr) sum_rows(part, small_each(a), a.p.heads_q * a.cols, dbias, s);
+  SGL_CHECK_LAUNCH();
+  return SGL_OK;
+}
+
+}  // namespace attn
+}  // namespace sgl

@@ -41,40 +41,39 @@ __device__ __forceinline__ void sigmoid_pair(float x, float &s, float &sn) {
 }
 
 // out[c] = sum over rows of part[row][c], c < width, in double and in one
-// order: 16 waves of a workgroup take rows w, w + 16, ... of 64 columns each.
-// blockIdx.y selects one of several such matrices.
-constexpr int kSumWaves = 16;
-static __global__ __launch_bounds__(kSumWaves * 64) void k_sum_rows(const float *__restrict__ part, int64_t rows,
-                                                                    int width, int64_t part_y,
-                                                                    float *__restrict__ out, int64_t out_y) {
-  __shared__ double s[kSumWaves][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane;
-  part += int64_t(blockIdx.y) * part_y;
+// order. A workgroup takes 8 columns (32 bytes of each row), a thread every
+// 128th row of one, 8 loads in flight: narrow matrices of many rows still
+// give every CU something (4,000 x 172: 20 us with 64 columns a workgroup).
+constexpr int kSumCols = 8, kSumRows = 128;
+static __global__ __launch_bounds__(kSumCols * kSumRows) void k_sum_rows(const float *__restrict__ part, int64_t rows,
+                                                                         int width, float *__restrict__ out) {
+  __shared__ double s[kSumRows][kSumCols];
+  const int col = threadIdx.x % kSumCols, w = threadIdx.x / kSumCols;
+  const int c = blockIdx.x * kSumCols + col;
   double a = 0.0;
   if (c < width) {
     int64_t r = w;
-    for (; r + 7 * kSumWaves < rows; r += 8 * kSumWaves) {
+    for (; r + 7 * kSumRows < rows; r += 8 * kSumRows) {
       float v[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = part[(r + u * kSumWaves) * width + c];
+      for (int u = 0; u < 8; ++u) v[u] = part[(r + u * kSumRows) * width + c];
 #pragma unroll
       for (int u = 0; u < 8; ++u) a += double(v[u]);
     }
-    for (; r < rows; r += kSumWaves) a += double(part[r * width + c]);
+    for (; r < rows; r += kSumRows) a += double(part[r * width + c]);
   }
-  s[w][lane] = a;
+  s[w][col] = a;
   __syncthreads();
-  if (w == 0 && c < width) {
-    for (int i = 1; i < kSumWaves; ++i) a += s[i][lane];
-    out[int64_t(blockIdx.y) * out_y + c] = float(a);
+  for (int d = kSumRows / 2; d > 0; d >>= 1) {
+    if (w < d) s[w][col] += s[w + d][col];
+    __syncthreads();
   }
+  if (w == 0 && c < width) out[c] = float(s[0][col]);
 }
 
-inline void sum_rows(const float *part, int64_t rows, int width, float *out, hipStream_t stream, int count = 1,
-                     int64_t part_y = 0, int64_t out_y = 0) {
-  launch(&k_sum_rows, dim3(unsigned((width + 63) / 64), unsigned(count)), dim3(kSumWaves * 64), 0, stream, part, rows,
-         width, part_y, out, out_y);
+inline void sum_rows(const float *part, int64_t rows, int width, float *out, hipStream_t stream) {
+  launch(&k_sum_rows, dim3(unsigned((width + kSumCols - 1) / kSumCols)), dim3(kSumCols * kSumRows), 0, stream, part,
+         rows, width, out);
 }
 
 }  // namespace sgl

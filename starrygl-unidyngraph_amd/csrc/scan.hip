@@ -32,6 +32,7 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kKeep = 8;             // steps between kept states
 constexpr int64_t kFill = 1 << 18;   // threads that fill the GPU: 16 waves a CU
+constexpr int64_t kPieces = kFill + kFill / 4;   // pieces x channel groups: the 5 waves a SIMD of the backward, once
 constexpr int kSubs = 8;             // pieces a workgroup of the cut form: kLanes channel groups each
 constexpr int kLanes = kBlock / kSubs;
 constexpr int kMaxSupers = 32;
@@ -392,7 +393,7 @@ __global__ __launch_bounds__(kBlock) void k_scan_bwd(ScanArgs a, const float *__
 int scan_vec(int32_t dtype, int32_t D) { return dtype != SGL_FP32 && D % 2 == 0 ? 2 : 1; }
 
 // Sequences whole where their channels fill half the GPU or a piece would be
-// shorter than kMinPiece; else cut so that the pieces fill it twice.
+// shorter than kMinPiece; else cut so that the pieces fill it.
 struct ScanPlan {
   int vec, supers;
   int64_t piece, groups;       // groups: rows of decay's partial sums
@@ -404,7 +405,7 @@ ScanPlan scan_plan(int32_t dtype, int64_t N, int64_t L, int32_t D) {
   const int64_t dv = (D + p.vec - 1) / p.vec, threads = N * dv;
   int64_t supers = 0;
   if (2 * threads < kFill) {
-    const int64_t want = (2 * kFill + threads * kSubs - 1) / (threads * kSubs);
+    const int64_t want = (kPieces + threads * kSubs - 1) / (threads * kSubs);
     supers = std::min<int64_t>({want, L / (kMinPiece * kSubs), int64_t(kMaxSupers)});
   }
   p.supers = 0;
@@ -414,8 +415,8 @@ ScanPlan scan_plan(int32_t dtype, int64_t N, int64_t L, int32_t D) {
     p.piece = (p.piece + kKeep - 1) / kKeep * kKeep;
     p.supers = int((L + p.piece * kSubs - 1) / (p.piece * kSubs));
     p.groups = N * p.supers;
-  } else {   // as many as fill the GPU twice, each with as many sequences
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(N, 2 * kFill / dv)), each = (N + most - 1) / most;
+  } else {   // as many as fill the GPU, each with as many sequences
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(N, kFill / dv)), each = (N + most - 1) / most;
     p.groups = (N + each - 1) / each;
   }
   p.sup = sgl::align_up(sizeof(float2) * size_t(N * p.supers * D));

@@ -109,8 +109,9 @@ SIGNATURES: dict[str, tuple] = {
     "sgl_gated_scan_forward": (ctypes.c_int, [_i32, _i64, _i64, _i32] + _SCAN + [_vp] * 4 + [_sz, _vp]),
     "sgl_gated_scan_backward": (ctypes.c_int, [_i32, _i64, _i64, _i32] + _SCAN + [_vp] * 8 + [_sz, _vp]),
     "sgl_cross_attention_workspace_bytes": (_sz, [_vp, _i32]),
-    "sgl_cross_attention_forward": (ctypes.c_int, [_vp] * 4 + [_sz, _vp]),
-    "sgl_cross_attention_backward": (ctypes.c_int, [_vp] * 9 + [_sz, _vp]),
+    "sgl_cross_attention_saves": (_i32, [_vp]),
+    "sgl_cross_attention_forward": (ctypes.c_int, [_vp] * 5 + [_sz, _vp]),
+    "sgl_cross_attention_backward": (ctypes.c_int, [_vp] * 10 + [_sz, _vp]),
     "sgl_gated_norm_workspace_bytes": (_sz, [_i64, _i32]),
     "sgl_gated_norm_forward": (ctypes.c_int, [_i32, _i64, _i32] + _NORM + [_vp] * 3),
     "sgl_gated_norm_backward": (ctypes.c_int, [_i32, _i64, _i32] + _NORM + [_vp] * 6 + [_i32, _vp, _sz, _vp]),

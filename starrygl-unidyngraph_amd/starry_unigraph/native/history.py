@@ -234,14 +234,16 @@ class _Attend(torch.autograd.Function):
         a, need = _Attend.problem(q, k, v, bias, fixed, resolution, two_sided, scale), any(ctx.needs_input_grad)
         N, Lq, Hq, dh = q.shape
         o = torch.empty(N, Lq, Hq, dh, dtype=q.dtype, device=dev)
-        lse = torch.empty(N, Lq * Hq, dtype=torch.float32, device=dev)
+        saves = lib.sgl_cross_attention_saves(ctypes.byref(a)) if need else 0
+        lse = torch.empty(N, Lq * Hq, dtype=torch.float32, device=dev) if saves & 1 else None
+        rest = torch.empty_like(o) if saves & 2 else None
         nb = lib.sgl_cross_attention_workspace_bytes(ctypes.byref(a), 0)
         ws = _capi.workspace(nb, dev) if nb else None
         with _guard(dev):
-            _capi.check(lib.sgl_cross_attention_forward(ctypes.byref(a), P(o), P(lse), P(ws), nb,
+            _capi.check(lib.sgl_cross_attention_forward(ctypes.byref(a), P(o), P(rest), P(lse), P(ws), nb,
                                                         _capi.stream_of(dev)), "cross_attention")
         if need:
-            ctx.save_for_backward(q, k, v, bias, o, lse, *fixed)
+            ctx.save_for_backward(q, k, v, bias, o if saves & 1 else None, rest, lse, *fixed)
             ctx.form = (resolution, two_sided, scale)
         return o
 
@@ -262,11 +264,11 @@ class _Attend(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, go):
-        q, k, v, bias, o, lse, *fixed = ctx.saved_tensors
+        q, k, v, bias, o, rest, lse, *fixed = ctx.saved_tensors
         lib, P, dev = _capi.lib(), _capi.ptr, q.device
         a = _Attend.problem(q, k, v, bias, fixed, *ctx.form)
         go = go.contiguous()
-        dq = torch.empty_like(o)
+        dq = torch.empty_like(go)
         dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
         dv = torch.empty(v.shape, dtype=v.dtype, device=dev)
         db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[3] else None
@@ -274,7 +276,7 @@ class _Attend(torch.autograd.Function):
         ws = _capi.workspace(nb, dev) if nb else None
         with _guard(dev):
             _capi.check(lib.sgl_cross_attention_backward(
-                ctypes.byref(a), P(o), P(lse), P(go), P(dq), P(dk), P(dv), P(db), P(ws), nb, _capi.stream_of(dev)),
+                ctypes.byref(a), P(o), P(rest), P(lse), P(go), P(dq), P(dk), P(dv), P(db), P(ws), nb, _capi.stream_of(dev)),
                 "cross_attention backward")
         return dq, dk, dv, db, None, None, None, None
 

@@ -104,7 +104,7 @@ def test_c_entries_refuse_bad_arguments():
     assert scan(0, 1, 1, 4, gaps=one) == 1 and "both" in err()
     assert scan(0, 1, 100000, 4) == 3 and "workspace" in err()
     p = _capi.Attention(dtype=0, heads_q=4, heads_kv=3, head_dim=8, n=1, lq=1, lk=1)
-    fwd = lambda: L.sgl_cross_attention_forward(ctypes.byref(p), one, one, None, 0, None)
+    fwd = lambda: L.sgl_cross_attention_forward(ctypes.byref(p), one, None, None, None, 0, None)
     assert fwd() == 1 and "heads" in err()
     p.heads_kv, p.head_dim = 2, 200
     assert fwd() == 1 and "head size" in err()
@@ -114,8 +114,13 @@ def test_c_entries_refuse_bad_arguments():
     p.buckets = 8
     assert fwd() == 1 and "positions" in err()
     p.q_pos = p.k_pos = 256
-    assert L.sgl_cross_attention_backward(ctypes.byref(p), one, one, one, one, one, one, one, None, 0, None) == 3
-    assert "workspace" in err()
+    back = lambda rest: L.sgl_cross_attention_backward(ctypes.byref(p), one, rest, one, one, one, one, one, one, None,
+                                                       0, None)
+    assert back(None) == 3 and "workspace" in err()
+    p.dtype, p.lk = 1, 100
+    assert L.sgl_cross_attention_saves(ctypes.byref(p)) == 3
+    assert back(None) == 1 and "rest" in err()
+    assert back(one) == 3 and "workspace" in err()
     norm = lambda dt, r, d, n=3: L.sgl_gated_norm_backward(
         dt, r, d, one, 1, one, 1, one, 1, one, None, None, None, None, 1e-5, 0, None, None, one, one, one, one, n,
         None, 0, None)
