@@ -285,42 +285,51 @@ __device__ __forceinline__ void stage_bias(float *table, const Args &a, int hk, 
   for (int c = tid; c < a.G * a.cols; c += threads) table[c] = a.p.bias[int64_t(hk) * a.G * a.cols + c] * kLog2e;
 }
 
+// A power of two near 1 / most (1 for 0 and what is not finite).
+__device__ __forceinline__ float unit_scale(float most) {
+  return most > 0.f && most < INFINITY ? ldexpf(1.f, -max(ilogbf(most), -126)) : 1.f;
+}
+
 // fp16 gradients: a power of two that brings the largest |do| near one, so
 // that ds keeps fp16's digits whatever the loss is scaled by.
 template <typename T>
 __device__ __forceinline__ float grad_scale(float most) {
-  if constexpr (std::is_same_v<T, fp16_t>) {
-    return most > 0.f && most < INFINITY ? ldexpf(1.f, -ilogbf(most)) : 1.f;
-  } else {
-    return 1.f;
-  }
+  return std::is_same_v<T, fp16_t> ? unit_scale(most) : 1.f;
 }
 // fp16: p goes into a product as 2^10 p, away from the subnormals.
 template <typename T>
 constexpr float kProbUp = std::is_same_v<T, fp16_t> ? 1024.f : 1.f;
 
-// A row's cells of the bias gradient: 16 lanes (c) x columns a wave; the four
-// lane groups add one after the other, so that every cell has one writer at a
-// time and sums in one order.
-__device__ __forceinline__ void clear_cells(float *cells, int n) {
-  for (int i = threadIdx.x & 63; i < n; i += kWave) cells[i] = 0.f;
+// The bias gradient's cells in LDS: [column][16] sums of ds for a set of row
+// blocks whose row c has one head, in fixed point (34 fractional bits in an
+// int64, relative to a power of two near the largest |do|): integer adds give
+// the same sum in any order, and the LDS adds them at 7 to 8 clocks an
+// instruction, four lanes a cell included, where float adds take 194 (3 a
+// lane; a read, an add and a write 11, in cells of a lane's own). A value
+// holds to 2^29 times that power; `seen`, the sum of magnitudes, tells beyond
+// it (and of NaN and infinities), and the gradient is NaN then.
+constexpr int kCellBits = 34;
+constexpr float kCellMax = 536870912.f;   // 2^29
+typedef unsigned long long Cell;
+__device__ __forceinline__ void clear_cells(Cell *cells, int n, int tid, int threads) {
+  for (int i = tid; i < n; i += threads) cells[i] = 0;
 }
 template <int N>
-__device__ __forceinline__ void add_cells(float *cells, const int (&col)[N][4], const float (&x)[N][4]) {
-  const int lane = threadIdx.x & 63, c = lane & 15;
+__device__ __forceinline__ void add_cells(Cell *cells, const int (&col)[N][4], const float (&x)[N][4], float up,
+                                          float &seen) {
+  const int c = threadIdx.x & 15;
+  const float f = up * 4.f;   // 2^34 = 2^2 2^32
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    if ((lane >> 4) == g) {
+  for (int k = 0; k < N; ++k)
 #pragma unroll
-      for (int k = 0; k < N; ++k)
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-          __hip_atomic_fetch_add(cells + col[k][v] * 16 + c, x[k][v], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    for (int v = 0; v < 4; ++v) {
+      const float t = x[k][v] * f, hi = floorf(t);
+      seen += fabsf(t);
+      const Cell val = (Cell(uint32_t(int(hi))) << 32) | uint32_t((t - hi) * 4294967296.f);
+      __hip_atomic_fetch_add(cells + col[k][v] * 16 + c, val, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
-    wave_sync();
-  }
 }
-
+__device__ __forceinline__ bool cells_hold(float seen) { return seen < 4.f * kCellMax; }
 // ------------------------------------------------------------------ launches
 int run_forward(const Args &a, void *o, void *rest, float *lse, void *workspace, hipStream_t s);
 size_t forward_bytes(const Args &a);

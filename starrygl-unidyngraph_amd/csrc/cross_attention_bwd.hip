@@ -16,7 +16,16 @@ template <typename T, int DP>
 struct DqLds {
   T k[kKeys * Tile<T, DP>::LD], v[kKeys * Tile<T, DP>::LD];
   PosTile<kKeys> pos;
+  float red[kWaves];
 };
+
+// Sets of cells a workgroup needs: where 16 rows hold every head the same
+// number of times, row c of every block has the same head (SHARE: of every
+// first block, and of every second one), and the waves share their cells.
+template <int NQ, bool SHARE>
+__host__ __device__ __forceinline__ int cell_sets(int G) {
+  return 16 % (SHARE ? G / 2 : G) == 0 ? (SHARE ? 2 : 1) : kWaves * NQ;
+}
 
 template <typename T, int DP, int NQ, bool SHARE>
 __global__ __launch_bounds__(kBlock) void k_attn_dq(Args a, int64_t tiles, const T *__restrict__ o,
@@ -34,8 +43,8 @@ __global__ __launch_bounds__(kBlock) void k_attn_dq(Args a, int64_t tiles, const
   const sgl_attention &p = a.p;
   const int dh = p.head_dim;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
-  // cells [wave][block][column][16]
-  float *cells = table + a.G * a.cols, *mine = cells + w * NQ * a.cols * 16;
+  const int sets = cell_sets<NQ, SHARE>(a.G);
+  Cell *cells = reinterpret_cast<Cell *>(smem + align_bytes(sizeof(s) + sizeof(float) * a.G * a.cols));
   int64_t id = blockIdx.x;
   const int64_t rt = id % tiles;
   id /= tiles;
@@ -49,13 +58,13 @@ __global__ __launch_bounds__(kBlock) void k_attn_dq(Args a, int64_t tiles, const
   const bool any = i0 < q.qlen;
   const bool one_tile = q.klen <= kKeys;
   if (biased) stage_bias(table, a, hk, threadIdx.x, kBlock);
-  if (part != nullptr) clear_cells(mine, NQ * a.cols * 16);
+  if (part != nullptr) clear_cells(cells, sets * a.cols * 16, threadIdx.x, kBlock);
   RowAt row[NQ];
   bool in[NQ], ok[NQ];
   FragOf<T> qf[NQ][ST], gf[NQ][ST];
   int64_t qpos[NP];
   int qrel[NP];
-  float delta[NQ], ls[NQ], gs[NQ];
+  float delta[NQ], ls[NQ], gs[NQ], top = 0.f;
   const int64_t base = biased && any ? q.qpos[i0 * p.qpos_t] : 0;
   const int64_t stat0 = (n * p.heads_kv + hk) * a.rows;
   bool qnear = true;
@@ -85,6 +94,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_dq(Args a, int64_t tiles, const
     }
     delta[b] = groups_sum(delta[b]);
     most = groups_max(most);
+    top = fmaxf(top, most);
     gs[b] = grad_scale<T>(most);
     const int64_t r = stat0 + row[b].i * a.G + row[b].h;
     ls[b] = ok[b] ? lse[r] : INFINITY;
@@ -97,6 +107,14 @@ __global__ __launch_bounds__(kBlock) void k_attn_dq(Args a, int64_t tiles, const
   }
   qnear = __all(qnear);
   const float c = p.scale * kLog2e;
+  float up = 1.f, seen = 0.f;   // the cells' power of two, for the whole workgroup
+  if (part != nullptr) {
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
+    if (lane == 0) s.red[w] = top;
+    __syncthreads();
+    up = unit_scale(fmaxf(fmaxf(s.red[0], s.red[1]), fmaxf(s.red[2], s.red[3])));
+  }
   f32x4 acc[NQ][DB];
 #pragma unroll
   for (int b = 0; b < NQ; ++b)
@@ -202,7 +220,10 @@ __global__ __launch_bounds__(kBlock) void k_attn_dq(Args a, int64_t tiles, const
         for (int v = 0; v < 4; ++v) y[b][kb][v] = x[b][kb][v] * (y[b][kb][v] - delta[b]);
     if (part != nullptr) {
 #pragma unroll
-      for (int b = 0; b < NQ; ++b) add_cells(mine + b * a.cols * 16, col[b < NP ? b : 0], y[b]);
+      for (int b = 0; b < NQ; ++b) {
+        const int set = sets == kWaves * NQ ? w * NQ + b : SHARE ? b : 0;
+        add_cells(cells + set * a.cols * 16, col[b < NP ? b : 0], y[b], up, seen);
+      }
     }
     if constexpr (std::is_same_v<T, fp16_t>) {
 #pragma unroll
@@ -234,26 +255,27 @@ __global__ __launch_bounds__(kBlock) void k_attn_dq(Args a, int64_t tiles, const
     for (int d = 0; d < DB; ++d) store4(dq + at, d * 16 + 4 * g, dh, acc[b][d] * f);
   }
   if (part != nullptr) {
-    // cell (wave, block, column, c) belongs to the head of that block's row c:
-    // a thread sums a (head, column) over them in order
+    // cell (set, column, c) belongs to the head of its blocks' row c: a thread
+    // sums a (head, column) over them
+    const bool held = __all(cells_hold(seen));
     __syncthreads();
+    if (lane == 0) s.red[w] = held ? 0.f : NAN;
+    __syncthreads();
+    const float bad = s.red[0] + s.red[1] + s.red[2] + s.red[3];
     float *out = part + ((n * tiles + rt) * p.heads_kv + hk) * a.G * a.cols;
     for (int x = threadIdx.x; x < a.G * a.cols; x += kBlock) {
       const int h = x / a.cols, cidx = x - h * a.cols;
-      float t = 0.f;
-      for (int wb = 0; wb < kWaves * NQ; ++wb) {
-        const int ww = wb / NQ, b = wb - ww * NQ;
-        const float *cell = cells + (wb * a.cols + cidx) * 16;
-        const int64_t first = SHARE ? t0 + ww * 16 : t0 + wb * 16;
-        int hh = row_at<SHARE>(first, b, a.G).h;   // the head of c = 0, then in turn
+      long long t = 0;
+      for (int set = 0; set < sets; ++set) {
+        const bool own = sets == kWaves * NQ;
+        const int ww = own ? set / NQ : 0, b = own ? set % NQ : SHARE ? set : 0;
+        const int h0 = row_at<SHARE>(SHARE ? t0 + ww * 16 : t0 + (own ? set : 0) * 16, b, a.G).h;   // of c = 0
         for (int i = 0; i < 16; ++i) {
           const int e = (i + cidx) & 15;   // (rotated: neighbouring columns in different banks)
-          int he = hh + (SHARE ? 2 : 1) * e;
-          he = he % a.G;
-          if (he == h) t += cell[e];
+          if ((h0 + (SHARE ? 2 : 1) * e) % a.G == h) t += static_cast<long long>(cells[(set * a.cols + cidx) * 16 + e]);
         }
       }
-      out[x] = t;
+      out[x] = float(double(t) * (1.0 / double(1ll << kCellBits)) / double(up)) + bad;
     }
   }
 }
@@ -451,8 +473,8 @@ size_t stat_bytes(const Args &a) { return align_up(sizeof(float2) * size_t(a.p.n
 template <typename T, int DP, int NQ, bool SHARE>
 int launch_dq(const Args &a, int64_t tiles, const void *o, const void *rest, const float *lse, const void *go, void *dq,
               float2 *stat, float *part, hipStream_t s) {
-  const size_t lds = sizeof(DqLds<T, DP>) + sizeof(float) * size_t(a.G) * a.cols +
-                     (part != nullptr ? sizeof(float) * kWaves * NQ * 16 * size_t(a.cols) : 0);
+  const size_t lds = align_bytes(sizeof(DqLds<T, DP>) + sizeof(float) * size_t(a.G) * a.cols) +
+                     (part != nullptr ? sizeof(Cell) * cell_sets<NQ, SHARE>(a.G) * 16 * size_t(a.cols) : 0);
   SGL_REQUIRE(lds <= 160 * 1024, "cross_attention_backward: %zu bytes of LDS", lds);
   SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_dq<T, DP, NQ, SHARE>), lds));
   launch(&k_attn_dq<T, DP, NQ, SHARE>, dim3(unsigned(a.p.n * a.p.heads_kv * tiles)), dim3(kBlock), lds, s, a, tiles,

@@ -24,6 +24,12 @@ struct SmallLds {
   PosTile<K> pos;
 };
 
+template <typename Lds>
+__host__ __device__ __forceinline__ size_t small_lds(const Args &a, int nq, bool cells) {   // bytes a wave
+  return align_bytes(sizeof(Lds) + sizeof(float) * size_t(a.G) * a.cols) +
+         (cells ? sizeof(Cell) * size_t(16 % a.G == 0 ? 1 : nq) * 16 * a.cols : 0);
+}
+
 template <typename T, int DP, int NQ, int NK>
 __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each, const T *__restrict__ go,
                                                            T *__restrict__ dq, T *__restrict__ dk,
@@ -37,11 +43,11 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
   const sgl_attention &p = a.p;
   const int dh = p.head_dim;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
-  const size_t per = align_bytes(sizeof(Lds) + sizeof(float) * (size_t(a.G) * a.cols +
-                                                                (part != nullptr ? size_t(NQ) * 16 * a.cols : 0)));
+  const size_t per = small_lds<Lds>(a, NQ, part != nullptr);
   Lds &s = *reinterpret_cast<Lds *>(smem + w * per);
   float *table = reinterpret_cast<float *>(smem + w * per + sizeof(Lds));
-  float *cells = table + a.G * a.cols;
+  Cell *cells = reinterpret_cast<Cell *>(smem + w * per + align_bytes(sizeof(Lds) + sizeof(float) * a.G * a.cols));
+  const int sets = 16 % a.G == 0 ? 1 : NQ;   // (one: row c of either block has the same head)
   const int64_t gw = int64_t(blockIdx.x) * (blockDim.x / kWave) + w;
   const int hk = int(gw % p.heads_kv);
   const int64_t first = gw / p.heads_kv;
@@ -49,7 +55,8 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
   const bool biased = p.bias != nullptr;
   const Buckets bk = buckets_of(p);
   if (biased) stage_bias(table, a, hk, lane, kWave);
-  if (part != nullptr) clear_cells(cells, NQ * 16 * a.cols);
+  if (part != nullptr) clear_cells(cells, sets * 16 * a.cols, lane, kWave);
+  float up = 0.f, seen = 0.f;   // the cells' power of two (0: nothing in them yet)
   wave_sync();
   RowAt row[NQ];
 #pragma unroll
@@ -95,17 +102,27 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
         const int d = st * M::KS + g * M::E;
         qf[b][st] = fix<T>(qf[b][st], d, dh);
         gf[b][st] = fix<T>(gf[b][st], d, dh);
-        if constexpr (std::is_same_v<T, fp16_t>) {
 #pragma unroll
-          for (int e = 0; e < M::E; ++e) most = fmaxf(most, fabsf(float(gf[b][st][e])));
-        }
+        for (int e = 0; e < M::E; ++e) most = fmaxf(most, fabsf(float(gf[b][st][e])));
         *reinterpret_cast<FragOf<T> *>(s.b + (b * 16 + cl) * L::LD + d) = gf[b][st];
       }
     float gs = 1.f;
-    if constexpr (std::is_same_v<T, fp16_t>) {
+    if (std::is_same_v<T, fp16_t> || part != nullptr) {
 #pragma unroll
       for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, kWave));
       gs = grad_scale<T>(most);
+    }
+    if (part != nullptr && most > 0.f) {   // (uniform) larger gradients than the cells' power is for: cells shifted
+      const float want = unit_scale(most);
+      if (up == 0.f) {
+        up = want;
+      } else if (want < up) {
+        const int by = min(ilogbf(up) - ilogbf(want), 63);
+        for (int i = lane; i < sets * 16 * a.cols; i += kWave) cells[i] = Cell(static_cast<long long>(cells[i]) >> by);
+        seen = ldexpf(seen, -by);
+        up = want;
+        wave_sync();
+      }
     }
     // scores and dp, (keys x rows)
     float x[NQ][NK][4], y[NQ][NK][4];
@@ -177,7 +194,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
       for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
         for (int v = 0; v < 4; ++v) y[b][kb][v] = x[b][kb][v] * (y[b][kb][v] - de);
-      if (part != nullptr) add_cells(cells + b * 16 * a.cols, col[b], y[b]);
+      if (part != nullptr) add_cells(cells + (sets == 1 ? 0 : b) * 16 * a.cols, col[b], y[b], up, seen);
       if constexpr (std::is_same_v<T, fp16_t>) {
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb)
@@ -273,15 +290,16 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
   }
   if (part != nullptr) {
     wave_sync();
+    const bool held = __all(cells_hold(seen));
     float *out = part + (first * p.heads_kv + hk) * a.G * a.cols;
     for (int x = lane; x < a.G * a.cols; x += kWave) {
       const int h = x / a.cols, cidx = x - h * a.cols;
-      float t = 0.f;
-      for (int r = 0; r < R; ++r) {
+      long long t = 0;
+      for (int r = 0; r < sets * 16; ++r) {
         const int e = (r & ~15) | ((r + cidx) & 15);
-        if (e % a.G == h) t += cells[((e >> 4) * a.cols + cidx) * 16 + (e & 15)];
+        if (e % a.G == h) t += static_cast<long long>(cells[((e >> 4) * a.cols + cidx) * 16 + (e & 15)]);
       }
-      out[x] = t;
+      out[x] = held ? float(double(t) * (1.0 / double(1ll << kCellBits)) / double(up == 0.f ? 1.f : up)) : NAN;
     }
   }
 }
@@ -296,9 +314,7 @@ int64_t small_each(const Args &a) {
 
 template <typename T, int DP, int NQ, int NK>
 int launch_small(const Args &a, const void *go, void *dq, void *dk, void *dv, float *part, hipStream_t s) {
-  const size_t per =
-      align_bytes(sizeof(SmallLds<T, DP, NQ, NK>) +
-                  sizeof(float) * (size_t(a.G) * a.cols + (part != nullptr ? size_t(NQ) * 16 * a.cols : 0)));
+  const size_t per = small_lds<SmallLds<T, DP, NQ, NK>>(a, NQ, part != nullptr);
   const int64_t wpb = std::min<int64_t>(kWaves, 160 * 1024 / int64_t(per));   // waves a workgroup
   SGL_REQUIRE(wpb > 0, "cross_attention_backward: %zu bytes of LDS", per);
   const size_t lds = per * size_t(wpb);
