@@ -899,8 +899,9 @@ int sgl_gated_scan_backward(int32_t dtype, int64_t N, int64_t L, int32_t D,
                             size_t workspace_bytes, hipStream_t stream);
 
 /* Attention of the rows of n sequences of up to lq query events over up to lk
- * key events, heads_q query heads sharing heads_kv key heads, each of
- * head_dim <= 128 elements, with a bias table over time distances. Tensors are
+ * key events, heads_q query heads sharing heads_kv key heads, each of head_dim
+ * elements (16 bytes of them at least, 128 at most: pad shorter heads with
+ * zeros), with a bias table over time distances. Tensors are
  * addressed by strides in elements, the last dimension contiguous. q_lens,
  * k_lens: int32 [n] (clamped; NULL: all). key_mask: bytes, 0 a dead key.
  * bias: fp32 [heads_q][buckets, or 2 buckets if two_sided] (at most 64

@@ -65,7 +65,7 @@ __device__ __forceinline__ FragOf<T> frag_of(const float (&x)[NB][4], int s) {
 // Elements [d, d + E) of a row of dh, 0 past it, from one 16-byte load at any
 // alignment: the last, partial vector is loaded from dh - E and moved down
 // (`fix`, after the load has landed, so that a tile's loads are issued
-// together). Rows shorter than a vector are read by their elements.
+// together). dh >= E.
 template <typename T>
 __device__ __forceinline__ FragOf<T> zero_frag() {
   FragOf<T> f;
@@ -77,21 +77,13 @@ template <typename T>
 __device__ __forceinline__ FragOf<T> load_raw(const T *row, bool ok, int d, int dh) {
   constexpr int E = Mma<T>::E;
   FragOf<T> f = zero_frag<T>();
-  if (ok && d < dh) {
-    if (dh >= E) {
-      __builtin_memcpy(&f, row + min(d, dh - E), sizeof(f));
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (e < dh) f[e] = row[e];
-    }
-  }
+  if (ok && d < dh) __builtin_memcpy(&f, row + min(d, dh - E), sizeof(f));
   return f;
 }
 template <typename T>
 __device__ __forceinline__ FragOf<T> fix(FragOf<T> f, int d, int dh) {
   constexpr int E = Mma<T>::E;
-  if (dh % E == 0 || dh < E) return f;   // uniform
+  if (dh % E == 0) return f;   // uniform
   const int by = (d + E - dh) * 8 * int(sizeof(T));   // bits past the row's end
   if (by <= 0 || d >= dh) return f;
   typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
@@ -197,22 +189,38 @@ __device__ __forceinline__ int64_t out_row(const Args &a, int64_t n, int hk, int
 // of a pair are two heads of the same 16 queries, so that a distance is
 // turned into its column once for both; t counts (query, head pair). Else t
 // counts the rows i G + h and the blocks follow each other.
+// Rows and queries are counted in 32 bits (divisions are long in 64).
 struct RowAt {
-  int64_t i;
+  uint32_t i;
   int h;
 };
 template <bool SHARE>
-__device__ __forceinline__ RowAt row_at(int64_t t, int block, int G) {
+__device__ __forceinline__ RowAt row_at(uint32_t t, int block, int G) {
   RowAt r;
   if constexpr (SHARE) {
-    const int half = G >> 1;
+    const uint32_t half = uint32_t(G) >> 1;
     r.i = half == 1 ? t : t / half;
     r.h = int(t - r.i * half) * 2 + block;
   } else {
-    r.i = G == 1 ? t : t / G;
-    r.h = int(t - r.i * G);
+    r.i = G == 1 ? t : t / uint32_t(G);
+    r.h = int(t - r.i * uint32_t(G));
   }
   return r;
+}
+// A workgroup's tile of a (sequence, key head).
+struct TileAt {
+  int64_t n;
+  int hk;
+  uint32_t tile;
+};
+__device__ __forceinline__ TileAt tile_at(uint32_t id, uint32_t tiles, int heads) {
+  TileAt t;
+  const uint32_t item = id / tiles;
+  t.tile = id - item * tiles;
+  const uint32_t n = item / uint32_t(heads);
+  t.n = n;
+  t.hk = int(item - n * uint32_t(heads));
+  return t;
 }
 
 // ------------------------------------------------------------------ the bias
@@ -231,10 +239,6 @@ __device__ __forceinline__ int bucket_of(uint32_t n, const Buckets &k) {
   const int sh = (31 - k.m) - __builtin_clz(n | (1u << k.m));
   return min(int(n >> sh) + (sh << k.m), k.last);
 }
-__device__ __forceinline__ int column(int d, const Buckets &k) {   // |d| < 2^31
-  if (k.add == 0) return bucket_of(uint32_t(max(d, 0)), k);        // uniform
-  return bucket_of(uint32_t(max(d, -d)), k) + ((d >> 31) & k.add);
-}
 __device__ __forceinline__ int column64(int64_t d, const Buckets &k) {
   const bool neg = d < 0;
   const uint64_t n64 = neg ? (k.add != 0 ? uint64_t(0) - uint64_t(d) : 0) : uint64_t(d);
@@ -248,41 +252,103 @@ struct PosTile {
   int rel[N];
   int64_t pos[N];
 };
-// The columns of 4 consecutive keys (or rows) of a tile against one position;
-// `sign` -1 where the tile holds the query positions.
-template <int N>
-__device__ __forceinline__ void columns4(int (&col)[4], const PosTile<N> &t, int at, int rel, int64_t pos, bool near_,
-                                         int sign, const Buckets &k) {
+// The columns of NB blocks of 16 keys (or rows) of a tile from `at` (4 of each
+// a lane) against one position; `sign` -1 where the tile holds the query
+// positions. One uniform branch for all of them, so that their steps overlap.
+template <int NB, int N>
+__device__ __forceinline__ void columns(int (&col)[NB][4], const PosTile<N> &t, int at, int rel, int64_t pos,
+                                        bool near_, int sign, const Buckets &k) {
   if (near_) {
-    int r[4];
-    __builtin_memcpy(r, t.rel + at, sizeof(r));
+    int d[NB][4];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) col[v] = column(sign > 0 ? rel - r[v] : r[v] - rel, k);
+    for (int b = 0; b < NB; ++b) {
+      int r[4];
+      __builtin_memcpy(r, t.rel + at + 16 * b, sizeof(r));
+#pragma unroll
+      for (int v = 0; v < 4; ++v) d[b][v] = sign > 0 ? rel - r[v] : r[v] - rel;
+    }
+    if (k.add == 0) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) col[b][v] = bucket_of(uint32_t(max(d[b][v], 0)), k);
+    } else {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          col[b][v] = bucket_of(uint32_t(max(d[b][v], -d[b][v])), k) + ((d[b][v] >> 31) & k.add);
+    }
   } else {
+#pragma unroll 1
+    for (int b = 0; b < NB; ++b) {
+      int c[4];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) col[v] = column64(sign > 0 ? pos - t.pos[at + v] : t.pos[at + v] - pos, k);
+      for (int v = 0; v < 4; ++v) {
+        const int64_t p = t.pos[at + 16 * b + v];
+        c[v] = column64(sign > 0 ? pos - p : p - pos, k);
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i)   // (static places)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) col[i][v] = i == b ? c[v] : col[i][v];
+    }
   }
 }
 
 // ------------------------------------------------------------------ small things
 __host__ __device__ constexpr size_t align_bytes(size_t n) { return (n + 15) & ~size_t(15); }   // a wave's LDS area
-// Sum or maximum over the four lane groups that hold one column.
+// Sum or maximum over the four lane groups that hold one column, by swapping
+// rows of 16 lanes and halves of the wave between two copies of the register.
 __device__ __forceinline__ float groups_sum(float v) {
-  v += __shfl_xor(v, 16, kWave);
-  return v + __shfl_xor(v, 32, kWave);
+  auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(h[0]) + __uint_as_float(h[1]);
+  auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 __device__ __forceinline__ float groups_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, kWave));
-  return fmaxf(v, __shfl_xor(v, 32, kWave));
+  auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+  auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 // LDS of one wave: its accesses are in order; nothing moves across this.
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
-// The bias table of a key head's G heads, times log2 e.
+// The bias table of a key head's G heads in LDS, times log2 e; an odd stride,
+// so that two heads' values of a column lie in different banks.
+__host__ __device__ __forceinline__ int table_ld(const Args &a) { return a.cols | 1; }
+__host__ __device__ __forceinline__ size_t table_bytes(const Args &a) {
+  return a.cols == 0 ? 0 : sizeof(float) * size_t(a.G) * size_t(table_ld(a));
+}
 __device__ __forceinline__ void stage_bias(float *table, const Args &a, int hk, int tid, int threads) {
-  for (int c = tid; c < a.G * a.cols; c += threads) table[c] = a.p.bias[int64_t(hk) * a.G * a.cols + c] * kLog2e;
+  for (int c = tid; c < a.G * a.cols; c += threads) {
+    const int h = c / a.cols;
+    table[h * table_ld(a) + c - h * a.cols] = a.p.bias[int64_t(hk) * a.G * a.cols + c] * kLog2e;
+  }
+}
+// x = x c + shift (+ the bias of each column) over blocks
+template <int NB>
+__device__ __forceinline__ void scale_scores(float (&x)[NB][4], float c, float shift, const float *row,
+                                             const int (&col)[NB][4], bool biased) {
+  if (biased) {
+    float t[NB][4];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) t[b][v] = row[col[b][v]];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) x[b][v] = fmaf(x[b][v], c, shift) + t[b][v];
+  } else {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) x[b][v] = fmaf(x[b][v], c, shift);
+  }
 }
 
 // A power of two near 1 / most (1 for 0 and what is not finite).
@@ -330,7 +396,162 @@ __device__ __forceinline__ void add_cells(Cell *cells, const int (&col)[N][4], c
     }
 }
 __device__ __forceinline__ bool cells_hold(float seen) { return seen < 4.f * kCellMax; }
+// ------------------------------------------------------------------ key tiles of a workgroup
+// Keys of a tile that KW waves share, 32 each (fp32 with four waves: 16).
+template <typename T>
+constexpr int tile_keys(int kw) {
+  return sizeof(T) == 2 ? 32 * kw : 64;
+}
+__device__ __forceinline__ constexpr uint32_t full_mask(int n) { return n >= 32 ? ~0u : (1u << n) - 1; }
+
+// Tiles in LDS: two where both leave room for a second workgroup (one barrier
+// a tile), else one.
+template <typename S>
+__host__ __device__ constexpr int buffers() {
+  return sizeof(S) <= 24 * 1024 ? 2 : 1;
+}
+
+// A tile of TK keys on its way from memory to LDS: every wave looks at the
+// tile's keys, one (or two) a lane, for liveness and positions; the rows go by
+// 16-byte units over the workgroup, dead ones as 0.
+template <typename T, int DP, int TK, int BLOCK>
+struct KeyTile {
+  using L = Tile<T, DP>;
+  static constexpr int W = TK / 64, PER = (TK * L::UPR + BLOCK - 1) / BLOCK, E = Mma<T>::E;
+  FragOf<T> kr[PER], vr[PER];
+  uint64_t live[W];
+  int64_t pos[W];
+  bool near_ = true;
+  __device__ __forceinline__ bool row_live(int r) const { return (live[W == 1 ? 0 : r >> 6] >> (r & 63)) & 1; }
+  __device__ __forceinline__ uint32_t live_of(int first, int n) const {   // first: a multiple of 16, uniform
+    return uint32_t(live[W == 1 ? 0 : first >> 6] >> (first & 63)) & full_mask(n);
+  }
+  __device__ __forceinline__ void load(const Seq<T> &q, const Args &a, int64_t j0, int64_t base, bool qnear) {
+    const int lane = threadIdx.x & 63;
+    const sgl_attention &p = a.p;
+    near_ = qnear;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int64_t j = j0 + 64 * i + lane;
+      const bool on = key_live(q, p, j);
+      live[i] = __ballot(on);
+      if (p.bias != nullptr) {
+        pos[i] = on ? q.kpos[j * p.kpos_t] : base;
+        near_ = near_ && __all(is_near(pos[i] - base));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = threadIdx.x + i * BLOCK, r = u / L::UPR, d = (u % L::UPR) * E;
+      const bool on = r < TK && row_live(min(r, TK - 1));
+      kr[i] = load_raw<T>(q.k + (j0 + r) * p.k_t, on, d, p.head_dim);
+      vr[i] = load_raw<T>(q.v + (j0 + r) * p.v_t, on, d, p.head_dim);
+    }
+  }
+  __device__ __forceinline__ void store(T *k, T *v, PosTile<TK> &t, const Args &a, int64_t base) const {
+    const int dh = a.p.head_dim;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = threadIdx.x + i * BLOCK, r = u / L::UPR, d = (u % L::UPR) * E;
+      if (TK * L::UPR % BLOCK == 0 || r < TK) {
+        *reinterpret_cast<FragOf<T> *>(k + r * L::LD + d) = fix<T>(kr[i], d, dh);
+        *reinterpret_cast<FragOf<T> *>(v + r * L::LD + d) = fix<T>(vr[i], d, dh);
+      }
+    }
+    if (a.p.bias != nullptr && threadIdx.x < 64) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        t.pos[64 * i + threadIdx.x] = pos[i];
+        t.rel[64 * i + threadIdx.x] = int(pos[i] - base);
+      }
+    }
+  }
+};
+
+// The KW waves of each row block (wave w: block w / KW) joined into the first
+// of them: the maximum, the sum and the products of NB accumulators a block.
+// The workgroup's LDS is free for it (every wave calls this).
+inline size_t join_bytes(int rw, int kw, int nq, int dp) {
+  return sizeof(float2) * 16 * size_t(rw * kw * nq) + sizeof(float) * 16 * size_t(rw * (kw - 1) * nq * dp);
+}
+// rows of products: wave w (its part above 0) and block b, [value][16]
+template <int KW, int NQ, int NB>
+__device__ __forceinline__ float *join_slot(float *pr, int w, int b) {
+  return pr + ((w / KW * (KW - 1) + w % KW - 1) * NQ + b) * (NB * 16 * 16);
+}
+template <int KW, int NQ, int NB>
+__device__ __forceinline__ void put_join(float *pr, const f32x4 (&acc)[NQ][NB]) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
+  if (w % KW == 0) return;
+#pragma unroll
+  for (int b = 0; b < NQ; ++b) {
+    float *t = join_slot<KW, NQ, NB>(pr, w, b);
+#pragma unroll
+    for (int d = 0; d < NB; ++d)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) t[(d * 16 + 4 * g + v) * 16 + cl] = acc[b][d][v];
+  }
+}
+template <int KW, int NQ, int NB>
+__device__ __forceinline__ void take_join(float *pr, f32x4 (&acc)[NQ][NB]) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
+  if (w % KW != 0) return;
+#pragma unroll
+  for (int k = 1; k < KW; ++k)
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+      const float *t = join_slot<KW, NQ, NB>(pr, w + k, b);
+#pragma unroll
+      for (int d = 0; d < NB; ++d)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) acc[b][d][v] += t[(d * 16 + 4 * g + v) * 16 + cl];
+    }
+}
+template <int RW, int KW, int NQ, int NB>
+__device__ __forceinline__ void join_waves(char *smem, float (&m)[NQ], float (&l)[NQ], f32x4 (&acc)[NQ][NB]) {
+  if constexpr (KW > 1) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15, w0 = w / KW * KW;
+    float2 *ml = reinterpret_cast<float2 *>(smem);
+    float *pr = reinterpret_cast<float *>(smem + sizeof(float2) * 16 * RW * KW * NQ);
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NQ; ++b)
+      if (g == 0) ml[(w * NQ + b) * 16 + cl] = make_float2(m[b], l[b]);
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < KW; ++i) top = fmaxf(top, ml[((w0 + i) * NQ + b) * 16 + cl].x);
+      const float at = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int i = 0; i < KW; ++i) {
+        const float2 e = ml[((w0 + i) * NQ + b) * 16 + cl];
+        sum += e.y * __builtin_amdgcn_exp2f(e.x - at);
+      }
+      const float f = __builtin_amdgcn_exp2f(m[b] - at);
+#pragma unroll
+      for (int d = 0; d < NB; ++d) acc[b][d] *= f;
+      m[b] = top;
+      l[b] = sum;
+    }
+    put_join<KW, NQ, NB>(pr, acc);
+    __syncthreads();
+    take_join<KW, NQ, NB>(pr, acc);
+  }
+}
+
 // ------------------------------------------------------------------ launches
+// Row tiles of a (sequence, key head), RW x NQ blocks each (SHARE: pairs).
+inline int64_t row_tiles(const Args &a, int nq, bool share, int rw) {
+  const int64_t count = share ? a.rows / 2 : a.rows, per = share ? 16 * rw : 16 * rw * nq;
+  return (count + per - 1) / per;
+}
+// Whether tiles of 128 rows fill the GPU: two blocks a wave then (each key
+// fragment read from LDS, and with an even G each column, serves two), eight
+// waves a workgroup; else 16 rows a workgroup, its four waves along the keys.
+inline bool many_rows(const Args &a) { return a.p.n * a.p.heads_kv * ((a.rows + 127) / 128) >= 192; }
+
 int run_forward(const Args &a, void *o, void *rest, float *lse, void *workspace, hipStream_t s);
 size_t forward_bytes(const Args &a);
 int run_backward(const Args &a, const void *o, const void *rest, const float *lse, const void *go, void *dq, void *dk,

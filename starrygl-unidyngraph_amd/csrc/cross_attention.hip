@@ -50,8 +50,9 @@ int check_attn(const sgl_attention *p) {
               "cross_attention: bad sizes");
   SGL_REQUIRE(p->heads_q > 0 && p->heads_kv > 0 && p->heads_q % p->heads_kv == 0,
               "cross_attention: %d query heads over %d key heads", p->heads_q, p->heads_kv);
-  SGL_REQUIRE(p->head_dim > 0 && p->head_dim <= sgl::attn::kMaxDim, "cross_attention: head size %d (1 to %d)",
-              p->head_dim, sgl::attn::kMaxDim);
+  const int least = p->dtype == SGL_FP32 ? 4 : 8;   // a row is read by 16-byte vectors
+  SGL_REQUIRE(p->head_dim >= least && p->head_dim <= sgl::attn::kMaxDim, "cross_attention: head size %d (%d to %d)",
+              p->head_dim, least, sgl::attn::kMaxDim);
   SGL_REQUIRE(p->heads_q / p->heads_kv <= 64, "cross_attention: more than 64 query heads to a key head");
   if (p->bias != nullptr) {
     SGL_REQUIRE(p->buckets > 0 && p->buckets * (p->two_sided ? 2 : 1) <= sgl::attn::kMaxCols,
@@ -63,7 +64,7 @@ int check_attn(const sgl_attention *p) {
   }
   SGL_REQUIRE(p->n == 0 || ((p->lq == 0 || p->q) && (p->lk == 0 || (p->k && p->v))), "cross_attention: NULL array");
   const int64_t rows = p->lq * (p->heads_q / p->heads_kv);
-  SGL_REQUIRE(p->n * p->heads_kv < INT_MAX && p->n * p->heads_kv * (std::max(rows, p->lk) / 64 + 1) < INT_MAX / 4,
+  SGL_REQUIRE(rows < INT_MAX && p->n * p->heads_kv < INT_MAX && p->n * p->heads_kv * (std::max(rows, p->lk) / 64 + 1) < INT_MAX / 4,
               "cross_attention: too many rows for one call");
   return SGL_OK;
 }

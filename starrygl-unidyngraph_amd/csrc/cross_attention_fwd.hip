@@ -6,66 +6,72 @@ namespace attn {
 namespace {
 
 // ------------------------------------------------------------------ many rows
-// A workgroup takes 4 x NQ blocks of 16 rows of a (sequence, key head), NQ a
-// wave, and walks the keys 64 at a time with the running maximum and sum of
-// the softmax (base 2). The next tile's keys and values are in flight while
-// the current one is worked on. The products are computed as (keys x rows) and
-// (head size x rows): a lane keeps one row a block, so its maximum, sum and
-// rescale are its own, joined over four lanes only. The accumulators are
-// rescaled only when the maximum has grown by more than 2^6: p stays below
-// 2^6, and the sum and the products carry the same factor.
+// A workgroup takes RW x NQ blocks of 16 rows of a (sequence, key head) and
+// walks its keys a tile at a time with the running maximum and sum of the
+// softmax (base 2); KW waves share each row block, each with its part of every
+// tile, and are joined at the end: two to four waves a SIMD, whose chains of
+// dependent steps (position, column, table, exp) fill each other's gaps, from
+// grids of one or two workgroups a CU. The next tile's keys and values are in
+// flight while the current one is worked on. The products are computed as
+// (keys x rows) and (head size x rows): a lane keeps one row a block, so its
+// maximum, sum and rescale are its own, joined over four lanes only. The
+// accumulators are rescaled only when the maximum has grown by more than 2^6:
+// p stays below 2^6, and the sum and the products carry the same factor.
 constexpr float kSlack = 6.f;
 
-template <typename T, int DP>
+template <typename T, int DP, int TK>
 struct FwdLds {
-  T k[kKeys * Tile<T, DP>::LD], v[kKeys * Tile<T, DP>::LD];
-  PosTile<kKeys> pos;
+  T k[TK * Tile<T, DP>::LD], v[TK * Tile<T, DP>::LD];
+  PosTile<TK> pos;
 };
 
-template <typename T, int DP, int NQ, bool SHARE>
-__global__ __launch_bounds__(kBlock) void k_attn_fwd(Args a, int64_t tiles, T *__restrict__ o, T *__restrict__ rest,
-                                                     float *__restrict__ lse) {
+template <typename T, int DP, int NQ, bool SHARE, int RW, int KW>
+__global__ __launch_bounds__(RW * KW * 64) void k_attn_fwd(Args a, int64_t tiles, T *__restrict__ o,
+                                                           T *__restrict__ rest, float *__restrict__ lse) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
-  constexpr int ST = DP / M::KS, DB = DP / 16, KB = kKeys / 16;
+  constexpr int TK = tile_keys<T>(KW), BLOCK = RW * KW * 64;
+  constexpr int ST = DP / M::KS, DB = DP / 16, KB = TK / 16 / KW;
   constexpr int NP = SHARE ? 1 : NQ;   // positions a lane holds
   extern __shared__ __align__(16) char smem[];
-  FwdLds<T, DP> &s = *reinterpret_cast<FwdLds<T, DP> *>(smem);
-  float *table = reinterpret_cast<float *>(smem + sizeof(s));
+  using S = FwdLds<T, DP, TK>;
+  constexpr int NB = buffers<S>();
+  S *const bufs = reinterpret_cast<S *>(smem);
+  float *table = reinterpret_cast<float *>(smem + NB * sizeof(S));
   const sgl_attention &p = a.p;
   const int dh = p.head_dim;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
-  int64_t id = blockIdx.x;
-  const int64_t rt = id % tiles;
-  id /= tiles;
-  const int hk = int(id % p.heads_kv);
-  const int64_t n = id / p.heads_kv;
+  const int wr = w / KW, k0 = (w % KW) * KB * 16;   // this wave's row blocks, and its first key of a tile
+  const TileAt at_ = tile_at(blockIdx.x, uint32_t(tiles), p.heads_kv);
+  const uint32_t rt = at_.tile;
+  const int hk = at_.hk;
+  const int64_t n = at_.n;
   const Seq<T> q = seq_of<T>(p, n, hk, a.G);
   const bool biased = p.bias != nullptr;
   const Buckets bk = buckets_of(p);
   // the workgroup's first query; nothing to do past the length
-  const int64_t t0 = rt * (SHARE ? 64 : 64 * NQ);
-  const int64_t i0 = row_at<SHARE>(t0, 0, a.G).i;
+  const uint32_t t0 = rt * (SHARE ? RW * 16 : RW * 16 * NQ);
+  const uint32_t i0 = row_at<SHARE>(t0, 0, a.G).i;
   const bool any = i0 < q.qlen;
-  if (biased) stage_bias(table, a, hk, threadIdx.x, kBlock);
+  if (biased) stage_bias(table, a, hk, threadIdx.x, BLOCK);
   RowAt row[NQ];
   bool in[NQ], ok[NQ];
   FragOf<T> qf[NQ][ST];
   int64_t qpos[NP];
   int qrel[NP];
-  const int64_t base = biased && any ? q.qpos[i0 * p.qpos_t] : 0;
+  const int64_t base = biased && any ? q.qpos[int64_t(i0) * p.qpos_t] : 0;
   bool qnear = true;
 #pragma unroll
   for (int b = 0; b < NQ; ++b) {
-    const int64_t t = SHARE ? t0 + w * 16 + cl : t0 + (w * NQ + b) * 16 + cl;
+    const uint32_t t = SHARE ? t0 + wr * 16 + cl : t0 + (wr * NQ + b) * 16 + cl;
     row[b] = row_at<SHARE>(t, b, a.G);
     in[b] = row[b].i < p.lq;
     ok[b] = row[b].i < q.qlen;
 #pragma unroll
     for (int st = 0; st < ST; ++st)
-      qf[b][st] = load_row<T>(q.q + row[b].i * p.q_t + row[b].h * p.q_h, ok[b], st * M::KS + g * M::E, dh);
+      qf[b][st] = load_row<T>(q.q + int64_t(row[b].i) * p.q_t + row[b].h * p.q_h, ok[b], st * M::KS + g * M::E, dh);
     if (b < NP) {
-      qpos[b] = biased && ok[b] ? q.qpos[row[b].i * p.qpos_t] : base;
+      qpos[b] = biased && ok[b] ? q.qpos[int64_t(row[b].i) * p.qpos_t] : base;
       qnear = qnear && is_near(qpos[b] - base);
       qrel[b] = int(qpos[b] - base);
     }
@@ -81,69 +87,44 @@ __global__ __launch_bounds__(kBlock) void k_attn_fwd(Args a, int64_t tiles, T *_
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // a tile in flight: one key a lane for liveness and position, the rows by units
-  constexpr int PER = kKeys * L::UPR / kBlock;
-  FragOf<T> kr[PER], vr[PER];
-  uint64_t live = 0;
-  bool near_ = true;
-  int64_t kp = 0;
-  auto load_tile = [&](int64_t j0) {
-    const bool on = key_live(q, p, j0 + lane);
-    live = __ballot(on);
-    if (biased) {
-      kp = on ? q.kpos[(j0 + lane) * p.kpos_t] : base;
-      near_ = qnear && __all(is_near(kp - base));
-    }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int u = threadIdx.x + i * kBlock, r = u / L::UPR, d = (u % L::UPR) * M::E;
-      const bool on_r = (live >> r) & 1;
-      kr[i] = load_raw<T>(q.k + (j0 + r) * p.k_t, on_r, d, dh);
-      vr[i] = load_raw<T>(q.v + (j0 + r) * p.v_t, on_r, d, dh);
-    }
-  };
-  if (any && q.klen > 0) load_tile(0);
-  for (int64_t j0 = 0; any && j0 < q.klen; j0 += kKeys) {
+  KeyTile<T, DP, TK, BLOCK> tile;
+  if (any && q.klen > 0) tile.load(q, a, 0, base, qnear);
+  int buf = 0;
+  for (int64_t j0 = 0; any && j0 < q.klen; j0 += TK) {
+    S &s = bufs[buf];
+    if constexpr (NB == 1) __syncthreads();
+    else buf ^= 1;
+    tile.store(s.k, s.v, s.pos, a, base);
+    const uint32_t on = tile.live_of(k0, KB * 16);   // this wave's keys
+    const bool near_now = tile.near_;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int u = threadIdx.x + i * kBlock, r = u / L::UPR, d = (u % L::UPR) * M::E;
-      *reinterpret_cast<FragOf<T> *>(s.k + r * L::LD + d) = fix<T>(kr[i], d, dh);
-      *reinterpret_cast<FragOf<T> *>(s.v + r * L::LD + d) = fix<T>(vr[i], d, dh);
-    }
-    if (biased && w == 0) {
-      s.pos.pos[lane] = kp;
-      s.pos.rel[lane] = int(kp - base);
-    }
-    const uint64_t on = live;
-    const bool near_now = near_;
-    __syncthreads();
-    if (j0 + kKeys < q.klen) load_tile(j0 + kKeys);
+    if (j0 + TK < q.klen) tile.load(q, a, j0 + TK, base, qnear);
     float x[NQ][KB][4], mx[NQ];
+    int col[NP][KB][4];
+    if (biased) {
 #pragma unroll
-    for (int b = 0; b < NQ; ++b) mx[b] = -INFINITY;
+      for (int b = 0; b < NP; ++b) columns(col[b], s.pos, k0 + 4 * g, qrel[b], qpos[b], near_now, 1, bk);
+    }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       FragOf<T> kf[ST];
 #pragma unroll
-      for (int st = 0; st < ST; ++st) kf[st] = L::frag(s.k, kb * 16, st * M::KS);
-      int col[4];
+      for (int st = 0; st < ST; ++st) kf[st] = L::frag(s.k, k0 + kb * 16, st * M::KS);
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {
         f32x4 sc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int st = 0; st < ST; ++st) sc = M::mma(kf[st], qf[b][st], sc);
-        if (biased) {
-          if (b < NP) columns4(col, s.pos, kb * 16 + 4 * g, qrel[b < NP ? b : 0], qpos[b < NP ? b : 0], near_now, 1, bk);
 #pragma unroll
-          for (int v = 0; v < 4; ++v) x[b][kb][v] = sc[v] * c + table[row[b].h * a.cols + col[v]];
-        } else {
-#pragma unroll
-          for (int v = 0; v < 4; ++v) x[b][kb][v] = sc[v] * c;
-        }
+        for (int v = 0; v < 4; ++v) x[b][kb][v] = sc[v];
       }
     }
-    if (on != ~0ull) {   // uniform
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+      mx[b] = -INFINITY;
+      scale_scores(x[b], c, 0.f, table + row[b].h * table_ld(a), col[b < NP ? b : 0], biased);
+    }
+    if (on != full_mask(KB * 16)) {   // uniform
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -159,9 +140,8 @@ __global__ __launch_bounds__(kBlock) void k_attn_fwd(Args a, int64_t tiles, T *_
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int v = 0; v < 4; ++v) mx[b] = fmaxf(mx[b], x[b][kb][v]);
-      mx[b] = groups_max(mx[b]);
       if (__any(mx[b] > m[b] + kSlack)) {   // (uniform over the wave; also the first live tile)
-        const float mn = fmaxf(m[b], mx[b]);
+        const float mn = fmaxf(m[b], groups_max(mx[b]));
         const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[b] - mn);
         l[b] *= alpha;
         m[b] = mn;
@@ -178,23 +158,26 @@ __global__ __launch_bounds__(kBlock) void k_attn_fwd(Args a, int64_t tiles, T *_
         }
     }
 #pragma unroll
-    for (int st = 0; st < kKeys / M::KS; ++st) {
+    for (int st = 0; st < KB * 16 / M::KS; ++st) {
       FragOf<T> pf[NQ];
 #pragma unroll
       for (int b = 0; b < NQ; ++b) pf[b] = frag_of<T>(x[b], st);
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        const FragOf<T> vf = L::template frag_t<kKeys>(s.v, d * 16, st * M::KS);
+        const FragOf<T> vf = L::template frag_t<TK>(s.v, d * 16, k0 + st * M::KS);
 #pragma unroll
         for (int b = 0; b < NQ; ++b) acc[b][d] = M::mma(vf, pf[b], acc[b][d]);
       }
     }
   }
 #pragma unroll
+  for (int b = 0; b < NQ; ++b) l[b] = groups_sum(l[b]);
+  join_waves<RW, KW, NQ, DB>(smem, m, l, acc);
+  if (w % KW != 0) return;
+#pragma unroll
   for (int b = 0; b < NQ; ++b) {
-    const float sum = groups_sum(l[b]);
     if (!in[b]) continue;
-    const float inv = ok[b] && sum > 0.f ? 1.f / sum : 0.f;
+    const float inv = ok[b] && l[b] > 0.f ? 1.f / l[b] : 0.f;
     const int64_t at = out_row(a, n, hk, row[b].i, row[b].h);
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
@@ -209,8 +192,8 @@ __global__ __launch_bounds__(kBlock) void k_attn_fwd(Args a, int64_t tiles, T *_
     }
     // log2 of the sum of 2^x; +inf where no key is live, so that p is 0 there
     if (lse != nullptr && g == 0)
-      lse[(n * p.heads_kv + hk) * a.rows + row[b].i * a.G + row[b].h] =
-          ok[b] && sum > 0.f ? m[b] + __log2f(sum) : INFINITY;
+      lse[(n * p.heads_kv + hk) * a.rows + int64_t(row[b].i) * a.G + row[b].h] =
+          ok[b] && l[b] > 0.f ? m[b] + __log2f(l[b]) : INFINITY;
   }
 }
 
@@ -242,16 +225,14 @@ __global__ __launch_bounds__(kBlock) void k_attn_few(Args a, int parts, int64_t 
   const int dh = p.head_dim;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
   using Lds = FewLds<T, DP, NQ>;
-  const size_t per = align_bytes(sizeof(Lds) + sizeof(float) * size_t(a.G) * a.cols);
+  const size_t per = align_bytes(sizeof(Lds) + table_bytes(a));
   Lds &s = *reinterpret_cast<Lds *>(smem + w * per);
   float *table = reinterpret_cast<float *>(smem + w * per + sizeof(Lds));
-  const int64_t items = p.n * p.heads_kv;
-  int64_t item = parts == 0 ? int64_t(blockIdx.x) * kWaves + w : blockIdx.x / parts;
-  const int part = parts == 0 ? 0 : int(blockIdx.x - item * parts);
-  const bool work = item < items;
-  if (parts == 0 && !work) return;   // (whole waves; no barrier follows in this form)
-  const int hk = int(item % p.heads_kv);
-  const int64_t n = item / p.heads_kv;
+  const TileAt at_ = parts == 0 ? tile_at(blockIdx.x * kWaves + w, 1, p.heads_kv)
+                                : tile_at(blockIdx.x, uint32_t(parts), p.heads_kv);
+  const int hk = at_.hk, part = int(at_.tile);
+  const int64_t n = at_.n, item = n * p.heads_kv + hk;
+  if (n >= p.n) return;   // (whole waves of the form without barriers)
   const Seq<T> q = seq_of<T>(p, n, hk, a.G);
   const bool biased = p.bias != nullptr;
   const Buckets bk = buckets_of(p);
@@ -268,13 +249,13 @@ __global__ __launch_bounds__(kBlock) void k_attn_few(Args a, int parts, int64_t 
   bool qnear = true;
 #pragma unroll
   for (int b = 0; b < NQ; ++b) {
-    row[b] = row_at<false>(b * 16 + cl, b, a.G);
+    row[b] = row_at<false>(uint32_t(b * 16 + cl), b, a.G);
     in[b] = row[b].i < p.lq;
     ok[b] = row[b].i < q.qlen;
 #pragma unroll
     for (int st = 0; st < ST; ++st)
-      qf[b][st] = load_row<T>(q.q + row[b].i * p.q_t + row[b].h * p.q_h, ok[b], st * M::KS + g * M::E, dh);
-    qpos[b] = biased && ok[b] ? q.qpos[row[b].i * p.qpos_t] : base;
+      qf[b][st] = load_row<T>(q.q + int64_t(row[b].i) * p.q_t + row[b].h * p.q_h, ok[b], st * M::KS + g * M::E, dh);
+    qpos[b] = biased && ok[b] ? q.qpos[int64_t(row[b].i) * p.qpos_t] : base;
     qnear = qnear && is_near(qpos[b] - base);
     qrel[b] = int(qpos[b] - base);
   }
@@ -341,24 +322,26 @@ __global__ __launch_bounds__(kBlock) void k_attn_few(Args a, int parts, int64_t 
 #pragma unroll
     for (int b = 0; b < NQ; ++b) {
       float mx = -INFINITY;
+      int col[KB][4];
+      if (biased) columns(col, s.pos, 4 * g, qrel[b], qpos[b], near_now, 1, bk);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         f32x4 sc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int st = 0; st < ST; ++st) sc = M::mma(kf[kb][st], qf[b][st], sc);
-        int col[4];
-        if (biased) columns4(col, s.pos, kb * 16 + 4 * g, qrel[b], qpos[b], near_now, 1, bk);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) x[b][kb][v] = sc[v];
+      }
+      scale_scores(x[b], c, 0.f, table + row[b].h * table_ld(a), col, biased);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          float t = sc[v] * c;
-          if (biased) t += table[row[b].h * a.cols + col[v]];
-          x[b][kb][v] = (on >> (kb * 16 + 4 * g + v)) & 1 ? t : -INFINITY;
+          x[b][kb][v] = (on >> (kb * 16 + 4 * g + v)) & 1 ? x[b][kb][v] : -INFINITY;
           mx = fmaxf(mx, x[b][kb][v]);
         }
-      }
-      mx = groups_max(mx);
       if (__any(mx > m[b] + kSlack)) {
-        const float mn = fmaxf(m[b], mx);
+        const float mn = fmaxf(m[b], groups_max(mx));
         const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[b] - mn);
         l[b] *= alpha;
         m[b] = mn;
@@ -390,53 +373,14 @@ __global__ __launch_bounds__(kBlock) void k_attn_few(Args a, int parts, int64_t 
 #pragma unroll
   for (int b = 0; b < NQ; ++b) l[b] = groups_sum(l[b]);
   if (parts != 0) {
-    // the four waves' parts into wave 0's terms: [wave][block][d][row] products, [wave][block][row] (m, l)
-    float2 *ml = reinterpret_cast<float2 *>(smem);
-    float *pr = reinterpret_cast<float *>(smem + sizeof(float2) * kWaves * NQ * 16);
-    __syncthreads();
-#pragma unroll
-    for (int b = 0; b < NQ; ++b)
-      if (g == 0) ml[(w * NQ + b) * 16 + cl] = make_float2(m[b], l[b]);
-    __syncthreads();
-#pragma unroll
-    for (int b = 0; b < NQ; ++b) {
-      float top = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < kWaves; ++i) top = fmaxf(top, ml[(i * NQ + b) * 16 + cl].x);
-      const float at = top == -INFINITY ? 0.f : top;
-#pragma unroll
-      for (int i = 0; i < kWaves; ++i) {
-        const float2 e = ml[(i * NQ + b) * 16 + cl];
-        sum += e.y * __builtin_amdgcn_exp2f(e.x - at);
-      }
-      const float f = __builtin_amdgcn_exp2f(m[b] - at);
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-          pr[((w * NQ + b) * DP + d * 16 + 4 * g + v) * 16 + cl] = acc[b][d][v] * f;
-      m[b] = top;
-      l[b] = sum;
-    }
-    __syncthreads();
+    join_waves<1, kWaves, NQ, DB>(smem, m, l, acc);
     if (w != 0) return;
-#pragma unroll
-    for (int b = 0; b < NQ; ++b)
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          float t = 0.f;
-#pragma unroll
-          for (int i = 0; i < kWaves; ++i) t += pr[((i * NQ + b) * DP + d * 16 + 4 * g + v) * 16 + cl];
-          acc[b][d][v] = t;
-        }
   }
 #pragma unroll
   for (int b = 0; b < NQ; ++b) {
     if (!in[b]) continue;
     if (parts > 1) {
-      const int64_t r = (item * parts + part) * a.rows + row[b].i * a.G + row[b].h;
+      const int64_t r = (item * parts + part) * a.rows + int64_t(row[b].i) * a.G + row[b].h;
 #pragma unroll
       for (int d = 0; d < DB; ++d) store4(pacc + r * dh, d * 16 + 4 * g, dh, acc[b][d]);
       if (g == 0) pml[r] = make_float2(m[b], l[b]);
@@ -456,7 +400,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_few(Args a, int parts, int64_t 
       }
     }
     if (lse != nullptr && g == 0)
-      lse[item * a.rows + row[b].i * a.G + row[b].h] = ok[b] && l[b] > 0.f ? m[b] + __log2f(l[b]) : INFINITY;
+      lse[item * a.rows + int64_t(row[b].i) * a.G + row[b].h] = ok[b] && l[b] > 0.f ? m[b] + __log2f(l[b]) : INFINITY;
   }
 }
 
@@ -524,10 +468,10 @@ template <typename T, int DP, int NQ>
 int launch_few(const Args &a, T *o, T *rest, float *lse, void *ws, hipStream_t s) {
   const int parts = few_parts(a);
   const int64_t items = a.p.n * a.p.heads_kv, keys = parts > 0 ? few_keys(a, parts) : 0;
-  const size_t per = align_bytes(sizeof(FewLds<T, DP, NQ>) + sizeof(float) * size_t(a.G) * a.cols);
+  const size_t per = align_bytes(sizeof(FewLds<T, DP, NQ>) + table_bytes(a));
   size_t lds = per * kWaves;
   if (parts > 0)
-    lds = std::max(lds, sizeof(float2) * kWaves * NQ * 16 + sizeof(float) * kWaves * NQ * 16 * size_t(DP));
+    lds = std::max(lds, join_bytes(1, kWaves, NQ, DP));
   float2 *ml = static_cast<float2 *>(ws);
   float *acc = reinterpret_cast<float *>(static_cast<char *>(ws) + (parts > 1 ? ml_bytes(a, parts) : 0));
   SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_few<T, DP, NQ>), lds));
@@ -540,13 +484,14 @@ int launch_few(const Args &a, T *o, T *rest, float *lse, void *ws, hipStream_t s
   return SGL_OK;
 }
 
-template <typename T, int DP, int NQ, bool SHARE>
+template <typename T, int DP, int NQ, bool SHARE, int RW, int KW>
 int launch_fwd(const Args &a, T *o, T *rest, float *lse, hipStream_t s) {
-  const int64_t count = SHARE ? a.rows / 2 : a.rows, per = SHARE ? 64 : 64 * NQ, tiles = (count + per - 1) / per;
-  const size_t lds = sizeof(FwdLds<T, DP>) + sizeof(float) * size_t(a.G) * a.cols;
-  SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_fwd<T, DP, NQ, SHARE>), lds));
-  launch(&k_attn_fwd<T, DP, NQ, SHARE>, dim3(unsigned(a.p.n * a.p.heads_kv * tiles)), dim3(kBlock), lds, s, a, tiles,
-         o, rest, lse);
+  const int64_t tiles = row_tiles(a, NQ, SHARE, RW);
+  const size_t lds = std::max(buffers<FwdLds<T, DP, tile_keys<T>(KW)>>() * sizeof(FwdLds<T, DP, tile_keys<T>(KW)>) + table_bytes(a),
+                              join_bytes(RW, KW, NQ, DP));
+  SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_fwd<T, DP, NQ, SHARE, RW, KW>), lds));
+  launch(&k_attn_fwd<T, DP, NQ, SHARE, RW, KW>, dim3(unsigned(a.p.n * a.p.heads_kv * tiles)), dim3(RW * KW * kWave),
+         lds, s, a, tiles, o, rest, lse);
   SGL_CHECK_LAUNCH();
   return SGL_OK;
 }
@@ -568,12 +513,9 @@ int run_forward(const Args &a, void *o, void *rest, float *lse, void *ws, hipStr
     T *to = static_cast<T *>(o), *tr = static_cast<T *>(rest);
     if (a.rows <= 16) return launch_few<T, DP, 1>(a, to, tr, lse, ws, s);
     if (a.rows <= kFewRows) return launch_few<T, DP, 2>(a, to, tr, lse, ws, s);
-    // two blocks a wave where that still fills the GPU: each key fragment read
-    // from LDS, and with an even G each column, then serves two
-    const int64_t groups = a.p.n * a.p.heads_kv * ((a.rows + 127) / 128);
-    if (groups < 256) return launch_fwd<T, DP, 1, false>(a, to, tr, lse, s);
-    if (a.G % 2 == 0) return launch_fwd<T, DP, 2, true>(a, to, tr, lse, s);
-    return launch_fwd<T, DP, 2, false>(a, to, tr, lse, s);
+    if (!many_rows(a)) return launch_fwd<T, DP, 1, false, 1, 4>(a, to, tr, lse, s);
+    if (a.G % 2 == 0) return launch_fwd<T, DP, 2, true, 4, 2>(a, to, tr, lse, s);
+    return launch_fwd<T, DP, 2, false, 4, 2>(a, to, tr, lse, s);
   });
 }
 

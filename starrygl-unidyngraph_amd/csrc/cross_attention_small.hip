@@ -26,7 +26,7 @@ struct SmallLds {
 
 template <typename Lds>
 __host__ __device__ __forceinline__ size_t small_lds(const Args &a, int nq, bool cells) {   // bytes a wave
-  return align_bytes(sizeof(Lds) + sizeof(float) * size_t(a.G) * a.cols) +
+  return align_bytes(sizeof(Lds) + table_bytes(a)) +
          (cells ? sizeof(Cell) * size_t(16 % a.G == 0 ? 1 : nq) * 16 * a.cols : 0);
 }
 
@@ -46,11 +46,11 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
   const size_t per = small_lds<Lds>(a, NQ, part != nullptr);
   Lds &s = *reinterpret_cast<Lds *>(smem + w * per);
   float *table = reinterpret_cast<float *>(smem + w * per + sizeof(Lds));
-  Cell *cells = reinterpret_cast<Cell *>(smem + w * per + align_bytes(sizeof(Lds) + sizeof(float) * a.G * a.cols));
+  Cell *cells = reinterpret_cast<Cell *>(smem + w * per + align_bytes(sizeof(Lds) + table_bytes(a)));
   const int sets = 16 % a.G == 0 ? 1 : NQ;   // (one: row c of either block has the same head)
-  const int64_t gw = int64_t(blockIdx.x) * (blockDim.x / kWave) + w;
-  const int hk = int(gw % p.heads_kv);
-  const int64_t first = gw / p.heads_kv;
+  const TileAt at_ = tile_at(blockIdx.x * (blockDim.x / kWave) + w, 1, p.heads_kv);
+  const int hk = at_.hk;
+  const int64_t first = at_.n;
   if (first >= each) return;   // (whole waves; there are no barriers)
   const bool biased = p.bias != nullptr;
   const Buckets bk = buckets_of(p);
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
   wave_sync();
   RowAt row[NQ];
 #pragma unroll
-  for (int b = 0; b < NQ; ++b) row[b] = row_at<false>(b * 16 + cl, b, a.G);
+  for (int b = 0; b < NQ; ++b) row[b] = row_at<false>(uint32_t(b * 16 + cl), b, a.G);
   const float c = p.scale * kLog2e;
   for (int64_t n = first; n < p.n; n += each) {
     const Seq<T> q = seq_of<T>(p, n, hk, a.G);
@@ -81,10 +81,10 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
 #pragma unroll
       for (int st = 0; st < ST; ++st) {
         const int d = st * M::KS + g * M::E;
-        qf[b][st] = load_raw<T>(q.q + row[b].i * p.q_t + row[b].h * p.q_h, ok[b], d, dh);
+        qf[b][st] = load_raw<T>(q.q + int64_t(row[b].i) * p.q_t + row[b].h * p.q_h, ok[b], d, dh);
         gf[b][st] = load_raw<T>(go + at, ok[b], d, dh);
       }
-      qpos[b] = biased && ok[b] ? q.qpos[row[b].i * p.qpos_t] : base;
+      qpos[b] = biased && ok[b] ? q.qpos[int64_t(row[b].i) * p.qpos_t] : base;
       near_ = near_ && is_near(qpos[b] - base);
       qrel[b] = int(qpos[b] - base);
     }
@@ -127,6 +127,10 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
     // scores and dp, (keys x rows)
     float x[NQ][NK][4], y[NQ][NK][4];
     int col[NQ][NK][4];
+    if (biased) {
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) columns(col[b], s.pos, 4 * g, qrel[b], qpos[b], near_, 1, bk);
+    }
 #pragma unroll
     for (int kb = 0; kb < NK; ++kb) {
       FragOf<T> kf[ST], vf[ST];
@@ -153,12 +157,9 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
           sc = M::mma(kf[st], qf[b][st], sc);
           dp = M::mma(vf[st], gf[b][st], dp);
         }
-        if (biased) columns4(col[b][kb], s.pos, kb * 16 + 4 * g, qrel[b], qpos[b], near_, 1, bk);
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          float t = sc[v] * c;
-          if (biased) t += table[row[b].h * a.cols + col[b][kb][v]];
-          x[b][kb][v] = (live >> (kb * 16 + 4 * g + v)) & 1 ? t : -INFINITY;
+          x[b][kb][v] = sc[v];
           y[b][kb][v] = dp[v];
         }
       }
@@ -167,10 +168,14 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
 #pragma unroll
     for (int b = 0; b < NQ; ++b) {
       float mx = -INFINITY, sum = 0.f, de = 0.f;
+      scale_scores(x[b], c, 0.f, table + row[b].h * table_ld(a), col[b], biased);
 #pragma unroll
       for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) mx = fmaxf(mx, x[b][kb][v]);
+        for (int v = 0; v < 4; ++v) {
+          x[b][kb][v] = (live >> (kb * 16 + 4 * g + v)) & 1 ? x[b][kb][v] : -INFINITY;
+          mx = fmaxf(mx, x[b][kb][v]);
+        }
       mx = groups_max(mx);
       const float at = mx == -INFINITY ? 0.f : mx;
 #pragma unroll

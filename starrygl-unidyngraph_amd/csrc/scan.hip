@@ -88,21 +88,26 @@ __device__ __forceinline__ Unit unit_of(const ScanArgs &a) {
   Unit u;
   if (a.supers == 0) {   // whole sequences: (n, d) side by side
     const int64_t i = int64_t(blockIdx.x) * kBlock + threadIdx.x;
-    u.n = i / dv;
-    u.d = int(i - u.n * dv) * V;
+    if (blockIdx.x < (1u << 24)) {   // (a 64-bit division is a long sequence of instructions)
+      const uint32_t n = uint32_t(i) / uint32_t(dv);
+      u.n = n;
+      u.d = int(uint32_t(i) - n * uint32_t(dv)) * V;
+    } else {
+      u.n = i / dv;
+      u.d = int(i - u.n * dv) * V;
+    }
     u.super = u.sub = 0;
     u.t0 = 0;
     u.t1 = a.L;
     u.ok = u.n < a.N;
   } else {   // a workgroup: kLanes channel groups x kSubs pieces
     const int blocks = (dv + kLanes - 1) / kLanes;
-    int64_t i = blockIdx.x;
-    const int cb = int(i % blocks);
-    i /= blocks;
-    u.super = int(i % a.supers);
-    u.n = i / a.supers;
+    const uint32_t i = blockIdx.x / uint32_t(blocks), cb = blockIdx.x - i * uint32_t(blocks);
+    const uint32_t n = i / uint32_t(a.supers);
+    u.super = int(i - n * uint32_t(a.supers));
+    u.n = n;
     u.sub = threadIdx.x / kLanes;
-    u.d = (cb * kLanes + threadIdx.x % kLanes) * V;
+    u.d = int(cb * kLanes + threadIdx.x % kLanes) * V;
     u.t0 = min((int64_t(u.super) * kSubs + u.sub) * a.piece, a.L);
     u.t1 = min(u.t0 + a.piece, a.L);
     u.ok = u.d < a.D;

@@ -208,8 +208,12 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens
     scale = dh ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"scale: {scale}")
-    return _Attend.apply(q, k, v, bias, (q_lens, k_lens, key_mask, q_pos if bias is not None else None,
+    least = 16 // q.element_size()
+    if dh < least:   # the kernels read 16 bytes of a head at a time: zeros add nothing to the products
+        q, k, v = (torch.nn.functional.pad(t, (0, least - dh)) for t in (q, k, v))
+    o = _Attend.apply(q, k, v, bias, (q_lens, k_lens, key_mask, q_pos if bias is not None else None,
                                          k_pos if bias is not None else None), int(resolution), bool(two_sided), scale)
+    return o if dh >= least else o[..., :dh]
 
 
 def distance_bucket(distance: torch.Tensor, buckets: int, resolution: int = 0) -> torch.Tensor:
