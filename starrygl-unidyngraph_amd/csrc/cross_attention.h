@@ -61,6 +61,23 @@ __device__ __forceinline__ FragOf<T> frag_of(const float (&x)[NB][4], int s) {
   return f;
 }
 
+// The same in three parts, each the rounding of what those before it left.
+template <typename T, int NB>
+__device__ __forceinline__ void split_frag_of(const float (&x)[NB][4], int s, FragOf<T> (&f)[3]) {
+  constexpr int B = Mma<T>::KS / 16;
+#pragma unroll
+  for (int b = 0; b < B; ++b)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      float e = s * B + b < NB ? x[s * B + b][v] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        f[i][4 * b + v] = T(e);
+        e -= float(T(e));
+      }
+    }
+}
+
 // ------------------------------------------------------------------ rows in memory
 // Elements [d, d + E) of a row of dh, 0 past it, from one 16-byte load at any
 // alignment: the last, partial vector is loaded from dh - E and moved down
@@ -110,6 +127,43 @@ __device__ __forceinline__ void store4(T *row, int d, int dh, f32x4 x) {
   }
 }
 
+// What rounding x to o left, kept in 16 bits beside o, and x of the two. bf16:
+// the low half of x's bits as a signed number (a tie that was rounded down is
+// one unit of 2^-24 off), so that o and rest are x; fp16: the difference, 2^11
+// as large so that it stays normal where o does (22 bits of x).
+template <typename T>
+__device__ __forceinline__ T rest_of(float x, T o) {
+  if constexpr (std::is_same_v<T, bf16_t>) {
+    const int low = int(__float_as_uint(x) - (uint32_t(__builtin_bit_cast(uint16_t, o)) << 16));
+    return __builtin_bit_cast(T, int16_t(min(low, 32767)));
+  } else {
+    return T((x - float(o)) * 2048.f);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float whole_of(T o, T rest) {
+  if constexpr (std::is_same_v<T, bf16_t>)
+    return __uint_as_float((uint32_t(__builtin_bit_cast(uint16_t, o)) << 16) + int(__builtin_bit_cast(int16_t, rest)));
+  else
+    return float(o) + float(rest) * (1.f / 2048.f);
+}
+
+// store4 of what it rounds away.
+template <typename T>
+__device__ __forceinline__ void store_rest(T *row, int d, int dh, f32x4 x) {
+  T t[4];
+#pragma unroll
+  for (int v = 0; v < 4; ++v) t[v] = rest_of<T>(x[v], T(x[v]));
+  if (d + 4 <= dh) {
+    store_n(row + d, t);
+  } else {
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      if (d + v < dh) row[d + v] = t[v];
+  }
+}
+
 // ------------------------------------------------------------------ rows in LDS
 // Row-major tiles of DP columns with 16 bytes of padding. `frag`: a fragment
 // along the row. `frag_t`: a fragment down the columns (column = lane % 16, the
@@ -155,6 +209,13 @@ struct Args {
   int64_t rows;      // lq * G
 };
 
+// A value at a uniform address that no kernel here writes: a scalar load.
+template <typename V>
+__device__ __forceinline__ V scalar_load(const V *p) {
+  typedef const __attribute__((address_space(4))) V *Const;
+  return *(Const)(p);
+}
+
 template <typename T>
 struct Seq {   // one (sequence, key head)
   const T *q, *k, *v;
@@ -168,8 +229,8 @@ __device__ __forceinline__ Seq<T> seq_of(const sgl_attention &p, int64_t n, int 
   s.q = static_cast<const T *>(p.q) + n * p.q_n + int64_t(hk) * G * p.q_h;
   s.k = static_cast<const T *>(p.k) + n * p.k_n + hk * p.k_h;
   s.v = static_cast<const T *>(p.v) + n * p.v_n + hk * p.v_h;
-  s.qlen = p.q_lens != nullptr ? min(max(int64_t(p.q_lens[n]), int64_t(0)), p.lq) : p.lq;
-  s.klen = p.k_lens != nullptr ? min(max(int64_t(p.k_lens[n]), int64_t(0)), p.lk) : p.lk;
+  s.qlen = p.q_lens != nullptr ? min(max(int64_t(scalar_load(p.q_lens + n)), int64_t(0)), p.lq) : p.lq;
+  s.klen = p.k_lens != nullptr ? min(max(int64_t(scalar_load(p.k_lens + n)), int64_t(0)), p.lk) : p.lk;
   s.mask = p.key_mask != nullptr ? p.key_mask + n * p.mask_n : nullptr;
   s.qpos = p.q_pos != nullptr ? p.q_pos + n * p.qpos_n : nullptr;
   s.kpos = p.k_pos != nullptr ? p.k_pos + n * p.kpos_n : nullptr;
@@ -215,9 +276,9 @@ struct TileAt {
 };
 __device__ __forceinline__ TileAt tile_at(uint32_t id, uint32_t tiles, int heads) {
   TileAt t;
-  const uint32_t item = id / tiles;
+  const uint32_t item = tiles == 1 ? id : __builtin_amdgcn_readfirstlane(id / tiles);   // (uniform: id is)
   t.tile = id - item * tiles;
-  const uint32_t n = item / uint32_t(heads);
+  const uint32_t n = heads == 1 ? item : __builtin_amdgcn_readfirstlane(item / uint32_t(heads));
   t.n = n;
   t.hk = int(item - n * uint32_t(heads));
   return t;
@@ -312,6 +373,10 @@ __device__ __forceinline__ float groups_max(float v) {
   auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
+// The wave's index in its workgroup, as a scalar: what depends on it alone is
+// then uniform to the compiler too (scalar loads, addresses and branches).
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 // LDS of one wave: its accesses are in order; nothing moves across this.
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -366,7 +431,7 @@ __device__ __forceinline__ float grad_scale(float most) {
 template <typename T>
 constexpr float kProbUp = std::is_same_v<T, fp16_t> ? 1024.f : 1.f;
 
-// The bias gradient's cells in LDS: [column][16] sums of ds for a set of row
+// The bias gradient's cells in LDS: [column][slots] sums of ds for a set of row
 // blocks whose row c has one head, in fixed point (34 fractional bits in an
 // int64, relative to a power of two near the largest |do|): integer adds give
 // the same sum in any order, and the LDS adds them at 7 to 8 clocks an
@@ -377,13 +442,16 @@ constexpr float kProbUp = std::is_same_v<T, fp16_t> ? 1024.f : 1.f;
 constexpr int kCellBits = 34;
 constexpr float kCellMax = 536870912.f;   // 2^29
 typedef unsigned long long Cell;
+// Cells a column: lane c of 16 adds into cell c mod slots; 8 where they
+// keep the heads apart (row c has head c mod heads), else 16.
+__host__ __device__ __forceinline__ int cell_slots(int heads) { return heads <= 8 && 16 % heads == 0 ? 8 : 16; }
 __device__ __forceinline__ void clear_cells(Cell *cells, int n, int tid, int threads) {
   for (int i = tid; i < n; i += threads) cells[i] = 0;
 }
 template <int N>
-__device__ __forceinline__ void add_cells(Cell *cells, const int (&col)[N][4], const float (&x)[N][4], float up,
-                                          float &seen) {
-  const int c = threadIdx.x & 15;
+__device__ __forceinline__ void add_cells(Cell *cells, const int (&col)[N][4], const float (&x)[N][4], int slots,
+                                          float up, float &seen) {
+  const int c = threadIdx.x & (slots - 1);
   const float f = up * 4.f;   // 2^34 = 2^2 2^32
 #pragma unroll
   for (int k = 0; k < N; ++k)
@@ -392,10 +460,18 @@ __device__ __forceinline__ void add_cells(Cell *cells, const int (&col)[N][4], c
       const float t = x[k][v] * f, hi = floorf(t);
       seen += fabsf(t);
       const Cell val = (Cell(uint32_t(int(hi))) << 32) | uint32_t((t - hi) * 4294967296.f);
-      __hip_atomic_fetch_add(cells + col[k][v] * 16 + c, val, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      __hip_atomic_fetch_add(cells + col[k][v] * slots + c, val, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
 }
 __device__ __forceinline__ bool cells_hold(float seen) { return seen < 4.f * kCellMax; }
+// Waves a SIMD that a kernel's registers leave room for (512 of them): asked of
+// the compiler, which otherwise spends registers on loads it could not issue
+// earlier anyway (two 8-wave workgroups a CU need 4).
+template <typename T, int DP>
+__host__ __device__ constexpr int simd_waves(int narrow, int wide) {   // heads up to 64 in 16 bits, or wider
+  return sizeof(T) == 2 && DP <= 64 ? narrow : wide;
+}
+
 // ------------------------------------------------------------------ key tiles of a workgroup
 // Keys of a tile that KW waves share, 32 each (fp32 with four waves: 16).
 template <typename T>
@@ -411,59 +487,90 @@ __host__ __device__ constexpr int buffers() {
   return sizeof(S) <= 24 * 1024 ? 2 : 1;
 }
 
-// A tile of TK keys on its way from memory to LDS: every wave looks at the
-// tile's keys, one (or two) a lane, for liveness and positions; the rows go by
-// 16-byte units over the workgroup, dead ones as 0.
+// The first n of 64 (n any sign)
+__device__ __forceinline__ uint64_t first_bits(int64_t n) { return n >= 64 ? ~0ull : n <= 0 ? 0 : (1ull << n) - 1; }
+
+// A tile of TK keys on its way from memory to LDS, by 16-byte units over the
+// workgroup. A thread's row offset and column are the same in every tile, so
+// its addresses are a uniform pointer and an offset kept. `load` only issues
+// loads (of every row inside the length: what it fetched is looked at in
+// `store`, a tile later, so that no wave waits for memory in between): there
+// the mask's bytes, one key a lane, become bits and dead rows 0, and the first
+// wave, which fetched the positions, tells whether all are near.
+template <int TK>
+struct KeyInfo {
+  PosTile<TK> pos;
+  int near_;
+};
 template <typename T, int DP, int TK, int BLOCK>
 struct KeyTile {
   using L = Tile<T, DP>;
-  static constexpr int W = TK / 64, PER = (TK * L::UPR + BLOCK - 1) / BLOCK, E = Mma<T>::E;
+  static constexpr int W = TK / 64, PER = (TK * L::UPR + BLOCK - 1) / BLOCK, E = Mma<T>::E, RSTEP = BLOCK / L::UPR;
+  static_assert(BLOCK % L::UPR == 0 && (PER == 1 || TK % RSTEP == 0), "units of a thread share their column");
   FragOf<T> kr[PER], vr[PER];
   uint64_t live[W];
-  int64_t pos[W];
-  bool near_ = true;
-  __device__ __forceinline__ bool row_live(int r) const { return (live[W == 1 ? 0 : r >> 6] >> (r & 63)) & 1; }
+  int64_t pos[W], koff, voff;
+  int byte[W], r0, d;
+  __device__ __forceinline__ KeyTile(const Args &a) {
+    r0 = threadIdx.x / L::UPR;
+    d = (threadIdx.x % L::UPR) * E;
+    const int at = min(d, a.p.head_dim - E);
+    koff = r0 * a.p.k_t + at;
+    voff = r0 * a.p.v_t + at;
+  }
   __device__ __forceinline__ uint32_t live_of(int first, int n) const {   // first: a multiple of 16, uniform
     return uint32_t(live[W == 1 ? 0 : first >> 6] >> (first & 63)) & full_mask(n);
   }
-  __device__ __forceinline__ void load(const Seq<T> &q, const Args &a, int64_t j0, int64_t base, bool qnear) {
+  __device__ __forceinline__ void load(const Seq<T> &q, const Args &a, int64_t j0) {
     const int lane = threadIdx.x & 63;
     const sgl_attention &p = a.p;
-    near_ = qnear;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      const int64_t j = j0 + 64 * i + lane;
-      const bool on = key_live(q, p, j);
-      live[i] = __ballot(on);
-      if (p.bias != nullptr) {
-        pos[i] = on ? q.kpos[j * p.kpos_t] : base;
-        near_ = near_ && __all(is_near(pos[i] - base));
+      live[i] = first_bits(q.klen - j0 - 64 * i);
+      const bool in = (live[i] >> lane) & 1;
+      byte[i] = 0;
+      pos[i] = 0;
+      if (q.mask != nullptr && in) byte[i] = q.mask[(j0 + 64 * i + lane) * p.mask_t];
+      if (p.bias != nullptr && threadIdx.x < 64 && in) pos[i] = q.kpos[(j0 + 64 * i + lane) * p.kpos_t];
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = r0 + i * RSTEP;
+      kr[i] = zero_frag<T>();
+      vr[i] = zero_frag<T>();
+      if (r < TK && d < p.head_dim && j0 + r < q.klen) {
+        __builtin_memcpy(&kr[i], q.k + (j0 + i * RSTEP) * p.k_t + koff, 16);
+        __builtin_memcpy(&vr[i], q.v + (j0 + i * RSTEP) * p.v_t + voff, 16);
       }
     }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int u = threadIdx.x + i * BLOCK, r = u / L::UPR, d = (u % L::UPR) * E;
-      const bool on = r < TK && row_live(min(r, TK - 1));
-      kr[i] = load_raw<T>(q.k + (j0 + r) * p.k_t, on, d, p.head_dim);
-      vr[i] = load_raw<T>(q.v + (j0 + r) * p.v_t, on, d, p.head_dim);
-    }
   }
-  __device__ __forceinline__ void store(T *k, T *v, PosTile<TK> &t, const Args &a, int64_t base) const {
-    const int dh = a.p.head_dim;
+  __device__ __forceinline__ void store(T *k, T *v, KeyInfo<TK> &t, const Seq<T> &q, const Args &a, int64_t base) {
+    const int dh = a.p.head_dim, lane = threadIdx.x & 63;
+    if (q.mask != nullptr) {   // uniform
+#pragma unroll
+      for (int i = 0; i < W; ++i) live[i] = __ballot(byte[i] != 0);
+    }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int u = threadIdx.x + i * BLOCK, r = u / L::UPR, d = (u % L::UPR) * E;
+      const int r = r0 + i * RSTEP;
       if (TK * L::UPR % BLOCK == 0 || r < TK) {
-        *reinterpret_cast<FragOf<T> *>(k + r * L::LD + d) = fix<T>(kr[i], d, dh);
-        *reinterpret_cast<FragOf<T> *>(v + r * L::LD + d) = fix<T>(vr[i], d, dh);
+        FragOf<T> kk = fix<T>(kr[i], d, dh), vv = fix<T>(vr[i], d, dh);
+        if (q.mask != nullptr && !((live[W == 1 ? 0 : r >> 6] >> (r & 63)) & 1)) kk = vv = zero_frag<T>();
+        *reinterpret_cast<FragOf<T> *>(k + r * L::LD + d) = kk;
+        *reinterpret_cast<FragOf<T> *>(v + r * L::LD + d) = vv;
       }
     }
     if (a.p.bias != nullptr && threadIdx.x < 64) {
+      bool near_ = true;
 #pragma unroll
       for (int i = 0; i < W; ++i) {
-        t.pos[64 * i + threadIdx.x] = pos[i];
-        t.rel[64 * i + threadIdx.x] = int(pos[i] - base);
+        const int64_t at = (live[i] >> lane) & 1 ? pos[i] : base;
+        near_ = near_ && is_near(at - base);
+        t.pos.pos[64 * i + lane] = at;
+        t.pos.rel[64 * i + lane] = int(at - base);
       }
+      near_ = __all(near_);
+      if (lane == 0) t.near_ = near_;
     }
   }
 };
@@ -481,7 +588,7 @@ __device__ __forceinline__ float *join_slot(float *pr, int w, int b) {
 }
 template <int KW, int NQ, int NB>
 __device__ __forceinline__ void put_join(float *pr, const f32x4 (&acc)[NQ][NB]) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
+  const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4, cl = lane & 15;
   if (w % KW == 0) return;
 #pragma unroll
   for (int b = 0; b < NQ; ++b) {
@@ -494,7 +601,7 @@ __device__ __forceinline__ void put_join(float *pr, const f32x4 (&acc)[NQ][NB]) 
 }
 template <int KW, int NQ, int NB>
 __device__ __forceinline__ void take_join(float *pr, f32x4 (&acc)[NQ][NB]) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
+  const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4, cl = lane & 15;
   if (w % KW != 0) return;
 #pragma unroll
   for (int k = 1; k < KW; ++k)
@@ -510,7 +617,7 @@ __device__ __forceinline__ void take_join(float *pr, f32x4 (&acc)[NQ][NB]) {
 template <int RW, int KW, int NQ, int NB>
 __device__ __forceinline__ void join_waves(char *smem, float (&m)[NQ], float (&l)[NQ], f32x4 (&acc)[NQ][NB]) {
   if constexpr (KW > 1) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15, w0 = w / KW * KW;
+    const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4, cl = lane & 15, w0 = w / KW * KW;
     float2 *ml = reinterpret_cast<float2 *>(smem);
     float *pr = reinterpret_cast<float *>(smem + sizeof(float2) * 16 * RW * KW * NQ);
     __syncthreads();
@@ -542,6 +649,11 @@ __device__ __forceinline__ void join_waves(char *smem, float (&m)[NQ], float (&l
 }
 
 // ------------------------------------------------------------------ launches
+// Two blocks a wave where their registers fit (fp32 heads above 64 would spill).
+template <typename T, int DP>
+constexpr bool two_blocks() {
+  return sizeof(T) == 2 || DP <= 64;
+}
 // Row tiles of a (sequence, key head), RW x NQ blocks each (SHARE: pairs).
 inline int64_t row_tiles(const Args &a, int nq, bool share, int rw) {
   const int64_t count = share ? a.rows / 2 : a.rows, per = share ? 16 * rw : 16 * rw * nq;

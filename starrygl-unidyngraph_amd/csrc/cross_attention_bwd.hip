@@ -13,12 +13,12 @@ namespace {
 // one tile it is the sum of p dp itself, which cancels exactly (a single key
 // has no gradient).
 template <typename T, int DP, int TK>
-struct DqLds {
+struct alignas(16) DqLds {
   T k[TK * Tile<T, DP>::LD], v[TK * Tile<T, DP>::LD];
-  PosTile<TK> pos;
+  KeyInfo<TK> info;
 };
 template <int ROWS>
-struct DqSums {
+struct alignas(16) DqSums {
   float red[8], delta[ROWS];
 };
 
@@ -31,10 +31,11 @@ __host__ __device__ __forceinline__ int cell_sets(int G) {
 }
 
 template <typename T, int DP, int NQ, bool SHARE, int RW, int KW>
-__global__ __launch_bounds__(RW * KW * 64) void k_attn_dq(Args a, int64_t tiles, const T *__restrict__ o,
+__global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t tiles, const T *__restrict__ o,
                                                           const T *__restrict__ rest, const float *__restrict__ lse,
                                                           const T *__restrict__ go, T *__restrict__ dq,
-                                                          float2 *__restrict__ rowstat, float *__restrict__ part) {
+                                                          float2 *__restrict__ rowstat, float *__restrict__ rowmost,
+                                                          float *__restrict__ part) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   constexpr int TK = tile_keys<T>(KW), BLOCK = RW * KW * 64, WAVES = RW * KW;
@@ -49,9 +50,9 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_dq(Args a, int64_t tiles,
   float *table = reinterpret_cast<float *>(smem + NB * sizeof(S) + sizeof(X));
   const sgl_attention &p = a.p;
   const int dh = p.head_dim;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
+  const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4, cl = lane & 15;
   const int wr = w / KW, k0 = (w % KW) * KB * 16;
-  const int sets = cell_sets<NQ, SHARE, RW>(a.G);
+  const int sets = cell_sets<NQ, SHARE, RW>(a.G), slots = cell_slots(SHARE ? a.G / 2 : a.G);
   Cell *cells = reinterpret_cast<Cell *>(smem + align_bytes(NB * sizeof(S) + sizeof(X) + table_bytes(a)));
   const TileAt at_ = tile_at(blockIdx.x, uint32_t(tiles), p.heads_kv);
   const uint32_t rt = at_.tile;
@@ -61,18 +62,18 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_dq(Args a, int64_t tiles,
   const bool biased = p.bias != nullptr;
   const Buckets bk = buckets_of(p);
   const uint32_t t0 = rt * (SHARE ? RW * 16 : RW * 16 * NQ);
-  const uint32_t i0 = row_at<SHARE>(t0, 0, a.G).i;
+  const uint32_t i0 = __builtin_amdgcn_readfirstlane(row_at<SHARE>(t0, 0, a.G).i);
   const bool any = i0 < q.qlen;
   const bool one_tile = q.klen <= kKeys;
   if (biased) stage_bias(table, a, hk, threadIdx.x, BLOCK);
-  if (part != nullptr) clear_cells(cells, sets * a.cols * 16, threadIdx.x, BLOCK);
+  if (part != nullptr) clear_cells(cells, sets * a.cols * slots, threadIdx.x, BLOCK);
   RowAt row[NQ];
   bool in[NQ], ok[NQ];
   FragOf<T> qf[NQ][ST], gf[NQ][ST];
   int64_t qpos[NP];
   int qrel[NP];
   float delta[NQ], ls[NQ], gs[NQ], top = 0.f;
-  const int64_t base = biased && any ? q.qpos[int64_t(i0) * p.qpos_t] : 0;
+  const int64_t base = biased && any ? scalar_load(q.qpos + int64_t(i0) * p.qpos_t) : 0;
   const int64_t stat0 = (n * p.heads_kv + hk) * a.rows;
   bool qnear = true;
 #pragma unroll
@@ -96,7 +97,7 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_dq(Args a, int64_t tiles,
         FragOf<T> rf = zero_frag<T>();
         if (rest != nullptr) rf = load_row<T>(rest + at, ok[b], d, dh);
 #pragma unroll
-        for (int e = 0; e < M::E; ++e) delta[b] += float(gf[b][st][e]) * (float(of[e]) + float(rf[e]));
+        for (int e = 0; e < M::E; ++e) delta[b] += float(gf[b][st][e]) * whole_of<T>(of[e], rf[e]);
       }
     }
     delta[b] = groups_sum(delta[b]);
@@ -105,7 +106,10 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_dq(Args a, int64_t tiles,
     gs[b] = grad_scale<T>(most);
     const int64_t r = stat0 + int64_t(row[b].i) * a.G + row[b].h;
     ls[b] = ok[b] ? lse[r] : INFINITY;
-    if (g == 0 && in[b] && w % KW == 0) rowstat[r] = make_float2(delta[b], most);
+    if (g == 0 && in[b] && w % KW == 0) {   // for dk and dv
+      rowstat[r] = make_float2(delta[b], ls[b]);
+      if (std::is_same_v<T, fp16_t>) rowmost[r] = most;
+    }
     if (b < NP) {
       qpos[b] = biased && ok[b] ? q.qpos[int64_t(row[b].i) * p.qpos_t] : base;
       qnear = qnear && is_near(qpos[b] - base);
@@ -129,23 +133,23 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_dq(Args a, int64_t tiles,
   for (int b = 0; b < NQ; ++b)
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  KeyTile<T, DP, TK, BLOCK> tile;
-  if (any && q.klen > 0) tile.load(q, a, 0, base, qnear);
+  KeyTile<T, DP, TK, BLOCK> tile(a);
+  if (any && q.klen > 0) tile.load(q, a, 0);
   int buf = 0;
   for (int64_t j0 = 0; any && j0 < q.klen; j0 += TK) {
     S &s = bufs[buf];
     if constexpr (NB == 1) __syncthreads();
     else buf ^= 1;
-    tile.store(s.k, s.v, s.pos, a, base);
+    tile.store(s.k, s.v, s.info, q, a, base);
     const uint32_t on = tile.live_of(k0, KB * 16);
-    const bool near_now = tile.near_;
     __syncthreads();
-    if (j0 + TK < q.klen) tile.load(q, a, j0 + TK, base, qnear);
+    if (j0 + TK < q.klen) tile.load(q, a, j0 + TK);
     float x[NQ][KB][4], y[NQ][KB][4];   // p and dp, then ds
     int col[NP][KB][4];
     if (biased) {
+      const bool near_now = qnear && s.info.near_ != 0;
 #pragma unroll
-      for (int b = 0; b < NP; ++b) columns(col[b], s.pos, k0 + 4 * g, qrel[b], qpos[b], near_now, 1, bk);
+      for (int b = 0; b < NP; ++b) columns(col[b], s.info.pos, k0 + 4 * g, qrel[b], qpos[b], near_now, 1, bk);
     }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
@@ -218,7 +222,7 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_dq(Args a, int64_t tiles,
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {
         const int set = sets == RW * NQ ? wr * NQ + b : SHARE ? b : 0;
-        add_cells(cells + set * a.cols * 16, col[b < NP ? b : 0], y[b], up, seen);
+        add_cells(cells + set * a.cols * slots, col[b < NP ? b : 0], y[b], slots, up, seen);
       }
     }
     if constexpr (std::is_same_v<T, fp16_t>) {
@@ -243,8 +247,8 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_dq(Args a, int64_t tiles,
     }
   }
   if (part != nullptr) {
-    // cell (set, column, c) belongs to the head of its blocks' row c: a thread
-    // sums a (head, column) over them
+    // cell (set, column, slot) belongs to the head of its blocks' row `slot`: a
+    // thread sums a (head, column) over them
     const bool held = __all(cells_hold(seen));
     __syncthreads();
     if (lane == 0) sx.red[w] = held ? 0.f : NAN;
@@ -260,9 +264,10 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_dq(Args a, int64_t tiles,
       for (int set = 0; set < sets; ++set) {
         const int ww = own ? set / NQ : 0, b = own ? set % NQ : SHARE ? set : 0;
         const int h0 = row_at<SHARE>(SHARE ? t0 + ww * 16 : t0 + (own ? set : 0) * 16, b, a.G).h;   // of c = 0
-        for (int i = 0; i < 16; ++i) {
-          const int e = (i + cidx) & 15;   // (rotated: neighbouring columns in different banks)
-          if ((h0 + (SHARE ? 2 : 1) * e) % a.G == h) t += static_cast<long long>(cells[(set * a.cols + cidx) * 16 + e]);
+        for (int i = 0; i < slots; ++i) {
+          const int e = (i + cidx) & (slots - 1);   // (rotated: neighbouring columns in different banks)
+          if ((h0 + (SHARE ? 2 : 1) * e) % a.G == h)
+            t += static_cast<long long>(cells[(set * a.cols + cidx) * slots + e]);
         }
       }
       out[x] = float(double(t) * (1.0 / double(1ll << kCellBits)) / double(up)) + bad;
@@ -289,35 +294,40 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_dq(Args a, int64_t tiles,
 // ------------------------------------------------------------------ dk, dv
 // A workgroup takes CW blocks of 16 keys (one a lane of 16) and walks the rows
 // of all G heads; RS waves share a key block, each with 32 rows of every tile,
-// and are joined at the end. With an even G the 32 are two heads of 16 queries
-// (SHARE). The next tile's rows are in flight while one is worked on.
+// and are joined at the end. The 32 rows of a step are two heads of 16
+// queries (SHARE, an even G) or 32 rows in order. The next tile's rows are in
+// flight while one is worked on: a thread's unit of a step lies at a uniform
+// pointer and an offset that it keeps (an odd G above one divides instead);
+// the first wave fetches what belongs to a row (D, lse, position).
 constexpr int kRows = 32;
 
 template <typename T, int DP, int TR>
-struct DkvLds {
+struct alignas(16) DkvLds {
   T q[TR * Tile<T, DP>::LD], go[TR * Tile<T, DP>::LD];
-  PosTile<TR> pos;
+  KeyInfo<TR> info;   // (of the rows)
   float lse[TR], delta[TR];
   int head[TR];
-  float red[8];
 };
 
 template <typename T, int DP, bool SHARE, int CW, int RS>
-__global__ __launch_bounds__(CW * RS * 64) void k_attn_dkv(Args a, int64_t tiles, const float *__restrict__ lse,
-                                                     const T *__restrict__ go, const float2 *__restrict__ rowstat,
-                                                     T *__restrict__ dk, T *__restrict__ dv) {
+__global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2))) void k_attn_dkv(Args a, int64_t tiles, const T *__restrict__ go,
+                                                           const float2 *__restrict__ rowstat,
+                                                           const float *__restrict__ rowmost, T *__restrict__ dk,
+                                                           T *__restrict__ dv) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   constexpr int TR = kRows * RS, BLOCK = CW * RS * 64, WAVES = CW * RS;
   using S = DkvLds<T, DP, TR>;
+  constexpr int NB = buffers<S>();
   constexpr int ST = DP / M::KS, DB = DP / 16, RB = kRows / 16, NP = SHARE ? 1 : RB;
   constexpr bool kHalf = std::is_same_v<T, fp16_t>;
   extern __shared__ __align__(16) char smem[];
-  S &s = *reinterpret_cast<S *>(smem);
-  float *table = reinterpret_cast<float *>(smem + sizeof(s));
+  S *const bufs = reinterpret_cast<S *>(smem);
+  float *red = reinterpret_cast<float *>(smem + NB * sizeof(S));
+  float *table = red + 8;
   const sgl_attention &p = a.p;
   const int dh = p.head_dim;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4;
+  const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4;
   const TileAt at_ = tile_at(blockIdx.x, uint32_t(tiles), p.heads_kv);
   const int64_t kt = at_.tile;
   const int hk = at_.hk;
@@ -330,22 +340,20 @@ __global__ __launch_bounds__(CW * RS * 64) void k_attn_dkv(Args a, int64_t tiles
   const Buckets bk = buckets_of(p);
   if (biased) stage_bias(table, a, hk, threadIdx.x, BLOCK);
   const int64_t stat0 = (n * p.heads_kv + hk) * a.rows;
-  // steps of 32 rows (blocks of 16 queries x head pairs, or 32 rows in order), RS of them a tile
-  const int pairs = a.G >> 1;
+  const uint32_t pairs = uint32_t(a.G) >> 1, qlen = uint32_t(q.qlen);
   const bool any = kt * CW * 16 < q.klen;
-  const uint32_t qlen = uint32_t(q.qlen);
-  const uint32_t steps = !any ? 0 : SHARE ? (qlen + 15) / 16 * uint32_t(pairs) : (qlen * a.G + kRows - 1) / kRows;
+  const uint32_t steps = !any ? 0 : SHARE ? (qlen + 15) / 16 * pairs : (qlen * a.G + kRows - 1) / kRows;
   float gs = 1.f;
   if constexpr (kHalf) {
     float most = 0.f;
     if (any)
-      for (uint32_t r = threadIdx.x; r < qlen * a.G; r += BLOCK) most = fmaxf(most, rowstat[stat0 + r].y);
+      for (uint32_t r = threadIdx.x; r < qlen * a.G; r += BLOCK) most = fmaxf(most, rowmost[stat0 + r]);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, kWave));
-    if (lane == 0) s.red[w] = most;
+    if (lane == 0) red[w] = most;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) most = fmaxf(most, s.red[i]);
+    for (int i = 0; i < WAVES; ++i) most = fmaxf(most, red[i]);
     gs = grad_scale<T>(most);
   }
   FragOf<T> kf[ST], vf[ST];
@@ -355,7 +363,7 @@ __global__ __launch_bounds__(CW * RS * 64) void k_attn_dkv(Args a, int64_t tiles
     kf[st] = load_row<T>(q.k + j * p.k_t, on, d, dh);
     vf[st] = load_row<T>(q.v + j * p.v_t, on, d, dh);
   }
-  const int64_t base = biased && steps > 0 ? q.qpos[0] : 0;
+  const int64_t base = biased && steps > 0 ? scalar_load(q.qpos) : 0;
   const int64_t kp = biased && on ? q.kpos[j * p.kpos_t] : base;
   const int krel = int(kp - base);
   const bool knear = __all(is_near(kp - base));
@@ -364,79 +372,113 @@ __global__ __launch_bounds__(CW * RS * 64) void k_attn_dkv(Args a, int64_t tiles
   f32x4 acc[2][DB];   // dk, dv
 #pragma unroll
   for (int b = 0; b < DB; ++b) acc[0][b] = acc[1][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-  constexpr int PER = (TR * L::UPR + BLOCK - 1) / BLOCK;
+  constexpr int RSTEP = BLOCK / L::UPR, PER = (TR + RSTEP - 1) / RSTEP, RL = (TR + 63) / 64;
+  static_assert(RSTEP % kRows == 0 || kRows % RSTEP == 0, "a pass of the workgroup keeps a thread's place in a step");
   FragOf<T> qr[PER], gr[PER];
-  constexpr int RL = (TR + 63) / 64;   // rows a lane looks at (every wave sees the whole tile)
-  int64_t qp[RL];
-  float ls[RL], de[RL];
-  int he[RL];
-  bool near_ = true;
-  auto row_of = [&](uint32_t step, int i) {   // row i of a step's 32
+  // a step's first row (i, h) and a thread's row x of its 32 from there
+  const bool flat = SHARE || a.G == 1;
+  auto first_of = [&](uint32_t step) {
     if constexpr (SHARE) {
-      const uint32_t ib = pairs == 1 ? step : step / uint32_t(pairs);
-      return RowAt{ib * 16 + (i & 15), int(step - ib * pairs) * 2 + (i >> 4)};
+      const uint32_t ib = pairs == 1 ? step : step / pairs;
+      return RowAt{ib * 16, int(step - ib * pairs) * 2};
     } else {
-      return row_at<false>(step * kRows + i, 0, a.G);
+      return row_at<false>(step * kRows, 0, a.G);
     }
   };
+  auto row_of = [&](const RowAt &f, uint32_t step, int x) {
+    if constexpr (SHARE) return RowAt{f.i + (x & 15), f.h + (x >> 4)};
+    else return flat ? RowAt{f.i + x, 0} : row_at<false>(step * kRows + x, 0, a.G);
+  };
+  const int r0 = threadIdx.x / L::UPR, d0 = (threadIdx.x % L::UPR) * M::E, at0 = min(d0, dh - M::E);
+  const int64_t go_t = int64_t(p.heads_q) * dh;
+  auto offset = [&](int x, int64_t t, int64_t h) { return SHARE ? (x & 15) * t + (x >> 4) * h : x * t; };
+  constexpr int PLACES = RSTEP < kRows ? kRows / RSTEP : 1;
+  static_assert(PLACES <= 8, "places of a thread in a step");
+  int64_t qo[PLACES], gofs[PLACES];
+#pragma unroll
+  for (int i = 0; i < PLACES; ++i) {
+    qo[i] = offset(r0 % kRows + i * RSTEP, p.q_t, p.q_h) + at0;
+    gofs[i] = offset(r0 % kRows + i * RSTEP, go_t, dh) + at0;
+  }
+  int64_t qp[RL];
+  float2 st_[RL];
+  int he[RL] = {};
   auto load_step = [&](uint32_t step) {
-    near_ = knear;
 #pragma unroll
     for (int i = 0; i < RL; ++i) {
-      const int rr = i * 64 + lane;
-      const RowAt r = row_of(step + rr / kRows, rr % kRows);
-      const bool ok = rr < TR && r.i < qlen;
-      ls[i] = ok ? lse[stat0 + int64_t(r.i) * a.G + r.h] : INFINITY;
-      de[i] = ok ? rowstat[stat0 + int64_t(r.i) * a.G + r.h].x : 0.f;
-      he[i] = r.h;
-      qp[i] = base;
-      if (biased) {
-        if (ok) qp[i] = q.qpos[int64_t(r.i) * p.qpos_t];
-        near_ = near_ && __all(is_near(qp[i] - base));
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int u = threadIdx.x + i * BLOCK, rr = u / L::UPR, d = (u % L::UPR) * M::E;
-      // (a wave's units lie in one step of 32 rows: its division is a scalar one)
-      const RowAt t = row_of(step + uint32_t(__builtin_amdgcn_readfirstlane(rr / kRows)), rr % kRows);
-      const bool okr = rr < TR && t.i < qlen;
-      qr[i] = load_raw<T>(q.q + int64_t(t.i) * p.q_t + t.h * p.q_h, okr, d, dh);
-      gr[i] = load_raw<T>(go + out_row(a, n, hk, t.i, t.h), okr, d, dh);
-    }
-  };
-  if (steps > 0) load_step(0);
-  for (uint32_t step = 0; step < steps; step += RS) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int u = threadIdx.x + i * BLOCK, rr = u / L::UPR, d = (u % L::UPR) * M::E;
-      if (rr < TR) {
-        *reinterpret_cast<FragOf<T> *>(s.q + rr * L::LD + d) = fix<T>(qr[i], d, dh);
-        *reinterpret_cast<FragOf<T> *>(s.go + rr * L::LD + d) = fix<T>(gr[i], d, dh);
-      }
-    }
-    if (w == 0) {
-#pragma unroll
-      for (int i = 0; i < RL; ++i) {
-        const int rr = i * 64 + lane;
-        if (rr < TR) {
-          s.lse[rr] = ls[i];
-          s.delta[rr] = de[i];
-          s.head[rr] = he[i] * table_ld(a);
-          s.pos.pos[rr] = qp[i];
-          s.pos.rel[rr] = int(qp[i] - base);
+      st_[i] = make_float2(0.f, INFINITY);
+      qp[i] = 0;
+      if (w == 0) {
+        const int x = i * 64 + lane;
+        const uint32_t sub = step + x / kRows;
+        const RowAt r = row_of(first_of(sub), sub, x % kRows);
+        he[i] = r.h;
+        if (x < TR && r.i < qlen) {
+          st_[i] = rowstat[stat0 + int64_t(r.i) * a.G + r.h];
+          if (biased) qp[i] = q.qpos[int64_t(r.i) * p.qpos_t];
         }
       }
     }
-    const bool near_now = near_;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int x = r0 + i * RSTEP;
+      // (a wave's rows lie in one step of 32)
+      const uint32_t sub = step + uint32_t(__builtin_amdgcn_readfirstlane(x / kRows));
+      const RowAt f = first_of(sub), t = row_of(f, sub, x % kRows);
+      qr[i] = zero_frag<T>();
+      gr[i] = zero_frag<T>();
+      if (x < TR && t.i < qlen && d0 < dh) {
+        if (flat) {
+          const T *qb = q.q + int64_t(f.i) * p.q_t + f.h * p.q_h;
+          const T *gb = go + out_row(a, n, hk, f.i, f.h);
+          __builtin_memcpy(&qr[i], qb + qo[i % PLACES], 16);
+          __builtin_memcpy(&gr[i], gb + gofs[i % PLACES], 16);
+        } else {
+          __builtin_memcpy(&qr[i], q.q + int64_t(t.i) * p.q_t + t.h * p.q_h + at0, 16);
+          __builtin_memcpy(&gr[i], go + out_row(a, n, hk, t.i, t.h) + at0, 16);
+        }
+      }
+    }
+  };
+  if (steps > 0) load_step(0);
+  int buf = 0;
+  for (uint32_t step = 0; step < steps; step += RS) {
+    S &s = bufs[buf];
+    if constexpr (NB == 1) __syncthreads();
+    else buf ^= 1;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int x = r0 + i * RSTEP;
+      if (TR % RSTEP == 0 || x < TR) {
+        *reinterpret_cast<FragOf<T> *>(s.q + x * L::LD + d0) = fix<T>(qr[i], d0, dh);
+        *reinterpret_cast<FragOf<T> *>(s.go + x * L::LD + d0) = fix<T>(gr[i], d0, dh);
+      }
+    }
+    if (w == 0) {
+      bool near_ = true;   // (looked at here, a tile after its load)
+#pragma unroll
+      for (int i = 0; i < RL; ++i) {
+        const int x = i * 64 + lane;
+        const int64_t at = st_[i].y == INFINITY ? base : qp[i];   // (no row, or one without p)
+        near_ = near_ && is_near(at - base);
+        if (x < TR) {
+          s.lse[x] = st_[i].y;
+          s.delta[x] = st_[i].x;
+          s.head[x] = he[i] * table_ld(a);
+          s.info.pos.pos[x] = at;
+          s.info.pos.rel[x] = int(at - base);
+        }
+      }
+      near_ = __all(near_);
+      if (lane == 0) s.info.near_ = near_;
+    }
     __syncthreads();
     if (step + RS < steps) load_step(step + RS);
     float x[RB][4], y[RB][4];   // p and ds, rows x this lane's key
     int col[RB][4];
     if (biased) {
       int own[NP][4];
-      columns(own, s.pos, x0 + 4 * g, krel, kp, near_now, -1, bk);
+      columns(own, s.info.pos, x0 + 4 * g, krel, kp, knear && s.info.near_ != 0, -1, bk);
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
@@ -497,9 +539,18 @@ __global__ __launch_bounds__(CW * RS * 64) void k_attn_dkv(Args a, int64_t tiles
 }
 
 // ------------------------------------------------------------------ host
-size_t stat_bytes(const Args &a) { return align_up(sizeof(float2) * size_t(a.p.n * a.p.heads_kv * a.rows)); }
+size_t stat_bytes(const Args &a) {
+  const size_t rows = size_t(a.p.n * a.p.heads_kv * a.rows);
+  return align_up(sizeof(float2) * rows) + (a.p.dtype == SGL_FP16 ? align_up(sizeof(float) * rows) : 0);
+}
+float *most_of(const Args &a, float2 *stat) {
+  return reinterpret_cast<float *>(reinterpret_cast<char *>(stat) +
+                                   align_up(sizeof(float2) * size_t(a.p.n * a.p.heads_kv * a.rows)));
+}
 int64_t dq_tiles(const Args &a) {
-  return many_rows(a) ? row_tiles(a, 2, a.G % 2 == 0, 4) : row_tiles(a, 1, false, 1);
+  if (!many_rows(a)) return row_tiles(a, 1, false, 1);
+  const bool two = a.p.dtype != SGL_FP32 || a.p.head_dim <= 64;   // two_blocks
+  return two ? row_tiles(a, 2, a.G % 2 == 0, 4) : row_tiles(a, 1, false, 4);
 }
 
 template <typename T, int DP, int NQ, bool SHARE, int RW, int KW>
@@ -508,27 +559,28 @@ int launch_dq(const Args &a, int64_t tiles, const void *o, const void *rest, con
   const size_t lds = std::max(
       align_bytes(buffers<DqLds<T, DP, tile_keys<T>(KW)>>() * sizeof(DqLds<T, DP, tile_keys<T>(KW)>) +
                   sizeof(DqSums<RW * KW * NQ * 16>) + table_bytes(a)) +
-          (part != nullptr ? sizeof(Cell) * cell_sets<NQ, SHARE, RW>(a.G) * 16 * size_t(a.cols) : 0),
+          (part != nullptr ? sizeof(Cell) * cell_sets<NQ, SHARE, RW>(a.G) * cell_slots(SHARE ? a.G / 2 : a.G) * size_t(a.cols) : 0),
       join_bytes(RW, KW, NQ, DP));
   SGL_REQUIRE(lds <= 160 * 1024, "cross_attention_backward: %zu bytes of LDS", lds);
   SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_dq<T, DP, NQ, SHARE, RW, KW>), lds));
   launch(&k_attn_dq<T, DP, NQ, SHARE, RW, KW>, dim3(unsigned(a.p.n * a.p.heads_kv * tiles)), dim3(RW * KW * kWave), lds,
          s, a, tiles, static_cast<const T *>(o), static_cast<const T *>(rest), lse, static_cast<const T *>(go),
-         static_cast<T *>(dq), stat, part);
+         static_cast<T *>(dq), stat, most_of(a, stat), part);
   SGL_CHECK_LAUNCH();
   return SGL_OK;
 }
 
 template <typename T, int DP, bool SHARE, int CW, int RS>
-int launch_dkv(const Args &a, const float *lse, const void *go, const float2 *stat, void *dk, void *dv,
-               hipStream_t s) {
+int launch_dkv(const Args &a, const void *go, float2 *stat, void *dk, void *dv, hipStream_t s) {
   const int64_t tiles = (a.p.lk + 16 * CW - 1) / (16 * CW);
-  const size_t lds = std::max(sizeof(DkvLds<T, DP, kRows * RS>) + table_bytes(a),
+  using S = DkvLds<T, DP, kRows * RS>;
+  const size_t lds = std::max(buffers<S>() * sizeof(S) + 8 * sizeof(float) + table_bytes(a),
                               join_bytes(CW, RS, 2, DP));
   SGL_REQUIRE(lds <= 160 * 1024, "cross_attention_backward: %zu bytes of LDS", lds);
   SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_dkv<T, DP, SHARE, CW, RS>), lds));
   launch(&k_attn_dkv<T, DP, SHARE, CW, RS>, dim3(unsigned(a.p.n * a.p.heads_kv * tiles)), dim3(CW * RS * kWave), lds, s,
-         a, tiles, lse, static_cast<const T *>(go), stat, static_cast<T *>(dk), static_cast<T *>(dv));
+         a, tiles, static_cast<const T *>(go), static_cast<const float2 *>(stat),
+         static_cast<const float *>(most_of(a, stat)), static_cast<T *>(dk), static_cast<T *>(dv));
   SGL_CHECK_LAUNCH();
   return SGL_OK;
 }
@@ -550,6 +602,7 @@ int run_backward(const Args &a, const void *o, const void *rest, const float *ls
     if (tiles > 0) {
       int rc;
       if (!many_rows(a)) rc = launch_dq<T, DP, 1, false, 1, 4>(a, tiles, o, rest, lse, go, dq, stat, part, s);
+      else if constexpr (!two_blocks<T, DP>()) rc = launch_dq<T, DP, 1, false, 4, 2>(a, tiles, o, rest, lse, go, dq, stat, part, s);
       else if (a.G % 2 == 0) rc = launch_dq<T, DP, 2, true, 4, 2>(a, tiles, o, rest, lse, go, dq, stat, part, s);
       else rc = launch_dq<T, DP, 2, false, 4, 2>(a, tiles, o, rest, lse, go, dq, stat, part, s);
       if (rc != SGL_OK) return rc;
@@ -561,11 +614,12 @@ int run_backward(const Args &a, const void *o, const void *rest, const float *ls
     }
     // 64 keys a workgroup where that fills the GPU, else 16, its four waves along the rows
     const bool wide = a.p.n * a.p.heads_kv * ((a.p.lk + 63) / 64) >= 192;
+    constexpr int RS = two_blocks<T, DP>() && DP <= 64 ? 1 : 2;   // (three 4-wave workgroups a CU, or one of 8)
     if (a.G % 2 == 0)
-      return wide ? launch_dkv<T, DP, true, 4, 2>(a, lse, go, stat, dk, dv, s)
-                  : launch_dkv<T, DP, true, 1, 4>(a, lse, go, stat, dk, dv, s);
-    return wide ? launch_dkv<T, DP, false, 4, 2>(a, lse, go, stat, dk, dv, s)
-                : launch_dkv<T, DP, false, 1, 4>(a, lse, go, stat, dk, dv, s);
+      return wide ? launch_dkv<T, DP, true, 4, RS>(a, go, stat, dk, dv, s)
+                  : launch_dkv<T, DP, true, 1, 4>(a, go, stat, dk, dv, s);
+    return wide ? launch_dkv<T, DP, false, 4, RS>(a, go, stat, dk, dv, s)
+                : launch_dkv<T, DP, false, 1, 4>(a, go, stat, dk, dv, s);
   });
 }
 

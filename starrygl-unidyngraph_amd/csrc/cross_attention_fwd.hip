@@ -17,16 +17,24 @@ namespace {
 // maximum, sum and rescale are its own, joined over four lanes only. The
 // accumulators are rescaled only when the maximum has grown by more than 2^6:
 // p stays below 2^6, and the sum and the products carry the same factor.
+// p is rounded to the operands' type for its product. Where a backward will
+// follow, what that rounding leaves is multiplied too (two more parts: 24 bits),
+// so that o and `rest` together hold o to 32 bits' precision: D = <do, o> meets
+// p dp in sums of a column over all rows and keys that nearly cancel, where an
+// error in D, the same for a whole row, does not. With p in one part the bias
+// table's gradient was 0.3 % off, with two 5e-6, with three 3e-6 (the error of
+// the formula in 32 bits throughout); the extra products take the forward of
+// 8 x 8 x 1000 x 2049 heads of 64 from 119 to 178 us.
 constexpr float kSlack = 6.f;
 
 template <typename T, int DP, int TK>
-struct FwdLds {
+struct alignas(16) FwdLds {
   T k[TK * Tile<T, DP>::LD], v[TK * Tile<T, DP>::LD];
-  PosTile<TK> pos;
+  KeyInfo<TK> info;
 };
 
-template <typename T, int DP, int NQ, bool SHARE, int RW, int KW>
-__global__ __launch_bounds__(RW * KW * 64) void k_attn_fwd(Args a, int64_t tiles, T *__restrict__ o,
+template <typename T, int DP, int NQ, bool SHARE, int RW, int KW, bool SPLIT>
+__global__ __launch_bounds__(RW * KW * 64, (simd_waves<T, DP>(4, 2))) void k_attn_fwd(Args a, int64_t tiles, T *__restrict__ o,
                                                            T *__restrict__ rest, float *__restrict__ lse) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
@@ -40,7 +48,7 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_fwd(Args a, int64_t tiles
   float *table = reinterpret_cast<float *>(smem + NB * sizeof(S));
   const sgl_attention &p = a.p;
   const int dh = p.head_dim;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
+  const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4, cl = lane & 15;
   const int wr = w / KW, k0 = (w % KW) * KB * 16;   // this wave's row blocks, and its first key of a tile
   const TileAt at_ = tile_at(blockIdx.x, uint32_t(tiles), p.heads_kv);
   const uint32_t rt = at_.tile;
@@ -51,7 +59,7 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_fwd(Args a, int64_t tiles
   const Buckets bk = buckets_of(p);
   // the workgroup's first query; nothing to do past the length
   const uint32_t t0 = rt * (SHARE ? RW * 16 : RW * 16 * NQ);
-  const uint32_t i0 = row_at<SHARE>(t0, 0, a.G).i;
+  const uint32_t i0 = __builtin_amdgcn_readfirstlane(row_at<SHARE>(t0, 0, a.G).i);
   const bool any = i0 < q.qlen;
   if (biased) stage_bias(table, a, hk, threadIdx.x, BLOCK);
   RowAt row[NQ];
@@ -59,7 +67,7 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_fwd(Args a, int64_t tiles
   FragOf<T> qf[NQ][ST];
   int64_t qpos[NP];
   int qrel[NP];
-  const int64_t base = biased && any ? q.qpos[int64_t(i0) * p.qpos_t] : 0;
+  const int64_t base = biased && any ? scalar_load(q.qpos + int64_t(i0) * p.qpos_t) : 0;
   bool qnear = true;
 #pragma unroll
   for (int b = 0; b < NQ; ++b) {
@@ -87,23 +95,23 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_fwd(Args a, int64_t tiles
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  KeyTile<T, DP, TK, BLOCK> tile;
-  if (any && q.klen > 0) tile.load(q, a, 0, base, qnear);
+  KeyTile<T, DP, TK, BLOCK> tile(a);
+  if (any && q.klen > 0) tile.load(q, a, 0);
   int buf = 0;
   for (int64_t j0 = 0; any && j0 < q.klen; j0 += TK) {
     S &s = bufs[buf];
     if constexpr (NB == 1) __syncthreads();
     else buf ^= 1;
-    tile.store(s.k, s.v, s.pos, a, base);
+    tile.store(s.k, s.v, s.info, q, a, base);
     const uint32_t on = tile.live_of(k0, KB * 16);   // this wave's keys
-    const bool near_now = tile.near_;
     __syncthreads();
-    if (j0 + TK < q.klen) tile.load(q, a, j0 + TK, base, qnear);
+    if (j0 + TK < q.klen) tile.load(q, a, j0 + TK);
     float x[NQ][KB][4], mx[NQ];
     int col[NP][KB][4];
     if (biased) {
+      const bool near_now = qnear && s.info.near_ != 0;
 #pragma unroll
-      for (int b = 0; b < NP; ++b) columns(col[b], s.pos, k0 + 4 * g, qrel[b], qpos[b], near_now, 1, bk);
+      for (int b = 0; b < NP; ++b) columns(col[b], s.info.pos, k0 + 4 * g, qrel[b], qpos[b], near_now, 1, bk);
     }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
@@ -157,17 +165,34 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_fwd(Args a, int64_t tiles
           l[b] += x[b][kb][v];
         }
     }
+    if constexpr (!SPLIT) {
 #pragma unroll
-    for (int st = 0; st < KB * 16 / M::KS; ++st) {
-      FragOf<T> pf[NQ];
+      for (int st = 0; st < KB * 16 / M::KS; ++st) {
+        FragOf<T> pf[NQ];
 #pragma unroll
-      for (int b = 0; b < NQ; ++b) pf[b] = frag_of<T>(x[b], st);
+        for (int b = 0; b < NQ; ++b) pf[b] = frag_of<T>(x[b], st);
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const FragOf<T> vf = L::template frag_t<TK>(s.v, d * 16, k0 + st * M::KS);
+        for (int d = 0; d < DB; ++d) {
+          const FragOf<T> vf = L::template frag_t<TK>(s.v, d * 16, k0 + st * M::KS);
 #pragma unroll
-        for (int b = 0; b < NQ; ++b) acc[b][d] = M::mma(vf, pf[b], acc[b][d]);
+          for (int b = 0; b < NQ; ++b) acc[b][d] = M::mma(vf, pf[b], acc[b][d]);
+        }
       }
+    } else {   // a block at a time, the values' fragments read again: no registers to keep them
+#pragma unroll
+      for (int b = 0; b < NQ; ++b)
+#pragma unroll
+        for (int st = 0; st < KB * 16 / M::KS; ++st) {
+          FragOf<T> pf[3];
+          split_frag_of<T>(x[b], st, pf);
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            const FragOf<T> vf = L::template frag_t<TK>(s.v, d * 16, k0 + st * M::KS);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) acc[b][d] = M::mma(vf, pf[i], acc[b][d]);
+          }
+        }
     }
   }
 #pragma unroll
@@ -183,12 +208,7 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_fwd(Args a, int64_t tiles
     for (int d = 0; d < DB; ++d) {
       const f32x4 v = acc[b][d] * inv;
       store4(o + at, d * 16 + 4 * g, dh, v);
-      if (rest != nullptr) {   // what rounding o left, for the backward's D
-        f32x4 e;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = v[i] - float(T(v[i]));
-        store4(rest + at, d * 16 + 4 * g, dh, e);
-      }
+      if (rest != nullptr) store_rest(rest + at, d * 16 + 4 * g, dh, v);   // for the backward's D
     }
     // log2 of the sum of 2^x; +inf where no key is live, so that p is 0 there
     if (lse != nullptr && g == 0)
@@ -208,13 +228,13 @@ __global__ __launch_bounds__(RW * KW * 64) void k_attn_fwd(Args a, int64_t tiles
 constexpr int kStep = 32;
 
 template <typename T, int DP, int NQ>
-struct FewLds {
+struct alignas(16) FewLds {
   T v[kStep * Tile<T, DP>::LD];
   PosTile<kStep> pos;
 };
 
-template <typename T, int DP, int NQ>
-__global__ __launch_bounds__(kBlock) void k_attn_few(Args a, int parts, int64_t part_keys, T *__restrict__ o,
+template <typename T, int DP, int NQ, bool SPLIT>
+__global__ __launch_bounds__(kBlock, (simd_waves<T, DP>(3, DP <= 64 ? 2 : 1))) void k_attn_few(Args a, int parts, int64_t part_keys, T *__restrict__ o,
                                                      T *__restrict__ rest, float *__restrict__ lse,
                                                      float *__restrict__ pacc, float2 *__restrict__ pml) {
   using M = Mma<T>;
@@ -223,7 +243,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_few(Args a, int parts, int64_t 
   extern __shared__ __align__(16) char smem[];
   const sgl_attention &p = a.p;
   const int dh = p.head_dim;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
+  const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4, cl = lane & 15;
   using Lds = FewLds<T, DP, NQ>;
   const size_t per = align_bytes(sizeof(Lds) + table_bytes(a));
   Lds &s = *reinterpret_cast<Lds *>(smem + w * per);
@@ -245,7 +265,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_few(Args a, int parts, int64_t 
   FragOf<T> qf[NQ][ST];
   int64_t qpos[NQ];
   int qrel[NQ];
-  const int64_t base = biased && q.qlen > 0 ? q.qpos[0] : 0;
+  const int64_t base = biased && q.qlen > 0 ? scalar_load(q.qpos) : 0;
   bool qnear = true;
 #pragma unroll
   for (int b = 0; b < NQ; ++b) {
@@ -275,42 +295,46 @@ __global__ __launch_bounds__(kBlock) void k_attn_few(Args a, int parts, int64_t 
   int64_t j0 = parts == 0 ? 0 : part * part_keys + w * kStep;
   constexpr int PER = kStep * L::UPR / kWave;
   FragOf<T> kr[KB][ST], vr[PER];
-  uint64_t live = 0;
-  bool near_ = true;
-  int64_t kp = 0;
-  auto load_tile = [&](int64_t j) {
-    const bool on = lane < kStep && key_live(q, p, j + lane);
-    live = __ballot(on);
-    if (biased) {
-      kp = on ? q.kpos[(j + lane) * p.kpos_t] : base;
-      near_ = qnear && __all(is_near(kp - base));
-    }
+  int64_t kpos = 0;
+  int byte = 0;
+  auto load_tile = [&](int64_t j) {   // (only issues loads: what they bring is looked at a step later)
+    const bool in = lane < kStep && j + lane < q.klen;
+    byte = 0;
+    kpos = 0;
+    if (q.mask != nullptr && in) byte = q.mask[(j + lane) * p.mask_t];
+    if (biased && in) kpos = q.kpos[(j + lane) * p.kpos_t];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int st = 0; st < ST; ++st)
-        kr[kb][st] = load_raw<T>(q.k + (j + kb * 16 + cl) * p.k_t, (live >> (kb * 16 + cl)) & 1, st * M::KS + g * M::E,
-                                 dh);
+        kr[kb][st] = load_raw<T>(q.k + (j + kb * 16 + cl) * p.k_t, j + kb * 16 + cl < q.klen, st * M::KS + g * M::E, dh);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int u = lane + i * kWave, r = u / L::UPR, d = (u % L::UPR) * M::E;
-      vr[i] = load_raw<T>(q.v + (j + r) * p.v_t, (live >> r) & 1, d, dh);
+      vr[i] = load_raw<T>(q.v + (j + r) * p.v_t, j + r < q.klen, d, dh);
     }
   };
   if (j0 < end) load_tile(j0);
   for (; j0 < end; j0 += stride) {
-    const uint64_t on = live;
-    const bool near_now = near_;
+    uint32_t on = uint32_t(first_bits(q.klen - j0));
+    if (q.mask != nullptr) on &= uint32_t(__ballot(byte != 0));
     FragOf<T> kf[KB][ST];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int st = 0; st < ST; ++st) kf[kb][st] = fix<T>(kr[kb][st], st * M::KS + g * M::E, dh);
+      for (int st = 0; st < ST; ++st) {
+        kf[kb][st] = fix<T>(kr[kb][st], st * M::KS + g * M::E, dh);
+        if (q.mask != nullptr && !((on >> (kb * 16 + cl)) & 1)) kf[kb][st] = zero_frag<T>();
+      }
+    const int64_t kp = lane < kStep && ((on >> (lane & 31)) & 1) ? kpos : base;
+    const bool near_now = qnear && __all(is_near(kp - base));
     wave_sync();   // the reads of the tile before are done
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int u = lane + i * kWave, r = u / L::UPR, d = (u % L::UPR) * M::E;
-      *reinterpret_cast<FragOf<T> *>(s.v + r * L::LD + d) = fix<T>(vr[i], d, dh);
+      FragOf<T> vv = fix<T>(vr[i], d, dh);
+      if (q.mask != nullptr && !((on >> r) & 1)) vv = zero_frag<T>();
+      *reinterpret_cast<FragOf<T> *>(s.v + r * L::LD + d) = vv;
     }
     if (biased && lane < kStep) {
       s.pos.pos[lane] = kp;
@@ -357,17 +381,34 @@ __global__ __launch_bounds__(kBlock) void k_attn_few(Args a, int parts, int64_t 
           l[b] += x[b][kb][v];
         }
     }
+    if constexpr (!SPLIT) {
 #pragma unroll
-    for (int st = 0; st < kStep / M::KS; ++st) {
-      FragOf<T> pf[NQ];
+      for (int st = 0; st < kStep / M::KS; ++st) {
+        FragOf<T> pf[NQ];
 #pragma unroll
-      for (int b = 0; b < NQ; ++b) pf[b] = frag_of<T>(x[b], st);
+        for (int b = 0; b < NQ; ++b) pf[b] = frag_of<T>(x[b], st);
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const FragOf<T> vf = L::template frag_t<kStep>(s.v, d * 16, st * M::KS);
+        for (int d = 0; d < DB; ++d) {
+          const FragOf<T> vf = L::template frag_t<kStep>(s.v, d * 16, st * M::KS);
 #pragma unroll
-        for (int b = 0; b < NQ; ++b) acc[b][d] = M::mma(vf, pf[b], acc[b][d]);
+          for (int b = 0; b < NQ; ++b) acc[b][d] = M::mma(vf, pf[b], acc[b][d]);
+        }
       }
+    } else {   // a block at a time, the values' fragments read again: no registers to keep them
+#pragma unroll
+      for (int b = 0; b < NQ; ++b)
+#pragma unroll
+        for (int st = 0; st < kStep / M::KS; ++st) {
+          FragOf<T> pf[3];
+          split_frag_of<T>(x[b], st, pf);
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            const FragOf<T> vf = L::template frag_t<kStep>(s.v, d * 16, st * M::KS);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) acc[b][d] = M::mma(vf, pf[i], acc[b][d]);
+          }
+        }
     }
   }
 #pragma unroll
@@ -392,12 +433,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_few(Args a, int parts, int64_t 
     for (int d = 0; d < DB; ++d) {
       const f32x4 v = acc[b][d] * inv;
       store4(o + at, d * 16 + 4 * g, dh, v);
-      if (rest != nullptr) {
-        f32x4 e;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = v[i] - float(T(v[i]));
-        store4(rest + at, d * 16 + 4 * g, dh, e);
-      }
+      if (rest != nullptr) store_rest(rest + at, d * 16 + 4 * g, dh, v);
     }
     if (lse != nullptr && g == 0)
       lse[item * a.rows + int64_t(row[b].i) * a.G + row[b].h] = ok[b] && l[b] > 0.f ? m[b] + __log2f(l[b]) : INFINITY;
@@ -424,6 +460,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_join(Args a, int parts, const f
   const float at = top == -INFINITY ? 0.f : top;
   float sum = 0.f, v0 = 0.f, v1 = 0.f;
   const int d = 2 * lane;
+#pragma unroll 8
   for (int k = 0; k < parts; ++k) {
     const int64_t row = (item * parts + k) * a.rows + r;
     const float2 e = pml[row];
@@ -439,8 +476,8 @@ __global__ __launch_bounds__(kBlock) void k_attn_join(Args a, int parts, const f
   if (d < dh) o[to + d] = T(v0);
   if (d + 1 < dh) o[to + d + 1] = T(v1);
   if (rest != nullptr) {
-    if (d < dh) rest[to + d] = T(v0 - float(T(v0)));
-    if (d + 1 < dh) rest[to + d + 1] = T(v1 - float(T(v1)));
+    if (d < dh) rest[to + d] = rest_of<T>(v0, T(v0));
+    if (d + 1 < dh) rest[to + d + 1] = rest_of<T>(v1, T(v1));
   }
   if (lse != nullptr && lane == 0) lse[x] = ok && sum > 0.f ? top + __log2f(sum) : INFINITY;
 }
@@ -464,7 +501,7 @@ size_t ml_bytes(const Args &a, int parts) {
   return align_up(sizeof(float2) * size_t(a.p.n * a.p.heads_kv) * size_t(parts) * size_t(a.rows));
 }
 
-template <typename T, int DP, int NQ>
+template <typename T, int DP, int NQ, bool SPLIT>
 int launch_few(const Args &a, T *o, T *rest, float *lse, void *ws, hipStream_t s) {
   const int parts = few_parts(a);
   const int64_t items = a.p.n * a.p.heads_kv, keys = parts > 0 ? few_keys(a, parts) : 0;
@@ -474,9 +511,9 @@ int launch_few(const Args &a, T *o, T *rest, float *lse, void *ws, hipStream_t s
     lds = std::max(lds, join_bytes(1, kWaves, NQ, DP));
   float2 *ml = static_cast<float2 *>(ws);
   float *acc = reinterpret_cast<float *>(static_cast<char *>(ws) + (parts > 1 ? ml_bytes(a, parts) : 0));
-  SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_few<T, DP, NQ>), lds));
+  SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_few<T, DP, NQ, SPLIT>), lds));
   const int64_t grid = parts == 0 ? (items + kWaves - 1) / kWaves : items * parts;
-  launch(&k_attn_few<T, DP, NQ>, dim3(unsigned(grid)), dim3(kBlock), lds, s, a, parts, keys, o, rest, lse, acc, ml);
+  launch(&k_attn_few<T, DP, NQ, SPLIT>, dim3(unsigned(grid)), dim3(kBlock), lds, s, a, parts, keys, o, rest, lse, acc, ml);
   if (parts > 1)
     launch(&k_attn_join<T>, dim3(unsigned((items * a.rows + kWaves - 1) / kWaves)), dim3(kBlock), 0, s, a, parts,
            static_cast<const float *>(acc), static_cast<const float2 *>(ml), o, rest, lse);
@@ -484,13 +521,13 @@ int launch_few(const Args &a, T *o, T *rest, float *lse, void *ws, hipStream_t s
   return SGL_OK;
 }
 
-template <typename T, int DP, int NQ, bool SHARE, int RW, int KW>
+template <typename T, int DP, int NQ, bool SHARE, int RW, int KW, bool SPLIT>
 int launch_fwd(const Args &a, T *o, T *rest, float *lse, hipStream_t s) {
   const int64_t tiles = row_tiles(a, NQ, SHARE, RW);
   const size_t lds = std::max(buffers<FwdLds<T, DP, tile_keys<T>(KW)>>() * sizeof(FwdLds<T, DP, tile_keys<T>(KW)>) + table_bytes(a),
                               join_bytes(RW, KW, NQ, DP));
-  SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_fwd<T, DP, NQ, SHARE, RW, KW>), lds));
-  launch(&k_attn_fwd<T, DP, NQ, SHARE, RW, KW>, dim3(unsigned(a.p.n * a.p.heads_kv * tiles)), dim3(RW * KW * kWave),
+  SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_fwd<T, DP, NQ, SHARE, RW, KW, SPLIT>), lds));
+  launch(&k_attn_fwd<T, DP, NQ, SHARE, RW, KW, SPLIT>, dim3(unsigned(a.p.n * a.p.heads_kv * tiles)), dim3(RW * KW * kWave),
          lds, s, a, tiles, o, rest, lse);
   SGL_CHECK_LAUNCH();
   return SGL_OK;
@@ -511,11 +548,21 @@ int run_forward(const Args &a, void *o, void *rest, float *lse, void *ws, hipStr
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
     T *to = static_cast<T *>(o), *tr = static_cast<T *>(rest);
-    if (a.rows <= 16) return launch_few<T, DP, 1>(a, to, tr, lse, ws, s);
-    if (a.rows <= kFewRows) return launch_few<T, DP, 2>(a, to, tr, lse, ws, s);
-    if (!many_rows(a)) return launch_fwd<T, DP, 1, false, 1, 4>(a, to, tr, lse, s);
-    if (a.G % 2 == 0) return launch_fwd<T, DP, 2, true, 4, 2>(a, to, tr, lse, s);
-    return launch_fwd<T, DP, 2, false, 4, 2>(a, to, tr, lse, s);
+    auto run = [&](auto split) -> int {
+      constexpr bool S = decltype(split)::value;
+      if (a.rows <= 16) return launch_few<T, DP, 1, S>(a, to, tr, lse, ws, s);
+      if (a.rows <= kFewRows) return launch_few<T, DP, 2, S>(a, to, tr, lse, ws, s);
+      if (!many_rows(a)) return launch_fwd<T, DP, 1, false, 1, 4, S>(a, to, tr, lse, s);
+      if constexpr (two_blocks<T, DP>()) {
+        if (a.G % 2 == 0) return launch_fwd<T, DP, 2, true, 4, 2, S>(a, to, tr, lse, s);
+        return launch_fwd<T, DP, 2, false, 4, 2, S>(a, to, tr, lse, s);
+      } else {
+        return launch_fwd<T, DP, 1, false, 4, 2, S>(a, to, tr, lse, s);
+      }
+    };
+    if constexpr (sizeof(T) == 2)
+      if (rest != nullptr) return run(std::true_type{});
+    return run(std::false_type{});
   });
 }
 

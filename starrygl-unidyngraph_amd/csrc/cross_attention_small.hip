@@ -15,7 +15,7 @@ namespace attn {
 namespace {
 
 template <typename T, int DP, int NQ, int NK>
-struct SmallLds {
+struct alignas(16) SmallLds {
   static constexpr int R = 16 * NQ, K = 16 * NK;
   static constexpr int kKeyTile = K * Tile<T, DP>::LD, kProbTile = R * Tile<T, K>::LD;
   // k, then p and ds in its place; do, then q in its place
@@ -27,11 +27,11 @@ struct SmallLds {
 template <typename Lds>
 __host__ __device__ __forceinline__ size_t small_lds(const Args &a, int nq, bool cells) {   // bytes a wave
   return align_bytes(sizeof(Lds) + table_bytes(a)) +
-         (cells ? sizeof(Cell) * size_t(16 % a.G == 0 ? 1 : nq) * 16 * a.cols : 0);
+         (cells ? sizeof(Cell) * size_t(16 % a.G == 0 ? 1 : nq) * cell_slots(a.G) * a.cols : 0);
 }
 
 template <typename T, int DP, int NQ, int NK>
-__global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each, const T *__restrict__ go,
+__global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(Args a, int64_t each, const T *__restrict__ go,
                                                            T *__restrict__ dq, T *__restrict__ dk,
                                                            T *__restrict__ dv, float *__restrict__ part) {
   using M = Mma<T>;
@@ -42,12 +42,12 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
   extern __shared__ __align__(16) char smem[];
   const sgl_attention &p = a.p;
   const int dh = p.head_dim;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
+  const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4, cl = lane & 15;
   const size_t per = small_lds<Lds>(a, NQ, part != nullptr);
   Lds &s = *reinterpret_cast<Lds *>(smem + w * per);
   float *table = reinterpret_cast<float *>(smem + w * per + sizeof(Lds));
   Cell *cells = reinterpret_cast<Cell *>(smem + w * per + align_bytes(sizeof(Lds) + table_bytes(a)));
-  const int sets = 16 % a.G == 0 ? 1 : NQ;   // (one: row c of either block has the same head)
+  const int sets = 16 % a.G == 0 ? 1 : NQ, slots = cell_slots(a.G);   // (one set: row c of either block has the same head)
   const TileAt at_ = tile_at(blockIdx.x * (blockDim.x / kWave) + w, 1, p.heads_kv);
   const int hk = at_.hk;
   const int64_t first = at_.n;
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
   const bool biased = p.bias != nullptr;
   const Buckets bk = buckets_of(p);
   if (biased) stage_bias(table, a, hk, lane, kWave);
-  if (part != nullptr) clear_cells(cells, sets * 16 * a.cols, lane, kWave);
+  if (part != nullptr) clear_cells(cells, sets * slots * a.cols, lane, kWave);
   float up = 0.f, seen = 0.f;   // the cells' power of two (0: nothing in them yet)
   wave_sync();
   RowAt row[NQ];
@@ -64,15 +64,27 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
   const float c = p.scale * kLog2e;
   for (int64_t n = first; n < p.n; n += each) {
     const Seq<T> q = seq_of<T>(p, n, hk, a.G);
-    const int64_t base = biased && q.qlen > 0 ? q.qpos[0] : 0;
-    const bool on_key = lane < K && q.qlen > 0 && key_live(q, p, lane);
-    const uint64_t live = __ballot(on_key);
-    int64_t kp = base;
-    if (biased && on_key) kp = q.kpos[lane * p.kpos_t];
+    const int64_t base = biased && q.qlen > 0 ? scalar_load(q.qpos) : 0;
+    // every load of the item is issued before anything is looked at
+    const bool in_key = lane < K && q.qlen > 0 && lane < q.klen;
+    int64_t kpos = 0;
+    int byte = 0;
+    if (biased && in_key) kpos = q.kpos[lane * p.kpos_t];
+    if (q.mask != nullptr && in_key) byte = q.mask[lane * p.mask_t];
+    FragOf<T> kf[NK][ST], vf[NK][ST];
+#pragma unroll
+    for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const int d = st * M::KS + g * M::E;
+        const int64_t j = kb * 16 + cl;
+        kf[kb][st] = load_raw<T>(q.k + j * p.k_t, q.qlen > 0 && j < q.klen, d, dh);
+        vf[kb][st] = load_raw<T>(q.v + j * p.v_t, q.qlen > 0 && j < q.klen, d, dh);
+      }
     FragOf<T> qf[NQ][ST], gf[NQ][ST];
     int64_t qpos[NQ];
     int qrel[NQ];
-    bool near_ = is_near(kp - base), ok[NQ];
+    bool ok[NQ];
     float most = 0.f;
 #pragma unroll
     for (int b = 0; b < NQ; ++b) {
@@ -84,7 +96,16 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
         qf[b][st] = load_raw<T>(q.q + int64_t(row[b].i) * p.q_t + row[b].h * p.q_h, ok[b], d, dh);
         gf[b][st] = load_raw<T>(go + at, ok[b], d, dh);
       }
-      qpos[b] = biased && ok[b] ? q.qpos[int64_t(row[b].i) * p.qpos_t] : base;
+      qpos[b] = 0;
+      if (biased && ok[b]) qpos[b] = q.qpos[int64_t(row[b].i) * p.qpos_t];
+    }
+    uint64_t live = q.qlen > 0 ? first_bits(q.klen) : 0;
+    if (q.mask != nullptr) live = __ballot(byte != 0);
+    const int64_t kp = lane < K && ((live >> lane) & 1) ? kpos : base;
+    bool near_ = is_near(kp - base);
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) {
+      if (!ok[b]) qpos[b] = base;
       near_ = near_ && is_near(qpos[b] - base);
       qrel[b] = int(qpos[b] - base);
     }
@@ -118,7 +139,8 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
         up = want;
       } else if (want < up) {
         const int by = min(ilogbf(up) - ilogbf(want), 63);
-        for (int i = lane; i < sets * 16 * a.cols; i += kWave) cells[i] = Cell(static_cast<long long>(cells[i]) >> by);
+        for (int i = lane; i < sets * slots * a.cols; i += kWave)
+          cells[i] = Cell(static_cast<long long>(cells[i]) >> by);
         seen = ldexpf(seen, -by);
         up = want;
         wave_sync();
@@ -133,29 +155,22 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
     }
 #pragma unroll
     for (int kb = 0; kb < NK; ++kb) {
-      FragOf<T> kf[ST], vf[ST];
       const bool on_r = (live >> (kb * 16 + cl)) & 1;
-      const int64_t j = kb * 16 + cl;
 #pragma unroll
       for (int st = 0; st < ST; ++st) {
         const int d = st * M::KS + g * M::E;
-        kf[st] = load_raw<T>(q.k + j * p.k_t, on_r, d, dh);
-        vf[st] = load_raw<T>(q.v + j * p.v_t, on_r, d, dh);
-      }
-#pragma unroll
-      for (int st = 0; st < ST; ++st) {
-        const int d = st * M::KS + g * M::E;
-        kf[st] = fix<T>(kf[st], d, dh);
-        vf[st] = fix<T>(vf[st], d, dh);
-        *reinterpret_cast<FragOf<T> *>(s.a + (kb * 16 + cl) * L::LD + d) = kf[st];
+        kf[kb][st] = fix<T>(kf[kb][st], d, dh);
+        vf[kb][st] = fix<T>(vf[kb][st], d, dh);
+        if (q.mask != nullptr && !on_r) kf[kb][st] = vf[kb][st] = zero_frag<T>();
+        *reinterpret_cast<FragOf<T> *>(s.a + (kb * 16 + cl) * L::LD + d) = kf[kb][st];
       }
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {
         f32x4 sc = {0.f, 0.f, 0.f, 0.f}, dp = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int st = 0; st < ST; ++st) {
-          sc = M::mma(kf[st], qf[b][st], sc);
-          dp = M::mma(vf[st], gf[b][st], dp);
+          sc = M::mma(kf[kb][st], qf[b][st], sc);
+          dp = M::mma(vf[kb][st], gf[b][st], dp);
         }
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
@@ -199,7 +214,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
       for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
         for (int v = 0; v < 4; ++v) y[b][kb][v] = x[b][kb][v] * (y[b][kb][v] - de);
-      if (part != nullptr) add_cells(cells + (sets == 1 ? 0 : b) * 16 * a.cols, col[b], y[b], up, seen);
+      if (part != nullptr) add_cells(cells + (sets == 1 ? 0 : b) * slots * a.cols, col[b], y[b], slots, up, seen);
       if constexpr (std::is_same_v<T, fp16_t>) {
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb)
@@ -300,10 +315,11 @@ __global__ __launch_bounds__(kBlock) void k_attn_small_bwd(Args a, int64_t each,
     for (int x = lane; x < a.G * a.cols; x += kWave) {
       const int h = x / a.cols, cidx = x - h * a.cols;
       long long t = 0;
-      for (int r = 0; r < sets * 16; ++r) {
-        const int e = (r & ~15) | ((r + cidx) & 15);
-        if (e % a.G == h) t += static_cast<long long>(cells[((e >> 4) * a.cols + cidx) * 16 + (e & 15)]);
-      }
+      for (int set = 0; set < sets; ++set)
+        for (int i = 0; i < slots; ++i) {
+          const int e = (i + cidx) & (slots - 1);
+          if ((set * 16 + e) % a.G == h) t += static_cast<long long>(cells[(set * a.cols + cidx) * slots + e]);
+        }
       out[x] = held ? float(double(t) * (1.0 / double(1ll << kCellBits)) / double(up == 0.f ? 1.f : up)) : NAN;
     }
   }
