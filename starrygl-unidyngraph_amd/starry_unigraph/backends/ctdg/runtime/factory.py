@@ -51,7 +51,7 @@ def build_ctdg_runtime(session_ctx: SessionContext, events=None) -> tuple[CTDGOn
     memory = CTDGMemoryBank(num_nodes=dataset.num_nodes, hidden_dim=hidden_dim, device=device,
                             mailbox_slots=mailbox_slots, edge_feat_dim=edge_feat_dim)
     embedding = str(c.get("embedding", "attention"))
-    shift, scale = dataset.inter_event_stats("train") if embedding == "time_projection" else (0.0, 1.0)
+    shift, scale = dataset.inter_event_stats("train") if embedding in ("time_projection", "history") else (0.0, 1.0)
     model = build_ctdg_model(str(cfg["model"]["family"]), num_nodes=dataset.num_nodes, hidden_dim=hidden_dim,
                              edge_feat_dim=edge_feat_dim, dim_time=dim_time, num_head=num_head, dropout=dropout,
                              att_dropout=att_dropout, embedding=embedding, time_shift=shift,

@@ -26,8 +26,8 @@ import torch.nn.functional as F
 from torch import nn
 
 from starry_unigraph.lib import _capi
-from starry_unigraph.native.step import ConvFunction, DeviceStep
-from starry_unigraph.runtime.modules import TimeEncode
+from starry_unigraph.native.step import ConvDims, ConvFunction, DeviceStep
+from starry_unigraph.runtime.modules import HistoryEncoder, TimeEncode
 
 
 class TemporalTransformerConv(nn.Module):
@@ -266,6 +266,38 @@ class CTDGTimeProjectionPredictor(nn.Module):
         return CTDGModelOutput(pos_logits=pos_logits, neg_logits=neg_logits)
 
 
+class CTDGHistoryPredictor(CTDGLinkPredictor):
+    """Link prediction on the roots' windows read as sequences
+    (HistoryEncoder), then the same edge predictor (models.py:313-324). The
+    reference has no such embedding; select it with ctdg.embedding = history.
+    It trains through autograd (no launch plans), in fp32."""
+
+    def __init__(self, num_nodes: int, hidden_dim: int, edge_feat_dim: int, num_head: int = 2,
+                 mean_gap: float = 1.0) -> None:
+        nn.Module.__init__(self)
+        self.hidden_dim = hidden_dim
+        self.conv = None
+        self.history = HistoryEncoder(hidden_dim, hidden_dim + edge_feat_dim, num_head, mean_gap=mean_gap)
+        self.src_fc = nn.Linear(hidden_dim, hidden_dim)
+        self.dst_fc = nn.Linear(hidden_dim, hidden_dim)
+        self.out_fc = nn.Linear(hidden_dim, 1)
+
+    def embedding_module(self) -> nn.Module:
+        return self.history
+
+    def roots(self, step: DeviceStep, dims: ConvDims) -> torch.Tensor:
+        """Embeddings [cap + 1, D] of a step's roots from its edge rows and
+        updated memory; zero past the live roots."""
+        b, K, W = step.buf, dims.fanout, dims.D + dims.F
+        live = torch.arange(b.cap, device=step.dev) < b.num_roots
+        cnt = torch.where(live, b.hop.cnt, 0)
+        events = b.X.view(-1, dims.C)[:b.cap * K].view(b.cap, K, dims.C)[..., :W]
+        inside = torch.arange(K, device=step.dev) < cnt.unsqueeze(1)
+        # (rows past a count hold an earlier step's events: the products over them have zero gradients)
+        y = self.history(b.new_mem[:b.cap], events, cnt, torch.where(inside, b.hop.dt[:b.cap * K].view(b.cap, K), 0.0))
+        return F.pad(torch.where(live.unsqueeze(1), y, 0.0), (0, 0, 0, 1))
+
+
 @dataclass(frozen=True)
 class CTDGModelSpec:
     model_cls: type[nn.Module]
@@ -282,7 +314,8 @@ def build_ctdg_model(model_family: str, *, num_nodes: int, hidden_dim: int, edge
                      embedding: str = "attention", time_shift: float = 0.0, time_scale: float = 1.0,
                      attention_gemm_dtype: str = "fp32") -> nn.Module:
     """models.py:345-386. ``embedding`` "attention" (the reference's model for
-    every family) or "time_projection" (config 2's JODIE embedding);
+    every family), "time_projection" (config 2's JODIE embedding) or "history"
+    (the window as a sequence; ``time_shift`` is its mean gap);
     ``attention_gemm_dtype`` "bf16": the attention and edge-predictor products
     on bf16 weight copies (benchmark configurations 4 and 5)."""
     spec = CTDG_MODEL_SPECS.get(model_family.lower())
@@ -291,8 +324,13 @@ def build_ctdg_model(model_family: str, *, num_nodes: int, hidden_dim: int, edge
     if embedding == "time_projection":
         return CTDGTimeProjectionPredictor(num_nodes=num_nodes, hidden_dim=hidden_dim, time_shift=time_shift,
                                            time_scale=time_scale)
+    if embedding == "history":
+        if attention_gemm_dtype != "fp32":
+            raise ValueError("ctdg.attention_gemm_dtype: the history embedding runs in fp32")
+        return CTDGHistoryPredictor(num_nodes=num_nodes, hidden_dim=hidden_dim, edge_feat_dim=edge_feat_dim,
+                                    num_head=num_head, mean_gap=time_shift)
     if embedding != "attention":
-        raise KeyError(f"unknown ctdg.embedding {embedding!r}: expected 'attention' or 'time_projection'")
+        raise KeyError(f"unknown ctdg.embedding {embedding!r}: expected 'attention', 'history' or 'time_projection'")
     model = spec.model_cls(num_nodes=num_nodes, hidden_dim=hidden_dim, edge_feat_dim=edge_feat_dim,
                            dim_time=dim_time, num_head=num_head, dropout=dropout, att_dropout=att_dropout)
     if getattr(model, "conv", None) is not None:

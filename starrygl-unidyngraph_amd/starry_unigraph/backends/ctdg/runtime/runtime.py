@@ -103,8 +103,11 @@ class CTDGOnlineRuntime:
         fan = int(sampler.fanout[0]) if sampler.fanout else 0
         # the time-projection model (config 2's JODIE) has no attention: its
         # back part is the projection, the predictor and their backward
-        self._proj = conv is None
-        if self._proj:
+        self._hist = getattr(core, "history", None) is not None
+        self._proj = conv is None and not self._hist
+        if self._hist:   # (its back part runs through autograd: no launch plans)
+            self.dims = ConvDims(D=memory.hidden_dim, F=max(1, dataset.edge_feat_dim), T=1, H=1, fanout=fan)
+        elif self._proj:
             if memory_updater is None:
                 raise ValueError("the time-projection embedding needs the memory updater (it embeds updated memory)")
             self.dims = ConvDims(D=memory.hidden_dim, F=max(1, dataset.edge_feat_dim), T=1, H=1, fanout=fan)
@@ -435,7 +438,7 @@ class CTDGOnlineRuntime:
         b = step.buf
         start = batch.start
         with_metrics = self.device_metrics and 0 < 2 * n <= _capi.SGL_LINK_METRICS_MAX_SCORES
-        planned = self.use_plans and n == b.max_batch and start >= 0 and step.timer is None
+        planned = self.use_plans and not self._hist and n == b.max_batch and start >= 0 and step.timer is None
         # metrics at the end of the back part, or deferred to the next front part on these buffers
         defer = planned and not self.collect_results
         if not defer:
@@ -569,7 +572,7 @@ class CTDGOnlineRuntime:
         that the step's fused update reads."""
         if not self._proj:
             step.edge_rows(self._dev["edge_feat"])
-        if train:
+        if train and not self._hist:
             self._param_update(step).advance()
 
     def _back_body(self, step: DeviceStep, train: bool, n: int) -> None:
@@ -577,6 +580,10 @@ class CTDGOnlineRuntime:
         backward and the fused weight-gradient + Adam update."""
         core = self._core()
         conv = core.conv
+        if self._hist:
+            self._history_back(step, train, n)
+            self._metrics_op(step, n)
+            return
         efeat_all = self._dev["edge_feat"]
         pparams = [core.src_fc.weight, core.src_fc.bias, core.dst_fc.weight, core.dst_fc.bias, core.out_fc.weight,
                    core.out_fc.bias]
@@ -609,6 +616,25 @@ class CTDGOnlineRuntime:
             step.conv_backward_kernel(cparams, efeat_all, pred_w=(pdet[0], pdet[2]), drop=drop)
             upd.run()
         self._metrics_op(step, n)
+
+    def _history_back(self, step: DeviceStep, train: bool, n: int) -> None:
+        """The back part of the history embedding: embeddings, edge predictor
+        and BCE (runtime.py:197-199) and, in training, autograd's backward
+        into the optimizer's flat gradients and its step."""
+        b = step.buf
+        core = self._core()
+        with torch.set_grad_enabled(train):
+            y = core.roots(step, self.dims)
+            out = core(y[b.ridx_src[:n]], y[b.ridx_dst[:n]], y[b.ridx_neg[:n]])
+            # BCE of 1 and 0 on the logits
+            loss = F.softplus(-out.pos_logits).mean() + F.softplus(out.neg_logits).mean()
+        if train:
+            self.optimizer.zero_grad()
+            loss.backward()
+            self.optimizer.step()
+        b.pos[:n].copy_(out.pos_logits.detach())
+        b.neg[:n].copy_(out.neg_logits.detach())
+        b.loss.copy_(loss.detach())
 
     def _metrics_op(self, step: DeviceStep, n: int) -> None:
         """The step's metrics into the next ring slot as the last op of its

@@ -1,3 +1,4 @@
+from .history import HistoryEncoder
 from .time_encode import TimeEncode
 
-__all__ = ["TimeEncode"]
+__all__ = ["HistoryEncoder", "TimeEncode"]
