@@ -63,20 +63,23 @@ struct Row {
   static constexpr int RPB = LPR > kWave ? 1 : 256 / LPR;   // rows of a workgroup at a time
   static constexpr int BLOCK = LPR > kWave ? LPR : 256;
 
-  static __device__ __forceinline__ void load(float (&r)[E], const T *p, int lane, int D) {
+  struct Raw {   // as loaded (the next row's, in flight)
+    T t[NV][V];
+  };
+  static __device__ __forceinline__ void load(Raw &r, const T *p, int lane, int D) {   // (NULL reads as 0)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * LPR + lane) * V;
-      T t[V];
-      if (c < D) {
-        sgl::load_n(t, p + c);
-      } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) t[j] = T(0.f);
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) r[i * V + j] = float(t[j]);
+      for (int j = 0; j < V; ++j) r.t[i][j] = T(0.f);
+      if (p != nullptr && c < D) sgl::load_n(r.t[i], p + c);
     }
+  }
+  static __device__ __forceinline__ void widen(float (&r)[E], const Raw &x) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) r[i * V + j] = float(x.t[i][j]);
   }
   static __device__ __forceinline__ void store(T *p, const float (&r)[E], int lane, int D) {
 #pragma unroll
@@ -152,11 +155,21 @@ __global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK)) void k_norm_fwd(NormAr
   R::weight(pb, a.post_b, 0.f, lane, a.D);
   R::weight(nw, a.pre_w, 1.f, lane, a.D);
   R::weight(nb, a.pre_b, 0.f, lane, a.D);
-  for (int64_t r = int64_t(blockIdx.x) * R::RPB + threadIdx.x / LPR; r < a.rows; r += int64_t(gridDim.x) * R::RPB) {
+  const int64_t step = int64_t(gridDim.x) * R::RPB;
+  typename R::Raw rx, rz, rg;
+  auto fetch = [&](int64_t r) {
+    R::load(rz, static_cast<const T *>(a.z) + r * a.sz, lane, a.D);
+    R::load(rx, static_cast<const T *>(a.x) + r * a.sx, lane, a.D);
+    R::load(rg, static_cast<const T *>(a.gate) + r * a.sg, lane, a.D);
+  };
+  int64_t r = int64_t(blockIdx.x) * R::RPB + threadIdx.x / LPR;
+  if (r < a.rows) fetch(r);
+  for (; r < a.rows; r += step) {
     float x[E], z[E], g[E];
-    R::load(z, static_cast<const T *>(a.z) + r * a.sz, lane, a.D);
-    R::load(x, static_cast<const T *>(a.x) + r * a.sx, lane, a.D);
-    R::load(g, static_cast<const T *>(a.gate) + r * a.sg, lane, a.D);
+    R::widen(z, rz);
+    R::widen(x, rx);
+    R::widen(g, rg);
+    if (r + step < a.rows) fetch(r + step);
     R::standard(z, lane, a.D, inv, a.eps, a.rms, s_red, slot);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -174,45 +187,48 @@ __global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK)) void k_norm_fwd(NormAr
 
 // part: this workgroup's sums, [5][D]: scale, post weight, pre weight, post
 // bias, pre bias (the biases' rows only with biases).
-template <typename T, int V, int NV, int LPR>
-__global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK)) void k_norm_bwd(NormArgs a, const T *__restrict__ gy,
+template <typename T, int V, int NV, int LPR, bool BIAS>
+__global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK), (LPR <= 256 && V * NV == 8 && !BIAS ? 3 : 1)) void k_norm_bwd(NormArgs a, const T *__restrict__ gy,
                                                                           const T *__restrict__ gn,
                                                                           T *__restrict__ dx, T *__restrict__ dz,
                                                                           T *__restrict__ dgate,
-                                                                          float *__restrict__ part, int nsum) {
+                                                                          float *__restrict__ part) {
   using R = Row<T, V, NV, LPR>;
   constexpr int E = R::E;
   __shared__ float s_red[LPR > 64 ? 2 * LPR / 64 : 1];
   int slot = 0;
   const int lane = threadIdx.x % LPR;
   const float inv = 1.f / float(a.D);
+  constexpr int NS = BIAS ? 5 : 3;   // sums kept
   float al[E], pw[E], pb[E], nw[E];
   R::weight(al, a.scale, 0.f, lane, a.D);
   R::weight(pw, a.post_w, 1.f, lane, a.D);
-  R::weight(pb, a.post_b, 0.f, lane, a.D);
+  R::weight(pb, BIAS ? a.post_b : nullptr, 0.f, lane, a.D);
   R::weight(nw, a.pre_w, 1.f, lane, a.D);
-  float sums[5][E];
+  float sums[NS][E];
 #pragma unroll
-  for (int k = 0; k < 5; ++k)
+  for (int k = 0; k < NS; ++k)
 #pragma unroll
     for (int e = 0; e < E; ++e) sums[k][e] = 0.f;
-  for (int64_t r = int64_t(blockIdx.x) * R::RPB + threadIdx.x / LPR; r < a.rows; r += int64_t(gridDim.x) * R::RPB) {
+  const int64_t step = int64_t(gridDim.x) * R::RPB;
+  typename R::Raw rx, rz, rg, ru, rq;
+  auto fetch = [&](int64_t r) {
+    R::load(rx, static_cast<const T *>(a.x) + r * a.sx, lane, a.D);
+    R::load(rz, static_cast<const T *>(a.z) + r * a.sz, lane, a.D);
+    R::load(rg, static_cast<const T *>(a.gate) + r * a.sg, lane, a.D);
+    R::load(ru, gn != nullptr ? gn + r * a.D : nullptr, lane, a.D);
+    R::load(rq, gy != nullptr ? gy + r * a.D : nullptr, lane, a.D);
+  };
+  int64_t r = int64_t(blockIdx.x) * R::RPB + threadIdx.x / LPR;
+  if (r < a.rows) fetch(r);
+  for (; r < a.rows; r += step) {
     float x[E], z[E], g[E], q[E], u[E];
-    R::load(x, static_cast<const T *>(a.x) + r * a.sx, lane, a.D);
-    R::load(z, static_cast<const T *>(a.z) + r * a.sz, lane, a.D);
-    R::load(g, static_cast<const T *>(a.gate) + r * a.sg, lane, a.D);
-    if (gn != nullptr) {
-      R::load(u, gn + r * a.D, lane, a.D);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) u[e] = 0.f;
-    }
-    if (gy != nullptr) {
-      R::load(q, gy + r * a.D, lane, a.D);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) q[e] = 0.f;
-    }
+    R::widen(x, rx);
+    R::widen(z, rz);
+    R::widen(g, rg);
+    R::widen(u, ru);
+    R::widen(q, rq);
+    if (r + step < a.rows) fetch(r + step);
     // y again
     const float zr = R::standard(z, lane, a.D, inv, a.eps, a.rms, s_red, slot);
 #pragma unroll
@@ -226,7 +242,7 @@ __global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK)) void k_norm_bwd(NormAr
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       sums[2][e] += u[e] * x[e];
-      sums[4][e] += u[e];
+      if constexpr (BIAS) sums[4][e] += u[e];
       u[e] *= nw[e];
     }
     R::through(u, x, yr, inv, a.rms, s_red, slot);
@@ -243,7 +259,7 @@ __global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK)) void k_norm_bwd(NormAr
       const float dpost = qs * al[e];
       g[e] = dpost * post * sn;
       sums[1][e] += dpost * z[e];
-      sums[3][e] += dpost;
+      if constexpr (BIAS) sums[3][e] += dpost;
       u[e] = dpost * pw[e];
     }
     R::store(dgate + r * a.D, g, lane, a.D);
@@ -254,8 +270,7 @@ __global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK)) void k_norm_bwd(NormAr
   if constexpr (R::RPB > 1) {
     __shared__ float s_sum[R::RPB * LPR * E];
 #pragma unroll
-    for (int k = 0; k < 5; ++k) {
-      if (k >= nsum) break;
+    for (int k = 0; k < NS; ++k) {
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < E; ++e) s_sum[(threadIdx.x / LPR) * (LPR * E) + e * LPR + lane] = sums[k][e];
@@ -265,28 +280,34 @@ __global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK)) void k_norm_bwd(NormAr
 #pragma unroll
         for (int g = 0; g < R::RPB; ++g) t += s_sum[g * (LPR * E) + c];
         const int e = c / LPR, col = ((e / V) * LPR + c % LPR) * V + e % V;
-        if (col < a.D) part[(int64_t(blockIdx.x) * nsum + k) * a.D + col] = t;
+        if (col < a.D) part[(int64_t(blockIdx.x) * NS + k) * a.D + col] = t;
       }
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < 5; ++k) {
-      if (k >= nsum) break;
+    for (int k = 0; k < NS; ++k) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const int c = (i * LPR + lane) * V + j;
-          if (c < a.D) part[(int64_t(blockIdx.x) * nsum + k) * a.D + c] = sums[k][i * V + j];
+          if (c < a.D) part[(int64_t(blockIdx.x) * NS + k) * a.D + c] = sums[k][i * V + j];
         }
     }
   }
 }
 
-constexpr unsigned kFwdGrid = 1536, kBwdGrid = 1024;
+constexpr unsigned kBwdGrid = 1024;   // most rows of partial sums
 
-unsigned norm_grid(int64_t rows, int rpb, unsigned most) {
-  return unsigned(std::max<int64_t>(1, std::min<int64_t>((rows + rpb - 1) / rpb, most)));
+// As many workgroups as are resident at once (each walks rows at that stride):
+// with more of them the last ones run alone (131073 rows of 512 in fp16: a
+// grid of 1.5 times that takes 142 and 249 us, this one 128 and 207).
+template <typename K>
+unsigned norm_grid(K kernel, int block, int64_t rows, int rpb, unsigned most) {
+  constexpr int kCUs = 256;
+  int each = 0;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, block, 0) != hipSuccess || each < 1) each = 2;
+  return unsigned(std::max<int64_t>(1, std::min<int64_t>({(rows + rpb - 1) / rpb, int64_t(most), int64_t(each) * kCUs})));
 }
 
 template <typename T, int V, int NV, int LPR>
@@ -294,14 +315,15 @@ int run_norm(const NormArgs &a, const void *gy, const void *gn, void *o1, void *
              bool back, hipStream_t s) {
   using R = Row<T, V, NV, LPR>;
   if (!back) {
-    sgl::launch(&k_norm_fwd<T, V, NV, LPR>, dim3(norm_grid(a.rows, R::RPB, kFwdGrid)), dim3(R::BLOCK), 0, s, a,
-                static_cast<T *>(o1), static_cast<T *>(o2));
+    const unsigned most = norm_grid(&k_norm_fwd<T, V, NV, LPR>, R::BLOCK, a.rows, R::RPB, UINT_MAX);
+    sgl::launch(&k_norm_fwd<T, V, NV, LPR>, dim3(most), dim3(R::BLOCK), 0, s, a, static_cast<T *>(o1),
+                static_cast<T *>(o2));
     return 0;
   }
-  const unsigned grid = norm_grid(a.rows, R::RPB, kBwdGrid);
-  sgl::launch(&k_norm_bwd<T, V, NV, LPR>, dim3(grid), dim3(R::BLOCK), 0, s, a, static_cast<const T *>(gy),
-              static_cast<const T *>(gn), static_cast<T *>(o1), static_cast<T *>(o2), static_cast<T *>(o3), part,
-              nsum);
+  const auto kernel = nsum == 5 ? &k_norm_bwd<T, V, NV, LPR, true> : &k_norm_bwd<T, V, NV, LPR, false>;
+  const unsigned grid = norm_grid(kernel, R::BLOCK, a.rows, R::RPB, kBwdGrid);
+  sgl::launch(kernel, dim3(grid), dim3(R::BLOCK), 0, s, a, static_cast<const T *>(gy), static_cast<const T *>(gn),
+              static_cast<T *>(o1), static_cast<T *>(o2), static_cast<T *>(o3), part);
   return int(grid);
 }
 

@@ -32,7 +32,7 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kKeep = 8;             // steps between kept states
 constexpr int64_t kFill = 1 << 18;   // threads that fill the GPU: 16 waves a CU
-constexpr int64_t kPieces = kFill + kFill / 4;   // pieces x channel groups: the 5 waves a SIMD of the backward, once
+constexpr int64_t kPieces = 2 * kFill;   // pieces x channel groups: two rounds of the backward (4 x 8191 x 256 in bf16: 160 us; 1.25 kFill 170, 0.75 183)
 constexpr int kSubs = 8;             // pieces a workgroup of the cut form: kLanes channel groups each
 constexpr int kLanes = kBlock / kSubs;
 constexpr int kMaxSupers = 32;
@@ -127,6 +127,17 @@ __device__ __forceinline__ void compose(float (&s)[V], const float2 *__restrict_
   for (int j = 0; j < V; ++j) s[j] = c[j].x * s[j] + c[j].y;
 }
 
+// The address of one step after another: a pointer moved by a stride, or left
+// (a step past the last one reads that again). A product a step of 64 bits cost
+// more than the step's own arithmetic.
+template <typename T>
+struct Steps {
+  const T *p;
+  int64_t by;
+  __device__ __forceinline__ Steps(const T *base, int64_t t, int64_t stride) : p(base + t * stride), by(stride) {}
+  __device__ __forceinline__ void next(bool go) { p += go ? by : 0; }
+};
+
 // The compositions of the pieces: forward (A = prod a, B = the state a piece
 // ends in from 0), or backward (B = a_0 lam_0 of the piece from nothing after
 // it), combined over the pieces before it (forward) or after it (backward) in
@@ -145,25 +156,29 @@ __global__ __launch_bounds__(kBlock) void k_scan_pieces(ScanArgs a, const T *__r
   if (u.ok) {
     const int64_t t0 = u.t0, t1 = min(u.t1, seq_len(a, u.n));
     const T *gate = static_cast<const T *>(a.gate) + u.n * a.gate_n + u.d;
-    const T *src = BACK ? gh + u.n * a.L * a.D + u.d : static_cast<const T *>(a.value) + u.n * a.value_n + u.d;
+    const T *src = BACK ? (gh != nullptr ? gh + u.n * a.L * a.D + u.d : nullptr) : static_cast<const T *>(a.value) + u.n * a.value_n + u.d;
     const int64_t src_t = BACK ? a.D : a.value_t;
     constexpr int U = 8;
+    Steps<T> pf(gate, t0, a.gate_t), px(src, t0, src_t);
+    Steps<float> pg(DECAY ? a.gaps + u.n * a.gaps_n : nullptr, t0, a.gaps_t);
     for (int64_t t = t0; t < t1; t += U) {
       T f[U][V], x[U][V];
       float gap[U];
       const int m = int(min(int64_t(U), t1 - t));
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        const int64_t at = BACK ? t1 - 1 - (t - t0) - min(k, m - 1) : t + min(k, m - 1);
-        sgl::load_n(f[k], gate + at * a.gate_t);
-        if (BACK && gh == nullptr) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) x[k][j] = T(0.f);
-        } else {
-          sgl::load_n(x[k], src + at * src_t);
-        }
-        gap[k] = DECAY ? a.gaps[u.n * a.gaps_n + at * a.gaps_t] : 0.f;
+        for (int j = 0; j < V; ++j) x[k][j] = T(0.f);
+        sgl::load_n(f[k], pf.p);
+        if (!BACK || gh != nullptr) sgl::load_n(x[k], px.p);
+        gap[k] = DECAY ? *pg.p : 0.f;
+        pf.next(k + 1 < m);
+        if (!BACK || gh != nullptr) px.next(k + 1 < m);
+        if (DECAY) pg.next(k + 1 < m);
       }
+      pf.next(m == U);   // (a last short group is not followed)
+      if (!BACK || gh != nullptr) px.next(m == U);
+      if (DECAY) pg.next(m == U);
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         if (k < m) {
@@ -172,7 +187,8 @@ __global__ __launch_bounds__(kBlock) void k_scan_pieces(ScanArgs a, const T *__r
             float ga, gb, sn;
             step_gate<DECAY>(float(f[k][j]), dec[j] * gap[k], ga, gb, sn);
             A[j] *= ga;
-            B[j] = BACK ? ga * (float(x[k][j]) + B[j]) : ga * B[j] + gb * float(x[k][j]);
+            // (backward too in the order of the steps: a step's gradient goes through every a before it)
+            B[j] = BACK ? B[j] + A[j] * float(x[k][j]) : ga * B[j] + gb * float(x[k][j]);
           }
         }
       }
@@ -234,6 +250,8 @@ __global__ __launch_bounds__(kBlock) void k_scan_fwd(ScanArgs a, T *__restrict__
   }
   constexpr int U = 8;
   static_assert(kKeep % U == 0, "kept states fall on the first step of a group");
+  Steps<T> pf(gate, t0, a.gate_t), px(value, t0, a.value_t);
+  Steps<float> pg(DECAY ? a.gaps + u.n * a.gaps_n : nullptr, t0, a.gaps_t);
   for (int64_t t = t0; t < t1; t += U) {
     if (t < live) {
       if (keep != nullptr && t % kKeep == 0) sgl::store_n(keep + (u.n * keeps + t / kKeep) * a.D + u.d, s);
@@ -242,11 +260,16 @@ __global__ __launch_bounds__(kBlock) void k_scan_fwd(ScanArgs a, T *__restrict__
       const int m = int(min(int64_t(U), live - t));
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        const int64_t at = t + min(k, m - 1);
-        sgl::load_n(f[k], gate + at * a.gate_t);
-        sgl::load_n(x[k], value + at * a.value_t);
-        gap[k] = DECAY ? a.gaps[u.n * a.gaps_n + at * a.gaps_t] : 0.f;
+        sgl::load_n(f[k], pf.p);
+        sgl::load_n(x[k], px.p);
+        gap[k] = DECAY ? *pg.p : 0.f;
+        pf.next(k + 1 < m);
+        px.next(k + 1 < m);
+        if (DECAY) pg.next(k + 1 < m);
       }
+      pf.next(m == U);   // (a last short group is not followed)
+      px.next(m == U);
+      if (DECAY) pg.next(m == U);
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         if (t + k < t1) {
@@ -294,28 +317,36 @@ __device__ __forceinline__ void walk_back(const ScanArgs &a, const Unit &u, int6
     sgl::store_n(dvalue + row0 + t * a.D, zero);
   }
   if (live <= t0) return;
-  for (int64_t b = (live - 1) / kKeep * kKeep; b >= t0; b -= kKeep) {
-    T f[kKeep][V], x[kKeep][V], gr[kKeep][V];
-    float gap[kKeep], s[V];
-    const int m = int(min(int64_t(kKeep), live - b));
+  // a block as loaded: the one before it is in flight while one is walked
+  T f[kKeep][V], x[kKeep][V], gr[kKeep][V];
+  float gap[kKeep], s[V];
+  auto fetch = [&](int64_t b, int m) {
+    Steps<T> pf(gate, b, a.gate_t), px(value, b, a.value_t), ph(gh != nullptr ? gh + row0 : nullptr, b, a.D);
+    Steps<float> pg(DECAY ? a.gaps + u.n * a.gaps_n : nullptr, b, a.gaps_t);
     sgl::load_n(s, keep + (u.n * keeps + b / kKeep) * a.D + u.d);
 #pragma unroll
     for (int k = 0; k < kKeep; ++k) {
-      const int64_t at = b + min(k, m - 1);
-      sgl::load_n(f[k], gate + at * a.gate_t);
-      sgl::load_n(x[k], value + at * a.value_t);
-      if (gh != nullptr) {
-        sgl::load_n(gr[k], gh + row0 + at * a.D);
-      } else {
+      sgl::load_n(f[k], pf.p);
+      sgl::load_n(x[k], px.p);
 #pragma unroll
-        for (int j = 0; j < V; ++j) gr[k][j] = zero[j];
-      }
-      gap[k] = DECAY ? a.gaps[u.n * a.gaps_n + at * a.gaps_t] : 0.f;
+      for (int j = 0; j < V; ++j) gr[k][j] = zero[j];
+      if (gh != nullptr) sgl::load_n(gr[k], ph.p);
+      gap[k] = DECAY ? *pg.p : 0.f;
+      pf.next(k + 1 < m);
+      px.next(k + 1 < m);
+      if (gh != nullptr) ph.next(k + 1 < m);
+      if (DECAY) pg.next(k + 1 < m);
     }
+  };
+  int64_t b = (live - 1) / kKeep * kKeep;
+  int m = int(live - b);
+  fetch(b, m);
+  for (;;) {
     // forward through the block: a, 1 - a, and the factors lam meets
-    float ga[kKeep][V], gb[kKeep][V], wl[kKeep][V], wg[kKeep][V];
+    float ga[kKeep][V], gb[kKeep][V], wl[kKeep][V], wg[kKeep][V], gn[kKeep];
+    T gl[kKeep][V];
 #pragma unroll
-    for (int k = 0; k < kKeep; ++k)
+    for (int k = 0; k < kKeep; ++k) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         float sn;
@@ -324,23 +355,35 @@ __device__ __forceinline__ void walk_back(const ScanArgs &a, const Unit &u, int6
         wl[k][j] = (s[j] - xv) * ga[k][j];   // d log a
         wg[k][j] = wl[k][j] * sn;            // d gate
         s[j] = ga[k][j] * s[j] + gb[k][j] * xv;
+        gl[k][j] = gr[k][j];
       }
+      gn[k] = gap[k];
+    }
+    const int64_t at = row0 + b * a.D;
+    const int now = m;
+    const bool more = b - kKeep >= t0;
+    if (more) {
+      b -= kKeep;
+      m = kKeep;
+      fetch(b, m);
+    }
 #pragma unroll
     for (int k = kKeep - 1; k >= 0; --k) {
-      if (k < m) {
+      if (k < now) {
         T og[V], ov[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float lam = float(gr[k][j]) + c[j];
+          const float lam = float(gl[k][j]) + c[j];
           c[j] = ga[k][j] * lam;
           og[j] = T(lam * wg[k][j]);
           ov[j] = T(lam * gb[k][j]);
-          if (DECAY) dsum[j] -= lam * wl[k][j] * gap[k];
+          if (DECAY) dsum[j] -= lam * wl[k][j] * gn[k];
         }
-        sgl::store_n(dgate + row0 + (b + k) * a.D, og);
-        sgl::store_n(dvalue + row0 + (b + k) * a.D, ov);
+        sgl::store_n(dgate + at + k * a.D, og);
+        sgl::store_n(dvalue + at + k * a.D, ov);
       }
     }
+    if (!more) return;
   }
 }
 

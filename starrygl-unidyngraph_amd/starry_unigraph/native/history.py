@@ -42,9 +42,19 @@ def _tensor(name: str, t, like: torch.Tensor, shape: tuple, dtype=None) -> torch
         raise ValueError(f"{name}: {t.dtype}, expected {want}")
     if t.device != like.device:
         raise ValueError(f"{name}: on {t.device}, expected {like.device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
     return t
+
+
+def _tracked(*tensors) -> bool:
+    """Whether autograd has to know of a call (without it nothing is kept)."""
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -102,12 +112,21 @@ def gated_scan(gate: torch.Tensor, value: torch.Tensor, *, lens: torch.Tensor | 
     if N == 0 or L == 0:   # nothing to run: empty rows, the states as they are
         last = state + 0.0 if state is not None else torch.zeros(N, D, device=gate.device)
         return gate + value, last if decay is None else last + 0.0 * decay
+    if not _tracked(gate, value, state, decay):
+        return _Scan.run(gate, value, state, decay, lens, gaps, False)[:2]
     return _Scan.apply(gate, value, state, decay, lens, gaps)
 
 
 class _Scan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, gate, value, state, decay, lens, gaps):
+    def forward(ctx, *args):
+        h, last, saved = _Scan.run(*args, True)
+        ctx.save_for_backward(*saved)
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    def run(gate, value, state, decay, lens, gaps, need):
         lib, P, dev = _capi.lib(), _capi.ptr, gate.device
         gate, value = _rows(gate), _rows(value)
         state = None if state is None else state.contiguous()
@@ -117,7 +136,7 @@ class _Scan(torch.autograd.Function):
         h = torch.empty(N, L, D, dtype=gate.dtype, device=dev)
         last = torch.empty(N, D, dtype=torch.float32, device=dev)
         keep = None
-        if any(ctx.needs_input_grad):
+        if need:
             keep = torch.empty(lib.sgl_gated_scan_keep_elems(N, L, D), dtype=torch.float32, device=dev)
         nb = lib.sgl_gated_scan_workspace_bytes(dt, N, L, D, 0, 0)
         ws = _capi.workspace(nb, dev) if nb else None
@@ -125,9 +144,7 @@ class _Scan(torch.autograd.Function):
             _capi.check(lib.sgl_gated_scan_forward(
                 dt, N, L, D, *_Scan.inputs(gate, value, lens, state, gaps, decay), P(h), P(last), P(keep), P(ws), nb,
                 _capi.stream_of(dev)), "gated_scan")
-        ctx.save_for_backward(gate, value, state, decay, lens, gaps, keep)
-        ctx.set_materialize_grads(False)
-        return h, last
+        return h, last, (gate, value, state, decay, lens, gaps, keep)
 
     @staticmethod
     def inputs(gate, value, lens, state, gaps, decay) -> tuple:
@@ -211,8 +228,11 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens
     least = 16 // q.element_size()
     if dh < least:   # the kernels read 16 bytes of a head at a time: zeros add nothing to the products
         q, k, v = (torch.nn.functional.pad(t, (0, least - dh)) for t in (q, k, v))
-    o = _Attend.apply(q, k, v, bias, (q_lens, k_lens, key_mask, q_pos if bias is not None else None,
-                                         k_pos if bias is not None else None), int(resolution), bool(two_sided), scale)
+    fixed = (q_lens, k_lens, key_mask) + ((q_pos, k_pos) if bias is not None else (None, None))
+    if _tracked(q, k, v, bias):
+        o = _Attend.apply(q, k, v, bias, fixed, int(resolution), bool(two_sided), scale)
+    else:
+        o = _Attend.run(q, k, v, bias, fixed, int(resolution), bool(two_sided), scale, False)[0]
     return o if dh >= least else o[..., :dh]
 
 
@@ -231,25 +251,30 @@ def distance_bucket(distance: torch.Tensor, buckets: int, resolution: int = 0) -
 
 class _Attend(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, bias, fixed, resolution, two_sided, scale):
+    def forward(ctx, *args):
+        o, saved, ctx.problem = _Attend.run(*args, True)
+        ctx.save_for_backward(*saved)
+        return o
+
+    @staticmethod
+    def run(q, k, v, bias, fixed, resolution, two_sided, scale, need):
+        """(o, the backward's tensors, the problem over their addresses)."""
         lib, P, dev = _capi.lib(), _capi.ptr, q.device
         q, k, v = _rows(q), _rows(k), _rows(v)
         bias = None if bias is None else bias.contiguous()
-        a, need = _Attend.problem(q, k, v, bias, fixed, resolution, two_sided, scale), any(ctx.needs_input_grad)
+        a = _Attend.problem(q, k, v, bias, fixed, resolution, two_sided, scale)
+        ref = ctypes.byref(a)
         N, Lq, Hq, dh = q.shape
         o = torch.empty(N, Lq, Hq, dh, dtype=q.dtype, device=dev)
-        saves = lib.sgl_cross_attention_saves(ctypes.byref(a)) if need else 0
+        saves = lib.sgl_cross_attention_saves(ref) if need else 0
         lse = torch.empty(N, Lq * Hq, dtype=torch.float32, device=dev) if saves & 1 else None
         rest = torch.empty_like(o) if saves & 2 else None
-        nb = lib.sgl_cross_attention_workspace_bytes(ctypes.byref(a), 0)
+        nb = lib.sgl_cross_attention_workspace_bytes(ref, 0)
         ws = _capi.workspace(nb, dev) if nb else None
         with _guard(dev):
-            _capi.check(lib.sgl_cross_attention_forward(ctypes.byref(a), P(o), P(rest), P(lse), P(ws), nb,
-                                                        _capi.stream_of(dev)), "cross_attention")
-        if need:
-            ctx.save_for_backward(q, k, v, bias, o if saves & 1 else None, rest, lse, *fixed)
-            ctx.form = (resolution, two_sided, scale)
-        return o
+            _capi.check(lib.sgl_cross_attention_forward(ref, P(o), P(rest), P(lse), P(ws), nb, _capi.stream_of(dev)),
+                        "cross_attention")
+        return o, (q, k, v, bias, o if saves & 1 else None, rest, lse, *fixed), a
 
     @staticmethod
     def problem(q, k, v, bias, fixed, resolution, two_sided, scale):
@@ -268,19 +293,19 @@ class _Attend(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, go):
-        q, k, v, bias, o, rest, lse, *fixed = ctx.saved_tensors
+        q, k, v, bias, o, rest, lse = ctx.saved_tensors[:7]   # (where the problem's addresses point)
         lib, P, dev = _capi.lib(), _capi.ptr, q.device
-        a = _Attend.problem(q, k, v, bias, fixed, *ctx.form)
+        a = ctypes.byref(ctx.problem)
         go = go.contiguous()
         dq = torch.empty_like(go)
         dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
         dv = torch.empty(v.shape, dtype=v.dtype, device=dev)
         db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[3] else None
-        nb = lib.sgl_cross_attention_workspace_bytes(ctypes.byref(a), 1)
+        nb = lib.sgl_cross_attention_workspace_bytes(a, 1)
         ws = _capi.workspace(nb, dev) if nb else None
         with _guard(dev):
             _capi.check(lib.sgl_cross_attention_backward(
-                ctypes.byref(a), P(o), P(rest), P(lse), P(go), P(dq), P(dk), P(dv), P(db), P(ws), nb, _capi.stream_of(dev)),
+                a, P(o), P(rest), P(lse), P(go), P(dq), P(dk), P(dv), P(db), P(ws), nb, _capi.stream_of(dev)),
                 "cross_attention backward")
         return dq, dk, dv, db, None, None, None, None
 
@@ -311,7 +336,10 @@ def gated_norm(x: torch.Tensor, z: torch.Tensor, gate: torch.Tensor, scale: torc
                     ("pre_weight", pre_weight), ("pre_bias", pre_bias)):
         if t is not None:
             _tensor(name, t, x, (D,), torch.float32)
-    return _Norm.apply(x, z, gate, scale, post_weight, pre_weight, post_bias, pre_bias, float(eps), bool(rms))
+    args = (x, z, gate, scale, post_weight, pre_weight, post_bias, pre_bias)
+    if _tracked(*args):
+        return _Norm.apply(*args, float(eps), bool(rms))
+    return _Norm.run(*args, float(eps), bool(rms))[:2]
 
 
 def _as_rows(t: torch.Tensor) -> torch.Tensor:
@@ -328,7 +356,15 @@ def _as_rows(t: torch.Tensor) -> torch.Tensor:
 
 class _Norm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, z, gate, scale, post_w, pre_w, post_b, pre_b, eps, rms):
+    def forward(ctx, *args):
+        y, n, saved = _Norm.run(*args)
+        ctx.save_for_backward(*saved)
+        ctx.form = (y.shape, *args[-2:])
+        ctx.set_materialize_grads(False)
+        return y, n
+
+    @staticmethod
+    def run(x, z, gate, scale, post_w, pre_w, post_b, pre_b, eps, rms):
         lib, P, dev = _capi.lib(), _capi.ptr, x.device
         shape = x.shape
         x, z, gate = _as_rows(x), _as_rows(z), _as_rows(gate)
@@ -340,10 +376,7 @@ class _Norm(torch.autograd.Function):
         with _guard(dev):
             _capi.check(lib.sgl_gated_norm_forward(dt, rows, D, *_Norm.inputs(x, z, gate, vecs), eps, rms, P(y), P(n),
                                                    _capi.stream_of(dev)), "gated_norm")
-        ctx.save_for_backward(x, z, gate, *vecs)
-        ctx.form = (shape, eps, rms)
-        ctx.set_materialize_grads(False)
-        return y, n
+        return y, n, (x, z, gate, *vecs)
 
     @staticmethod
     def inputs(x, z, gate, vecs) -> tuple:
