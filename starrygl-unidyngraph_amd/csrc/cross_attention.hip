@@ -24,8 +24,15 @@
 // blocks come out of the MFMA with the reduction index of the product that
 // follows in a lane's own registers (key x row blocks for o and dq, row x
 // key blocks for dk and dv), so p and ds go from one product to the next
-// without leaving the registers; the other operand is read from a transposed
-// tile whose columns are permuted to that order.
+// without leaving the registers; the other operand is read down the columns of
+// the row-major tile in that order (16-bit types: the transposing LDS read).
+//
+// Which kernels run, by size (both sides measured at the rules):
+//   rows = lq G <= 32       one wave a (sequence, key head), or the keys split
+//                           over workgroups and joined where sequences are few
+//   rows <= 32, lk <= 64    the backward in one wave, nothing kept for it
+//   more                    tiles in LDS; 8 waves a workgroup where that gives
+//                           192 workgroups or more, else 4 waves along the keys
 #include <climits>
 
 #include "cross_attention.h"

@@ -22,9 +22,11 @@ namespace {
 // so that o and `rest` together hold o to 32 bits' precision: D = <do, o> meets
 // p dp in sums of a column over all rows and keys that nearly cancel, where an
 // error in D, the same for a whole row, does not. With p in one part the bias
-// table's gradient was 0.3 % off, with two 5e-6, with three 3e-6 (the error of
-// the formula in 32 bits throughout); the extra products take the forward of
-// 8 x 8 x 1000 x 2049 heads of 64 from 119 to 178 us.
+// table's gradient was 0.3 % off, with two 4.6e-6, with three 3.9e-6 (the
+// formula in float32 throughout: 2.9e-6); the extra products take the forward
+// of 8 sequences, 8 heads of 64 (2 key heads), 1000 x 2049, from 119 to 176 us
+// (21 GFLOP). A block of rows at a time then, its values' fragments read again:
+// kept in registers for all blocks they spill (220 us).
 constexpr float kSlack = 6.f;
 
 template <typename T, int DP, int TK>
@@ -224,7 +226,10 @@ __global__ __launch_bounds__(RW * KW * 64, (simd_waves<T, DP>(4, 2))) void k_att
 // a time, the next ones in flight. One wave takes a short sequence (`parts` 0);
 // long ones are split over the four waves of `parts` workgroups, whose
 // (maximum, sum, products) are joined in LDS and, with several workgroups, by
-// a second kernel.
+// a second kernel. Bound by the chain of loads of a wave (counts, then keys and
+// positions, then the values' LDS tile) at three waves a SIMD: 32 x 8192 keys,
+// 2 heads of 64 in bf16, 28 us and 11 joined (105 MB: 3.7 TB/s in the first);
+// 4000 windows of 20 x 32, 4 heads of 43: 67 us (1.9 TB/s).
 constexpr int kStep = 32;
 
 template <typename T, int DP, int NQ>

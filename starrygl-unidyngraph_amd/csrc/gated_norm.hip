@@ -14,7 +14,12 @@
 // from the tensors it reads anyway, so the forward stores none. The weights'
 // gradients are sums over rows: a lane keeps its columns' sums over the rows
 // its workgroup walks, and the workgroups' rows of sums are added by
-// k_sum_rows in one order.
+// k_sum_rows in one order. The next row's values are in flight while a row is
+// worked on.
+//
+// Measured: 131073 rows of 512 in fp16, rms: 131 us forward, 208 backward, 5.1
+// TB/s both (a copy of 2 GiB reaches 4.9); 24000 rows of 172 in bf16: 19 and 27
+// us, 2.4 TB/s, two or three rows a wave; 400 rows of 100 in fp32: 4 us.
 #include <climits>
 
 #include "history.h"
@@ -187,6 +192,8 @@ __global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK)) void k_norm_fwd(NormAr
 
 // part: this workgroup's sums, [5][D]: scale, post weight, pre weight, post
 // bias, pre bias (the biases' rows only with biases).
+// (three waves a SIMD where a lane holds 8 columns: 168 registers, a few of them
+// spilled, 206 us where two waves take 230 at 131073 x 512)
 template <typename T, int V, int NV, int LPR, bool BIAS>
 __global__ __launch_bounds__((Row<T, V, NV, LPR>::BLOCK), (LPR <= 256 && V * NV == 8 && !BIAS ? 3 : 1)) void k_norm_bwd(NormArgs a, const T *__restrict__ gy,
                                                                           const T *__restrict__ gn,

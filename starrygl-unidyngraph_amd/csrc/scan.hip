@@ -22,7 +22,13 @@
 // The forward keeps the state in fp32 at every kKeep-th step; the backward
 // walks blocks of kKeep steps last to first, computing a block's states again
 // in registers from the kept one, so it neither reads the (rounded) outputs
-// nor differentiates through their rounding.
+// nor differentiates through their rounding; the block before is in flight
+// meanwhile (without that 217 us where it is now 122).
+//
+// Measured, bf16: 8000 windows of up to 32 x 172 with decay 74 us forward and
+// 122 backward (3.2 TB/s both; a copy reaches 4.9); 16 x 8191 x 256 25 + 37
+// and 35 + 64 us (pieces + walk; the inputs are read twice). One event of 400
+// x 100 in fp32: 4 us, a launch.
 #include <climits>
 
 #include "history.h"
@@ -32,7 +38,9 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kKeep = 8;             // steps between kept states
 constexpr int64_t kFill = 1 << 18;   // threads that fill the GPU: 16 waves a CU
-constexpr int64_t kPieces = 2 * kFill;   // pieces x channel groups: two rounds of the backward (4 x 8191 x 256 in bf16: 160 us; 1.25 kFill 170, 0.75 183)
+// pieces x channel groups: two rounds of the backward's workgroups (16 x 8191 x
+// 256 in bf16, both directions: 160 us; 1.25 kFill 170, 0.75 kFill 183)
+constexpr int64_t kPieces = 2 * kFill;
 constexpr int kSubs = 8;             // pieces a workgroup of the cut form: kLanes channel groups each
 constexpr int kLanes = kBlock / kSubs;
 constexpr int kMaxSupers = 32;
