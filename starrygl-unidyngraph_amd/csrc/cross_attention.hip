@@ -71,7 +71,11 @@ int check_attn(const sgl_attention *p) {
   }
   SGL_REQUIRE(p->n == 0 || ((p->lq == 0 || p->q) && (p->lk == 0 || (p->k && p->v))), "cross_attention: NULL array");
   const int64_t rows = p->lq * (p->heads_q / p->heads_kv);
-  SGL_REQUIRE(rows < INT_MAX && p->n * p->heads_kv < INT_MAX && p->n * p->heads_kv * (std::max(rows, p->lk) / 64 + 1) < INT_MAX / 4,
+  // a launch has fewer than 2^32 threads: one wave an item (few rows, few keys),
+  // else at most a workgroup of 512 for each 64 rows or keys of one
+  const int64_t items = p->n * p->heads_kv, most = std::max(rows, p->lk);
+  const bool one_wave = rows <= sgl::attn::kSmallRows && p->lk <= sgl::attn::kSmallKeys;
+  SGL_REQUIRE(rows < INT_MAX && items < (1 << 25) && (one_wave || items * (most / 64 + 1) < (1 << 23)),
               "cross_attention: too many rows for one call");
   return SGL_OK;
 }

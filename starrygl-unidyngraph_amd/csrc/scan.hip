@@ -534,7 +534,8 @@ float *place_work(ScanArgs &a, const ScanPlan &p, void *workspace) {
 int check_scan(int32_t dtype, int64_t N, int64_t L, int32_t D, const ScanArgs &a) {
   SGL_REQUIRE(dtype >= 0 && dtype <= SGL_FP16, "gated_scan: unknown element type %d", dtype);
   SGL_REQUIRE(N >= 0 && L >= 0 && D > 0 && N < INT_MAX && L < INT_MAX, "gated_scan: bad sizes");
-  SGL_REQUIRE(N * D < int64_t(INT_MAX) * (kBlock / 2), "gated_scan: %lld sequences of %d channels are too many",
+  // (a launch has fewer than 2^32 threads: one for each channel)
+  SGL_REQUIRE(N * D <= (int64_t(1) << 32) - kBlock, "gated_scan: %lld sequences of %d channels are too many",
               (long long)N, D);
   SGL_REQUIRE((a.gaps == nullptr) == (a.decay == nullptr), "gated_scan: give both gaps and decay or neither");
   SGL_REQUIRE(N == 0 || L == 0 || (a.gate && a.value), "gated_scan: NULL array");

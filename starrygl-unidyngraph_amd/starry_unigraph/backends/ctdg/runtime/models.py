@@ -291,7 +291,7 @@ class CTDGHistoryPredictor(CTDGLinkPredictor):
         b, K, W = step.buf, dims.fanout, dims.D + dims.F
         live = torch.arange(b.cap, device=step.dev) < b.num_roots
         cnt = torch.where(live, b.hop.cnt, 0)
-        events = b.X.view(-1, dims.C)[:b.cap * K].view(b.cap, K, dims.C)[..., :W]
+        events = b.X[:b.cap * K * dims.C].view(b.cap, K, dims.C)[..., :W]
         inside = torch.arange(K, device=step.dev) < cnt.unsqueeze(1)
         # (rows past a count hold an earlier step's events: the products over them have zero gradients)
         y = self.history(b.new_mem[:b.cap], events, cnt, torch.where(inside, b.hop.dt[:b.cap * K].view(b.cap, K), 0.0))

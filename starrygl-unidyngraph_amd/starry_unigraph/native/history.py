@@ -252,13 +252,14 @@ def distance_bucket(distance: torch.Tensor, buckets: int, resolution: int = 0) -
 class _Attend(torch.autograd.Function):
     @staticmethod
     def forward(ctx, *args):
-        o, saved, ctx.problem = _Attend.run(*args, True)
+        o, saved = _Attend.run(*args, True)
         ctx.save_for_backward(*saved)
+        ctx.form = args[5:]
         return o
 
     @staticmethod
     def run(q, k, v, bias, fixed, resolution, two_sided, scale, need):
-        """(o, the backward's tensors, the problem over their addresses)."""
+        """(o, the backward's tensors)."""
         lib, P, dev = _capi.lib(), _capi.ptr, q.device
         q, k, v = _rows(q), _rows(k), _rows(v)
         bias = None if bias is None else bias.contiguous()
@@ -274,7 +275,7 @@ class _Attend(torch.autograd.Function):
         with _guard(dev):
             _capi.check(lib.sgl_cross_attention_forward(ref, P(o), P(rest), P(lse), P(ws), nb, _capi.stream_of(dev)),
                         "cross_attention")
-        return o, (q, k, v, bias, o if saves & 1 else None, rest, lse, *fixed), a
+        return o, (q, k, v, bias, o if saves & 1 else None, rest, lse, *fixed)
 
     @staticmethod
     def problem(q, k, v, bias, fixed, resolution, two_sided, scale):
@@ -293,9 +294,10 @@ class _Attend(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, go):
-        q, k, v, bias, o, rest, lse = ctx.saved_tensors[:7]   # (where the problem's addresses point)
+        q, k, v, bias, o, rest, lse, *fixed = ctx.saved_tensors
         lib, P, dev = _capi.lib(), _capi.ptr, q.device
-        a = ctypes.byref(ctx.problem)
+        # (from the tensors as they are now: a hook on saved tensors may bring them back elsewhere)
+        a = ctypes.byref(_Attend.problem(q, k, v, bias, fixed, *ctx.form))
         go = go.contiguous()
         dq = torch.empty_like(go)
         dk = torch.empty(k.shape, dtype=k.dtype, device=dev)

@@ -145,3 +145,19 @@ def test_calls_on_two_streams_do_not_meet(ops, gpu):
     torch.cuda.synchronize()
     for (o, g), (wo, wg) in zip(out, alone):
         assert torch.equal(o, wo) and all(torch.equal(g[k], wg[k]) for k in wg)
+
+
+def test_saved_tensors_may_come_back_elsewhere(ops, gpu):
+    """Hooks that move what a backward reads (host offloading, recomputation)
+    give the same gradients."""
+    for case in (FORMS[9], (5, 1, 10, 2, 2, 50, FP32, 32, 0, False, True, False)):
+        t, kw, _ = _inputs(ops, *case)
+        _, want = _run_attend(ops, t, kw, gpu)
+        with torch.autograd.graph.save_on_cpu():
+            _, got = _run_attend(ops, t, kw, gpu)
+        assert all(torch.equal(got[k], want[k]) for k in want)
+    t, gh, gl = _scan_inputs(4, 40, 50, FP32, True, True, True)
+    want = _run_scan(ops, t, gh, gl, gpu)[2]
+    with torch.autograd.graph.save_on_cpu():
+        got = _run_scan(ops, t, gh, gl, gpu)[2]
+    assert all(torch.equal(got[k], want[k]) for k in want)
