@@ -228,7 +228,7 @@ __global__ __launch_bounds__(RW * KW * 64, (simd_waves<T, DP>(4, 2))) void k_att
 // (maximum, sum, products) are joined in LDS and, with several workgroups, by
 // a second kernel. Bound by the chain of loads of a wave (counts, then keys and
 // positions, then the values' LDS tile) at three waves a SIMD: 32 x 8192 keys,
-// 2 heads of 64 in bf16, 28 us and 11 joined (105 MB: 3.7 TB/s in the first);
+// 2 heads of 64 in bf16, 28 us and 4 joined (105 MB: 3.7 TB/s in the first);
 // 4000 windows of 20 x 32, 4 heads of 43: 67 us (1.9 TB/s).
 constexpr int kStep = 32;
 
@@ -445,34 +445,51 @@ __global__ __launch_bounds__(kBlock, (simd_waves<T, DP>(3, DP <= 64 ? 2 : 1))) v
   }
 }
 
-// The parts of a row joined: one wave a row, a lane two neighbouring values.
+// The parts of a row joined: one wave a row, a lane two neighbouring values. All
+// loads of sixteen parts go out at once: 256 rows of 64 from 16 parts take 4 us,
+// where a pass over the maxima first took 11.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_attn_join(Args a, int parts, const float *__restrict__ pacc,
                                                       const float2 *__restrict__ pml, T *__restrict__ o,
                                                       T *__restrict__ rest, float *__restrict__ lse) {
   const sgl_attention &p = a.p;
   const int lane = threadIdx.x & 63, dh = p.head_dim;
-  const int64_t x = int64_t(blockIdx.x) * kWaves + (threadIdx.x >> 6);   // (item, row)
-  if (x >= p.n * p.heads_kv * a.rows) return;
-  const int64_t item = x / a.rows, r = x - item * a.rows;
-  const int64_t n = item / p.heads_kv, i = r / a.G;
-  const int hk = int(item - n * p.heads_kv), h = int(r - i * a.G);
+  const uint32_t x = blockIdx.x * kWaves + wave_index();   // (item, row)
+  const uint32_t rows = uint32_t(a.rows), all = uint32_t(p.n * p.heads_kv) * rows;
+  if (x >= all) return;
+  const uint32_t item = x / rows, r = x - item * rows;
+  const int64_t n = item / uint32_t(p.heads_kv), i = r / uint32_t(a.G);
+  const int hk = int(item - uint32_t(n) * p.heads_kv), h = int(r - uint32_t(i) * a.G);
   const bool ok = p.q_lens == nullptr || i < p.q_lens[n];
-  float top = -INFINITY;
-  for (int k = lane; k < parts; k += kWave) top = fmaxf(top, pml[(item * parts + k) * a.rows + r].x);
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
-  const float at = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, v0 = 0.f, v1 = 0.f;
+  // a group of parts at a time, its sums rescaled where its maximum is larger
+  constexpr int U = 16;
+  float top = -INFINITY, sum = 0.f, v0 = 0.f, v1 = 0.f;
   const int d = 2 * lane;
-#pragma unroll 8
-  for (int k = 0; k < parts; ++k) {
-    const int64_t row = (item * parts + k) * a.rows + r;
-    const float2 e = pml[row];
-    const float f = __builtin_amdgcn_exp2f(e.x - at);
-    sum += e.y * f;
-    if (d < dh) v0 += f * pacc[row * dh + d];
-    if (d + 1 < dh) v1 += f * pacc[row * dh + d + 1];
+  for (int k0 = 0; k0 < parts; k0 += U) {
+    float2 e[U];
+    float w0[U], w1[U];
+    float most = top;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int64_t row = (int64_t(item) * parts + min(k0 + k, parts - 1)) * rows + r;
+      e[k] = pml[row];
+      w0[k] = d < dh ? pacc[row * dh + d] : 0.f;
+      w1[k] = d + 1 < dh ? pacc[row * dh + d + 1] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) most = fmaxf(most, e[k].x);
+    const float at = most == -INFINITY ? 0.f : most, f0 = __builtin_amdgcn_exp2f(top - at);
+    sum *= f0;
+    v0 *= f0;
+    v1 *= f0;
+    top = most;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const float f = k0 + k < parts ? __builtin_amdgcn_exp2f(e[k].x - at) : 0.f;
+      sum += e[k].y * f;
+      v0 += f * w0[k];
+      v1 += f * w1[k];
+    }
   }
   const float inv = ok && sum > 0.f ? 1.f / sum : 0.f;
   const int64_t to = out_row(a, n, hk, i, h);
