@@ -61,9 +61,12 @@ __device__ __forceinline__ FragOf<T> frag_of(const float (&x)[NB][4], int s) {
   return f;
 }
 
-// The same in three parts, each the rounding of what those before it left.
+// The same in parts that together hold 22 bits (fp16: two) or 24 (bf16: three)
+// of a value, each the rounding of what those before it left.
+template <typename T>
+constexpr int kParts = std::is_same_v<T, fp16_t> ? 2 : 3;
 template <typename T, int NB>
-__device__ __forceinline__ void split_frag_of(const float (&x)[NB][4], int s, FragOf<T> (&f)[3]) {
+__device__ __forceinline__ void split_frag_of(const float (&x)[NB][4], int s, FragOf<T> (&f)[kParts<T>]) {
   constexpr int B = Mma<T>::KS / 16;
 #pragma unroll
   for (int b = 0; b < B; ++b)
@@ -71,7 +74,7 @@ __device__ __forceinline__ void split_frag_of(const float (&x)[NB][4], int s, Fr
     for (int v = 0; v < 4; ++v) {
       float e = s * B + b < NB ? x[s * B + b][v] : 0.f;
 #pragma unroll
-      for (int i = 0; i < 3; ++i) {
+      for (int i = 0; i < kParts<T>; ++i) {
         f[i][4 * b + v] = T(e);
         e -= float(T(e));
       }

@@ -180,11 +180,13 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
     }
 #pragma unroll
     for (int b = 0; b < NQ; ++b) {
-      scale_scores(x[b], c, -ls[b], table + row[b].h * table_ld(a), col[b < NP ? b : 0], biased);
+      // (the forward's scores to the bit, then less lse: taken off within the fma, its rounding is one error for a
+      // row and column, which the table's gradient keeps; and a single key's p is 1)
+      scale_scores(x[b], c, 0.f, table + row[b].h * table_ld(a), col[b < NP ? b : 0], biased);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) x[b][kb][v] = __builtin_amdgcn_exp2f(x[b][kb][v]);
+        for (int v = 0; v < 4; ++v) x[b][kb][v] = __builtin_amdgcn_exp2f(x[b][kb][v] - ls[b]);
     }
     if (on != full_mask(KB * 16)) {   // uniform
 #pragma unroll

@@ -18,15 +18,16 @@ namespace {
 // accumulators are rescaled only when the maximum has grown by more than 2^6:
 // p stays below 2^6, and the sum and the products carry the same factor.
 // p is rounded to the operands' type for its product. Where a backward will
-// follow, what that rounding leaves is multiplied too (two more parts: 24 bits),
-// so that o and `rest` together hold o to 32 bits' precision: D = <do, o> meets
-// p dp in sums of a column over all rows and keys that nearly cancel, where an
-// error in D, the same for a whole row, does not. With p in one part the bias
-// table's gradient was 0.3 % off, with two 4.6e-6, with three 3.9e-6 (the
-// formula in float32 throughout: 2.9e-6); the extra products take the forward
-// of 8 sequences, 8 heads of 64 (2 key heads), 1000 x 2049, from 119 to 176 us
-// (21 GFLOP). A block of rows at a time then, its values' fragments read again:
-// kept in registers for all blocks they spill (220 us).
+// follow, what that rounding leaves is multiplied too (kParts in all), so that o
+// and `rest` together hold o as float32 would: D = <do, o> meets p dp in sums
+// of a column over all rows and keys that nearly cancel, where an error in D,
+// the same for a whole row, does not. In bf16 with p in one part the bias
+// table's gradient of 8 sequences, 8 heads of 64 (2 key heads), 1000 x 2049 was
+// 2.6e-3 off, in two 4.6e-6, in three 3.9e-6 (the formula in float32 throughout:
+// 2.9e-6); of 4 sequences of one row and 444 keys 6.4e-5 in two, 9e-6 in three
+// (5e-6). The first takes 119, 149 or 177 us forward (21 GFLOP). A block of
+// rows at a time then, its values' fragments read again: kept in registers for
+// all blocks they spill (220 us).
 constexpr float kSlack = 6.f;
 
 template <typename T, int DP, int TK>
@@ -185,14 +186,14 @@ __global__ __launch_bounds__(RW * KW * 64, (simd_waves<T, DP>(4, 2))) void k_att
       for (int b = 0; b < NQ; ++b)
 #pragma unroll
         for (int st = 0; st < KB * 16 / M::KS; ++st) {
-          FragOf<T> pf[3];
+          FragOf<T> pf[kParts<T>];
           split_frag_of<T>(x[b], st, pf);
           asm volatile("" ::: "memory");
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
             const FragOf<T> vf = L::template frag_t<TK>(s.v, d * 16, k0 + st * M::KS);
 #pragma unroll
-            for (int i = 0; i < 3; ++i) acc[b][d] = M::mma(vf, pf[i], acc[b][d]);
+            for (int i = 0; i < kParts<T>; ++i) acc[b][d] = M::mma(vf, pf[i], acc[b][d]);
           }
         }
     }
@@ -404,14 +405,14 @@ __global__ __launch_bounds__(kBlock, (simd_waves<T, DP>(3, DP <= 64 ? 2 : 1))) v
       for (int b = 0; b < NQ; ++b)
 #pragma unroll
         for (int st = 0; st < kStep / M::KS; ++st) {
-          FragOf<T> pf[3];
+          FragOf<T> pf[kParts<T>];
           split_frag_of<T>(x[b], st, pf);
           asm volatile("" ::: "memory");
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
             const FragOf<T> vf = L::template frag_t<kStep>(s.v, d * 16, st * M::KS);
 #pragma unroll
-            for (int i = 0; i < 3; ++i) acc[b][d] = M::mma(vf, pf[i], acc[b][d]);
+            for (int i = 0; i < kParts<T>; ++i) acc[b][d] = M::mma(vf, pf[i], acc[b][d]);
           }
         }
     }

@@ -161,3 +161,13 @@ def test_saved_tensors_may_come_back_elsewhere(ops, gpu):
     with torch.autograd.graph.save_on_cpu():
         got = _run_scan(ops, t, gh, gl, gpu)[2]
     assert all(torch.equal(got[k], want[k]) for k in want)
+
+
+@pytest.mark.parametrize("case", [(3, 100, 1, 3, 3, 100, BF16), (27, 400, 1, 4, 1, 64, FP16), (5, 20, 1, 12, 3, 64, FP32),
+                                  (300, 80, 1, 2, 1, 32, BF16), (4, 3, 1, 4, 2, 40, FP16)], ids=str)
+def test_a_single_key_has_no_gradient(ops, gpu, case):
+    """p is 1 whatever q, k and the bias are: their gradients are 0, not small."""
+    t, kw, _ = _inputs(ops, *case, 17, 1, True, False, False)
+    _, grads = _run_attend(ops, t, kw, gpu)
+    for k in ("dq", "dk", "dbias"):
+        assert not grads[k].any(), (k, float(grads[k].abs().max()))
