@@ -436,7 +436,7 @@ constexpr float kProbUp = std::is_same_v<T, fp16_t> ? 1024.f : 1.f;
 
 // The bias gradient's cells in LDS: [column][slots] sums of ds for a set of row
 // blocks whose row c has one head, in fixed point (34 fractional bits in an
-// int64, relative to a power of two near the largest |do|): integer adds give
+// int64, 33 of them used, relative to a power of two near the largest |do|): integer adds give
 // the same sum in any order, and the LDS adds them at 7 to 8 clocks an
 // instruction, four lanes a cell included, where float adds take 194 (3 a
 // lane; a read, an add and a write 11, in cells of a lane's own). A value
@@ -460,9 +460,12 @@ __device__ __forceinline__ void add_cells(Cell *cells, const int (&col)[N][4], c
   for (int k = 0; k < N; ++k)
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
-      const float t = x[k][v] * f, hi = floorf(t);
+      // the nearest integer and a signed rest, which is exact (from the integer below, a small negative value's
+      // rest lies next to one and has lost its digits)
+      const float t = x[k][v] * f, hi = rintf(t);
       seen += fabsf(t);
-      const Cell val = (Cell(uint32_t(int(hi))) << 32) | uint32_t((t - hi) * 4294967296.f);
+      const int lo = int((t - hi) * 2147483648.f);   // in units of 2^-31 of t, so two of a cell's
+      const Cell val = (Cell(uint32_t(int(hi) + (lo >> 31))) << 32) | (uint32_t(lo) << 1);
       __hip_atomic_fetch_add(cells + col[k][v] * slots + c, val, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
 }
