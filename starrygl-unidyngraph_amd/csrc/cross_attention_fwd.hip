@@ -205,7 +205,7 @@ __global__ __launch_bounds__(RW * KW * 64, (simd_waves<T, DP>(4, 2))) void k_att
 #pragma unroll
   for (int b = 0; b < NQ; ++b) {
     if (!in[b]) continue;
-    const float inv = ok[b] && l[b] > 0.f ? 1.f / l[b] : 0.f;
+    const float inv = ok[b] && l[b] != 0.f ? 1.f / l[b] : 0.f;
     const int64_t at = out_row(a, n, hk, row[b].i, row[b].h);
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
@@ -213,10 +213,10 @@ __global__ __launch_bounds__(RW * KW * 64, (simd_waves<T, DP>(4, 2))) void k_att
       store4(o + at, d * 16 + 4 * g, dh, v);
       if (rest != nullptr) store_rest(rest + at, d * 16 + 4 * g, dh, v);   // for the backward's D
     }
-    // log2 of the sum of 2^x; +inf where no key is live, so that p is 0 there
+    // log2 of the sum of 2^x; +inf where no key is live, so that p is 0 there (a NaN score's row keeps its NaN)
     if (lse != nullptr && g == 0)
       lse[(n * p.heads_kv + hk) * a.rows + int64_t(row[b].i) * a.G + row[b].h] =
-          ok[b] && l[b] > 0.f ? m[b] + __log2f(l[b]) : INFINITY;
+          ok[b] && l[b] != 0.f ? m[b] + __log2f(l[b]) : INFINITY;
   }
 }
 
@@ -433,7 +433,7 @@ __global__ __launch_bounds__(kBlock, (simd_waves<T, DP>(3, DP <= 64 ? 2 : 1))) v
       if (g == 0) pml[r] = make_float2(m[b], l[b]);
       continue;
     }
-    const float inv = ok[b] && l[b] > 0.f ? 1.f / l[b] : 0.f;
+    const float inv = ok[b] && l[b] != 0.f ? 1.f / l[b] : 0.f;
     const int64_t at = out_row(a, n, hk, row[b].i, row[b].h);
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
@@ -442,7 +442,7 @@ __global__ __launch_bounds__(kBlock, (simd_waves<T, DP>(3, DP <= 64 ? 2 : 1))) v
       if (rest != nullptr) store_rest(rest + at, d * 16 + 4 * g, dh, v);
     }
     if (lse != nullptr && g == 0)
-      lse[item * a.rows + int64_t(row[b].i) * a.G + row[b].h] = ok[b] && l[b] > 0.f ? m[b] + __log2f(l[b]) : INFINITY;
+      lse[item * a.rows + int64_t(row[b].i) * a.G + row[b].h] = ok[b] && l[b] != 0.f ? m[b] + __log2f(l[b]) : INFINITY;
   }
 }
 
@@ -492,7 +492,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_join(Args a, int parts, const f
       v1 += f * w1[k];
     }
   }
-  const float inv = ok && sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = ok && sum != 0.f ? 1.f / sum : 0.f;
   const int64_t to = out_row(a, n, hk, i, h);
   v0 *= inv;
   v1 *= inv;
@@ -502,7 +502,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_join(Args a, int parts, const f
     if (d < dh) rest[to + d] = rest_of<T>(v0, T(v0));
     if (d + 1 < dh) rest[to + d + 1] = rest_of<T>(v1, T(v1));
   }
-  if (lse != nullptr && lane == 0) lse[x] = ok && sum > 0.f ? top + __log2f(sum) : INFINITY;
+  if (lse != nullptr && lane == 0) lse[x] = ok && sum != 0.f ? top + __log2f(sum) : INFINITY;
 }
 
 // ------------------------------------------------------------------ host

@@ -204,7 +204,7 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
           sum += x[b][kb][v];
         }
       sum = groups_sum(sum);
-      const float inv = ok[b] && sum > 0.f ? 1.f / sum : 0.f;
+      const float inv = ok[b] && sum != 0.f ? 1.f / sum : 0.f;   // (NaN stays)
 #pragma unroll
       for (int kb = 0; kb < NK; ++kb)
 #pragma unroll

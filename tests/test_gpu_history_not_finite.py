@@ -1,0 +1,82 @@
+"""Infinities and NaN in live places of the cross attention: they reach what
+the definition lets them reach, and nothing else."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_history import _rand
+
+pytestmark = pytest.mark.gpu
+FP32, BF16, FP16 = torch.float32, torch.bfloat16, torch.float16
+
+FORMS = [  # N, Lq, Lk, Hq, Hkv, dh
+    (3, 8, 16, 4, 2, 16),      # one wave a sequence
+    (3, 40, 50, 4, 2, 16),     # all keys in one tile
+    (3, 40, 200, 4, 2, 16),
+    (3, 1, 900, 4, 2, 16),     # a long history in parts
+    (96, 128, 130, 4, 2, 16),  # eight waves a workgroup, two heads of the same queries
+    (70, 128, 130, 3, 1, 16),
+]
+
+
+@pytest.fixture(scope="module")
+def ops(gpu):
+    from starry_unigraph.native import history
+    return history
+
+
+def _inputs(form, dtype, mask=False):
+    N, Lq, Lk, Hq, Hkv, dh = form
+    g = torch.Generator().manual_seed(Lk)
+    t = dict(q=_rand(g, N, Lq, Hq, dh, dtype=dtype), k=_rand(g, N, Lk, Hkv, dh, dtype=dtype),
+             v=_rand(g, N, Lk, Hkv, dh, dtype=dtype), go=_rand(g, N, Lq, Hq, dh, dtype=dtype), bias=_rand(g, Hq, 12))
+    t["q_pos"], t["k_pos"] = (torch.randint(0, 500, (N, L), generator=g) for L in (Lq, Lk))
+    t["key_mask"] = torch.rand(N, Lk, generator=g) < 0.7 if mask else None
+    return t
+
+
+def _run(ops, t, dev):
+    d = {k: x.to(dev) if x is not None else None for k, x in t.items()}
+    leaves = [d[k].requires_grad_() for k in ("q", "k", "v", "bias")]
+    o = ops.cross_attention(d["q"], d["k"], d["v"], bias=d["bias"], q_pos=d["q_pos"], k_pos=d["k_pos"],
+                            key_mask=d["key_mask"])
+    return [x.detach().cpu() for x in (o, *torch.autograd.grad(o, leaves, d["go"]))]
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_a_nan_score_spoils_its_row_and_what_sums_over_it(ops, gpu, form, dtype):
+    """One query row's NaN: its o and dq, and dk and dv of every key that it
+    attends to; no other row, head or sequence."""
+    t = _inputs(form, dtype)
+    clean = _run(ops, t, gpu)
+    n, i, h = 1, form[1] - 1, 1
+    t["q"][n, i, h, 3] = math.nan
+    o, dq, dk, dv, db = _run(ops, t, gpu)
+    for got, want in ((o, clean[0]), (dq, clean[1])):
+        assert torch.isnan(got[n, i, h]).all()
+        got[n, i, h] = want[n, i, h]
+        assert torch.equal(got, want)
+    for got, want in ((dk, clean[2]), (dv, clean[3])):
+        assert torch.isnan(got[n, :, 0]).all()   # (head 1's key head)
+        got[n, :, 0] = want[n, :, 0]
+        assert torch.equal(got, want)
+    assert torch.isnan(db[h]).any()
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_one_nan_score_of_a_row_spoils_the_others(ops, gpu, form, dtype):
+    """A live key's NaN: the softmax of every row of its key head is NaN at
+    every key, so o, dq, dk and dv of that head are."""
+    t = _inputs(form, dtype)
+    clean = _run(ops, t, gpu)
+    G = form[3] // form[4]
+    t["k"][2, form[2] // 2, 0, 5] = math.nan
+    out = _run(ops, t, gpu)
+    for got, want, heads in zip(out[:4], clean, (G, G, 1, 1)):
+        assert torch.isnan(got[2, :, :heads]).all()
+        got[2, :, :heads] = want[2, :, :heads]
+        assert torch.equal(got, want)
+    assert torch.isnan(out[4][:G]).any(1).all()
