@@ -224,6 +224,16 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int v = 0; v < 4; ++v) y[b][kb][v] = x[b][kb][v] * (y[b][kb][v] - delta[b]);
+    if (on != full_mask(KB * 16)) {   // (0 too where do, and with it D, is not finite)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const bool dead = !((on >> (kb * 16 + 4 * g + v)) & 1);
+#pragma unroll
+          for (int b = 0; b < NQ; ++b) y[b][kb][v] = dead ? 0.f : y[b][kb][v];
+        }
+    }
     if (part != nullptr) {
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {
@@ -542,8 +552,10 @@ __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2
   const float fk = p.scale / gs, fv = 1.f / kProbUp<T>;
 #pragma unroll
   for (int b = 0; b < DB; ++b) {
-    store4(dk + row, b * 16 + 4 * g, dh, acc[0][b] * fk);
-    store4(dv + row, b * 16 + 4 * g, dh, acc[1][b] * fv);
+    // (a dead key's sums are of p = 0, which an infinity in do or q makes NaN)
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    store4(dk + row, b * 16 + 4 * g, dh, on ? acc[0][b] * fk : zero);
+    store4(dv + row, b * 16 + 4 * g, dh, on ? acc[1][b] * fv : zero);
   }
 }
 

@@ -216,7 +216,8 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
 #pragma unroll
       for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) y[b][kb][v] = x[b][kb][v] * (y[b][kb][v] - de);
+        for (int v = 0; v < 4; ++v)   // (0 at a dead key also where do, and with it D, is not finite)
+          y[b][kb][v] = (live >> (kb * 16 + 4 * g + v)) & 1 ? x[b][kb][v] * (y[b][kb][v] - de) : 0.f;
       if (part != nullptr) add_cells(cells + (sets == 1 ? 0 : b) * slots * a.cols, col[b], y[b], slots, up, seen);
       if constexpr (std::is_same_v<T, fp16_t>) {
 #pragma unroll
@@ -306,7 +307,8 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
 #pragma unroll
           for (int st = 0; st < RS; ++st)
             acc = M::mma(L::template frag_t<R>(s.b, d * 16, st * M::KS), pf[st], acc);
-          if (j < p.lk) store4(out + at, d * 16 + 4 * g, dh, acc * f);
+          // (a dead key's sum is of p = 0, which an infinity in do or q makes NaN)
+          if (j < p.lk) store4(out + at, d * 16 + 4 * g, dh, (live >> j) & 1 ? acc * f : f32x4{0.f, 0.f, 0.f, 0.f});
         }
       }
     }

@@ -80,3 +80,38 @@ def test_one_nan_score_of_a_row_spoils_the_others(ops, gpu, form, dtype):
         got[2, :, :heads] = want[2, :, :heads]
         assert torch.equal(got, want)
     assert torch.isnan(out[4][:G]).any(1).all()
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_masked_keys_have_no_gradient_beside_an_infinite_one(ops, gpu, form, dtype, bad):
+    """A gradient of o that is not finite: keys left out by the mask, and rows
+    whose mask leaves nothing, have zero gradients all the same."""
+    t = _inputs(form, dtype, mask=True)
+    t["key_mask"][0] = False
+    clean = _run(ops, t, gpu)
+    t["go"][0, 0, :, 2] = bad   # rows without a live key: nothing changes anywhere
+    for got, want in zip(_run(ops, t, gpu), clean):
+        assert torch.equal(got, want)
+    t["go"][1, form[1] - 1, 0, 4] = bad
+    _, dq, dk, dv, db = _run(ops, t, gpu)
+    dead = ~t["key_mask"]
+    assert not dk[dead].any() and not dv[dead].any()
+    # (D = <do, o> is an infinity: ds is one too at keys whose dp has the other sign, and NaN elsewhere)
+    assert not torch.isfinite(dk[1, ~dead[1], 0]).any()
+    dq[1, form[1] - 1, 0] = clean[1][1, form[1] - 1, 0]
+    assert torch.equal(dq, clean[1])
+    for got, want in ((dk, clean[2]), (dv, clean[3])):
+        got[1, :, 0] = want[1, :, 0]
+        assert torch.equal(got, want)
+    assert not torch.isfinite(db[0]).all()
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_masked_keys_have_no_gradient_beside_an_infinite_query(ops, gpu, form):
+    t = _inputs(form, FP32, mask=True)
+    t["q"][1, 0, 0, 4] = math.inf
+    _, _, dk, dv, _ = _run(ops, t, gpu)
+    dead = ~t["key_mask"]
+    assert not dk[dead].any() and not dv[dead].any()
