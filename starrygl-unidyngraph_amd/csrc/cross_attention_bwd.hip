@@ -36,9 +36,9 @@ __host__ __device__ __forceinline__ int cell_sets(int G) {
 
 template <typename T, int DP, int NQ, bool SHARE, int RW, int KW>
 __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t tiles, const T *__restrict__ o,
-                                                          const T *__restrict__ rest, const float *__restrict__ lse,
+                                                          const T *__restrict__ rest, const float2 *__restrict__ lse,
                                                           const T *__restrict__ go, T *__restrict__ dq,
-                                                          float2 *__restrict__ rowstat, float *__restrict__ rowmost,
+                                                          float *__restrict__ rowdelta, float *__restrict__ rowmost,
                                                           float *__restrict__ part) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
@@ -76,7 +76,8 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
   FragOf<T> qf[NQ][ST], gf[NQ][ST];
   int64_t qpos[NP];
   int qrel[NP];
-  float delta[NQ], ls[NQ], gs[NQ], top = 0.f;
+  float delta[NQ], gs[NQ], top = 0.f;
+  float2 ls[NQ];
   const int64_t base = biased && any ? scalar_load(q.qpos + int64_t(i0) * p.qpos_t) : 0;
   const int64_t stat0 = (n * p.heads_kv + hk) * a.rows;
   bool qnear = true;
@@ -109,9 +110,9 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
     top = fmaxf(top, most);
     gs[b] = grad_scale<T>(most);
     const int64_t r = stat0 + int64_t(row[b].i) * a.G + row[b].h;
-    ls[b] = ok[b] ? lse[r] : INFINITY;
+    ls[b] = ok[b] ? lse[r] : make_float2(INFINITY, 0.f);
     if (g == 0 && in[b] && w % KW == 0) {   // for dk and dv
-      rowstat[r] = make_float2(delta[b], ls[b]);
+      rowdelta[r] = delta[b];
       if (std::is_same_v<T, fp16_t>) rowmost[r] = most;
     }
     if (b < NP) {
@@ -180,13 +181,13 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
     }
 #pragma unroll
     for (int b = 0; b < NQ; ++b) {
-      // (the forward's scores to the bit, then less lse: taken off within the fma, its rounding is one error for a
-      // row and column, which the table's gradient keeps; and a single key's p is 1)
+      // (the forward's scores to the bit, then less the row's maximum and sum: taken off within the fma, its rounding
+      // is one error for a row and column, which the table's gradient keeps; and a single key's p is 1)
       scale_scores(x[b], c, 0.f, table + row[b].h * table_ld(a), col[b < NP ? b : 0], biased);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) x[b][kb][v] = __builtin_amdgcn_exp2f(x[b][kb][v] - ls[b]);
+        for (int v = 0; v < 4; ++v) x[b][kb][v] = __builtin_amdgcn_exp2f((x[b][kb][v] - ls[b].x) - ls[b].y);
     }
     if (on != full_mask(KB * 16)) {   // uniform
 #pragma unroll
@@ -215,7 +216,7 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
         delta[b] = 0.f;
 #pragma unroll
         for (int i = 0; i < KW; ++i) delta[b] += sx.delta[((wr * KW + i) * NQ + b) * 16 + cl];
-        if (g == 0 && in[b] && w % KW == 0) rowstat[stat0 + int64_t(row[b].i) * a.G + row[b].h].x = delta[b];
+        if (g == 0 && in[b] && w % KW == 0) rowdelta[stat0 + int64_t(row[b].i) * a.G + row[b].h] = delta[b];
       }
     }
 #pragma unroll
@@ -314,7 +315,7 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
 // queries (SHARE, an even G) or 32 rows in order. The next tile's rows are in
 // flight while one is worked on: a thread's unit of a step lies at a uniform
 // pointer and an offset that it keeps (an odd G above one divides instead);
-// the first wave fetches what belongs to a row (D, lse, position). Bound by
+// the first wave fetches what belongs to a row (D, maximum, sum, position). Bound by
 // what a SIMD issues and LDS together (24 fragment reads and 8 table reads a
 // step of 512 scores) at two waves a SIMD: at the same size 232 us, and the same
 // with 32 keys and 64 rows a workgroup (235) or 8 waves of it (257).
@@ -324,13 +325,14 @@ template <typename T, int DP, int TR>
 struct alignas(16) DkvLds {
   T q[TR * Tile<T, DP>::LD], go[TR * Tile<T, DP>::LD];
   KeyInfo<TR> info;   // (of the rows)
-  float lse[TR], delta[TR];
+  float most[TR], sum[TR], delta[TR];
   int head[TR];
 };
 
 template <typename T, int DP, bool SHARE, int CW, int RS>
 __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2))) void k_attn_dkv(Args a, int64_t tiles, const T *__restrict__ go,
-                                                           const float2 *__restrict__ rowstat,
+                                                           const float2 *__restrict__ lse,
+                                                           const float *__restrict__ rowdelta,
                                                            const float *__restrict__ rowmost, T *__restrict__ dk,
                                                            T *__restrict__ dv) {
   using M = Mma<T>;
@@ -421,11 +423,13 @@ __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2
   }
   int64_t qp[RL];
   float2 st_[RL];
+  float de_[RL];
   int he[RL] = {};
   auto load_step = [&](uint32_t step) {
 #pragma unroll
     for (int i = 0; i < RL; ++i) {
-      st_[i] = make_float2(0.f, INFINITY);
+      st_[i] = make_float2(INFINITY, 0.f);
+      de_[i] = 0.f;
       qp[i] = 0;
       if (w == 0) {
         const int x = i * 64 + lane;
@@ -433,7 +437,8 @@ __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2
         const RowAt r = row_of(first_of(sub), sub, x % kRows);
         he[i] = r.h;
         if (x < TR && r.i < qlen) {
-          st_[i] = rowstat[stat0 + int64_t(r.i) * a.G + r.h];
+          st_[i] = lse[stat0 + int64_t(r.i) * a.G + r.h];
+          de_[i] = rowdelta[stat0 + int64_t(r.i) * a.G + r.h];
           if (biased) qp[i] = q.qpos[int64_t(r.i) * p.qpos_t];
         }
       }
@@ -478,11 +483,12 @@ __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2
 #pragma unroll
       for (int i = 0; i < RL; ++i) {
         const int x = i * 64 + lane;
-        const int64_t at = st_[i].y == INFINITY ? base : qp[i];   // (no row, or one without p)
+        const int64_t at = st_[i].x == INFINITY ? base : qp[i];   // (no row, or one without p)
         near_ = near_ && is_near(at - base);
         if (x < TR) {
-          s.lse[x] = st_[i].y;
-          s.delta[x] = st_[i].x;
+          s.most[x] = st_[i].x;
+          s.sum[x] = st_[i].y;
+          s.delta[x] = de_[i];
           s.head[x] = he[i] * table_ld(a);
           s.info.pos.pos[x] = at;
           s.info.pos.rel[x] = int(at - base);
@@ -503,10 +509,11 @@ __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2
 #pragma unroll
         for (int v = 0; v < 4; ++v) col[rb][v] = own[rb < NP ? rb : 0][v] + s.head[x0 + rb * 16 + 4 * g + v];
     }
-    float lsv[RB][4], dev[RB][4];
+    float mov[RB][4], suv[RB][4], dev[RB][4];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      __builtin_memcpy(lsv[rb], s.lse + x0 + rb * 16 + 4 * g, sizeof(lsv[rb]));
+      __builtin_memcpy(mov[rb], s.most + x0 + rb * 16 + 4 * g, sizeof(mov[rb]));
+      __builtin_memcpy(suv[rb], s.sum + x0 + rb * 16 + 4 * g, sizeof(suv[rb]));
       __builtin_memcpy(dev[rb], s.delta + x0 + rb * 16 + 4 * g, sizeof(dev[rb]));
       f32x4 sc = {0.f, 0.f, 0.f, 0.f}, dp = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -525,7 +532,7 @@ __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2
     for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        const float pr = on ? __builtin_amdgcn_exp2f(x[rb][v] - lsv[rb][v]) * kProbUp<T> : 0.f;
+        const float pr = on ? __builtin_amdgcn_exp2f((x[rb][v] - mov[rb][v]) - suv[rb][v]) * kProbUp<T> : 0.f;
         x[rb][v] = pr;
         y[rb][v] = pr * ((y[rb][v] - dev[rb][v]) * dsf);
       }
@@ -562,11 +569,11 @@ __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2
 // ------------------------------------------------------------------ host
 size_t stat_bytes(const Args &a) {
   const size_t rows = size_t(a.p.n * a.p.heads_kv * a.rows);
-  return align_up(sizeof(float2) * rows) + (a.p.dtype == SGL_FP16 ? align_up(sizeof(float) * rows) : 0);
+  return align_up(sizeof(float) * rows) * (a.p.dtype == SGL_FP16 ? 2 : 1);
 }
-float *most_of(const Args &a, float2 *stat) {
+float *most_of(const Args &a, float *stat) {
   return reinterpret_cast<float *>(reinterpret_cast<char *>(stat) +
-                                   align_up(sizeof(float2) * size_t(a.p.n * a.p.heads_kv * a.rows)));
+                                   align_up(sizeof(float) * size_t(a.p.n * a.p.heads_kv * a.rows)));
 }
 int64_t dq_tiles(const Args &a) {
   if (!many_rows(a)) return row_tiles(a, 1, false, 1);
@@ -575,8 +582,8 @@ int64_t dq_tiles(const Args &a) {
 }
 
 template <typename T, int DP, int NQ, bool SHARE, int RW, int KW>
-int launch_dq(const Args &a, int64_t tiles, const void *o, const void *rest, const float *lse, const void *go, void *dq,
-              float2 *stat, float *part, hipStream_t s) {
+int launch_dq(const Args &a, int64_t tiles, const void *o, const void *rest, const float2 *lse, const void *go, void *dq,
+              float *stat, float *part, hipStream_t s) {
   const size_t lds = std::max(
       align_bytes(buffers<DqLds<T, DP, tile_keys<T>(KW)>>() * sizeof(DqLds<T, DP, tile_keys<T>(KW)>) +
                   sizeof(DqSums<RW * KW * NQ * 16>) + table_bytes(a)) +
@@ -592,7 +599,7 @@ int launch_dq(const Args &a, int64_t tiles, const void *o, const void *rest, con
 }
 
 template <typename T, int DP, bool SHARE, int CW, int RS>
-int launch_dkv(const Args &a, const void *go, float2 *stat, void *dk, void *dv, hipStream_t s) {
+int launch_dkv(const Args &a, const float2 *lse, const void *go, float *stat, void *dk, void *dv, hipStream_t s) {
   const int64_t tiles = (a.p.lk + 16 * CW - 1) / (16 * CW);
   using S = DkvLds<T, DP, kRows * RS>;
   const size_t lds = std::max(buffers<S>() * sizeof(S) + 8 * sizeof(float) + table_bytes(a),
@@ -600,7 +607,7 @@ int launch_dkv(const Args &a, const void *go, float2 *stat, void *dk, void *dv, 
   SGL_REQUIRE(lds <= 160 * 1024, "cross_attention_backward: %zu bytes of LDS", lds);
   SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_dkv<T, DP, SHARE, CW, RS>), lds));
   launch(&k_attn_dkv<T, DP, SHARE, CW, RS>, dim3(unsigned(a.p.n * a.p.heads_kv * tiles)), dim3(CW * RS * kWave), lds, s,
-         a, tiles, static_cast<const T *>(go), static_cast<const float2 *>(stat),
+         a, tiles, static_cast<const T *>(go), lse, static_cast<const float *>(stat),
          static_cast<const float *>(most_of(a, stat)), static_cast<T *>(dk), static_cast<T *>(dv));
   SGL_CHECK_LAUNCH();
   return SGL_OK;
@@ -612,9 +619,10 @@ size_t backward_bytes(const Args &a) {
   return stat_bytes(a) + sizeof(float) * size_t(a.p.n * dq_tiles(a)) * a.p.heads_q * a.cols;
 }
 
-int run_backward(const Args &a, const void *o, const void *rest, const float *lse, const void *go, void *dq, void *dk,
+int run_backward(const Args &a, const void *o, const void *rest, const float *stats, const void *go, void *dq, void *dk,
                  void *dv, float *dbias, void *ws, hipStream_t s) {
-  float2 *stat = static_cast<float2 *>(ws);
+  const float2 *lse = reinterpret_cast<const float2 *>(stats);
+  float *stat = static_cast<float *>(ws);
   float *part = dbias != nullptr ? reinterpret_cast<float *>(static_cast<char *>(ws) + stat_bytes(a)) : nullptr;
   const int64_t tiles = dq_tiles(a);
   return by_instance(a.p, [&](auto t, auto dp) {
@@ -637,10 +645,10 @@ int run_backward(const Args &a, const void *o, const void *rest, const float *ls
     const bool wide = a.p.n * a.p.heads_kv * ((a.p.lk + 63) / 64) >= 192;
     constexpr int RS = two_blocks<T, DP>() && DP <= 64 ? 1 : 2;   // (three 4-wave workgroups a CU, or one of 8)
     if (a.G % 2 == 0)
-      return wide ? launch_dkv<T, DP, true, 4, RS>(a, go, stat, dk, dv, s)
-                  : launch_dkv<T, DP, true, 1, 4>(a, go, stat, dk, dv, s);
-    return wide ? launch_dkv<T, DP, false, 4, RS>(a, go, stat, dk, dv, s)
-                : launch_dkv<T, DP, false, 1, 4>(a, go, stat, dk, dv, s);
+      return wide ? launch_dkv<T, DP, true, 4, RS>(a, lse, go, stat, dk, dv, s)
+                  : launch_dkv<T, DP, true, 1, 4>(a, lse, go, stat, dk, dv, s);
+    return wide ? launch_dkv<T, DP, false, 4, RS>(a, lse, go, stat, dk, dv, s)
+                : launch_dkv<T, DP, false, 1, 4>(a, lse, go, stat, dk, dv, s);
   });
 }
 

@@ -30,6 +30,15 @@ namespace {
 // all blocks they spill (220 us).
 constexpr float kSlack = 6.f;
 
+// What the backward reads of a row's softmax: the maximum m that the sum is
+// relative to and log2 of the sum, so that p = 2^((x - m) - log2 l). The two
+// apart: in one number log2 l is lost beside a large m (all of a row's buckets
+// at -1e9, say), and p is 1 at every key. Infinite without a live key: p is 0
+// there. A NaN score's row keeps its NaN.
+__device__ __forceinline__ float2 row_sum(float m, float l, bool ok) {
+  return ok && l != 0.f ? make_float2(m, __log2f(l)) : make_float2(INFINITY, 0.f);
+}
+
 template <typename T, int DP, int TK>
 struct alignas(16) FwdLds {
   T k[TK * Tile<T, DP>::LD], v[TK * Tile<T, DP>::LD];
@@ -38,7 +47,7 @@ struct alignas(16) FwdLds {
 
 template <typename T, int DP, int NQ, bool SHARE, int RW, int KW, bool SPLIT>
 __global__ __launch_bounds__(RW * KW * 64, (simd_waves<T, DP>(4, 2))) void k_attn_fwd(Args a, int64_t tiles, T *__restrict__ o,
-                                                           T *__restrict__ rest, float *__restrict__ lse) {
+                                                           T *__restrict__ rest, float2 *__restrict__ lse) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   constexpr int TK = tile_keys<T>(KW), BLOCK = RW * KW * 64;
@@ -213,10 +222,8 @@ __global__ __launch_bounds__(RW * KW * 64, (simd_waves<T, DP>(4, 2))) void k_att
       store4(o + at, d * 16 + 4 * g, dh, v);
       if (rest != nullptr) store_rest(rest + at, d * 16 + 4 * g, dh, v);   // for the backward's D
     }
-    // log2 of the sum of 2^x; +inf where no key is live, so that p is 0 there (a NaN score's row keeps its NaN)
     if (lse != nullptr && g == 0)
-      lse[(n * p.heads_kv + hk) * a.rows + int64_t(row[b].i) * a.G + row[b].h] =
-          ok[b] && l[b] != 0.f ? m[b] + __log2f(l[b]) : INFINITY;
+      lse[(n * p.heads_kv + hk) * a.rows + int64_t(row[b].i) * a.G + row[b].h] = row_sum(m[b], l[b], ok[b]);
   }
 }
 
@@ -241,7 +248,7 @@ struct alignas(16) FewLds {
 
 template <typename T, int DP, int NQ, bool SPLIT>
 __global__ __launch_bounds__(kBlock, (simd_waves<T, DP>(3, DP <= 64 ? 2 : 1))) void k_attn_few(Args a, int parts, int64_t part_keys, T *__restrict__ o,
-                                                     T *__restrict__ rest, float *__restrict__ lse,
+                                                     T *__restrict__ rest, float2 *__restrict__ lse,
                                                      float *__restrict__ pacc, float2 *__restrict__ pml) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
@@ -442,7 +449,7 @@ __global__ __launch_bounds__(kBlock, (simd_waves<T, DP>(3, DP <= 64 ? 2 : 1))) v
       if (rest != nullptr) store_rest(rest + at, d * 16 + 4 * g, dh, v);
     }
     if (lse != nullptr && g == 0)
-      lse[item * a.rows + int64_t(row[b].i) * a.G + row[b].h] = ok[b] && l[b] != 0.f ? m[b] + __log2f(l[b]) : INFINITY;
+      lse[item * a.rows + int64_t(row[b].i) * a.G + row[b].h] = row_sum(m[b], l[b], ok[b]);
   }
 }
 
@@ -452,7 +459,7 @@ __global__ __launch_bounds__(kBlock, (simd_waves<T, DP>(3, DP <= 64 ? 2 : 1))) v
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_attn_join(Args a, int parts, const float *__restrict__ pacc,
                                                       const float2 *__restrict__ pml, T *__restrict__ o,
-                                                      T *__restrict__ rest, float *__restrict__ lse) {
+                                                      T *__restrict__ rest, float2 *__restrict__ lse) {
   const sgl_attention &p = a.p;
   const int lane = threadIdx.x & 63, dh = p.head_dim;
   const uint32_t x = blockIdx.x * kWaves + wave_index();   // (item, row)
@@ -502,7 +509,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_join(Args a, int parts, const f
     if (d < dh) rest[to + d] = rest_of<T>(v0, T(v0));
     if (d + 1 < dh) rest[to + d + 1] = rest_of<T>(v1, T(v1));
   }
-  if (lse != nullptr && lane == 0) lse[x] = ok && sum != 0.f ? top + __log2f(sum) : INFINITY;
+  if (lse != nullptr && lane == 0) lse[x] = row_sum(top, sum, ok);
 }
 
 // ------------------------------------------------------------------ host
@@ -525,7 +532,7 @@ size_t ml_bytes(const Args &a, int parts) {
 }
 
 template <typename T, int DP, int NQ, bool SPLIT>
-int launch_few(const Args &a, T *o, T *rest, float *lse, void *ws, hipStream_t s) {
+int launch_few(const Args &a, T *o, T *rest, float2 *lse, void *ws, hipStream_t s) {
   const int parts = few_parts(a);
   const int64_t items = a.p.n * a.p.heads_kv, keys = parts > 0 ? few_keys(a, parts) : 0;
   const size_t per = align_bytes(sizeof(FewLds<T, DP, NQ>) + table_bytes(a));
@@ -545,7 +552,7 @@ int launch_few(const Args &a, T *o, T *rest, float *lse, void *ws, hipStream_t s
 }
 
 template <typename T, int DP, int NQ, bool SHARE, int RW, int KW, bool SPLIT>
-int launch_fwd(const Args &a, T *o, T *rest, float *lse, hipStream_t s) {
+int launch_fwd(const Args &a, T *o, T *rest, float2 *lse, hipStream_t s) {
   const int64_t tiles = row_tiles(a, NQ, SHARE, RW);
   const size_t lds = std::max(buffers<FwdLds<T, DP, tile_keys<T>(KW)>>() * sizeof(FwdLds<T, DP, tile_keys<T>(KW)>) + table_bytes(a),
                               join_bytes(RW, KW, NQ, DP));
@@ -566,7 +573,8 @@ size_t forward_bytes(const Args &a) {
          sizeof(float) * size_t(a.p.n * a.p.heads_kv) * size_t(parts) * size_t(a.rows) * size_t(a.p.head_dim);
 }
 
-int run_forward(const Args &a, void *o, void *rest, float *lse, void *ws, hipStream_t s) {
+int run_forward(const Args &a, void *o, void *rest, float *stats, void *ws, hipStream_t s) {
+  float2 *lse = reinterpret_cast<float2 *>(stats);
   return by_instance(a.p, [&](auto t, auto dp) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;

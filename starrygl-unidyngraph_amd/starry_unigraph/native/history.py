@@ -268,7 +268,7 @@ class _Attend(torch.autograd.Function):
         N, Lq, Hq, dh = q.shape
         o = torch.empty(N, Lq, Hq, dh, dtype=q.dtype, device=dev)
         saves = lib.sgl_cross_attention_saves(ref) if need else 0
-        lse = torch.empty(N, Lq * Hq, dtype=torch.float32, device=dev) if saves & 1 else None
+        lse = torch.empty(N, Lq * Hq, 2, dtype=torch.float32, device=dev) if saves & 1 else None
         rest = torch.empty_like(o) if saves & 2 else None
         nb = lib.sgl_cross_attention_workspace_bytes(ref, 0)
         ws = _capi.workspace(nb, dev) if nb else None
