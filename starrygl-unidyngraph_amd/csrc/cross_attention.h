@@ -2,6 +2,8 @@
 // the three types, row tiles in LDS, distances to bias columns.
 #pragma once
 
+#include <cfloat>
+
 #include "history.h"
 
 namespace sgl {
@@ -386,15 +388,21 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 // The bias table of a key head's G heads in LDS, times log2 e; an odd stride,
-// so that two heads' values of a column lie in different banks.
+// so that two heads' values of a column lie in different banks. A finite value
+// stays finite: rows whose keys all have the type's lowest one are rows of
+// equal scores, as in a softmax that is not taken to base 2.
 __host__ __device__ __forceinline__ int table_ld(const Args &a) { return a.cols | 1; }
 __host__ __device__ __forceinline__ size_t table_bytes(const Args &a) {
   return a.cols == 0 ? 0 : sizeof(float) * size_t(a.G) * size_t(table_ld(a));
 }
+__device__ __forceinline__ float base2(float b) {
+  const float t = b * kLog2e;
+  return fabsf(t) == INFINITY && fabsf(b) != INFINITY ? copysignf(FLT_MAX, b) : t;
+}
 __device__ __forceinline__ void stage_bias(float *table, const Args &a, int hk, int tid, int threads) {
   for (int c = tid; c < a.G * a.cols; c += threads) {
     const int h = c / a.cols;
-    table[h * table_ld(a) + c - h * a.cols] = a.p.bias[int64_t(hk) * a.G * a.cols + c] * kLog2e;
+    table[h * table_ld(a) + c - h * a.cols] = base2(a.p.bias[int64_t(hk) * a.G * a.cols + c]);
   }
 }
 // x = x c + shift (+ the bias of each column) over blocks

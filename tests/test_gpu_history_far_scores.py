@@ -69,3 +69,39 @@ def test_a_rows_weights_sum_to_one_at_large_scores(ops, gpu, form):
     # p: a sum of Lk, two exponentials, a logarithm of at most 10 (2^-21 of it, times ln 2); dv: sums over the rows
     tol = ((Lk + Lq * Hq // Hkv + 16) * ho.F + 2.0 ** -20) * size
     assert ((dv.double().sum(1) - want).abs() <= tol).all(), ((dv.double().sum(1) - want).abs() / size).max()
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_buckets_at_the_types_lowest_value(ops, gpu, form, dtype):
+    """Keys after the query in buckets of float32's lowest value, a mask in the
+    table. Rows with an earlier key ignore them, to the bit as with -inf in the
+    table; rows with none weigh their keys equally (their scores differ by less
+    than the lowest value's last place), as a table of equal values over q = 0."""
+    t = _inputs(form, dtype)
+    t["q_pos"][1] = -1   # (sequence 1: every key lies after every query)
+    low = torch.finfo(FP32).min
+    t["bias"][:, :2], t["bias"][:, 2:] = torch.tensor([0.3, -0.2]), low
+    got = _run(ops, t, gpu)
+    t["bias"][:, 2:] = -math.inf
+    cut = _run(ops, t, gpu)
+    rest = torch.arange(form[0]) != 1
+    behind = (t["q_pos"][:, :, None] < t["k_pos"][:, None, :]).all(2)   # rows without an earlier key
+    keep = rest & ~behind.any(1)
+    for g, c in zip(got[:4], cut):
+        assert torch.equal(g[keep], c[keep])
+    t["bias"].zero_()
+    t["q"].zero_()
+    flat = _run(ops, t, gpu)
+    for i in (0, 3):   # o and dv: what does not depend on q itself
+        assert torch.equal(got[i][1], flat[i][1])
+    assert torch.isfinite(got[4]).all()
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_rows_of_minus_infinity_are_empty(ops, gpu, form):
+    """A table of -inf leaves a row nothing: zeros, as by the key mask."""
+    t = _inputs(form, FP32)
+    t["bias"].fill_(-math.inf)
+    for got in _run(ops, t, gpu):
+        assert not got.any()
