@@ -378,6 +378,40 @@ __device__ __forceinline__ float groups_max(float v) {
   auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
+// The largest magnitude of what is put in, over the lane and then the wave. By
+// the bits without the sign, which order as the magnitudes do (two 16-bit
+// elements an operation) and put NaN last, so that it is not passed over.
+template <typename T>
+struct Largest {
+  uint32_t bits = 0;
+  __device__ __forceinline__ void add(FragOf<T> f) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    const u32x4 w = __builtin_bit_cast(u32x4, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4)
+        bits = max(bits, w[i] & 0x7FFFFFFFu);
+      else
+        bits = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, bits),
+                                                                      __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu)));
+    }
+  }
+  __device__ __forceinline__ float wave() const {
+    uint32_t m = sizeof(T) == 4 ? bits : max(bits & 0xFFFFu, bits >> 16);
+    // rows of 16 lanes rotated by 8, 4, 2 and 1, then rows and halves of the wave swapped
+    m = max(m, uint32_t(__builtin_amdgcn_mov_dpp(int(m), 0x128, 0xF, 0xF, true)));
+    m = max(m, uint32_t(__builtin_amdgcn_mov_dpp(int(m), 0x124, 0xF, 0xF, true)));
+    m = max(m, uint32_t(__builtin_amdgcn_mov_dpp(int(m), 0x122, 0xF, 0xF, true)));
+    m = max(m, uint32_t(__builtin_amdgcn_mov_dpp(int(m), 0x121, 0xF, 0xF, true)));
+    auto h = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    m = max(h[0], h[1]);
+    auto q = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+    m = max(q[0], q[1]);
+    if constexpr (sizeof(T) == 4) return __uint_as_float(m);
+    else return float(__builtin_bit_cast(T, uint16_t(m)));
+  }
+};
 // The wave's index in its workgroup, as a scalar: what depends on it alone is
 // then uniform to the compiler too (scalar loads, addresses and branches).
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
@@ -443,15 +477,16 @@ template <typename T>
 constexpr float kProbUp = std::is_same_v<T, fp16_t> ? 1024.f : 1.f;
 
 // The bias gradient's cells in LDS: [column][slots] sums of ds for a set of row
-// blocks whose row c has one head, in fixed point (34 fractional bits in an
-// int64, 33 of them used, relative to a power of two near the largest |do|): integer adds give
+// blocks whose row c has one head, in fixed point: integer adds give
 // the same sum in any order, and the LDS adds them at 7 to 8 clocks an
 // instruction, four lanes a cell included, where float adds take 194 (3 a
-// lane; a read, an add and a write 11, in cells of a lane's own). A value
-// holds to 2^29 times that power; `seen`, the sum of magnitudes, tells beyond
-// it (and of NaN and infinities), and the gradient is NaN then.
-constexpr int kCellBits = 34;
-constexpr float kCellMax = 536870912.f;   // 2^29
+// lane; a read, an add and a write 11, in cells of a lane's own). The unit is
+// 2^-62 of a bound on everything that is added: |ds_ij| <= p_ij (|dp_ij| +
+// |D_i|), |dp_ij| and |D_i| are at most |do_i|_1 times the largest |v|, and a
+// row's p sum to one, so no sum of any of the terms exceeds 2 max|v| sum |do|
+// (twice which a cell holds). A term 2^38 times smaller than that still has the
+// 24 bits of a float.
+constexpr int kCellBits = 32;   // fractional bits of a term times the power of two
 typedef unsigned long long Cell;
 // Cells a column: lane c of 16 adds into cell c mod slots; 8 where they
 // keep the heads apart (row c has head c mod heads), else 16.
@@ -459,25 +494,31 @@ __host__ __device__ __forceinline__ int cell_slots(int heads) { return heads <= 
 __device__ __forceinline__ void clear_cells(Cell *cells, int n, int tid, int threads) {
   for (int i = tid; i < n; i += threads) cells[i] = 0;
 }
+// The cells' power of two for sums of magnitudes up to `most`: below 2^30 (1
+// for 0 and what is not finite).
+__device__ __forceinline__ float cell_scale(float most) {
+  return most > 0.f && most < INFINITY ? ldexpf(1.f, min(29 - ilogbf(most), 127)) : 1.f;
+}
 template <int N>
 __device__ __forceinline__ void add_cells(Cell *cells, const int (&col)[N][4], const float (&x)[N][4], int slots,
-                                          float up, float &seen) {
+                                          float up) {
   const int c = threadIdx.x & (slots - 1);
-  const float f = up * 4.f;   // 2^34 = 2^2 2^32
 #pragma unroll
   for (int k = 0; k < N; ++k)
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       // the nearest integer and a signed rest, which is exact (from the integer below, a small negative value's
       // rest lies next to one and has lost its digits)
-      const float t = x[k][v] * f, hi = rintf(t);
-      seen += fabsf(t);
+      const float t = x[k][v] * up, hi = rintf(t);
       const int lo = int((t - hi) * 2147483648.f);   // in units of 2^-31 of t, so two of a cell's
       const Cell val = (Cell(uint32_t(int(hi) + (lo >> 31))) << 32) | (uint32_t(lo) << 1);
       __hip_atomic_fetch_add(cells + col[k][v] * slots + c, val, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
 }
-__device__ __forceinline__ bool cells_hold(float seen) { return seen < 4.f * kCellMax; }
+// What the cells' sum t is worth.
+__device__ __forceinline__ float cell_value(long long t, float up) {
+  return float(double(t) * (1.0 / double(1ll << kCellBits)) / double(up));
+}
 // Waves a SIMD that a kernel's registers leave room for (512 of them): asked of
 // the compiler, which otherwise spends registers on loads it could not issue
 // earlier anyway (two 8-wave workgroups a CU need 4).

@@ -13,9 +13,45 @@ namespace {
 // one tile it is the sum of p dp itself, which cancels exactly (a single key
 // has no gradient). The table's gradient is summed in 64-bit cells of fixed
 // point in LDS (a float atomic of LDS costs 194 clocks a wave, an integer one
-// 8), 34 bits below a power of two near the workgroup's largest |do|; sums that
-// would not fit are NaN. 8 sequences, 8 heads of 64, 1000 x 2049 in bf16: 185
+// 8), relative to a bound on their sum; where that is not finite (a do, v or
+// score that is not, or magnitudes whose product overflows) the workgroup's
+// part is NaN. 8 sequences, 8 heads of 64, 1000 x 2049 in bf16: 185
 // us; workgroups of 4 waves instead of 8: 202.
+
+// The largest |v| of the live keys of a (sequence, key head), a part of its
+// keys a workgroup: what bounds the cells. A kernel of its own, 5 us: it reads
+// v once, where every row tile's workgroup would have to before its first cell.
+inline int vmost_parts(const Args &a) {   // (a workgroup's four loads a thread, 64 workgroups at most)
+  const int dp = a.p.head_dim <= 32 ? 32 : a.p.head_dim <= 64 ? 64 : 128, e = a.p.dtype == SGL_FP32 ? 4 : 8;
+  const int64_t keys = 4 * kBlock * e / dp;
+  return int(std::min<int64_t>(64, (a.p.lk + keys - 1) / keys));
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kBlock) void k_attn_vmost(Args a, int parts, float *__restrict__ vmost) {
+  using L = Tile<T, DP>;
+  constexpr int E = Mma<T>::E, RPB = kBlock / L::UPR, U = 4;
+  __shared__ uint32_t red[kWaves];
+  const TileAt at_ = tile_at(blockIdx.x, uint32_t(parts), a.p.heads_kv);
+  const Seq<T> q = seq_of<T>(a.p, at_.n, at_.hk, a.G);
+  const int r0 = threadIdx.x / L::UPR, d = (threadIdx.x % L::UPR) * E, w = wave_index();
+  Largest<T> most;
+  for (int64_t j0 = int64_t(at_.tile) * (RPB * U); j0 < q.klen; j0 += int64_t(parts) * (RPB * U)) {
+    FragOf<T> f[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t j = j0 + u * RPB + r0;
+      f[u] = load_raw<T>(q.v + j * a.p.v_t, key_live(q, a.p, j), d, a.p.head_dim);   // (a last vector's overlap is v too)
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) most.add(f[u]);
+  }
+  const float x = most.wave();
+  if ((threadIdx.x & 63) == 0) red[w] = __float_as_uint(x);   // (as bits: NaN is the largest)
+  __syncthreads();
+  if (threadIdx.x == 0) vmost[blockIdx.x] = __uint_as_float(max(max(red[0], red[1]), max(red[2], red[3])));
+}
+
 template <typename T, int DP, int TK>
 struct alignas(16) DqLds {
   T k[TK * Tile<T, DP>::LD], v[TK * Tile<T, DP>::LD];
@@ -39,7 +75,8 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
                                                           const T *__restrict__ rest, const float2 *__restrict__ lse,
                                                           const T *__restrict__ go, T *__restrict__ dq,
                                                           float *__restrict__ rowdelta, float *__restrict__ rowmost,
-                                                          float *__restrict__ part) {
+                                                          float *__restrict__ part,
+                                                          const float *__restrict__ vmost, int vparts) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   constexpr int TK = tile_keys<T>(KW), BLOCK = RW * KW * 64, WAVES = RW * KW;
@@ -76,7 +113,7 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
   FragOf<T> qf[NQ][ST], gf[NQ][ST];
   int64_t qpos[NP];
   int qrel[NP];
-  float delta[NQ], gs[NQ], top = 0.f;
+  float delta[NQ], gs[NQ], size = 0.f;   // size: this lane's share of the rows' |do|_1
   float2 ls[NQ];
   const int64_t base = biased && any ? scalar_load(q.qpos + int64_t(i0) * p.qpos_t) : 0;
   const int64_t stat0 = (n * p.heads_kv + hk) * a.rows;
@@ -88,7 +125,7 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
     in[b] = row[b].i < p.lq;
     ok[b] = row[b].i < q.qlen;
     const int64_t at = out_row(a, n, hk, row[b].i, row[b].h);
-    float most = 0.f;
+    float most = 0.f, sum = 0.f;
     delta[b] = 0.f;
 #pragma unroll
     for (int st = 0; st < ST; ++st) {
@@ -96,7 +133,10 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
       qf[b][st] = load_row<T>(q.q + int64_t(row[b].i) * p.q_t + row[b].h * p.q_h, ok[b], d, dh);
       gf[b][st] = load_row<T>(go + at, ok[b], d, dh);
 #pragma unroll
-      for (int e = 0; e < M::E; ++e) most = fmaxf(most, fabsf(float(gf[b][st][e])));
+      for (int e = 0; e < M::E; ++e) {
+        most = fmaxf(most, fabsf(float(gf[b][st][e])));
+        sum += fabsf(float(gf[b][st][e]));
+      }
       if (!one_tile) {
         const FragOf<T> of = load_row<T>(o + at, ok[b], d, dh);
         FragOf<T> rf = zero_frag<T>();
@@ -107,10 +147,11 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
     }
     delta[b] = groups_sum(delta[b]);
     most = groups_max(most);
-    top = fmaxf(top, most);
     gs[b] = grad_scale<T>(most);
     const int64_t r = stat0 + int64_t(row[b].i) * a.G + row[b].h;
     ls[b] = ok[b] ? lse[r] : make_float2(INFINITY, 0.f);
+    // (rows without p count for nothing, whatever their do; a NaN score for NaN)
+    if (w % KW == 0) size += ls[b].y != ls[b].y ? NAN : ls[b].x == INFINITY ? 0.f : sum;
     if (g == 0 && in[b] && w % KW == 0) {   // for dk and dv
       rowdelta[r] = delta[b];
       if (std::is_same_v<T, fp16_t>) rowmost[r] = most;
@@ -123,15 +164,19 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
   }
   qnear = __all(qnear);
   const float c = p.scale * kLog2e;
-  float up = 1.f, seen = 0.f;   // the cells' power of two, for the whole workgroup
+  float up = 1.f, bad = 0.f;   // the cells' power of two, for the whole workgroup; NaN if they cannot hold
   if (part != nullptr) {
-#pragma unroll
-    for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
-    if (lane == 0) sx.red[w] = top;
+    Largest<float> vm;
+    if (lane < vparts) vm.bits = __float_as_uint(vmost[(n * p.heads_kv + hk) * vparts + lane]);
+    size = wave_reduce_sum(size);
+    if (lane == 0) sx.red[w] = size;
     __syncthreads();
+    size = 0.f;
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) top = fmaxf(top, sx.red[i]);
-    up = unit_scale(top);
+    for (int i = 0; i < WAVES; ++i) size += sx.red[i];
+    const float most = 2.f * vm.wave() * size;
+    up = cell_scale(most);
+    bad = most < INFINITY ? 0.f : NAN;
   }
   f32x4 acc[NQ][DB];
 #pragma unroll
@@ -239,7 +284,7 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
 #pragma unroll
       for (int b = 0; b < NQ; ++b) {
         const int set = sets == RW * NQ ? wr * NQ + b : SHARE ? b : 0;
-        add_cells(cells + set * a.cols * slots, col[b < NP ? b : 0], y[b], slots, up, seen);
+        add_cells(cells + set * a.cols * slots, col[b < NP ? b : 0], y[b], slots, up);
       }
     }
     if constexpr (std::is_same_v<T, fp16_t>) {
@@ -266,13 +311,7 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
   if (part != nullptr) {
     // cell (set, column, slot) belongs to the head of its blocks' row `slot`: a
     // thread sums a (head, column) over them
-    const bool held = __all(cells_hold(seen));
     __syncthreads();
-    if (lane == 0) sx.red[w] = held ? 0.f : NAN;
-    __syncthreads();
-    float bad = 0.f;
-#pragma unroll
-    for (int i = 0; i < WAVES; ++i) bad += sx.red[i];
     const bool own = sets == RW * NQ;
     float *out = part + ((n * tiles + rt) * p.heads_kv + hk) * a.G * a.cols;
     for (int x = threadIdx.x; x < a.G * a.cols; x += BLOCK) {
@@ -287,7 +326,7 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
             t += static_cast<long long>(cells[(set * a.cols + cidx) * slots + e]);
         }
       }
-      out[x] = float(double(t) * (1.0 / double(1ll << kCellBits)) / double(up)) + bad;
+      out[x] = cell_value(t, up) + bad;
     }
   }
   if constexpr (KW > 1) {
@@ -583,7 +622,10 @@ int64_t dq_tiles(const Args &a) {
 
 template <typename T, int DP, int NQ, bool SHARE, int RW, int KW>
 int launch_dq(const Args &a, int64_t tiles, const void *o, const void *rest, const float2 *lse, const void *go, void *dq,
-              float *stat, float *part, hipStream_t s) {
+              float *stat, float *part, float *vmost, hipStream_t s) {
+  const int vparts = vmost_parts(a);
+  if (part != nullptr && vparts > 0)
+    launch(&k_attn_vmost<T, DP>, dim3(unsigned(a.p.n * a.p.heads_kv * vparts)), dim3(kBlock), 0, s, a, vparts, vmost);
   const size_t lds = std::max(
       align_bytes(buffers<DqLds<T, DP, tile_keys<T>(KW)>>() * sizeof(DqLds<T, DP, tile_keys<T>(KW)>) +
                   sizeof(DqSums<RW * KW * NQ * 16>) + table_bytes(a)) +
@@ -593,7 +635,7 @@ int launch_dq(const Args &a, int64_t tiles, const void *o, const void *rest, con
   SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_dq<T, DP, NQ, SHARE, RW, KW>), lds));
   launch(&k_attn_dq<T, DP, NQ, SHARE, RW, KW>, dim3(unsigned(a.p.n * a.p.heads_kv * tiles)), dim3(RW * KW * kWave), lds,
          s, a, tiles, static_cast<const T *>(o), static_cast<const T *>(rest), lse, static_cast<const T *>(go),
-         static_cast<T *>(dq), stat, most_of(a, stat), part);
+         static_cast<T *>(dq), stat, most_of(a, stat), part, static_cast<const float *>(vmost), vparts);
   SGL_CHECK_LAUNCH();
   return SGL_OK;
 }
@@ -613,10 +655,14 @@ int launch_dkv(const Args &a, const float2 *lse, const void *go, float *stat, vo
   return SGL_OK;
 }
 
+size_t part_bytes(const Args &a) {
+  return align_up(sizeof(float) * size_t(a.p.n * dq_tiles(a)) * a.p.heads_q * a.cols);
+}
+
 }  // namespace
 
 size_t backward_bytes(const Args &a) {
-  return stat_bytes(a) + sizeof(float) * size_t(a.p.n * dq_tiles(a)) * a.p.heads_q * a.cols;
+  return stat_bytes(a) + part_bytes(a) + (a.cols > 0 ? sizeof(float) * size_t(a.p.n * a.p.heads_kv) * vmost_parts(a) : 0);
 }
 
 int run_backward(const Args &a, const void *o, const void *rest, const float *stats, const void *go, void *dq, void *dk,
@@ -624,16 +670,17 @@ int run_backward(const Args &a, const void *o, const void *rest, const float *st
   const float2 *lse = reinterpret_cast<const float2 *>(stats);
   float *stat = static_cast<float *>(ws);
   float *part = dbias != nullptr ? reinterpret_cast<float *>(static_cast<char *>(ws) + stat_bytes(a)) : nullptr;
+  float *vmost = dbias != nullptr ? reinterpret_cast<float *>(static_cast<char *>(ws) + stat_bytes(a) + part_bytes(a)) : nullptr;
   const int64_t tiles = dq_tiles(a);
   return by_instance(a.p, [&](auto t, auto dp) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
     if (tiles > 0) {
       int rc;
-      if (!many_rows(a)) rc = launch_dq<T, DP, 1, false, 1, 4>(a, tiles, o, rest, lse, go, dq, stat, part, s);
-      else if constexpr (!two_blocks<T, DP>()) rc = launch_dq<T, DP, 1, false, 4, 2>(a, tiles, o, rest, lse, go, dq, stat, part, s);
-      else if (a.G % 2 == 0) rc = launch_dq<T, DP, 2, true, 4, 2>(a, tiles, o, rest, lse, go, dq, stat, part, s);
-      else rc = launch_dq<T, DP, 2, false, 4, 2>(a, tiles, o, rest, lse, go, dq, stat, part, s);
+      if (!many_rows(a)) rc = launch_dq<T, DP, 1, false, 1, 4>(a, tiles, o, rest, lse, go, dq, stat, part, vmost, s);
+      else if constexpr (!two_blocks<T, DP>()) rc = launch_dq<T, DP, 1, false, 4, 2>(a, tiles, o, rest, lse, go, dq, stat, part, vmost, s);
+      else if (a.G % 2 == 0) rc = launch_dq<T, DP, 2, true, 4, 2>(a, tiles, o, rest, lse, go, dq, stat, part, vmost, s);
+      else rc = launch_dq<T, DP, 2, false, 4, 2>(a, tiles, o, rest, lse, go, dq, stat, part, vmost, s);
       if (rc != SGL_OK) return rc;
     }
     if (dbias != nullptr) sum_rows(part, a.p.n * tiles, a.p.heads_q * a.cols, dbias, s);

@@ -59,7 +59,8 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
   const Buckets bk = buckets_of(p);
   if (biased) stage_bias(table, a, hk, lane, kWave);
   if (part != nullptr) clear_cells(cells, sets * slots * a.cols, lane, kWave);
-  float up = 0.f, seen = 0.f;   // the cells' power of two (0: nothing in them yet)
+  // the cells' power of two (0: nothing in them yet), the bound on all that was added, NaN if they cannot hold
+  float up = 0.f, reach = 0.f, bad = 0.f;
   wave_sync();
   RowAt row[NQ];
 #pragma unroll
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
     int64_t qpos[NQ];
     int qrel[NQ];
     bool ok[NQ];
-    float most = 0.f;
+    Largest<T> gm, vm;   // |do|, |v|
 #pragma unroll
     for (int b = 0; b < NQ; ++b) {
       ok[b] = row[b].i < q.qlen;
@@ -126,29 +127,12 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
         const int d = st * M::KS + g * M::E;
         qf[b][st] = fix<T>(qf[b][st], d, dh);
         gf[b][st] = fix<T>(gf[b][st], d, dh);
-#pragma unroll
-        for (int e = 0; e < M::E; ++e) most = fmaxf(most, fabsf(float(gf[b][st][e])));
+        gm.add(gf[b][st]);
         *reinterpret_cast<FragOf<T> *>(s.b + (b * 16 + cl) * L::LD + d) = gf[b][st];
       }
     float gs = 1.f;
-    if (std::is_same_v<T, fp16_t> || part != nullptr) {
-#pragma unroll
-      for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, kWave));
-      gs = grad_scale<T>(most);
-    }
-    if (part != nullptr && most > 0.f) {   // (uniform) larger gradients than the cells' power is for: cells shifted
-      const float want = unit_scale(most);
-      if (up == 0.f) {
-        up = want;
-      } else if (want < up) {
-        const int by = min(ilogbf(up) - ilogbf(want), 63);
-        for (int i = lane; i < sets * slots * a.cols; i += kWave)
-          cells[i] = Cell(static_cast<long long>(cells[i]) >> by);
-        seen = ldexpf(seen, -by);
-        up = want;
-        wave_sync();
-      }
-    }
+    const float most = gm.wave();
+    gs = grad_scale<T>(most);
     // scores and dp, (keys x rows)
     float x[NQ][NK][4], y[NQ][NK][4];
     int col[NQ][NK][4];
@@ -165,6 +149,7 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
         kf[kb][st] = fix<T>(kf[kb][st], d, dh);
         vf[kb][st] = fix<T>(vf[kb][st], d, dh);
         if (q.mask != nullptr && !on_r) kf[kb][st] = vf[kb][st] = zero_frag<T>();
+        vm.add(vf[kb][st]);
         *reinterpret_cast<FragOf<T> *>(s.a + (kb * 16 + cl) * L::LD + d) = kf[kb][st];
       }
 #pragma unroll
@@ -180,6 +165,22 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
           x[b][kb][v] = sc[v];
           y[b][kb][v] = dp[v];
         }
+      }
+    }
+    if (part != nullptr && live != 0) {   // (uniform) beyond what the cells' power is for: cells shifted
+      // (each row's |do|_1 by dh times the largest |do|)
+      reach += 2.f * vm.wave() * (most * float(a.rows * dh));
+      const float want = cell_scale(reach);
+      if (!(reach < INFINITY)) {
+        bad = NAN;
+      } else if (up == 0.f) {
+        up = reach > 0.f ? want : 0.f;
+      } else if (want < up) {
+        const int by = min(ilogbf(up) - ilogbf(want), 63);
+        for (int i = lane; i < sets * slots * a.cols; i += kWave)
+          cells[i] = Cell(static_cast<long long>(cells[i]) >> by);
+        up = want;
+        wave_sync();
       }
     }
     // p, D and ds
@@ -205,6 +206,7 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
         }
       sum = groups_sum(sum);
       const float inv = ok[b] && sum != 0.f ? 1.f / sum : 0.f;   // (NaN stays)
+      if (ok[b] && sum != sum) bad = NAN;
 #pragma unroll
       for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
@@ -218,7 +220,7 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
 #pragma unroll
         for (int v = 0; v < 4; ++v)   // (0 at a dead key also where do, and with it D, is not finite)
           y[b][kb][v] = (live >> (kb * 16 + 4 * g + v)) & 1 ? x[b][kb][v] * (y[b][kb][v] - de) : 0.f;
-      if (part != nullptr) add_cells(cells + (sets == 1 ? 0 : b) * slots * a.cols, col[b], y[b], slots, up, seen);
+      if (part != nullptr) add_cells(cells + (sets == 1 ? 0 : b) * slots * a.cols, col[b], y[b], slots, up);
       if constexpr (std::is_same_v<T, fp16_t>) {
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb)
@@ -315,7 +317,7 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
   }
   if (part != nullptr) {
     wave_sync();
-    const bool held = __all(cells_hold(seen));
+    const bool held = __all(bad == 0.f);
     float *out = part + (first * p.heads_kv + hk) * a.G * a.cols;
     for (int x = lane; x < a.G * a.cols; x += kWave) {
       const int h = x / a.cols, cidx = x - h * a.cols;
@@ -325,7 +327,7 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
           const int e = (i + cidx) & (slots - 1);
           if ((set * 16 + e) % a.G == h) t += static_cast<long long>(cells[(set * a.cols + cidx) * slots + e]);
         }
-      out[x] = held ? float(double(t) * (1.0 / double(1ll << kCellBits)) / double(up == 0.f ? 1.f : up)) : NAN;
+      out[x] = held ? cell_value(t, up == 0.f ? 1.f : up) : NAN;
     }
   }
 }

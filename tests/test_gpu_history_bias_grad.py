@@ -48,10 +48,11 @@ def _even(form, dtype, value, grads):
     return t, want
 
 
-def _dbias(ops, t, dev):
+def _dbias(ops, t, dev, resolution=0):
     d = {k: x.to(dev) for k, x in t.items()}
     d["bias"].requires_grad_()
-    o = ops.cross_attention(d["q"], d["k"], d["v"], bias=d["bias"], q_pos=d["q_pos"], k_pos=d["k_pos"])
+    o = ops.cross_attention(d["q"], d["k"], d["v"], bias=d["bias"], q_pos=d["q_pos"], k_pos=d["k_pos"],
+                            resolution=resolution)
     return torch.autograd.grad(o, d["bias"], d["go"])[0].cpu().double()
 
 
@@ -68,3 +69,55 @@ def test_small_negative_terms_count_as_positive_ones_do(ops, gpu, form, dtype, v
     t, want = _even(form, dtype, value, torch.ones(form[1]))
     got = _dbias(ops, t, gpu)
     assert ((got - want).abs() <= TOL * want.abs()).all(), (got, want)
+
+
+@pytest.mark.parametrize("value, grad", [(2.0 ** -40, 1.0), (2.0 ** -100, 1.0), (2.0 ** -30, 2.0 ** -50),
+                                         (2.0 ** 26, 1.0), (2.0 ** 28, 1.0), (2.0 ** 60, 2.0 ** 30), (2.0 ** 30, 2.0 ** -60)])
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_sums_of_any_magnitude(ops, gpu, form, dtype, value, grad):
+    """Neither lost below the cells' last place nor wrapped above their first:
+    a cell is shared by many lanes and waves, and all of them add to one here."""
+    t, want = _even(form, dtype, value, torch.full((form[1],), grad))
+    got = _dbias(ops, t, gpu)
+    assert ((got - want).abs() <= TOL * want.abs()).all(), (got, want)
+
+
+@pytest.mark.parametrize("big", [2.0 ** 10, 2.0 ** 20])
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_one_rows_large_gradient_leaves_the_others(ops, gpu, form, dtype, big):
+    """Row 0's gradient is far larger and its distances have columns of their
+    own: the other columns are as exact beside it as alone."""
+    if dtype == FP16:
+        big = min(big, 2.0 ** 15)
+    grads = torch.ones(form[1])
+    grads[0] = big
+    t, want = _even(form, dtype, 2.0 ** -6, grads)
+    t["q_pos"][:, 0] = 12   # distances 2 and 3, with two buckets an octave columns 2 and 3
+    far = want[:, :2] * big / float(grads.double().sum())
+    want[:, :2] -= far
+    want[:, 2:] = far
+    got = _dbias(ops, t, gpu, resolution=1)
+    assert ((got - want).abs() <= TOL * want.abs()).all(), (got, want)
+
+
+@pytest.mark.parametrize("std", [1e-6, 1e-4, 1e-2, 1.0, 1e3, 1e6])
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("case", [(5, 6, 40, 4, 2, 24), (3, 70, 150, 4, 2, 24), (30, 128, 130, 4, 1, 24)], ids=str)
+def test_values_of_any_deviation(ops, gpu, case, dtype, std):
+    """Random inputs, values scaled: within the bounds of float32 products and
+    sums, as at a deviation of one."""
+    N, Lq, Lk, Hq, Hkv, dh = case
+    g = torch.Generator().manual_seed(Lk)
+    r = lambda *s: torch.randn(*s, generator=g)
+    t = dict(q=r(N, Lq, Hq, dh), k=r(N, Lk, Hkv, dh), v=r(N, Lk, Hkv, dh) * std, go=r(N, Lq, Hq, dh))
+    t = {k: x.to(dtype) for k, x in t.items()}
+    t["bias"] = r(Hq, 12)
+    t["q_pos"], t["k_pos"] = (torch.randint(0, 3000, (N, L), generator=g) for L in (Lq, Lk))
+    cols = ho.columns(t["q_pos"], t["k_pos"], 12, 0, False)
+    wide = {k: x.float() if k in ("q", "k", "v", "go") else x for k, x in t.items() if k not in ("q_pos", "k_pos")}
+    want, bound = ho.attend(**wide, cols=cols)
+    got = _dbias(ops, t, gpu)
+    bad = ~((got - want["dbias"]).abs() <= bound["dbias"])
+    assert not bad.any(), float(((got - want["dbias"]).abs() / bound["dbias"]).max())
