@@ -461,16 +461,35 @@ __device__ __forceinline__ void scale_scores(float (&x)[NB][4], float c, float s
   }
 }
 
-// A power of two near 1 / most (1 for 0 and what is not finite).
-__device__ __forceinline__ float unit_scale(float most) {
-  return most > 0.f && most < INFINITY ? ldexpf(1.f, -max(ilogbf(most), -126)) : 1.f;
+// fp16: ds goes into a product times a power of two that follows its largest
+// magnitude so far, whatever do, v and p are of: from a start that any value
+// passes, ds beyond 2^15 (the type ends at 2^16) brings the largest to 2^10, and
+// what was summed at the old power is rescaled. The normal numbers then reach
+// 2^24 below the largest term of a sum.
+constexpr float kFirstScale = 0x1p100f, kMostHalf = 32768.f;
+__device__ __forceinline__ float half_scale(float most) {   // (1 for what is not finite)
+  return most < INFINITY ? ldexpf(1.f, min(10 - ilogbf(most), 100)) : 1.f;
 }
-
-// fp16 gradients: a power of two that brings the largest |do| near one, so
-// that ds keeps fp16's digits whatever the loss is scaled by.
-template <typename T>
-__device__ __forceinline__ float grad_scale(float most) {
-  return std::is_same_v<T, fp16_t> ? unit_scale(most) : 1.f;
+// Blocks' y = ds of a lane's column (a row or key that four lane groups share)
+// times that power, the accumulators with it.
+template <int NB, int DB>
+__device__ __forceinline__ void follow_scale(float (&y)[NB][4], float &scale, f32x4 (&acc)[DB]) {
+  float most = 0.f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) most = fmaxf(most, fabsf(y[b][v]));
+  if (__any(most * scale > kMostHalf)) {   // (uniform over the wave; the first terms, then seldom)
+    most = groups_max(most);
+    const float now = most * scale > kMostHalf ? half_scale(most) : scale;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[d] *= now / scale;
+    scale = now;
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) y[b][v] *= scale;
 }
 // fp16: p goes into a product as 2^10 p, away from the subnormals.
 template <typename T>

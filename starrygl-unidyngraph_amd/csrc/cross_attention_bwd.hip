@@ -74,8 +74,7 @@ template <typename T, int DP, int NQ, bool SHARE, int RW, int KW>
 __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t tiles, const T *__restrict__ o,
                                                           const T *__restrict__ rest, const float2 *__restrict__ lse,
                                                           const T *__restrict__ go, T *__restrict__ dq,
-                                                          float *__restrict__ rowdelta, float *__restrict__ rowmost,
-                                                          float *__restrict__ part,
+                                                          float *__restrict__ rowdelta, float *__restrict__ part,
                                                           const float *__restrict__ vmost, int vparts) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
@@ -113,7 +112,7 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
   FragOf<T> qf[NQ][ST], gf[NQ][ST];
   int64_t qpos[NP];
   int qrel[NP];
-  float delta[NQ], gs[NQ], size = 0.f;   // size: this lane's share of the rows' |do|_1
+  float delta[NQ], size = 0.f;   // size: this lane's share of the rows' |do|_1
   float2 ls[NQ];
   const int64_t base = biased && any ? scalar_load(q.qpos + int64_t(i0) * p.qpos_t) : 0;
   const int64_t stat0 = (n * p.heads_kv + hk) * a.rows;
@@ -125,7 +124,7 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
     in[b] = row[b].i < p.lq;
     ok[b] = row[b].i < q.qlen;
     const int64_t at = out_row(a, n, hk, row[b].i, row[b].h);
-    float most = 0.f, sum = 0.f;
+    float sum = 0.f;
     delta[b] = 0.f;
 #pragma unroll
     for (int st = 0; st < ST; ++st) {
@@ -133,10 +132,7 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
       qf[b][st] = load_row<T>(q.q + int64_t(row[b].i) * p.q_t + row[b].h * p.q_h, ok[b], d, dh);
       gf[b][st] = load_row<T>(go + at, ok[b], d, dh);
 #pragma unroll
-      for (int e = 0; e < M::E; ++e) {
-        most = fmaxf(most, fabsf(float(gf[b][st][e])));
-        sum += fabsf(float(gf[b][st][e]));
-      }
+      for (int e = 0; e < M::E; ++e) sum += fabsf(float(gf[b][st][e]));
       if (!one_tile) {
         const FragOf<T> of = load_row<T>(o + at, ok[b], d, dh);
         FragOf<T> rf = zero_frag<T>();
@@ -146,16 +142,11 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
       }
     }
     delta[b] = groups_sum(delta[b]);
-    most = groups_max(most);
-    gs[b] = grad_scale<T>(most);
     const int64_t r = stat0 + int64_t(row[b].i) * a.G + row[b].h;
     ls[b] = ok[b] ? lse[r] : make_float2(INFINITY, 0.f);
     // (rows without p count for nothing, whatever their do; a NaN score for NaN)
     if (w % KW == 0) size += ls[b].y != ls[b].y ? NAN : ls[b].x == INFINITY ? 0.f : sum;
-    if (g == 0 && in[b] && w % KW == 0) {   // for dk and dv
-      rowdelta[r] = delta[b];
-      if (std::is_same_v<T, fp16_t>) rowmost[r] = most;
-    }
+    if (g == 0 && in[b] && w % KW == 0) rowdelta[r] = delta[b];   // for dk and dv
     if (b < NP) {
       qpos[b] = biased && ok[b] ? q.qpos[int64_t(row[b].i) * p.qpos_t] : base;
       qnear = qnear && is_near(qpos[b] - base);
@@ -179,10 +170,13 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
     bad = most < INFINITY ? 0.f : NAN;
   }
   f32x4 acc[NQ][DB];
+  float gs[NQ];   // (fp16) what ds of this wave's rows is multiplied by
 #pragma unroll
-  for (int b = 0; b < NQ; ++b)
+  for (int b = 0; b < NQ; ++b) {
+    gs[b] = kFirstScale;
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   KeyTile<T, DP, TK, BLOCK> tile(a);
   if (any && q.klen > 0) tile.load(q, a, 0);
   int buf = 0;
@@ -289,11 +283,7 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
     }
     if constexpr (std::is_same_v<T, fp16_t>) {
 #pragma unroll
-      for (int b = 0; b < NQ; ++b)
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) y[b][kb][v] *= gs[b];
+      for (int b = 0; b < NQ; ++b) follow_scale(y[b], gs[b], acc[b]);
     }
 #pragma unroll
     for (int st = 0; st < KB * 16 / M::KS; ++st) {
@@ -329,6 +319,12 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
       out[x] = cell_value(t, up) + bad;
     }
   }
+  if constexpr (std::is_same_v<T, fp16_t>) {
+#pragma unroll
+    for (int b = 0; b < NQ; ++b)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) acc[b][d] *= 1.f / gs[b];
+  }
   if constexpr (KW > 1) {
     float *pr = reinterpret_cast<float *>(smem);
     __syncthreads();
@@ -340,10 +336,9 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
 #pragma unroll
   for (int b = 0; b < NQ; ++b) {
     if (!in[b]) continue;
-    const float f = p.scale / gs[b];
     const int64_t at = out_row(a, n, hk, row[b].i, row[b].h);
 #pragma unroll
-    for (int d = 0; d < DB; ++d) store4(dq + at, d * 16 + 4 * g, dh, acc[b][d] * f);
+    for (int d = 0; d < DB; ++d) store4(dq + at, d * 16 + 4 * g, dh, acc[b][d] * p.scale);
   }
 }
 
@@ -372,19 +367,17 @@ template <typename T, int DP, bool SHARE, int CW, int RS>
 __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2))) void k_attn_dkv(Args a, int64_t tiles, const T *__restrict__ go,
                                                            const float2 *__restrict__ lse,
                                                            const float *__restrict__ rowdelta,
-                                                           const float *__restrict__ rowmost, T *__restrict__ dk,
-                                                           T *__restrict__ dv) {
+                                                           T *__restrict__ dk, T *__restrict__ dv) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
-  constexpr int TR = kRows * RS, BLOCK = CW * RS * 64, WAVES = CW * RS;
+  constexpr int TR = kRows * RS, BLOCK = CW * RS * 64;
   using S = DkvLds<T, DP, TR>;
   constexpr int NB = buffers<S>();
   constexpr int ST = DP / M::KS, DB = DP / 16, RB = kRows / 16, NP = SHARE ? 1 : RB;
   constexpr bool kHalf = std::is_same_v<T, fp16_t>;
   extern __shared__ __align__(16) char smem[];
   S *const bufs = reinterpret_cast<S *>(smem);
-  float *red = reinterpret_cast<float *>(smem + NB * sizeof(S));
-  float *table = red + 8;
+  float *table = reinterpret_cast<float *>(smem + NB * sizeof(S));
   const sgl_attention &p = a.p;
   const int dh = p.head_dim;
   const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4;
@@ -403,19 +396,6 @@ __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2
   const uint32_t pairs = uint32_t(a.G) >> 1, qlen = uint32_t(q.qlen);
   const bool any = kt * CW * 16 < q.klen;
   const uint32_t steps = !any ? 0 : SHARE ? (qlen + 15) / 16 * pairs : (qlen * a.G + kRows - 1) / kRows;
-  float gs = 1.f;
-  if constexpr (kHalf) {
-    float most = 0.f;
-    if (any)
-      for (uint32_t r = threadIdx.x; r < qlen * a.G; r += BLOCK) most = fmaxf(most, rowmost[stat0 + r]);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, kWave));
-    if (lane == 0) red[w] = most;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < WAVES; ++i) most = fmaxf(most, red[i]);
-    gs = grad_scale<T>(most);
-  }
   FragOf<T> kf[ST], vf[ST];
 #pragma unroll
   for (int st = 0; st < ST; ++st) {
@@ -428,7 +408,7 @@ __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2
   const int krel = int(kp - base);
   const bool knear = __all(is_near(kp - base));
   const float c = p.scale * kLog2e;
-  const float dsf = gs / kProbUp<T>;
+  float gs = kFirstScale;   // (fp16) what ds of this wave's keys is multiplied by
   f32x4 acc[2][DB];   // dk, dv
 #pragma unroll
   for (int b = 0; b < DB; ++b) acc[0][b] = acc[1][b] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -571,10 +551,11 @@ __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2
     for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        const float pr = on ? __builtin_amdgcn_exp2f((x[rb][v] - mov[rb][v]) - suv[rb][v]) * kProbUp<T> : 0.f;
-        x[rb][v] = pr;
-        y[rb][v] = pr * ((y[rb][v] - dev[rb][v]) * dsf);
+        const float pr = on ? __builtin_amdgcn_exp2f((x[rb][v] - mov[rb][v]) - suv[rb][v]) : 0.f;
+        x[rb][v] = pr * kProbUp<T>;
+        y[rb][v] = pr * (y[rb][v] - dev[rb][v]);
       }
+    if constexpr (kHalf) follow_scale(y, gs, acc[0]);
 #pragma unroll
     for (int st = 0; st < kRows / M::KS; ++st) {
       const FragOf<T> pf = frag_of<T>(x, st), df = frag_of<T>(y, st);
@@ -584,6 +565,10 @@ __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2
         acc[1][b] = M::mma(L::template frag_t<kRows>(s.go, b * 16, x0 + st * M::KS), pf, acc[1][b]);
       }
     }
+  }
+  if constexpr (kHalf) {
+#pragma unroll
+    for (int b = 0; b < DB; ++b) acc[0][b] *= 1.f / gs;
   }
   if constexpr (RS > 1) {
     float *pr = reinterpret_cast<float *>(smem);
@@ -595,7 +580,7 @@ __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2
   }
   if (j >= p.lk) return;
   const int64_t row = ((n * p.lk + j) * p.heads_kv + hk) * dh;
-  const float fk = p.scale / gs, fv = 1.f / kProbUp<T>;
+  const float fk = p.scale, fv = 1.f / kProbUp<T>;
 #pragma unroll
   for (int b = 0; b < DB; ++b) {
     // (a dead key's sums are of p = 0, which an infinity in do or q makes NaN)
@@ -606,14 +591,7 @@ __global__ __launch_bounds__(CW * RS * 64, (RS == 4 ? 1 : simd_waves<T, DP>(3, 2
 }
 
 // ------------------------------------------------------------------ host
-size_t stat_bytes(const Args &a) {
-  const size_t rows = size_t(a.p.n * a.p.heads_kv * a.rows);
-  return align_up(sizeof(float) * rows) * (a.p.dtype == SGL_FP16 ? 2 : 1);
-}
-float *most_of(const Args &a, float *stat) {
-  return reinterpret_cast<float *>(reinterpret_cast<char *>(stat) +
-                                   align_up(sizeof(float) * size_t(a.p.n * a.p.heads_kv * a.rows)));
-}
+size_t stat_bytes(const Args &a) { return align_up(sizeof(float) * size_t(a.p.n * a.p.heads_kv * a.rows)); }
 int64_t dq_tiles(const Args &a) {
   if (!many_rows(a)) return row_tiles(a, 1, false, 1);
   const bool two = a.p.dtype != SGL_FP32 || a.p.head_dim <= 64;   // two_blocks
@@ -635,7 +613,7 @@ int launch_dq(const Args &a, int64_t tiles, const void *o, const void *rest, con
   SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_dq<T, DP, NQ, SHARE, RW, KW>), lds));
   launch(&k_attn_dq<T, DP, NQ, SHARE, RW, KW>, dim3(unsigned(a.p.n * a.p.heads_kv * tiles)), dim3(RW * KW * kWave), lds,
          s, a, tiles, static_cast<const T *>(o), static_cast<const T *>(rest), lse, static_cast<const T *>(go),
-         static_cast<T *>(dq), stat, most_of(a, stat), part, static_cast<const float *>(vmost), vparts);
+         static_cast<T *>(dq), stat, part, static_cast<const float *>(vmost), vparts);
   SGL_CHECK_LAUNCH();
   return SGL_OK;
 }
@@ -644,13 +622,13 @@ template <typename T, int DP, bool SHARE, int CW, int RS>
 int launch_dkv(const Args &a, const float2 *lse, const void *go, float *stat, void *dk, void *dv, hipStream_t s) {
   const int64_t tiles = (a.p.lk + 16 * CW - 1) / (16 * CW);
   using S = DkvLds<T, DP, kRows * RS>;
-  const size_t lds = std::max(buffers<S>() * sizeof(S) + 8 * sizeof(float) + table_bytes(a),
+  const size_t lds = std::max(buffers<S>() * sizeof(S) + table_bytes(a),
                               join_bytes(CW, RS, 2, DP));
   SGL_REQUIRE(lds <= 160 * 1024, "cross_attention_backward: %zu bytes of LDS", lds);
   SGL_CHECK_HIP(ensure_dynamic_lds(reinterpret_cast<const void *>(&k_attn_dkv<T, DP, SHARE, CW, RS>), lds));
   launch(&k_attn_dkv<T, DP, SHARE, CW, RS>, dim3(unsigned(a.p.n * a.p.heads_kv * tiles)), dim3(CW * RS * kWave), lds, s,
          a, tiles, static_cast<const T *>(go), lse, static_cast<const float *>(stat),
-         static_cast<const float *>(most_of(a, stat)), static_cast<T *>(dk), static_cast<T *>(dv));
+         static_cast<T *>(dk), static_cast<T *>(dv));
   SGL_CHECK_LAUNCH();
   return SGL_OK;
 }

@@ -130,9 +130,6 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
         gm.add(gf[b][st]);
         *reinterpret_cast<FragOf<T> *>(s.b + (b * 16 + cl) * L::LD + d) = gf[b][st];
       }
-    float gs = 1.f;
-    const float most = gm.wave();
-    gs = grad_scale<T>(most);
     // scores and dp, (keys x rows)
     float x[NQ][NK][4], y[NQ][NK][4];
     int col[NQ][NK][4];
@@ -169,7 +166,7 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
     }
     if (part != nullptr && live != 0) {   // (uniform) beyond what the cells' power is for: cells shifted
       // (each row's |do|_1 by dh times the largest |do|)
-      reach += 2.f * vm.wave() * (most * float(a.rows * dh));
+      reach += 2.f * vm.wave() * (gm.wave() * float(a.rows * dh));
       const float want = cell_scale(reach);
       if (!(reach < INFINITY)) {
         bad = NAN;
@@ -221,7 +218,18 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
         for (int v = 0; v < 4; ++v)   // (0 at a dead key also where do, and with it D, is not finite)
           y[b][kb][v] = (live >> (kb * 16 + 4 * g + v)) & 1 ? x[b][kb][v] * (y[b][kb][v] - de) : 0.f;
       if (part != nullptr) add_cells(cells + (sets == 1 ? 0 : b) * slots * a.cols, col[b], y[b], slots, up);
-      if constexpr (std::is_same_v<T, fp16_t>) {
+    }
+    float fk = p.scale;
+    if constexpr (std::is_same_v<T, fp16_t>) {   // one power of two for the item's ds
+      Largest<float> dm;
+#pragma unroll
+      for (int b = 0; b < NQ; ++b)
+#pragma unroll
+        for (int kb = 0; kb < NK; ++kb) dm.add(f32x4{y[b][kb][0], y[b][kb][1], y[b][kb][2], y[b][kb][3]});
+      const float most = dm.wave(), gs = most > 0.f ? half_scale(most) : 1.f;
+      fk = p.scale / gs;
+#pragma unroll
+      for (int b = 0; b < NQ; ++b)
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
@@ -229,9 +237,7 @@ __global__ __launch_bounds__(kBlock, (DP <= 64 ? 2 : 1)) void k_attn_small_bwd(A
             y[b][kb][v] *= gs;
             x[b][kb][v] *= kProbUp<T>;
           }
-      }
     }
-    const float fk = p.scale / gs;
     // dq (head size x rows)
     wave_sync();
     {
