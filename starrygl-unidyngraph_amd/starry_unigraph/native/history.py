@@ -12,7 +12,8 @@ A sequence is a row of a padded tensor and a count, as the sampler returns its
 windows (``PaddedHop``: ``cnt`` and ``[rows, fanout]`` entries). Nothing past a
 count is read, and outputs and gradients there are zero. Work is enqueued on
 the current stream of the tensors' device; gradients are the same from run to
-run. The reference has no counterpart: its embedding attends with one query
+run. Gradients are of reverse mode and first order; a tangent (forward mode) is
+refused. The reference has no counterpart: its embedding attends with one query
 row over the window (backends/ctdg/runtime/models.py:77-137) and its memory
 runs a GRU over the mailbox slots (models.py:214-254).
 """
@@ -23,6 +24,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from starry_unigraph.lib import _capi
@@ -45,6 +47,16 @@ def _tensor(name: str, t, like: torch.Tensor, shape: tuple, dtype=None) -> torch
     if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
     return t
+
+
+def _no_tangents(*tensors) -> None:
+    """Refuses forward-mode derivatives (the operators have none; a call that
+    autograd does not see would drop them)."""
+    if getattr(forward_ad, "_current_level", 0) < 0:   # no dual level is open
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("no forward-mode derivative: a tensor carries a tangent")
 
 
 def _tracked(*tensors) -> bool:
@@ -112,6 +124,7 @@ def gated_scan(gate: torch.Tensor, value: torch.Tensor, *, lens: torch.Tensor | 
     if N == 0 or L == 0:   # nothing to run: empty rows, the states as they are
         last = state + 0.0 if state is not None else torch.zeros(N, D, device=gate.device)
         return gate + value, last if decay is None else last + 0.0 * decay
+    _no_tangents(gate, value, state, gaps, decay)
     if not _tracked(gate, value, state, decay):
         return _Scan.run(gate, value, state, decay, lens, gaps, False)[:2]
     return _Scan.apply(gate, value, state, decay, lens, gaps)
@@ -225,6 +238,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens
     scale = dh ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"scale: {scale}")
+    _no_tangents(q, k, v, bias)
     least = 16 // q.element_size()
     if dh < least:   # the kernels read 16 bytes of a head at a time: zeros add nothing to the products
         q, k, v = (torch.nn.functional.pad(t, (0, least - dh)) for t in (q, k, v))
@@ -339,6 +353,7 @@ def gated_norm(x: torch.Tensor, z: torch.Tensor, gate: torch.Tensor, scale: torc
         if t is not None:
             _tensor(name, t, x, (D,), torch.float32)
     args = (x, z, gate, scale, post_weight, pre_weight, post_bias, pre_bias)
+    _no_tangents(*args)
     if _tracked(*args):
         return _Norm.apply(*args, float(eps), bool(rms))
     return _Norm.run(*args, float(eps), bool(rms))[:2]
