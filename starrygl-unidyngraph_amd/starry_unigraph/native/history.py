@@ -197,8 +197,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens
                     k_pos: torch.Tensor | None = None, resolution: int = 0, two_sided: bool = False,
                     scale: float | None = None) -> torch.Tensor:
     """Attention of ``q`` [N, Lq, Hq, dh] over the states ``k``, ``v``
-    [N, Lk, Hkv, dh] of another length (Hq a multiple of Hkv: consecutive query
-    heads share a key head; dh up to 128): softmax over the live keys of
+    [N, Lk, Hkv, dh] of another length (Hq a multiple of Hkv, at most 64 times:
+    consecutive query heads share a key head; dh up to 128): softmax over the live keys of
     ``scale * <q, k> + bias``, ``scale`` dh**-0.5 by default.
 
     ``q_lens``, ``k_lens``: int32 [N], the events of each sequence (default
@@ -219,6 +219,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens
     _tensor("v", v, q, (N, Lk, Hkv, dh))
     if Hq == 0 or Hkv == 0 or Hq % Hkv:
         raise ValueError(f"q: {Hq} heads over {Hkv} key heads, expected a multiple")
+    if Hq // Hkv > 64:
+        raise ValueError(f"q: {Hq} heads over {Hkv} key heads, at most 64 to one")
     if not 1 <= dh <= 128:
         raise ValueError(f"q: heads of {dh}, expected 1 to 128")
     q_lens, k_lens = _lens("q_lens", q_lens, q, N), _lens("k_lens", k_lens, q, N)

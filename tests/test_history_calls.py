@@ -72,3 +72,10 @@ def test_forward_mode_tangents_are_refused(anywhere, call, shapes):
             torch.func.jvp(lambda t: call(**{name: t}), (_f(*shape),), (torch.ones(shape),))
     with pytest.raises(anywhere):
         call()
+
+
+def test_more_query_heads_than_a_key_head_takes(anywhere):
+    with pytest.raises(anywhere):
+        _attend(q=_f(2, 3, 128, 8), bias=None)
+    with pytest.raises(ValueError, match="at most 64"):
+        _attend(q=_f(2, 3, 130, 8), bias=None)
