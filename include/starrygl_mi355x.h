@@ -956,7 +956,8 @@ int sgl_gated_norm_forward(int32_t dtype, int64_t rows, int32_t D,
                            void *n, hipStream_t stream);
 size_t sgl_gated_norm_workspace_bytes(int64_t rows, int32_t D);
 /* gy, gn (either may be NULL: 0) -> dx, dz, dgate and dparams fp32 [nsum][D]:
- * the gradients of scale, post_w, pre_w (nsum 3) and post_b, pre_b (nsum 5). */
+ * the gradients of scale, post_w, pre_w (nsum 3: without biases) and post_b,
+ * pre_b (nsum 5). */
 int sgl_gated_norm_backward(int32_t dtype, int64_t rows, int32_t D,
                             const void *x, int64_t sx, const void *z,
                             int64_t sz, const void *gate, int64_t sg,

@@ -407,6 +407,8 @@ extern "C" int sgl_gated_norm_backward(int32_t dtype, int64_t rows, int32_t D, c
   const NormArgs a{x, z, gate, sx, sz, sg, scale, post_w, post_b, pre_w, pre_b, eps, rms, D, rows};
   if (const int rc = check_norm(dtype, rows, D, a)) return rc;
   SGL_REQUIRE(nsum == 3 || nsum == 5, "gated_norm_backward: %d parameter gradients (3 or 5)", nsum);
+  // (the form of 3 has no biases in its y)
+  SGL_REQUIRE(nsum == 5 || (post_b == nullptr && pre_b == nullptr), "gated_norm_backward: biases need 5 parameter gradients");
   SGL_REQUIRE(dparams != nullptr, "gated_norm_backward: NULL array");
   if (rows > 0) {
     SGL_REQUIRE(dx && dz && dgate, "gated_norm_backward: NULL array");

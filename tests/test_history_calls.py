@@ -79,3 +79,16 @@ def test_more_query_heads_than_a_key_head_takes(anywhere):
         _attend(q=_f(2, 3, 128, 8), bias=None)
     with pytest.raises(ValueError, match="at most 64"):
         _attend(q=_f(2, 3, 130, 8), bias=None)
+
+
+def test_norm_backward_with_biases_gives_their_gradients():
+    """The C entry's form of three parameter gradients forms y without biases."""
+    L = _capi.load_library()
+    one = 4096   # (never read: the checks come first)
+    back = lambda post_b, pre_b, nsum: L.sgl_gated_norm_backward(
+        0, 2, 8, one, 8, one, 8, one, 8, one, one, post_b, one, pre_b, 1e-5, 0, one, one, one, one, one, one, nsum, None,
+        0, None)
+    for biases in ((one, None), (None, one), (one, one)):
+        assert back(*biases, 3) == 1 and b"biases need 5" in L.sgl_last_error()
+        assert back(*biases, 5) == 3   # (no workspace given)
+    assert back(None, None, 3) == 3
