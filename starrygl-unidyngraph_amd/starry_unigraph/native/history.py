@@ -205,7 +205,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens
     all; clamped). ``key_mask``: bool [N, Lk], False a key that is left out.
     ``bias``: float32 [Hq, C], C at most 64: a learned value for each head and
     bucket of the distance ``q_pos - k_pos`` (int64 event times or indexes,
-    [N, Lq] and [N, Lk]). ``two_sided``: C is twice the buckets, the second
+    [N, Lq] and [N, Lk], whose differences are int64 too). ``two_sided``: C is twice the buckets, the second
     half for keys after the query; else such keys count as distance 0. The
     buckets are ``distance_bucket``'s, 2**resolution an octave. Returns
     [N, Lq, Hq, dh], zero in rows without a live key. Differentiable in q, k, v
@@ -258,7 +258,7 @@ def distance_bucket(distance: torch.Tensor, buckets: int, resolution: int = 0) -
     octave has 2**resolution; the last of the ``buckets`` takes everything
     beyond it. A two-sided table adds ``buckets`` where the distance is
     negative. The kernels compute the same from integers."""
-    d = distance.abs().clamp(max=0xFFFFFFFF)
+    d = distance.clamp(-0xFFFFFFFF, 0xFFFFFFFF).abs()   # (int64's lowest value has no absolute value)
     e = torch.full_like(d, resolution)
     for b in range(resolution + 1, 32):
         e = e + (d >= (1 << b))

@@ -92,3 +92,11 @@ def test_norm_backward_with_biases_gives_their_gradients():
         assert back(*biases, 3) == 1 and b"biases need 5" in L.sgl_last_error()
         assert back(*biases, 5) == 3   # (no workspace given)
     assert back(None, None, 3) == 3
+
+
+def test_distance_bucket_of_the_farthest_distances():
+    """int64's ends fall into the last bucket, as the kernels have them."""
+    ends = torch.tensor([torch.iinfo(torch.int64).min, torch.iinfo(torch.int64).min + 1, torch.iinfo(torch.int64).max,
+                         -(1 << 32), 1 << 32])
+    for buckets, resolution in ((1, 0), (20, 0), (64, 1)):
+        assert history.distance_bucket(ends, buckets, resolution).tolist() == [buckets - 1] * 5
