@@ -926,8 +926,9 @@ typedef struct sgl_attention {
 /* o [n, lq, heads_q, head_dim]; rows past a query length and rows without a
  * live key are 0. What the backward reads of the forward, by the bits of
  * sgl_cross_attention_saves: 1: o and lse (fp32 [n, heads_kv, lq * heads_q /
- * heads_kv, 2]: a row's maximum and log2 of its sum, base 2), 2: rest (like o, 16 bits of what rounding o left). lse and rest may be NULL
- * where they are not needed. The problem struct is HOST memory. */
+ * heads_kv, 2]: a row's maximum and log2 of its sum, base 2), 2: rest (like o,
+ * 16 bits of what rounding o left). lse and rest may be NULL where they are not
+ * needed. The problem struct is HOST memory. */
 int32_t sgl_cross_attention_saves(const sgl_attention *problem);
 size_t sgl_cross_attention_workspace_bytes(const sgl_attention *problem,
                                            int32_t backward);

@@ -27,7 +27,12 @@
 // without leaving the registers; the other operand is read down the columns of
 // the row-major tile in that order (16-bit types: the transposing LDS read).
 //
-// Which kernels run, by size (both sides measured at the rules):
+// Which kernels run, by size (both sides of each rule, heads of 64, us: 2,000
+// sequences of 32 rows x 64 keys in bf16, forward and backward, 134 in one wave
+// and 274 in tiles; 500 of 32 x 200 forward 39 and 77 to 93; 24 of 512 x 600,
+// which are 192 workgroups, 146 and 371, in fp32 268 and 385; half as many in
+// fp32 172 by the four waves and 234. In bf16 the eight waves are ahead from
+// 96 on, 135 for 196: the threshold is fp32's):
 //   rows = lq G <= 32       one wave a (sequence, key head), or the keys split
 //                           over workgroups and joined where sequences are few
 //   rows <= 32, lk <= 64    the backward in one wave, nothing kept for it

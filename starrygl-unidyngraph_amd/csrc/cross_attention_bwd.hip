@@ -7,18 +7,8 @@ namespace sgl {
 namespace attn {
 namespace {
 
-// ------------------------------------------------------------------ dq, dbias, D
-// As the forward with many rows. D = <do, o> takes o with what its rounding
-// left (rest), so that the sums that should cancel do; where all keys lie in
-// one tile it is the sum of p dp itself, which cancels exactly (a single key
-// has no gradient). The table's gradient is summed in 64-bit cells of fixed
-// point in LDS (a float atomic of LDS costs 194 clocks a wave, an integer one
-// 8), relative to a bound on their sum; where that is not finite (a do, v or
-// score that is not, or magnitudes whose product overflows) the workgroup's
-// part is NaN. 8 sequences, 8 heads of 64, 1000 x 2049 in bf16: 185
-// us; workgroups of 4 waves instead of 8: 202.
-
-// The largest |v| of the live keys of a (sequence, key head), a part of its
+// ------------------------------------------------------------------ the largest |v|
+// Of the live keys of a (sequence, key head), a part of its
 // keys a workgroup: what bounds the cells. A kernel of its own, 5 us: it reads
 // v once, where every row tile's workgroup would have to before its first cell.
 inline int vmost_parts(const Args &a) {   // (a workgroup's four loads a thread, 64 workgroups at most)
@@ -52,6 +42,16 @@ __global__ __launch_bounds__(kBlock) void k_attn_vmost(Args a, int parts, float 
   if (threadIdx.x == 0) vmost[blockIdx.x] = __uint_as_float(max(max(red[0], red[1]), max(red[2], red[3])));
 }
 
+// ------------------------------------------------------------------ dq, dbias, D
+// As the forward with many rows. D = <do, o> takes o with what its rounding
+// left (rest), so that the sums that should cancel do; where all keys lie in
+// one tile it is the sum of p dp itself, which cancels exactly (a single key
+// has no gradient). The table's gradient is summed in 64-bit cells of fixed
+// point in LDS (a float atomic of LDS costs 194 clocks a wave, an integer one
+// 8), relative to a bound on their sum; where that is not finite (a do, v or
+// score that is not, or magnitudes whose product overflows) the workgroup's
+// part is NaN. 8 sequences, 8 heads of 64, 1000 x 2049 in bf16: 195
+// us; of workgroups of 4 waves instead of 8 a tenth more.
 template <typename T, int DP, int TK>
 struct alignas(16) DqLds {
   T k[TK * Tile<T, DP>::LD], v[TK * Tile<T, DP>::LD];
@@ -351,8 +351,8 @@ __global__ __launch_bounds__(RW * KW * 64, (2)) void k_attn_dq(Args a, int64_t t
 // pointer and an offset that it keeps (an odd G above one divides instead);
 // the first wave fetches what belongs to a row (D, maximum, sum, position). Bound by
 // what a SIMD issues and LDS together (24 fragment reads and 8 table reads a
-// step of 512 scores) at two waves a SIMD: at the same size 232 us, and the same
-// with 32 keys and 64 rows a workgroup (235) or 8 waves of it (257).
+// step of 512 scores) at two waves a SIMD: at the same size 245 us; with 32 keys
+// and 64 rows a workgroup the same, with 8 waves of it a tenth more.
 constexpr int kRows = 32;
 
 template <typename T, int DP, int TR>

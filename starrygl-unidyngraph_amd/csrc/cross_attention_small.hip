@@ -7,10 +7,10 @@
 // fragments; k, do and q pass through the wave's LDS for the products down
 // their columns, p and ds to be read with the rows as the reduction index. A
 // wave walks items of one key head, so that the bias' gradient is one row of
-// partial sums a wave. 4000 windows of 20 x 32, 4 heads of 43 in bf16: 114 us,
+// partial sums a wave. 4000 windows of 20 x 32, 4 heads of 43 in bf16: 118 us,
 // bound by a wave's chain of loads and products at two waves a SIMD (a pass of
 // both directions went from 1313 to 323 us when this form and one wave an item
-// in the forward took over from the tiled kernels; 186 now).
+// in the forward took over from the tiled kernels; 186 to 190 now).
 #include "cross_attention.h"
 
 namespace sgl {

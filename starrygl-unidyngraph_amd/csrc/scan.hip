@@ -37,7 +37,7 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kKeep = 8;             // steps between kept states
-constexpr int64_t kFill = 1 << 18;   // threads that fill the GPU: 16 waves a CU
+constexpr int64_t kFill = 1 << 18;   // threads that fill the GPU: 16 waves a CU (the backward holds 8 at a time)
 // pieces x channel groups: two rounds of the backward's workgroups (16 x 8191 x
 // 256 in bf16, both directions: 160 us; 1.25 kFill 170, 0.75 kFill 183)
 constexpr int64_t kPieces = 2 * kFill;

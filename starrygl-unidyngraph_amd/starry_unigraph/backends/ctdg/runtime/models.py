@@ -270,7 +270,8 @@ class CTDGHistoryPredictor(CTDGLinkPredictor):
     """Link prediction on the roots' windows read as sequences
     (HistoryEncoder), then the same edge predictor (models.py:313-324). The
     reference has no such embedding; select it with ctdg.embedding = history.
-    It trains through autograd (no launch plans), in fp32."""
+    It trains through autograd (no launch plans), in fp32, and has no dropout:
+    ctdg.dropout and ctdg.att_dropout have no effect on it."""
 
     def __init__(self, num_nodes: int, hidden_dim: int, edge_feat_dim: int, num_head: int = 2,
                  mean_gap: float = 1.0) -> None:

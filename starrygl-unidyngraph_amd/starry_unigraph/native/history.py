@@ -198,17 +198,18 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_lens
                     scale: float | None = None) -> torch.Tensor:
     """Attention of ``q`` [N, Lq, Hq, dh] over the states ``k``, ``v``
     [N, Lk, Hkv, dh] of another length (Hq a multiple of Hkv, at most 64 times:
-    consecutive query heads share a key head; dh up to 128): softmax over the live keys of
-    ``scale * <q, k> + bias``, ``scale`` dh**-0.5 by default.
+    consecutive query heads share a key head; dh up to 128): softmax over the
+    live keys of ``scale * <q, k> + bias``, ``scale`` dh**-0.5 by default.
 
     ``q_lens``, ``k_lens``: int32 [N], the events of each sequence (default
     all; clamped). ``key_mask``: bool [N, Lk], False a key that is left out.
     ``bias``: float32 [Hq, C], C at most 64: a learned value for each head and
     bucket of the distance ``q_pos - k_pos`` (int64 event times or indexes,
-    [N, Lq] and [N, Lk], whose differences are int64 too). ``two_sided``: C is twice the buckets, the second
-    half for keys after the query; else such keys count as distance 0. The
-    buckets are ``distance_bucket``'s, 2**resolution an octave. Returns
-    [N, Lq, Hq, dh], zero in rows without a live key. Differentiable in q, k, v
+    [N, Lq] and [N, Lk], whose differences are int64 too). ``two_sided``: C is
+    twice the buckets, the second half for keys after the query; else such keys
+    count as distance 0. The buckets are ``distance_bucket``'s, 2**resolution an
+    octave. Returns [N, Lq, Hq, dh], zero in rows without a live key (or with
+    -inf in the table for all of them). Differentiable in q, k, v
     and bias. One new event per sequence is Lq = 1."""
     _first("q", q, 4)
     N, Lq, Hq, dh = q.shape
