@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define SGL_ABI_VERSION 25
+#define SGL_ABI_VERSION 26
 
 #define SGL_OK 0
 #define SGL_ERR_INVALID 1   /* bad argument (host-checked) */
@@ -969,6 +969,73 @@ int sgl_gated_norm_backward(int32_t dtype, int64_t rows, int32_t D,
                             void *dgate, float *dparams, int32_t nsum,
                             void *workspace, size_t workspace_bytes,
                             hipStream_t stream);
+
+/* Losses of rows over every candidate (a table's rows), with the scores
+ * s = (scale <h, w> + bias) / temperature never stored. h [n, dim] and table
+ * [v, dim] of one type, rows h_stride and table_stride elements apart, dim
+ * 16 / sizeof(element) to 256; bias fp32 [v] or NULL. A candidate with bias
+ * -inf is left out: its row is not used and may hold anything. The struct is
+ * HOST memory. */
+typedef struct sgl_candidates {
+  int32_t dtype, dim;
+  int64_t n, v;
+  const void *h, *table;
+  int64_t h_stride, table_stride;
+  const float *bias;
+  float scale, temperature;
+} sgl_candidates;
+
+/* A teacher's entries (ids int64 [n, k], -1: none; logits fp32 [n, k]; k up to
+ * 1024) as targets: weight = softmax(logits / temperature) over a row's live
+ * entries, entries of one candidate put together in the first (the others -1),
+ * konst [n] = sum of weight log weight over the entries. */
+int sgl_candidates_teacher(int64_t n, int32_t k, int64_t v, const int64_t *ids,
+                           const float *logits, float temperature,
+                           int32_t *ids_out, float *weight, float *konst,
+                           hipStream_t stream);
+/* what: 0 the loss alone, 1 the loss with dir, 2 the backward. */
+size_t sgl_candidates_workspace_bytes(const sgl_candidates *problem,
+                                      int32_t what);
+/* loss [n] = temperature^2 (konst + sum_k weight (lse - s_id)). Targets: either
+ * `target` int64 [n] (one a row at weight 1; negative: the row's loss is 0;
+ * past the table: NaN; k = 1) or ids, weight, konst of
+ * sgl_candidates_teacher. A target that is left out: inf. For the backward
+ * (NULL: not kept): stat fp32 [2, n], dir fp32 [n, dim] (the loss's direction
+ * in h), and with `target` ids_out int32 [n]. Rows whose loss is 0, inf or NaN
+ * for these reasons have no gradient. */
+int sgl_candidates_forward(const sgl_candidates *problem,
+                           const int64_t *target, const int32_t *ids,
+                           const float *weight, const float *konst, int32_t k,
+                           float *loss, float *stat, float *dir,
+                           int32_t *ids_out, void *workspace,
+                           size_t workspace_bytes, hipStream_t stream);
+/* g [n] -> dh (like h, contiguous; from dir; NULL: not computed), dtable (like
+ * the table, contiguous; NULL: not computed) and with it dbias fp32 [v] (or
+ * NULL). weight NULL: 1 (ids_out of the forward). */
+int sgl_candidates_backward(const sgl_candidates *problem, const float *stat,
+                            const int32_t *ids, const float *weight, int32_t k,
+                            const float *dir, const float *g, void *dh,
+                            void *dtable, float *dbias, void *workspace,
+                            size_t workspace_bytes, hipStream_t stream);
+
+/* One tensor of a rotation: x [n, len, heads, dh] at its strides, y
+ * contiguous, pos int64 [n, len] at its strides. */
+typedef struct sgl_rotary_side {
+  const void *x;
+  void *y;
+  const int64_t *pos;
+  int64_t len, x_n, x_t, x_h, pos_n, pos_t;
+  int32_t heads;
+} sgl_rotary_side;
+
+/* Pairs of the first `rot` of dh channels turned by pos * freqs[i] (freqs:
+ * double [rot / 2]) and scaled by gain, the other channels copied: pairs (i, i +
+ * rot / 2), or interleaved != 0 (2 i, 2 i + 1). inverse != 0: by the negative
+ * angles (the gradient). k may be NULL. The structs are HOST memory. */
+int sgl_rotary(int32_t dtype, int64_t n, int32_t dh, int32_t rot,
+               const sgl_rotary_side *q, const sgl_rotary_side *k,
+               const double *freqs, int32_t interleaved, float gain,
+               int32_t inverse, hipStream_t stream);
 
 #ifdef __cplusplus
 }

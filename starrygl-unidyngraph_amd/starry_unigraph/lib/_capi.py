@@ -17,7 +17,7 @@ import torch  # loads the HIP runtime first, so the library binds to the same on
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libstarrygl_mi355x.so"
 LIB_PATH = os.path.join(_HERE, LIB_NAME)
-ABI_VERSION = 25
+ABI_VERSION = 26
 
 SGL_DERR_NODE_RANGE = 1
 SGL_DERR_EID_RANGE = 2
@@ -112,6 +112,11 @@ SIGNATURES: dict[str, tuple] = {
     "sgl_cross_attention_saves": (_i32, [_vp]),
     "sgl_cross_attention_forward": (ctypes.c_int, [_vp] * 5 + [_sz, _vp]),
     "sgl_cross_attention_backward": (ctypes.c_int, [_vp] * 10 + [_sz, _vp]),
+    "sgl_candidates_teacher": (ctypes.c_int, [_i64, _i32, _i64, _vp, _vp, ctypes.c_float] + [_vp] * 4),
+    "sgl_candidates_workspace_bytes": (_sz, [_vp, _i32]),
+    "sgl_candidates_forward": (ctypes.c_int, [_vp] * 5 + [_i32] + [_vp] * 5 + [_sz, _vp]),
+    "sgl_candidates_backward": (ctypes.c_int, [_vp] * 4 + [_i32] + [_vp] * 6 + [_sz, _vp]),
+    "sgl_rotary": (ctypes.c_int, [_i32, _i64, _i32, _i32, _vp, _vp, _vp, _i32, ctypes.c_float, _i32, _vp]),
     "sgl_gated_norm_workspace_bytes": (_sz, [_i64, _i32]),
     "sgl_gated_norm_forward": (ctypes.c_int, [_i32, _i64, _i32] + _NORM + [_vp] * 3),
     "sgl_gated_norm_backward": (ctypes.c_int, [_i32, _i64, _i32] + _NORM + [_vp] * 6 + [_i32, _vp, _sz, _vp]),
@@ -232,6 +237,19 @@ class Attention(ctypes.Structure):
                [("mask_n", _i64), ("mask_t", _i64), ("bias", _vp)] + \
                [(n, _i32) for n in ("buckets", "resolution", "two_sided")] + [("scale", ctypes.c_float)] + \
                [("q_pos", _vp), ("k_pos", _vp)] + [(n, _i64) for n in ("qpos_n", "qpos_t", "kpos_n", "kpos_t")]
+
+
+class Candidates(ctypes.Structure):
+    """struct sgl_candidates of include/starrygl_mi355x.h."""
+    _fields_ = [("dtype", _i32), ("dim", _i32), ("n", _i64), ("v", _i64), ("h", _vp), ("table", _vp),
+                ("h_stride", _i64), ("table_stride", _i64), ("bias", _vp), ("scale", ctypes.c_float),
+                ("temperature", ctypes.c_float)]
+
+
+class RotarySide(ctypes.Structure):
+    """struct sgl_rotary_side of include/starrygl_mi355x.h."""
+    _fields_ = [("x", _vp), ("y", _vp), ("pos", _vp)] + \
+               [(n, _i64) for n in ("len", "x_n", "x_t", "x_h", "pos_n", "pos_t")] + [("heads", _i32)]
 
 
 SGL_OP_MAX_ARGS = 64

@@ -1,0 +1,184 @@
+"""Losses over every candidate node, each a set of fused HIP kernels with its
+gradient (float32, bfloat16 or float16 tensors on a GPU):
+
+* ``cross_entropy``: the softmax cross entropy of rows over all rows of a table
+  (which node comes next, out of all of them);
+* ``distillation``: the divergence of that softmax from a teacher's, given the
+  teacher's top candidates and their logits.
+
+The scores [rows, candidates] are never stored: the table is walked in pieces
+with a running softmax, and the gradient of the table forms them again. Work is
+enqueued on the current stream of the tensors' device; results and gradients
+are the same from run to run. Gradients are of reverse mode and first order; a
+tangent (forward mode) is refused. The reference has no counterpart: it scores
+an event against one drawn negative
+(backends/ctdg/runtime/models.py:313-324, runtime.py:124-136).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from starry_unigraph.lib import _capi
+from starry_unigraph.native.history import _as_rows, _first, _guard, _no_grad, _no_tangents, _rows, _tensor, _tracked
+
+MAX_DIM = 256       # channels of a row
+MAX_TARGETS = 1024  # a teacher's entries of a row
+
+
+def cross_entropy(h: torch.Tensor, table: torch.Tensor, target: torch.Tensor, *, bias: torch.Tensor | None = None,
+                  scale: float = 1.0) -> torch.Tensor:
+    """``logsumexp_v(s_v) - s_target`` of each row over all candidates, ``s_v =
+    scale * <h, table_v> + bias_v``: float32, like ``target``.
+
+    ``h``: [..., D]; ``table``: [V, D] of the same type, D up to 256; ``target``:
+    int64 [...], the candidate that came: a row with a negative one (padding) is
+    left out, its loss 0 (``h`` may hold anything there); with one of V or more
+    the loss is NaN and has no gradient. ``bias``: float32 [V], a learned
+    value of each candidate, or -inf for those that are left out: their rows of
+    the table may hold anything and have gradients of 0 (a target that is left
+    out: the loss is inf and the row has no gradient; if all are, 0).
+    Differentiable in h, table and bias. One new event is one row."""
+    rows = _check(h, table, bias, scale)
+    if target.dtype != torch.int64 or target.shape != h.shape[:-1] or target.device != h.device:
+        raise ValueError(f"target: {target.dtype} {tuple(target.shape)} on {target.device}, expected int64 "
+                         f"{tuple(h.shape[:-1])} on {h.device}")
+    _no_tangents(h, table, bias)
+    return _call(rows, table, bias, target.reshape(-1).contiguous(), None, float(scale), 1.0).view(h.shape[:-1])
+
+
+def distillation(h: torch.Tensor, table: torch.Tensor, ids: torch.Tensor, logits: torch.Tensor, *,
+                 bias: torch.Tensor | None = None, scale: float = 1.0, temperature: float = 1.0) -> torch.Tensor:
+    """``T^2 * sum_k q_k (log q_k - log p_ids_k)`` of each row: the divergence of
+    the row's softmax over all candidates, ``p = softmax((scale * <h, table_v>
+    + bias_v) / T)``, from a teacher's over its top ones, ``q = softmax(logits /
+    T)`` over the row's live entries. float32 [...].
+
+    ``h``, ``table``, ``bias`` and ``scale`` as in :func:`cross_entropy`.
+    ``ids``: int64 [..., K], K up to 1024, the teacher's candidates in any order
+    (negative: no entry; the same one twice: two entries); ``logits``: float32
+    [..., K], without gradient (-inf: no entry). A row without an entry has
+    loss 0 and no gradient; one with an id of V or more NaN and none; one that
+    wants a candidate that is left out inf and none. Differentiable in h, table and
+    bias."""
+    rows = _check(h, table, bias, scale)
+    temperature = float(temperature)
+    if not (0.0 < temperature < math.inf):
+        raise ValueError(f"temperature: {temperature}, expected a positive number")
+    if ids.dtype != torch.int64 or ids.dim() != h.dim() or ids.shape[:-1] != h.shape[:-1] or ids.device != h.device:
+        raise ValueError(f"ids: {ids.dtype} {tuple(ids.shape)} on {ids.device}, expected int64 "
+                         f"[{', '.join(str(n) for n in h.shape[:-1])}, K] on {h.device}")
+    K = ids.shape[-1]
+    if not 1 <= K <= MAX_TARGETS:
+        raise ValueError(f"ids: {K} entries a row, expected 1 to {MAX_TARGETS}")
+    _tensor("logits", logits, h, ids.shape, torch.float32)
+    _no_grad("logits", logits)
+    _no_tangents(h, table, bias, logits)
+    entries = (ids.reshape(-1, K).contiguous(), logits.reshape(-1, K).contiguous())
+    return _call(rows, table, bias, None, entries, float(scale), temperature).view(h.shape[:-1])
+
+
+def _check(h, table, bias, scale) -> torch.Tensor:
+    """``h`` as rows, its and the table's types, shapes and device checked."""
+    _first("h", h, max(h.dim(), 1))
+    D = h.shape[-1]
+    if not 1 <= D <= MAX_DIM:
+        raise ValueError(f"h: rows of {D}, expected 1 to {MAX_DIM}")
+    if table.dim() != 2:
+        raise ValueError(f"table: {table.dim()} dimensions, expected 2")
+    V = table.shape[0]
+    _tensor("table", table, h, (V, D))
+    if V == 0:
+        raise ValueError("table: no candidates")
+    if bias is not None:
+        _tensor("bias", bias, h, (V,), torch.float32)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale: {scale}")
+    return _as_rows(h) if h.dim() != 1 else h.unsqueeze(0)
+
+
+def _call(h, table, bias, target, entries, scale, temperature) -> torch.Tensor:
+    if h.shape[0] == 0:   # no rows: an empty loss that every operand gets a gradient of 0 from
+        zero = (h.sum() + table[:0].sum()).float()
+        return h.new_zeros(0, dtype=torch.float32) + (zero if bias is None else zero + bias[:0].sum())
+    least = 16 // h.element_size()
+    if h.shape[1] < least:   # the kernels read 16 bytes of a row at a time: zeros add nothing to the products
+        h, table = (torch.nn.functional.pad(t, (0, least - t.shape[1])) for t in (h, table))
+    args = (h, table, bias, target, entries, scale, temperature)
+    if _tracked(h, table, bias):
+        return _Loss.apply(*args)
+    return _Loss.run(*args, (False, False))[0]
+
+
+class _Loss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *args):
+        h, table, bias = args[:3]
+        need = (h.requires_grad, table.requires_grad or (bias is not None and bias.requires_grad))
+        loss, saved = _Loss.run(*args, need)
+        ctx.save_for_backward(*saved)
+        ctx.form = args[5:]
+        return loss
+
+    @staticmethod
+    def run(h, table, bias, target, entries, scale, temperature, need):
+        """(loss, the backward's tensors); ``need``: gradients of the rows, of
+        the table or bias."""
+        lib, P, dev = _capi.lib(), _capi.ptr, h.device
+        h, table = _rows(h), _rows(table)
+        bias = None if bias is None else bias.contiguous()
+        N, D = h.shape
+        a = ctypes.byref(_Loss.problem(h, table, bias, scale, temperature))
+        f32 = dict(dtype=torch.float32, device=dev)
+        loss = torch.empty(N, **f32)
+        stat = torch.empty(2, N, **f32) if any(need) else None
+        direction = torch.empty(N, D, **f32) if need[0] else None
+        nb = lib.sgl_candidates_workspace_bytes(a, 1 if need[0] else 0)
+        ws = _capi.workspace(nb, dev)
+        with _guard(dev):
+            stream = _capi.stream_of(dev)
+            if entries is None:
+                ids, weight, konst, K = torch.empty(N, 1, dtype=torch.int32, device=dev) if need[1] else None, None, None, 1
+                _capi.check(lib.sgl_candidates_forward(
+                    a, P(target), None, None, None, 1, P(loss), P(stat), P(direction), P(ids), P(ws), nb, stream),
+                    "cross_entropy")
+            else:
+                K = entries[0].shape[1]
+                ids = torch.empty(N, K, dtype=torch.int32, device=dev)
+                weight, konst = torch.empty(N, K, **f32), torch.empty(N, **f32)
+                _capi.check(lib.sgl_candidates_teacher(
+                    N, K, table.shape[0], P(entries[0]), P(entries[1]), temperature, P(ids), P(weight), P(konst),
+                    stream), "distillation")
+                _capi.check(lib.sgl_candidates_forward(
+                    a, None, P(ids), P(weight), P(konst), K, P(loss), P(stat), P(direction), None, P(ws), nb, stream),
+                    "distillation")
+        return loss, (h, table, bias, stat, ids if need[1] else None, weight if need[1] else None, direction)
+
+    @staticmethod
+    def problem(h, table, bias, scale, temperature):
+        P = _capi.ptr
+        return _capi.Candidates(_capi.DTYPES[h.dtype], h.shape[1], h.shape[0], table.shape[0], P(h), P(table),
+                                h.stride(0), table.stride(0), P(bias), scale, temperature)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        h, table, bias, stat, ids, weight, direction = ctx.saved_tensors
+        lib, P, dev = _capi.lib(), _capi.ptr, h.device
+        # (from the tensors as they are now: a hook on saved tensors may bring them back elsewhere)
+        a = ctypes.byref(_Loss.problem(h, table, bias, *ctx.form))
+        g = g.contiguous()
+        want = ctx.needs_input_grad
+        dh = torch.empty(h.shape, dtype=h.dtype, device=dev) if want[0] else None
+        dt = torch.empty(table.shape, dtype=table.dtype, device=dev) if want[1] or want[2] else None
+        db = torch.empty_like(bias) if want[2] else None
+        nb = lib.sgl_candidates_workspace_bytes(a, 2) if dt is not None else 0
+        ws = _capi.workspace(nb, dev) if nb else None
+        with _guard(dev):
+            _capi.check(lib.sgl_candidates_backward(
+                a, P(stat), P(ids), P(weight), ids.shape[1] if ids is not None else 1, P(direction), P(g), P(dh), P(dt),
+                P(db), P(ws), nb, _capi.stream_of(dev)), "candidates backward")
+        return dh, dt if want[1] else None, db, None, None, None, None

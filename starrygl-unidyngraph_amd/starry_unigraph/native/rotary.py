@@ -1,0 +1,134 @@
+"""Rotary positions for the attention over windows of events
+(``history.cross_attention``): pairs of a head's channels of queries and keys
+turned by an angle that grows with the event's time or index, so that their
+scores depend on the distance of the two. A fused HIP kernel with its gradient
+(float32, bfloat16 or float16 tensors on a GPU).
+
+Work is enqueued on the current stream of the tensors' device. Gradients are of
+reverse mode and first order; a tangent (forward mode) is refused. The reference
+has no counterpart: its attention sees a neighbour's age through a learned
+cosine encoding (runtime/modules/time_encode.py:41-58).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from starry_unigraph.lib import _capi
+from starry_unigraph.native.history import _first, _guard, _no_tangents, _rows, _tensor, _tracked
+
+
+def frequencies(dims: int, *, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                trained: int | None = None, low: float = 1.0, high: float = 32.0,
+                device: torch.device | str = "cuda") -> torch.Tensor:
+    """The angles a unit of position of ``dims`` rotated channels, one a pair:
+    ``base ** (-2 i / dims)``, float64 [dims / 2]. ``scaling`` fits them to
+    positions ``factor`` times as long (or to another unit of time):
+
+    * "linear": every angle divided by ``factor``;
+    * "base": the base raised so that the longest wave is ``factor`` times as
+      long and the shortest stays;
+    * "wavelength": waves that turn more than ``high`` times over ``trained``
+      positions stay, those of less than ``low`` are divided by ``factor``, and
+      those between blend."""
+    if dims < 0 or dims % 2:
+        raise ValueError(f"dims: {dims}, expected an even number")
+    if not (base > 0 and math.isfinite(base)) or not (factor > 0 and math.isfinite(factor)):
+        raise ValueError(f"base {base}, factor {factor}: expected positive numbers")
+    if scaling == "base" and dims > 2:
+        base = base * factor ** (dims / (dims - 2))
+    f = base ** (torch.arange(0, dims, 2, dtype=torch.float64) * (-1.0 / max(dims, 1)))
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "wavelength":
+        if trained is None or trained < 1 or not low < high:
+            raise ValueError(f"wavelength scaling: trained {trained}, low {low}, high {high}")
+        keep = ((f * (trained / (2.0 * math.pi)) - low) / (high - low)).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+    elif scaling not in ("none", "base"):
+        raise ValueError(f"scaling: {scaling!r}, expected 'none', 'linear', 'base' or 'wavelength'")
+    return f.to(device)
+
+
+def rotate(q: torch.Tensor, k: torch.Tensor | None, q_pos: torch.Tensor, k_pos: torch.Tensor | None,
+           freqs: torch.Tensor, *, interleaved: bool = False,
+           gain: float = 1.0) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """``q`` [N, Lq, Hq, dh] and ``k`` [N, Lk, Hkv, dh] with the pairs of their
+    first 2 P channels turned by ``position * freqs`` and scaled by ``gain``; the
+    other channels as they are. ``k`` and ``k_pos`` may both be None.
+
+    ``q_pos``, ``k_pos``: int64 [N, Lq], [N, Lk] (any values: angles are exact
+    for far positions too). ``freqs``: float64 [P], 2 P <= dh, the angle a unit
+    of position of each pair (``frequencies``); no gradient. Pairs are channels
+    (i, i + P), or with ``interleaved`` (2 i, 2 i + 1). Differentiable in q and
+    k. One new event per sequence is L = 1."""
+    _first("q", q, 4)
+    N, Lq, Hq, dh = q.shape
+    if dh == 0:
+        raise ValueError("q: heads of 0 channels")
+    if (k is None) != (k_pos is None):
+        raise ValueError("k and k_pos: give both or neither")
+    _tensor("q_pos", q_pos, q, (N, Lq), torch.int64)
+    if k is not None:
+        if k.dim() != 4:
+            raise ValueError(f"k: {k.dim()} dimensions, expected 4")
+        _tensor("k", k, q, (N, k.shape[1], k.shape[2], dh))
+        _tensor("k_pos", k_pos, q, (N, k.shape[1]), torch.int64)
+    if freqs.dim() != 1 or 2 * freqs.shape[0] > dh:
+        raise ValueError(f"freqs: shape {tuple(freqs.shape)}, expected [pairs] of at most {dh // 2} pairs")
+    _tensor("freqs", freqs, q, freqs.shape, torch.float64)
+    if freqs.requires_grad:
+        raise ValueError("freqs: has no gradient here (detach it)")
+    gain = float(gain)
+    if not math.isfinite(gain):
+        raise ValueError(f"gain: {gain}")
+    _no_tangents(q, k)
+    args = (q, k, q_pos, k_pos, freqs.contiguous(), bool(interleaved), gain)
+    if _tracked(q, k):
+        return _Rotate.apply(*args)
+    return _Rotate.run(*args, False)
+
+
+class _Rotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_pos, k_pos, freqs, interleaved, gain):
+        ctx.save_for_backward(q_pos, k_pos, freqs)
+        ctx.form = (interleaved, gain)
+        ctx.set_materialize_grads(False)
+        return _Rotate.run(q, k, q_pos, k_pos, freqs, interleaved, gain, False)
+
+    @staticmethod
+    def run(q, k, q_pos, k_pos, freqs, interleaved, gain, inverse):
+        lib, P = _capi.lib(), _capi.ptr
+        one = q if q is not None else k
+        dev, dh = one.device, one.shape[3]
+        outs, sides, held = [], [], []
+        for x, pos in ((q, q_pos), (k, k_pos)):
+            if x is None:
+                outs.append(None)
+                sides.append(None)
+                continue
+            x = _rows(x)
+            y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+            outs.append(y)
+            held.append(x)
+            sides.append(_capi.RotarySide(P(x), P(y), P(pos), x.shape[1], *x.stride()[:3], *pos.stride(), x.shape[2]))
+        if sides[0] is None:
+            sides = [sides[1], None]
+        ref = [None if s is None else ctypes.byref(s) for s in sides]
+        with _guard(dev):
+            _capi.check(lib.sgl_rotary(_capi.DTYPES[one.dtype], one.shape[0], dh, 2 * freqs.shape[0], *ref, P(freqs),
+                                       interleaved, gain, inverse, _capi.stream_of(dev)), "rotate")
+        return tuple(outs)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        if gq is None and gk is None:
+            return (None,) * 7
+        q_pos, k_pos, freqs = ctx.saved_tensors
+        dq, dk = _Rotate.run(gq, gk, q_pos, k_pos, freqs, *ctx.form, True)
+        return dq, dk, None, None, None, None, None
