@@ -993,29 +993,34 @@ int sgl_candidates_teacher(int64_t n, int32_t k, int64_t v, const int64_t *ids,
                            const float *logits, float temperature,
                            int32_t *ids_out, float *weight, float *konst,
                            hipStream_t stream);
-/* what: 0 the loss alone, 1 the loss with dir, 2 the backward. */
-size_t sgl_candidates_workspace_bytes(const sgl_candidates *problem,
+/* what: 0 the loss alone, 1 the loss with dir, 2 the backward; k targets a row. */
+size_t sgl_candidates_workspace_bytes(const sgl_candidates *problem, int32_t k,
                                       int32_t what);
+/* Whether n rows with labels are worked on in an order of their own (rows
+ * without a target set aside): the forward then takes `order` int32 [n + 1]. */
+int32_t sgl_candidates_orders(int64_t n);
 /* loss [n] = temperature^2 (konst + sum_k weight (lse - s_id)). Targets: either
  * `target` int64 [n] (one a row at weight 1; negative: the row's loss is 0;
  * past the table: NaN; k = 1) or ids, weight, konst of
  * sgl_candidates_teacher. A target that is left out: inf. For the backward
  * (NULL: not kept): stat fp32 [2, n], dir fp32 [n, dim] (the loss's direction
- * in h), and with `target` ids_out int32 [n]. Rows whose loss is 0, inf or NaN
- * for these reasons have no gradient. */
+ * in h), with `target` ids_out int32 [n]; `order` (written; NULL: as they are)
+ * where sgl_candidates_orders says so. Rows whose loss is 0, inf or NaN for these
+ * reasons have no gradient. */
 int sgl_candidates_forward(const sgl_candidates *problem,
                            const int64_t *target, const int32_t *ids,
                            const float *weight, const float *konst, int32_t k,
                            float *loss, float *stat, float *dir,
-                           int32_t *ids_out, void *workspace,
+                           int32_t *ids_out, int32_t *order, void *workspace,
                            size_t workspace_bytes, hipStream_t stream);
 /* g [n] -> dh (like h, contiguous; from dir; NULL: not computed), dtable (like
  * the table, contiguous; NULL: not computed) and with it dbias fp32 [v] (or
- * NULL). weight NULL: 1 (ids_out of the forward). */
+ * NULL). weight NULL: 1 (ids_out of the forward, k = 1); order: the forward's. */
 int sgl_candidates_backward(const sgl_candidates *problem, const float *stat,
                             const int32_t *ids, const float *weight, int32_t k,
-                            const float *dir, const float *g, void *dh,
-                            void *dtable, float *dbias, void *workspace,
+                            const int32_t *order, const float *dir,
+                            const float *g, void *dh, void *dtable,
+                            float *dbias, void *workspace,
                             size_t workspace_bytes, hipStream_t stream);
 
 /* One tensor of a rotation: x [n, len, heads, dh] at its strides, y

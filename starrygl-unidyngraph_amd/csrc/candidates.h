@@ -106,41 +106,68 @@ struct Tile32 {
   }
 };
 
-// A tile's YT rows on their way from memory to LDS: 16 bytes a load, a row's
-// partial last one taken from D - E (it writes what its neighbour writes, with
-// the same values; columns past D are cleared once). Loads and stores are then
-// all whole and unconditional. Rows past `rows` are read as the last one and
-// written as zeros, as are those with `out` set: they may hold anything.
+// A tile's YT rows on their way from memory to LDS: 16 bytes a load, eight
+// lanes a row and 128 bytes of it, 32 rows a step. A row's partial last load is
+// taken from D - E (it writes what its neighbour writes, with the same values;
+// columns past D are cleared once), so that loads and stores are all whole.
+// Rows past the tensor's end are read as the last one and written as zeros, as
+// are those marked -inf: they may hold anything.
+constexpr int64_t kMaxStride = 1 << 22;   // of a row: a tile's offsets stay in 32 bits
 template <typename T, int DP, int YT>
 struct Stage {
   using Tl = Tile32<T, DP>;
-  static constexpr int E = Tl::E, UPR = Tl::UPR, NL = YT * UPR / kBlock;
-  static_assert(YT * UPR % kBlock == 0, "whole rounds of the workgroup");
-  FragOf<T> f[NL];
-  bool out[NL];
-  static __device__ __forceinline__ int row(int i) { return (int(threadIdx.x) + i * kBlock) / UPR; }
-  static __device__ __forceinline__ int col(int i, int D) {
-    return min((int(threadIdx.x) + i * kBlock) % UPR * E, D - E);
-  }
-  // base: the tile's first row
-  __device__ __forceinline__ void fetch(const T *base, int64_t stride, int64_t rows, int D) {
+  static constexpr int E = Tl::E, CB = Tl::UPR / 8, RB = YT / 32, SZ = int(sizeof(T));
+  static_assert(kBlock == 256 && YT % 32 == 0 && Tl::UPR % 8 == 0, "eight lanes a row of 32");
+  FragOf<T> f[RB][CB];
+  float mark[RB];      // a value that may still be on its way
+  uint32_t from[CB];   // bytes from the tile's first row
+  int to[CB];          // elements of the tile
+  int stride;          // bytes
+  __device__ __forceinline__ Stage(int64_t row_stride, int D) : stride(int(row_stride) * SZ) {
+    const int r = threadIdx.x >> 3;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int r = int(min(int64_t(row(i)), rows - 1));
-      out[i] = row(i) >= rows;
-      __builtin_memcpy(&f[i], base + r * stride + col(i, D), sizeof(f[i]));
+    for (int c = 0; c < CB; ++c) {
+      const int col = min((c * 8 + int(threadIdx.x & 7)) * E, D - E);
+      from[c] = uint32_t(r * stride + col * SZ);
+      to[c] = r * Tl::LD + col;
     }
   }
-  __device__ __forceinline__ void put(T *tile, int D) const {
+  // base: the tile's first row, of `rows` to the end; marks (or NULL): a value of each
+  __device__ __forceinline__ void fetch(const T *base, int rows, const float *marks) {
+    const char *b = reinterpret_cast<const char *>(base);
+    const int r = threadIdx.x >> 3;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const FragOf<T> g = out[i] ? zero_frag<T>() : f[i];
-      __builtin_memcpy(tile + row(i) * Tl::LD + col(i, D), &g, sizeof(g));
+    for (int i = 0; i < RB; ++i) {
+      // (rows past the end: back to the last one)
+      const int back = rows >= YT ? 0 : max(32 * i + r - (rows - 1), 0);
+#pragma unroll
+      for (int c = 0; c < CB; ++c)
+        __builtin_memcpy(&f[i][c], b + (from[c] + uint32_t((32 * i - back) * stride)), sizeof(f[i][c]));
+      if (marks != nullptr) mark[i] = marks[32 * i + r - back];
+    }
+  }
+  __device__ __forceinline__ void put(T *tile, int rows, bool marked) const {
+    const int r = threadIdx.x >> 3;
+    if (!marked && rows >= YT) {
+#pragma unroll
+      for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int c = 0; c < CB; ++c) __builtin_memcpy(tile + to[c] + 32 * i * Tl::LD, &f[i][c], sizeof(f[i][c]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        const bool out = 32 * i + r >= rows || (marked && mark[i] == -INFINITY);
+#pragma unroll
+        for (int c = 0; c < CB; ++c) {
+          const FragOf<T> g = out ? zero_frag<T>() : f[i][c];
+          __builtin_memcpy(tile + to[c] + 32 * i * Tl::LD, &g, sizeof(g));
+        }
+      }
     }
   }
   static __device__ __forceinline__ void clear(T *tile) {
-    for (int u = threadIdx.x; u < YT * UPR; u += kBlock)
-      *reinterpret_cast<FragOf<T> *>(tile + u / UPR * Tl::LD + u % UPR * E) = zero_frag<T>();
+    for (int u = threadIdx.x; u < YT * Tl::UPR; u += kBlock)
+      *reinterpret_cast<FragOf<T> *>(tile + u / Tl::UPR * Tl::LD + u % Tl::UPR * E) = zero_frag<T>();
   }
 };
 // A lane's fragments of an outer row (zeros past D and for `out`).
@@ -217,35 +244,68 @@ struct Problem {
   int D;
   float c, cb, scale, temperature;
 };
-// A candidate's bias to base 2. Finite ones stay finite.
-__device__ __forceinline__ float bias2(const Problem &p, int64_t v) {
-  const float b = p.bias[v], t = b * p.cb;
+// A bias to base 2. Finite ones stay finite.
+__device__ __forceinline__ float bias2_of(const Problem &p, float b) {
+  const float t = b * p.cb;
   return fabsf(t) == INFINITY && fabsf(b) != INFINITY ? copysignf(FLT_MAX, b) : t;
 }
+__device__ __forceinline__ float bias2(const Problem &p, int64_t v) { return bias2_of(p, p.bias[v]); }
+
+// Outer tiles x inner tiles in one line, outer first, shared out evenly: a
+// workgroup w takes units [b_w, b_(w+1)) of it, b_w = w units / groups, and so
+// pieces of one or more outer tiles; the piece of outer tile x of workgroup w is
+// number w + x (each step along the line raises one of the two or both).
+// Whole rounds of the GPU then cost nothing, whatever the numbers of tiles are
+// (600 rows are three tiles of 256 over 256 workgroups).
+struct Line {
+  int64_t units;
+  int inner, groups;
+  __host__ __device__ Line(int64_t outer, int64_t in, int most)
+      : units(outer * in), inner(int(in)), groups(units < most ? int(units) : most) {}
+  __device__ __forceinline__ int64_t begin(int64_t w) const { return w * units / groups; }
+  __device__ __forceinline__ int64_t group_of(int64_t unit) const { return ((unit + 1) * groups - 1) / units; }
+};
+constexpr int kGroups = 256;   // workgroups of a launch: one a CU
 
 // ------------------------------------------------------------------ launches
-// What a forward leaves for each split of the table and row (its own maximum
-// as used, its sum) and, with `dir`, sum_v p_v w_v at that maximum.
-struct Partials {
-  float *m, *l, *o;   // [splits][N], [splits][N], [splits][N][dp]
-  int64_t splits;
-  int dp;
+// Rows in the order that they are worked on: those with a target first.
+// order, live NULL: all, as they are.
+struct Order {
+  const int32_t *order;   // [N]
+  const int32_t *live;    // [1]: how many have one
+  __device__ __forceinline__ int64_t row(int64_t at) const { return order != nullptr ? order[at] : at; }
+  __device__ __forceinline__ int64_t count(int64_t N) const { return live != nullptr ? int64_t(*live) : N; }
 };
-int64_t forward_splits(int32_t dtype, const Problem &p, bool dir);
+// What a forward leaves for each piece (Line) of 32 wx rows and WY waves
+// along the table: its own maximum as used, its sum and, with a direction,
+// sum_v p_v w_v at that maximum.
+struct Partials {
+  float *m, *l, *o;   // [pieces][wy][rows], the same, [pieces][wy][rows][dp]
+  int64_t ytiles;
+  int rows, wy, dp;
+};
 int padded_dim(int D);
-void forward_partials(int32_t dtype, const Problem &p, const Partials &out, bool dir, hipStream_t stream);
+Partials forward_shape(int32_t dtype, const Problem &p);   // (without its arrays)
+void forward_partials(int32_t dtype, const Problem &p, const Order &order, const Partials &out, hipStream_t stream);
 
 struct RowCoef {
   const float *nm, *gl, *gq;   // [N]: minus the maximum, g T / l, g T (dead rows: -inf, 0, 0)
-  const int32_t *ids;          // [N][K], -1: none; no candidate twice in a row
-  const float *weight;         // [N][K] or NULL: 1
+  const int32_t *live;         // [1] or NULL: rows that count (the first ones)
+  const int32_t *ids;          // [N], -1: none, with index NULL; else
+  const int32_t *index;        // [ytiles][vblocks + 1]: a row tile's entries by candidate block
+  const int2 *entries;         // [N K], a row tile's first at tile * rows * K: candidate of the block * 64 + row
+                               // of the tile, weight
+  int64_t vblocks;
   int K;
 };
-int64_t table_grad_splits(int32_t dtype, const Problem &p);
-// dtable (type of the table, contiguous) and dbias (or NULL); part: with more
-// than one split fp32 [splits][V][dp + 1].
+void route_targets(int32_t dtype, int64_t N, int64_t V, int K, const int32_t *ids, const float *weight, int32_t *index,
+                   int2 *entries, hipStream_t stream);
+int table_grad_tile(int32_t dtype);     // rows of a tile
+int table_grad_block(int32_t dtype);    // candidates of a wave
+// fp32 elements of `part` (0: not needed).
+int64_t table_grad_part(int32_t dtype, const Problem &p);
 void table_grad(int32_t dtype, const Problem &p, const RowCoef &r, void *dtable, float *dbias, float *part,
-                int64_t splits, hipStream_t stream);
+                hipStream_t stream);
 
 }  // namespace cand
 }  // namespace sgl

@@ -85,9 +85,38 @@ __global__ __launch_bounds__(kBlock) void k_teacher(TeacherArgs a) {
   if (lane == 0) a.konst[n] = bad ? NAN : live_row ? konst : 0.f;
 }
 
+// ------------------------------------------------------------------ the rows with a target first
+// order[]: the rows with a target in their order, then the others; live[0]: how
+// many have one. A workgroup counts the targets before its 1,024 rows itself
+// (a quarter of a megabyte at most a workgroup up to kOrderMost rows).
+constexpr int kOrderRows = 1024;
+constexpr int64_t kOrderLeast = 1024, kOrderMost = 1 << 18;
+__global__ __launch_bounds__(kOrderRows) void k_order(const int64_t *target, int64_t N, int64_t V, int32_t *order,
+                                                      int32_t *live) {
+  __shared__ int waves[kOrderRows / kWave];
+  const int tid = threadIdx.x;
+  const int64_t n0 = int64_t(blockIdx.x) * kOrderRows, n = n0 + tid;
+  auto has = [&](int64_t at) { return uint64_t(target[at]) < uint64_t(V); };
+  int count = 0, total = 0;
+  for (int64_t i = tid; i < N; i += kOrderRows) {
+    const int on = has(i) ? 1 : 0;
+    total += on;
+    if (i < n0) count += on;
+  }
+  int before, all;
+  block_exclusive_scan<int, kOrderRows>(count, waves, before);
+  block_exclusive_scan<int, kOrderRows>(total, waves, all);
+  const bool here = n < N, on = here && has(n);
+  int ignored;
+  const int at = before + block_exclusive_scan<int, kOrderRows>(on ? 1 : 0, waves, ignored);
+  if (here) order[on ? at : all + (n - at)] = int32_t(n);
+  if (n == 0) *live = all;
+}
+
 // ------------------------------------------------------------------ joining the pieces
 struct FinishArgs {
   Problem p;
+  Order order;
   Partials in;
   const int64_t *target;   // [N], or NULL:
   const int32_t *ids;      // [N][K]
@@ -97,32 +126,43 @@ struct FinishArgs {
   int32_t *ids_out;           // of `target`
 };
 constexpr int kCols = kMaxDim / kWave;   // columns of a lane
+constexpr int kBatch = 8;                // targets whose rows are on their way together
 
 // W waves a row, 4 / W rows a workgroup.
 template <typename T, int W, bool DIR>
 __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
   __shared__ float parts[kWaves][DIR ? kMaxDim : 1];
-  __shared__ float sums[kWaves];
-  __shared__ int outs[kWaves];
+  __shared__ float sums[kWaves][3];
   const Problem &p = a.p;
   const int lane = threadIdx.x & 63, wave = attn::wave_index(), w = wave % W;
-  const int64_t n = int64_t(blockIdx.x) * (kWaves / W) + wave / W;
-  const bool here = n < p.N;
-  const int64_t row = here ? n : p.N - 1;   // (a row past the end joins the barriers)
+  const int64_t at = int64_t(blockIdx.x) * (kWaves / W) + wave / W;
+  const bool here = at < p.N;
+  const int64_t pos = here ? at : p.N - 1;   // (a row past the end joins the barriers)
+  const int64_t row = a.order.row(pos), live_rows = a.order.count(p.N);
   const T *h = static_cast<const T *>(p.h) + row * p.hs;
+  const int64_t target = a.target != nullptr ? a.target[row] : 0;
 
+  // the row's partials: the waves along the table of consecutive pieces
+  int n = 0;
+  int64_t first = 0;
+  if (pos < live_rows) {
+    const Line line((live_rows + a.in.rows - 1) / a.in.rows, a.in.ytiles, kGroups);
+    const int64_t xt = pos / a.in.rows, w0 = line.group_of(xt * line.inner);
+    n = int(line.group_of((xt + 1) * line.inner - 1) - w0 + 1) * a.in.wy;
+    first = (w0 + xt) * a.in.wy * a.in.rows + (pos - xt * a.in.rows);
+  }
+  const float *pm = a.in.m + first, *pl = a.in.l + first;
   float mx = -INFINITY;
-  for (int64_t s = lane; s < a.in.splits; s += kWave) mx = fmaxf(mx, a.in.m[s * p.N + row]);
+  for (int s = lane; s < n; s += kWave) mx = fmaxf(mx, pm[s * a.in.rows]);
   mx = wave_max(mx);
   float l = 0.f;
-  for (int64_t s = lane; s < a.in.splits; s += kWave) {
-    const float m = a.in.m[s * p.N + row];
-    // (a piece without a live candidate has sum 0)
-    l += m == -INFINITY ? a.in.l[s * p.N + row] : a.in.l[s * p.N + row] * exp2_fast(m - mx);
+  for (int s = lane; s < n; s += kWave) {
+    const float m = pm[s * a.in.rows], y = pl[s * a.in.rows];
+    l += m == -INFINITY ? y : y * exp2_fast(m - mx);   // (a piece without a live candidate has sum 0)
   }
   l = wave_sum(l);
 
-  // the targets: sum of q (mx - s), and of q w
+  // the targets: sum of q (mx - s), of q, of q w
   float x[kCols], tw[kCols];
 #pragma unroll
   for (int j = 0; j < kCols; ++j) {
@@ -130,82 +170,93 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
     x[j] = d < p.D ? float(h[d]) : 0.f;
     tw[j] = 0.f;
   }
-  float far = 0.f, want = 0.f;
-  bool out = false;
-  for (int k = w; k < a.K; k += W) {
-    int64_t id;
-    float q = 1.f;
-    if (a.target != nullptr) {
-      id = a.target[row];
-      if (id >= p.V) id = -1;
-    } else {
-      id = a.ids[row * a.K + k];
-      q = a.weight[row * a.K + k];
+  float far = 0.f, want = 0.f, out = 0.f;
+  for (int k0 = w * kBatch; k0 < a.K; k0 += W * kBatch) {
+    int id = -1;
+    float q = 0.f, b = 0.f;
+    if (lane < kBatch && k0 + lane < a.K) {
+      if (a.target != nullptr) {
+        id = uint64_t(target) < uint64_t(p.V) ? int(target) : -1;
+        q = 1.f;
+      } else {
+        id = a.ids[row * a.K + k0 + lane];
+        q = a.weight[row * a.K + k0 + lane];
+      }
+      if (id < 0) q = 0.f;
+      else if (p.bias != nullptr) b = bias2(p, id);
     }
-    if (id < 0) continue;
-    const float b = p.bias != nullptr ? bias2(p, id) : 0.f;
     want += q;
     if (b == -INFINITY) {   // left out: its row is not read
-      out = true;
-      continue;
+      out = 1.f;
+      id = -1;
     }
-    const T *t = static_cast<const T *>(p.table) + id * p.ts;
-    float dot = 0.f;
+    float y[kBatch][kCols], dot[kBatch];
 #pragma unroll
-    for (int j = 0; j < kCols; ++j) {
-      const int d = lane + kWave * j;
-      const float y = d < p.D ? float(t[d]) : 0.f;
-      dot = fmaf(x[j], y, dot);
-      tw[j] = fmaf(q, y, tw[j]);
+    for (int i = 0; i < kBatch; ++i) {
+      const int c = __builtin_amdgcn_readlane(id, i);
+      const T *t = static_cast<const T *>(p.table) + int64_t(max(c, 0)) * p.ts;
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) {
+        const int d = lane + kWave * j;
+        y[i][j] = c >= 0 && d < p.D ? float(t[d]) : 0.f;
+      }
     }
-    far += q * (mx - fmaf(wave_sum(dot), p.c, b));
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const float qi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(q), i));
+      dot[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) {
+        dot[i] = fmaf(x[j], y[i][j], dot[i]);
+        tw[j] = fmaf(qi, y[i][j], tw[j]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) dot[i] = wave_sum(dot[i]);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (lane == i && id >= 0) far += q * (mx - fmaf(dot[i], p.c, b));
   }
+  far = wave_sum(far);
+  want = wave_sum(want);
+  out = wave_max(out);
   if constexpr (W > 1) {
-    if (lane == 0) sums[wave] = far, outs[wave] = out;
+    if (lane == 0) sums[wave][0] = far, sums[wave][1] = want, sums[wave][2] = out;
     __syncthreads();
-    far = 0.f;
-    out = false;
+    far = want = out = 0.f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) far += sums[i], out |= outs[i] != 0;
-    __syncthreads();
-    if (lane == 0) sums[wave] = want;
-    __syncthreads();
-    want = 0.f;
-#pragma unroll
-    for (int i = 0; i < W; ++i) want += sums[i];
+    for (int i = 0; i < W; ++i) far += sums[i][0], want += sums[i][1], out = fmaxf(out, sums[i][2]);
   }
   const bool wanted = !(want == 0.f);   // (NaN: a row that its teacher spoils)
-  const bool live = wanted && !out && mx > -INFINITY;
+  const bool spoilt = mx == -INFINITY && !(l == 0.f);   // (no score but NaN)
+  const bool grad = wanted && out == 0.f && (mx > -INFINITY || spoilt);
   if (here && w == 0 && lane == 0) {
     float loss;
     if (!wanted) {
-      loss = a.target != nullptr ? (a.target[n] >= p.V ? NAN : 0.f) : a.konst[n];
+      loss = a.target != nullptr ? (target >= p.V ? NAN : 0.f) : a.konst[row];
     } else if (mx == -INFINITY) {
-      loss = l == 0.f ? 0.f : NAN;   // no live candidate (or only NaN)
-    } else if (out) {
+      loss = spoilt ? NAN : 0.f;   // (no live candidate)
+    } else if (out != 0.f) {
       loss = INFINITY;
     } else {
-      const float konst = a.target != nullptr ? 0.f : a.konst[n];
+      const float konst = a.target != nullptr ? 0.f : a.konst[row];
       loss = p.temperature * p.temperature * (konst + kLn2 * (far + want * __builtin_amdgcn_logf(l)));
       loss = loss < 0.f ? 0.f : loss;   // (rounding: it is not negative)
     }
-    a.loss[n] = loss;
+    a.loss[row] = loss;
     if (a.stat != nullptr) {
-      const bool grad = live || (wanted && !out && l != 0.f);   // (NaN scores alone: NaN gradients)
-      a.stat[n] = grad ? mx : 0.f;
-      a.stat[p.N + n] = grad ? 1.f / l : 0.f;
+      a.stat[row] = grad ? mx : 0.f;
+      a.stat[p.N + row] = grad ? 1.f / l : 0.f;
     }
-    if (a.ids_out != nullptr) {
-      const int64_t t = a.target[n];
-      a.ids_out[n] = t >= 0 && t < p.V ? int32_t(t) : -1;
-    }
+    if (a.ids_out != nullptr) a.ids_out[row] = uint64_t(target) < uint64_t(p.V) ? int32_t(target) : -1;
   }
   if constexpr (DIR) {
     float o[kCols] = {};
-    const int64_t step = p.N * a.in.dp;
-    const float *src = a.in.o + row * a.in.dp;
-    for (int64_t s = w; s < a.in.splits; s += W) {
-      const float m = a.in.m[s * p.N + row];
+    const float *src = a.in.o + first * a.in.dp;
+    const int64_t step = int64_t(a.in.rows) * a.in.dp;
+#pragma unroll 4
+    for (int s = w; s < n; s += W) {
+      const float m = pm[s * a.in.rows];
       const float f = m == -INFINITY ? 1.f : exp2_fast(m - mx);
 #pragma unroll
       for (int j = 0; j < kCols; ++j) {
@@ -213,7 +264,6 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
         if (d < p.D) o[j] = fmaf(src[s * step + d], f, o[j]);
       }
     }
-    const bool grad = live || (wanted && !out && l != 0.f);
     if constexpr (W > 1) {
 #pragma unroll
       for (int j = 0; j < kCols; ++j) parts[wave][lane + kWave * j] = o[j] / l - tw[j];
@@ -228,32 +278,43 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
 #pragma unroll
         for (int i = 1; i < W; ++i) e += parts[i][d];
       }
-      if (here && d < p.D) a.dir[n * p.D + d] = grad ? e : 0.f;
+      if (here && d < p.D) a.dir[row * p.D + d] = grad ? e : 0.f;
     }
   }
 }
 
 // ------------------------------------------------------------------ the gradients' rows
+// In the order that the table's gradient takes them: with `order` the rows
+// that have a target, theirs packed.
 struct RowArgs {
   Problem p;
+  Order order;
   const float *stat, *dir, *g;
+  const int32_t *ids;        // [N] or NULL
   void *dh;                  // or NULL
   float *nm, *gl, *gq;       // or NULL
+  void *packed;              // [N][D], and their ids, with `order`
+  int32_t *packed_ids;
 };
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_rows(RowArgs a) {
   const Problem &p = a.p;
   const int lane = threadIdx.x & 63;
-  const int64_t n = int64_t(blockIdx.x) * kWaves + attn::wave_index();
-  if (n >= p.N) return;
+  const int64_t pos = int64_t(blockIdx.x) * kWaves + attn::wave_index();
+  if (pos >= p.N) return;
+  const int64_t n = a.order.row(pos);
   const float m = a.stat[n], il = a.stat[p.N + n];
   const bool live = !(il == 0.f);
   const float g = live ? a.g[n] * p.temperature : 0.f;
   if (a.nm != nullptr && lane == 0) {
-    a.nm[n] = !live ? -INFINITY : m == INFINITY ? NAN : -m;
-    a.gl[n] = g * il;
-    a.gq[n] = g;
+    a.nm[pos] = !live ? -INFINITY : m == INFINITY ? NAN : -m;
+    a.gl[pos] = g * il;
+    a.gq[pos] = g;
+    if (a.packed_ids != nullptr) a.packed_ids[pos] = a.ids[n];
   }
+  if (a.packed != nullptr && live)
+    for (int d = lane; d < p.D; d += kWave)
+      static_cast<T *>(a.packed)[pos * p.D + d] = static_cast<const T *>(p.h)[n * p.hs + d];
   if (a.dh != nullptr)
     for (int d = lane; d < p.D; d += kWave)
       static_cast<T *>(a.dh)[n * p.D + d] = T(live ? g * p.scale * a.dir[n * p.D + d] : 0.f);
@@ -268,7 +329,9 @@ int make_problem(const sgl_candidates *c, Problem &p) {
   // (a workgroup a row where four waves share one: 2^24 of 256 threads make a launch)
   SGL_REQUIRE(c->n >= 0 && c->n <= kMaxRows && c->v > 0 && c->v < INT32_MAX - 512,
               "candidates: %lld rows over %lld candidates are too many (or none)", (long long)c->n, (long long)c->v);
-  SGL_REQUIRE(c->h_stride >= 0 && c->table_stride >= 0, "candidates: negative row stride");
+  SGL_REQUIRE(c->h_stride >= 0 && c->table_stride >= 0 && c->h_stride <= kMaxStride && c->table_stride <= kMaxStride,
+              "candidates: row strides of %lld and %lld elements (0 to %lld)", (long long)c->h_stride,
+              (long long)c->table_stride, (long long)kMaxStride);
   SGL_REQUIRE(c->n == 0 || (c->h != nullptr && c->table != nullptr), "candidates: NULL array");
   SGL_REQUIRE(c->temperature > 0.f && c->temperature < INFINITY && c->scale - c->scale == 0.f,
               "candidates: scale %g, temperature %g", double(c->scale), double(c->temperature));
@@ -289,28 +352,43 @@ int make_problem(const sgl_candidates *c, Problem &p) {
 
 Partials carve_forward(void *ws, int32_t dtype, const Problem &p, bool dir, size_t *bytes) {
   Carver c(ws);
-  Partials out{};
-  out.splits = forward_splits(dtype, p, dir);
-  out.dp = padded_dim(p.D);
-  out.m = c.take<float>(size_t(out.splits) * size_t(p.N));
-  out.l = c.take<float>(size_t(out.splits) * size_t(p.N));
-  out.o = dir ? c.take<float>(size_t(out.splits) * size_t(p.N) * size_t(out.dp)) : nullptr;
+  Partials out = forward_shape(dtype, p);
+  const size_t pieces = size_t((p.N + out.rows - 1) / out.rows + kGroups) * size_t(out.wy) * size_t(out.rows);
+  out.m = c.take<float>(pieces);
+  out.l = c.take<float>(pieces);
+  out.o = dir ? c.take<float>(pieces * size_t(out.dp)) : nullptr;
   *bytes = c.used;
   return out;
 }
 
+// Rows without a target are set aside where there are rows enough to gain more
+// than the launch that orders them costs.
+bool orders(int64_t N) { return N >= kOrderLeast && N <= kOrderMost; }
+
 struct Grad {
   float *nm, *gl, *gq, *part;
-  int64_t splits;
+  char *packed;
+  int32_t *ids, *index;
+  int2 *entries;
 };
-Grad carve_backward(void *ws, int32_t dtype, const Problem &p, size_t *bytes) {
+Grad carve_backward(void *ws, int32_t dtype, const Problem &p, int K, bool ordered, size_t *bytes) {
   Carver c(ws);
   Grad g{};
   g.nm = c.take<float>(size_t(p.N));
   g.gl = c.take<float>(size_t(p.N));
   g.gq = c.take<float>(size_t(p.N));
-  g.splits = table_grad_splits(dtype, p);
-  g.part = g.splits > 1 ? c.take<float>(size_t(g.splits) * size_t(p.V) * size_t(padded_dim(p.D) + 1)) : nullptr;
+  if (ordered) {
+    g.packed = c.take<char>(size_t(p.N) * size_t(p.D) * (dtype == SGL_FP32 ? 4 : 2));
+    g.ids = c.take<int32_t>(size_t(p.N));
+  }
+  if (K > 1) {
+    const int yt = table_grad_tile(dtype), vb = table_grad_block(dtype);
+    const size_t tiles = size_t((p.N + yt - 1) / yt);
+    g.index = c.take<int32_t>(tiles * size_t((p.V + vb - 1) / vb + 1));
+    g.entries = c.take<int2>(tiles * size_t(yt) * size_t(K));
+  }
+  const int64_t part = table_grad_part(dtype, p);
+  g.part = part > 0 ? c.take<float>(size_t(part)) : nullptr;
   *bytes = c.used;
   return g;
 }
@@ -318,7 +396,7 @@ Grad carve_backward(void *ws, int32_t dtype, const Problem &p, size_t *bytes) {
 template <typename T>
 void finish(const FinishArgs &a, hipStream_t stream) {
   // four waves a row where they have pieces or targets enough to share
-  const bool wide = a.in.splits >= 16 || a.K >= 16;
+  const bool wide = a.K >= 16 || a.in.wy > 1 || a.p.N <= 16 * a.in.rows;
   const dim3 grid(unsigned(wide ? a.p.N : (a.p.N + kWaves - 1) / kWaves));
   if (a.dir != nullptr) {
     if (wide) launch(&k_finish<T, kWaves, true>, grid, dim3(kBlock), 0, stream, a);
@@ -346,34 +424,41 @@ extern "C" int sgl_candidates_teacher(int64_t n, int32_t k, int64_t v, const int
   return SGL_OK;
 }
 
-extern "C" size_t sgl_candidates_workspace_bytes(const sgl_candidates *problem, int32_t what) {
+extern "C" size_t sgl_candidates_workspace_bytes(const sgl_candidates *problem, int32_t k, int32_t what) {
   Problem p;
-  if (make_problem(problem, p) != SGL_OK || p.N == 0) return 0;
+  if (make_problem(problem, p) != SGL_OK || p.N == 0 || k <= 0 || k > kMaxTargets) return 0;
   size_t bytes = 0;
-  if (what == 2) carve_backward(nullptr, problem->dtype, p, &bytes);
+  if (what == 2) carve_backward(nullptr, problem->dtype, p, k, k == 1 && orders(p.N), &bytes);
   else carve_forward(nullptr, problem->dtype, p, what == 1, &bytes);
   return bytes;
 }
 
+extern "C" int32_t sgl_candidates_orders(int64_t n) { return orders(n) ? 1 : 0; }
+
 extern "C" int sgl_candidates_forward(const sgl_candidates *problem, const int64_t *target, const int32_t *ids,
                                       const float *weight, const float *konst, int32_t k, float *loss, float *stat,
-                                      float *dir, int32_t *ids_out, void *workspace, size_t workspace_bytes,
-                                      hipStream_t stream) {
+                                      float *dir, int32_t *ids_out, int32_t *order, void *workspace,
+                                      size_t workspace_bytes, hipStream_t stream) {
   Problem p;
   if (const int rc = make_problem(problem, p)) return rc;
   SGL_REQUIRE(k > 0 && k <= kMaxTargets && (target == nullptr || k == 1), "candidates_forward: %d targets a row", k);
   if (p.N == 0) return SGL_OK;
-  SGL_REQUIRE(loss && (target != nullptr ? ids == nullptr : ids && weight && konst && !ids_out),
+  SGL_REQUIRE(loss && (target != nullptr ? ids == nullptr : ids && weight && konst && !ids_out && !order),
               "candidates_forward: NULL array, or labels and a teacher's entries at once");
   SGL_REQUIRE(dir == nullptr || stat != nullptr, "candidates_forward: dir without stat");
+  SGL_REQUIRE(order == nullptr || orders(p.N), "candidates_forward: no order of %lld rows", (long long)p.N);
   size_t need = 0;
   const Partials part = carve_forward(workspace, problem->dtype, p, dir != nullptr, &need);
   if (workspace == nullptr || workspace_bytes < need) {
     sgl::set_error("candidates_forward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     return SGL_ERR_WORKSPACE;
   }
-  forward_partials(problem->dtype, p, part, dir != nullptr, stream);
-  const FinishArgs a{p, part, target, ids, weight, konst, k, loss, stat, dir, ids_out};
+  const Order o{order, order != nullptr ? order + p.N : nullptr};
+  if (order != nullptr)
+    sgl::launch(&k_order, dim3(unsigned((p.N + kOrderRows - 1) / kOrderRows)), dim3(kOrderRows), 0, stream, target, p.N,
+                p.V, order, order + p.N);
+  forward_partials(problem->dtype, p, o, part, stream);
+  const FinishArgs a{p, o, part, target, ids, weight, konst, k, loss, stat, dir, ids_out};
   if (problem->dtype == SGL_FP32) finish<float>(a, stream);
   else if (problem->dtype == SGL_BF16) finish<bf16_t>(a, stream);
   else finish<fp16_t>(a, stream);
@@ -382,32 +467,44 @@ extern "C" int sgl_candidates_forward(const sgl_candidates *problem, const int64
 }
 
 extern "C" int sgl_candidates_backward(const sgl_candidates *problem, const float *stat, const int32_t *ids,
-                                       const float *weight, int32_t k, const float *dir, const float *g, void *dh,
-                                       void *dtable, float *dbias, void *workspace, size_t workspace_bytes,
-                                       hipStream_t stream) {
+                                       const float *weight, int32_t k, const int32_t *order, const float *dir,
+                                       const float *g, void *dh, void *dtable, float *dbias, void *workspace,
+                                       size_t workspace_bytes, hipStream_t stream) {
   Problem p;
   if (const int rc = make_problem(problem, p)) return rc;
   SGL_REQUIRE(k > 0 && k <= kMaxTargets, "candidates_backward: %d targets a row", k);
   SGL_REQUIRE(p.N > 0, "candidates_backward: no rows");
-  SGL_REQUIRE(stat && g && (dh == nullptr || dir) && (dtable == nullptr || ids), "candidates_backward: NULL array");
+  SGL_REQUIRE(stat && g && (dh == nullptr || dir) && (dtable == nullptr || (ids && (k == 1 || weight))),
+              "candidates_backward: NULL array");
   SGL_REQUIRE(dbias == nullptr || dtable != nullptr, "candidates_backward: dbias without dtable");
+  SGL_REQUIRE(order == nullptr || (k == 1 && orders(p.N)), "candidates_backward: no order of %lld rows", (long long)p.N);
   Grad w{};
   if (dtable != nullptr) {
     size_t need = 0;
-    w = carve_backward(workspace, problem->dtype, p, &need);
+    w = carve_backward(workspace, problem->dtype, p, k, order != nullptr, &need);
     if (workspace == nullptr || workspace_bytes < need) {
       sgl::set_error("candidates_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
       return SGL_ERR_WORKSPACE;
     }
   }
-  const RowArgs a{p, stat, dir, g, dh, w.nm, w.gl, w.gq};
+  const Order o{order, order != nullptr ? order + p.N : nullptr};
+  const RowArgs a{p, o, stat, dir, g, ids, dh, w.nm, w.gl, w.gq, w.packed, w.ids};
   const dim3 grid(unsigned((p.N + kWaves - 1) / kWaves));
   if (problem->dtype == SGL_FP32) sgl::launch(&k_rows<float>, grid, dim3(kBlock), 0, stream, a);
   else if (problem->dtype == SGL_BF16) sgl::launch(&k_rows<bf16_t>, grid, dim3(kBlock), 0, stream, a);
   else sgl::launch(&k_rows<fp16_t>, grid, dim3(kBlock), 0, stream, a);
   if (dtable != nullptr) {
-    const RowCoef r{w.nm, w.gl, w.gq, ids, weight, k};
-    table_grad(problem->dtype, p, r, dtable, dbias, w.part, w.splits, stream);
+    RowCoef r{w.nm, w.gl, w.gq, o.live, w.ids != nullptr ? w.ids : ids, w.index, w.entries, 0, k};
+    if (w.packed != nullptr) {
+      p.h = w.packed;
+      p.hs = p.D;
+    }
+    if (k > 1) {
+      const int vb = table_grad_block(problem->dtype);
+      r.vblocks = (p.V + vb - 1) / vb;
+      route_targets(problem->dtype, p.N, p.V, k, ids, weight, w.index, w.entries, stream);
+    }
+    table_grad(problem->dtype, p, r, dtable, dbias, w.part, stream);
   }
   SGL_CHECK_LAUNCH();
   return SGL_OK;

@@ -11,8 +11,8 @@ struct BwdArgs {
   Problem p;
   RowCoef r;
   void *dtable;
-  float *dbias, *part;
-  int64_t xtiles, ytiles, splits;
+  float *dbias, *part;   // part: [pieces][candidates of a workgroup][dp + 1]
+  int most;              // workgroups at most
 };
 
 // fp16: a coefficient goes into the product times a power of two a candidate
@@ -34,23 +34,60 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
   constexpr int LD = Tl::LD;
   constexpr int YT = sizeof(T) == 4 ? 32 : 64, YS = YT / 32, XT = 32 * XB * kWaves, QL = YT + 4;
   constexpr bool HALF = std::is_same_v<T, fp16_t>;
+  constexpr int WV = 32 * XB;   // candidates of a wave
   extern __shared__ __align__(16) char lds[];
   T *tiles = reinterpret_cast<T *>(lds);
   float *coef = reinterpret_cast<float *>(lds + size_t(2) * YT * LD * sizeof(T));   // [2][3][YT]
-  float *q = coef + 2 * 3 * YT;   // [XT][QL]: what the tile's rows want of the candidates; zero between uses
-  int *hit = reinterpret_cast<int *>(q + XT * QL);   // [waves]: whether any of a wave's is wanted
+  // [XT][QL]: what the tile's rows want of the candidates; zero between uses. A wave writes, reads and
+  // clears its own candidates' part.
+  float *q_all = coef + 2 * 3 * YT;
 
   const Problem &p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, col = lane & 31;
   const int wave = attn::wave_index();
-  const int64_t xt = int64_t(blockIdx.x) / a.splits, split = int64_t(blockIdx.x) % a.splits;
-  const int64_t t0 = split * a.ytiles / a.splits, t1 = (split + 1) * a.ytiles / a.splits;
-  const int64_t v0 = xt * XT;
+  float *q = q_all + wave * WV * QL;
+  const int64_t N = a.r.live != nullptr ? int64_t(*a.r.live) : p.N;
+  const Line line((p.V + XT - 1) / XT, max((N + YT - 1) / YT, int64_t(1)), a.most);
+  const int w = blockIdx.x;
+  if (w >= line.groups) return;
+  const int64_t u1 = line.begin(w + 1);
   const T *rows_h = static_cast<const T *>(p.h);
 
+  Stage<T, DP, YT> next(p.hs, p.D);
+  float nc[3];
+  int nid = -1, ne0 = 0, ne1 = 0;
+  auto fetch = [&](int t, int xt) {
+    const int64_t y0 = int64_t(t) * YT;
+    const int rows = max(int(min(N - y0, int64_t(YT))), 1);
+    next.fetch(rows_h + y0 * p.hs, rows, a.r.nm + y0);   // (a row without a gradient may hold anything)
+    if (tid < YT) {
+      const int64_t n = y0 + min(tid, rows - 1);
+      nc[0] = a.r.nm[n];
+      nc[1] = a.r.gl[n];
+      nc[2] = a.r.gq[n];
+    }
+    if (a.r.index == nullptr) {
+      nid = a.r.ids[y0 + min(lane, rows - 1)];
+    } else {
+      const int64_t vb = int64_t(xt) * kWaves + wave;
+      const int32_t *at = a.r.index + int64_t(t) * (a.r.vblocks + 1) + min(vb, a.r.vblocks - 1);
+      ne0 = attn::scalar_load(at);
+      ne1 = vb < a.r.vblocks ? attn::scalar_load(at + 1) : ne0;
+    }
+  };
+  for (int i = tid; i < XT * QL; i += kBlock) q_all[i] = 0.f;
+  Stage<T, DP, YT>::clear(tiles);
+  Stage<T, DP, YT>::clear(tiles + YT * LD);
+  int64_t u = line.begin(w);
+  int xt = int(u / line.inner), t = int(u - int64_t(xt) * line.inner), buf = 0;
+  fetch(t, xt);
+  __syncthreads();
+
+#pragma unroll 1
+  for (; u < u1; ++xt) {   // an outer tile's piece
   FragOf<T> xf[XB][NK];
   float b2[XB], db[XB], sc[XB];
-  const int64_t x0 = v0 + wave * (32 * XB) + col;
+  const int64_t x0 = int64_t(xt) * XT + wave * WV + col;
 #pragma unroll
   for (int xb = 0; xb < XB; ++xb) {
     const int64_t x = min(x0 + 32 * xb, p.V - 1);
@@ -66,56 +103,33 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[xb][d][r] = 0.f;
-
-  Stage<T, DP, YT> next;
-  float nc[3] = {-INFINITY, 0.f, 0.f};
-  auto fetch = [&](int64_t t) {
-    const int64_t y0 = t * YT, rows = p.N - y0;
-    next.fetch(rows_h + y0 * p.hs, p.hs, rows, p.D);
-    // rows without a gradient may hold anything
-#pragma unroll
-    for (int i = 0; i < next.NL; ++i)
-      next.out[i] |= a.r.nm[y0 + min(int64_t(next.row(i)), rows - 1)] == -INFINITY;
-    if (tid < YT) {
-      const bool ok = tid < rows;
-      const int64_t n = y0 + (ok ? tid : 0);
-      nc[0] = ok ? a.r.nm[n] : -INFINITY;
-      nc[1] = ok ? a.r.gl[n] : 0.f;
-      nc[2] = ok ? a.r.gq[n] : 0.f;
-    }
-  };
-  for (int i = tid; i < XT * QL; i += kBlock) q[i] = 0.f;
-  if (tid < kWaves) hit[tid] = 0;
-  Stage<T, DP, YT>::clear(tiles);
-  Stage<T, DP, YT>::clear(tiles + YT * LD);
-  __syncthreads();
-  if (t0 < t1) fetch(t0);
-
-  const int K = a.r.K;
+  const int first = t, end = int(min(int64_t(line.inner), t + (u1 - u)));
+  u += end - t;
 #pragma unroll 1
-  for (int64_t t = t0; t < t1; ++t) {
-    const int buf = int(t - t0) & 1;
+  for (; t < end; ++t) {
     T *tile = tiles + buf * YT * LD;
     float *cf = coef + buf * 3 * YT;
-    next.put(tile, p.D);
-    if (tid < YT) cf[tid] = nc[0], cf[YT + tid] = nc[1], cf[2 * YT + tid] = nc[2];
-    // the tile's targets among the workgroup's candidates
-    const int64_t y0 = t * YT, e0 = y0 * K;
-    const int ne = int(min(int64_t(YT), p.N - y0)) * K;
-    bool any = false;
-    for (int e = tid; e < ne; e += kBlock) any |= uint64_t(int64_t(a.r.ids[e0 + e]) - v0) < uint64_t(XT);
-    if (__syncthreads_or(any)) {   // (the waves are done with the tile before: q is clear)
-      for (int e = tid; e < ne; e += kBlock) {
-        const int64_t x = int64_t(a.r.ids[e0 + e]) - v0;
-        if (uint64_t(x) < uint64_t(XT)) {   // each place at most once: a row has a candidate once
-          q[x * QL + e / K] = a.r.weight != nullptr ? a.r.weight[e0 + e] : 1.f;
-          hit[int(x) / (32 * XB)] = 1;
-        }
-      }
-      __syncthreads();
+    buf ^= 1;
+    const int rows = int(min(N - int64_t(t) * YT, int64_t(YT)));
+    next.put(tile, rows, true);
+    if (tid < YT) {
+      cf[tid] = tid < rows ? nc[0] : -INFINITY;
+      cf[YT + tid] = tid < rows ? nc[1] : 0.f;
+      cf[2 * YT + tid] = tid < rows ? nc[2] : 0.f;
     }
-    if (t + 1 < t1) fetch(t + 1);
-    const bool wanted = hit[wave] != 0;
+    // what the tile's rows want of the wave's candidates: a row has a candidate once, so each place once
+    const int64_t mine = int64_t(nid) - (int64_t(xt) * XT + wave * WV);
+    const bool one = a.r.index == nullptr && lane < rows && nid >= 0 && uint64_t(mine) < uint64_t(WV);
+    const int e0 = ne0, e1 = ne1;
+    const int2 *entries = a.r.entries + int64_t(t) * YT * a.r.K;
+    const bool wanted = __any(one) || e0 < e1;
+    if (one) q[mine * QL + lane] = 1.f;
+    for (int e = e0 + lane; e < e1; e += kWave) {
+      const int2 x = entries[e];
+      q[(x.x >> 6) * QL + (x.x & 63)] = __int_as_float(x.y);
+    }
+    __syncthreads();
+    if (t + 1 < end || u < u1) fetch(t + 1 < end ? t + 1 : 0, t + 1 < end ? xt : xt + 1);
 #pragma unroll 1
     for (int ys = 0; ys < YS; ++ys) {
       const int row0 = ys * 32;
@@ -149,7 +163,7 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
 #pragma unroll
           for (int xb = 0; xb < XB; ++xb) {
             float w[4];
-            __builtin_memcpy(w, q + (wave * (32 * XB) + 32 * xb + col) * QL + row0 + 8 * i + 4 * h, sizeof(w));
+            __builtin_memcpy(w, q + (32 * xb + col) * QL + row0 + 8 * i + 4 * h, sizeof(w));
 #pragma unroll
             for (int v = 0; v < 4; ++v) s[xb][4 * i + v] = fmaf(-gq[v], w[v], s[xb][4 * i + v]);
           }
@@ -201,28 +215,33 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
         }
       }
     }
-    if (wanted) {   // the wave's own part: clear before the next tile's targets come
-      for (int i = lane; i < 32 * XB * QL; i += kWave) q[wave * 32 * XB * QL + i] = 0.f;
-      if (lane == 0) hit[wave] = 0;
+    if (wanted) {
+      attn::wave_sync();
+      if (one) q[mine * QL + lane] = 0.f;
+      for (int e = e0 + lane; e < e1; e += kWave) {
+        const int x = entries[e].x;
+        q[(x >> 6) * QL + (x & 63)] = 0.f;
+      }
     }
   }
 
+  const bool whole = first == 0 && end == line.inner;
 #pragma unroll
   for (int xb = 0; xb < XB; ++xb) {
     const int64_t x = x0 + 32 * xb;
     const float sum = pair_sum(db[xb]);
     if (x >= p.V) continue;
     const float by = HALF ? p.scale / sc[xb] : p.scale;
-    if (a.part != nullptr) {
-      float *row = a.part + (split * p.V + x) * (DP + 1);
+    if (!whole) {
+      float *row = a.part + (int64_t(w + xt) * XT + wave * WV + 32 * xb + col) * (DP + 1);
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float w[4];
+          float y[4];
 #pragma unroll
-          for (int v = 0; v < 4; ++v) w[v] = o[xb][d][4 * i + v] * by;
-          store_n(row + 32 * d + 8 * i + 4 * h, w);
+          for (int v = 0; v < 4; ++v) y[v] = o[xb][d][4 * i + v] * by;
+          store_n(row + 32 * d + 8 * i + 4 * h, y);
         }
       if (h == 0) row[DP] = sum;
     } else {
@@ -231,57 +250,121 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
       for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          f32x4 w;
+          f32x4 y;
 #pragma unroll
-          for (int v = 0; v < 4; ++v) w[v] = o[xb][d][4 * i + v] * by;
-          attn::store4<T>(row, 32 * d + 8 * i + 4 * h, p.D, w);
+          for (int v = 0; v < 4; ++v) y[v] = o[xb][d][4 * i + v] * by;
+          attn::store4<T>(row, 32 * d + 8 * i + 4 * h, p.D, y);
         }
       if (a.dbias != nullptr && h == 0) a.dbias[x] = sum;
     }
   }
+  t = 0;
+  }
 }
 
-// The splits' sums in their order, rounded once.
+// Candidates whose rows were shared out: the pieces' sums in their order,
+// rounded once.
 template <typename T>
-__global__ __launch_bounds__(256) void k_join_grad(const float *part, int64_t splits, int64_t V, int D, int dp,
-                                                   T *dtable, float *dbias) {
-  const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (at >= V * (D + 1)) return;
-  const int64_t v = at / (D + 1);
-  const int d = int(at - v * (D + 1));
-  if (d == D && dbias == nullptr) return;
-  const float *src = part + v * (dp + 1) + (d == D ? dp : d);
+__global__ __launch_bounds__(kBlock) void k_join_grad(BwdArgs a, int xtile, int ytile, int dp) {
+  const Problem &p = a.p;
+  const int64_t at = int64_t(blockIdx.x) * kBlock + threadIdx.x;
+  if (at >= p.V * (p.D + 1)) return;
+  const int64_t v = at / (p.D + 1);
+  const int d = int(at - v * (p.D + 1));
+  if (d == p.D && a.dbias == nullptr) return;
+  const int64_t N = a.r.live != nullptr ? int64_t(*a.r.live) : p.N;
+  const Line line((p.V + xtile - 1) / xtile, max((N + ytile - 1) / ytile, int64_t(1)), a.most);
+  const int64_t xt = v / xtile, w0 = line.group_of(xt * line.inner), w1 = line.group_of((xt + 1) * line.inner - 1);
+  if (w0 == w1) return;   // (written whole)
+  const int64_t step = int64_t(xtile) * (dp + 1);
+  const float *src = a.part + (w0 + xt) * step + (v - xt * xtile) * (dp + 1) + (d == p.D ? dp : d);
+  const int n = int(w1 - w0) + 1;
   float x = 0.f;
-  int64_t s = 0;
-  for (; s + 8 <= splits; s += 8) {
+  int s = 0;
+  for (; s + 8 <= n; s += 8) {
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = src[(s + i) * V * (dp + 1)];
+    for (int i = 0; i < 8; ++i) y[i] = src[(s + i) * step];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x += y[i];
   }
-  for (; s < splits; ++s) x += src[s * V * (dp + 1)];
-  if (d == D) dbias[v] = x;
-  else dtable[v * D + d] = T(x);
+  for (; s < n; ++s) x += src[s * step];
+  if (d == p.D) a.dbias[v] = x;
+  else static_cast<T *>(a.dtable)[v * p.D + d] = T(x);
 }
 
-// Which form: candidates of a workgroup, rows of a tile.
+// ------------------------------------------------------------------ several targets a row
+// A row tile's entries in the order of the candidates' blocks (those of a
+// wave), with the place where each block begins: one workgroup a row tile
+// counts, sums and places them in LDS, kBins blocks at a time. (The order of a
+// block's entries varies; each is a place of its own.)
+constexpr int kRouteBlock = 1024, kBins = 12 * kRouteBlock;
+struct RouteArgs {
+  const int32_t *ids;     // [N][K]
+  const float *weight;
+  int64_t N, vblocks;
+  int K, ytile, vblock;
+  int32_t *index;
+  int2 *entries;
+};
+__global__ __launch_bounds__(kRouteBlock) void k_route(RouteArgs a) {
+  __shared__ int bins[kBins];
+  __shared__ int waves[kRouteBlock / kWave];
+  const int tid = threadIdx.x;
+  const int64_t y0 = int64_t(blockIdx.x) * a.ytile, e0 = y0 * a.K;
+  const int n = int(min(int64_t(a.ytile), a.N - y0)) * a.K;
+  int32_t *index = a.index + int64_t(blockIdx.x) * (a.vblocks + 1);
+  int2 *entries = a.entries + int64_t(blockIdx.x) * a.ytile * a.K;
+  int base = 0;
+  for (int64_t b0 = 0; b0 < a.vblocks; b0 += kBins) {
+    for (int i = tid; i < kBins; i += kRouteBlock) bins[i] = 0;
+    __syncthreads();
+    for (int e = tid; e < n; e += kRouteBlock) {
+      const int id = a.ids[e0 + e];
+      const int64_t b = id / a.vblock - b0;
+      if (id >= 0 && b >= 0 && b < kBins) atomicAdd(&bins[b], 1);
+    }
+    __syncthreads();
+    constexpr int PER = kBins / kRouteBlock;
+    int c[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      c[i] = sum;
+      sum += bins[tid * PER + i];
+    }
+    int total;
+    const int before = base + block_exclusive_scan<int, kRouteBlock>(sum, waves, total);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      bins[tid * PER + i] = before + c[i];
+      if (b0 + tid * PER + i <= a.vblocks) index[b0 + tid * PER + i] = before + c[i];
+    }
+    __syncthreads();
+    for (int e = tid; e < n; e += kRouteBlock) {
+      const int id = a.ids[e0 + e];
+      const int64_t b = id / a.vblock - b0;
+      if (id >= 0 && b >= 0 && b < kBins)
+        entries[atomicAdd(&bins[b], 1)] =
+            make_int2((id - int(b0 + b) * a.vblock) * 64 + e / a.K, __float_as_int(a.weight[e0 + e]));
+    }
+    base += total;
+    __syncthreads();
+  }
+  if (tid == 0) index[a.vblocks] = base;
+}
+
+// Candidates of a workgroup, rows of a tile.
 template <typename T>
 constexpr int kXTile = sizeof(T) == 4 ? 128 : 256;
 template <typename T>
 constexpr int kYTile = sizeof(T) == 4 ? 32 : 64;
 
+// A workgroup an outer tile where whole rounds of them leave little over, else
+// the line shared out over one round.
 template <typename T>
-int64_t pieces_of(const Problem &p) {
-  const int64_t xt = (p.V + kXTile<T> - 1) / kXTile<T>, yt = (p.N + kYTile<T> - 1) / kYTile<T>;
-  int64_t best = 1;
-  double cost = 1e300;
-  for (int64_t s = 1; s <= std::min<int64_t>(yt, 256); ++s) {
-    const int64_t per = (yt + s - 1) / s, rounds = (xt * s + 255) / 256;
-    const double t = double(rounds) * (double(per) + 4.0) + (s > 1 ? 4.0 + 0.02 * double(s * xt) : 0.0);
-    if (t < cost) cost = t, best = s;
-  }
-  return best;
+int groups_of(const Problem &p) {
+  const int64_t xt = (p.V + kXTile<T> - 1) / kXTile<T>;
+  return xt >= 8 * kGroups ? int(xt) : kGroups;
 }
 
 template <typename T, int DB>
@@ -289,27 +372,32 @@ void run(const BwdArgs &a, hipStream_t stream) {
   constexpr int XB = sizeof(T) == 4 ? 1 : 2;
   constexpr int LD = Tile32<T, 32 * DB>::LD, YT = kYTile<T>, XT = kXTile<T>;
   static_assert(XT == 32 * XB * kWaves, "");
-  constexpr size_t bytes = size_t(2) * YT * LD * sizeof(T) + sizeof(float) * (6 * YT + XT * (YT + 4) + kWaves);
+  constexpr size_t bytes = size_t(2) * YT * LD * sizeof(T) + sizeof(float) * (6 * YT + XT * (YT + 4));
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
   auto *k = &k_table_grad<T, DB, XB>;
   (void)ensure_dynamic_lds(reinterpret_cast<const void *>(k), bytes);
-  launch(k, dim3(unsigned(a.xtiles * a.splits)), dim3(kBlock), bytes, stream, a);
+  const Line line((a.p.V + XT - 1) / XT, (a.p.N + YT - 1) / YT, a.most);
+  launch(k, dim3(unsigned(line.groups)), dim3(kBlock), bytes, stream, a);
 }
 template <typename T>
-void pick(const Problem &p, const RowCoef &r, void *dtable, float *dbias, float *part, int64_t splits,
-          hipStream_t stream) {
-  const BwdArgs a{p, r, dtable, dbias, splits > 1 ? part : nullptr, (p.V + kXTile<T> - 1) / kXTile<T>,
-                  (p.N + kYTile<T> - 1) / kYTile<T>, splits};
+void pick(const Problem &p, const RowCoef &r, void *dtable, float *dbias, float *part, hipStream_t stream) {
+  const BwdArgs a{p, r, dtable, dbias, part, groups_of<T>(p)};
   const int dp = padded_dim(p.D);
   if (dp == 64) run<T, 2>(a, stream);
   else if (dp == 128) run<T, 4>(a, stream);
   else if (dp == 192) run<T, 6>(a, stream);
   else run<T, 8>(a, stream);
-  if (splits > 1) {
+  if (part != nullptr) {
     const int64_t n = p.V * (p.D + 1);
-    launch(&k_join_grad<T>, dim3(unsigned((n + 255) / 256)), dim3(256), 0, stream, static_cast<const float *>(part),
-           splits, p.V, p.D, dp, static_cast<T *>(dtable), dbias);
+    launch(&k_join_grad<T>, dim3(unsigned((n + kBlock - 1) / kBlock)), dim3(kBlock), 0, stream, a, kXTile<T>, kYTile<T>,
+           dp);
   }
+}
+template <typename T>
+int64_t part_of(const Problem &p) {
+  const int64_t xt = (p.V + kXTile<T> - 1) / kXTile<T>;
+  if (groups_of<T>(p) == xt) return 0;
+  return (xt + kGroups) * kXTile<T> * (padded_dim(p.D) + 1);
 }
 
 }  // namespace
@@ -317,15 +405,24 @@ void pick(const Problem &p, const RowCoef &r, void *dtable, float *dbias, float 
 namespace sgl {
 namespace cand {
 
-int64_t table_grad_splits(int32_t dtype, const Problem &p) {
-  return dtype == SGL_FP32 ? pieces_of<float>(p) : pieces_of<bf16_t>(p);
+int table_grad_tile(int32_t dtype) { return dtype == SGL_FP32 ? kYTile<float> : kYTile<bf16_t>; }
+int table_grad_block(int32_t dtype) { return (dtype == SGL_FP32 ? kXTile<float> : kXTile<bf16_t>) / kWaves; }
+int64_t table_grad_part(int32_t dtype, const Problem &p) {
+  return dtype == SGL_FP32 ? part_of<float>(p) : part_of<bf16_t>(p);
+}
+
+void route_targets(int32_t dtype, int64_t N, int64_t V, int K, const int32_t *ids, const float *weight, int32_t *index,
+                   int2 *entries, hipStream_t stream) {
+  const int yt = table_grad_tile(dtype), vb = table_grad_block(dtype);
+  const RouteArgs a{ids, weight, N, (V + vb - 1) / vb, K, yt, vb, index, entries};
+  launch(&k_route, dim3(unsigned((N + yt - 1) / yt)), dim3(kRouteBlock), 0, stream, a);
 }
 
 void table_grad(int32_t dtype, const Problem &p, const RowCoef &r, void *dtable, float *dbias, float *part,
-                int64_t splits, hipStream_t stream) {
-  if (dtype == SGL_FP32) return pick<float>(p, r, dtable, dbias, part, splits, stream);
-  if (dtype == SGL_BF16) return pick<bf16_t>(p, r, dtable, dbias, part, splits, stream);
-  return pick<fp16_t>(p, r, dtable, dbias, part, splits, stream);
+                hipStream_t stream) {
+  if (dtype == SGL_FP32) return pick<float>(p, r, dtable, dbias, part, stream);
+  if (dtype == SGL_BF16) return pick<bf16_t>(p, r, dtable, dbias, part, stream);
+  return pick<fp16_t>(p, r, dtable, dbias, part, stream);
 }
 
 }  // namespace cand

@@ -9,8 +9,8 @@ using namespace sgl::cand;
 
 struct FwdArgs {
   Problem p;
+  Order order;
   Partials out;
-  int64_t xtiles, ytiles, splits, deal;   // splits: pieces of the table (each WY partials), dealt to `deal` XCDs
 };
 
 // fp16: p lies in 2^-24 .. 2^16, so the row's maximum is put at 2^7 (with the
@@ -21,6 +21,8 @@ constexpr float kTop = std::is_same_v<T, fp16_t> ? 7.f : 0.f;
 // this many powers of two: exact whichever maximum is used, and most tiles
 // then rescale nothing.
 constexpr float kSlack = 8.f;
+
+constexpr int64_t kFewRows = 32;   // up to here a workgroup's waves share them and split the table
 
 // XB blocks of 32 rows a wave; WX waves along the rows, 4 / WX along the table.
 template <typename T, int DB, int XB, int WX, bool DIR>
@@ -38,19 +40,39 @@ __global__ __launch_bounds__(kBlock, 1) void k_forward(FwdArgs a) {
   const Problem &p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = attn::wave_index(), wx = wave % WX, wy = wave / WX;
-  // workgroups of one piece of the table are dealt to one XCD: they share its L2
-  const int64_t id = blockIdx.x, j = id / a.deal;
-  const int64_t split = id % a.deal + a.deal * (j / a.xtiles), xt = j % a.xtiles;
-  if (split >= a.splits) return;
-  const int64_t t0 = split * a.ytiles / a.splits, t1 = (split + 1) * a.ytiles / a.splits;
+  constexpr int XT = 32 * XB * WX;
+  const int64_t N = a.order.count(p.N);
+  const Line line((N + XT - 1) / XT, (p.V + YT - 1) / YT, kGroups);
+  const int w = blockIdx.x;
+  if (w >= line.groups) return;
+  const int64_t u1 = line.begin(w + 1);
   const T *table = static_cast<const T *>(p.table);
+  const bool biased = p.bias != nullptr;
 
+  Stage<T, DP, YT> next(p.ts, p.D);
+  float nb = 0.f;   // the bias of the next tile's row tid
+  auto rows_of = [&](int t) { return int(min(p.V - int64_t(t) * YT, int64_t(YT))); };
+  auto fetch = [&](int t) {
+    const int64_t y0 = int64_t(t) * YT;
+    const int rows = rows_of(t);
+    next.fetch(table + y0 * p.ts, rows, biased ? p.bias + y0 : nullptr);
+    if (biased && tid < YT) nb = p.bias[y0 + min(tid, rows - 1)];
+  };
+#pragma unroll
+  for (int i = 0; i < NBUF; ++i) Stage<T, DP, YT>::clear(tiles + i * YT * LD);
+  int64_t u = line.begin(w);
+  int xt = int(u / line.inner), t = int(u - int64_t(xt) * line.inner), buf = 0;
+  fetch(t);
+  __syncthreads();
+
+#pragma unroll 1
+  for (; u < u1; ++xt) {   // an outer tile's piece
   FragOf<T> xf[XB][NK];
-  const int64_t x0 = (xt * WX + wx) * (32 * XB) + (lane & 31);
+  const int64_t x0 = (int64_t(xt) * WX + wx) * (32 * XB) + (lane & 31);
 #pragma unroll
   for (int xb = 0; xb < XB; ++xb) {
-    const int64_t x = x0 + 32 * xb;
-    load_outer<T>(xf[xb], static_cast<const T *>(p.h) + min(x, p.N - 1) * p.hs, x >= p.N, p.D);
+    const int64_t x = x0 + 32 * xb, row = a.order.row(min(x, N - 1));
+    load_outer<T>(xf[xb], static_cast<const T *>(p.h) + row * p.hs, x >= N, p.D);
   }
   float m[XB], mu[XB], l[XB], lc[XB];
   f32x16 o[XB][DIR ? DB : 1];
@@ -64,32 +86,19 @@ __global__ __launch_bounds__(kBlock, 1) void k_forward(FwdArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[xb][d][r] = 0.f;
   }
-
-  Stage<T, DP, YT> next;
-  float nb = 0.f;   // the bias of the next tile's row tid, to base 2
-  auto fetch = [&](int64_t t) {
-    const int64_t y0 = t * YT, rows = p.V - y0;
-    next.fetch(table + y0 * p.ts, p.ts, rows, p.D);
-    if (p.bias != nullptr) {
-#pragma unroll
-      for (int i = 0; i < next.NL; ++i) next.out[i] |= p.bias[y0 + min(int64_t(next.row(i)), rows - 1)] == -INFINITY;
-    }
-    if (tid < YT) nb = tid >= rows ? -INFINITY : p.bias != nullptr ? bias2(p, y0 + tid) : 0.f;
-  };
-#pragma unroll
-  for (int i = 0; i < NBUF; ++i) Stage<T, DP, YT>::clear(tiles + i * YT * LD);
-  __syncthreads();
-  if (t0 < t1) fetch(t0);
+  const int end = int(min(int64_t(line.inner), t + (u1 - u)));
+  u += end - t;
 #pragma unroll 1
-  for (int64_t t = t0; t < t1; ++t) {
-    const int buf = NBUF == 2 ? int(t - t0) & 1 : 0;
+  for (; t < end; ++t) {
     T *tile = tiles + buf * YT * LD;
     float *b2 = b2s + buf * YT;
-    if (NBUF == 1 && t > t0) __syncthreads();
-    next.put(tile, p.D);
-    if (tid < YT) b2[tid] = nb;
+    if (NBUF == 1) __syncthreads();
+    const int rows = rows_of(t);
+    next.put(tile, rows, biased);
+    if (tid < YT) b2[tid] = tid >= rows ? -INFINITY : biased ? bias2_of(p, nb) : 0.f;
     __syncthreads();
-    if (t + 1 < t1) fetch(t + 1);
+    if (t + 1 < end || u < u1) fetch(t + 1 < end ? t + 1 : 0);   // (the next outer tile's first)
+    if (NBUF == 2) buf ^= 1;
 #pragma unroll 1
     for (int ys = 0; ys < YS; ++ys) {
       const int row0 = (wy * YS + ys) * 32;
@@ -158,18 +167,18 @@ __global__ __launch_bounds__(kBlock, 1) void k_forward(FwdArgs a) {
     }
   }
 
-  const int64_t part = split * WY + wy;
+  const int64_t part = int64_t(w + xt) * WY + wy;
 #pragma unroll
   for (int xb = 0; xb < XB; ++xb) {
-    const int64_t x = x0 + 32 * xb;
+    const int at = wx * (32 * XB) + 32 * xb + (lane & 31);
     const float sum = pair_sum(l[xb]);
-    if (x >= p.N) continue;
+    if (x0 + 32 * xb >= N) continue;
     if (h == 0) {
-      a.out.m[part * p.N + x] = m[xb] == -INFINITY ? -INFINITY : mu[xb];
-      a.out.l[part * p.N + x] = sum;
+      a.out.m[part * XT + at] = m[xb] == -INFINITY ? -INFINITY : mu[xb];
+      a.out.l[part * XT + at] = sum;
     }
     if constexpr (DIR) {
-      float *row = a.out.o + (part * p.N + x) * DP;
+      float *row = a.out.o + (part * XT + at) * DP;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -181,33 +190,11 @@ __global__ __launch_bounds__(kBlock, 1) void k_forward(FwdArgs a) {
         }
     }
   }
-}
-
-// Which form: rows of a workgroup, waves along the rows.
-struct Form {
-  int rows, waves_y, ytile;
-};
-template <typename T>
-Form form_of(int64_t N) {
-  if (N <= 32) return Form{32, 4, 128};
-  return Form{sizeof(T) == 4 ? 128 : 256, 1, 64};
-}
-
-template <typename T>
-int64_t pieces_of(const Problem &p) {
-  const Form f = form_of<T>(p.N);
-  const int64_t xt = (p.N + f.rows - 1) / f.rows, yt = (p.V + f.ytile - 1) / f.ytile;
-  // one workgroup a CU at a time: whole rounds of 256, the fewest that come near it
-  int64_t best = 1;
-  double cost = 1e300;
-  for (int64_t s = 1; s <= std::min<int64_t>(yt, 512); ++s) {
-    const int64_t per = (yt + s - 1) / s, rounds = (xt * s + 255) / 256;
-    const double t = double(rounds) * (double(per) + 4.0) + 0.02 * double(s * xt);
-    if (t < cost) cost = t, best = s;
+  t = 0;
   }
-  return best;
 }
 
+// Which form: by the rows.
 template <typename T, int DB, int XB, int WX, bool DIR>
 void run(const FwdArgs &a, hipStream_t stream) {
   constexpr int DP = 32 * DB, LD = Tile32<T, DP>::LD, YS = WX == kWaves ? 2 : 1, YT = 32 * YS * (kWaves / WX);
@@ -216,13 +203,13 @@ void run(const FwdArgs &a, hipStream_t stream) {
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
   auto *k = &k_forward<T, DB, XB, WX, DIR>;
   (void)ensure_dynamic_lds(reinterpret_cast<const void *>(k), bytes);
-  const int64_t grid = a.deal * a.xtiles * ((a.splits + a.deal - 1) / a.deal);
-  launch(k, dim3(unsigned(grid)), dim3(kBlock), bytes, stream, a);
+  const Line line((a.p.N + 32 * XB * WX - 1) / (32 * XB * WX), (a.p.V + YT - 1) / YT, kGroups);
+  launch(k, dim3(unsigned(line.groups)), dim3(kBlock), bytes, stream, a);
 }
 template <typename T, int DB, bool DIR>
 void pick_form(const FwdArgs &a, hipStream_t stream) {
   constexpr int XB = sizeof(T) == 4 ? 1 : 2;
-  if (a.p.N <= 32)
+  if (a.p.N <= kFewRows)
     run<T, DB, 1, 1, DIR>(a, stream);
   else
     run<T, DB, XB, 4, DIR>(a, stream);
@@ -237,12 +224,8 @@ void pick_dim(const FwdArgs &a, hipStream_t stream) {
   }
 }
 template <typename T>
-void pick_dir(const Problem &p, const Partials &out, bool dir, hipStream_t stream) {
-  const Form f = form_of<T>(p.N);
-  const int64_t splits = out.splits / f.waves_y;
-  const FwdArgs a{p, out, (p.N + f.rows - 1) / f.rows, (p.V + f.ytile - 1) / f.ytile, splits,
-                  std::min<int64_t>(splits, 8)};
-  if (dir) pick_dim<T, true>(a, stream);
+void pick_dir(const FwdArgs &a, hipStream_t stream) {
+  if (a.out.o != nullptr) pick_dim<T, true>(a, stream);
   else pick_dim<T, false>(a, stream);
 }
 
@@ -253,16 +236,21 @@ namespace cand {
 
 int padded_dim(int D) { return (D + 63) / 64 * 64; }
 
-int64_t forward_splits(int32_t dtype, const Problem &p, bool) {
-  const int wy = p.N <= 32 ? 4 : 1;
-  if (dtype == SGL_FP32) return pieces_of<float>(p) * wy;
-  return pieces_of<bf16_t>(p) * wy;
+Partials forward_shape(int32_t dtype, const Problem &p) {
+  Partials s{};
+  const bool few = p.N <= kFewRows;
+  s.rows = few ? 32 : dtype == SGL_FP32 ? 128 : 256;
+  s.wy = few ? 4 : 1;
+  s.ytiles = (p.V + (few ? 127 : 63)) / (few ? 128 : 64);
+  s.dp = padded_dim(p.D);
+  return s;
 }
 
-void forward_partials(int32_t dtype, const Problem &p, const Partials &out, bool dir, hipStream_t stream) {
-  if (dtype == SGL_FP32) return pick_dir<float>(p, out, dir, stream);
-  if (dtype == SGL_BF16) return pick_dir<bf16_t>(p, out, dir, stream);
-  return pick_dir<fp16_t>(p, out, dir, stream);
+void forward_partials(int32_t dtype, const Problem &p, const Order &order, const Partials &out, hipStream_t stream) {
+  const FwdArgs a{p, order, out};
+  if (dtype == SGL_FP32) return pick_dir<float>(a, stream);
+  if (dtype == SGL_BF16) return pick_dir<bf16_t>(a, stream);
+  return pick_dir<fp16_t>(a, stream);
 }
 
 }  // namespace cand

@@ -27,6 +27,7 @@ from starry_unigraph.native.history import _as_rows, _first, _guard, _no_grad, _
 
 MAX_DIM = 256       # channels of a row
 MAX_TARGETS = 1024  # a teacher's entries of a row
+MAX_STRIDE = 1 << 22   # elements from row to row that the kernels take
 
 
 def cross_entropy(h: torch.Tensor, table: torch.Tensor, target: torch.Tensor, *, bias: torch.Tensor | None = None,
@@ -113,6 +114,12 @@ def _call(h, table, bias, target, entries, scale, temperature) -> torch.Tensor:
     return _Loss.run(*args, (False, False))[0]
 
 
+def _near(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with a contiguous last dimension and rows at most MAX_STRIDE apart."""
+    t = _rows(t)
+    return t if t.stride(0) <= MAX_STRIDE else t.contiguous()
+
+
 class _Loss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, *args):
@@ -128,34 +135,42 @@ class _Loss(torch.autograd.Function):
         """(loss, the backward's tensors); ``need``: gradients of the rows, of
         the table or bias."""
         lib, P, dev = _capi.lib(), _capi.ptr, h.device
-        h, table = _rows(h), _rows(table)
+        h, table = _near(h), _near(table)
         bias = None if bias is None else bias.contiguous()
         N, D = h.shape
         a = ctypes.byref(_Loss.problem(h, table, bias, scale, temperature))
         f32 = dict(dtype=torch.float32, device=dev)
         loss = torch.empty(N, **f32)
-        stat = torch.empty(2, N, **f32) if any(need) else None
+        stat = torch.empty(2, N, **f32) if need[0] or need[1] else None
         direction = torch.empty(N, D, **f32) if need[0] else None
-        nb = lib.sgl_candidates_workspace_bytes(a, 1 if need[0] else 0)
+        ids = weight = konst = order = None
+        K = 1
+        if entries is None:
+            if need[1]:
+                ids = torch.empty(N, dtype=torch.int32, device=dev)
+            if lib.sgl_candidates_orders(N):
+                order = torch.empty(N + 1, dtype=torch.int32, device=dev)
+        else:
+            K = entries[0].shape[1]
+            ids = torch.empty(N, K, dtype=torch.int32, device=dev)
+            weight, konst = torch.empty(N, K, **f32), torch.empty(N, **f32)
+        nb = lib.sgl_candidates_workspace_bytes(a, K, 1 if need[0] else 0)
         ws = _capi.workspace(nb, dev)
         with _guard(dev):
             stream = _capi.stream_of(dev)
             if entries is None:
-                ids, weight, konst, K = torch.empty(N, 1, dtype=torch.int32, device=dev) if need[1] else None, None, None, 1
-                _capi.check(lib.sgl_candidates_forward(
-                    a, P(target), None, None, None, 1, P(loss), P(stat), P(direction), P(ids), P(ws), nb, stream),
-                    "cross_entropy")
+                rc = lib.sgl_candidates_forward(a, P(target), None, None, None, 1, P(loss), P(stat), P(direction), P(ids),
+                                                P(order), P(ws), nb, stream)
             else:
-                K = entries[0].shape[1]
-                ids = torch.empty(N, K, dtype=torch.int32, device=dev)
-                weight, konst = torch.empty(N, K, **f32), torch.empty(N, **f32)
                 _capi.check(lib.sgl_candidates_teacher(
                     N, K, table.shape[0], P(entries[0]), P(entries[1]), temperature, P(ids), P(weight), P(konst),
                     stream), "distillation")
-                _capi.check(lib.sgl_candidates_forward(
-                    a, None, P(ids), P(weight), P(konst), K, P(loss), P(stat), P(direction), None, P(ws), nb, stream),
-                    "distillation")
-        return loss, (h, table, bias, stat, ids if need[1] else None, weight if need[1] else None, direction)
+                rc = lib.sgl_candidates_forward(a, None, P(ids), P(weight), P(konst), K, P(loss), P(stat), P(direction),
+                                                None, None, P(ws), nb, stream)
+            _capi.check(rc, "cross_entropy" if entries is None else "distillation")
+        if not need[1]:
+            ids = weight = None
+        return loss, (h, table, bias, stat, ids, weight, order, direction)
 
     @staticmethod
     def problem(h, table, bias, scale, temperature):
@@ -166,7 +181,7 @@ class _Loss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        h, table, bias, stat, ids, weight, direction = ctx.saved_tensors
+        h, table, bias, stat, ids, weight, order, direction = ctx.saved_tensors
         lib, P, dev = _capi.lib(), _capi.ptr, h.device
         # (from the tensors as they are now: a hook on saved tensors may bring them back elsewhere)
         a = ctypes.byref(_Loss.problem(h, table, bias, *ctx.form))
@@ -175,10 +190,11 @@ class _Loss(torch.autograd.Function):
         dh = torch.empty(h.shape, dtype=h.dtype, device=dev) if want[0] else None
         dt = torch.empty(table.shape, dtype=table.dtype, device=dev) if want[1] or want[2] else None
         db = torch.empty_like(bias) if want[2] else None
-        nb = lib.sgl_candidates_workspace_bytes(a, 2) if dt is not None else 0
+        K = weight.shape[1] if weight is not None else 1
+        nb = lib.sgl_candidates_workspace_bytes(a, K, 2) if dt is not None else 0
         ws = _capi.workspace(nb, dev) if nb else None
         with _guard(dev):
             _capi.check(lib.sgl_candidates_backward(
-                a, P(stat), P(ids), P(weight), ids.shape[1] if ids is not None else 1, P(direction), P(g), P(dh), P(dt),
-                P(db), P(ws), nb, _capi.stream_of(dev)), "candidates backward")
+                a, P(stat), P(ids), P(weight), K, P(order), P(direction), P(g), P(dh), P(dt), P(db), P(ws), nb,
+                _capi.stream_of(dev)), "candidates backward")
         return dh, dt if want[1] else None, db, None, None, None, None

@@ -159,16 +159,17 @@ def _problem(**kw):
     (dict(v=0), b"too many"),
     (dict(v=1 << 31), b"too many"),
     (dict(h_stride=-1), b"stride"),
+    (dict(table_stride=(1 << 22) + 1), b"stride"),
     (dict(table=None), b"NULL"),
     (dict(scale=float("inf")), b"scale"),
     (dict(temperature=0.0), b"temperature"),
 ])
 def test_entry_points_refuse(kw, match):
     lib, ref = _capi.lib(), ctypes.byref(_problem(**kw))
-    assert lib.sgl_candidates_workspace_bytes(ref, 1) == 0
-    assert lib.sgl_candidates_forward(ref, 4096, None, None, None, 1, 4096, None, None, None, 4096, 1 << 40, None) != 0
+    assert lib.sgl_candidates_workspace_bytes(ref, 1, 1) == 0
+    assert lib.sgl_candidates_forward(ref, 4096, None, None, None, 1, 4096, None, None, None, None, 4096, 1 << 40, None) != 0
     assert match in lib.sgl_last_error()
-    assert lib.sgl_candidates_backward(ref, 4096, 4096, None, 1, 4096, 4096, 4096, 4096, None, 4096, 1 << 40, None) != 0
+    assert lib.sgl_candidates_backward(ref, 4096, 4096, None, 1, None, 4096, 4096, 4096, 4096, None, 4096, 1 << 40, None) != 0
     assert match in lib.sgl_last_error()
 
 
@@ -176,23 +177,26 @@ def test_entry_points_refuse_their_arrays():
     lib, ref = _capi.lib(), ctypes.byref(_problem())
     fwd_ = lambda *a: lib.sgl_candidates_forward(ref, *a, None)
     for what, rc in (
-            (b"targets a row", fwd_(4096, None, None, None, 2, 4096, None, None, None, 4096, 1 << 40)),
-            (b"targets a row", fwd_(None, 4096, 4096, 4096, 1025, 4096, None, None, None, 4096, 1 << 40)),
-            (b"NULL array", fwd_(None, 4096, None, 4096, 3, 4096, None, None, None, 4096, 1 << 40)),
-            (b"labels and", fwd_(4096, 4096, None, None, 1, 4096, None, None, None, 4096, 1 << 40)),
-            (b"NULL array", fwd_(4096, None, None, None, 1, None, None, None, None, 4096, 1 << 40)),
-            (b"dir without", fwd_(4096, None, None, None, 1, 4096, None, 4096, None, 4096, 1 << 40)),
-            (b"workspace", fwd_(4096, None, None, None, 1, 4096, None, None, None, 4096, 16)),
-            (b"workspace", fwd_(4096, None, None, None, 1, 4096, None, None, None, None, 1 << 40)),
+            (b"targets a row", fwd_(4096, None, None, None, 2, 4096, None, None, None, None, 4096, 1 << 40)),
+            (b"targets a row", fwd_(None, 4096, 4096, 4096, 1025, 4096, None, None, None, None, 4096, 1 << 40)),
+            (b"NULL array", fwd_(None, 4096, None, 4096, 3, 4096, None, None, None, None, 4096, 1 << 40)),
+            (b"labels and", fwd_(4096, 4096, None, None, 1, 4096, None, None, None, None, 4096, 1 << 40)),
+            (b"NULL array", fwd_(4096, None, None, None, 1, None, None, None, None, None, 4096, 1 << 40)),
+            (b"dir without", fwd_(4096, None, None, None, 1, 4096, None, 4096, None, None, 4096, 1 << 40)),
+            (b"workspace", fwd_(4096, None, None, None, 1, 4096, None, None, None, None, 4096, 16)),
+            (b"workspace", fwd_(4096, None, None, None, 1, 4096, None, None, None, None, None, 1 << 40)),
+            (b"no order", fwd_(4096, None, None, None, 1, 4096, None, None, None, 4096, 4096, 1 << 40)),
     ):
         assert rc != 0, what
     bwd = lambda *a: lib.sgl_candidates_backward(ref, *a, None)
-    for args in ((None, 4096, None, 1, 4096, 4096, 4096, 4096, None, 4096, 1 << 40),
-                 (4096, 4096, None, 1, None, 4096, 4096, 4096, None, 4096, 1 << 40),
-                 (4096, None, None, 1, 4096, 4096, 4096, 4096, None, 4096, 1 << 40),
-                 (4096, 4096, None, 1, 4096, 4096, 4096, None, 4096, 4096, 1 << 40),
-                 (4096, 4096, None, 0, 4096, 4096, 4096, 4096, None, 4096, 1 << 40),
-                 (4096, 4096, None, 1, 4096, 4096, 4096, 4096, None, 4096, 16)):
+    for args in ((None, 4096, None, 1, None, 4096, 4096, 4096, 4096, None, 4096, 1 << 40),
+                 (4096, 4096, None, 1, None, None, 4096, 4096, 4096, None, 4096, 1 << 40),
+                 (4096, None, None, 1, None, 4096, 4096, 4096, 4096, None, 4096, 1 << 40),
+                 (4096, 4096, None, 1, None, 4096, 4096, 4096, None, 4096, 4096, 1 << 40),
+                 (4096, 4096, None, 1, 4096, 4096, 4096, 4096, 4096, None, 4096, 1 << 40),   # no order of ten rows
+                 (4096, 4096, None, 3, None, 4096, 4096, 4096, 4096, None, 4096, 1 << 40),   # no weights
+                 (4096, 4096, None, 0, None, 4096, 4096, 4096, 4096, None, 4096, 1 << 40),
+                 (4096, 4096, None, 1, None, 4096, 4096, 4096, 4096, None, 4096, 16)):
         assert bwd(*args) != 0, args
     assert lib.sgl_candidates_teacher(10, 0, 20, 4096, 4096, 1.0, 4096, 4096, 4096, None) != 0
     assert lib.sgl_candidates_teacher(10, 1025, 20, 4096, 4096, 1.0, 4096, 4096, 4096, None) != 0
