@@ -985,42 +985,34 @@ typedef struct sgl_candidates {
   float scale, temperature;
 } sgl_candidates;
 
-/* A teacher's entries (ids int64 [n, k], -1: none; logits fp32 [n, k]; k up to
- * 1024) as targets: weight = softmax(logits / temperature) over a row's live
- * entries, entries of one candidate put together in the first (the others -1),
- * konst [n] = sum of weight log weight over the entries. */
-int sgl_candidates_teacher(int64_t n, int32_t k, int64_t v, const int64_t *ids,
-                           const float *logits, float temperature,
-                           int32_t *ids_out, float *weight, float *konst,
-                           hipStream_t stream);
-/* what: 0 the loss alone, 1 the loss with dir, 2 the backward; k targets a row. */
+/* Memory that the forward writes for the backward (and for its own steps), and
+ * workspaces. k: targets a row; teacher != 0: a teacher's entries, else labels
+ * (k = 1); need: gradients that will be asked for (1 of the rows, 2 of the table
+ * and the bias). */
+size_t sgl_candidates_keep_bytes(const sgl_candidates *problem, int32_t k,
+                                 int32_t teacher, int32_t need);
 size_t sgl_candidates_workspace_bytes(const sgl_candidates *problem, int32_t k,
-                                      int32_t what);
-/* Whether n rows with labels are worked on in an order of their own (rows
- * without a target set aside): the forward then takes `order` int32 [n + 1]. */
-int32_t sgl_candidates_orders(int64_t n);
-/* loss [n] = temperature^2 (konst + sum_k weight (lse - s_id)). Targets: either
- * `target` int64 [n] (one a row at weight 1; negative: the row's loss is 0;
- * past the table: NaN; k = 1) or ids, weight, konst of
- * sgl_candidates_teacher. A target that is left out: inf. For the backward
- * (NULL: not kept): stat fp32 [2, n], dir fp32 [n, dim] (the loss's direction
- * in h), with `target` ids_out int32 [n]; `order` (written; NULL: as they are)
- * where sgl_candidates_orders says so. Rows whose loss is 0, inf or NaN for these
- * reasons have no gradient. */
+                                      int32_t teacher, int32_t need,
+                                      int32_t backward);
+/* loss [n]. Labels (target int64 [n], k = 1): lse - s_target; a negative one: 0;
+ * past the table: NaN. A teacher's entries (ids int64 [n, k], negative: none;
+ * logits fp32 [n, k], -inf: none; k up to 1024): temperature^2 * sum q (log q -
+ * log p) with q the softmax of logits / temperature over the row's entries; a row
+ * without one: 0; an id past the table: NaN. A target that is left out: inf;
+ * every candidate left out: 0. Rows with a loss for one of these reasons have no
+ * gradient. */
 int sgl_candidates_forward(const sgl_candidates *problem,
-                           const int64_t *target, const int32_t *ids,
-                           const float *weight, const float *konst, int32_t k,
-                           float *loss, float *stat, float *dir,
-                           int32_t *ids_out, int32_t *order, void *workspace,
-                           size_t workspace_bytes, hipStream_t stream);
-/* g [n] -> dh (like h, contiguous; from dir; NULL: not computed), dtable (like
- * the table, contiguous; NULL: not computed) and with it dbias fp32 [v] (or
- * NULL). weight NULL: 1 (ids_out of the forward, k = 1); order: the forward's. */
-int sgl_candidates_backward(const sgl_candidates *problem, const float *stat,
-                            const int32_t *ids, const float *weight, int32_t k,
-                            const int32_t *order, const float *dir,
-                            const float *g, void *dh, void *dtable,
-                            float *dbias, void *workspace,
+                           const int64_t *target, const int64_t *ids,
+                           const float *logits, int32_t k, int32_t need,
+                           float *loss, void *keep, size_t keep_bytes,
+                           void *workspace, size_t workspace_bytes,
+                           hipStream_t stream);
+/* g [n] -> dh (like h, contiguous), dtable (like the table, contiguous) and with
+ * it dbias fp32 [v]; each may be NULL: not computed. */
+int sgl_candidates_backward(const sgl_candidates *problem, int32_t k,
+                            int32_t teacher, int32_t need, const void *keep,
+                            size_t keep_bytes, const float *g, void *dh,
+                            void *dtable, float *dbias, void *workspace,
                             size_t workspace_bytes, hipStream_t stream);
 
 /* One tensor of a rotation: x [n, len, heads, dh] at its strides, y

@@ -170,6 +170,13 @@ struct Stage {
       *reinterpret_cast<FragOf<T> *>(tile + u / Tl::UPR * Tl::LD + u % Tl::UPR * E) = zero_frag<T>();
   }
 };
+// A value that the compiler takes as new: what is formed from it inside a loop
+// is not formed before it and kept (masks and addresses of a piece's start and
+// end otherwise fill the registers of the loop between).
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
 // A lane's fragments of an outer row (zeros past D and for `out`).
 template <typename T, int NK>
 __device__ __forceinline__ void load_outer(FragOf<T> (&f)[NK], const T *row, bool out, int D) {
@@ -231,6 +238,12 @@ __device__ __forceinline__ void scale_blocks(f32x16 (&o)[NB], float by) {
       o[d][r] = x;
     }
   asm volatile("s_nop 7" ::: "memory");
+}
+__device__ __forceinline__ float abs_max16(const f32x16 &p) {   // (three operands an instruction)
+  float a = fabsf(p[0]);
+#pragma unroll
+  for (int i = 1; i < 15; i += 2) a = fmaxf(fmaxf(a, fabsf(p[i])), fabsf(p[i + 1]));
+  return fmaxf(a, fabsf(p[15]));
 }
 // 2^x by the hardware instruction (1 ulp; results under 2^-126 are 0).
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -298,11 +311,11 @@ struct RowCoef {
   int64_t vblocks;
   int K;
 };
-void route_targets(int32_t dtype, int64_t N, int64_t V, int K, const int32_t *ids, const float *weight, int32_t *index,
+void route_targets(int32_t dtype, const Problem &p, int K, const int32_t *ids, const float *weight, int32_t *index,
                    int2 *entries, hipStream_t stream);
-int table_grad_tile(int32_t dtype);     // rows of a tile
-int table_grad_block(int32_t dtype);    // candidates of a wave
-// fp32 elements of `part` (0: not needed).
+int table_grad_tile(int32_t dtype, int D);   // rows of a tile
+int table_grad_block(int32_t dtype);         // candidates of a wave
+// fp32 elements of `part` at most (those of tiles that are not shared out are never touched).
 int64_t table_grad_part(int32_t dtype, const Problem &p);
 void table_grad(int32_t dtype, const Problem &p, const RowCoef &r, void *dtable, float *dbias, float *part,
                 hipStream_t stream);

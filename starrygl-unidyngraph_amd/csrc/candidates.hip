@@ -125,8 +125,22 @@ struct FinishArgs {
   float *loss, *stat, *dir;   // stat: [2][N] the maximum and 1 / sum (0: no gradient)
   int32_t *ids_out;           // of `target`
 };
-constexpr int kCols = kMaxDim / kWave;   // columns of a lane
-constexpr int kBatch = 8;                // targets whose rows are on their way together
+constexpr int kBatch = 8;     // targets whose rows are on their way together
+constexpr int kAhead = 4;     // partials of a lane
+
+// A lane's four columns of a row of D: 4 lane on, the last lane's the row's
+// last four (some of them its neighbour's too: `own` marks those that are not).
+struct Cols {
+  int d;
+  bool here, own[4];
+  __device__ __forceinline__ explicit Cols(int D) {
+    const int at = 4 * int(threadIdx.x & 63);
+    here = at < D;
+    d = min(at, D - 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) own[j] = here && d + j >= at;
+  }
+};
 
 // W waves a row, 4 / W rows a workgroup.
 template <typename T, int W, bool DIR>
@@ -139,8 +153,10 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
   const bool here = at < p.N;
   const int64_t pos = here ? at : p.N - 1;   // (a row past the end joins the barriers)
   const int64_t row = a.order.row(pos), live_rows = a.order.count(p.N);
-  const T *h = static_cast<const T *>(p.h) + row * p.hs;
   const int64_t target = a.target != nullptr ? a.target[row] : 0;
+  const Cols c(p.D);
+  T raw[4];
+  load_n(raw, static_cast<const T *>(p.h) + row * p.hs + c.d);
 
   // the row's partials: the waves along the table of consecutive pieces
   int n = 0;
@@ -152,25 +168,39 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
     first = (w0 + xt) * a.in.wy * a.in.rows + (pos - xt * a.in.rows);
   }
   const float *pm = a.in.m + first, *pl = a.in.l + first;
-  float mx = -INFINITY;
-  for (int s = lane; s < n; s += kWave) mx = fmaxf(mx, pm[s * a.in.rows]);
-  mx = wave_max(mx);
-  float l = 0.f;
-  for (int s = lane; s < n; s += kWave) {
-    const float m = pm[s * a.in.rows], y = pl[s * a.in.rows];
-    l += m == -INFINITY ? y : y * exp2_fast(m - mx);   // (a piece without a live candidate has sum 0)
-  }
-  l = wave_sum(l);
-
-  // the targets: sum of q (mx - s), of q, of q w
-  float x[kCols], tw[kCols];
+  // the first of them at once: their loads, the row's and the targets' overlap
+  float m[kAhead], s[kAhead];
 #pragma unroll
-  for (int j = 0; j < kCols; ++j) {
-    const int d = lane + kWave * j;
-    x[j] = d < p.D ? float(h[d]) : 0.f;
+  for (int i = 0; i < kAhead; ++i) {
+    const int k = lane + i * kWave;
+    m[i] = k < n ? pm[k * a.in.rows] : -INFINITY;
+    s[i] = k < n ? pl[k * a.in.rows] : 0.f;
+  }
+
+  // the targets: sum of -q s, of q, of q w
+  float x[4], tw[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[j] = c.own[j] ? float(raw[j]) : 0.f;
     tw[j] = 0.f;
   }
+  float mx = -INFINITY, l = 0.f;
+  auto join = [&]() {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) mx = fmaxf(mx, m[i]);
+    for (int k = lane + kAhead * kWave; k < n; k += kWave) mx = fmaxf(mx, pm[k * a.in.rows]);
+    mx = wave_max(mx);
+    // (a piece without a live candidate has sum 0)
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) l += m[i] == -INFINITY ? s[i] : s[i] * exp2_fast(m[i] - mx);
+    for (int k = lane + kAhead * kWave; k < n; k += kWave) {
+      const float y = pm[k * a.in.rows], z = pl[k * a.in.rows];
+      l += y == -INFINITY ? z : z * exp2_fast(y - mx);
+    }
+    l = wave_sum(l);
+  };
   float far = 0.f, want = 0.f, out = 0.f;
+  bool joined = false;
   for (int k0 = w * kBatch; k0 < a.K; k0 += W * kBatch) {
     int id = -1;
     float q = 0.f, b = 0.f;
@@ -190,25 +220,26 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
       out = 1.f;
       id = -1;
     }
-    float y[kBatch][kCols], dot[kBatch];
+    T y[kBatch][4];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int c = __builtin_amdgcn_readlane(id, i);
-      const T *t = static_cast<const T *>(p.table) + int64_t(max(c, 0)) * p.ts;
+      const int v = __builtin_amdgcn_readlane(id, i);
+      if (v >= 0) load_n(y[i], static_cast<const T *>(p.table) + int64_t(v) * p.ts + c.d);
+      else
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) {
-        const int d = lane + kWave * j;
-        y[i][j] = c >= 0 && d < p.D ? float(t[d]) : 0.f;
-      }
+        for (int j = 0; j < 4; ++j) y[i][j] = T(0.f);
     }
+    if (!joined) join(), joined = true;
+    float dot[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const float qi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(q), i));
       dot[i] = 0.f;
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) {
-        dot[i] = fmaf(x[j], y[i][j], dot[i]);
-        tw[j] = fmaf(qi, y[i][j], tw[j]);
+      for (int j = 0; j < 4; ++j) {
+        const float z = c.own[j] ? float(y[i][j]) : 0.f;   // (times a row's zeros: not of another lane's NaN)
+        dot[i] = fmaf(x[j], z, dot[i]);
+        tw[j] = fmaf(qi, float(y[i][j]), tw[j]);
       }
     }
 #pragma unroll
@@ -217,6 +248,7 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
     for (int i = 0; i < kBatch; ++i)
       if (lane == i && id >= 0) far += q * (mx - fmaf(dot[i], p.c, b));
   }
+  if (!joined) join();
   far = wave_sum(far);
   want = wave_sum(want);
   out = wave_max(out);
@@ -251,34 +283,35 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
     if (a.ids_out != nullptr) a.ids_out[row] = uint64_t(target) < uint64_t(p.V) ? int32_t(target) : -1;
   }
   if constexpr (DIR) {
-    float o[kCols] = {};
-    const float *src = a.in.o + first * a.in.dp;
+    float o[4] = {};
+    const float *src = a.in.o + first * a.in.dp + c.d;
     const int64_t step = int64_t(a.in.rows) * a.in.dp;
 #pragma unroll 4
-    for (int s = w; s < n; s += W) {
-      const float m = pm[s * a.in.rows];
-      const float f = m == -INFINITY ? 1.f : exp2_fast(m - mx);
+    for (int k = w; k < n; k += W) {
+      const float y = pm[k * a.in.rows];
+      const float f = y == -INFINITY ? 1.f : exp2_fast(y - mx);
+      float z[4];
+      load_n(z, src + k * step);
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) {
-        const int d = lane + kWave * j;
-        if (d < p.D) o[j] = fmaf(src[s * step + d], f, o[j]);
-      }
+      for (int j = 0; j < 4; ++j) o[j] = fmaf(z[j], f, o[j]);
     }
+    float e[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[j] = o[j] / l - tw[j];
     if constexpr (W > 1) {
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) parts[wave][lane + kWave * j] = o[j] / l - tw[j];
+      for (int j = 0; j < 4; ++j) parts[wave][4 * lane + j] = e[j];
       __syncthreads();
+      if (w != 0) return;
+#pragma unroll
+      for (int i = 1; i < W; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] += parts[i][4 * lane + j];
     }
+    if (here && c.here) {
 #pragma unroll
-    for (int j = 0; j < kCols; ++j) {
-      const int d = lane + kWave * j;
-      float e = o[j] / l - tw[j];
-      if constexpr (W > 1) {
-        if (w != 0) continue;
-#pragma unroll
-        for (int i = 1; i < W; ++i) e += parts[i][d];
-      }
-      if (here && d < p.D) a.dir[row * p.D + d] = grad ? e : 0.f;
+      for (int j = 0; j < 4; ++j) e[j] = grad ? e[j] : 0.f;
+      store_n(a.dir + row * p.D + c.d, e);
     }
   }
 }
@@ -303,6 +336,7 @@ __global__ __launch_bounds__(kBlock) void k_rows(RowArgs a) {
   const int64_t pos = int64_t(blockIdx.x) * kWaves + attn::wave_index();
   if (pos >= p.N) return;
   const int64_t n = a.order.row(pos);
+  const Cols c(p.D);
   const float m = a.stat[n], il = a.stat[p.N + n];
   const bool live = !(il == 0.f);
   const float g = live ? a.g[n] * p.temperature : 0.f;
@@ -312,12 +346,20 @@ __global__ __launch_bounds__(kBlock) void k_rows(RowArgs a) {
     a.gq[pos] = g;
     if (a.packed_ids != nullptr) a.packed_ids[pos] = a.ids[n];
   }
-  if (a.packed != nullptr && live)
-    for (int d = lane; d < p.D; d += kWave)
-      static_cast<T *>(a.packed)[pos * p.D + d] = static_cast<const T *>(p.h)[n * p.hs + d];
-  if (a.dh != nullptr)
-    for (int d = lane; d < p.D; d += kWave)
-      static_cast<T *>(a.dh)[n * p.D + d] = T(live ? g * p.scale * a.dir[n * p.D + d] : 0.f);
+  if (!c.here) return;
+  if (a.packed != nullptr && live) {
+    T x[4];
+    load_n(x, static_cast<const T *>(p.h) + n * p.hs + c.d);
+    store_n(static_cast<T *>(a.packed) + pos * p.D + c.d, x);
+  }
+  if (a.dh != nullptr) {
+    float e[4] = {};
+    if (live) load_n(e, a.dir + n * p.D + c.d);
+    T x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = T(live ? g * p.scale * e[j] : 0.f);
+    store_n(static_cast<T *>(a.dh) + n * p.D + c.d, x);
+  }
 }
 
 // ------------------------------------------------------------------ entry points
@@ -365,32 +407,59 @@ Partials carve_forward(void *ws, int32_t dtype, const Problem &p, bool dir, size
 // than the launch that orders them costs.
 bool orders(int64_t N) { return N >= kOrderLeast && N <= kOrderMost; }
 
+// What the backward reads of the forward (and the forward's own steps of each other).
+struct Keep {
+  float *stat, *dir, *weight, *konst;
+  int32_t *ids, *order;
+};
+constexpr int32_t kNeedRows = 1, kNeedTable = 2;
+Keep carve_keep(void *keep, const Problem &p, int K, bool teacher, int32_t need, size_t *bytes) {
+  Carver c(keep);
+  Keep k{};
+  const size_t n = size_t(p.N), e = n * size_t(K);
+  if (need != 0) k.stat = c.take<float>(2 * n);
+  if (need & kNeedRows) k.dir = c.take<float>(n * size_t(p.D));
+  if (teacher || (need & kNeedTable)) k.ids = c.take<int32_t>(e);
+  if (teacher) {
+    k.weight = c.take<float>(e);
+    k.konst = c.take<float>(n);
+  } else if (orders(p.N)) {
+    k.order = c.take<int32_t>(n + 1);
+  }
+  *bytes = c.used;
+  return k;
+}
+
 struct Grad {
   float *nm, *gl, *gq, *part;
   char *packed;
   int32_t *ids, *index;
   int2 *entries;
 };
-Grad carve_backward(void *ws, int32_t dtype, const Problem &p, int K, bool ordered, size_t *bytes) {
+Grad carve_backward(void *ws, int32_t dtype, const Problem &p, int K, bool teacher, size_t *bytes) {
   Carver c(ws);
   Grad g{};
   g.nm = c.take<float>(size_t(p.N));
   g.gl = c.take<float>(size_t(p.N));
   g.gq = c.take<float>(size_t(p.N));
-  if (ordered) {
-    g.packed = c.take<char>(size_t(p.N) * size_t(p.D) * (dtype == SGL_FP32 ? 4 : 2));
-    g.ids = c.take<int32_t>(size_t(p.N));
-  }
-  if (K > 1) {
-    const int yt = table_grad_tile(dtype), vb = table_grad_block(dtype);
+  if (teacher) {
+    const int yt = table_grad_tile(dtype, p.D), vb = table_grad_block(dtype);
     const size_t tiles = size_t((p.N + yt - 1) / yt);
     g.index = c.take<int32_t>(tiles * size_t((p.V + vb - 1) / vb + 1));
     g.entries = c.take<int2>(tiles * size_t(yt) * size_t(K));
+  } else if (orders(p.N)) {
+    g.packed = c.take<char>(size_t(p.N) * size_t(p.D) * (dtype == SGL_FP32 ? 4 : 2));
+    g.ids = c.take<int32_t>(size_t(p.N));
   }
-  const int64_t part = table_grad_part(dtype, p);
-  g.part = part > 0 ? c.take<float>(size_t(part)) : nullptr;
+  g.part = c.take<float>(size_t(table_grad_part(dtype, p)));
   *bytes = c.used;
   return g;
+}
+
+int check_room(const char *what, const void *room, size_t bytes, size_t need) {
+  if (need == 0 || (room != nullptr && bytes >= need)) return SGL_OK;
+  sgl::set_error("candidates: %s of %zu bytes, %zu needed", what, room != nullptr ? bytes : 0, need);
+  return SGL_ERR_WORKSPACE;
 }
 
 template <typename T>
@@ -409,56 +478,52 @@ void finish(const FinishArgs &a, hipStream_t stream) {
 
 }  // namespace
 
-extern "C" int sgl_candidates_teacher(int64_t n, int32_t k, int64_t v, const int64_t *ids, const float *logits,
-                                      float temperature, int32_t *ids_out, float *weight, float *konst,
-                                      hipStream_t stream) {
-  SGL_REQUIRE(n >= 0 && n <= kMaxRows && v > 0 && v < INT32_MAX - 512 && k > 0 && k <= kMaxTargets,
-              "candidates_teacher: %lld rows of %d entries (1 to %d)", (long long)n, k, kMaxTargets);
-  SGL_REQUIRE(temperature > 0.f && temperature < INFINITY, "candidates_teacher: temperature %g", double(temperature));
-  if (n == 0) return SGL_OK;
-  SGL_REQUIRE(ids && logits && ids_out && weight && konst, "candidates_teacher: NULL array");
-  const TeacherArgs a{ids, logits, n, v, k, temperature, ids_out, weight, konst};
-  sgl::launch(&k_teacher, dim3(unsigned((n + kWaves - 1) / kWaves)), dim3(kBlock), size_t(kWaves) * 8 * size_t(k), stream,
-         a);
-  SGL_CHECK_LAUNCH();
-  return SGL_OK;
-}
-
-extern "C" size_t sgl_candidates_workspace_bytes(const sgl_candidates *problem, int32_t k, int32_t what) {
+extern "C" size_t sgl_candidates_keep_bytes(const sgl_candidates *problem, int32_t k, int32_t teacher, int32_t need) {
   Problem p;
-  if (make_problem(problem, p) != SGL_OK || p.N == 0 || k <= 0 || k > kMaxTargets) return 0;
   size_t bytes = 0;
-  if (what == 2) carve_backward(nullptr, problem->dtype, p, k, k == 1 && orders(p.N), &bytes);
-  else carve_forward(nullptr, problem->dtype, p, what == 1, &bytes);
+  if (make_problem(problem, p) != SGL_OK || k <= 0 || k > kMaxTargets) return 0;
+  carve_keep(nullptr, p, k, teacher != 0, need, &bytes);
   return bytes;
 }
 
-extern "C" int32_t sgl_candidates_orders(int64_t n) { return orders(n) ? 1 : 0; }
+extern "C" size_t sgl_candidates_workspace_bytes(const sgl_candidates *problem, int32_t k, int32_t teacher,
+                                                 int32_t need, int32_t backward) {
+  Problem p;
+  size_t bytes = 0;
+  if (make_problem(problem, p) != SGL_OK || k <= 0 || k > kMaxTargets) return 0;
+  if (backward == 0) carve_forward(nullptr, problem->dtype, p, (need & kNeedRows) != 0, &bytes);
+  else if (need & kNeedTable) carve_backward(nullptr, problem->dtype, p, k, teacher != 0, &bytes);
+  return bytes;
+}
 
-extern "C" int sgl_candidates_forward(const sgl_candidates *problem, const int64_t *target, const int32_t *ids,
-                                      const float *weight, const float *konst, int32_t k, float *loss, float *stat,
-                                      float *dir, int32_t *ids_out, int32_t *order, void *workspace,
-                                      size_t workspace_bytes, hipStream_t stream) {
+extern "C" int sgl_candidates_forward(const sgl_candidates *problem, const int64_t *target, const int64_t *ids,
+                                      const float *logits, int32_t k, int32_t need, float *loss, void *keep,
+                                      size_t keep_bytes, void *workspace, size_t workspace_bytes, hipStream_t stream) {
   Problem p;
   if (const int rc = make_problem(problem, p)) return rc;
-  SGL_REQUIRE(k > 0 && k <= kMaxTargets && (target == nullptr || k == 1), "candidates_forward: %d targets a row", k);
+  SGL_REQUIRE(k > 0 && k <= kMaxTargets && (target == nullptr || k == 1), "candidates: %d targets a row", k);
+  SGL_REQUIRE(need >= 0 && need <= (kNeedRows | kNeedTable), "candidates: need %d", need);
   if (p.N == 0) return SGL_OK;
-  SGL_REQUIRE(loss && (target != nullptr ? ids == nullptr : ids && weight && konst && !ids_out && !order),
-              "candidates_forward: NULL array, or labels and a teacher's entries at once");
-  SGL_REQUIRE(dir == nullptr || stat != nullptr, "candidates_forward: dir without stat");
-  SGL_REQUIRE(order == nullptr || orders(p.N), "candidates_forward: no order of %lld rows", (long long)p.N);
-  size_t need = 0;
-  const Partials part = carve_forward(workspace, problem->dtype, p, dir != nullptr, &need);
-  if (workspace == nullptr || workspace_bytes < need) {
-    sgl::set_error("candidates_forward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-    return SGL_ERR_WORKSPACE;
-  }
-  const Order o{order, order != nullptr ? order + p.N : nullptr};
-  if (order != nullptr)
+  SGL_REQUIRE(loss && (target != nullptr ? ids == nullptr && logits == nullptr : ids != nullptr && logits != nullptr),
+              "candidates: NULL array, or labels and a teacher's entries at once");
+  const bool teacher = target == nullptr;
+  size_t room = 0;
+  const Keep kept = carve_keep(keep, p, k, teacher, need, &room);
+  if (const int rc = check_room("memory for the backward", keep, keep_bytes, room)) return rc;
+  const Partials part = carve_forward(workspace, problem->dtype, p, (need & kNeedRows) != 0, &room);
+  if (const int rc = check_room("workspace", workspace, workspace_bytes, room)) return rc;
+  if (teacher) {
+    const TeacherArgs a{ids, logits, p.N, p.V, k, p.temperature, kept.ids, kept.weight, kept.konst};
+    sgl::launch(&k_teacher, dim3(unsigned((p.N + kWaves - 1) / kWaves)), dim3(kBlock), size_t(kWaves) * 8 * size_t(k),
+                stream, a);
+  } else if (kept.order != nullptr) {
     sgl::launch(&k_order, dim3(unsigned((p.N + kOrderRows - 1) / kOrderRows)), dim3(kOrderRows), 0, stream, target, p.N,
-                p.V, order, order + p.N);
+                p.V, kept.order, kept.order + p.N);
+  }
+  const Order o{kept.order, kept.order != nullptr ? kept.order + p.N : nullptr};
   forward_partials(problem->dtype, p, o, part, stream);
-  const FinishArgs a{p, o, part, target, ids, weight, konst, k, loss, stat, dir, ids_out};
+  const FinishArgs a{p,           o, part, target,    teacher ? kept.ids : nullptr, kept.weight, kept.konst, k, loss,
+                     kept.stat, kept.dir, teacher ? nullptr : kept.ids};
   if (problem->dtype == SGL_FP32) finish<float>(a, stream);
   else if (problem->dtype == SGL_BF16) finish<bf16_t>(a, stream);
   else finish<fp16_t>(a, stream);
@@ -466,43 +531,40 @@ extern "C" int sgl_candidates_forward(const sgl_candidates *problem, const int64
   return SGL_OK;
 }
 
-extern "C" int sgl_candidates_backward(const sgl_candidates *problem, const float *stat, const int32_t *ids,
-                                       const float *weight, int32_t k, const int32_t *order, const float *dir,
-                                       const float *g, void *dh, void *dtable, float *dbias, void *workspace,
-                                       size_t workspace_bytes, hipStream_t stream) {
+extern "C" int sgl_candidates_backward(const sgl_candidates *problem, int32_t k, int32_t teacher, int32_t need,
+                                       const void *keep, size_t keep_bytes, const float *g, void *dh, void *dtable,
+                                       float *dbias, void *workspace, size_t workspace_bytes, hipStream_t stream) {
   Problem p;
   if (const int rc = make_problem(problem, p)) return rc;
-  SGL_REQUIRE(k > 0 && k <= kMaxTargets, "candidates_backward: %d targets a row", k);
-  SGL_REQUIRE(p.N > 0, "candidates_backward: no rows");
-  SGL_REQUIRE(stat && g && (dh == nullptr || dir) && (dtable == nullptr || (ids && (k == 1 || weight))),
-              "candidates_backward: NULL array");
-  SGL_REQUIRE(dbias == nullptr || dtable != nullptr, "candidates_backward: dbias without dtable");
-  SGL_REQUIRE(order == nullptr || (k == 1 && orders(p.N)), "candidates_backward: no order of %lld rows", (long long)p.N);
+  SGL_REQUIRE(k > 0 && k <= kMaxTargets && (teacher != 0 || k == 1), "candidates_backward: %d targets a row", k);
+  SGL_REQUIRE(need > 0 && need <= (kNeedRows | kNeedTable) && p.N > 0, "candidates_backward: need %d of %lld rows", need,
+              (long long)p.N);
+  SGL_REQUIRE(g != nullptr && (dh == nullptr || (need & kNeedRows)) && (dtable == nullptr || (need & kNeedTable)) &&
+              (dbias == nullptr || dtable != nullptr), "candidates_backward: a gradient that the forward did not prepare");
+  size_t room = 0;
+  const Keep kept = carve_keep(const_cast<void *>(keep), p, k, teacher != 0, need, &room);
+  if (const int rc = check_room("memory for the backward", keep, keep_bytes, room)) return rc;
   Grad w{};
   if (dtable != nullptr) {
-    size_t need = 0;
-    w = carve_backward(workspace, problem->dtype, p, k, order != nullptr, &need);
-    if (workspace == nullptr || workspace_bytes < need) {
-      sgl::set_error("candidates_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-      return SGL_ERR_WORKSPACE;
-    }
+    w = carve_backward(workspace, problem->dtype, p, k, teacher != 0, &room);
+    if (const int rc = check_room("workspace", workspace, workspace_bytes, room)) return rc;
   }
-  const Order o{order, order != nullptr ? order + p.N : nullptr};
-  const RowArgs a{p, o, stat, dir, g, ids, dh, w.nm, w.gl, w.gq, w.packed, w.ids};
+  const Order o{kept.order, kept.order != nullptr ? kept.order + p.N : nullptr};
+  const RowArgs a{p, o, kept.stat, kept.dir, g, kept.ids, dh, w.nm, w.gl, w.gq, w.packed, w.ids};
   const dim3 grid(unsigned((p.N + kWaves - 1) / kWaves));
   if (problem->dtype == SGL_FP32) sgl::launch(&k_rows<float>, grid, dim3(kBlock), 0, stream, a);
   else if (problem->dtype == SGL_BF16) sgl::launch(&k_rows<bf16_t>, grid, dim3(kBlock), 0, stream, a);
   else sgl::launch(&k_rows<fp16_t>, grid, dim3(kBlock), 0, stream, a);
   if (dtable != nullptr) {
-    RowCoef r{w.nm, w.gl, w.gq, o.live, w.ids != nullptr ? w.ids : ids, w.index, w.entries, 0, k};
+    RowCoef r{w.nm, w.gl, w.gq, o.live, w.ids != nullptr ? w.ids : kept.ids, w.index, w.entries, 0, k};
     if (w.packed != nullptr) {
       p.h = w.packed;
       p.hs = p.D;
     }
-    if (k > 1) {
+    if (teacher != 0) {
       const int vb = table_grad_block(problem->dtype);
       r.vblocks = (p.V + vb - 1) / vb;
-      route_targets(problem->dtype, p.N, p.V, k, ids, weight, w.index, w.entries, stream);
+      route_targets(problem->dtype, p, k, kept.ids, kept.weight, w.index, w.entries, stream);
     }
     table_grad(problem->dtype, p, r, dtable, dbias, w.part, stream);
   }

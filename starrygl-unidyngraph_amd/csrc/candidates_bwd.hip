@@ -11,8 +11,7 @@ struct BwdArgs {
   Problem p;
   RowCoef r;
   void *dtable;
-  float *dbias, *part;   // part: [pieces][candidates of a workgroup][dp + 1]
-  int most;              // workgroups at most
+  float *dbias, *part;   // part: [pieces][candidates of a workgroup][dp + 4]
 };
 
 // fp16: a coefficient goes into the product times a power of two a candidate
@@ -25,6 +24,13 @@ __device__ __forceinline__ float half_scale(float most) {   // (1 for what is no
   return e >= 255 ? 1.f : __uint_as_float(uint32_t(min(max(264 - e, 1), 254)) << 23);
 }
 
+// Candidates of a workgroup, rows of a tile (32 where more of them on their way
+// would not fit in the registers).
+template <typename T>
+constexpr int kXTile = sizeof(T) == 4 ? 128 : 256;
+template <typename T, int DB>
+constexpr int kYTile = sizeof(T) == 4 || DB == 8 ? 32 : 64;
+
 // XB blocks of 32 candidates a wave, four waves along the candidates.
 template <typename T, int DB, int XB>
 __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
@@ -32,14 +38,14 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
   constexpr int KS = M::KS, DP = 32 * DB, NK = DP / KS;
   using Tl = Tile32<T, DP>;
   constexpr int LD = Tl::LD;
-  constexpr int YT = sizeof(T) == 4 ? 32 : 64, YS = YT / 32, XT = 32 * XB * kWaves, QL = YT + 4;
+  constexpr int YT = kYTile<T, DB>, YS = YT / 32, XT = 32 * XB * kWaves, QL = 32 + 4;
   constexpr bool HALF = std::is_same_v<T, fp16_t>;
   constexpr int WV = 32 * XB;   // candidates of a wave
   extern __shared__ __align__(16) char lds[];
   T *tiles = reinterpret_cast<T *>(lds);
   float *coef = reinterpret_cast<float *>(lds + size_t(2) * YT * LD * sizeof(T));   // [2][3][YT]
-  // [XT][QL]: what the tile's rows want of the candidates; zero between uses. A wave writes, reads and
-  // clears its own candidates' part.
+  // [XT][QL]: what 32 rows want of the candidates; zero between uses. A wave writes, reads and clears
+  // its own candidates' part.
   float *q_all = coef + 2 * 3 * YT;
 
   const Problem &p = a.p;
@@ -47,7 +53,7 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
   const int wave = attn::wave_index();
   float *q = q_all + wave * WV * QL;
   const int64_t N = a.r.live != nullptr ? int64_t(*a.r.live) : p.N;
-  const Line line((p.V + XT - 1) / XT, max((N + YT - 1) / YT, int64_t(1)), a.most);
+  const Line line((p.V + XT - 1) / XT, max((N + YT - 1) / YT, int64_t(1)), kGroups);
   const int w = blockIdx.x;
   if (w >= line.groups) return;
   const int64_t u1 = line.begin(w + 1);
@@ -75,7 +81,7 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
       ne1 = vb < a.r.vblocks ? attn::scalar_load(at + 1) : ne0;
     }
   };
-  for (int i = tid; i < XT * QL; i += kBlock) q_all[i] = 0.f;
+  for (int i = tid; i < XT * QL / 4; i += kBlock) reinterpret_cast<f32x4 *>(q_all)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   Stage<T, DP, YT>::clear(tiles);
   Stage<T, DP, YT>::clear(tiles + YT * LD);
   int64_t u = line.begin(w);
@@ -86,13 +92,14 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
 #pragma unroll 1
   for (; u < u1; ++xt) {   // an outer tile's piece
   FragOf<T> xf[XB][NK];
+  const int D = fresh(p.D);
   float b2[XB], db[XB], sc[XB];
   const int64_t x0 = int64_t(xt) * XT + wave * WV + col;
 #pragma unroll
   for (int xb = 0; xb < XB; ++xb) {
     const int64_t x = min(x0 + 32 * xb, p.V - 1);
     b2[xb] = p.bias != nullptr ? bias2(p, x) : 0.f;
-    load_outer<T>(xf[xb], static_cast<const T *>(p.table) + x * p.ts, b2[xb] == -INFINITY, p.D);
+    load_outer<T>(xf[xb], static_cast<const T *>(p.table) + x * p.ts, b2[xb] == -INFINITY, D);
     db[xb] = 0.f;
     sc[xb] = kFirstScale;
   }
@@ -123,16 +130,19 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
     const int e0 = ne0, e1 = ne1;
     const int2 *entries = a.r.entries + int64_t(t) * YT * a.r.K;
     const bool wanted = __any(one) || e0 < e1;
-    if (one) q[mine * QL + lane] = 1.f;
-    for (int e = e0 + lane; e < e1; e += kWave) {
-      const int2 x = entries[e];
-      q[(x.x >> 6) * QL + (x.x & 63)] = __int_as_float(x.y);
-    }
     __syncthreads();
     if (t + 1 < end || u < u1) fetch(t + 1 < end ? t + 1 : 0, t + 1 < end ? xt : xt + 1);
 #pragma unroll 1
     for (int ys = 0; ys < YS; ++ys) {
       const int row0 = ys * 32;
+      if (wanted) {
+        if (one && (lane >> 5) == ys) q[mine * QL + (lane & 31)] = 1.f;
+        for (int e = e0 + lane; e < e1; e += kWave) {
+          const int2 x = entries[e];
+          if (((x.x >> 5) & 1) == ys) q[(x.x >> 6) * QL + (x.x & 31)] = __int_as_float(x.y);
+        }
+        attn::wave_sync();
+      }
       f32x16 s[XB];
 #pragma unroll
       for (int xb = 0; xb < XB; ++xb)
@@ -163,10 +173,16 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
 #pragma unroll
           for (int xb = 0; xb < XB; ++xb) {
             float w[4];
-            __builtin_memcpy(w, q + (32 * xb + col) * QL + row0 + 8 * i + 4 * h, sizeof(w));
+            __builtin_memcpy(w, q + (32 * xb + col) * QL + 8 * i + 4 * h, sizeof(w));
 #pragma unroll
             for (int v = 0; v < 4; ++v) s[xb][4 * i + v] = fmaf(-gq[v], w[v], s[xb][4 * i + v]);
           }
+        }
+        attn::wave_sync();
+        if (one && (lane >> 5) == ys) q[mine * QL + (lane & 31)] = 0.f;
+        for (int e = e0 + lane; e < e1; e += kWave) {
+          const int x = entries[e].x;
+          if (((x >> 5) & 1) == ys) q[(x >> 6) * QL + (x & 31)] = 0.f;
         }
       }
       if (a.dbias != nullptr) {
@@ -178,14 +194,7 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
         bool over = false;
 #pragma unroll
         for (int xb = 0; xb < XB; ++xb) {
-          float m[16];
-#pragma unroll
-          for (int r = 0; r < 16; ++r) m[r] = fabsf(s[xb][r]);
-#pragma unroll
-          for (int d = 8; d > 0; d >>= 1)
-#pragma unroll
-            for (int r = 0; r < d; ++r) m[r] = fmaxf(m[r], m[r + d]);
-          most[xb] = pair_max(m[0]);
+          most[xb] = pair_max(abs_max16(s[xb]));
           over |= most[xb] * sc[xb] > kMostHalf;
         }
         if (__any(over)) {
@@ -215,16 +224,9 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
         }
       }
     }
-    if (wanted) {
-      attn::wave_sync();
-      if (one) q[mine * QL + lane] = 0.f;
-      for (int e = e0 + lane; e < e1; e += kWave) {
-        const int x = entries[e].x;
-        q[(x >> 6) * QL + (x & 63)] = 0.f;
-      }
-    }
   }
 
+  const int width = fresh(p.D);
   const bool whole = first == 0 && end == line.inner;
 #pragma unroll
   for (int xb = 0; xb < XB; ++xb) {
@@ -233,7 +235,7 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
     if (x >= p.V) continue;
     const float by = HALF ? p.scale / sc[xb] : p.scale;
     if (!whole) {
-      float *row = a.part + (int64_t(w + xt) * XT + wave * WV + 32 * xb + col) * (DP + 1);
+      float *row = a.part + (int64_t(w + xt) * XT + wave * WV + 32 * xb + col) * (DP + 4);
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -245,7 +247,7 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
         }
       if (h == 0) row[DP] = sum;
     } else {
-      T *row = static_cast<T *>(a.dtable) + x * p.D;
+      T *row = static_cast<T *>(a.dtable) + x * width;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -253,7 +255,7 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
           f32x4 y;
 #pragma unroll
           for (int v = 0; v < 4; ++v) y[v] = o[xb][d][4 * i + v] * by;
-          attn::store4<T>(row, 32 * d + 8 * i + 4 * h, p.D, y);
+          attn::store4<T>(row, 32 * d + 8 * i + 4 * h, width, y);
         }
       if (a.dbias != nullptr && h == 0) a.dbias[x] = sum;
     }
@@ -262,35 +264,38 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
   }
 }
 
-// Candidates whose rows were shared out: the pieces' sums in their order,
-// rounded once.
+// Outer tiles whose rows were shared out: the pieces' sums in their order,
+// rounded once. Workgroup b of kJoin parts looks after the tile that workgroup
+// b / kJoin + 1 begins inside of, unless an earlier one does.
+constexpr int kJoin = 8;
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_join_grad(BwdArgs a, int xtile, int ytile, int dp) {
   const Problem &p = a.p;
-  const int64_t at = int64_t(blockIdx.x) * kBlock + threadIdx.x;
-  if (at >= p.V * (p.D + 1)) return;
-  const int64_t v = at / (p.D + 1);
-  const int d = int(at - v * (p.D + 1));
-  if (d == p.D && a.dbias == nullptr) return;
   const int64_t N = a.r.live != nullptr ? int64_t(*a.r.live) : p.N;
-  const Line line((p.V + xtile - 1) / xtile, max((N + ytile - 1) / ytile, int64_t(1)), a.most);
-  const int64_t xt = v / xtile, w0 = line.group_of(xt * line.inner), w1 = line.group_of((xt + 1) * line.inner - 1);
-  if (w0 == w1) return;   // (written whole)
-  const int64_t step = int64_t(xtile) * (dp + 1);
-  const float *src = a.part + (w0 + xt) * step + (v - xt * xtile) * (dp + 1) + (d == p.D ? dp : d);
-  const int n = int(w1 - w0) + 1;
-  float x = 0.f;
-  int s = 0;
-  for (; s + 8 <= n; s += 8) {
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = src[(s + i) * step];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x += y[i];
+  const Line line((p.V + xtile - 1) / xtile, max((N + ytile - 1) / ytile, int64_t(1)), kGroups);
+  const int w = blockIdx.x / kJoin + 1, part = blockIdx.x % kJoin;
+  if (w >= line.groups) return;
+  const int64_t u = line.begin(w), xt = u / line.inner;
+  if (u == xt * line.inner || line.begin(w - 1) > xt * line.inner) return;
+  const int64_t w0 = w - 1, w1 = line.group_of((xt + 1) * line.inner - 1);
+  const int ld = dp + 4, n = int(w1 - w0) + 1, units = (p.D + 3) / 4 + 1;   // four columns a thread, and the bias
+  const int64_t step = int64_t(xtile) * ld;
+  const float *first = a.part + (w0 + xt) * step;
+  const int rows = int(min(int64_t(xtile), p.V - xt * xtile));
+  const int r0 = rows * part / kJoin, r1 = rows * (part + 1) / kJoin;
+  for (int i = threadIdx.x; i < (r1 - r0) * units; i += kBlock) {
+    const int r = r0 + i / units, c = i % units, d = c == units - 1 ? dp : 4 * c;
+    const int64_t v = xt * xtile + r;
+    const float *src = first + int64_t(r) * ld + d;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) x += *reinterpret_cast<const f32x4 *>(src + s * step);
+    if (d == dp) {
+      if (a.dbias != nullptr) a.dbias[v] = x[0];
+    } else {
+      attn::store4<T>(static_cast<T *>(a.dtable) + v * p.D, d, p.D, x);
+    }
   }
-  for (; s < n; ++s) x += src[s * step];
-  if (d == p.D) a.dbias[v] = x;
-  else static_cast<T *>(a.dtable)[v * p.D + d] = T(x);
 }
 
 // ------------------------------------------------------------------ several targets a row
@@ -353,51 +358,29 @@ __global__ __launch_bounds__(kRouteBlock) void k_route(RouteArgs a) {
   if (tid == 0) index[a.vblocks] = base;
 }
 
-// Candidates of a workgroup, rows of a tile.
-template <typename T>
-constexpr int kXTile = sizeof(T) == 4 ? 128 : 256;
-template <typename T>
-constexpr int kYTile = sizeof(T) == 4 ? 32 : 64;
-
-// A workgroup an outer tile where whole rounds of them leave little over, else
-// the line shared out over one round.
-template <typename T>
-int groups_of(const Problem &p) {
-  const int64_t xt = (p.V + kXTile<T> - 1) / kXTile<T>;
-  return xt >= 8 * kGroups ? int(xt) : kGroups;
-}
-
 template <typename T, int DB>
 void run(const BwdArgs &a, hipStream_t stream) {
   constexpr int XB = sizeof(T) == 4 ? 1 : 2;
-  constexpr int LD = Tile32<T, 32 * DB>::LD, YT = kYTile<T>, XT = kXTile<T>;
+  constexpr int LD = Tile32<T, 32 * DB>::LD, YT = kYTile<T, DB>, XT = kXTile<T>;
   static_assert(XT == 32 * XB * kWaves, "");
-  constexpr size_t bytes = size_t(2) * YT * LD * sizeof(T) + sizeof(float) * (6 * YT + XT * (YT + 4));
+  constexpr size_t bytes = size_t(2) * YT * LD * sizeof(T) + sizeof(float) * (6 * YT + XT * 36);
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
   auto *k = &k_table_grad<T, DB, XB>;
   (void)ensure_dynamic_lds(reinterpret_cast<const void *>(k), bytes);
-  const Line line((a.p.V + XT - 1) / XT, (a.p.N + YT - 1) / YT, a.most);
+  const Line line((a.p.V + XT - 1) / XT, (a.p.N + YT - 1) / YT, kGroups);
   launch(k, dim3(unsigned(line.groups)), dim3(kBlock), bytes, stream, a);
+  if (line.groups > 1)
+    launch(&k_join_grad<T>, dim3(unsigned(line.groups - 1) * kJoin), dim3(kBlock), 0, stream, a, XT, YT, 32 * DB);
 }
 template <typename T>
 void pick(const Problem &p, const RowCoef &r, void *dtable, float *dbias, float *part, hipStream_t stream) {
-  const BwdArgs a{p, r, dtable, dbias, part, groups_of<T>(p)};
-  const int dp = padded_dim(p.D);
-  if (dp == 64) run<T, 2>(a, stream);
-  else if (dp == 128) run<T, 4>(a, stream);
-  else if (dp == 192) run<T, 6>(a, stream);
-  else run<T, 8>(a, stream);
-  if (part != nullptr) {
-    const int64_t n = p.V * (p.D + 1);
-    launch(&k_join_grad<T>, dim3(unsigned((n + kBlock - 1) / kBlock)), dim3(kBlock), 0, stream, a, kXTile<T>, kYTile<T>,
-           dp);
+  const BwdArgs a{p, r, dtable, dbias, part};
+  switch (padded_dim(p.D)) {
+    case 64: return run<T, 2>(a, stream);
+    case 128: return run<T, 4>(a, stream);
+    case 192: return run<T, 6>(a, stream);
+    default: return run<T, 8>(a, stream);
   }
-}
-template <typename T>
-int64_t part_of(const Problem &p) {
-  const int64_t xt = (p.V + kXTile<T> - 1) / kXTile<T>;
-  if (groups_of<T>(p) == xt) return 0;
-  return (xt + kGroups) * kXTile<T> * (padded_dim(p.D) + 1);
 }
 
 }  // namespace
@@ -405,15 +388,19 @@ int64_t part_of(const Problem &p) {
 namespace sgl {
 namespace cand {
 
-int table_grad_tile(int32_t dtype) { return dtype == SGL_FP32 ? kYTile<float> : kYTile<bf16_t>; }
+int table_grad_tile(int32_t dtype, int D) {
+  return dtype == SGL_FP32 ? 32 : padded_dim(D) == 256 ? kYTile<bf16_t, 8> : kYTile<bf16_t, 2>;
+}
 int table_grad_block(int32_t dtype) { return (dtype == SGL_FP32 ? kXTile<float> : kXTile<bf16_t>) / kWaves; }
 int64_t table_grad_part(int32_t dtype, const Problem &p) {
-  return dtype == SGL_FP32 ? part_of<float>(p) : part_of<bf16_t>(p);
+  const int64_t xtile = dtype == SGL_FP32 ? kXTile<float> : kXTile<bf16_t>;
+  return ((p.V + xtile - 1) / xtile + kGroups) * xtile * (padded_dim(p.D) + 4);
 }
 
-void route_targets(int32_t dtype, int64_t N, int64_t V, int K, const int32_t *ids, const float *weight, int32_t *index,
+void route_targets(int32_t dtype, const Problem &p, int K, const int32_t *ids, const float *weight, int32_t *index,
                    int2 *entries, hipStream_t stream) {
-  const int yt = table_grad_tile(dtype), vb = table_grad_block(dtype);
+  const int64_t N = p.N, V = p.V;
+  const int yt = table_grad_tile(dtype, p.D), vb = table_grad_block(dtype);
   const RouteArgs a{ids, weight, N, (V + vb - 1) / vb, K, yt, vb, index, entries};
   launch(&k_route, dim3(unsigned((N + yt - 1) / yt)), dim3(kRouteBlock), 0, stream, a);
 }

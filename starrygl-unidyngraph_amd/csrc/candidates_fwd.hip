@@ -24,6 +24,11 @@ constexpr float kSlack = 8.f;
 
 constexpr int64_t kFewRows = 32;   // up to here a workgroup's waves share them and split the table
 
+// Blocks of 32 candidates of a wave in a tile: two for fewer barriers, one
+// where the tile on its way would not fit in the registers.
+template <typename T, int DB, int WX>
+constexpr int kSubTiles = WX == kWaves && DB < 8 ? 2 : 1;
+
 // XB blocks of 32 rows a wave; WX waves along the rows, 4 / WX along the table.
 template <typename T, int DB, int XB, int WX, bool DIR>
 __global__ __launch_bounds__(kBlock, 1) void k_forward(FwdArgs a) {
@@ -31,7 +36,7 @@ __global__ __launch_bounds__(kBlock, 1) void k_forward(FwdArgs a) {
   constexpr int KS = M::KS, DP = 32 * DB, NK = DP / KS;
   using Tl = Tile32<T, DP>;
   constexpr int LD = Tl::LD;
-  constexpr int WY = kWaves / WX, YS = WX == kWaves ? 2 : 1, YT = 32 * YS * WY;
+  constexpr int WY = kWaves / WX, YS = kSubTiles<T, DB, WX>, YT = 32 * YS * WY;
   constexpr int NBUF = 2 * YT * LD * int(sizeof(T)) <= 140 * 1024 ? 2 : 1;
   extern __shared__ __align__(16) char lds[];
   T *tiles = reinterpret_cast<T *>(lds);
@@ -68,11 +73,12 @@ __global__ __launch_bounds__(kBlock, 1) void k_forward(FwdArgs a) {
 #pragma unroll 1
   for (; u < u1; ++xt) {   // an outer tile's piece
   FragOf<T> xf[XB][NK];
+  const int D = fresh(p.D);
   const int64_t x0 = (int64_t(xt) * WX + wx) * (32 * XB) + (lane & 31);
 #pragma unroll
   for (int xb = 0; xb < XB; ++xb) {
     const int64_t x = x0 + 32 * xb, row = a.order.row(min(x, N - 1));
-    load_outer<T>(xf[xb], static_cast<const T *>(p.h) + row * p.hs, x >= N, p.D);
+    load_outer<T>(xf[xb], static_cast<const T *>(p.h) + row * p.hs, x >= N, D);
   }
   float m[XB], mu[XB], l[XB], lc[XB];
   f32x16 o[XB][DIR ? DB : 1];
@@ -197,7 +203,7 @@ __global__ __launch_bounds__(kBlock, 1) void k_forward(FwdArgs a) {
 // Which form: by the rows.
 template <typename T, int DB, int XB, int WX, bool DIR>
 void run(const FwdArgs &a, hipStream_t stream) {
-  constexpr int DP = 32 * DB, LD = Tile32<T, DP>::LD, YS = WX == kWaves ? 2 : 1, YT = 32 * YS * (kWaves / WX);
+  constexpr int DP = 32 * DB, LD = Tile32<T, DP>::LD, YS = kSubTiles<T, DB, WX>, YT = 32 * YS * (kWaves / WX);
   constexpr int NBUF = 2 * YT * LD * int(sizeof(T)) <= 140 * 1024 ? 2 : 1;
   constexpr size_t bytes = size_t(NBUF) * YT * (LD * sizeof(T) + sizeof(float));
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
@@ -241,8 +247,9 @@ Partials forward_shape(int32_t dtype, const Problem &p) {
   const bool few = p.N <= kFewRows;
   s.rows = few ? 32 : dtype == SGL_FP32 ? 128 : 256;
   s.wy = few ? 4 : 1;
-  s.ytiles = (p.V + (few ? 127 : 63)) / (few ? 128 : 64);
   s.dp = padded_dim(p.D);
+  const int64_t ytile = few ? 128 : s.dp == 256 ? 32 : 64;
+  s.ytiles = (p.V + ytile - 1) / ytile;
   return s;
 }
 

@@ -112,11 +112,10 @@ SIGNATURES: dict[str, tuple] = {
     "sgl_cross_attention_saves": (_i32, [_vp]),
     "sgl_cross_attention_forward": (ctypes.c_int, [_vp] * 5 + [_sz, _vp]),
     "sgl_cross_attention_backward": (ctypes.c_int, [_vp] * 10 + [_sz, _vp]),
-    "sgl_candidates_teacher": (ctypes.c_int, [_i64, _i32, _i64, _vp, _vp, ctypes.c_float] + [_vp] * 4),
-    "sgl_candidates_workspace_bytes": (_sz, [_vp, _i32, _i32]),
-    "sgl_candidates_orders": (_i32, [_i64]),
-    "sgl_candidates_forward": (ctypes.c_int, [_vp] * 5 + [_i32] + [_vp] * 6 + [_sz, _vp]),
-    "sgl_candidates_backward": (ctypes.c_int, [_vp] * 4 + [_i32] + [_vp] * 7 + [_sz, _vp]),
+    "sgl_candidates_keep_bytes": (_sz, [_vp] + [_i32] * 3),
+    "sgl_candidates_workspace_bytes": (_sz, [_vp] + [_i32] * 4),
+    "sgl_candidates_forward": (ctypes.c_int, [_vp] * 4 + [_i32] * 2 + [_vp] * 2 + [_sz, _vp, _sz, _vp]),
+    "sgl_candidates_backward": (ctypes.c_int, [_vp] + [_i32] * 3 + [_vp, _sz] + [_vp] * 5 + [_sz, _vp]),
     "sgl_rotary": (ctypes.c_int, [_i32, _i64, _i32, _i32, _vp, _vp, _vp, _i32, ctypes.c_float, _i32, _vp]),
     "sgl_gated_norm_workspace_bytes": (_sz, [_i64, _i32]),
     "sgl_gated_norm_forward": (ctypes.c_int, [_i32, _i64, _i32] + _NORM + [_vp] * 3),

@@ -108,10 +108,9 @@ def _call(h, table, bias, target, entries, scale, temperature) -> torch.Tensor:
     least = 16 // h.element_size()
     if h.shape[1] < least:   # the kernels read 16 bytes of a row at a time: zeros add nothing to the products
         h, table = (torch.nn.functional.pad(t, (0, least - t.shape[1])) for t in (h, table))
-    args = (h, table, bias, target, entries, scale, temperature)
     if _tracked(h, table, bias):
-        return _Loss.apply(*args)
-    return _Loss.run(*args, (False, False))[0]
+        return _Loss.apply(h, table, bias, target, entries, scale, temperature)
+    return _Loss.run(h, table, bias, target, entries, scale, temperature, 0)[0]
 
 
 def _near(t: torch.Tensor) -> torch.Tensor:
@@ -122,55 +121,33 @@ def _near(t: torch.Tensor) -> torch.Tensor:
 
 class _Loss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, *args):
-        h, table, bias = args[:3]
-        need = (h.requires_grad, table.requires_grad or (bias is not None and bias.requires_grad))
-        loss, saved = _Loss.run(*args, need)
+    def forward(ctx, h, table, bias, target, entries, scale, temperature):
+        # the gradients that will be asked for: 1 of the rows, 2 of the table and bias
+        need = int(h.requires_grad) + 2 * int(table.requires_grad or (bias is not None and bias.requires_grad))
+        loss, saved, K = _Loss.run(h, table, bias, target, entries, scale, temperature, need)
         ctx.save_for_backward(*saved)
-        ctx.form = args[5:]
+        ctx.form = (scale, temperature, K, entries is not None, need)
         return loss
 
     @staticmethod
     def run(h, table, bias, target, entries, scale, temperature, need):
-        """(loss, the backward's tensors); ``need``: gradients of the rows, of
-        the table or bias."""
+        """(loss, the backward's tensors, targets a row)."""
         lib, P, dev = _capi.lib(), _capi.ptr, h.device
         h, table = _near(h), _near(table)
         bias = None if bias is None else bias.contiguous()
-        N, D = h.shape
+        teacher = entries is not None
+        ids, logits = entries if teacher else (None, None)
+        K = ids.shape[1] if teacher else 1
         a = ctypes.byref(_Loss.problem(h, table, bias, scale, temperature))
-        f32 = dict(dtype=torch.float32, device=dev)
-        loss = torch.empty(N, **f32)
-        stat = torch.empty(2, N, **f32) if need[0] or need[1] else None
-        direction = torch.empty(N, D, **f32) if need[0] else None
-        ids = weight = konst = order = None
-        K = 1
-        if entries is None:
-            if need[1]:
-                ids = torch.empty(N, dtype=torch.int32, device=dev)
-            if lib.sgl_candidates_orders(N):
-                order = torch.empty(N + 1, dtype=torch.int32, device=dev)
-        else:
-            K = entries[0].shape[1]
-            ids = torch.empty(N, K, dtype=torch.int32, device=dev)
-            weight, konst = torch.empty(N, K, **f32), torch.empty(N, **f32)
-        nb = lib.sgl_candidates_workspace_bytes(a, K, 1 if need[0] else 0)
+        loss = torch.empty(h.shape[0], dtype=torch.float32, device=dev)
+        nk = lib.sgl_candidates_keep_bytes(a, K, teacher, need)
+        keep = _capi.workspace(nk, dev) if nk else None
+        nb = lib.sgl_candidates_workspace_bytes(a, K, teacher, need, 0)
         ws = _capi.workspace(nb, dev)
         with _guard(dev):
-            stream = _capi.stream_of(dev)
-            if entries is None:
-                rc = lib.sgl_candidates_forward(a, P(target), None, None, None, 1, P(loss), P(stat), P(direction), P(ids),
-                                                P(order), P(ws), nb, stream)
-            else:
-                _capi.check(lib.sgl_candidates_teacher(
-                    N, K, table.shape[0], P(entries[0]), P(entries[1]), temperature, P(ids), P(weight), P(konst),
-                    stream), "distillation")
-                rc = lib.sgl_candidates_forward(a, None, P(ids), P(weight), P(konst), K, P(loss), P(stat), P(direction),
-                                                None, None, P(ws), nb, stream)
-            _capi.check(rc, "cross_entropy" if entries is None else "distillation")
-        if not need[1]:
-            ids = weight = None
-        return loss, (h, table, bias, stat, ids, weight, order, direction)
+            _capi.check(lib.sgl_candidates_forward(a, P(target), P(ids), P(logits), K, need, P(loss), P(keep), nk, P(ws), nb,
+                                                   _capi.stream_of(dev)), "distillation" if teacher else "cross_entropy")
+        return loss, (h, table, bias, keep), K
 
     @staticmethod
     def problem(h, table, bias, scale, temperature):
@@ -181,20 +158,19 @@ class _Loss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        h, table, bias, stat, ids, weight, order, direction = ctx.saved_tensors
+        h, table, bias, keep = ctx.saved_tensors
+        scale, temperature, K, teacher, need = ctx.form
         lib, P, dev = _capi.lib(), _capi.ptr, h.device
         # (from the tensors as they are now: a hook on saved tensors may bring them back elsewhere)
-        a = ctypes.byref(_Loss.problem(h, table, bias, *ctx.form))
+        a = ctypes.byref(_Loss.problem(h, table, bias, scale, temperature))
         g = g.contiguous()
         want = ctx.needs_input_grad
         dh = torch.empty(h.shape, dtype=h.dtype, device=dev) if want[0] else None
         dt = torch.empty(table.shape, dtype=table.dtype, device=dev) if want[1] or want[2] else None
         db = torch.empty_like(bias) if want[2] else None
-        K = weight.shape[1] if weight is not None else 1
-        nb = lib.sgl_candidates_workspace_bytes(a, K, 2) if dt is not None else 0
+        nb = lib.sgl_candidates_workspace_bytes(a, K, teacher, need, 1) if dt is not None else 0
         ws = _capi.workspace(nb, dev) if nb else None
         with _guard(dev):
-            _capi.check(lib.sgl_candidates_backward(
-                a, P(stat), P(ids), P(weight), K, P(order), P(direction), P(g), P(dh), P(dt), P(db), P(ws), nb,
-                _capi.stream_of(dev)), "candidates backward")
+            _capi.check(lib.sgl_candidates_backward(a, K, teacher, need, P(keep), keep.numel(), P(g), P(dh), P(dt), P(db),
+                                                    P(ws), nb, _capi.stream_of(dev)), "candidates backward")
         return dh, dt if want[1] else None, db, None, None, None, None

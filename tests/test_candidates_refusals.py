@@ -166,42 +166,38 @@ def _problem(**kw):
 ])
 def test_entry_points_refuse(kw, match):
     lib, ref = _capi.lib(), ctypes.byref(_problem(**kw))
-    assert lib.sgl_candidates_workspace_bytes(ref, 1, 1) == 0
-    assert lib.sgl_candidates_forward(ref, 4096, None, None, None, 1, 4096, None, None, None, None, 4096, 1 << 40, None) != 0
+    assert lib.sgl_candidates_workspace_bytes(ref, 1, 0, 3, 0) == 0 and lib.sgl_candidates_keep_bytes(ref, 1, 0, 3) == 0
+    big = 1 << 40
+    assert lib.sgl_candidates_forward(ref, 4096, None, None, 1, 3, 4096, 4096, big, 4096, big, None) != 0
     assert match in lib.sgl_last_error()
-    assert lib.sgl_candidates_backward(ref, 4096, 4096, None, 1, None, 4096, 4096, 4096, 4096, None, 4096, 1 << 40, None) != 0
+    assert lib.sgl_candidates_backward(ref, 1, 0, 3, 4096, big, 4096, 4096, 4096, None, 4096, big, None) != 0
     assert match in lib.sgl_last_error()
 
 
 def test_entry_points_refuse_their_arrays():
-    lib, ref = _capi.lib(), ctypes.byref(_problem())
-    fwd_ = lambda *a: lib.sgl_candidates_forward(ref, *a, None)
-    for what, rc in (
-            (b"targets a row", fwd_(4096, None, None, None, 2, 4096, None, None, None, None, 4096, 1 << 40)),
-            (b"targets a row", fwd_(None, 4096, 4096, 4096, 1025, 4096, None, None, None, None, 4096, 1 << 40)),
-            (b"NULL array", fwd_(None, 4096, None, 4096, 3, 4096, None, None, None, None, 4096, 1 << 40)),
-            (b"labels and", fwd_(4096, 4096, None, None, 1, 4096, None, None, None, None, 4096, 1 << 40)),
-            (b"NULL array", fwd_(4096, None, None, None, 1, None, None, None, None, None, 4096, 1 << 40)),
-            (b"dir without", fwd_(4096, None, None, None, 1, 4096, None, 4096, None, None, 4096, 1 << 40)),
-            (b"workspace", fwd_(4096, None, None, None, 1, 4096, None, None, None, None, 4096, 16)),
-            (b"workspace", fwd_(4096, None, None, None, 1, 4096, None, None, None, None, None, 1 << 40)),
-            (b"no order", fwd_(4096, None, None, None, 1, 4096, None, None, None, 4096, 4096, 1 << 40)),
-    ):
-        assert rc != 0, what
-    bwd = lambda *a: lib.sgl_candidates_backward(ref, *a, None)
-    for args in ((None, 4096, None, 1, None, 4096, 4096, 4096, 4096, None, 4096, 1 << 40),
-                 (4096, 4096, None, 1, None, None, 4096, 4096, 4096, None, 4096, 1 << 40),
-                 (4096, None, None, 1, None, 4096, 4096, 4096, 4096, None, 4096, 1 << 40),
-                 (4096, 4096, None, 1, None, 4096, 4096, 4096, None, 4096, 4096, 1 << 40),
-                 (4096, 4096, None, 1, 4096, 4096, 4096, 4096, 4096, None, 4096, 1 << 40),   # no order of ten rows
-                 (4096, 4096, None, 3, None, 4096, 4096, 4096, 4096, None, 4096, 1 << 40),   # no weights
-                 (4096, 4096, None, 0, None, 4096, 4096, 4096, 4096, None, 4096, 1 << 40),
-                 (4096, 4096, None, 1, None, 4096, 4096, 4096, 4096, None, 4096, 16)):
-        assert bwd(*args) != 0, args
-    assert lib.sgl_candidates_teacher(10, 0, 20, 4096, 4096, 1.0, 4096, 4096, 4096, None) != 0
-    assert lib.sgl_candidates_teacher(10, 1025, 20, 4096, 4096, 1.0, 4096, 4096, 4096, None) != 0
-    assert lib.sgl_candidates_teacher(10, 5, 20, 4096, None, 1.0, 4096, 4096, 4096, None) != 0
-    assert lib.sgl_candidates_teacher(10, 5, 20, 4096, 4096, -1.0, 4096, 4096, 4096, None) != 0
+    lib, ref, big = _capi.lib(), ctypes.byref(_problem()), 1 << 40
+    good = dict(target=4096, ids=None, logits=None, k=1, need=3, loss=4096, keep=4096, nk=big, ws=4096, nb=big)
+    for kw, what in (
+            (dict(k=2), b"2 targets"), (dict(k=0), b"0 targets"),
+            (dict(target=None, ids=4096, logits=4096, k=1025), b"1025 targets"),
+            (dict(target=None, ids=4096, k=3), b"NULL array"), (dict(target=None), b"NULL array"),
+            (dict(ids=4096), b"at once"), (dict(logits=4096), b"at once"), (dict(loss=None), b"NULL array"),
+            (dict(need=4), b"need 4"), (dict(need=-1), b"need -1"), (dict(keep=None), b"for the backward"),
+            (dict(nk=16), b"for the backward"), (dict(ws=None), b"workspace"), (dict(nb=16), b"workspace")):
+        args = {**good, **kw}
+        assert lib.sgl_candidates_forward(ref, *args.values(), None) != 0, kw
+        assert what in lib.sgl_last_error(), kw
+    good = dict(k=1, teacher=0, need=3, keep=4096, nk=big, g=4096, dh=4096, dtable=4096, dbias=None, ws=4096, nb=big)
+    for kw, what in (
+            (dict(k=2), b"2 targets"), (dict(k=0, teacher=1), b"0 targets"), (dict(need=0), b"need 0"),
+            (dict(g=None), b"did not prepare"), (dict(need=1), b"did not prepare"), (dict(need=2), b"did not prepare"),
+            (dict(dtable=None, dbias=4096), b"did not prepare"), (dict(keep=None), b"for the backward"),
+            (dict(nk=16), b"for the backward"), (dict(ws=None), b"workspace"), (dict(nb=16), b"workspace")):
+        args = {**good, **kw}
+        assert lib.sgl_candidates_backward(ref, *args.values(), None) != 0, kw
+        assert what in lib.sgl_last_error(), kw
+    none = ctypes.byref(_problem(n=0))
+    assert lib.sgl_candidates_backward(none, *good.values(), None) != 0
     side = _capi.RotarySide(4096, 4096, 4096, 5, 40, 8, 8, 5, 1, 1)
     s = ctypes.byref(side)
     for args in ((3, 2, 8, 8, s, s, 4096, 0, 1.0, 0), (0, -1, 8, 8, s, s, 4096, 0, 1.0, 0),
