@@ -14,6 +14,8 @@
 // softmax; the gradient takes x from the table and y from the rows.
 #pragma once
 
+#include <utility>
+
 #include "cross_attention.h"
 
 namespace sgl {
@@ -65,11 +67,11 @@ __device__ __forceinline__ int half_of_wave() { return (threadIdx.x >> 5) & 1; }
 
 // Accumulators [4 B s, 4 B (s + 1)) as the operand of reduction step s.
 template <typename T>
-__device__ __forceinline__ FragOf<T> frag_of16(const f32x16 &p, int s) {
+__device__ __forceinline__ FragOf<T> frag_of16(const f32x16 &p, int s, float by = 1.f) {
   FragOf<T> f;
   constexpr int E = Mma32<T>::E;
 #pragma unroll
-  for (int e = 0; e < E; ++e) f[e] = T(p[s * E + e]);
+  for (int e = 0; e < E; ++e) f[e] = T(p[s * E + e] * by);
   return f;
 }
 
@@ -230,14 +232,22 @@ __device__ __forceinline__ void scale_blocks(f32x16 (&o)[NB], float by) {
 #pragma unroll
   for (int d = 0; d < NB; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float x = o[d][r], t;
-      asm volatile("v_accvgpr_read_b32 %1, %0\n\ts_nop 1\n\tv_mul_f32 %1, %1, %2\n\ts_nop 1\n\tv_accvgpr_write_b32 %0, %1"
-                   : "+a"(x), "=&v"(t)
+    for (int r = 0; r < 16; r += 4) {
+      float x[4], t[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = o[d][r + i];
+      asm volatile("v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\t"
+                   "v_accvgpr_read_b32 %6, %2\n\tv_accvgpr_read_b32 %7, %3\n\t"
+                   "v_mul_f32 %4, %4, %8\n\tv_mul_f32 %5, %5, %8\n\t"
+                   "v_mul_f32 %6, %6, %8\n\tv_mul_f32 %7, %7, %8\n\t"
+                   "v_accvgpr_write_b32 %0, %4\n\tv_accvgpr_write_b32 %1, %5\n\t"
+                   "v_accvgpr_write_b32 %2, %6\n\tv_accvgpr_write_b32 %3, %7"
+                   : "+a"(x[0]), "+a"(x[1]), "+a"(x[2]), "+a"(x[3]), "=&v"(t[0]), "=&v"(t[1]), "=&v"(t[2]), "=&v"(t[3])
                    : "v"(by));
-      o[d][r] = x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[d][r + i] = x[i];
     }
-  asm volatile("s_nop 7" ::: "memory");
+  asm volatile("s_nop 15" ::: "memory");
 }
 __device__ __forceinline__ float abs_max16(const f32x16 &p) {   // (three operands an instruction)
   float a = fabsf(p[0]);
@@ -247,6 +257,19 @@ __device__ __forceinline__ float abs_max16(const f32x16 &p) {   // (three operan
 }
 // 2^x by the hardware instruction (1 ulp; results under 2^-126 are 0).
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// f(0) .. f(N - 1) with constants for arguments.
+template <typename F, int... J>
+__device__ __forceinline__ void each(std::integer_sequence<int, J...>, F &&f) {
+  (f(std::integral_constant<int, J>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F &&f) {
+  each(std::make_integer_sequence<int, N>{}, f);
+}
+// Between two chunks of a step: the compiler's scheduler moves nothing across,
+// so that a chunk's vector instructions stay beside its matrix instructions.
+__device__ __forceinline__ void chunk_end() { __builtin_amdgcn_sched_barrier(0); }
 
 // The problem as the kernels take it. Scores are to base 2: c <h, w> + cb bias.
 struct Problem {

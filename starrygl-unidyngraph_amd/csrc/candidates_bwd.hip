@@ -16,12 +16,14 @@ struct BwdArgs {
 
 // fp16: a coefficient goes into the product times a power of two a candidate
 // that follows its largest magnitude so far (from a start that any value
-// passes: beyond 2^15 the largest is brought to 2^10), so that terms keep their
-// digits down to 2^-24 of the largest whatever the gradients and p are of.
+// passes: beyond 2^15 the largest is brought to 2^4, far enough below that a
+// target after many small p does not do it again), so that terms keep their
+// digits down to 2^-18 of the largest, and some of them to 2^-28, whatever the
+// gradients and p are of.
 constexpr float kFirstScale = 0x1p100f, kMostHalf = 32768.f;
 __device__ __forceinline__ float half_scale(float most) {   // (1 for what is not finite)
   const int e = int(__float_as_uint(most) >> 23);           // most >= 0
-  return e >= 255 ? 1.f : __uint_as_float(uint32_t(min(max(264 - e, 1), 254)) << 23);
+  return e >= 255 ? 1.f : __uint_as_float(uint32_t(min(max(258 - e, 1), 254)) << 23);
 }
 
 // Candidates of a workgroup, rows of a tile (32 where more of them on their way
@@ -29,7 +31,7 @@ __device__ __forceinline__ float half_scale(float most) {   // (1 for what is no
 template <typename T>
 constexpr int kXTile = sizeof(T) == 4 ? 128 : 256;
 template <typename T, int DB>
-constexpr int kYTile = sizeof(T) == 4 || DB == 8 ? 32 : 64;
+constexpr int kYTile = sizeof(T) == 4 || DB >= 6 ? 32 : 64;
 
 // XB blocks of 32 candidates a wave, four waves along the candidates.
 template <typename T, int DB, int XB>
@@ -60,7 +62,7 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
   const T *rows_h = static_cast<const T *>(p.h);
 
   Stage<T, DP, YT> next(p.hs, p.D);
-  float nc[3];
+  float c_nm = 0.f, c_gl = 0.f, c_gq = 0.f;
   int nid = -1, ne0 = 0, ne1 = 0;
   auto fetch = [&](int t, int xt) {
     const int64_t y0 = int64_t(t) * YT;
@@ -68,18 +70,22 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
     next.fetch(rows_h + y0 * p.hs, rows, a.r.nm + y0);   // (a row without a gradient may hold anything)
     if (tid < YT) {
       const int64_t n = y0 + min(tid, rows - 1);
-      nc[0] = a.r.nm[n];
-      nc[1] = a.r.gl[n];
-      nc[2] = a.r.gq[n];
+      c_nm = a.r.nm[n];
+      c_gl = a.r.gl[n];
+      c_gq = a.r.gq[n];
     }
+    int id = -1, from = 0, to = 0;   // (all three assigned on either way: one store behind a choice of places is memory)
     if (a.r.index == nullptr) {
-      nid = a.r.ids[y0 + min(lane, rows - 1)];
+      id = a.r.ids[y0 + min(lane, rows - 1)];
     } else {
       const int64_t vb = int64_t(xt) * kWaves + wave;
       const int32_t *at = a.r.index + int64_t(t) * (a.r.vblocks + 1) + min(vb, a.r.vblocks - 1);
-      ne0 = attn::scalar_load(at);
-      ne1 = vb < a.r.vblocks ? attn::scalar_load(at + 1) : ne0;
+      from = attn::scalar_load(at);
+      to = vb < a.r.vblocks ? attn::scalar_load(at + 1) : from;
     }
+    nid = id;
+    ne0 = from;
+    ne1 = to;
   };
   for (int i = tid; i < XT * QL / 4; i += kBlock) reinterpret_cast<f32x4 *>(q_all)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   Stage<T, DP, YT>::clear(tiles);
@@ -120,13 +126,13 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
     const int rows = int(min(N - int64_t(t) * YT, int64_t(YT)));
     next.put(tile, rows, true);
     if (tid < YT) {
-      cf[tid] = tid < rows ? nc[0] : -INFINITY;
-      cf[YT + tid] = tid < rows ? nc[1] : 0.f;
-      cf[2 * YT + tid] = tid < rows ? nc[2] : 0.f;
+      cf[tid] = tid < rows ? c_nm : -INFINITY;
+      cf[YT + tid] = tid < rows ? c_gl : 0.f;
+      cf[2 * YT + tid] = tid < rows ? c_gq : 0.f;
     }
     // what the tile's rows want of the wave's candidates: a row has a candidate once, so each place once
-    const int64_t mine = int64_t(nid) - (int64_t(xt) * XT + wave * WV);
-    const bool one = a.r.index == nullptr && lane < rows && nid >= 0 && uint64_t(mine) < uint64_t(WV);
+    const int mine = nid - (xt * XT + wave * WV);   // (nid -1: none of the wave's, -1 but for the first candidates)
+    const bool one = a.r.index == nullptr && lane < rows && nid >= 0 && uint32_t(mine) < uint32_t(WV);
     const int e0 = ne0, e1 = ne1;
     const int2 *entries = a.r.entries + int64_t(t) * YT * a.r.K;
     const bool wanted = __any(one) || e0 < e1;
@@ -154,18 +160,20 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
 #pragma unroll
         for (int xb = 0; xb < XB; ++xb) s[xb] = M::mma(f, xf[xb][k], s[xb]);
       }
+      auto coefficients = [&]() {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float nm[4], gl[4];
-        __builtin_memcpy(nm, cf + row0 + 8 * i + 4 * h, sizeof(nm));
-        __builtin_memcpy(gl, cf + YT + row0 + 8 * i + 4 * h, sizeof(gl));
+        for (int i = 0; i < 4; ++i) {
+          float nm[4], gl[4];
+          __builtin_memcpy(nm, cf + row0 + 8 * i + 4 * h, sizeof(nm));
+          __builtin_memcpy(gl, cf + YT + row0 + 8 * i + 4 * h, sizeof(gl));
 #pragma unroll
-        for (int xb = 0; xb < XB; ++xb)
+          for (int xb = 0; xb < XB; ++xb)
 #pragma unroll
-          for (int v = 0; v < 4; ++v)
-            s[xb][4 * i + v] = exp2_fast(fmaf(s[xb][4 * i + v], p.c, b2[xb]) + nm[v]) * gl[v];
-      }
-      if (wanted) {
+            for (int v = 0; v < 4; ++v)
+              s[xb][4 * i + v] = exp2_fast(fmaf(s[xb][4 * i + v], p.c, b2[xb]) + nm[v]) * gl[v];
+        }
+      };
+      auto targets = [&]() {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float gq[4];
@@ -184,44 +192,39 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
           const int x = entries[e].x;
           if (((x >> 5) & 1) == ys) q[(x >> 6) * QL + (x & 31)] = 0.f;
         }
-      }
-      if (a.dbias != nullptr) {
-#pragma unroll
-        for (int xb = 0; xb < XB; ++xb) db[xb] += sum16(s[xb]);
-      }
-      if constexpr (HALF) {
-        float most[XB];
-        bool over = false;
-#pragma unroll
-        for (int xb = 0; xb < XB; ++xb) {
-          most[xb] = pair_max(abs_max16(s[xb]));
-          over |= most[xb] * sc[xb] > kMostHalf;
-        }
-        if (__any(over)) {
+      };
+      auto product = [&]() {
+        if constexpr (HALF) {
 #pragma unroll
           for (int xb = 0; xb < XB; ++xb) {
-            const float to = most[xb] * sc[xb] > kMostHalf ? half_scale(most[xb]) : sc[xb];
-            const float by = to / sc[xb];
-            sc[xb] = to;
-            scale_blocks(o[xb], by);
+            const float most = pair_max(abs_max16(s[xb]));
+            const bool over = most * sc[xb] > kMostHalf;
+            if (__any(over)) {
+              const float to = over ? half_scale(most) : sc[xb];
+              scale_blocks(o[xb], to / sc[xb]);
+              sc[xb] = to;
+            }
           }
         }
 #pragma unroll
-        for (int xb = 0; xb < XB; ++xb)
+        for (int st = 0; st < 32 / KS; ++st) {
+          FragOf<T> pf[XB];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[xb][r] *= sc[xb];
-      }
+          for (int xb = 0; xb < XB; ++xb) pf[xb] = frag_of16<T>(s[xb], st, HALF ? sc[xb] : 1.f);
 #pragma unroll
-      for (int st = 0; st < 32 / KS; ++st) {
-        FragOf<T> pf[XB];
+          for (int d = 0; d < DB; ++d) {
+            const FragOf<T> f = Tl::frag_t(tile, 32 * d, row0, st);
 #pragma unroll
-        for (int xb = 0; xb < XB; ++xb) pf[xb] = frag_of16<T>(s[xb], st);
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          const FragOf<T> f = Tl::frag_t(tile, 32 * d, row0, st);
-#pragma unroll
-          for (int xb = 0; xb < XB; ++xb) o[xb][d] = M::mma(f, pf[xb], o[xb][d]);
+            for (int xb = 0; xb < XB; ++xb) o[xb][d] = M::mma(f, pf[xb], o[xb][d]);
+          }
         }
+      };
+      coefficients();
+      if (wanted) targets();
+      product();
+      if (a.dbias != nullptr) {
+#pragma unroll
+        for (int xb = 0; xb < XB; ++xb) db[xb] += sum16(s[xb]);
       }
     }
   }
@@ -389,7 +392,7 @@ namespace sgl {
 namespace cand {
 
 int table_grad_tile(int32_t dtype, int D) {
-  return dtype == SGL_FP32 ? 32 : padded_dim(D) == 256 ? kYTile<bf16_t, 8> : kYTile<bf16_t, 2>;
+  return dtype == SGL_FP32 ? 32 : padded_dim(D) >= 192 ? kYTile<bf16_t, 8> : kYTile<bf16_t, 2>;
 }
 int table_grad_block(int32_t dtype) { return (dtype == SGL_FP32 ? kXTile<float> : kXTile<bf16_t>) / kWaves; }
 int64_t table_grad_part(int32_t dtype, const Problem &p) {
