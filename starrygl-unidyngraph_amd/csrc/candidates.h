@@ -324,20 +324,28 @@ int padded_dim(int D);
 Partials forward_shape(int32_t dtype, const Problem &p);   // (without its arrays)
 void forward_partials(int32_t dtype, const Problem &p, const Order &order, const Partials &out, hipStream_t stream);
 
+// The rows as the table's gradient takes them: tiles that are copied to LDS as
+// they lie. A tile: its rows, `ld` elements apart, zeros past the last channel,
+// then for each row minus the maximum, g T / l, g T and the candidate wanted of
+// labels (-1: none); rows without a gradient and past the last one: zeros, -inf, 0, 0, -1.
+struct Image {
+  int rows, ld;    // of a tile, elements of a row
+  int64_t bytes;   // of a tile
+};
+Image grad_image(int32_t dtype, int D);
+
 struct RowCoef {
-  const float *nm, *gl, *gq;   // [N]: minus the maximum, g T / l, g T (dead rows: -inf, 0, 0)
-  const int32_t *live;         // [1] or NULL: rows that count (the first ones)
-  const int32_t *ids;          // [N], -1: none, with index NULL; else
-  const int32_t *index;        // [ytiles][vblocks + 1]: a row tile's entries by candidate block
-  const int2 *entries;         // [N K], a row tile's first at tile * rows * K: candidate of the block * 64 + row
-                               // of the tile, weight
+  const char *image;
+  const int32_t *live;     // [1] or NULL: rows that count (the first ones)
+  const int32_t *index;    // NULL: labels; else [tiles][vblocks + 1]: a tile's entries by candidate block
+  const int2 *entries;     // [N K], a tile's first at tile * rows * K: candidate of the block * 64 + row of the
+                           // tile, weight
   int64_t vblocks;
   int K;
 };
 void route_targets(int32_t dtype, const Problem &p, int K, const int32_t *ids, const float *weight, int32_t *index,
                    int2 *entries, hipStream_t stream);
-int table_grad_tile(int32_t dtype, int D);   // rows of a tile
-int table_grad_block(int32_t dtype);         // candidates of a wave
+int table_grad_block(int32_t dtype);    // candidates of a wave
 // fp32 elements of `part` at most (those of tiles that are not shared out are never touched).
 int64_t table_grad_part(int32_t dtype, const Problem &p);
 void table_grad(int32_t dtype, const Problem &p, const RowCoef &r, void *dtable, float *dbias, float *part,

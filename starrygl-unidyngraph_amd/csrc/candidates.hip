@@ -317,42 +317,50 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
 }
 
 // ------------------------------------------------------------------ the gradients' rows
-// In the order that the table's gradient takes them: with `order` the rows
-// that have a target, theirs packed.
+// dh, and the rows' image for the table's gradient, in its order: with `order`
+// those that have a target, then tiles filled up.
 struct RowArgs {
   Problem p;
   Order order;
   const float *stat, *dir, *g;
-  const int32_t *ids;        // [N] or NULL
+  const int32_t *ids;        // [N] of labels, or NULL
   void *dh;                  // or NULL
-  float *nm, *gl, *gq;       // or NULL
-  void *packed;              // [N][D], and their ids, with `order`
-  int32_t *packed_ids;
+  char *image;               // or NULL
+  Image im;
 };
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_rows(RowArgs a) {
   const Problem &p = a.p;
   const int lane = threadIdx.x & 63;
   const int64_t pos = int64_t(blockIdx.x) * kWaves + attn::wave_index();
-  if (pos >= p.N) return;
-  const int64_t n = a.order.row(pos);
-  const Cols c(p.D);
-  const float m = a.stat[n], il = a.stat[p.N + n];
+  const bool here = pos < p.N;
+  const int64_t n = here ? a.order.row(pos) : 0;
+  const float m = here ? a.stat[n] : 0.f, il = here ? a.stat[p.N + n] : 0.f;
   const bool live = !(il == 0.f);
   const float g = live ? a.g[n] * p.temperature : 0.f;
-  if (a.nm != nullptr && lane == 0) {
-    a.nm[pos] = !live ? -INFINITY : m == INFINITY ? NAN : -m;
-    a.gl[pos] = g * il;
-    a.gq[pos] = g;
-    if (a.packed_ids != nullptr) a.packed_ids[pos] = a.ids[n];
+  if (a.image != nullptr) {
+    const int64_t tile = pos / a.im.rows;
+    const int r = int(pos - tile * a.im.rows);
+    char *image = a.image + tile * a.im.bytes;
+    T *row = reinterpret_cast<T *>(image) + r * a.im.ld;
+    const T *h = static_cast<const T *>(p.h) + n * p.hs;
+    const int width = a.im.ld - 16 / int(sizeof(T));   // (the padding is not read)
+    if (4 * lane < width) {
+      T x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = live && 4 * lane + j < p.D ? h[4 * lane + j] : T(0.f);
+      store_n(row + 4 * lane, x);
+    }
+    if (lane == 0) {
+      float *c = reinterpret_cast<float *>(image + a.im.rows * a.im.ld * int(sizeof(T))) + r;
+      c[0] = !live ? -INFINITY : m == INFINITY ? NAN : -m;
+      c[a.im.rows] = g * il;
+      c[2 * a.im.rows] = g;
+      reinterpret_cast<int32_t *>(c)[3 * a.im.rows] = live && a.ids != nullptr ? a.ids[n] : -1;
+    }
   }
-  if (!c.here) return;
-  if (a.packed != nullptr && live) {
-    T x[4];
-    load_n(x, static_cast<const T *>(p.h) + n * p.hs + c.d);
-    store_n(static_cast<T *>(a.packed) + pos * p.D + c.d, x);
-  }
-  if (a.dh != nullptr) {
+  const Cols c(p.D);
+  if (a.dh != nullptr && here && c.here) {
     float e[4] = {};
     if (live) load_n(e, a.dir + n * p.D + c.d);
     T x[4];
@@ -431,25 +439,21 @@ Keep carve_keep(void *keep, const Problem &p, int K, bool teacher, int32_t need,
 }
 
 struct Grad {
-  float *nm, *gl, *gq, *part;
-  char *packed;
-  int32_t *ids, *index;
+  char *image;
+  float *part;
+  int32_t *index;
   int2 *entries;
 };
 Grad carve_backward(void *ws, int32_t dtype, const Problem &p, int K, bool teacher, size_t *bytes) {
   Carver c(ws);
   Grad g{};
-  g.nm = c.take<float>(size_t(p.N));
-  g.gl = c.take<float>(size_t(p.N));
-  g.gq = c.take<float>(size_t(p.N));
+  const Image im = grad_image(dtype, p.D);
+  const size_t tiles = size_t((p.N + im.rows - 1) / im.rows);
+  g.image = c.take<char>(tiles * size_t(im.bytes));
   if (teacher) {
-    const int yt = table_grad_tile(dtype, p.D), vb = table_grad_block(dtype);
-    const size_t tiles = size_t((p.N + yt - 1) / yt);
+    const int vb = table_grad_block(dtype);
     g.index = c.take<int32_t>(tiles * size_t((p.V + vb - 1) / vb + 1));
-    g.entries = c.take<int2>(tiles * size_t(yt) * size_t(K));
-  } else if (orders(p.N)) {
-    g.packed = c.take<char>(size_t(p.N) * size_t(p.D) * (dtype == SGL_FP32 ? 4 : 2));
-    g.ids = c.take<int32_t>(size_t(p.N));
+    g.entries = c.take<int2>(tiles * size_t(im.rows) * size_t(K));
   }
   g.part = c.take<float>(size_t(table_grad_part(dtype, p)));
   *bytes = c.used;
@@ -550,17 +554,15 @@ extern "C" int sgl_candidates_backward(const sgl_candidates *problem, int32_t k,
     if (const int rc = check_room("workspace", workspace, workspace_bytes, room)) return rc;
   }
   const Order o{kept.order, kept.order != nullptr ? kept.order + p.N : nullptr};
-  const RowArgs a{p, o, kept.stat, kept.dir, g, kept.ids, dh, w.nm, w.gl, w.gq, w.packed, w.ids};
-  const dim3 grid(unsigned((p.N + kWaves - 1) / kWaves));
+  const Image im = grad_image(problem->dtype, p.D);
+  const int64_t rows = dtable != nullptr ? (p.N + im.rows - 1) / im.rows * im.rows : p.N;
+  const RowArgs a{p, o, kept.stat, kept.dir, g, teacher != 0 ? nullptr : kept.ids, dh, w.image, im};
+  const dim3 grid(unsigned((rows + kWaves - 1) / kWaves));
   if (problem->dtype == SGL_FP32) sgl::launch(&k_rows<float>, grid, dim3(kBlock), 0, stream, a);
   else if (problem->dtype == SGL_BF16) sgl::launch(&k_rows<bf16_t>, grid, dim3(kBlock), 0, stream, a);
   else sgl::launch(&k_rows<fp16_t>, grid, dim3(kBlock), 0, stream, a);
   if (dtable != nullptr) {
-    RowCoef r{w.nm, w.gl, w.gq, o.live, w.ids != nullptr ? w.ids : kept.ids, w.index, w.entries, 0, k};
-    if (w.packed != nullptr) {
-      p.h = w.packed;
-      p.hs = p.D;
-    }
+    RowCoef r{w.image, o.live, w.index, w.entries, 0, k};
     if (teacher != 0) {
       const int vb = table_grad_block(problem->dtype);
       r.vblocks = (p.V + vb - 1) / vb;

@@ -33,22 +33,27 @@ constexpr int kXTile = sizeof(T) == 4 ? 128 : 256;
 template <typename T, int DB>
 constexpr int kYTile = sizeof(T) == 4 || DB >= 6 ? 32 : 64;
 
+template <typename T, int DB>
+struct Tiles {
+  static constexpr int YT = kYTile<T, DB>, LD = Tile32<T, 32 * DB>::LD;
+  static constexpr int ROWS = YT * LD * int(sizeof(T)), BYTES = ROWS + 16 * YT;
+  static_assert(BYTES % 1024 == 0, "whole loads of a wave");
+};
+
 // XB blocks of 32 candidates a wave, four waves along the candidates.
 template <typename T, int DB, int XB>
 __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
   using M = Mma32<T>;
   constexpr int KS = M::KS, DP = 32 * DB, NK = DP / KS;
   using Tl = Tile32<T, DP>;
-  constexpr int LD = Tl::LD;
   constexpr int YT = kYTile<T, DB>, YS = YT / 32, XT = 32 * XB * kWaves, QL = 32 + 4;
   constexpr bool HALF = std::is_same_v<T, fp16_t>;
   constexpr int WV = 32 * XB;   // candidates of a wave
   extern __shared__ __align__(16) char lds[];
-  T *tiles = reinterpret_cast<T *>(lds);
-  float *coef = reinterpret_cast<float *>(lds + size_t(2) * YT * LD * sizeof(T));   // [2][3][YT]
+  using Im = Tiles<T, DB>;
   // [XT][QL]: what 32 rows want of the candidates; zero between uses. A wave writes, reads and clears
   // its own candidates' part.
-  float *q_all = coef + 2 * 3 * YT;
+  float *q_all = reinterpret_cast<float *>(lds + 2 * Im::BYTES);
 
   const Problem &p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, col = lane & 31;
@@ -59,37 +64,24 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
   const int w = blockIdx.x;
   if (w >= line.groups) return;
   const int64_t u1 = line.begin(w + 1);
-  const T *rows_h = static_cast<const T *>(p.h);
 
-  Stage<T, DP, YT> next(p.hs, p.D);
-  float c_nm = 0.f, c_gl = 0.f, c_gq = 0.f;
-  int nid = -1, ne0 = 0, ne1 = 0;
+  constexpr int NL = (Im::BYTES + 16 * kBlock - 1) / (16 * kBlock);
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 next[NL];
+  int ne0 = 0, ne1 = 0;
   auto fetch = [&](int t, int xt) {
-    const int64_t y0 = int64_t(t) * YT;
-    const int rows = max(int(min(N - y0, int64_t(YT))), 1);
-    next.fetch(rows_h + y0 * p.hs, rows, a.r.nm + y0);   // (a row without a gradient may hold anything)
-    if (tid < YT) {
-      const int64_t n = y0 + min(tid, rows - 1);
-      c_nm = a.r.nm[n];
-      c_gl = a.r.gl[n];
-      c_gq = a.r.gq[n];
-    }
-    int id = -1, from = 0, to = 0;   // (all three assigned on either way: one store behind a choice of places is memory)
-    if (a.r.index == nullptr) {
-      id = a.r.ids[y0 + min(lane, rows - 1)];
-    } else {
+    const u32x4 *src = reinterpret_cast<const u32x4 *>(a.r.image + int64_t(t) * Im::BYTES);
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      if ((i + 1) * 16 * kBlock <= Im::BYTES || (i * kWaves + wave) * 1024 < Im::BYTES) next[i] = src[i * kBlock + tid];
+    if (a.r.index != nullptr) {
       const int64_t vb = int64_t(xt) * kWaves + wave;
       const int32_t *at = a.r.index + int64_t(t) * (a.r.vblocks + 1) + min(vb, a.r.vblocks - 1);
-      from = attn::scalar_load(at);
-      to = vb < a.r.vblocks ? attn::scalar_load(at + 1) : from;
+      ne0 = attn::scalar_load(at);
+      ne1 = vb < a.r.vblocks ? attn::scalar_load(at + 1) : ne0;
     }
-    nid = id;
-    ne0 = from;
-    ne1 = to;
   };
   for (int i = tid; i < XT * QL / 4; i += kBlock) reinterpret_cast<f32x4 *>(q_all)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  Stage<T, DP, YT>::clear(tiles);
-  Stage<T, DP, YT>::clear(tiles + YT * LD);
   int64_t u = line.begin(w);
   int xt = int(u / line.inner), t = int(u - int64_t(xt) * line.inner), buf = 0;
   fetch(t, xt);
@@ -120,23 +112,22 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
   u += end - t;
 #pragma unroll 1
   for (; t < end; ++t) {
-    T *tile = tiles + buf * YT * LD;
-    float *cf = coef + buf * 3 * YT;
+    char *image = lds + buf * Im::BYTES;
+    const T *tile = reinterpret_cast<const T *>(image);
+    const float *cf = reinterpret_cast<const float *>(image + Im::ROWS);
     buf ^= 1;
-    const int rows = int(min(N - int64_t(t) * YT, int64_t(YT)));
-    next.put(tile, rows, true);
-    if (tid < YT) {
-      cf[tid] = tid < rows ? c_nm : -INFINITY;
-      cf[YT + tid] = tid < rows ? c_gl : 0.f;
-      cf[2 * YT + tid] = tid < rows ? c_gq : 0.f;
-    }
-    // what the tile's rows want of the wave's candidates: a row has a candidate once, so each place once
-    const int mine = nid - (xt * XT + wave * WV);   // (nid -1: none of the wave's, -1 but for the first candidates)
-    const bool one = a.r.index == nullptr && lane < rows && nid >= 0 && uint32_t(mine) < uint32_t(WV);
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      if ((i + 1) * 16 * kBlock <= Im::BYTES || (i * kWaves + wave) * 1024 < Im::BYTES)
+        reinterpret_cast<u32x4 *>(image)[i * kBlock + tid] = next[i];
     const int e0 = ne0, e1 = ne1;
     const int2 *entries = a.r.entries + int64_t(t) * YT * a.r.K;
-    const bool wanted = __any(one) || e0 < e1;
     __syncthreads();
+    // what the tile's rows want of the wave's candidates: a row has a candidate once, so each place once
+    const int id = a.r.index == nullptr && lane < YT ? reinterpret_cast<const int *>(cf)[3 * YT + lane] : -1;
+    const int mine = id - (xt * XT + wave * WV);
+    const bool one = id >= 0 && uint32_t(mine) < uint32_t(WV);
+    const bool wanted = __any(one) || e0 < e1;
     if (t + 1 < end || u < u1) fetch(t + 1 < end ? t + 1 : 0, t + 1 < end ? xt : xt + 1);
 #pragma unroll 1
     for (int ys = 0; ys < YS; ++ys) {
@@ -364,9 +355,9 @@ __global__ __launch_bounds__(kRouteBlock) void k_route(RouteArgs a) {
 template <typename T, int DB>
 void run(const BwdArgs &a, hipStream_t stream) {
   constexpr int XB = sizeof(T) == 4 ? 1 : 2;
-  constexpr int LD = Tile32<T, 32 * DB>::LD, YT = kYTile<T, DB>, XT = kXTile<T>;
+  constexpr int YT = kYTile<T, DB>, XT = kXTile<T>;
   static_assert(XT == 32 * XB * kWaves, "");
-  constexpr size_t bytes = size_t(2) * YT * LD * sizeof(T) + sizeof(float) * (6 * YT + XT * 36);
+  constexpr size_t bytes = size_t(2) * Tiles<T, DB>::BYTES + sizeof(float) * XT * 36;
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
   auto *k = &k_table_grad<T, DB, XB>;
   (void)ensure_dynamic_lds(reinterpret_cast<const void *>(k), bytes);
@@ -391,9 +382,16 @@ void pick(const Problem &p, const RowCoef &r, void *dtable, float *dbias, float 
 namespace sgl {
 namespace cand {
 
-int table_grad_tile(int32_t dtype, int D) {
-  return dtype == SGL_FP32 ? 32 : padded_dim(D) >= 192 ? kYTile<bf16_t, 8> : kYTile<bf16_t, 2>;
+template <typename T>
+Image image_of(int D) {
+  switch (padded_dim(D)) {
+    case 64: return Image{Tiles<T, 2>::YT, Tiles<T, 2>::LD, Tiles<T, 2>::BYTES};
+    case 128: return Image{Tiles<T, 4>::YT, Tiles<T, 4>::LD, Tiles<T, 4>::BYTES};
+    case 192: return Image{Tiles<T, 6>::YT, Tiles<T, 6>::LD, Tiles<T, 6>::BYTES};
+    default: return Image{Tiles<T, 8>::YT, Tiles<T, 8>::LD, Tiles<T, 8>::BYTES};
+  }
 }
+Image grad_image(int32_t dtype, int D) { return dtype == SGL_FP32 ? image_of<float>(D) : image_of<bf16_t>(D); }
 int table_grad_block(int32_t dtype) { return (dtype == SGL_FP32 ? kXTile<float> : kXTile<bf16_t>) / kWaves; }
 int64_t table_grad_part(int32_t dtype, const Problem &p) {
   const int64_t xtile = dtype == SGL_FP32 ? kXTile<float> : kXTile<bf16_t>;
@@ -403,7 +401,7 @@ int64_t table_grad_part(int32_t dtype, const Problem &p) {
 void route_targets(int32_t dtype, const Problem &p, int K, const int32_t *ids, const float *weight, int32_t *index,
                    int2 *entries, hipStream_t stream) {
   const int64_t N = p.N, V = p.V;
-  const int yt = table_grad_tile(dtype, p.D), vb = table_grad_block(dtype);
+  const int yt = grad_image(dtype, p.D).rows, vb = table_grad_block(dtype);
   const RouteArgs a{ids, weight, N, (V + vb - 1) / vb, K, yt, vb, index, entries};
   launch(&k_route, dim3(unsigned((N + yt - 1) / yt)), dim3(kRouteBlock), 0, stream, a);
 }
