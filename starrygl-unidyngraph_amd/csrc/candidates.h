@@ -1,8 +1,8 @@
 // What the kernels over all candidates share: the problem, 32 x 32 matrix
 // products over the three types, row tiles in LDS.
 //
-// One engine serves the forward and the table's gradient. A wave keeps 32 or
-// 64 outer rows x (as the columns of its products) and walks over inner rows y
+// One engine serves the forward and the table's gradient. A wave keeps 32
+// outer rows x (as the columns of its products) and walks over inner rows y
 // in tiles that the workgroup shares:
 //   S^T[y, x] = <y, x>      (reduction over the channels)
 //   P^T[y, x] = f(S^T)      (elementwise, in the accumulators)
@@ -66,8 +66,8 @@ struct Mma32<fp16_t> {
 __device__ __forceinline__ int half_of_wave() { return (threadIdx.x >> 5) & 1; }
 
 // Accumulators [4 B s, 4 B (s + 1)) as the operand of reduction step s.
-template <typename T>
-__device__ __forceinline__ FragOf<T> frag_of16(const f32x16 &p, int s, float by = 1.f) {
+template <typename T, typename V>
+__device__ __forceinline__ FragOf<T> frag_of16(const V &p, int s, float by = 1.f) {
   FragOf<T> f;
   constexpr int E = Mma32<T>::E;
 #pragma unroll
@@ -109,17 +109,17 @@ struct Tile32 {
 };
 
 // A tile's YT rows on their way from memory to LDS: 16 bytes a load, eight
-// lanes a row and 128 bytes of it, 32 rows a step. A row's partial last load is
+// lanes a row and 128 bytes of it, BLOCK / 8 rows a step. A row's partial last load is
 // taken from D - E (it writes what its neighbour writes, with the same values;
 // columns past D are cleared once), so that loads and stores are all whole.
 // Rows past the tensor's end are read as the last one and written as zeros, as
 // are those marked -inf: they may hold anything.
 constexpr int64_t kMaxStride = 1 << 22;   // of a row: a tile's offsets stay in 32 bits
-template <typename T, int DP, int YT>
+template <typename T, int DP, int YT, int BLOCK = kBlock>
 struct Stage {
   using Tl = Tile32<T, DP>;
-  static constexpr int E = Tl::E, CB = Tl::UPR / 8, RB = YT / 32, SZ = int(sizeof(T));
-  static_assert(kBlock == 256 && YT % 32 == 0 && Tl::UPR % 8 == 0, "eight lanes a row of 32");
+  static constexpr int E = Tl::E, CB = Tl::UPR / 8, ROWS = BLOCK / 8, RB = YT / ROWS, SZ = int(sizeof(T));
+  static_assert(YT % ROWS == 0 && Tl::UPR % 8 == 0, "eight lanes a row");
   FragOf<T> f[RB][CB];
   float mark[RB];      // a value that may still be on its way
   uint32_t from[CB];   // bytes from the tile's first row
@@ -141,11 +141,11 @@ struct Stage {
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
       // (rows past the end: back to the last one)
-      const int back = rows >= YT ? 0 : max(32 * i + r - (rows - 1), 0);
+      const int back = rows >= YT ? 0 : max(ROWS * i + r - (rows - 1), 0);
 #pragma unroll
       for (int c = 0; c < CB; ++c)
-        __builtin_memcpy(&f[i][c], b + (from[c] + uint32_t((32 * i - back) * stride)), sizeof(f[i][c]));
-      if (marks != nullptr) mark[i] = marks[32 * i + r - back];
+        __builtin_memcpy(&f[i][c], b + (from[c] + uint32_t((ROWS * i - back) * stride)), sizeof(f[i][c]));
+      if (marks != nullptr) mark[i] = marks[ROWS * i + r - back];
     }
   }
   __device__ __forceinline__ void put(T *tile, int rows, bool marked) const {
@@ -154,21 +154,21 @@ struct Stage {
 #pragma unroll
       for (int i = 0; i < RB; ++i)
 #pragma unroll
-        for (int c = 0; c < CB; ++c) __builtin_memcpy(tile + to[c] + 32 * i * Tl::LD, &f[i][c], sizeof(f[i][c]));
+        for (int c = 0; c < CB; ++c) __builtin_memcpy(tile + to[c] + ROWS * i * Tl::LD, &f[i][c], sizeof(f[i][c]));
     } else {
 #pragma unroll
       for (int i = 0; i < RB; ++i) {
-        const bool out = 32 * i + r >= rows || (marked && mark[i] == -INFINITY);
+        const bool out = ROWS * i + r >= rows || (marked && mark[i] == -INFINITY);
 #pragma unroll
         for (int c = 0; c < CB; ++c) {
           const FragOf<T> g = out ? zero_frag<T>() : f[i][c];
-          __builtin_memcpy(tile + to[c] + 32 * i * Tl::LD, &g, sizeof(g));
+          __builtin_memcpy(tile + to[c] + ROWS * i * Tl::LD, &g, sizeof(g));
         }
       }
     }
   }
   static __device__ __forceinline__ void clear(T *tile) {
-    for (int u = threadIdx.x; u < YT * Tl::UPR; u += kBlock)
+    for (int u = threadIdx.x; u < YT * Tl::UPR; u += BLOCK)
       *reinterpret_cast<FragOf<T> *>(tile + u / Tl::UPR * Tl::LD + u % Tl::UPR * E) = zero_frag<T>();
   }
 };
@@ -201,7 +201,8 @@ __device__ __forceinline__ float pair_max(float v) {
   auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
 }
-__device__ __forceinline__ float sum16(const f32x16 &p) {
+template <typename V>
+__device__ __forceinline__ float sum16(const V &p) {
   float a[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) a[i] = p[i] + p[i + 8];
@@ -211,7 +212,8 @@ __device__ __forceinline__ float sum16(const f32x16 &p) {
     for (int i = 0; i < d; ++i) a[i] += a[i + d];
   return a[0];
 }
-__device__ __forceinline__ float max16(const f32x16 &p) {
+template <typename V>
+__device__ __forceinline__ float max16(const V &p) {
   float a[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) a[i] = fmaxf(p[i], p[i + 8]);
@@ -221,13 +223,21 @@ __device__ __forceinline__ float max16(const f32x16 &p) {
     for (int i = 0; i < d; ++i) a[i] = fmaxf(a[i], a[i + d]);
   return a[0];
 }
-// Accumulator blocks times a factor, in place in the matrix unit's registers.
-// Written out because a rescale that seldom runs sits behind a branch, where
-// the compiler otherwise keeps the blocks in two places and moves all of them
-// on the path that does nothing (256 moves a block of 32 rows). The waits are a
-// matrix product's before its result is read and a write's before the next one.
-template <int NB>
+// Accumulator blocks times a factor. With one wave a SIMD (ALONE) they lie in
+// the matrix unit's own registers, and the factor is applied in place by hand:
+// behind a branch that is seldom taken the compiler otherwise keeps the blocks
+// in two places and moves all of them on the path that does nothing (256 moves
+// a step of 64 rows of 256 channels). The waits are a matrix product's before its
+// result is read and a write's before the next one.
+template <bool ALONE, int NB>
 __device__ __forceinline__ void scale_blocks(f32x16 (&o)[NB], float by) {
+  if constexpr (!ALONE) {
+#pragma unroll
+    for (int d = 0; d < NB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] *= by;
+    return;
+  }
   asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
 #pragma unroll
   for (int d = 0; d < NB; ++d)
@@ -249,7 +259,8 @@ __device__ __forceinline__ void scale_blocks(f32x16 (&o)[NB], float by) {
     }
   asm volatile("s_nop 15" ::: "memory");
 }
-__device__ __forceinline__ float abs_max16(const f32x16 &p) {   // (three operands an instruction)
+template <typename V>
+__device__ __forceinline__ float abs_max16(const V &p) {   // (three operands an instruction)
   float a = fabsf(p[0]);
 #pragma unroll
   for (int i = 1; i < 15; i += 2) a = fmaxf(fmaxf(a, fabsf(p[i])), fabsf(p[i + 1]));
@@ -257,19 +268,6 @@ __device__ __forceinline__ float abs_max16(const f32x16 &p) {   // (three operan
 }
 // 2^x by the hardware instruction (1 ulp; results under 2^-126 are 0).
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// f(0) .. f(N - 1) with constants for arguments.
-template <typename F, int... J>
-__device__ __forceinline__ void each(std::integer_sequence<int, J...>, F &&f) {
-  (f(std::integral_constant<int, J>{}), ...);
-}
-template <int N, typename F>
-__device__ __forceinline__ void each(F &&f) {
-  each(std::make_integer_sequence<int, N>{}, f);
-}
-// Between two chunks of a step: the compiler's scheduler moves nothing across,
-// so that a chunk's vector instructions stay beside its matrix instructions.
-__device__ __forceinline__ void chunk_end() { __builtin_amdgcn_sched_barrier(0); }
 
 // The problem as the kernels take it. Scores are to base 2: c <h, w> + cb bias.
 struct Problem {
@@ -301,7 +299,43 @@ struct Line {
   __device__ __forceinline__ int64_t begin(int64_t w) const { return w * units / groups; }
   __device__ __forceinline__ int64_t group_of(int64_t unit) const { return ((unit + 1) * groups - 1) / units; }
 };
-constexpr int kGroups = 256;   // workgroups of a launch: one a CU
+
+// How the work is cut: waves of a workgroup (32 outer rows each), steps of 32
+// inner rows a tile, workgroups of a launch (all resident) and waves a SIMD.
+// Two waves a SIMD: one's vector work and LDS reads run beside the other's
+// matrix instructions (one wave of 64 rows reads half as much from LDS and
+// took 5 to 12 % longer: 404 us and 360 for 768 x 570,074 x 172 bf16). 16-bit
+// types have them in one workgroup, so that a tile is read once for 256 rows;
+// fp32, whose matrix instructions take 16 times as long, in two of 128 rows,
+// which fill up ragged numbers of rows better. fp32 rows of more than 128
+// channels would spill in half the registers (450 us for 412).
+template <typename T, int DB>
+struct Plan {
+  static constexpr bool WIDE = sizeof(T) == 4 && DB >= 6;
+  static constexpr int WAVES = sizeof(T) == 4 ? 4 : 8, SUB = sizeof(T) == 4 && DB > 4 ? 1 : 2;
+  static constexpr int PER_SIMD = WIDE ? 1 : 2, GROUPS_PER_TWO = sizeof(T) == 4 && !WIDE ? 1 : 2;   // CUs of two
+  static constexpr int GROUPS = 512 / GROUPS_PER_TWO;
+};
+// Steps of a product along the channels that are left out where a row ends
+// before them (DB counts rows in 64 channels). fp32 alone: 100 channels of 128 270 -> 250 us;
+// in 16 bits the branch costs what the step does.
+template <typename T>
+constexpr int kTrim = sizeof(T) == 4 ? 64 / Mma32<T>::KS - 1 : 0;
+// f(a value of the element type, the row's blocks of 32 as a constant).
+template <typename F>
+auto pick_dim(int32_t dtype, int D, F &&f) {
+  auto dims = [&](auto t) {
+    switch ((D + 63) / 64) {
+      case 1: return f(t, std::integral_constant<int, 2>{});
+      case 2: return f(t, std::integral_constant<int, 4>{});
+      case 3: return f(t, std::integral_constant<int, 6>{});
+      default: return f(t, std::integral_constant<int, 8>{});
+    }
+  };
+  if (dtype == SGL_FP32) return dims(float{});
+  if (dtype == SGL_BF16) return dims(bf16_t{});
+  return dims(fp16_t{});
+}
 
 // ------------------------------------------------------------------ launches
 // Rows in the order that they are worked on: those with a target first.
@@ -312,13 +346,12 @@ struct Order {
   __device__ __forceinline__ int64_t row(int64_t at) const { return order != nullptr ? order[at] : at; }
   __device__ __forceinline__ int64_t count(int64_t N) const { return live != nullptr ? int64_t(*live) : N; }
 };
-// What a forward leaves for each piece (Line) of 32 wx rows and WY waves
-// along the table: its own maximum as used, its sum and, with a direction,
-// sum_v p_v w_v at that maximum.
+// What a forward leaves for each piece (Line) and wave along the table: its
+// own maximum as used, its sum and, with a direction, sum_v p_v w_v at that maximum.
 struct Partials {
   float *m, *l, *o;   // [pieces][wy][rows], the same, [pieces][wy][rows][dp]
   int64_t ytiles;
-  int rows, wy, dp;
+  int rows, wy, dp, groups;
 };
 int padded_dim(int D);
 Partials forward_shape(int32_t dtype, const Problem &p);   // (without its arrays)
@@ -345,7 +378,7 @@ struct RowCoef {
 };
 void route_targets(int32_t dtype, const Problem &p, int K, const int32_t *ids, const float *weight, int32_t *index,
                    int2 *entries, hipStream_t stream);
-int table_grad_block(int32_t dtype);    // candidates of a wave
+constexpr int kGradBlock = 32;   // candidates of a wave
 // fp32 elements of `part` at most (those of tiles that are not shared out are never touched).
 int64_t table_grad_part(int32_t dtype, const Problem &p);
 void table_grad(int32_t dtype, const Problem &p, const RowCoef &r, void *dtable, float *dbias, float *part,

@@ -8,12 +8,25 @@ namespace {
 using namespace sgl;
 using namespace sgl::cand;
 
-// Sum over the wave, the same in every lane.
-__device__ __forceinline__ float wave_sum(float v) { return wave_reduce_sum(v); }
+// Sum, maximum over the wave, the same in every lane: rows of 16 lanes rotated
+// by 8, 4, 2 and 1, then rows and halves of the wave swapped.
+template <int CTRL>
+__device__ __forceinline__ float turned(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v += turned<0x128>(v);
+  v += turned<0x124>(v);
+  v += turned<0x122>(v);
+  v += turned<0x121>(v);
+  return attn::groups_sum(v);
+}
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int d = kWave / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, kWave));
-  return v;
+  v = fmaxf(v, turned<0x128>(v));
+  v = fmaxf(v, turned<0x124>(v));
+  v = fmaxf(v, turned<0x122>(v));
+  v = fmaxf(v, turned<0x121>(v));
+  return attn::groups_max(v);
 }
 
 // ------------------------------------------------------------------ a teacher's distribution
@@ -98,6 +111,7 @@ __global__ __launch_bounds__(kOrderRows) void k_order(const int64_t *target, int
   const int64_t n0 = int64_t(blockIdx.x) * kOrderRows, n = n0 + tid;
   auto has = [&](int64_t at) { return uint64_t(target[at]) < uint64_t(V); };
   int count = 0, total = 0;
+#pragma unroll 8
   for (int64_t i = tid; i < N; i += kOrderRows) {
     const int on = has(i) ? 1 : 0;
     total += on;
@@ -125,7 +139,6 @@ struct FinishArgs {
   float *loss, *stat, *dir;   // stat: [2][N] the maximum and 1 / sum (0: no gradient)
   int32_t *ids_out;           // of `target`
 };
-constexpr int kBatch = 8;     // targets whose rows are on their way together
 constexpr int kAhead = 4;     // partials of a lane
 
 // A lane's four columns of a row of D: 4 lane on, the last lane's the row's
@@ -142,11 +155,11 @@ struct Cols {
   }
 };
 
-// W waves a row, 4 / W rows a workgroup.
-template <typename T, int W, bool DIR>
+// W waves a row, 4 / W rows a workgroup; targets in batches of BATCH.
+template <typename T, int W, int BATCH, bool DIR>
 __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
-  __shared__ float parts[kWaves][DIR ? kMaxDim : 1];
-  __shared__ float sums[kWaves][3];
+  __shared__ float parts[kWaves][DIR && W > 1 ? kMaxDim : 1];
+  __shared__ float sums[2][kWaves][3];
   const Problem &p = a.p;
   const int lane = threadIdx.x & 63, wave = attn::wave_index(), w = wave % W;
   const int64_t at = int64_t(blockIdx.x) * (kWaves / W) + wave / W;
@@ -158,53 +171,32 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
   T raw[4];
   load_n(raw, static_cast<const T *>(p.h) + row * p.hs + c.d);
 
-  // the row's partials: the waves along the table of consecutive pieces
+  // the row's partials: the waves along the table of consecutive pieces, shared by the row's waves
   int n = 0;
   int64_t first = 0;
   if (pos < live_rows) {
-    const Line line((live_rows + a.in.rows - 1) / a.in.rows, a.in.ytiles, kGroups);
+    const Line line((live_rows + a.in.rows - 1) / a.in.rows, a.in.ytiles, a.in.groups);
     const int64_t xt = pos / a.in.rows, w0 = line.group_of(xt * line.inner);
     n = int(line.group_of((xt + 1) * line.inner - 1) - w0 + 1) * a.in.wy;
     first = (w0 + xt) * a.in.wy * a.in.rows + (pos - xt * a.in.rows);
   }
   const float *pm = a.in.m + first, *pl = a.in.l + first;
-  // the first of them at once: their loads, the row's and the targets' overlap
+  // (the first of them at once: their loads, the row's and the targets' overlap)
   float m[kAhead], s[kAhead];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
-    const int k = lane + i * kWave;
+    const int k = w * kWave + lane + i * (W * kWave);
     m[i] = k < n ? pm[k * a.in.rows] : -INFINITY;
     s[i] = k < n ? pl[k * a.in.rows] : 0.f;
   }
-
-  // the targets: sum of -q s, of q, of q w
-  float x[4], tw[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    x[j] = c.own[j] ? float(raw[j]) : 0.f;
-    tw[j] = 0.f;
-  }
-  float mx = -INFINITY, l = 0.f;
-  auto join = [&]() {
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) mx = fmaxf(mx, m[i]);
-    for (int k = lane + kAhead * kWave; k < n; k += kWave) mx = fmaxf(mx, pm[k * a.in.rows]);
-    mx = wave_max(mx);
-    // (a piece without a live candidate has sum 0)
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) l += m[i] == -INFINITY ? s[i] : s[i] * exp2_fast(m[i] - mx);
-    for (int k = lane + kAhead * kWave; k < n; k += kWave) {
-      const float y = pm[k * a.in.rows], z = pl[k * a.in.rows];
-      l += y == -INFINITY ? z : z * exp2_fast(y - mx);
-    }
-    l = wave_sum(l);
-  };
-  float far = 0.f, want = 0.f, out = 0.f;
-  bool joined = false;
-  for (int k0 = w * kBatch; k0 < a.K; k0 += W * kBatch) {
-    int id = -1;
-    float q = 0.f, b = 0.f;
-    if (lane < kBatch && k0 + lane < a.K) {
+  // the first targets' rows
+  int id = -1;
+  float q = 0.f, b = 0.f, want = 0.f, out = 0.f;
+  T y[BATCH][4];
+  auto ask = [&](int k0) {
+    id = -1;
+    q = b = 0.f;
+    if (lane < BATCH && k0 + lane < a.K) {
       if (a.target != nullptr) {
         id = uint64_t(target) < uint64_t(p.V) ? int(target) : -1;
         q = 1.f;
@@ -220,44 +212,79 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
       out = 1.f;
       id = -1;
     }
-    T y[kBatch][4];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
+    for (int i = 0; i < BATCH; ++i) {
       const int v = __builtin_amdgcn_readlane(id, i);
       if (v >= 0) load_n(y[i], static_cast<const T *>(p.table) + int64_t(v) * p.ts + c.d);
       else
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[i][j] = T(0.f);
     }
-    if (!joined) join(), joined = true;
-    float dot[kBatch];
+  };
+  int k0 = w * BATCH;
+  ask(k0);
+
+  // the maximum and the sum of all partials (a piece without a live candidate has sum 0)
+  float mx = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
+  for (int i = 0; i < kAhead; ++i) mx = fmaxf(mx, m[i]);
+  for (int k = w * kWave + lane + kAhead * W * kWave; k < n; k += W * kWave) mx = fmaxf(mx, pm[k * a.in.rows]);
+  mx = wave_max(mx);
+  auto at_max = [&](float y, float z) { return y == -INFINITY ? z : z * exp2_fast(y - mx); };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) l += at_max(m[i], s[i]);
+  for (int k = w * kWave + lane + kAhead * W * kWave; k < n; k += W * kWave)
+    l += at_max(pm[k * a.in.rows], pl[k * a.in.rows]);
+  l = wave_sum(l);
+  if constexpr (W > 1) {
+    if (lane == 0) sums[0][wave][0] = mx, sums[0][wave][1] = l;
+    __syncthreads();
+    mx = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) mx = fmaxf(mx, sums[0][i][0]);
+#pragma unroll
+    for (int i = 0; i < W; ++i) l += at_max(sums[0][i][0], sums[0][i][1]);
+  }
+
+  // the targets: sum of q (mx - s), of q, of q w
+  float x[4], tw[4], far = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[j] = c.own[j] ? float(raw[j]) : 0.f;
+    tw[j] = 0.f;
+  }
+  while (true) {
+    float dot[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
       const float qi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(q), i));
       dot[i] = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float z = c.own[j] ? float(y[i][j]) : 0.f;   // (times a row's zeros: not of another lane's NaN)
+        const float z = c.own[j] ? float(y[i][j]) : 0.f;   // (not 0 times a neighbour's NaN)
         dot[i] = fmaf(x[j], z, dot[i]);
         tw[j] = fmaf(qi, float(y[i][j]), tw[j]);
       }
     }
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) dot[i] = wave_sum(dot[i]);
+    for (int i = 0; i < BATCH; ++i) dot[i] = wave_sum(dot[i]);
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i)
+    for (int i = 0; i < BATCH; ++i)
       if (lane == i && id >= 0) far += q * (mx - fmaf(dot[i], p.c, b));
+    k0 += W * BATCH;
+    if (k0 >= a.K) break;
+    ask(k0);
   }
-  if (!joined) join();
   far = wave_sum(far);
   want = wave_sum(want);
   out = wave_max(out);
   if constexpr (W > 1) {
-    if (lane == 0) sums[wave][0] = far, sums[wave][1] = want, sums[wave][2] = out;
+    if (lane == 0) sums[1][wave][0] = far, sums[1][wave][1] = want, sums[1][wave][2] = out;
     __syncthreads();
     far = want = out = 0.f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) far += sums[i][0], want += sums[i][1], out = fmaxf(out, sums[i][2]);
+    for (int i = 0; i < W; ++i) far += sums[1][i][0], want += sums[1][i][1], out = fmaxf(out, sums[1][i][2]);
   }
   const bool wanted = !(want == 0.f);   // (NaN: a row that its teacher spoils)
   const bool spoilt = mx == -INFINITY && !(l == 0.f);   // (no score but NaN)
@@ -283,13 +310,13 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
     if (a.ids_out != nullptr) a.ids_out[row] = uint64_t(target) < uint64_t(p.V) ? int32_t(target) : -1;
   }
   if constexpr (DIR) {
+    if (W == 1 && !grad) return;   // (not read)
     float o[4] = {};
     const float *src = a.in.o + first * a.in.dp + c.d;
     const int64_t step = int64_t(a.in.rows) * a.in.dp;
 #pragma unroll 4
     for (int k = w; k < n; k += W) {
-      const float y = pm[k * a.in.rows];
-      const float f = y == -INFINITY ? 1.f : exp2_fast(y - mx);
+      const float f = at_max(pm[k * a.in.rows], 1.f);
       float z[4];
       load_n(z, src + k * step);
 #pragma unroll
@@ -308,11 +335,7 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) e[j] += parts[i][4 * lane + j];
     }
-    if (here && c.here) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) e[j] = grad ? e[j] : 0.f;
-      store_n(a.dir + row * p.D + c.d, e);
-    }
+    if (here && c.here && grad) store_n(a.dir + row * p.D + c.d, e);
   }
 }
 
@@ -403,7 +426,7 @@ int make_problem(const sgl_candidates *c, Problem &p) {
 Partials carve_forward(void *ws, int32_t dtype, const Problem &p, bool dir, size_t *bytes) {
   Carver c(ws);
   Partials out = forward_shape(dtype, p);
-  const size_t pieces = size_t((p.N + out.rows - 1) / out.rows + kGroups) * size_t(out.wy) * size_t(out.rows);
+  const size_t pieces = size_t((p.N + out.rows - 1) / out.rows + out.groups) * size_t(out.wy) * size_t(out.rows);
   out.m = c.take<float>(pieces);
   out.l = c.take<float>(pieces);
   out.o = dir ? c.take<float>(pieces * size_t(out.dp)) : nullptr;
@@ -451,8 +474,7 @@ Grad carve_backward(void *ws, int32_t dtype, const Problem &p, int K, bool teach
   const size_t tiles = size_t((p.N + im.rows - 1) / im.rows);
   g.image = c.take<char>(tiles * size_t(im.bytes));
   if (teacher) {
-    const int vb = table_grad_block(dtype);
-    g.index = c.take<int32_t>(tiles * size_t((p.V + vb - 1) / vb + 1));
+    g.index = c.take<int32_t>(tiles * size_t((p.V + kGradBlock - 1) / kGradBlock + 1));
     g.entries = c.take<int2>(tiles * size_t(im.rows) * size_t(K));
   }
   g.part = c.take<float>(size_t(table_grad_part(dtype, p)));
@@ -468,16 +490,17 @@ int check_room(const char *what, const void *room, size_t bytes, size_t need) {
 
 template <typename T>
 void finish(const FinishArgs &a, hipStream_t stream) {
-  // four waves a row where they have pieces or targets enough to share
+  // four waves a row where they have partials or targets enough to share
   const bool wide = a.K >= 16 || a.in.wy > 1 || a.p.N <= 16 * a.in.rows;
   const dim3 grid(unsigned(wide ? a.p.N : (a.p.N + kWaves - 1) / kWaves));
-  if (a.dir != nullptr) {
-    if (wide) launch(&k_finish<T, kWaves, true>, grid, dim3(kBlock), 0, stream, a);
-    else launch(&k_finish<T, 1, true>, grid, dim3(kBlock), 0, stream, a);
-  } else {
-    if (wide) launch(&k_finish<T, kWaves, false>, grid, dim3(kBlock), 0, stream, a);
-    else launch(&k_finish<T, 1, false>, grid, dim3(kBlock), 0, stream, a);
-  }
+  auto go = [&](auto *k) { launch(k, grid, dim3(kBlock), 0, stream, a); };
+  auto pick = [&](auto batch) {
+    constexpr int B = batch.value;
+    if (a.dir != nullptr) wide ? go(&k_finish<T, kWaves, B, true>) : go(&k_finish<T, 1, B, true>);
+    else wide ? go(&k_finish<T, kWaves, B, false>) : go(&k_finish<T, 1, B, false>);
+  };
+  if (a.K == 1) pick(std::integral_constant<int, 1>{});
+  else pick(std::integral_constant<int, 8>{});
 }
 
 }  // namespace
@@ -564,8 +587,7 @@ extern "C" int sgl_candidates_backward(const sgl_candidates *problem, int32_t k,
   if (dtable != nullptr) {
     RowCoef r{w.image, o.live, w.index, w.entries, 0, k};
     if (teacher != 0) {
-      const int vb = table_grad_block(problem->dtype);
-      r.vblocks = (p.V + vb - 1) / vb;
+      r.vblocks = (p.V + kGradBlock - 1) / kGradBlock;
       route_targets(problem->dtype, p, k, kept.ids, kept.weight, w.index, w.entries, stream);
     }
     table_grad(problem->dtype, p, r, dtable, dbias, w.part, stream);

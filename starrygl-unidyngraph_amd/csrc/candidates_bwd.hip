@@ -26,62 +26,59 @@ __device__ __forceinline__ float half_scale(float most) {   // (1 for what is no
   return e >= 255 ? 1.f : __uint_as_float(uint32_t(min(max(258 - e, 1), 254)) << 23);
 }
 
-// Candidates of a workgroup, rows of a tile (32 where more of them on their way
-// would not fit in the registers).
-template <typename T>
-constexpr int kXTile = sizeof(T) == 4 ? 128 : 256;
-template <typename T, int DB>
-constexpr int kYTile = sizeof(T) == 4 || DB >= 6 ? 32 : 64;
-
+// A tile in memory and in LDS (Image): steps of 32 rows.
 template <typename T, int DB>
 struct Tiles {
-  static constexpr int YT = kYTile<T, DB>, LD = Tile32<T, 32 * DB>::LD;
+  static constexpr int SUB = sizeof(T) == 4 || DB == 8 ? 1 : 2;
+  static constexpr int YT = 32 * SUB, LD = Tile32<T, 32 * DB>::LD;
   static constexpr int ROWS = YT * LD * int(sizeof(T)), BYTES = ROWS + 16 * YT;
+  static constexpr int XT = 32 * Plan<T, DB>::WAVES;   // candidates of a workgroup
+  static constexpr int QL = 32 + 4;
   static_assert(BYTES % 1024 == 0, "whole loads of a wave");
 };
 
-// XB blocks of 32 candidates a wave, four waves along the candidates.
-template <typename T, int DB, int XB>
-__global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
+// A wave has 32 candidates.
+template <typename T, int DB, int WAVES, int PER_SIMD>
+__global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) {
   using M = Mma32<T>;
-  constexpr int KS = M::KS, DP = 32 * DB, NK = DP / KS;
-  using Tl = Tile32<T, DP>;
-  constexpr int YT = kYTile<T, DB>, YS = YT / 32, XT = 32 * XB * kWaves, QL = 32 + 4;
-  constexpr bool HALF = std::is_same_v<T, fp16_t>;
-  constexpr int WV = 32 * XB;   // candidates of a wave
-  extern __shared__ __align__(16) char lds[];
   using Im = Tiles<T, DB>;
-  // [XT][QL]: what 32 rows want of the candidates; zero between uses. A wave writes, reads and clears
-  // its own candidates' part.
+  constexpr int BLOCK = 64 * WAVES;
+  constexpr int KS = M::KS, DP = 32 * DB, NK = DP / KS, TRIM = kTrim<T>, YT = Im::YT, XT = Im::XT, QL = Im::QL;
+  using Tl = Tile32<T, DP>;
+  constexpr bool HALF = std::is_same_v<T, fp16_t>;
+  extern __shared__ __align__(16) char lds[];
+  // [XT][QL]: what 32 rows want of the candidates; zero between uses. A wave writes, reads and clears its
+  // own candidates' part.
   float *q_all = reinterpret_cast<float *>(lds + 2 * Im::BYTES);
 
   const Problem &p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, col = lane & 31;
   const int wave = attn::wave_index();
-  float *q = q_all + wave * WV * QL;
+  float *q = q_all + wave * 32 * QL;
   const int64_t N = a.r.live != nullptr ? int64_t(*a.r.live) : p.N;
-  const Line line((p.V + XT - 1) / XT, max((N + YT - 1) / YT, int64_t(1)), kGroups);
+  const Line line((p.V + XT - 1) / XT, max((N + YT - 1) / YT, int64_t(1)), Plan<T, DB>::GROUPS);
   const int w = blockIdx.x;
   if (w >= line.groups) return;
   const int64_t u1 = line.begin(w + 1);
 
-  constexpr int NL = (Im::BYTES + 16 * kBlock - 1) / (16 * kBlock);
+  constexpr int NL = (Im::BYTES + 16 * BLOCK - 1) / (16 * BLOCK);
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   u32x4 next[NL];
   int ne0 = 0, ne1 = 0;
+  auto loads = [&](int i) { return (i + 1) * 16 * BLOCK <= Im::BYTES || (i * WAVES + wave) * 1024 < Im::BYTES; };
   auto fetch = [&](int t, int xt) {
     const u32x4 *src = reinterpret_cast<const u32x4 *>(a.r.image + int64_t(t) * Im::BYTES);
 #pragma unroll
     for (int i = 0; i < NL; ++i)
-      if ((i + 1) * 16 * kBlock <= Im::BYTES || (i * kWaves + wave) * 1024 < Im::BYTES) next[i] = src[i * kBlock + tid];
+      if (loads(i)) next[i] = src[i * BLOCK + tid];
     if (a.r.index != nullptr) {
-      const int64_t vb = int64_t(xt) * kWaves + wave;
+      const int64_t vb = int64_t(xt) * WAVES + wave;
       const int32_t *at = a.r.index + int64_t(t) * (a.r.vblocks + 1) + min(vb, a.r.vblocks - 1);
       ne0 = attn::scalar_load(at);
       ne1 = vb < a.r.vblocks ? attn::scalar_load(at + 1) : ne0;
     }
   };
-  for (int i = tid; i < XT * QL / 4; i += kBlock) reinterpret_cast<f32x4 *>(q_all)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = tid; i < XT * QL / 4; i += BLOCK) reinterpret_cast<f32x4 *>(q_all)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   int64_t u = line.begin(w);
   int xt = int(u / line.inner), t = int(u - int64_t(xt) * line.inner), buf = 0;
   fetch(t, xt);
@@ -89,172 +86,129 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
 
 #pragma unroll 1
   for (; u < u1; ++xt) {   // an outer tile's piece
-  FragOf<T> xf[XB][NK];
-  const int D = fresh(p.D);
-  float b2[XB], db[XB], sc[XB];
-  const int64_t x0 = int64_t(xt) * XT + wave * WV + col;
-#pragma unroll
-  for (int xb = 0; xb < XB; ++xb) {
-    const int64_t x = min(x0 + 32 * xb, p.V - 1);
-    b2[xb] = p.bias != nullptr ? bias2(p, x) : 0.f;
-    load_outer<T>(xf[xb], static_cast<const T *>(p.table) + x * p.ts, b2[xb] == -INFINITY, D);
-    db[xb] = 0.f;
-    sc[xb] = kFirstScale;
-  }
-  f32x16 o[XB][DB];
-#pragma unroll
-  for (int xb = 0; xb < XB; ++xb)
+    FragOf<T> xf[NK];
+    const int D = fresh(p.D);
+    const int64_t x = int64_t(xt) * XT + wave * 32 + col, xr = min(x, p.V - 1);
+    const float b2 = p.bias != nullptr ? bias2(p, xr) : 0.f;
+    load_outer<T>(xf, static_cast<const T *>(p.table) + xr * p.ts, b2 == -INFINITY, D);
+    float db = 0.f, sc = kFirstScale;
+    f32x16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[xb][d][r] = 0.f;
-  const int first = t, end = int(min(int64_t(line.inner), t + (u1 - u)));
-  u += end - t;
+      for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    const int first = t, end = int(min(int64_t(line.inner), t + (u1 - u)));
+    u += end - t;
 #pragma unroll 1
-  for (; t < end; ++t) {
-    char *image = lds + buf * Im::BYTES;
-    const T *tile = reinterpret_cast<const T *>(image);
-    const float *cf = reinterpret_cast<const float *>(image + Im::ROWS);
-    buf ^= 1;
+    for (; t < end; ++t) {
+      char *image = lds + buf * Im::BYTES;
+      const T *tile = reinterpret_cast<const T *>(image);
+      const float *cf = reinterpret_cast<const float *>(image + Im::ROWS);
+      buf ^= 1;
 #pragma unroll
-    for (int i = 0; i < NL; ++i)
-      if ((i + 1) * 16 * kBlock <= Im::BYTES || (i * kWaves + wave) * 1024 < Im::BYTES)
-        reinterpret_cast<u32x4 *>(image)[i * kBlock + tid] = next[i];
-    const int e0 = ne0, e1 = ne1;
-    const int2 *entries = a.r.entries + int64_t(t) * YT * a.r.K;
-    __syncthreads();
-    // what the tile's rows want of the wave's candidates: a row has a candidate once, so each place once
-    const int id = a.r.index == nullptr && lane < YT ? reinterpret_cast<const int *>(cf)[3 * YT + lane] : -1;
-    const int mine = id - (xt * XT + wave * WV);
-    const bool one = id >= 0 && uint32_t(mine) < uint32_t(WV);
-    const bool wanted = __any(one) || e0 < e1;
-    if (t + 1 < end || u < u1) fetch(t + 1 < end ? t + 1 : 0, t + 1 < end ? xt : xt + 1);
+      for (int i = 0; i < NL; ++i)
+        if (loads(i)) reinterpret_cast<u32x4 *>(image)[i * BLOCK + tid] = next[i];
+      const int e0 = ne0, e1 = ne1;
+      const int2 *entries = a.r.entries + int64_t(t) * YT * a.r.K;
+      __syncthreads();
+      // what the tile's rows want of the wave's candidates: a row has a candidate once, so each place once
+      const int id = a.r.index == nullptr && lane < YT ? reinterpret_cast<const int *>(cf)[3 * YT + lane] : -1;
+      const int mine = id - (xt * XT + wave * 32);
+      const bool one = id >= 0 && uint32_t(mine) < 32u;
+      const bool wanted = __any(one) || e0 < e1;
+      if (t + 1 < end || u < u1) fetch(t + 1 < end ? t + 1 : 0, t + 1 < end ? xt : xt + 1);
 #pragma unroll 1
-    for (int ys = 0; ys < YS; ++ys) {
-      const int row0 = ys * 32;
-      if (wanted) {
-        if (one && (lane >> 5) == ys) q[mine * QL + (lane & 31)] = 1.f;
-        for (int e = e0 + lane; e < e1; e += kWave) {
-          const int2 x = entries[e];
-          if (((x.x >> 5) & 1) == ys) q[(x.x >> 6) * QL + (x.x & 31)] = __int_as_float(x.y);
+      for (int ys = 0; ys < Im::SUB; ++ys) {
+        const int row0 = ys * 32;
+        if (wanted) {
+          if (one && (lane >> 5) == ys) q[mine * QL + (lane & 31)] = 1.f;
+          for (int k = e0 + lane; k < e1; k += kWave) {
+            const int2 e = entries[k];
+            if (((e.x >> 5) & 1) == ys) q[(e.x >> 6) * QL + (e.x & 31)] = __int_as_float(e.y);
+          }
+          attn::wave_sync();
         }
-        attn::wave_sync();
-      }
-      f32x16 s[XB];
+        f32x16 s;
 #pragma unroll
-      for (int xb = 0; xb < XB; ++xb)
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[xb][r] = 0.f;
-#pragma unroll
-      for (int k = 0; k < NK; ++k) {
-        const FragOf<T> f = Tl::frag(tile, row0, k * KS);
-#pragma unroll
-        for (int xb = 0; xb < XB; ++xb) s[xb] = M::mma(f, xf[xb][k], s[xb]);
-      }
-      auto coefficients = [&]() {
+        for (int k = 0; k < NK; ++k)
+          if (k < NK - TRIM || k * KS < p.D) s = M::mma(Tl::frag(tile, row0, k * KS), xf[k], s);
+        float c[16];   // (numbers of their own: as the product's block they would be moved between the register files)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float nm[4], gl[4];
           __builtin_memcpy(nm, cf + row0 + 8 * i + 4 * h, sizeof(nm));
           __builtin_memcpy(gl, cf + YT + row0 + 8 * i + 4 * h, sizeof(gl));
 #pragma unroll
-          for (int xb = 0; xb < XB; ++xb)
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-              s[xb][4 * i + v] = exp2_fast(fmaf(s[xb][4 * i + v], p.c, b2[xb]) + nm[v]) * gl[v];
+          for (int v = 0; v < 4; ++v) c[4 * i + v] = exp2_fast(fmaf(s[4 * i + v], p.c, b2) + nm[v]) * gl[v];
         }
-      };
-      auto targets = [&]() {
+        if (wanted) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float gq[4];
-          __builtin_memcpy(gq, cf + 2 * YT + row0 + 8 * i + 4 * h, sizeof(gq));
+          for (int i = 0; i < 4; ++i) {
+            float gq[4], y[4];
+            __builtin_memcpy(gq, cf + 2 * YT + row0 + 8 * i + 4 * h, sizeof(gq));
+            __builtin_memcpy(y, q + col * QL + 8 * i + 4 * h, sizeof(y));
 #pragma unroll
-          for (int xb = 0; xb < XB; ++xb) {
-            float w[4];
-            __builtin_memcpy(w, q + (32 * xb + col) * QL + 8 * i + 4 * h, sizeof(w));
-#pragma unroll
-            for (int v = 0; v < 4; ++v) s[xb][4 * i + v] = fmaf(-gq[v], w[v], s[xb][4 * i + v]);
+            for (int v = 0; v < 4; ++v) c[4 * i + v] = fmaf(-gq[v], y[v], c[4 * i + v]);
+          }
+          attn::wave_sync();
+          if (one && (lane >> 5) == ys) q[mine * QL + (lane & 31)] = 0.f;
+          for (int k = e0 + lane; k < e1; k += kWave) {
+            const int e = entries[k].x;
+            if (((e >> 5) & 1) == ys) q[(e >> 6) * QL + (e & 31)] = 0.f;
           }
         }
-        attn::wave_sync();
-        if (one && (lane >> 5) == ys) q[mine * QL + (lane & 31)] = 0.f;
-        for (int e = e0 + lane; e < e1; e += kWave) {
-          const int x = entries[e].x;
-          if (((x >> 5) & 1) == ys) q[(x >> 6) * QL + (x & 31)] = 0.f;
-        }
-      };
-      auto product = [&]() {
         if constexpr (HALF) {
-#pragma unroll
-          for (int xb = 0; xb < XB; ++xb) {
-            const float most = pair_max(abs_max16(s[xb]));
-            const bool over = most * sc[xb] > kMostHalf;
-            if (__any(over)) {
-              const float to = over ? half_scale(most) : sc[xb];
-              scale_blocks(o[xb], to / sc[xb]);
-              sc[xb] = to;
-            }
+          const float most = pair_max(abs_max16(c));
+          const bool over = most * sc > kMostHalf;
+          if (__any(over)) {
+            const float to = over ? half_scale(most) : sc;
+            scale_blocks<PER_SIMD == 1>(o, to / sc);
+            sc = to;
           }
         }
 #pragma unroll
         for (int st = 0; st < 32 / KS; ++st) {
-          FragOf<T> pf[XB];
+          const FragOf<T> pf = frag_of16<T>(c, st, HALF ? sc : 1.f);
 #pragma unroll
-          for (int xb = 0; xb < XB; ++xb) pf[xb] = frag_of16<T>(s[xb], st, HALF ? sc[xb] : 1.f);
-#pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            const FragOf<T> f = Tl::frag_t(tile, 32 * d, row0, st);
-#pragma unroll
-            for (int xb = 0; xb < XB; ++xb) o[xb][d] = M::mma(f, pf[xb], o[xb][d]);
-          }
+          for (int d = 0; d < DB; ++d) o[d] = M::mma(Tl::frag_t(tile, 32 * d, row0, st), pf, o[d]);
         }
-      };
-      coefficients();
-      if (wanted) targets();
-      product();
-      if (a.dbias != nullptr) {
-#pragma unroll
-        for (int xb = 0; xb < XB; ++xb) db[xb] += sum16(s[xb]);
+        if (a.dbias != nullptr) db += sum16(c);
       }
     }
-  }
 
-  const int width = fresh(p.D);
-  const bool whole = first == 0 && end == line.inner;
+    const int width = fresh(p.D);
+    const bool whole = first == 0 && end == line.inner;
+    const float sum = pair_sum(db), by = HALF ? p.scale / sc : p.scale;
+    if (x < p.V) {
+      if (!whole) {
+        float *row = a.part + (int64_t(w + xt) * XT + wave * 32 + col) * (DP + 4);
 #pragma unroll
-  for (int xb = 0; xb < XB; ++xb) {
-    const int64_t x = x0 + 32 * xb;
-    const float sum = pair_sum(db[xb]);
-    if (x >= p.V) continue;
-    const float by = HALF ? p.scale / sc[xb] : p.scale;
-    if (!whole) {
-      float *row = a.part + (int64_t(w + xt) * XT + wave * WV + 32 * xb + col) * (DP + 4);
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
+          for (int i = 0; i < 4; ++i) {
+            float y[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float y[4];
+            for (int v = 0; v < 4; ++v) y[v] = o[d][4 * i + v] * by;
+            store_n(row + 32 * d + 8 * i + 4 * h, y);
+          }
+        if (h == 0) row[DP] = sum;
+      } else {
+        T *row = static_cast<T *>(a.dtable) + x * width;
 #pragma unroll
-          for (int v = 0; v < 4; ++v) y[v] = o[xb][d][4 * i + v] * by;
-          store_n(row + 32 * d + 8 * i + 4 * h, y);
-        }
-      if (h == 0) row[DP] = sum;
-    } else {
-      T *row = static_cast<T *>(a.dtable) + x * width;
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
+          for (int i = 0; i < 4; ++i) {
+            f32x4 y;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f32x4 y;
-#pragma unroll
-          for (int v = 0; v < 4; ++v) y[v] = o[xb][d][4 * i + v] * by;
-          attn::store4<T>(row, 32 * d + 8 * i + 4 * h, width, y);
-        }
-      if (a.dbias != nullptr && h == 0) a.dbias[x] = sum;
+            for (int v = 0; v < 4; ++v) y[v] = o[d][4 * i + v] * by;
+            attn::store4<T>(row, 32 * d + 8 * i + 4 * h, width, y);
+          }
+        if (a.dbias != nullptr && h == 0) a.dbias[x] = sum;
+      }
     }
-  }
-  t = 0;
+    t = 0;
   }
 }
 
@@ -263,10 +217,10 @@ __global__ __launch_bounds__(kBlock, 1) void k_table_grad(BwdArgs a) {
 // b / kJoin + 1 begins inside of, unless an earlier one does.
 constexpr int kJoin = 8;
 template <typename T>
-__global__ __launch_bounds__(kBlock) void k_join_grad(BwdArgs a, int xtile, int ytile, int dp) {
+__global__ __launch_bounds__(kBlock) void k_join_grad(BwdArgs a, int xtile, int ytile, int dp, int groups) {
   const Problem &p = a.p;
   const int64_t N = a.r.live != nullptr ? int64_t(*a.r.live) : p.N;
-  const Line line((p.V + xtile - 1) / xtile, max((N + ytile - 1) / ytile, int64_t(1)), kGroups);
+  const Line line((p.V + xtile - 1) / xtile, max((N + ytile - 1) / ytile, int64_t(1)), groups);
   const int w = blockIdx.x / kJoin + 1, part = blockIdx.x % kJoin;
   if (w >= line.groups) return;
   const int64_t u = line.begin(w), xt = u / line.inner;
@@ -354,27 +308,17 @@ __global__ __launch_bounds__(kRouteBlock) void k_route(RouteArgs a) {
 
 template <typename T, int DB>
 void run(const BwdArgs &a, hipStream_t stream) {
-  constexpr int XB = sizeof(T) == 4 ? 1 : 2;
-  constexpr int YT = kYTile<T, DB>, XT = kXTile<T>;
-  static_assert(XT == 32 * XB * kWaves, "");
-  constexpr size_t bytes = size_t(2) * Tiles<T, DB>::BYTES + sizeof(float) * XT * 36;
-  static_assert(bytes <= 160 * 1024, "LDS of a CU");
-  auto *k = &k_table_grad<T, DB, XB>;
+  using P = Plan<T, DB>;
+  using Im = Tiles<T, DB>;
+  constexpr size_t bytes = size_t(2) * Im::BYTES + sizeof(float) * Im::XT * Im::QL;
+  static_assert(bytes <= 160 * 1024 * P::GROUPS_PER_TWO / 2, "LDS of a CU");
+  auto *k = &k_table_grad<T, DB, P::WAVES, P::PER_SIMD>;
   (void)ensure_dynamic_lds(reinterpret_cast<const void *>(k), bytes);
-  const Line line((a.p.V + XT - 1) / XT, (a.p.N + YT - 1) / YT, kGroups);
-  launch(k, dim3(unsigned(line.groups)), dim3(kBlock), bytes, stream, a);
+  const Line line((a.p.V + Im::XT - 1) / Im::XT, (a.p.N + Im::YT - 1) / Im::YT, P::GROUPS);
+  launch(k, dim3(unsigned(line.groups)), dim3(64 * P::WAVES), bytes, stream, a);
   if (line.groups > 1)
-    launch(&k_join_grad<T>, dim3(unsigned(line.groups - 1) * kJoin), dim3(kBlock), 0, stream, a, XT, YT, 32 * DB);
-}
-template <typename T>
-void pick(const Problem &p, const RowCoef &r, void *dtable, float *dbias, float *part, hipStream_t stream) {
-  const BwdArgs a{p, r, dtable, dbias, part};
-  switch (padded_dim(p.D)) {
-    case 64: return run<T, 2>(a, stream);
-    case 128: return run<T, 4>(a, stream);
-    case 192: return run<T, 6>(a, stream);
-    default: return run<T, 8>(a, stream);
-  }
+    launch(&k_join_grad<T>, dim3(unsigned(line.groups - 1) * kJoin), dim3(kBlock), 0, stream, a, int(Im::XT), int(Im::YT),
+           32 * DB, int(P::GROUPS));
 }
 
 }  // namespace
@@ -382,35 +326,31 @@ void pick(const Problem &p, const RowCoef &r, void *dtable, float *dbias, float 
 namespace sgl {
 namespace cand {
 
-template <typename T>
-Image image_of(int D) {
-  switch (padded_dim(D)) {
-    case 64: return Image{Tiles<T, 2>::YT, Tiles<T, 2>::LD, Tiles<T, 2>::BYTES};
-    case 128: return Image{Tiles<T, 4>::YT, Tiles<T, 4>::LD, Tiles<T, 4>::BYTES};
-    case 192: return Image{Tiles<T, 6>::YT, Tiles<T, 6>::LD, Tiles<T, 6>::BYTES};
-    default: return Image{Tiles<T, 8>::YT, Tiles<T, 8>::LD, Tiles<T, 8>::BYTES};
-  }
+Image grad_image(int32_t dtype, int D) {
+  return pick_dim(dtype, D, [](auto t, auto db) {
+    using Im = Tiles<decltype(t), db.value>;
+    return Image{Im::YT, Im::LD, Im::BYTES};
+  });
 }
-Image grad_image(int32_t dtype, int D) { return dtype == SGL_FP32 ? image_of<float>(D) : image_of<bf16_t>(D); }
-int table_grad_block(int32_t dtype) { return (dtype == SGL_FP32 ? kXTile<float> : kXTile<bf16_t>) / kWaves; }
 int64_t table_grad_part(int32_t dtype, const Problem &p) {
-  const int64_t xtile = dtype == SGL_FP32 ? kXTile<float> : kXTile<bf16_t>;
-  return ((p.V + xtile - 1) / xtile + kGroups) * xtile * (padded_dim(p.D) + 4);
+  return pick_dim(dtype, p.D, [&](auto t, auto db) {
+    using P = Plan<decltype(t), db.value>;
+    constexpr int64_t xtile = 32 * P::WAVES;
+    return ((p.V + xtile - 1) / xtile + P::GROUPS) * xtile * (32 * db.value + 4);
+  });
 }
 
 void route_targets(int32_t dtype, const Problem &p, int K, const int32_t *ids, const float *weight, int32_t *index,
                    int2 *entries, hipStream_t stream) {
-  const int64_t N = p.N, V = p.V;
-  const int yt = grad_image(dtype, p.D).rows, vb = table_grad_block(dtype);
-  const RouteArgs a{ids, weight, N, (V + vb - 1) / vb, K, yt, vb, index, entries};
-  launch(&k_route, dim3(unsigned((N + yt - 1) / yt)), dim3(kRouteBlock), 0, stream, a);
+  const int yt = grad_image(dtype, p.D).rows;
+  const RouteArgs a{ids, weight, p.N, (p.V + kGradBlock - 1) / kGradBlock, K, yt, kGradBlock, index, entries};
+  launch(&k_route, dim3(unsigned((p.N + yt - 1) / yt)), dim3(kRouteBlock), 0, stream, a);
 }
 
 void table_grad(int32_t dtype, const Problem &p, const RowCoef &r, void *dtable, float *dbias, float *part,
                 hipStream_t stream) {
-  if (dtype == SGL_FP32) return pick<float>(p, r, dtable, dbias, part, stream);
-  if (dtype == SGL_BF16) return pick<bf16_t>(p, r, dtable, dbias, part, stream);
-  return pick<fp16_t>(p, r, dtable, dbias, part, stream);
+  const BwdArgs a{p, r, dtable, dbias, part};
+  pick_dim(dtype, p.D, [&](auto t, auto db) { run<decltype(t), db.value>(a, stream); });
 }
 
 }  // namespace cand

@@ -22,22 +22,20 @@ constexpr float kTop = std::is_same_v<T, fp16_t> ? 7.f : 0.f;
 // then rescale nothing.
 constexpr float kSlack = 8.f;
 
-constexpr int64_t kFewRows = 32;   // up to here a workgroup's waves share them and split the table
+// Two tiles in LDS, one being filled while the other is read, or one where two
+// do not fit.
+template <typename T, int DB, int YT>
+constexpr int kBuffers = 2 * YT * Tile32<T, 32 * DB>::LD * int(sizeof(T)) <= 140 * 1024 ? 2 : 1;
 
-// Blocks of 32 candidates of a wave in a tile: two for fewer barriers, one
-// where the tile on its way would not fit in the registers.
-template <typename T, int DB, int WX>
-constexpr int kSubTiles = WX == kWaves && DB < 8 ? 2 : 1;
-
-// XB blocks of 32 rows a wave; WX waves along the rows, 4 / WX along the table.
-template <typename T, int DB, int XB, int WX, bool DIR>
-__global__ __launch_bounds__(kBlock, 1) void k_forward(FwdArgs a) {
+// A wave has 32 rows; WX waves lie along the rows, WY along the table (few rows:
+// each has 32 candidates of a tile of its own, and leaves a partial of its
+// own). SUB steps of 32 candidates a tile.
+template <typename T, int DB, int WX, int WY, int SUB, int PER_SIMD, bool DIR>
+__global__ __launch_bounds__(64 * WX * WY, PER_SIMD) void k_forward(FwdArgs a) {
   using M = Mma32<T>;
-  constexpr int KS = M::KS, DP = 32 * DB, NK = DP / KS;
+  constexpr int BLOCK = 64 * WX * WY, KS = M::KS, DP = 32 * DB, NK = DP / KS, TRIM = kTrim<T>;
   using Tl = Tile32<T, DP>;
-  constexpr int LD = Tl::LD;
-  constexpr int WY = kWaves / WX, YS = kSubTiles<T, DB, WX>, YT = 32 * YS * WY;
-  constexpr int NBUF = 2 * YT * LD * int(sizeof(T)) <= 140 * 1024 ? 2 : 1;
+  constexpr int LD = Tl::LD, YT = 32 * SUB * WY, XT = 32 * WX, NBUF = kBuffers<T, DB, YT>;
   extern __shared__ __align__(16) char lds[];
   T *tiles = reinterpret_cast<T *>(lds);
   float *b2s = reinterpret_cast<float *>(lds + size_t(NBUF) * YT * LD * sizeof(T));
@@ -45,16 +43,15 @@ __global__ __launch_bounds__(kBlock, 1) void k_forward(FwdArgs a) {
   const Problem &p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = attn::wave_index(), wx = wave % WX, wy = wave / WX;
-  constexpr int XT = 32 * XB * WX;
   const int64_t N = a.order.count(p.N);
-  const Line line((N + XT - 1) / XT, (p.V + YT - 1) / YT, kGroups);
+  const Line line((N + XT - 1) / XT, (p.V + YT - 1) / YT, a.out.groups);
   const int w = blockIdx.x;
   if (w >= line.groups) return;
   const int64_t u1 = line.begin(w + 1);
   const T *table = static_cast<const T *>(p.table);
   const bool biased = p.bias != nullptr;
 
-  Stage<T, DP, YT> next(p.ts, p.D);
+  Stage<T, DP, YT, BLOCK> next(p.ts, p.D);
   float nb = 0.f;   // the bias of the next tile's row tid
   auto rows_of = [&](int t) { return int(min(p.V - int64_t(t) * YT, int64_t(YT))); };
   auto fetch = [&](int t) {
@@ -64,7 +61,7 @@ __global__ __launch_bounds__(kBlock, 1) void k_forward(FwdArgs a) {
     if (biased && tid < YT) nb = p.bias[y0 + min(tid, rows - 1)];
   };
 #pragma unroll
-  for (int i = 0; i < NBUF; ++i) Stage<T, DP, YT>::clear(tiles + i * YT * LD);
+  for (int i = 0; i < NBUF; ++i) Stage<T, DP, YT, BLOCK>::clear(tiles + i * YT * LD);
   int64_t u = line.begin(w);
   int xt = int(u / line.inner), t = int(u - int64_t(xt) * line.inner), buf = 0;
   fetch(t);
@@ -72,167 +69,133 @@ __global__ __launch_bounds__(kBlock, 1) void k_forward(FwdArgs a) {
 
 #pragma unroll 1
   for (; u < u1; ++xt) {   // an outer tile's piece
-  FragOf<T> xf[XB][NK];
-  const int D = fresh(p.D);
-  const int64_t x0 = (int64_t(xt) * WX + wx) * (32 * XB) + (lane & 31);
-#pragma unroll
-  for (int xb = 0; xb < XB; ++xb) {
-    const int64_t x = x0 + 32 * xb, row = a.order.row(min(x, N - 1));
-    load_outer<T>(xf[xb], static_cast<const T *>(p.h) + row * p.hs, x >= N, D);
-  }
-  float m[XB], mu[XB], l[XB], lc[XB];
-  f32x16 o[XB][DIR ? DB : 1];
-#pragma unroll
-  for (int xb = 0; xb < XB; ++xb) {
-    m[xb] = -INFINITY;
-    mu[xb] = -kTop<T>;
-    l[xb] = lc[xb] = 0.f;
+    FragOf<T> xf[NK];
+    const int D = fresh(p.D);
+    const int64_t x = (int64_t(xt) * WX + wx) * 32 + (lane & 31);
+    load_outer<T>(xf, static_cast<const T *>(p.h) + a.order.row(min(x, N - 1)) * p.hs, x >= N, D);
+    // the maximum, as used, the sum and its compensation (a row's sum has up to 2^15 terms)
+    float m = -INFINITY, mu = -kTop<T>, l = 0.f, lc = 0.f;
+    f32x16 o[DIR ? DB : 1];
 #pragma unroll
     for (int d = 0; d < (DIR ? DB : 1); ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[xb][d][r] = 0.f;
-  }
-  const int end = int(min(int64_t(line.inner), t + (u1 - u)));
-  u += end - t;
+      for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    const int end = int(min(int64_t(line.inner), t + (u1 - u)));
+    u += end - t;
 #pragma unroll 1
-  for (; t < end; ++t) {
-    T *tile = tiles + buf * YT * LD;
-    float *b2 = b2s + buf * YT;
-    if (NBUF == 1) __syncthreads();
-    const int rows = rows_of(t);
-    next.put(tile, rows, biased);
-    if (tid < YT) b2[tid] = tid >= rows ? -INFINITY : biased ? bias2_of(p, nb) : 0.f;
-    __syncthreads();
-    if (t + 1 < end || u < u1) fetch(t + 1 < end ? t + 1 : 0);   // (the next outer tile's first)
-    if (NBUF == 2) buf ^= 1;
+    for (; t < end; ++t) {
+      T *tile = tiles + buf * YT * LD;
+      float *b2 = b2s + buf * YT;
+      if (NBUF == 1) __syncthreads();
+      const int rows = rows_of(t);
+      next.put(tile, rows, biased);
+      if (tid < YT) b2[tid] = tid >= rows ? -INFINITY : biased ? bias2_of(p, nb) : 0.f;
+      __syncthreads();
+      if (t + 1 < end || u < u1) fetch(t + 1 < end ? t + 1 : 0);   // (the next outer tile's first)
+      if (NBUF == 2) buf ^= 1;
 #pragma unroll 1
-    for (int ys = 0; ys < YS; ++ys) {
-      const int row0 = (wy * YS + ys) * 32;
-      f32x16 s[XB];
+      for (int ys = 0; ys < SUB; ++ys) {
+        const int row0 = (wy * SUB + ys) * 32;
+        f32x16 s;
 #pragma unroll
-      for (int xb = 0; xb < XB; ++xb)
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[xb][r] = 0.f;
+        for (int k = 0; k < NK; ++k)
+          if (k < NK - TRIM || k * KS < p.D) s = M::mma(Tl::frag(tile, row0, k * KS), xf[k], s);
 #pragma unroll
-      for (int k = 0; k < NK; ++k) {
-        const FragOf<T> f = Tl::frag(tile, row0, k * KS);
+        for (int i = 0; i < 4; ++i) {
+          float b[4];
+          __builtin_memcpy(b, b2 + row0 + 8 * i + 4 * h, sizeof(b));
 #pragma unroll
-        for (int xb = 0; xb < XB; ++xb) s[xb] = M::mma(f, xf[xb][k], s[xb]);
-      }
-      float top[XB];
-      bool grow = false;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float b[4];
-        __builtin_memcpy(b, b2 + row0 + 8 * i + 4 * h, sizeof(b));
-#pragma unroll
-        for (int xb = 0; xb < XB; ++xb)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) s[xb][4 * i + v] = fmaf(s[xb][4 * i + v], p.c, b[v]);
-      }
-#pragma unroll
-      for (int xb = 0; xb < XB; ++xb) {
-        top[xb] = pair_max(max16(s[xb]));
-        grow |= top[xb] > m[xb] + kSlack;
-      }
-      if (__any(grow)) {
-#pragma unroll
-        for (int xb = 0; xb < XB; ++xb) {
-          const float mn = fmaxf(m[xb], top[xb]);
-          const float by = mn == m[xb] ? 1.f : exp2_fast(m[xb] - mn);
-          m[xb] = mn;
-          mu[xb] = (mn == -INFINITY ? 0.f : mn) - kTop<T>;
-          l[xb] *= by;
-          lc[xb] *= by;
-          if constexpr (DIR) scale_blocks(o[xb], by);
+          for (int v = 0; v < 4; ++v) s[4 * i + v] = fmaf(s[4 * i + v], p.c, b[v]);
         }
-      }
+        const float top = pair_max(max16(s));
+        if (__any(top > m + kSlack)) {
+          const float mn = fmaxf(m, top);
+          const float by = mn == m ? 1.f : exp2_fast(m - mn);
+          m = mn;
+          mu = (mn == -INFINITY ? 0.f : mn) - kTop<T>;
+          l *= by;
+          lc *= by;
+          if constexpr (DIR) scale_blocks<PER_SIMD == 1>(o, by);
+        }
 #pragma unroll
-      for (int xb = 0; xb < XB; ++xb) {
+        for (int r = 0; r < 16; ++r) s[r] = exp2_fast(s[r] - mu);
+        const float add = sum16(s) - lc, sum = l + add;
+        lc = (sum - l) - add;
+        l = sum;
+        if constexpr (DIR) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[xb][r] = exp2_fast(s[xb][r] - mu[xb]);
-        // a compensated sum of the blocks' sums: a row's sum has up to 2^15 of them
-        const float add = sum16(s[xb]) - lc[xb], sum = l[xb] + add;
-        lc[xb] = (sum - l[xb]) - add;
-        l[xb] = sum;
-      }
-      if constexpr (DIR) {
+          for (int st = 0; st < 32 / KS; ++st) {
+            const FragOf<T> pf = frag_of16<T>(s, st);
 #pragma unroll
-        for (int st = 0; st < 32 / KS; ++st) {
-          FragOf<T> pf[XB];
-#pragma unroll
-          for (int xb = 0; xb < XB; ++xb) pf[xb] = frag_of16<T>(s[xb], st);
-#pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            const FragOf<T> f = Tl::frag_t(tile, 32 * d, row0, st);
-#pragma unroll
-            for (int xb = 0; xb < XB; ++xb) o[xb][d] = M::mma(f, pf[xb], o[xb][d]);
+            for (int d = 0; d < DB; ++d) o[d] = M::mma(Tl::frag_t(tile, 32 * d, row0, st), pf, o[d]);
           }
         }
       }
     }
-  }
 
-  const int64_t part = int64_t(w + xt) * WY + wy;
+    const int64_t at = (int64_t(w + xt) * WY + wy) * XT + wx * 32 + (lane & 31);
+    const float sum = pair_sum(l);
+    if (x < N) {
+      if (h == 0) {
+        a.out.m[at] = m == -INFINITY ? -INFINITY : mu;
+        a.out.l[at] = sum;
+      }
+      if constexpr (DIR) {
+        float *row = a.out.o + at * DP;
 #pragma unroll
-  for (int xb = 0; xb < XB; ++xb) {
-    const int at = wx * (32 * XB) + 32 * xb + (lane & 31);
-    const float sum = pair_sum(l[xb]);
-    if (x0 + 32 * xb >= N) continue;
-    if (h == 0) {
-      a.out.m[part * XT + at] = m[xb] == -INFINITY ? -INFINITY : mu[xb];
-      a.out.l[part * XT + at] = sum;
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float q[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) q[v] = o[d][4 * i + v];
+            store_n(row + 32 * d + 8 * i + 4 * h, q);
+          }
+      }
     }
-    if constexpr (DIR) {
-      float *row = a.out.o + (part * XT + at) * DP;
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float q[4];
-#pragma unroll
-          for (int v = 0; v < 4; ++v) q[v] = o[xb][d][4 * i + v];
-          store_n(row + 32 * d + 8 * i + 4 * h, q);
-        }
-    }
-  }
-  t = 0;
+    t = 0;
   }
 }
 
-// Which form: by the rows.
-template <typename T, int DB, int XB, int WX, bool DIR>
-void run(const FwdArgs &a, hipStream_t stream) {
-  constexpr int DP = 32 * DB, LD = Tile32<T, DP>::LD, YS = kSubTiles<T, DB, WX>, YT = 32 * YS * (kWaves / WX);
-  constexpr int NBUF = 2 * YT * LD * int(sizeof(T)) <= 140 * 1024 ? 2 : 1;
-  constexpr size_t bytes = size_t(NBUF) * YT * (LD * sizeof(T) + sizeof(float));
-  static_assert(bytes <= 160 * 1024, "LDS of a CU");
-  auto *k = &k_forward<T, DB, XB, WX, DIR>;
-  (void)ensure_dynamic_lds(reinterpret_cast<const void *>(k), bytes);
-  const Line line((a.p.N + 32 * XB * WX - 1) / (32 * XB * WX), (a.p.V + YT - 1) / YT, kGroups);
-  launch(k, dim3(unsigned(line.groups)), dim3(kBlock), bytes, stream, a);
+// Up to here a workgroup's waves share the rows and split the table.
+constexpr int64_t kFewRows = 32;
+constexpr int kFewWaves = 4;
+template <typename T, int DB>
+Partials shape_of(const Problem &p) {
+  using P = Plan<T, DB>;
+  Partials s{};
+  const bool few = p.N <= kFewRows;
+  s.rows = few ? 32 : 32 * P::WAVES;
+  s.wy = few ? kFewWaves : 1;
+  s.dp = 32 * DB;
+  s.groups = few ? 256 : P::GROUPS;
+  const int ytile = few ? 32 * kFewWaves : 32 * P::SUB;
+  s.ytiles = (p.V + ytile - 1) / ytile;
+  return s;
 }
 template <typename T, int DB, bool DIR>
-void pick_form(const FwdArgs &a, hipStream_t stream) {
-  constexpr int XB = sizeof(T) == 4 ? 1 : 2;
+void run(const FwdArgs &a, hipStream_t stream) {
+  using P = Plan<T, DB>;
+  const Line line((a.p.N + a.out.rows - 1) / a.out.rows, a.out.ytiles, a.out.groups);
+  auto go = [&](auto *k, int threads, size_t bytes) {
+    (void)ensure_dynamic_lds(reinterpret_cast<const void *>(k), bytes);
+    launch(k, dim3(unsigned(line.groups)), dim3(unsigned(threads)), bytes, stream, a);
+  };
+  constexpr size_t row = Tile32<T, 32 * DB>::LD * sizeof(T) + sizeof(float);
+  constexpr int few = 32 * kFewWaves, many = 32 * P::SUB;
+  constexpr size_t few_bytes = kBuffers<T, DB, few> * few * row, many_bytes = kBuffers<T, DB, many> * many * row;
+  static_assert(few_bytes <= 160 * 1024 && many_bytes <= 160 * 1024 * P::GROUPS_PER_TWO / 2, "LDS of a CU");
   if (a.p.N <= kFewRows)
-    run<T, DB, 1, 1, DIR>(a, stream);
+    go(&k_forward<T, DB, 1, kFewWaves, 1, P::PER_SIMD, DIR>, 64 * kFewWaves, few_bytes);
   else
-    run<T, DB, XB, 4, DIR>(a, stream);
+    go(&k_forward<T, DB, P::WAVES, 1, P::SUB, P::PER_SIMD, DIR>, 64 * P::WAVES, many_bytes);
 }
-template <typename T, bool DIR>
-void pick_dim(const FwdArgs &a, hipStream_t stream) {
-  switch (padded_dim(a.p.D)) {
-    case 64: return pick_form<T, 2, DIR>(a, stream);
-    case 128: return pick_form<T, 4, DIR>(a, stream);
-    case 192: return pick_form<T, 6, DIR>(a, stream);
-    default: return pick_form<T, 8, DIR>(a, stream);
-  }
-}
-template <typename T>
-void pick_dir(const FwdArgs &a, hipStream_t stream) {
-  if (a.out.o != nullptr) pick_dim<T, true>(a, stream);
-  else pick_dim<T, false>(a, stream);
+template <typename T, int DB>
+void pick(const FwdArgs &a, hipStream_t stream) {
+  if (a.out.o != nullptr) run<T, DB, true>(a, stream);
+  else run<T, DB, false>(a, stream);
 }
 
 }  // namespace
@@ -243,21 +206,12 @@ namespace cand {
 int padded_dim(int D) { return (D + 63) / 64 * 64; }
 
 Partials forward_shape(int32_t dtype, const Problem &p) {
-  Partials s{};
-  const bool few = p.N <= kFewRows;
-  s.rows = few ? 32 : dtype == SGL_FP32 ? 128 : 256;
-  s.wy = few ? 4 : 1;
-  s.dp = padded_dim(p.D);
-  const int64_t ytile = few ? 128 : s.dp == 256 ? 32 : 64;
-  s.ytiles = (p.V + ytile - 1) / ytile;
-  return s;
+  return pick_dim(dtype, p.D, [&](auto t, auto db) { return shape_of<decltype(t), db.value>(p); });
 }
 
 void forward_partials(int32_t dtype, const Problem &p, const Order &order, const Partials &out, hipStream_t stream) {
   const FwdArgs a{p, order, out};
-  if (dtype == SGL_FP32) return pick_dir<float>(a, stream);
-  if (dtype == SGL_BF16) return pick_dir<bf16_t>(a, stream);
-  return pick_dir<fp16_t>(a, stream);
+  pick_dim(dtype, p.D, [&](auto t, auto db) { pick<decltype(t), db.value>(a, stream); });
 }
 
 }  // namespace cand
