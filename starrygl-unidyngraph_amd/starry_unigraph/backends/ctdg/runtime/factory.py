@@ -50,12 +50,13 @@ def build_ctdg_runtime(session_ctx: SessionContext, events=None) -> tuple[CTDGOn
                                 world_size=session_ctx.dist.world_size)
     memory = CTDGMemoryBank(num_nodes=dataset.num_nodes, hidden_dim=hidden_dim, device=device,
                             mailbox_slots=mailbox_slots, edge_feat_dim=edge_feat_dim)
-    embedding = str(c.get("embedding", "attention"))
+    embedding, objective = str(c.get("embedding", "attention")), str(c.get("objective", "link"))
     shift, scale = dataset.inter_event_stats("train") if embedding in ("time_projection", "history") else (0.0, 1.0)
     model = build_ctdg_model(str(cfg["model"]["family"]), num_nodes=dataset.num_nodes, hidden_dim=hidden_dim,
                              edge_feat_dim=edge_feat_dim, dim_time=dim_time, num_head=num_head, dropout=dropout,
                              att_dropout=att_dropout, embedding=embedding, time_shift=shift,
-                             time_scale=scale,
+                             time_scale=scale, positions=str(c.get("positions", "bias")), objective=objective,
+                             candidates=dataset.dst.unique() if objective == "next_node" else None,
                              attention_gemm_dtype=str(c.get("attention_gemm_dtype", "fp32"))).to(device)
     memory_updater = CTDGMemoryUpdater(hidden_dim=hidden_dim, mailbox_slot_dim=2 * hidden_dim + edge_feat_dim,
                                        mailbox_slots=mailbox_slots,

@@ -27,7 +27,7 @@ from torch import nn
 
 from starry_unigraph.lib import _capi
 from starry_unigraph.native.step import ConvDims, ConvFunction, DeviceStep
-from starry_unigraph.runtime.modules import HistoryEncoder, TimeEncode
+from starry_unigraph.runtime.modules import CandidateHead, HistoryEncoder, TimeEncode
 
 
 class TemporalTransformerConv(nn.Module):
@@ -274,11 +274,12 @@ class CTDGHistoryPredictor(CTDGLinkPredictor):
     ctdg.dropout and ctdg.att_dropout have no effect on it."""
 
     def __init__(self, num_nodes: int, hidden_dim: int, edge_feat_dim: int, num_head: int = 2,
-                 mean_gap: float = 1.0) -> None:
+                 mean_gap: float = 1.0, positions: str = "bias") -> None:
         nn.Module.__init__(self)
         self.hidden_dim = hidden_dim
         self.conv = None
-        self.history = HistoryEncoder(hidden_dim, hidden_dim + edge_feat_dim, num_head, mean_gap=mean_gap)
+        self.history = HistoryEncoder(hidden_dim, hidden_dim + edge_feat_dim, num_head, mean_gap=mean_gap,
+                                      positions=positions)
         self.src_fc = nn.Linear(hidden_dim, hidden_dim)
         self.dst_fc = nn.Linear(hidden_dim, hidden_dim)
         self.out_fc = nn.Linear(hidden_dim, 1)
@@ -299,6 +300,28 @@ class CTDGHistoryPredictor(CTDGLinkPredictor):
         return F.pad(torch.where(live.unsqueeze(1), y, 0.0), (0, 0, 0, 1))
 
 
+class CTDGNextNodePredictor(CTDGHistoryPredictor):
+    """The history embedding of an event's source, and which node comes next to
+    it out of all candidates (CandidateHead), in place of the edge predictor
+    and its one negative; select it with ctdg.objective = next_node. Its
+    logits are the scores of the destination and of the drawn negative."""
+
+    def __init__(self, num_nodes: int, hidden_dim: int, edge_feat_dim: int, num_head: int = 2,
+                 mean_gap: float = 1.0, positions: str = "bias", candidates: torch.Tensor | None = None) -> None:
+        nn.Module.__init__(self)
+        self.hidden_dim = hidden_dim
+        self.conv = None
+        self.history = HistoryEncoder(hidden_dim, hidden_dim + edge_feat_dim, num_head, mean_gap=mean_gap,
+                                      positions=positions)
+        self.src_fc = nn.Linear(hidden_dim, hidden_dim)
+        self.head = CandidateHead(torch.arange(num_nodes) if candidates is None else candidates, num_nodes, hidden_dim)
+
+    def forward(self, src_emb: torch.Tensor, dst: torch.Tensor, neg: torch.Tensor) -> CTDGModelOutput:
+        """``src_emb`` [N, D]; ``dst``, ``neg``: node ids int64 [N]."""
+        h = self.src_fc(src_emb)
+        return CTDGModelOutput(pos_logits=self.head(h, dst), neg_logits=self.head(h, neg))
+
+
 @dataclass(frozen=True)
 class CTDGModelSpec:
     model_cls: type[nn.Module]
@@ -313,23 +336,32 @@ CTDG_MODEL_SPECS: dict[str, CTDGModelSpec] = {
 def build_ctdg_model(model_family: str, *, num_nodes: int, hidden_dim: int, edge_feat_dim: int, dim_time: int = 100,
                      num_head: int = 2, dropout: float = 0.1, att_dropout: float = 0.1,
                      embedding: str = "attention", time_shift: float = 0.0, time_scale: float = 1.0,
-                     attention_gemm_dtype: str = "fp32") -> nn.Module:
+                     attention_gemm_dtype: str = "fp32", positions: str = "bias", objective: str = "link",
+                     candidates: torch.Tensor | None = None) -> nn.Module:
     """models.py:345-386. ``embedding`` "attention" (the reference's model for
     every family), "time_projection" (config 2's JODIE embedding) or "history"
     (the window as a sequence; ``time_shift`` is its mean gap);
     ``attention_gemm_dtype`` "bf16": the attention and edge-predictor products
-    on bf16 weight copies (benchmark configurations 4 and 5)."""
+    on bf16 weight copies (benchmark configurations 4 and 5). With the history
+    embedding ``positions`` "bias" or "rotary" is how it sees an event's age,
+    and ``objective`` "next_node" learns which of ``candidates`` (node ids;
+    None: every node) comes next instead of links against drawn negatives."""
     spec = CTDG_MODEL_SPECS.get(model_family.lower())
     if spec is None:
         raise KeyError(f"Unsupported CTDG model family: {model_family}")
+    if objective not in ("link", "next_node"):
+        raise KeyError(f"unknown ctdg.objective {objective!r}: expected 'link' or 'next_node'")
+    if embedding != "history" and (positions != "bias" or objective != "link"):
+        raise ValueError("ctdg.positions and ctdg.objective: options of ctdg.embedding = history")
     if embedding == "time_projection":
         return CTDGTimeProjectionPredictor(num_nodes=num_nodes, hidden_dim=hidden_dim, time_shift=time_shift,
                                            time_scale=time_scale)
     if embedding == "history":
         if attention_gemm_dtype != "fp32":
             raise ValueError("ctdg.attention_gemm_dtype: the history embedding runs in fp32")
-        return CTDGHistoryPredictor(num_nodes=num_nodes, hidden_dim=hidden_dim, edge_feat_dim=edge_feat_dim,
-                                    num_head=num_head, mean_gap=time_shift)
+        kw = dict(num_nodes=num_nodes, hidden_dim=hidden_dim, edge_feat_dim=edge_feat_dim, num_head=num_head,
+                  mean_gap=time_shift, positions=positions)
+        return CTDGHistoryPredictor(**kw) if objective == "link" else CTDGNextNodePredictor(**kw, candidates=candidates)
     if embedding != "attention":
         raise KeyError(f"unknown ctdg.embedding {embedding!r}: expected 'attention', 'history' or 'time_projection'")
     model = spec.model_cls(num_nodes=num_nodes, hidden_dim=hidden_dim, edge_feat_dim=edge_feat_dim,

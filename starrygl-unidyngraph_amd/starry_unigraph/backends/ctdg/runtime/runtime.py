@@ -22,7 +22,7 @@ from __future__ import annotations
 
 import time
 from dataclasses import dataclass
-from typing import Any, Iterable
+from typing import Any, Callable, Iterable
 
 import torch
 import torch.nn.functional as F
@@ -104,6 +104,7 @@ class CTDGOnlineRuntime:
         # the time-projection model (config 2's JODIE) has no attention: its
         # back part is the projection, the predictor and their backward
         self._hist = getattr(core, "history", None) is not None
+        self._next_node = self._hist and getattr(core, "head", None) is not None
         self._proj = conv is None and not self._hist
         if self._hist:   # (its back part runs through autograd: no launch plans)
             self.dims = ConvDims(D=memory.hidden_dim, F=max(1, dataset.edge_feat_dim), T=1, H=1, fanout=fan)
@@ -171,6 +172,10 @@ class CTDGOnlineRuntime:
         # its products in bf16 (the fused update keeps them current; dirty:
         # rebuild from the parameters before the next step)
         self._bf16: Bf16Shadow | None = None
+        # a larger model's answers that the next-node objective learns from as
+        # well (set_teacher), and those of the step at hand
+        self._teacher: tuple | None = None
+        self._taught: tuple | None = None
         self._bf16_dirty = True
         self._bf16_ver: tuple = ()
         self._back_metrics = False
@@ -450,6 +455,7 @@ class CTDGOnlineRuntime:
             src, dst, ts, ef = self._device_batch(batch)
             self._front_body(step, split, n, src, dst, buf[off:off + n] if off >= 0 else buf, ts, ef, None)
             self._commit_body(step, train)
+            self._taught = self._teacher[0](batch) if train and self._teacher is not None else None
             self._back_body(step, train, n)
             self.fence()
         else:
@@ -619,15 +625,18 @@ class CTDGOnlineRuntime:
 
     def _history_back(self, step: DeviceStep, train: bool, n: int) -> None:
         """The back part of the history embedding: embeddings, edge predictor
-        and BCE (runtime.py:197-199) and, in training, autograd's backward
+        and BCE (runtime.py:197-199), or the next-node objective, and, in training, autograd's backward
         into the optimizer's flat gradients and its step."""
         b = step.buf
         core = self._core()
         with torch.set_grad_enabled(train):
             y = core.roots(step, self.dims)
-            out = core(y[b.ridx_src[:n]], y[b.ridx_dst[:n]], y[b.ridx_neg[:n]])
-            # BCE of 1 and 0 on the logits
-            loss = F.softplus(-out.pos_logits).mean() + F.softplus(out.neg_logits).mean()
+            if self._next_node:
+                out, loss = self._next_node_loss(core, y, b, n)
+            else:
+                out = core(y[b.ridx_src[:n]], y[b.ridx_dst[:n]], y[b.ridx_neg[:n]])
+                # BCE of 1 and 0 on the logits
+                loss = F.softplus(-out.pos_logits).mean() + F.softplus(out.neg_logits).mean()
         if train:
             self.optimizer.zero_grad()
             loss.backward()
@@ -635,6 +644,38 @@ class CTDGOnlineRuntime:
         b.pos[:n].copy_(out.pos_logits.detach())
         b.neg[:n].copy_(out.neg_logits.detach())
         b.loss.copy_(loss.detach())
+
+    def _next_node_loss(self, core, y: torch.Tensor, b, n: int) -> tuple:
+        """(logits, loss) of the next-node objective: the mean cross entropy of
+        the destinations over all candidates, and with a teacher its
+        divergence."""
+        nodes = F.pad(b.roots[:b.cap], (0, 1), value=-1)
+        src, dst, neg = y[b.ridx_src[:n]], nodes[b.ridx_dst[:n]], nodes[b.ridx_neg[:n]]
+        with torch.no_grad():
+            out = core(src, dst, neg)
+        h = core.src_fc(src)
+        loss = core.head.loss(h, dst).mean()
+        if self._taught is not None:
+            (ids, logits), self._taught = self._taught, None
+            _, weight, temperature = self._teacher
+            loss = (1.0 - weight) * loss + weight * core.head.distill(h, ids, logits, temperature).mean()
+        return out, loss
+
+    def set_teacher(self, teacher: Callable | None, weight: float = 0.5, temperature: float = 1.0) -> None:
+        """Training steps of ctdg.objective = next_node learn from a larger
+        model as well: ``teacher(batch)`` gives its top candidates of each event,
+        (node ids int64 [n, K], logits float32 [n, K]) on the runtime's device
+        (a negative id, one that is no candidate, or a logit of -inf: no
+        entry). The step's loss is then ``(1 - weight) * cross entropy + weight *
+        divergence`` at ``temperature``. None: no teacher. The reference has no
+        counterpart."""
+        if not self._next_node:
+            raise ValueError("set_teacher: needs ctdg.embedding = history and ctdg.objective = next_node")
+        if not 0.0 <= weight <= 1.0:
+            raise ValueError(f"set_teacher: weight {weight}, expected 0 to 1")
+        if not 0.0 < temperature < float("inf"):
+            raise ValueError(f"set_teacher: temperature {temperature}, expected a positive number")
+        self._teacher = None if teacher is None else (teacher, float(weight), float(temperature))
 
     def _metrics_op(self, step: DeviceStep, n: int) -> None:
         """The step's metrics into the next ring slot as the last op of its

@@ -1,4 +1,5 @@
+from .candidates import CandidateHead
 from .history import HistoryEncoder
 from .time_encode import TimeEncode
 
-__all__ = ["HistoryEncoder", "TimeEncode"]
+__all__ = ["CandidateHead", "HistoryEncoder", "TimeEncode"]

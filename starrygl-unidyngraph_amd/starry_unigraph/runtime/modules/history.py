@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
-from starry_unigraph.native import history
+from starry_unigraph.native import history, rotary
 
 
 class HistoryEncoder(nn.Module):
@@ -19,24 +19,36 @@ class HistoryEncoder(nn.Module):
         f, v, c    = W_f x, W_v x, W_c x
         h          = gated_scan(f, v)       gate decays with the time between events
         y, n       = gated_norm(x, h, c)                 residual, then the next norm
-        o          = cross_attention(W_q root, W_k n, W_v' n)   bias by event age
+        o          = cross_attention(W_q root, W_k n, W_v' n)   event ages by ``positions``
         _, out     = gated_norm(root, W_o o, W_g o)
 
     ``mean_gap``: the time that the decay rates start around (they are learned,
-    one a channel, from 1/64 to 4 per mean gap)."""
+    one a channel, from 1/64 to 4 per mean gap). ``positions``: how the
+    attention sees an event's age, "bias" (a learned bias by ``buckets`` of it)
+    or "rotary" (queries and keys turned by it, the fastest pair one radian a
+    mean gap)."""
 
-    def __init__(self, dim: int, event_dim: int, heads: int = 2, buckets: int = 32, mean_gap: float = 1.0) -> None:
+    def __init__(self, dim: int, event_dim: int, heads: int = 2, buckets: int = 32, mean_gap: float = 1.0,
+                 positions: str = "bias") -> None:
         super().__init__()
         if dim % heads:
             raise ValueError(f"history embedding: {dim} channels over {heads} heads")
-        self.dim, self.event_dim, self.heads = dim, event_dim, heads
+        if positions not in ("bias", "rotary"):
+            raise ValueError(f"history embedding: positions {positions!r}, expected 'bias' or 'rotary'")
+        if positions == "rotary" and dim // heads < 2:
+            raise ValueError("history embedding: rotary positions need heads of 2 channels or more")
+        self.dim, self.event_dim, self.heads, self.positions = dim, event_dim, heads, positions
         self.per_gap = 1.0 / mean_gap if mean_gap > 0 else 1.0
         self.inp = nn.Linear(event_dim, dim)
         self.gates = nn.Linear(dim, 3 * dim)
         self.log_rate = nn.Parameter(torch.linspace(-6.0, 2.0, dim) * 0.6931471805599453)
         self.q = nn.Linear(dim, dim)
         self.kv = nn.Linear(dim, 2 * dim)
-        self.age_bias = nn.Parameter(torch.zeros(heads, buckets))
+        if positions == "bias":
+            self.age_bias = nn.Parameter(torch.zeros(heads, buckets))
+        else:
+            self.register_buffer("freqs", rotary.frequencies(dim // heads // 2 * 2, scaling="linear",
+                                                             factor=1.0 / self.per_gap, device="cpu"), persistent=False)
         self.out = nn.Linear(dim, 2 * dim)
         self.norms = nn.ParameterDict({
             **{f"{at}_{w}_{k}": nn.Parameter((torch.ones if k == "w" else torch.zeros)(dim))
@@ -64,8 +76,12 @@ class HistoryEncoder(nn.Module):
         h, _ = history.gated_scan(f, v, lens=cnt, gaps=gaps, decay=self.log_rate.exp())
         _, n = self._norm("event", x, h, c)
         k, w = self.kv(n).view(N, K, 2, H, D // H).unbind(2)
-        o = history.cross_attention(self.q(root).view(N, 1, H, D // H), k, w, k_lens=cnt, bias=self.age_bias,
-                                    q_pos=torch.zeros(N, 1, dtype=torch.int64, device=age.device),
-                                    k_pos=age.to(torch.int64).neg())
+        q = self.q(root).view(N, 1, H, D // H)
+        q_pos, k_pos = torch.zeros(N, 1, dtype=torch.int64, device=age.device), age.to(torch.int64).neg()
+        if self.positions == "rotary":
+            q, k = rotary.rotate(q, k, q_pos, k_pos, self.freqs)
+            o = history.cross_attention(q, k, w, k_lens=cnt)
+        else:
+            o = history.cross_attention(q, k, w, k_lens=cnt, bias=self.age_bias, q_pos=q_pos, k_pos=k_pos)
         z, gate = self.out(o.reshape(N, D)).split(D, -1)
         return self._norm("root", root, z, gate)[1]
