@@ -7,14 +7,18 @@
 // angle of a position of 1e9 has no digits left of the turn). The gradient is
 // the same rotation the other way round.
 //
-// Memory bounds it: every element is read and written once.
+// Memory bounds it, every element read and written once: 16 sequences of 8,191
+// x (8 + 2) heads of 128 in fp16 120 us, 5.6 TB/s (a large copy: 5.1); 4,000 x
+// (20 + 32) x 4 heads of 43 in bf16, odd rows of 86 bytes, 41 us when just
+// written and 57 from memory; 400
+// x 1 x 2 heads of 50, one new event each, 4 us, the launch.
 #include "history.h"
 
 namespace {
 
 using namespace sgl;
 
-constexpr int kBlock = 256;
+constexpr int kBlock = 256, kSteps = 512;
 
 struct Side {
   const void *x;
@@ -63,99 +67,106 @@ __device__ __forceinline__ uint64_t turn_step(double f) {
   return fraction(hi) + fraction(lo);
 }
 
+// A workgroup forms the frequencies' steps once where they are few (SHARED: up
+// to kSteps pairs; 64-bit floating point of every lane
+// otherwise: one head of 172 in fp16 38 us for 57, two of 100 with 64 turned 39
+// for 53).
 // A lane owns VEC consecutive channels of a row (both halves' in the half
-// layout) for a range of its heads; the angle is formed once for all of them.
-// The lanes past the rotated channels copy.
-template <typename T, int VEC, bool INTER>
+// layout) for all its heads; the angles are formed once for all of them. A
+// part's last lane takes its last VEC channels, some of them its neighbour's
+// too (it writes the same bits: each product and sum is rounded as written), so
+// that loads and stores are all whole (4 heads of 44 in bf16: 123 us with the
+// last ones one by one, 30 so); channels that are not rotated and fewer than VEC
+// go one by one.
+template <typename T, int VEC, bool INTER, bool SHARED>
 __global__ __launch_bounds__(kBlock) void k_rotate(RotArgs a) {
   const int sd = int64_t(blockIdx.x) >= a.side[1].first ? 1 : 0;
   const Side &s = a.side[sd];
   const int half = a.rot / 2;
-  // units of a row: pairs of the rotated part, then the rest
-  const int pairs = INTER ? VEC / 2 : VEC;                 // pairs a unit holds
-  const int ru = (half + pairs - 1) / pairs, cu = (a.dh - a.rot + VEC - 1) / VEC, units = ru + cu;
+  constexpr int PV = INTER ? VEC / 2 : VEC;   // pairs of a lane
+  const int ru = (half + PV - 1) / PV, cu = (a.dh - a.rot + VEC - 1) / VEC, units = ru + cu;
   const int64_t at = (int64_t(blockIdx.x) - s.first) * kBlock + threadIdx.x;
   const int64_t row = at / units;
+  __shared__ uint64_t steps[SHARED ? kSteps : 1];
+  if constexpr (SHARED) {
+    for (int i = threadIdx.x; i < half; i += kBlock) steps[i] = turn_step(a.freqs[i]);
+    __syncthreads();
+  }
   if (row >= s.rows) return;
   const int u = int(at - row * units);
   const int64_t n = row / s.L, t = row - n * s.L;
   const T *x = static_cast<const T *>(s.x) + n * s.sn + t * s.st;
   T *y = static_cast<T *>(s.y) + row * s.H * a.dh;
   if (u >= ru) {   // what is not rotated
-    const int d = a.rot + (u - ru) * VEC, w = min(VEC, a.dh - d);
+    const int rest = a.dh - a.rot;
+    const int d = a.rot + max(min((u - ru) * VEC, rest - VEC), 0);
+#pragma unroll 4
     for (int h = 0; h < s.H; ++h, x += s.sh, y += a.dh) {
-      if (w == VEC) {
+      if (rest >= VEC) {
         T v[VEC];
         load_n(v, x + d);
         store_n(y + d, v);
       } else {
-        for (int i = 0; i < w; ++i) y[d + i] = x[d + i];
+        for (int i = 0; i < rest; ++i) y[d + i] = x[d + i];
       }
     }
     return;
   }
-  const int p0 = u * pairs, np = min(pairs, half - p0);
+  const int p0 = min(u * PV, half - PV);
   const int64_t pos = s.pos[n * s.pn + t * s.pt];
-  constexpr int PV = INTER ? VEC / 2 : VEC;
   float sn[PV], cs[PV];
 #pragma unroll
   for (int i = 0; i < PV; ++i) {
-    sincos_turns(uint64_t(pos) * turn_step(a.freqs[p0 + min(i, np - 1)]), sn[i], cs[i]);
+    sincos_turns(uint64_t(pos) * (SHARED ? steps[p0 + i] : turn_step(a.freqs[p0 + i])), sn[i], cs[i]);
     sn[i] *= a.gain * a.way;
     cs[i] *= a.gain;
   }
+#pragma unroll 4
   for (int h = 0; h < s.H; ++h, x += s.sh, y += a.dh) {
     if constexpr (INTER) {
       T v[VEC];
-      if (np == PV) {
-        load_n(v, x + 2 * p0);
+      load_n(v, x + 2 * p0);
 #pragma unroll
-        for (int i = 0; i < PV; ++i) {
-          const float p = float(v[2 * i]), q = float(v[2 * i + 1]);
-          v[2 * i] = T(p * cs[i] - q * sn[i]);
-          v[2 * i + 1] = T(p * sn[i] + q * cs[i]);
-        }
-        store_n(y + 2 * p0, v);
-      } else {
-#pragma unroll
-        for (int i = 0; i < PV; ++i)
-          if (i < np) {
-            const float p = float(x[2 * (p0 + i)]), q = float(x[2 * (p0 + i) + 1]);
-            y[2 * (p0 + i)] = T(p * cs[i] - q * sn[i]);
-            y[2 * (p0 + i) + 1] = T(p * sn[i] + q * cs[i]);
-          }
+      for (int i = 0; i < PV; ++i) {
+        const float p = float(v[2 * i]), q = float(v[2 * i + 1]);
+        v[2 * i] = T(fmaf(p, cs[i], -(q * sn[i])));
+        v[2 * i + 1] = T(fmaf(p, sn[i], q * cs[i]));
       }
+      store_n(y + 2 * p0, v);
     } else {
-      if (np == PV) {
-        T v[VEC], w[VEC];
-        load_n(v, x + p0);
-        load_n(w, x + half + p0);
+      T v[VEC], w[VEC];
+      load_n(v, x + p0);
+      load_n(w, x + half + p0);
 #pragma unroll
-        for (int i = 0; i < PV; ++i) {
-          const float p = float(v[i]), q = float(w[i]);
-          v[i] = T(p * cs[i] - q * sn[i]);
-          w[i] = T(p * sn[i] + q * cs[i]);
-        }
-        store_n(y + p0, v);
-        store_n(y + half + p0, w);
-      } else {
-#pragma unroll
-        for (int i = 0; i < PV; ++i)
-          if (i < np) {
-            const float p = float(x[p0 + i]), q = float(x[half + p0 + i]);
-            y[p0 + i] = T(p * cs[i] - q * sn[i]);
-            y[half + p0 + i] = T(p * sn[i] + q * cs[i]);
-          }
+      for (int i = 0; i < PV; ++i) {
+        const float p = float(v[i]), q = float(w[i]);
+        v[i] = T(fmaf(p, cs[i], -(q * sn[i])));
+        w[i] = T(fmaf(p, sn[i], q * cs[i]));
       }
+      store_n(y + p0, v);
+      store_n(y + half + p0, w);
     }
   }
 }
 
+template <typename T, int VEC, bool INTER>
+void go(RotArgs a, dim3 grid, hipStream_t stream) {
+  if (a.rot / 2 <= kSteps) launch(&k_rotate<T, VEC, INTER, true>, grid, dim3(kBlock), 0, stream, a);
+  else launch(&k_rotate<T, VEC, INTER, false>, grid, dim3(kBlock), 0, stream, a);
+}
 template <typename T, bool INTER>
 int run(RotArgs a, hipStream_t stream) {
-  constexpr int VEC = 16 / int(sizeof(T));
-  const int pairs = INTER ? VEC / 2 : VEC, half = a.rot / 2;
-  const int64_t units = (half + pairs - 1) / pairs + (a.dh - a.rot + VEC - 1) / VEC;
+  constexpr int MOST = (INTER ? 16 : 8) / int(sizeof(T)), LEAST = INTER ? 2 : 1;
+  const int half = a.rot / 2;
+  // A lane moves 16 bytes at a time (two loads of 8 in the half layout), or half
+  // of that where rows are not whole words (4 heads of 43 in bf16, interleaved 54 us
+  // with 16 bytes and 43 with 8, halves 53 with 8 and 45 with 4; 44 channels: 30
+  // with 8, 31 with 4; 128: 87 and 94), and no more than the pairs there are.
+  int vec = MOST;
+  if (a.dh * int(sizeof(T)) % 4 != 0) vec /= 2;
+  while (vec > LEAST && half > 0 && half < (INTER ? vec / 2 : vec)) vec /= 2;
+  const int pairs = INTER ? vec / 2 : vec;
+  const int64_t units = (half + pairs - 1) / pairs + (a.dh - a.rot + vec - 1) / vec;
   int64_t grid = 0;
   for (int i = 0; i < 2; ++i) {
     a.side[i].first = grid;
@@ -164,7 +175,10 @@ int run(RotArgs a, hipStream_t stream) {
   if (a.side[1].rows == 0) a.side[1].first = INT64_MAX;
   SGL_REQUIRE(grid < (1 << 24), "rotary: too many rows");   // (a launch has 2^32 threads)
   if (grid == 0) return SGL_OK;
-  launch(&k_rotate<T, VEC, INTER>, dim3(unsigned(grid)), dim3(kBlock), 0, stream, a);
+  const dim3 g{unsigned(grid)};
+  if (vec == MOST) go<T, MOST, INTER>(a, g, stream);
+  else if (MOST / 2 > LEAST && vec == MOST / 2) go<T, MOST / 2, INTER>(a, g, stream);
+  else go<T, LEAST, INTER>(a, g, stream);
   SGL_CHECK_LAUNCH();
   return SGL_OK;
 }

@@ -142,7 +142,7 @@ def test_step_and_gradients_match_the_definitions(gpu, monkeypatch, taught, posi
         ids, logits = (t.cpu() for t in _teacher(rt)(batches[303]))
         loss = 0.75 * loss + 0.25 * model.head.distill(h, ids, logits, 2.0).mean()
     loss.backward()
-    assert abs(out["loss"] - float(loss)) < 1e-5
+    assert abs(out["loss"] - float(loss.detach())) < 1e-5
     want = model.head(h, dst)
     assert torch.allclose(b.pos[:n].cpu().double(), want, rtol=1e-4, atol=1e-5)
     for name, p in model.named_parameters():
