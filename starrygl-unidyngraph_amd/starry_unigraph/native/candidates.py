@@ -48,7 +48,7 @@ def cross_entropy(h: torch.Tensor, table: torch.Tensor, target: torch.Tensor, *,
         raise ValueError(f"target: {target.dtype} {tuple(target.shape)} on {target.device}, expected int64 "
                          f"{tuple(h.shape[:-1])} on {h.device}")
     _no_tangents(h, table, bias)
-    return _call(rows, table, bias, target.reshape(-1).contiguous(), None, float(scale), 1.0).view(h.shape[:-1])
+    return _shaped(_call(rows, table, bias, target.reshape(-1).contiguous(), None, float(scale), 1.0), h)
 
 
 def distillation(h: torch.Tensor, table: torch.Tensor, ids: torch.Tensor, logits: torch.Tensor, *,
@@ -79,7 +79,7 @@ def distillation(h: torch.Tensor, table: torch.Tensor, ids: torch.Tensor, logits
     _no_grad("logits", logits)
     _no_tangents(h, table, bias, logits)
     entries = (ids.reshape(-1, K).contiguous(), logits.reshape(-1, K).contiguous())
-    return _call(rows, table, bias, None, entries, float(scale), temperature).view(h.shape[:-1])
+    return _shaped(_call(rows, table, bias, None, entries, float(scale), temperature), h)
 
 
 def _check(h, table, bias, scale) -> torch.Tensor:
@@ -111,6 +111,11 @@ def _call(h, table, bias, target, entries, scale, temperature) -> torch.Tensor:
     if _tracked(h, table, bias):
         return _Loss.apply(h, table, bias, target, entries, scale, temperature)
     return _Loss.run(h, table, bias, target, entries, scale, temperature, 0)[0]
+
+
+def _shaped(loss: torch.Tensor, h: torch.Tensor) -> torch.Tensor:
+    """``loss`` [rows] like ``h``'s rows (rows in a line stay: a view is a step of autograd's)."""
+    return loss if h.dim() == 2 else loss.view(h.shape[:-1])
 
 
 def _near(t: torch.Tensor) -> torch.Tensor:
