@@ -316,20 +316,32 @@ struct Plan {
   static constexpr int PER_SIMD = WIDE ? 1 : 2, GROUPS_PER_TWO = sizeof(T) == 4 && !WIDE ? 1 : 2;   // CUs of two
   static constexpr int GROUPS = 512 / GROUPS_PER_TWO;
 };
-// Steps of a product along the channels that are left out where a row ends
-// before them (DB counts rows in 64 channels). fp32 alone: 100 channels of 128 270 -> 250 us;
-// in 16 bits the branch costs what the step does.
+// Steps of a product along the channels that are left out by a branch where a
+// row ends before them (DB counts rows in 64 channels). fp32 alone: 100 channels
+// of 128 270 -> 250 us; in 16 bits the branch costs what the step does (pick_dim's
+// constants).
 template <typename T>
 constexpr int kTrim = sizeof(T) == 4 ? 64 / Mma32<T>::KS - 1 : 0;
-// f(a value of the element type, the row's blocks of 32 as a constant).
+// f(a value of the element type, the row's blocks of 32 as a constant, and of
+// its last 64 channels the steps of 16 past its end that are left out: up to 2, in 16
+// bits; 768 x 570,074 in bf16, forward and gradient: 160 channels of 192 307 + 381 us,
+// 281 + 349 without two, 172 317 + 389 and 308 + 379 without one).
 template <typename F>
 auto pick_dim(int32_t dtype, int D, F &&f) {
+  auto cuts = [&](auto t, auto db) {
+    const int past = sizeof(t) == 4 ? 0 : (32 * db.value - D) / 16;
+    if constexpr (sizeof(t) == 2) {
+      if (past == 1) return f(t, db, std::integral_constant<int, 1>{});
+      if (past >= 2) return f(t, db, std::integral_constant<int, 2>{});
+    }
+    return f(t, db, std::integral_constant<int, 0>{});
+  };
   auto dims = [&](auto t) {
     switch ((D + 63) / 64) {
-      case 1: return f(t, std::integral_constant<int, 2>{});
-      case 2: return f(t, std::integral_constant<int, 4>{});
-      case 3: return f(t, std::integral_constant<int, 6>{});
-      default: return f(t, std::integral_constant<int, 8>{});
+      case 1: return cuts(t, std::integral_constant<int, 2>{});
+      case 2: return cuts(t, std::integral_constant<int, 4>{});
+      case 3: return cuts(t, std::integral_constant<int, 6>{});
+      default: return cuts(t, std::integral_constant<int, 8>{});
     }
   };
   if (dtype == SGL_FP32) return dims(float{});

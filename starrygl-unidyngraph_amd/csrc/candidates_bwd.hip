@@ -39,12 +39,12 @@ struct Tiles {
 };
 
 // A wave has 32 candidates.
-template <typename T, int DB, int WAVES, int PER_SIMD>
+template <typename T, int DB, int CUT, int WAVES, int PER_SIMD>
 __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) {
   using M = Mma32<T>;
   using Im = Tiles<T, DB>;
   constexpr int BLOCK = 64 * WAVES;
-  constexpr int KS = M::KS, DP = 32 * DB, NK = DP / KS, TRIM = kTrim<T>, YT = Im::YT, XT = Im::XT, QL = Im::QL;
+  constexpr int KS = M::KS, DP = 32 * DB, NK = DP / KS - CUT, TRIM = kTrim<T>, OB = DB - CUT / 2, YT = Im::YT, XT = Im::XT, QL = Im::QL;
   using Tl = Tile32<T, DP>;
   constexpr bool HALF = std::is_same_v<T, fp16_t>;
   extern __shared__ __align__(16) char lds[];
@@ -96,9 +96,9 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) 
     const float b2 = p.bias != nullptr ? bias2(p, xr) : 0.f;
     load_outer<T>(xf, static_cast<const T *>(p.table) + xr * p.ts, b2 == -INFINITY, D);
     float db = 0.f, sc = kFirstScale;
-    f32x16 o[DB];
+    f32x16 o[OB];
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+    for (int d = 0; d < OB; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
     const int first = t, end = int(min(int64_t(line.inner), t + (u1 - u)));
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) 
         for (int st = 0; st < 32 / KS; ++st) {
           const FragOf<T> pf = frag_of16<T>(c, st, HALF ? sc : 1.f);
 #pragma unroll
-          for (int d = 0; d < DB; ++d) o[d] = M::mma(Tl::frag_t(tile, 32 * d, row0, st), pf, o[d]);
+          for (int d = 0; d < OB; ++d) o[d] = M::mma(Tl::frag_t(tile, 32 * d, row0, st), pf, o[d]);
         }
         if (a.dbias != nullptr) db += sum16(c);
       }
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) 
       if (!whole) {
         float *row = a.part + (int64_t(w + xt) * XT + wave * 32 + col) * (DP + 4);
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int d = 0; d < OB; ++d)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float y[4];
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) 
       } else {
         T *row = static_cast<T *>(a.dtable) + x * width;
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int d = 0; d < OB; ++d)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             f32x4 y;
@@ -308,13 +308,13 @@ __global__ __launch_bounds__(kRouteBlock) void k_route(RouteArgs a) {
   if (tid == 0) index[a.vblocks] = base;
 }
 
-template <typename T, int DB>
+template <typename T, int DB, int CUT>
 void run(const BwdArgs &a, hipStream_t stream) {
   using P = Plan<T, DB>;
   using Im = Tiles<T, DB>;
   constexpr size_t bytes = size_t(2) * Im::BYTES + sizeof(float) * Im::XT * Im::QL;
   static_assert(bytes <= 160 * 1024 * P::GROUPS_PER_TWO / 2, "LDS of a CU");
-  auto *k = &k_table_grad<T, DB, P::WAVES, P::PER_SIMD>;
+  auto *k = &k_table_grad<T, DB, CUT, P::WAVES, P::PER_SIMD>;
   (void)ensure_dynamic_lds(reinterpret_cast<const void *>(k), bytes);
   const Line line((a.p.V + Im::XT - 1) / Im::XT, (a.p.N + Im::YT - 1) / Im::YT, P::GROUPS);
   launch(k, dim3(unsigned(line.groups)), dim3(64 * P::WAVES), bytes, stream, a);
@@ -329,13 +329,13 @@ namespace sgl {
 namespace cand {
 
 Image grad_image(int32_t dtype, int D) {
-  return pick_dim(dtype, D, [](auto t, auto db) {
+  return pick_dim(dtype, D, [](auto t, auto db, auto) {
     using Im = Tiles<decltype(t), db.value>;
     return Image{Im::YT, Im::LD, Im::BYTES};
   });
 }
 int64_t table_grad_part(int32_t dtype, const Problem &p) {
-  return pick_dim(dtype, p.D, [&](auto t, auto db) {
+  return pick_dim(dtype, p.D, [&](auto t, auto db, auto) {
     using P = Plan<decltype(t), db.value>;
     constexpr int64_t xtile = 32 * P::WAVES;
     return ((p.V + xtile - 1) / xtile + P::GROUPS) * xtile * (32 * db.value + 4);
@@ -352,7 +352,7 @@ void route_targets(int32_t dtype, const Problem &p, int K, const int32_t *ids, c
 void table_grad(int32_t dtype, const Problem &p, const RowCoef &r, void *dtable, float *dbias, float *part,
                 hipStream_t stream) {
   const BwdArgs a{p, r, dtable, dbias, part};
-  pick_dim(dtype, p.D, [&](auto t, auto db) { run<decltype(t), db.value>(a, stream); });
+  pick_dim(dtype, p.D, [&](auto t, auto db, auto cut) { run<decltype(t), db.value, cut.value>(a, stream); });
 }
 
 }  // namespace cand

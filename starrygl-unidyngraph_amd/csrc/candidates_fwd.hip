@@ -30,10 +30,10 @@ constexpr int kBuffers = 2 * YT * Tile32<T, 32 * DB>::LD * int(sizeof(T)) <= 140
 // A wave has 32 rows; WX waves lie along the rows, WY along the table (few rows:
 // each has 32 candidates of a tile of its own, and leaves a partial of its
 // own). SUB steps of 32 candidates a tile.
-template <typename T, int DB, int WX, int WY, int SUB, int PER_SIMD, bool DIR>
+template <typename T, int DB, int CUT, int WX, int WY, int SUB, int PER_SIMD, bool DIR>
 __global__ __launch_bounds__(64 * WX * WY, PER_SIMD) void k_forward(FwdArgs a) {
   using M = Mma32<T>;
-  constexpr int BLOCK = 64 * WX * WY, KS = M::KS, DP = 32 * DB, NK = DP / KS, TRIM = kTrim<T>;
+  constexpr int BLOCK = 64 * WX * WY, KS = M::KS, DP = 32 * DB, NK = DP / KS - CUT, TRIM = kTrim<T>, OB = DB - CUT / 2;
   using Tl = Tile32<T, DP>;
   constexpr int LD = Tl::LD, YT = 32 * SUB * WY, XT = 32 * WX, NBUF = kBuffers<T, DB, YT>;
   extern __shared__ __align__(16) char lds[];
@@ -75,9 +75,9 @@ __global__ __launch_bounds__(64 * WX * WY, PER_SIMD) void k_forward(FwdArgs a) {
     load_outer<T>(xf, static_cast<const T *>(p.h) + a.order.row(min(x, N - 1)) * p.hs, x >= N, D);
     // the maximum, as used, the sum and its compensation (a row's sum has up to 2^15 terms)
     float m = -INFINITY, mu = -kTop<T>, l = 0.f, lc = 0.f;
-    f32x16 o[DIR ? DB : 1];
+    f32x16 o[DIR ? OB : 1];
 #pragma unroll
-    for (int d = 0; d < (DIR ? DB : 1); ++d)
+    for (int d = 0; d < (DIR ? OB : 1); ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
     const int end = int(min(int64_t(line.inner), t + (u1 - u)));
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(64 * WX * WY, PER_SIMD) void k_forward(FwdArgs a) {
           for (int st = 0; st < 32 / KS; ++st) {
             const FragOf<T> pf = frag_of16<T>(s, st);
 #pragma unroll
-            for (int d = 0; d < DB; ++d) o[d] = M::mma(Tl::frag_t(tile, 32 * d, row0, st), pf, o[d]);
+            for (int d = 0; d < OB; ++d) o[d] = M::mma(Tl::frag_t(tile, 32 * d, row0, st), pf, o[d]);
           }
         }
       }
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(64 * WX * WY, PER_SIMD) void k_forward(FwdArgs a) {
       if constexpr (DIR) {
         float *row = a.out.o + at * DP;
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int d = 0; d < OB; ++d)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float q[4];
@@ -175,7 +175,7 @@ Partials shape_of(const Problem &p) {
   s.ytiles = (p.V + ytile - 1) / ytile;
   return s;
 }
-template <typename T, int DB, bool DIR>
+template <typename T, int DB, int CUT, bool DIR>
 void run(const FwdArgs &a, hipStream_t stream) {
   using P = Plan<T, DB>;
   const Line line((a.p.N + a.out.rows - 1) / a.out.rows, a.out.ytiles, a.out.groups);
@@ -188,14 +188,14 @@ void run(const FwdArgs &a, hipStream_t stream) {
   constexpr size_t few_bytes = kBuffers<T, DB, few> * few * row, many_bytes = kBuffers<T, DB, many> * many * row;
   static_assert(few_bytes <= 160 * 1024 && many_bytes <= 160 * 1024 * P::GROUPS_PER_TWO / 2, "LDS of a CU");
   if (a.p.N <= kFewRows)
-    go(&k_forward<T, DB, 1, kFewWaves, 1, P::PER_SIMD, DIR>, 64 * kFewWaves, few_bytes);
+    go(&k_forward<T, DB, 0, 1, kFewWaves, 1, P::PER_SIMD, DIR>, 64 * kFewWaves, few_bytes);
   else
-    go(&k_forward<T, DB, P::WAVES, 1, P::SUB, P::PER_SIMD, DIR>, 64 * P::WAVES, many_bytes);
+    go(&k_forward<T, DB, CUT, P::WAVES, 1, P::SUB, P::PER_SIMD, DIR>, 64 * P::WAVES, many_bytes);
 }
-template <typename T, int DB>
+template <typename T, int DB, int CUT>
 void pick(const FwdArgs &a, hipStream_t stream) {
-  if (a.out.o != nullptr) run<T, DB, true>(a, stream);
-  else run<T, DB, false>(a, stream);
+  if (a.out.o != nullptr) run<T, DB, CUT, true>(a, stream);
+  else run<T, DB, CUT, false>(a, stream);
 }
 
 }  // namespace
@@ -206,12 +206,16 @@ namespace cand {
 int padded_dim(int D) { return (D + 63) / 64 * 64; }
 
 Partials forward_shape(int32_t dtype, const Problem &p) {
-  return pick_dim(dtype, p.D, [&](auto t, auto db) { return shape_of<decltype(t), db.value>(p); });
+  return pick_dim(dtype, p.D, [&](auto t, auto db, auto) { return shape_of<decltype(t), db.value>(p); });
 }
 
 void forward_partials(int32_t dtype, const Problem &p, const Order &order, const Partials &out, hipStream_t stream) {
   const FwdArgs a{p, order, out};
-  pick_dim(dtype, p.D, [&](auto t, auto db) { pick<decltype(t), db.value>(a, stream); });
+  pick_dim(dtype, p.D, [&](auto t, auto db, auto cut) {
+    // (7 of 8 steps are slower than 8: 768 x 570,074 x 104 in bf16 262 us for 239; 6 faster, as 11 of 12 are)
+    constexpr int CUT = db.value == 4 && cut.value == 1 ? 0 : cut.value;
+    pick<decltype(t), db.value, CUT>(a, stream);
+  });
 }
 
 }  // namespace cand
