@@ -1,5 +1,14 @@
 // Softmax over all candidates: each row's maximum and sum over a piece of the
 // table and, for training, sum_v p_v w_v of that piece.
+//
+// One pass over the table: a tile of it gives scores, the running maximum and
+// sum (what was summed is rescaled when the maximum has grown), and the tile's
+// share of sum p w. 2 N V D operations, 4 with sum p w: the matrix unit
+// bounds it, at the rate that the card's power leaves (a large library product
+// 1,099 TFLOP/s in bf16): 4,096 x 570,074 x 172 in bf16 1,557 us, 1,032; rows of
+// 100 channels 786 (7 and 8 steps of 16 are run for 6.25); 600 x 100,000 x 172 in
+// fp32 400 us, 103 of 152. A few rows: the table's bytes, 1 x 1,140,149 x 172 in 72
+// us, 5.4 TB/s.
 #include "candidates.h"
 
 namespace {
@@ -162,15 +171,29 @@ __global__ __launch_bounds__(64 * WX * WY, PER_SIMD) void k_forward(FwdArgs a) {
 // Up to here a workgroup's waves share the rows and split the table.
 constexpr int64_t kFewRows = 32;
 constexpr int kFewWaves = 4;
+// 16-bit rows in two workgroups a CU of four waves, where tiles of 128 rows
+// leave out a sixth of what tiles of 256 take (600 rows: 640 of 768). Each
+// then reads the table for half as many rows. 570,074 x 172 in bf16, 256 / 128: 100
+// rows 110 / 84 us, 384 202 / 184, 600 299 / 283, 512 218 / 233, 1,200 512 / 548; not
+// beyond 192 channels (their registers spill there: 600 x 256 499 / 825).
+template <typename T, int DB>
+struct Half {
+  static constexpr bool AT_ALL = sizeof(T) == 2 && DB <= 6;
+  static constexpr int WAVES = 4, GROUPS = 512;
+  static bool takes(int64_t N) {
+    const int64_t whole = (N + 255) / 256 * 256, halves = (N + 127) / 128 * 128;
+    return AT_ALL && 6 * halves <= 5 * whole;
+  }
+};
 template <typename T, int DB>
 Partials shape_of(const Problem &p) {
   using P = Plan<T, DB>;
   Partials s{};
-  const bool few = p.N <= kFewRows;
-  s.rows = few ? 32 : 32 * P::WAVES;
+  const bool few = p.N <= kFewRows, half = !few && Half<T, DB>::takes(p.N);
+  s.rows = few ? 32 : 32 * (half ? Half<T, DB>::WAVES : P::WAVES);
   s.wy = few ? kFewWaves : 1;
   s.dp = 32 * DB;
-  s.groups = few ? 256 : P::GROUPS;
+  s.groups = few ? 256 : half ? Half<T, DB>::GROUPS : P::GROUPS;
   const int ytile = few ? 32 * kFewWaves : 32 * P::SUB;
   s.ytiles = (p.V + ytile - 1) / ytile;
   return s;
@@ -178,6 +201,7 @@ Partials shape_of(const Problem &p) {
 template <typename T, int DB, int CUT, bool DIR>
 void run(const FwdArgs &a, hipStream_t stream) {
   using P = Plan<T, DB>;
+  using H = Half<T, DB>;
   const Line line((a.p.N + a.out.rows - 1) / a.out.rows, a.out.ytiles, a.out.groups);
   auto go = [&](auto *k, int threads, size_t bytes) {
     (void)ensure_dynamic_lds(reinterpret_cast<const void *>(k), bytes);
@@ -187,10 +211,17 @@ void run(const FwdArgs &a, hipStream_t stream) {
   constexpr int few = 32 * kFewWaves, many = 32 * P::SUB;
   constexpr size_t few_bytes = kBuffers<T, DB, few> * few * row, many_bytes = kBuffers<T, DB, many> * many * row;
   static_assert(few_bytes <= 160 * 1024 && many_bytes <= 160 * 1024 * P::GROUPS_PER_TWO / 2, "LDS of a CU");
-  if (a.p.N <= kFewRows)
+  static_assert(!H::AT_ALL || many_bytes <= 80 * 1024, "two workgroups a CU");
+  if (a.p.N <= kFewRows) {
     go(&k_forward<T, DB, 0, 1, kFewWaves, 1, P::PER_SIMD, DIR>, 64 * kFewWaves, few_bytes);
-  else
-    go(&k_forward<T, DB, CUT, P::WAVES, 1, P::SUB, P::PER_SIMD, DIR>, 64 * P::WAVES, many_bytes);
+    return;
+  }
+  if constexpr (H::AT_ALL)
+    if (H::takes(a.p.N)) {
+      go(&k_forward<T, DB, CUT, H::WAVES, 1, P::SUB, P::PER_SIMD, DIR>, 64 * H::WAVES, many_bytes);
+      return;
+    }
+  go(&k_forward<T, DB, CUT, P::WAVES, 1, P::SUB, P::PER_SIMD, DIR>, 64 * P::WAVES, many_bytes);
 }
 template <typename T, int DB, int CUT>
 void pick(const FwdArgs &a, hipStream_t stream) {

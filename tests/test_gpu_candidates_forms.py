@@ -26,6 +26,11 @@ FORMS = [  # N, V, D, dtype, bias: the last channels' steps of 16 left out (0, 1
     (300, 300, 239, BF16, True),
     (300, 300, 104, FP32, True),
     (300, 300, 185, FP32, False),
+    # whole and half tiles of rows
+    (250, 500, 90, BF16, True),
+    (250, 500, 172, FP16, False),
+    (1100, 200, 160, BF16, True),
+    (100, 500, 172, BF16, True),
     # pieces of the table and of the rows shared by workgroups, ragged at both ends
     (600, 20011, 100, BF16, False),
     (270, 40003, 172, FP16, True),
