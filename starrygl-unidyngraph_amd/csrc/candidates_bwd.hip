@@ -44,8 +44,12 @@ struct Tiles {
   static_assert(BYTES % 1024 == 0, "whole loads of a wave");
 };
 
-// A wave has 32 candidates.
-template <typename T, int DB, int CUT, int WAVES, int PER_SIMD>
+// A wave has 32 candidates. What the tile's rows want of them is added behind
+// the scores: a label a row, in the image (TEACHER false), or a teacher's
+// entries, which are asked for before the scores and land while these are formed
+// (1,200 x 1,140,149 x 172 in bf16, 64 entries a row: 1,309 us with their loads
+// where they are used, 1,178 so).
+template <typename T, int DB, int CUT, int WAVES, int PER_SIMD, bool TEACHER>
 __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) {
   using M = Mma32<T>;
   using Im = Tiles<T, DB>;
@@ -82,7 +86,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) 
     for (int i = 0; i < NL; ++i)
       if (loads(i))
         __builtin_amdgcn_global_load_lds((Global)(src + i * 16 * BLOCK), (Lds)(dst + i * 16 * BLOCK), 16, 0, 0);
-    if (a.r.index != nullptr) {
+    if constexpr (TEACHER) {
       const int64_t vb = int64_t(xt) * WAVES + wave;
       const int32_t *at = a.r.index + int64_t(t) * (a.r.vblocks + 1) + min(vb, a.r.vblocks - 1);
       ne0 = attn::scalar_load(at);
@@ -120,20 +124,18 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) 
       __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this wave's part of the tile has landed
       __syncthreads();
       // what the tile's rows want of the wave's candidates: a row has a candidate once, so each place once
-      const int id = a.r.index == nullptr && lane < YT ? reinterpret_cast<const int *>(cf)[3 * YT + lane] : -1;
+      const int id = !TEACHER && lane < YT ? reinterpret_cast<const int *>(cf)[3 * YT + lane] : -1;
       const int mine = id - (xt * XT + wave * 32);
       const bool one = id >= 0 && uint32_t(mine) < 32u;
-      const bool wanted = __any(one) || e0 < e1;
+      const bool wanted = TEACHER ? e0 < e1 : __any(one);
+      int2 entry = make_int2(-1, 0);   // the lane's of the first 64: on its way while the scores are formed
+      if (TEACHER && e0 + lane < e1) entry = entries[e0 + lane];
       if (t + 1 < end || u < u1) fetch(t + 1 < end ? t + 1 : 0, t + 1 < end ? xt : xt + 1, buf);
 #pragma unroll 1
       for (int ys = 0; ys < Im::SUB; ++ys) {
         const int row0 = ys * 32;
-        if (wanted) {
+        if (!TEACHER && wanted) {
           if (one && (lane >> 5) == ys) q[mine * QL + (lane & 31)] = 1.f;
-          for (int k = e0 + lane; k < e1; k += kWave) {
-            const int2 e = entries[k];
-            if (((e.x >> 5) & 1) == ys) q[(e.x >> 6) * QL + (e.x & 31)] = __int_as_float(e.y);
-          }
           attn::wave_sync();
         }
         f32x16 s;
@@ -152,6 +154,16 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) 
           for (int v = 0; v < 4; ++v) c[4 * i + v] = exp2_fast(fmaf(s[4 * i + v], p.c, b2) + nm[v]) * gl[v];
         }
         if (wanted) {
+          const bool first = entry.x >= 0 && ((entry.x >> 5) & 1) == ys;
+          float *to = q + (entry.x >> 6) * QL + (entry.x & 31);
+          if constexpr (TEACHER) {
+            if (first) *to = __int_as_float(entry.y);
+            for (int k = e0 + kWave + lane; k < e1; k += kWave) {
+              const int2 e = entries[k];
+              if (((e.x >> 5) & 1) == ys) q[(e.x >> 6) * QL + (e.x & 31)] = __int_as_float(e.y);
+            }
+            attn::wave_sync();
+          }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float gq[4], y[4];
@@ -161,10 +173,14 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) 
             for (int v = 0; v < 4; ++v) c[4 * i + v] = fmaf(-gq[v], y[v], c[4 * i + v]);
           }
           attn::wave_sync();
-          if (one && (lane >> 5) == ys) q[mine * QL + (lane & 31)] = 0.f;
-          for (int k = e0 + lane; k < e1; k += kWave) {
-            const int e = entries[k].x;
-            if (((e >> 5) & 1) == ys) q[(e >> 6) * QL + (e & 31)] = 0.f;
+          if constexpr (TEACHER) {
+            if (first) *to = 0.f;
+            for (int k = e0 + kWave + lane; k < e1; k += kWave) {
+              const int e = entries[k].x;
+              if (((e >> 5) & 1) == ys) q[(e >> 6) * QL + (e & 31)] = 0.f;
+            }
+          } else if (one && (lane >> 5) == ys) {
+            q[mine * QL + (lane & 31)] = 0.f;
           }
         }
         if constexpr (HALF) {
@@ -256,9 +272,11 @@ __global__ __launch_bounds__(kBlock) void k_join_grad(BwdArgs a, int xtile, int 
 
 // ------------------------------------------------------------------ several targets a row
 // A row tile's entries in the order of the candidates' blocks (those of a
-// wave), with the place where each block begins: one workgroup a row tile
-// counts, sums and places them in LDS, kBins blocks at a time. (The order of a
-// block's entries varies; each is a place of its own.)
+// wave), with the place where each block begins: a workgroup a row tile and
+// kBins blocks counts, sums and places the entries of its blocks in LDS, behind
+// those of earlier ones. (The order of a block's entries varies; each is a
+// place of its own.) 64 x 64 entries over 35,630 blocks: 28 us with one workgroup
+// a row tile, 12 so.
 constexpr int kRouteBlock = 1024, kBins = 12 * kRouteBlock;
 struct RouteArgs {
   const int32_t *ids;     // [N][K]
@@ -272,46 +290,43 @@ __global__ __launch_bounds__(kRouteBlock) void k_route(RouteArgs a) {
   __shared__ int bins[kBins];
   __shared__ int waves[kRouteBlock / kWave];
   const int tid = threadIdx.x;
-  const int64_t y0 = int64_t(blockIdx.x) * a.ytile, e0 = y0 * a.K;
+  const int64_t y0 = int64_t(blockIdx.x) * a.ytile, e0 = y0 * a.K, b0 = int64_t(blockIdx.y) * kBins;
   const int n = int(min(int64_t(a.ytile), a.N - y0)) * a.K;
   int32_t *index = a.index + int64_t(blockIdx.x) * (a.vblocks + 1);
   int2 *entries = a.entries + int64_t(blockIdx.x) * a.ytile * a.K;
-  int base = 0;
-  for (int64_t b0 = 0; b0 < a.vblocks; b0 += kBins) {
-    for (int i = tid; i < kBins; i += kRouteBlock) bins[i] = 0;
-    __syncthreads();
-    for (int e = tid; e < n; e += kRouteBlock) {
-      const int id = a.ids[e0 + e];
-      const int64_t b = id / a.vblock - b0;
-      if (id >= 0 && b >= 0 && b < kBins) atomicAdd(&bins[b], 1);
-    }
-    __syncthreads();
-    constexpr int PER = kBins / kRouteBlock;
-    int c[PER], sum = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      c[i] = sum;
-      sum += bins[tid * PER + i];
-    }
-    int total;
-    const int before = base + block_exclusive_scan<int, kRouteBlock>(sum, waves, total);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      bins[tid * PER + i] = before + c[i];
-      if (b0 + tid * PER + i <= a.vblocks) index[b0 + tid * PER + i] = before + c[i];
-    }
-    __syncthreads();
-    for (int e = tid; e < n; e += kRouteBlock) {
-      const int id = a.ids[e0 + e];
-      const int64_t b = id / a.vblock - b0;
-      if (id >= 0 && b >= 0 && b < kBins)
-        entries[atomicAdd(&bins[b], 1)] =
-            make_int2((id - int(b0 + b) * a.vblock) * 64 + e / a.K, __float_as_int(a.weight[e0 + e]));
-    }
-    base += total;
-    __syncthreads();
+  for (int i = tid; i < kBins; i += kRouteBlock) bins[i] = 0;
+  __syncthreads();
+  int earlier = 0;
+  for (int e = tid; e < n; e += kRouteBlock) {
+    const int id = a.ids[e0 + e];
+    const int64_t b = id / a.vblock - b0;
+    if (id >= 0 && b < 0) ++earlier;
+    if (id >= 0 && b >= 0 && b < kBins) atomicAdd(&bins[b], 1);
   }
-  if (tid == 0) index[a.vblocks] = base;
+  int base, total;
+  block_exclusive_scan<int, kRouteBlock>(earlier, waves, base);
+  constexpr int PER = kBins / kRouteBlock;
+  int c[PER], sum = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    c[i] = sum;
+    sum += bins[tid * PER + i];
+  }
+  const int before = base + block_exclusive_scan<int, kRouteBlock>(sum, waves, total);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    bins[tid * PER + i] = before + c[i];
+    if (b0 + tid * PER + i < a.vblocks) index[b0 + tid * PER + i] = before + c[i];
+  }
+  if (tid == 0 && blockIdx.y == gridDim.y - 1) index[a.vblocks] = base + total;
+  __syncthreads();
+  for (int e = tid; e < n; e += kRouteBlock) {
+    const int id = a.ids[e0 + e];
+    const int64_t b = id / a.vblock - b0;
+    if (id >= 0 && b >= 0 && b < kBins)
+      entries[atomicAdd(&bins[b], 1)] =
+          make_int2((id - int(b0 + b) * a.vblock) * 64 + e / a.K, __float_as_int(a.weight[e0 + e]));
+  }
 }
 
 template <typename T, int DB, int CUT>
@@ -320,7 +335,8 @@ void run(const BwdArgs &a, hipStream_t stream) {
   using Im = Tiles<T, DB>;
   constexpr size_t bytes = size_t(2) * Im::BYTES + sizeof(float) * Im::XT * Im::QL;
   static_assert(bytes <= 160 * 1024 * P::GROUPS_PER_TWO / 2, "LDS of a CU");
-  auto *k = &k_table_grad<T, DB, CUT, P::WAVES, P::PER_SIMD>;
+  auto *k = a.r.index != nullptr ? &k_table_grad<T, DB, CUT, P::WAVES, P::PER_SIMD, true>
+                                 : &k_table_grad<T, DB, CUT, P::WAVES, P::PER_SIMD, false>;
   (void)ensure_dynamic_lds(reinterpret_cast<const void *>(k), bytes);
   const Line line((a.p.V + Im::XT - 1) / Im::XT, (a.p.N + Im::YT - 1) / Im::YT, P::GROUPS);
   launch(k, dim3(unsigned(line.groups)), dim3(64 * P::WAVES), bytes, stream, a);
@@ -352,7 +368,8 @@ void route_targets(int32_t dtype, const Problem &p, int K, const int32_t *ids, c
                    int2 *entries, hipStream_t stream) {
   const int yt = grad_image(dtype, p.D).rows;
   const RouteArgs a{ids, weight, p.N, (p.V + kGradBlock - 1) / kGradBlock, K, yt, kGradBlock, index, entries};
-  launch(&k_route, dim3(unsigned((p.N + yt - 1) / yt)), dim3(kRouteBlock), 0, stream, a);
+  launch(&k_route, dim3(unsigned((p.N + yt - 1) / yt), unsigned((a.vblocks + kBins - 1) / kBins)), dim3(kRouteBlock), 0,
+         stream, a);
 }
 
 void table_grad(int32_t dtype, const Problem &p, const RowCoef &r, void *dtable, float *dbias, float *part,
