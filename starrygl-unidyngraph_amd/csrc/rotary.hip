@@ -9,9 +9,8 @@
 //
 // Memory bounds it, every element read and written once: 16 sequences of 8,191
 // x (8 + 2) heads of 128 in fp16 120 us, 5.6 TB/s (a large copy: 5.1); 4,000 x
-// (20 + 32) x 4 heads of 43 in bf16, odd rows of 86 bytes, 41 us when just
-// written and 57 from memory; 400
-// x 1 x 2 heads of 50, one new event each, 4 us, the launch.
+// (20 + 32) x 4 heads of 43 in bf16 30 us, 4.7 TB/s; 400 x 1 x 2 heads of 50, one
+// new event each, 4 us, the launch.
 #include "history.h"
 
 namespace {
@@ -67,6 +66,18 @@ __device__ __forceinline__ uint64_t turn_step(double f) {
   return fraction(hi) + fraction(lo);
 }
 
+// a cos - b sin and a sin + b cos, rounded to 32 bits before the type's (one
+// rounding less in some places and not in others would give lanes that write the
+// same channel different bits).
+template <typename T>
+__device__ __forceinline__ void turn(T &a, T &b, float sn, float cs) {
+  const float p = float(a), q = float(b);
+  float x = fmaf(p, cs, -(q * sn)), y = fmaf(p, sn, q * cs);
+  asm("" : "+v"(x), "+v"(y));
+  a = T(x);
+  b = T(y);
+}
+
 // A workgroup forms the frequencies' steps once where they are few (SHARED: up
 // to kSteps pairs; 64-bit floating point of every lane
 // otherwise: one head of 172 in fp16 38 us for 57, two of 100 with 64 turned 39
@@ -74,7 +85,7 @@ __device__ __forceinline__ uint64_t turn_step(double f) {
 // A lane owns VEC consecutive channels of a row (both halves' in the half
 // layout) for all its heads; the angles are formed once for all of them. A
 // part's last lane takes its last VEC channels, some of them its neighbour's
-// too (it writes the same bits: each product and sum is rounded as written), so
+// too (it writes the same bits), so
 // that loads and stores are all whole (4 heads of 44 in bf16: 123 us with the
 // last ones one by one, 30 so); channels that are not rotated and fewer than VEC
 // go one by one.
@@ -121,32 +132,91 @@ __global__ __launch_bounds__(kBlock) void k_rotate(RotArgs a) {
     sn[i] *= a.gain * a.way;
     cs[i] *= a.gain;
   }
-#pragma unroll 4
   for (int h = 0; h < s.H; ++h, x += s.sh, y += a.dh) {
     if constexpr (INTER) {
       T v[VEC];
       load_n(v, x + 2 * p0);
 #pragma unroll
-      for (int i = 0; i < PV; ++i) {
-        const float p = float(v[2 * i]), q = float(v[2 * i + 1]);
-        v[2 * i] = T(fmaf(p, cs[i], -(q * sn[i])));
-        v[2 * i + 1] = T(fmaf(p, sn[i], q * cs[i]));
-      }
+      for (int i = 0; i < PV; ++i)
+        turn(v[2 * i], v[2 * i + 1], sn[i], cs[i]);
       store_n(y + 2 * p0, v);
     } else {
       T v[VEC], w[VEC];
       load_n(v, x + p0);
       load_n(w, x + half + p0);
 #pragma unroll
-      for (int i = 0; i < PV; ++i) {
-        const float p = float(v[i]), q = float(w[i]);
-        v[i] = T(fmaf(p, cs[i], -(q * sn[i])));
-        w[i] = T(fmaf(p, sn[i], q * cs[i]));
-      }
+      for (int i = 0; i < PV; ++i)
+        turn(v[i], w[i], sn[i], cs[i]);
       store_n(y + p0, v);
       store_n(y + half + p0, w);
     }
   }
+}
+
+// Heads of an odd number of channels, whose rows lie one behind the other: a
+// workgroup's rows as one stretch, in and out 16 bytes at a time and turned in LDS
+// (a lane's own loads and stores would straddle). 4,000 x (20 + 32) x 4 heads of 43,
+// interleaved, in bf16 30 us for 41, in fp32 58 for 104, 8 heads of 127 in bf16 166
+// for 279; 200 x (20 + 32) x 4 of 43 6.0 for 5.5: taken where there are two
+// workgroups a CU.
+constexpr int kStretchRows = 256;
+template <typename T>
+constexpr int kStretch = 16384 / int(sizeof(T));   // elements of a workgroup's rows
+template <typename T, bool INTER>
+__global__ __launch_bounds__(kBlock) void k_rotate_odd(RotArgs a, int tile_rows) {
+  __shared__ __align__(16) T tile[kStretch<T>];
+  __shared__ uint64_t steps[kSteps];
+  __shared__ int64_t pos[kStretchRows];
+  const int sd = int64_t(blockIdx.x) >= a.side[1].first ? 1 : 0, tid = threadIdx.x;
+  const Side &s = a.side[sd];
+  const int64_t row0 = (int64_t(blockIdx.x) - s.first) * tile_rows;
+  const int rows = int(min(int64_t(tile_rows), s.rows - row0)), width = s.H * a.dh, n = rows * width, half = a.rot / 2;
+  const T *x = static_cast<const T *>(s.x) + row0 * width;
+  T *y = static_cast<T *>(s.y) + row0 * width;
+  constexpr int E = 16 / int(sizeof(T));
+  auto copy = [&](T *to, const T *from) {
+    for (int i = tid * E; i + E <= n; i += kBlock * E) {
+      T v[E];
+      load_n(v, from + i);
+      store_n(to + i, v);
+    }
+    for (int i = n / E * E + tid; i < n; i += kBlock) to[i] = from[i];
+  };
+  copy(tile, x);
+  for (int i = tid; i < half; i += kBlock) steps[i] = turn_step(a.freqs[i]);
+  for (int i = tid; i < rows; i += kBlock) {
+    const int64_t seq = (row0 + i) / s.L, t = row0 + i - seq * s.L;
+    pos[i] = s.pos[seq * s.pn + t * s.pt];
+  }
+  __syncthreads();
+  for (int i = tid; i < rows * half; i += kBlock) {
+    const int r = i / half, p = i - r * half;
+    float sn, cs;
+    sincos_turns(uint64_t(pos[r]) * steps[p], sn, cs);
+    sn *= a.gain * a.way;
+    cs *= a.gain;
+    T *v = tile + r * width + (INTER ? 2 * p : p);
+    constexpr int one = INTER ? 1 : 0;
+    const int other = one != 0 ? 1 : half;
+    for (int h = 0; h < s.H; ++h, v += a.dh) turn(v[0], v[other], sn, cs);
+  }
+  __syncthreads();
+  copy(y, tile);
+}
+// Rows of a workgroup (16 bytes each workgroup's start), or 0: not of that kind.
+template <typename T>
+int odd_rows(const RotArgs &a) {
+  if (a.dh % 2 == 0 || a.rot == 0) return 0;
+  int most = kStretchRows;
+  int64_t all = 0;
+  for (const Side &s : a.side) {
+    if (s.rows == 0) continue;
+    const int64_t width = int64_t(s.H) * a.dh;
+    if (width > kStretch<T> / 8 || s.sh != a.dh || s.st != width || (s.sn != s.L * width && s.rows != s.L)) return 0;
+    most = min(most, int(kStretch<T> / width) / 8 * 8);
+    all += s.rows;
+  }
+  return all / most >= 512 ? most : 0;
 }
 
 template <typename T, int VEC, bool INTER>
@@ -158,6 +228,18 @@ template <typename T, bool INTER>
 int run(RotArgs a, hipStream_t stream) {
   constexpr int MOST = (INTER ? 16 : 8) / int(sizeof(T)), LEAST = INTER ? 2 : 1;
   const int half = a.rot / 2;
+  if (const int rows = odd_rows<T>(a)) {
+    int64_t grid = 0;
+    for (int i = 0; i < 2; ++i) {
+      a.side[i].first = grid;
+      grid += (a.side[i].rows + rows - 1) / rows;
+    }
+    if (a.side[1].rows == 0) a.side[1].first = INT64_MAX;
+    SGL_REQUIRE(grid < (1 << 24), "rotary: too many rows");
+    launch(&k_rotate_odd<T, INTER>, dim3(unsigned(grid)), dim3(kBlock), 0, stream, a, rows);
+    SGL_CHECK_LAUNCH();
+    return SGL_OK;
+  }
   // A lane moves 16 bytes at a time (two loads of 8 in the half layout), or half
   // of that where rows are not whole words (4 heads of 43 in bf16, interleaved 54 us
   // with 16 bytes and 43 with 8, halves 53 with 8 and 45 with 4; 44 channels: 30

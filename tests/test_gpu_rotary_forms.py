@@ -23,6 +23,13 @@ FORMS = [  # N, L, H, dh, pairs, dtype
     (2, 3, 1, 1030, 515, FP16),   # more pairs than a workgroup keeps
     (2, 3, 1, 1031, 513, FP32),
     (40, 31, 1, 100, 32, BF16),   # several workgroups
+    # rows of an odd number of channels, many: turned in LDS, stretches that end anywhere
+    (601, 35, 3, 43, 21, BF16),
+    (700, 41, 1, 43, 16, FP16),
+    (257, 33, 2, 127, 63, FP16),
+    (600, 251, 1, 3, 1, BF16),
+    (300, 43, 2, 43, 21, FP32),
+    (150, 41, 1, 121, 5, FP32),
 ]
 
 
