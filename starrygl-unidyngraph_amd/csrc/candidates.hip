@@ -425,6 +425,8 @@ int make_problem(const sgl_candidates *c, Problem &p) {
   p.temperature = c->temperature;
   p.c = float(double(c->scale) * 1.4426950408889634 / double(c->temperature));
   p.cb = float(1.4426950408889634 / double(c->temperature));
+  SGL_REQUIRE(p.c - p.c == 0.f && p.cb < INFINITY && p.temperature * p.temperature < INFINITY,
+              "candidates: scale %g over temperature %g is out of range", double(c->scale), double(c->temperature));
   return SGL_OK;
 }
 

@@ -20,10 +20,10 @@ import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from starry_unigraph.lib import _capi
-from starry_unigraph.native.history import _as_rows, _first, _guard, _no_grad, _no_tangents, _rows, _tensor, _tracked
+from starry_unigraph.native.history import (_as_rows, _first, _first_order, _guard, _no_grad, _no_tangents, _rows,
+                                            _tensor, _tracked)
 
 MAX_DIM = 256       # channels of a row
 MAX_TARGETS = 1024  # a teacher's entries of a row
@@ -69,6 +69,8 @@ def distillation(h: torch.Tensor, table: torch.Tensor, ids: torch.Tensor, logits
     temperature = float(temperature)
     if not (0.0 < temperature < math.inf):
         raise ValueError(f"temperature: {temperature}, expected a positive number")
+    if not max(abs(scale), 1.0) / temperature < 2e38 or not temperature < 1e19:
+        raise ValueError(f"temperature: {temperature} with a scale of {scale} is out of float32's range")
     if ids.dtype != torch.int64 or ids.dim() != h.dim() or ids.shape[:-1] != h.shape[:-1] or ids.device != h.device:
         raise ValueError(f"ids: {ids.dtype} {tuple(ids.shape)} on {ids.device}, expected int64 "
                          f"[{', '.join(str(n) for n in h.shape[:-1])}, K] on {h.device}")
@@ -96,7 +98,7 @@ def _check(h, table, bias, scale) -> torch.Tensor:
         raise ValueError("table: no candidates")
     if bias is not None:
         _tensor("bias", bias, h, (V,), torch.float32)
-    if not math.isfinite(scale):
+    if not abs(scale) < 2e38:   # (float32's range, with log2 e)
         raise ValueError(f"scale: {scale}")
     return _as_rows(h) if h.dim() != 1 else h.unsqueeze(0)
 
@@ -129,14 +131,14 @@ class _Loss(torch.autograd.Function):
     def forward(ctx, h, table, bias, target, entries, scale, temperature):
         # the gradients that will be asked for: 1 of the rows, 2 of the table and bias
         need = int(h.requires_grad) + 2 * int(table.requires_grad or (bias is not None and bias.requires_grad))
-        loss, saved, K = _Loss.run(h, table, bias, target, entries, scale, temperature, need)
+        loss, saved, K, room = _Loss.run(h, table, bias, target, entries, scale, temperature, need)
         ctx.save_for_backward(*saved)
-        ctx.form = (scale, temperature, K, entries is not None, need)
+        ctx.form = (scale, temperature, K, entries is not None, need, room)
         return loss
 
     @staticmethod
     def run(h, table, bias, target, entries, scale, temperature, need):
-        """(loss, the backward's tensors, targets a row)."""
+        """(loss, the backward's tensors, targets a row, bytes of the backward's workspace)."""
         lib, P, dev = _capi.lib(), _capi.ptr, h.device
         h, table = _near(h), _near(table)
         bias = None if bias is None else bias.contiguous()
@@ -152,7 +154,7 @@ class _Loss(torch.autograd.Function):
         with _guard(dev):
             _capi.check(lib.sgl_candidates_forward(a, P(target), P(ids), P(logits), K, need, P(loss), P(keep), nk, P(ws), nb,
                                                    _capi.stream_of(dev)), "distillation" if teacher else "cross_entropy")
-        return loss, (h, table, bias, keep), K
+        return loss, (h, table, bias, keep), K, lib.sgl_candidates_workspace_bytes(a, K, teacher, need, 1) if need else 0
 
     @staticmethod
     def problem(h, table, bias, scale, temperature):
@@ -161,10 +163,10 @@ class _Loss(torch.autograd.Function):
                                 h.stride(0), table.stride(0), P(bias), scale, temperature)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, g):
         h, table, bias, keep = ctx.saved_tensors
-        scale, temperature, K, teacher, need = ctx.form
+        scale, temperature, K, teacher, need, room = ctx.form
         lib, P, dev = _capi.lib(), _capi.ptr, h.device
         # (from the tensors as they are now: a hook on saved tensors may bring them back elsewhere)
         a = ctypes.byref(_Loss.problem(h, table, bias, scale, temperature))
@@ -173,7 +175,7 @@ class _Loss(torch.autograd.Function):
         dh = torch.empty(h.shape, dtype=h.dtype, device=dev) if want[0] else None
         dt = torch.empty(table.shape, dtype=table.dtype, device=dev) if want[1] or want[2] else None
         db = torch.empty_like(bias) if want[2] else None
-        nb = lib.sgl_candidates_workspace_bytes(a, K, teacher, need, 1) if dt is not None else 0
+        nb = room if dt is not None else 0
         ws = _capi.workspace(nb, dev) if nb else None
         with _guard(dev):
             _capi.check(lib.sgl_candidates_backward(a, K, teacher, need, P(keep), keep.numel(), P(g), P(dh), P(dt), P(db),

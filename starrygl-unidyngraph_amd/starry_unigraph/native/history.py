@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 
 import torch
@@ -30,11 +31,25 @@ from torch.autograd.function import once_differentiable
 from starry_unigraph.lib import _capi
 
 _NO_GUARD = contextlib.nullcontext()
+# (torch.cuda.current_device() less its layers: a call's host time counts)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _guard(dev: torch.device):
     """The device's context, where it is not the current one already."""
-    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _NO_GUARD if dev.index == _current_device() else torch.cuda.device(dev)
+
+
+def _first_order(backward):
+    """once_differentiable, with its work only where gradients of gradients are
+    recorded (a backward pass runs on autograd's own thread, where each step of
+    Python costs several times what it does elsewhere)."""
+    recorded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def _tensor(name: str, t, like: torch.Tensor, shape: tuple, dtype=None) -> torch.Tensor:

@@ -15,10 +15,9 @@ import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from starry_unigraph.lib import _capi
-from starry_unigraph.native.history import _first, _guard, _no_tangents, _rows, _tensor, _tracked
+from starry_unigraph.native.history import _first, _first_order, _guard, _no_tangents, _rows, _tensor, _tracked
 
 
 def frequencies(dims: int, *, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
@@ -125,7 +124,7 @@ class _Rotate(torch.autograd.Function):
         return tuple(outs)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, gq, gk):
         if gq is None and gk is None:
             return (None,) * 7

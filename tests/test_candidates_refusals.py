@@ -207,3 +207,12 @@ def test_entry_points_refuse_their_arrays():
         assert lib.sgl_rotary(*args, None) != 0, args
     side.y = None
     assert lib.sgl_rotary(0, 2, 8, 8, s, None, 4096, 0, 1.0, 0, None) != 0
+
+
+@pytest.mark.parametrize("scale, temperature", [(1.0, 1e-39), (1e30, 1e-20), (1.0, 1e20), (3e38, 1.0)])
+def test_factors_beyond_float32_are_refused(anywhere, scale, temperature):
+    with pytest.raises(ValueError, match="temperature|scale"):
+        candidates.distillation(_f(2, 8), _f(5, 8), _i(2, 4), _f(2, 4), scale=scale, temperature=temperature)
+    lib, ref = _capi.lib(), ctypes.byref(_problem(scale=scale, temperature=temperature))
+    assert lib.sgl_candidates_forward(ref, 4096, None, None, 1, 3, 4096, 4096, 1 << 40, 4096, 1 << 40, None) != 0
+    assert b"temperature" in lib.sgl_last_error()
