@@ -17,6 +17,7 @@ an event against one drawn negative
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -126,58 +127,78 @@ def _near(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(0) <= MAX_STRIDE else t.contiguous()
 
 
+@functools.lru_cache(maxsize=256)
+def _bytes(dtype: int, dim: int, n: int, v: int, K: int, teacher: bool, need: int) -> tuple[int, int, int]:
+    """What the forward keeps for the backward, its workspace, the backward's."""
+    lib = _capi.lib()
+    a = ctypes.byref(_capi.Candidates(dtype, dim, n, v, 16, 16, dim, dim, None, 1.0, 1.0))   # (never read)
+    return (lib.sgl_candidates_keep_bytes(a, K, teacher, need), lib.sgl_candidates_workspace_bytes(a, K, teacher, need, 0),
+            lib.sgl_candidates_workspace_bytes(a, K, teacher, need, 1) if need else 0)
+
+
+# (Few steps of Python from here: they bound a training call of a small batch, and
+# take twice as long on the thread that autograd runs the backward on.)
+def _at(h, table, bias) -> tuple:
+    return h.data_ptr(), table.data_ptr(), h.stride(0), table.stride(0), None if bias is None else bias.data_ptr()
+
+
+def _problem(h, table, at, scale, temperature):
+    return ctypes.byref(_capi.Candidates(_capi.DTYPES[h.dtype], h.shape[1], h.shape[0], table.shape[0], *at, scale,
+                                         temperature))
+
+
 class _Loss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, table, bias, target, entries, scale, temperature):
         # the gradients that will be asked for: 1 of the rows, 2 of the table and bias
         need = int(h.requires_grad) + 2 * int(table.requires_grad or (bias is not None and bias.requires_grad))
-        loss, saved, K, room = _Loss.run(h, table, bias, target, entries, scale, temperature, need)
+        loss, saved, ctx.form = _Loss.run(h, table, bias, target, entries, scale, temperature, need)
         ctx.save_for_backward(*saved)
-        ctx.form = (scale, temperature, K, entries is not None, need, room)
         return loss
 
     @staticmethod
     def run(h, table, bias, target, entries, scale, temperature, need):
-        """(loss, the backward's tensors, targets a row, bytes of the backward's workspace)."""
-        lib, P, dev = _capi.lib(), _capi.ptr, h.device
+        """(loss, the backward's tensors, its other values)."""
+        dev = h.device
         h, table = _near(h), _near(table)
-        bias = None if bias is None else bias.contiguous()
+        if bias is not None:
+            bias = bias.contiguous()
         teacher = entries is not None
-        ids, logits = entries if teacher else (None, None)
-        K = ids.shape[1] if teacher else 1
-        a = ctypes.byref(_Loss.problem(h, table, bias, scale, temperature))
+        K, ids, logits = 1, None, None
+        if teacher:
+            K, ids, logits = entries[0].shape[1], entries[0].data_ptr(), entries[1].data_ptr()
+        kept, room, back = _bytes(_capi.DTYPES[h.dtype], h.shape[1], h.shape[0], table.shape[0], K, teacher, need)
+        at = _at(h, table, bias)
+        a = _problem(h, table, at, scale, temperature)
         loss = torch.empty(h.shape[0], dtype=torch.float32, device=dev)
-        nk = lib.sgl_candidates_keep_bytes(a, K, teacher, need)
-        keep = _capi.workspace(nk, dev) if nk else None
-        nb = lib.sgl_candidates_workspace_bytes(a, K, teacher, need, 0)
-        ws = _capi.workspace(nb, dev)
+        keep = _capi.workspace(kept, dev) if kept else None
+        ws = _capi.workspace(room, dev)
         with _guard(dev):
-            _capi.check(lib.sgl_candidates_forward(a, P(target), P(ids), P(logits), K, need, P(loss), P(keep), nk, P(ws), nb,
-                                                   _capi.stream_of(dev)), "distillation" if teacher else "cross_entropy")
-        return loss, (h, table, bias, keep), K, lib.sgl_candidates_workspace_bytes(a, K, teacher, need, 1) if need else 0
-
-    @staticmethod
-    def problem(h, table, bias, scale, temperature):
-        P = _capi.ptr
-        return _capi.Candidates(_capi.DTYPES[h.dtype], h.shape[1], h.shape[0], table.shape[0], P(h), P(table),
-                                h.stride(0), table.stride(0), P(bias), scale, temperature)
+            _capi.check(_capi.lib().sgl_candidates_forward(
+                a, None if teacher else target.data_ptr(), ids, logits, K, need, loss.data_ptr(),
+                keep.data_ptr() if kept else None, kept, ws.data_ptr(), room, _capi.stream_of(dev)),
+                "distillation" if teacher else "cross_entropy")
+        return loss, (h, table, bias, keep), (a, at, scale, temperature, K, teacher, need, kept, back)
 
     @staticmethod
     @_first_order
     def backward(ctx, g):
         h, table, bias, keep = ctx.saved_tensors
-        scale, temperature, K, teacher, need, room = ctx.form
-        lib, P, dev = _capi.lib(), _capi.ptr, h.device
-        # (from the tensors as they are now: a hook on saved tensors may bring them back elsewhere)
-        a = ctypes.byref(_Loss.problem(h, table, bias, scale, temperature))
+        a, at, scale, temperature, K, teacher, need, kept, room = ctx.form
+        now = _at(h, table, bias)
+        if now != at:   # (a hook on saved tensors has brought them back elsewhere)
+            a = _problem(h, table, now, scale, temperature)
         g = g.contiguous()
-        want = ctx.needs_input_grad
-        dh = torch.empty(h.shape, dtype=h.dtype, device=dev) if want[0] else None
-        dt = torch.empty(table.shape, dtype=table.dtype, device=dev) if want[1] or want[2] else None
-        db = torch.empty_like(bias) if want[2] else None
-        nb = room if dt is not None else 0
-        ws = _capi.workspace(nb, dev) if nb else None
-        with _guard(dev):
-            _capi.check(lib.sgl_candidates_backward(a, K, teacher, need, P(keep), keep.numel(), P(g), P(dh), P(dt), P(db),
-                                                    P(ws), nb, _capi.stream_of(dev)), "candidates backward")
-        return dh, dt if want[1] else None, db, None, None, None, None
+        rows, candidates, values, *_ = ctx.needs_input_grad
+        dh = h.new_empty(h.shape) if rows else None
+        dt = db = ws = None
+        if candidates or values:
+            dt, ws = table.new_empty(table.shape), _capi.workspace(room, h.device)
+            db = bias.new_empty(bias.shape) if values else None
+        with _guard(h.device):
+            _capi.check(_capi.lib().sgl_candidates_backward(
+                a, K, teacher, need, keep.data_ptr(), kept, g.data_ptr(), dh.data_ptr() if rows else None,
+                None if dt is None else dt.data_ptr(), db.data_ptr() if values else None,
+                None if ws is None else ws.data_ptr(), 0 if ws is None else room, _capi.stream_of(h.device)),
+                "candidates backward")
+        return dh, dt if candidates else None, db, None, None, None, None

@@ -42,8 +42,8 @@ def _guard(dev: torch.device):
 
 def _first_order(backward):
     """once_differentiable, with its work only where gradients of gradients are
-    recorded (a backward pass runs on autograd's own thread, where each step of
-    Python costs several times what it does elsewhere)."""
+    recorded (a backward pass runs on autograd's own thread, where a step of
+    Python takes twice as long as elsewhere)."""
     recorded = once_differentiable(backward)
 
     @functools.wraps(backward)

@@ -91,6 +91,14 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, q_pos: torch.Tensor, k_pos: 
     return _Rotate.run(*args, False)
 
 
+def _side(x, y, pos):
+    """The C struct of ``x`` (its last dimension contiguous), ``y`` and their positions."""
+    sn, st, sh, _ = x.stride()
+    pn, pt = pos.stride()
+    return ctypes.byref(_capi.RotarySide(x.data_ptr(), y.data_ptr(), pos.data_ptr(), x.shape[1], sn, st, sh, pn, pt,
+                                         x.shape[2]))
+
+
 class _Rotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_pos, k_pos, freqs, interleaved, gain):
@@ -101,27 +109,23 @@ class _Rotate(torch.autograd.Function):
 
     @staticmethod
     def run(q, k, q_pos, k_pos, freqs, interleaved, gain, inverse):
-        lib, P = _capi.lib(), _capi.ptr
+        """(q, k) turned (None stays None)."""
         one = q if q is not None else k
-        dev, dh = one.device, one.shape[3]
-        outs, sides, held = [], [], []
-        for x, pos in ((q, q_pos), (k, k_pos)):
-            if x is None:
-                outs.append(None)
-                sides.append(None)
-                continue
-            x = _rows(x)
-            y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-            outs.append(y)
-            held.append(x)
-            sides.append(_capi.RotarySide(P(x), P(y), P(pos), x.shape[1], *x.stride()[:3], *pos.stride(), x.shape[2]))
-        if sides[0] is None:
-            sides = [sides[1], None]
-        ref = [None if s is None else ctypes.byref(s) for s in sides]
+        dev, new_q, new_k, sides = one.device, None, None, []
+        if q is not None:
+            q = _rows(q)
+            new_q = q.new_empty(q.shape)
+            sides.append(_side(q, new_q, q_pos))
+        if k is not None:
+            k = _rows(k)
+            new_k = k.new_empty(k.shape)
+            sides.append(_side(k, new_k, k_pos))
         with _guard(dev):
-            _capi.check(lib.sgl_rotary(_capi.DTYPES[one.dtype], one.shape[0], dh, 2 * freqs.shape[0], *ref, P(freqs),
-                                       interleaved, gain, inverse, _capi.stream_of(dev)), "rotate")
-        return tuple(outs)
+            _capi.check(_capi.lib().sgl_rotary(
+                _capi.DTYPES[one.dtype], one.shape[0], one.shape[3], 2 * freqs.shape[0], sides[0],
+                sides[1] if len(sides) == 2 else None, freqs.data_ptr(), interleaved, gain, inverse,
+                _capi.stream_of(dev)), "rotate")
+        return new_q, new_k
 
     @staticmethod
     @_first_order
