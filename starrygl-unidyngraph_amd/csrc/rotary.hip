@@ -79,16 +79,14 @@ __device__ __forceinline__ void turn(T &a, T &b, float sn, float cs) {
 }
 
 // A workgroup forms the frequencies' steps once where they are few (SHARED: up
-// to kSteps pairs; 64-bit floating point of every lane
-// otherwise: one head of 172 in fp16 38 us for 57, two of 100 with 64 turned 39
-// for 53).
+// to kSteps pairs; 64-bit floating point of every lane otherwise: one head of 172
+// in fp16 38 us for 57, two of 100 with 64 turned 39 for 53).
 // A lane owns VEC consecutive channels of a row (both halves' in the half
 // layout) for all its heads; the angles are formed once for all of them. A
 // part's last lane takes its last VEC channels, some of them its neighbour's
-// too (it writes the same bits), so
-// that loads and stores are all whole (4 heads of 44 in bf16: 123 us with the
-// last ones one by one, 30 so); channels that are not rotated and fewer than VEC
-// go one by one.
+// too (it writes the same bits), so that loads and stores are all whole (4 heads
+// of 44 in bf16: 123 us with the last ones one by one, 30 so); channels that are
+// not rotated and fewer than VEC go one by one.
 template <typename T, int VEC, bool INTER, bool SHARED>
 __global__ __launch_bounds__(kBlock) void k_rotate(RotArgs a) {
   const int sd = int64_t(blockIdx.x) >= a.side[1].first ? 1 : 0;

@@ -203,3 +203,19 @@ def test_hooks_repeated_backward_and_second_order(ops, gpu):  # noqa: F811
         leaves[1].mul_(2.0)   # a saved tensor written in between
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         torch.autograd.grad(loss, leaves, go)
+
+
+@pytest.mark.parametrize("scale", [1.0, -1.0, 0.0, 40.0])
+@pytest.mark.parametrize("N,V,D,dtype", [(5, 1000, 64, BF16), (300, 640, 100, FP16), (520, 1111, 172, BF16),
+                                         (300, 999, 100, FP32), (2000, 129, 256, BF16)])
+def test_loss_alone(ops, gpu, N, V, D, dtype, scale):  # noqa: F811
+    """Without gradients and a bias, scores that grow along the table or fall."""
+    g, h, w, _, go = _inputs(N + D, N, V, D, dtype, False)
+    for growth in (torch.linspace(0.1, 3.0, V), torch.linspace(3.0, 0.1, V)):
+        table = (w.float().abs() * growth[:, None]).to(dtype)
+        rows = h.abs()
+        t = torch.randint(0, V, (N,), generator=g)
+        want, bound = co.loss(rows, table, *co.labels(t), go, scale=scale)
+        with torch.no_grad():
+            got = ops.cross_entropy(rows.to(gpu), table.to(gpu), t.to(gpu), scale=scale)
+        _close(got, want["loss"], bound["loss"], "loss")
