@@ -226,8 +226,8 @@ __device__ __forceinline__ float max16(const V &p) {
 // Accumulator blocks times a factor. With one wave a SIMD (ALONE) they lie in
 // the matrix unit's own registers, and the factor is applied in place by hand:
 // behind a branch that is seldom taken the compiler otherwise keeps the blocks
-// in two places and moves all of them on the path that does nothing (256 moves
-// a step of 64 rows of 256 channels). The waits are a matrix product's before its
+// in two places and moves all of them on the path that does nothing (128 moves
+// a step of 256 channels). The waits are a matrix product's before its
 // result is read and a write's before the next one.
 template <bool ALONE, int NB>
 __device__ __forceinline__ void scale_blocks(f32x16 (&o)[NB], float by) {

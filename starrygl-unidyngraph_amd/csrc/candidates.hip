@@ -571,10 +571,11 @@ extern "C" int sgl_candidates_backward(const sgl_candidates *problem, int32_t k,
   Problem p;
   if (const int rc = make_problem(problem, p)) return rc;
   SGL_REQUIRE(k > 0 && k <= kMaxTargets && (teacher != 0 || k == 1), "candidates_backward: %d targets a row", k);
-  SGL_REQUIRE(need > 0 && need <= (kNeedRows | kNeedTable) && p.N > 0, "candidates_backward: need %d of %lld rows", need,
-              (long long)p.N);
+  SGL_REQUIRE(need > 0 && need <= (kNeedRows | kNeedTable) && p.N > 0, "candidates_backward: need %d of %lld rows",
+              need, (long long)p.N);
   SGL_REQUIRE(g != nullptr && (dh == nullptr || (need & kNeedRows)) && (dtable == nullptr || (need & kNeedTable)) &&
-              (dbias == nullptr || dtable != nullptr), "candidates_backward: a gradient that the forward did not prepare");
+              (dbias == nullptr || dtable != nullptr),
+              "candidates_backward: a gradient that the forward did not prepare");
   size_t room = 0;
   const Keep kept = carve_keep(const_cast<void *>(keep), p, k, teacher != 0, need, &room);
   if (const int rc = check_room("memory for the backward", keep, keep_bytes, room)) return rc;

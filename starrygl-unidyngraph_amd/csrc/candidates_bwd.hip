@@ -54,7 +54,8 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) 
   using M = Mma32<T>;
   using Im = Tiles<T, DB>;
   constexpr int BLOCK = 64 * WAVES;
-  constexpr int KS = M::KS, DP = 32 * DB, NK = DP / KS - CUT, TRIM = kTrim<T>, OB = DB - CUT / 2, YT = Im::YT, XT = Im::XT, QL = Im::QL;
+  constexpr int KS = M::KS, DP = 32 * DB, NK = DP / KS - CUT, TRIM = kTrim<T>, OB = DB - CUT / 2;
+  constexpr int YT = Im::YT, XT = Im::XT, QL = Im::QL;
   using Tl = Tile32<T, DP>;
   constexpr bool HALF = std::is_same_v<T, fp16_t>;
   extern __shared__ __align__(16) char lds[];
@@ -341,8 +342,8 @@ void run(const BwdArgs &a, hipStream_t stream) {
   const Line line((a.p.V + Im::XT - 1) / Im::XT, (a.p.N + Im::YT - 1) / Im::YT, P::GROUPS);
   launch(k, dim3(unsigned(line.groups)), dim3(64 * P::WAVES), bytes, stream, a);
   if (line.groups > 1)
-    launch(&k_join_grad<T>, dim3(unsigned(line.groups - 1) * kJoin), dim3(kBlock), 0, stream, a, int(Im::XT), int(Im::YT),
-           32 * DB, int(P::GROUPS));
+    launch(&k_join_grad<T>, dim3(unsigned(line.groups - 1) * kJoin), dim3(kBlock), 0, stream, a, int(Im::XT),
+           int(Im::YT), 32 * DB, int(P::GROUPS));
 }
 
 }  // namespace

@@ -132,7 +132,8 @@ def _bytes(dtype: int, dim: int, n: int, v: int, K: int, teacher: bool, need: in
     """What the forward keeps for the backward, its workspace, the backward's."""
     lib = _capi.lib()
     a = ctypes.byref(_capi.Candidates(dtype, dim, n, v, 16, 16, dim, dim, None, 1.0, 1.0))   # (never read)
-    return (lib.sgl_candidates_keep_bytes(a, K, teacher, need), lib.sgl_candidates_workspace_bytes(a, K, teacher, need, 0),
+    return (lib.sgl_candidates_keep_bytes(a, K, teacher, need),
+            lib.sgl_candidates_workspace_bytes(a, K, teacher, need, 0),
             lib.sgl_candidates_workspace_bytes(a, K, teacher, need, 1) if need else 0)
 
 
