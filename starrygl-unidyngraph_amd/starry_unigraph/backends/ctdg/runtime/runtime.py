@@ -453,10 +453,11 @@ class CTDGOnlineRuntime:
             if self._front_stream is not None:   # negatives drawn on the front stream
                 torch.cuda.current_stream(self.device).wait_stream(self._front_stream)
             src, dst, ts, ef = self._device_batch(batch)
-            self._front_body(step, split, n, src, dst, buf[off:off + n] if off >= 0 else buf, ts, ef, None)
+            neg = buf[off:off + n] if off >= 0 else buf
+            self._front_body(step, split, n, src, dst, neg, ts, ef, None)
             self._commit_body(step, train)
             self._taught = self._teacher[0](batch) if train and self._teacher is not None else None
-            self._back_body(step, train, n)
+            self._back_body(step, train, n, dst, neg)
             self.fence()
         else:
             # the negatives must sit at the batch's place in the stream-wide array
@@ -581,13 +582,15 @@ class CTDGOnlineRuntime:
         if train and not self._hist:
             self._param_update(step).advance()
 
-    def _back_body(self, step: DeviceStep, train: bool, n: int) -> None:
+    def _back_body(self, step: DeviceStep, train: bool, n: int, dst=None, neg=None) -> None:
         """Attention forward, edge predictor + BCE and, in training, the
-        backward and the fused weight-gradient + Adam update."""
+        backward and the fused weight-gradient + Adam update. ``dst``, ``neg``:
+        the batch's destinations and negatives (the history embedding alone:
+        its steps are not planned)."""
         core = self._core()
         conv = core.conv
         if self._hist:
-            self._history_back(step, train, n)
+            self._history_back(step, train, n, dst, neg)
             self._metrics_op(step, n)
             return
         efeat_all = self._dev["edge_feat"]
@@ -623,7 +626,7 @@ class CTDGOnlineRuntime:
             upd.run()
         self._metrics_op(step, n)
 
-    def _history_back(self, step: DeviceStep, train: bool, n: int) -> None:
+    def _history_back(self, step: DeviceStep, train: bool, n: int, dst: torch.Tensor, neg: torch.Tensor) -> None:
         """The back part of the history embedding: embeddings, edge predictor
         and BCE (runtime.py:197-199), or the next-node objective, and, in training, autograd's backward
         into the optimizer's flat gradients and its step."""
@@ -632,7 +635,7 @@ class CTDGOnlineRuntime:
         with torch.set_grad_enabled(train):
             y = core.roots(step, self.dims)
             if self._next_node:
-                out, loss = self._next_node_loss(core, y, b, n)
+                out, loss = self._next_node_loss(core, y[b.ridx_src[:n]], dst, neg)
             else:
                 out = core(y[b.ridx_src[:n]], y[b.ridx_dst[:n]], y[b.ridx_neg[:n]])
                 # BCE of 1 and 0 on the logits
@@ -645,12 +648,11 @@ class CTDGOnlineRuntime:
         b.neg[:n].copy_(out.neg_logits.detach())
         b.loss.copy_(loss.detach())
 
-    def _next_node_loss(self, core, y: torch.Tensor, b, n: int) -> tuple:
+    def _next_node_loss(self, core, src: torch.Tensor, dst: torch.Tensor, neg: torch.Tensor) -> tuple:
         """(logits, loss) of the next-node objective: the mean cross entropy of
         the destinations over all candidates, and with a teacher its
-        divergence."""
-        nodes = F.pad(b.roots[:b.cap], (0, 1), value=-1)
-        src, dst, neg = y[b.ridx_src[:n]], nodes[b.ridx_dst[:n]], nodes[b.ridx_neg[:n]]
+        divergence. ``src``: the sources' embeddings; ``dst``, ``neg``: node
+        ids (a drawn negative is seldom one of the batch's roots)."""
         with torch.no_grad():
             out = core(src, dst, neg)
         h = core.src_fc(src)
