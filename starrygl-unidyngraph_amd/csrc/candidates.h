@@ -75,6 +75,26 @@ __device__ __forceinline__ FragOf<T> frag_of16(const V &p, int s, float by = 1.f
   return f;
 }
 
+// Sum of a fragment's values as a product takes them: bf16 by the two-element
+// dot product with ones (within 3 x 2^-24 of each of its four sums, measured), fp16 by
+// additions that take 16 bits (its dot product is off by 2^-21).
+__device__ __forceinline__ float frag_sum(FragOf<bf16_t> f) {
+  typedef __bf16 Two __attribute__((ext_vector_type(2)));
+  float a = 0.f, b = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; e += 4) {
+    a = __builtin_amdgcn_fdot2_f32_bf16(Two{f[e], f[e + 1]}, Two{1.f, 1.f}, a, false);
+    b = __builtin_amdgcn_fdot2_f32_bf16(Two{f[e + 2], f[e + 3]}, Two{1.f, 1.f}, b, false);
+  }
+  return a + b;
+}
+__device__ __forceinline__ float frag_sum(FragOf<fp16_t> f) {
+  float a[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) a[e] = float(f[e]) + float(f[e + 4]);
+  return (a[0] + a[1]) + (a[2] + a[3]);
+}
+
 // Row-major tiles of DP columns, 16 bytes of padding a row.
 template <typename T, int DP>
 struct Tile32 {
@@ -167,9 +187,15 @@ struct Stage {
       }
     }
   }
-  static __device__ __forceinline__ void clear(T *tile) {
-    for (int u = threadIdx.x; u < YT * Tl::UPR; u += BLOCK)
-      *reinterpret_cast<FragOf<T> *>(tile + u / Tl::UPR * Tl::LD + u % Tl::UPR * E) = zero_frag<T>();
+  // zeros, and ones in column `one` (at or past D, where put leaves them; -1: none)
+  static __device__ __forceinline__ void clear(T *tile, int one = -1) {
+    for (int u = threadIdx.x; u < YT * Tl::UPR; u += BLOCK) {
+      FragOf<T> f = zero_frag<T>();
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (u % Tl::UPR * E + e == one) f[e] = T(1.f);
+      *reinterpret_cast<FragOf<T> *>(tile + u / Tl::UPR * Tl::LD + u % Tl::UPR * E) = f;
+    }
   }
 };
 // A value that the compiler takes as new: what is formed from it inside a loop
@@ -361,11 +387,13 @@ struct Order {
   __device__ __forceinline__ int64_t count(int64_t N) const { return live != nullptr ? int64_t(*live) : N; }
 };
 // What a forward leaves for each piece (Line) and wave along the table: its
-// own maximum as used, its sum and, with a direction, sum_v p_v w_v at that maximum.
+// own maximum as used, its sum and, with a direction, sum_v p_v w_v at that maximum
+// and the sum of the p_v as rounded there (16-bit types; fp32: the sum itself): in
+// column `ones` of o, where the tiles hold ones, or in r (no column is free: -1).
 struct Partials {
-  float *m, *l, *o;   // [pieces][wy][rows], the same, [pieces][wy][rows][dp]
+  float *m, *l, *r, *o;   // [pieces][wy][rows], the same twice, [pieces][wy][rows][dp]
   int64_t ytiles;
-  int rows, wy, dp, groups;
+  int rows, wy, dp, groups, ones;
 };
 int padded_dim(int D);
 Partials forward_shape(int32_t dtype, const Problem &p);   // (without its arrays)

@@ -185,14 +185,21 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
     n = int(line.group_of((xt + 1) * line.inner - 1) - w0 + 1) * a.in.wy;
     first = (w0 + xt) * a.in.wy * a.in.rows + (pos - xt * a.in.rows);
   }
-  const float *pm = a.in.m + first, *pl = a.in.l + first;
+  constexpr bool ROUNDED = DIR && sizeof(T) == 2;
+  const float *pm = a.in.m + first, *pl = a.in.l + first, *pr = nullptr;
+  int step_r = a.in.rows;   // of the rounded sums
+  if constexpr (ROUNDED) {
+    if (a.in.ones >= 0) step_r *= a.in.dp;
+    pr = a.in.ones >= 0 ? a.in.o + first * a.in.dp + a.in.ones : a.in.r + first;
+  }
   // (the first of them at once: their loads, the row's and the targets' overlap)
-  float m[kAhead], s[kAhead];
+  float m[kAhead], s[kAhead], rs[kAhead];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
     const int k = w * kWave + lane + i * (W * kWave);
     m[i] = k < n ? pm[k * a.in.rows] : -INFINITY;
     s[i] = k < n ? pl[k * a.in.rows] : 0.f;
+    rs[i] = ROUNDED && k < n ? pr[k * step_r] : 0.f;
   }
   // the first targets' rows
   int id = -1;
@@ -230,27 +237,37 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
   ask(k0);
 
   // the maximum and the sum of all partials (a piece without a live candidate has sum 0)
-  float mx = -INFINITY, l = 0.f;
+  float mx = -INFINITY, l = 0.f, lr = 0.f;
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) mx = fmaxf(mx, m[i]);
   for (int k = w * kWave + lane + kAhead * W * kWave; k < n; k += W * kWave) mx = fmaxf(mx, pm[k * a.in.rows]);
   mx = wave_max(mx);
   auto at_max = [&](float y, float z) { return y == -INFINITY ? z : z * exp2_fast(y - mx); };
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) l += at_max(m[i], s[i]);
-  for (int k = w * kWave + lane + kAhead * W * kWave; k < n; k += W * kWave)
+  for (int i = 0; i < kAhead; ++i) {
+    l += at_max(m[i], s[i]);
+    if constexpr (ROUNDED) lr += at_max(m[i], rs[i]);
+  }
+  for (int k = w * kWave + lane + kAhead * W * kWave; k < n; k += W * kWave) {
     l += at_max(pm[k * a.in.rows], pl[k * a.in.rows]);
+    if constexpr (ROUNDED) lr += at_max(pm[k * a.in.rows], pr[k * step_r]);
+  }
   l = wave_sum(l);
+  if constexpr (ROUNDED) lr = wave_sum(lr);
   if constexpr (W > 1) {
-    if (lane == 0) sums[0][wave][0] = mx, sums[0][wave][1] = l;
+    if (lane == 0) sums[0][wave][0] = mx, sums[0][wave][1] = l, sums[0][wave][2] = lr;
     __syncthreads();
     mx = -INFINITY;
-    l = 0.f;
+    l = lr = 0.f;
 #pragma unroll
     for (int i = 0; i < W; ++i) mx = fmaxf(mx, sums[0][i][0]);
 #pragma unroll
-    for (int i = 0; i < W; ++i) l += at_max(sums[0][i][0], sums[0][i][1]);
+    for (int i = 0; i < W; ++i) {
+      l += at_max(sums[0][i][0], sums[0][i][1]);
+      if constexpr (ROUNDED) lr += at_max(sums[0][i][0], sums[0][i][2]);
+    }
   }
+  if constexpr (!ROUNDED) lr = l;
 
   // the targets: sum of q (mx - s), of q, of q w
   float x[4], tw[4], far = 0.f;
@@ -329,7 +346,7 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
     }
     float e[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) e[j] = o[j] / l - tw[j];
+    for (int j = 0; j < 4; ++j) e[j] = o[j] / lr - tw[j];
     if constexpr (W > 1) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) parts[wave][4 * lane + j] = e[j];
@@ -436,6 +453,7 @@ Partials carve_forward(void *ws, int32_t dtype, const Problem &p, bool dir, size
   const size_t pieces = size_t((p.N + out.rows - 1) / out.rows + out.groups) * size_t(out.wy) * size_t(out.rows);
   out.m = c.take<float>(pieces);
   out.l = c.take<float>(pieces);
+  out.r = dir && dtype != SGL_FP32 && out.ones < 0 ? c.take<float>(pieces) : nullptr;
   out.o = dir ? c.take<float>(pieces * size_t(out.dp)) : nullptr;
   *bytes = c.used;
   return out;

@@ -38,11 +38,13 @@ constexpr int kBuffers = 2 * YT * Tile32<T, 32 * DB>::LD * int(sizeof(T)) <= 140
 
 // A wave has 32 rows; WX waves lie along the rows, WY along the table (few rows:
 // each has 32 candidates of a tile of its own, and leaves a partial of its
-// own). SUB steps of 32 candidates a tile.
-template <typename T, int DB, int CUT, int WX, int WY, int SUB, int PER_SIMD, bool DIR>
+// own). SUB steps of 32 candidates a tile. COUNT: no column of the tiles is free
+// to sum p as rounded (a branch in the loop cost the products 2.6 %).
+template <typename T, int DB, int CUT, int WX, int WY, int SUB, int PER_SIMD, bool DIR, bool COUNT>
 __global__ __launch_bounds__(64 * WX * WY, PER_SIMD) void k_forward(FwdArgs a) {
   using M = Mma32<T>;
   constexpr int BLOCK = 64 * WX * WY, KS = M::KS, DP = 32 * DB, NK = DP / KS - CUT, TRIM = kTrim<T>, OB = DB - CUT / 2;
+  static_assert(!COUNT || (DIR && sizeof(T) == 2), "p is rounded");
   using Tl = Tile32<T, DP>;
   constexpr int LD = Tl::LD, YT = 32 * SUB * WY, XT = 32 * WX, NBUF = kBuffers<T, DB, YT>;
   extern __shared__ __align__(16) char lds[];
@@ -70,7 +72,7 @@ __global__ __launch_bounds__(64 * WX * WY, PER_SIMD) void k_forward(FwdArgs a) {
     if (biased && tid < YT) nb = p.bias[y0 + min(tid, rows - 1)];
   };
 #pragma unroll
-  for (int i = 0; i < NBUF; ++i) Stage<T, DP, YT, BLOCK>::clear(tiles + i * YT * LD);
+  for (int i = 0; i < NBUF; ++i) Stage<T, DP, YT, BLOCK>::clear(tiles + i * YT * LD, DIR ? a.out.ones : -1);
   int64_t u = line.begin(w);
   int xt = int(u / line.inner), t = int(u - int64_t(xt) * line.inner), buf = 0;
   fetch(t);
@@ -84,6 +86,10 @@ __global__ __launch_bounds__(64 * WX * WY, PER_SIMD) void k_forward(FwdArgs a) {
     load_outer<T>(xf, static_cast<const T *>(p.h) + a.order.row(min(x, N - 1)) * p.hs, x >= N, D);
     // the maximum, as used, the sum and its compensation (a row's sum has up to 2^15 terms)
     float m = -INFINITY, mu = -kTop<T>, l = 0.f, lc = 0.f;
+    // What the sum of p as rounded for sum p w has beyond l (COUNT). Where a tile has a column to spare it holds
+    // ones, and the product sums them: 4,000 x 1,140,149 x 172 in bf16, both passes, 6,582 us with the vector unit's
+    // sums, 6,366 so, 6,328 with none; 4,000 x 50,001 x 256 in fp16, no column to spare, 665 for 652.
+    float off = 0.f;
     f32x16 o[DIR ? OB : 1];
 #pragma unroll
     for (int d = 0; d < (DIR ? OB : 1); ++d)
@@ -132,17 +138,20 @@ __global__ __launch_bounds__(64 * WX * WY, PER_SIMD) void k_forward(FwdArgs a) {
           mu = (mn == -INFINITY ? 0.f : mn) - kTop<T>;
           l *= by;
           lc *= by;
+          if constexpr (COUNT) off *= by;
           if constexpr (DIR) scale_blocks<PER_SIMD == 1>(o, by);
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = exp2_fast(DIR ? s[r] - mu : fmaf(s[r], by_c, -mu));
-        const float add = sum16(s) - lc, sum = l + add;
+        const float here = sum16(s), add = here - lc, sum = l + add;
         lc = (sum - l) - add;
         l = sum;
+        if constexpr (COUNT) off -= here;
         if constexpr (DIR) {
 #pragma unroll
           for (int st = 0; st < 32 / KS; ++st) {
             const FragOf<T> pf = frag_of16<T>(s, st);
+            if constexpr (COUNT) off += frag_sum(pf);
 #pragma unroll
             for (int d = 0; d < OB; ++d) o[d] = M::mma(Tl::frag_t(tile, 32 * d, row0, st), pf, o[d]);
           }
@@ -151,11 +160,12 @@ __global__ __launch_bounds__(64 * WX * WY, PER_SIMD) void k_forward(FwdArgs a) {
     }
 
     const int64_t at = (int64_t(w + xt) * WY + wy) * XT + wx * 32 + (lane & 31);
-    const float sum = pair_sum(l);
+    const float sum = pair_sum(l), rounded = COUNT ? pair_sum(l + off) : 0.f;
     if (x < N) {
       if (h == 0) {
         a.out.m[at] = m == -INFINITY ? -INFINITY : mu;
         a.out.l[at] = sum;
+        if constexpr (COUNT) a.out.r[at] = rounded;
       }
       if constexpr (DIR) {
         float *row = a.out.o + at * DP;
@@ -174,6 +184,10 @@ __global__ __launch_bounds__(64 * WX * WY, PER_SIMD) void k_forward(FwdArgs a) {
   }
 }
 
+// Steps of 16 channels left out: 7 of 8 are slower than 8 (768 x 570,074 x 104 in
+// bf16 262 us for 239), 6 faster, as 11 of 12 are.
+template <int DB, int CUT>
+constexpr int kForwardCut = DB == 4 && CUT == 1 ? 0 : CUT;
 // Up to here a workgroup's waves share the rows and split the table.
 constexpr int64_t kFewRows = 32;
 constexpr int kFewWaves = 4;
@@ -191,7 +205,7 @@ struct Half {
     return AT_ALL && 6 * halves <= 5 * whole;
   }
 };
-template <typename T, int DB>
+template <typename T, int DB, int CUT>
 Partials shape_of(const Problem &p) {
   using P = Plan<T, DB>;
   Partials s{};
@@ -199,12 +213,13 @@ Partials shape_of(const Problem &p) {
   s.rows = few ? 32 : 32 * (half ? Half<T, DB>::WAVES : P::WAVES);
   s.wy = few ? kFewWaves : 1;
   s.dp = 32 * DB;
+  s.ones = sizeof(T) == 2 && p.D < 32 * (few ? DB : DB - CUT / 2) ? p.D : -1;
   s.groups = few ? 256 : half ? Half<T, DB>::GROUPS : P::GROUPS;
   const int ytile = few ? 32 * kFewWaves : 32 * P::SUB;
   s.ytiles = (p.V + ytile - 1) / ytile;
   return s;
 }
-template <typename T, int DB, int CUT, bool DIR>
+template <typename T, int DB, int CUT, bool DIR, bool COUNT>
 void run(const FwdArgs &a, hipStream_t stream) {
   using P = Plan<T, DB>;
   using H = Half<T, DB>;
@@ -219,20 +234,22 @@ void run(const FwdArgs &a, hipStream_t stream) {
   static_assert(few_bytes <= 160 * 1024 && many_bytes <= 160 * 1024 * P::GROUPS_PER_TWO / 2, "LDS of a CU");
   static_assert(!H::AT_ALL || many_bytes <= 80 * 1024, "two workgroups a CU");
   if (a.p.N <= kFewRows) {
-    go(&k_forward<T, DB, 0, 1, kFewWaves, 1, P::PER_SIMD, DIR>, 64 * kFewWaves, few_bytes);
+    if constexpr (!COUNT || CUT == 0)   // (these tiles keep all columns: one is free where steps are left out)
+      go(&k_forward<T, DB, 0, 1, kFewWaves, 1, P::PER_SIMD, DIR, COUNT>, 64 * kFewWaves, few_bytes);
     return;
   }
   if constexpr (H::AT_ALL)
     if (H::takes(a.p.N)) {
-      go(&k_forward<T, DB, CUT, H::WAVES, 1, P::SUB, P::PER_SIMD, DIR>, 64 * H::WAVES, many_bytes);
+      go(&k_forward<T, DB, CUT, H::WAVES, 1, P::SUB, P::PER_SIMD, DIR, COUNT>, 64 * H::WAVES, many_bytes);
       return;
     }
-  go(&k_forward<T, DB, CUT, P::WAVES, 1, P::SUB, P::PER_SIMD, DIR>, 64 * P::WAVES, many_bytes);
+  go(&k_forward<T, DB, CUT, P::WAVES, 1, P::SUB, P::PER_SIMD, DIR, COUNT>, 64 * P::WAVES, many_bytes);
 }
 template <typename T, int DB, int CUT>
 void pick(const FwdArgs &a, hipStream_t stream) {
-  if (a.out.o != nullptr) run<T, DB, CUT, true>(a, stream);
-  else run<T, DB, CUT, false>(a, stream);
+  if (a.out.o == nullptr) run<T, DB, CUT, false, false>(a, stream);
+  else if (a.out.r == nullptr) run<T, DB, CUT, true, false>(a, stream);
+  else if constexpr (sizeof(T) == 2 && CUT != 1) run<T, DB, CUT, true, true>(a, stream);   // (a column is free with 1)
 }
 
 }  // namespace
@@ -243,15 +260,15 @@ namespace cand {
 int padded_dim(int D) { return (D + 63) / 64 * 64; }
 
 Partials forward_shape(int32_t dtype, const Problem &p) {
-  return pick_dim(dtype, p.D, [&](auto t, auto db, auto) { return shape_of<decltype(t), db.value>(p); });
+  return pick_dim(dtype, p.D, [&](auto t, auto db, auto cut) {
+    return shape_of<decltype(t), db.value, kForwardCut<db.value, cut.value>>(p);
+  });
 }
 
 void forward_partials(int32_t dtype, const Problem &p, const Order &order, const Partials &out, hipStream_t stream) {
   const FwdArgs a{p, order, out};
   pick_dim(dtype, p.D, [&](auto t, auto db, auto cut) {
-    // (7 of 8 steps are slower than 8: 768 x 570,074 x 104 in bf16 262 us for 239; 6 faster, as 11 of 12 are)
-    constexpr int CUT = db.value == 4 && cut.value == 1 ? 0 : cut.value;
-    pick<decltype(t), db.value, CUT>(a, stream);
+    pick<decltype(t), db.value, kForwardCut<db.value, cut.value>>(a, stream);
   });
 }
 
