@@ -3,9 +3,10 @@
 //
 // (a, b) -> gain (a cos t - b sin t, a sin t + b cos t), t = position * f_i.
 // The angle is kept in turns, as a 64-bit fraction: position times f_i / 2 pi
-// modulo 1 is one integer product, exact for every int64 position (a float
-// angle of a position of 1e9 has no digits left of the turn). The gradient is
-// the same rotation the other way round.
+// modulo 1 is an integer product, and with f_i / 2 pi to 128 bits it is within
+// 2^-63 of a turn at every int64 position (a float angle of a position of 1e9 has
+// no digits left of the turn, a 64-bit f_i / 2 pi is 0.6 rad off at nanosecond
+// stamps of 1.7e18). The gradient is the same rotation the other way round.
 //
 // Memory bounds it, every element read and written once: 16 sequences of 8,191
 // x (8 + 2) heads of 128 in fp16 120 us, 5.6 TB/s (a large copy: 5.1); 4,000 x
@@ -52,18 +53,50 @@ __device__ __forceinline__ void sincos_turns(uint64_t turns, float &s, float &c)
   c = ((quarter + 1) & 2) != 0 ? -v : v;
 }
 
-// A frequency (angle a unit of position) in turns, modulo 1, as a 64-bit
-// fraction: f / 2 pi to 106 bits (1 / 2 pi in two doubles), so that its fraction
-// has them all.
-__device__ __forceinline__ uint64_t turn_step(double f) {
-  constexpr double kHi = 0x1.45f306dc9c883p-3, kLo = -0x1.6b01ec5417056p-57;
-  const double hi = f * kHi, lo = fma(f, kLo, fma(f, kHi, -hi));
-  auto fraction = [](double x) {   // x modulo 1, in 2^-64 (of the magnitude: its steps are exact)
-    const double m = fabs(x), r = m - floor(m), up = floor(r * 4294967296.0);
-    const uint64_t u = (uint64_t(up) << 32) + uint64_t((r * 4294967296.0 - up) * 4294967296.0);
-    return x < 0.0 ? 0 - u : u;
-  };
-  return fraction(hi) + fraction(lo);
+// A frequency (angle a unit of position) in turns, modulo 1: (hi 2^64 + lo) / 2^128.
+struct Step {
+  uint64_t hi, lo;
+};
+// m 2^e / 2 pi of a double m 2^e, with 1 / 2 pi to 320 bits: as many behind a
+// turn's point as a position has in front of it, and 64 more, for any
+// frequency under 2^128.
+__device__ __forceinline__ Step turn_step(double f) {
+  constexpr uint64_t kInv[5] = {0x28be60db9391054aull, 0x7f09d5f47d4d3770ull, 0x36d8a5664f10e410ull,
+                                0x7f9458eaf7aef158ull, 0x6dc91b8e909374b8ull};
+  const uint64_t bits = uint64_t(__double_as_longlong(f));
+  const int ex = int(bits >> 52) & 0x7FF, e = max(ex, 1) - 1075;
+  const uint64_t m = (bits & ((1ull << 52) - 1)) | (ex != 0 ? 1ull << 52 : 0ull);
+  uint64_t w0 = kInv[0], w1 = kInv[1], w2 = kInv[2];
+  if (e > 0) {   // (whole turns of 2^e / 2 pi are left out)
+    const int by = e & 63;
+    const bool far = e >= 64;
+    const uint64_t v0 = far ? kInv[1] : kInv[0], v1 = far ? kInv[2] : kInv[1], v2 = far ? kInv[3] : kInv[2],
+                   v3 = far ? kInv[4] : kInv[3];
+    w0 = by != 0 ? v0 << by | v1 >> (64 - by) : v0;
+    w1 = by != 0 ? v1 << by | v2 >> (64 - by) : v1;
+    w2 = by != 0 ? v2 << by | v3 >> (64 - by) : v2;
+  }
+  // m times it: p3 whole turns, then the fraction's words p2 and p1
+  const uint64_t p1 = m * w1 + __umul64hi(m, w2), c1 = p1 < m * w1 ? 1 : 0;
+  const uint64_t t = m * w0 + __umul64hi(m, w1), p2 = t + c1;
+  const uint64_t p3 = __umul64hi(m, w0) + (t < m * w0 ? 1 : 0) + (p2 < t ? 1 : 0);
+  Step s{p2, p1};
+  if (e < 0) {   // 2^e of it
+    const int r = -e, by = r & 63;
+    const uint64_t x0 = r < 64 ? p2 : r < 128 ? p3 : 0, up = r < 64 ? p3 : 0;
+    const uint64_t x1 = r < 64 ? p1 : r < 128 ? p2 : r < 192 ? p3 : 0;
+    s.hi = by != 0 ? x0 >> by | up << (64 - by) : x0;
+    s.lo = by != 0 ? x1 >> by | x0 << (64 - by) : x1;
+  }
+  if (f < 0.0) {
+    s.lo = 0 - s.lo;
+    s.hi = 0 - s.hi - (s.lo != 0 ? 1 : 0);
+  }
+  return s;
+}
+// The position's turns, modulo 1, as a 64-bit fraction (within two of its units).
+__device__ __forceinline__ uint64_t turns_at(int64_t pos, const Step &s) {
+  return uint64_t(pos) * s.hi + __umul64hi(uint64_t(pos), s.lo) - (pos < 0 ? s.lo : 0);
 }
 
 // a cos - b sin and a sin + b cos, rounded to 32 bits before the type's (one
@@ -96,7 +129,7 @@ __global__ __launch_bounds__(kBlock) void k_rotate(RotArgs a) {
   const int ru = (half + PV - 1) / PV, cu = (a.dh - a.rot + VEC - 1) / VEC, units = ru + cu;
   const int64_t at = (int64_t(blockIdx.x) - s.first) * kBlock + threadIdx.x;
   const int64_t row = at / units;
-  __shared__ uint64_t steps[SHARED ? kSteps : 1];
+  __shared__ Step steps[SHARED ? kSteps : 1];
   if constexpr (SHARED) {
     for (int i = threadIdx.x; i < half; i += kBlock) steps[i] = turn_step(a.freqs[i]);
     __syncthreads();
@@ -126,7 +159,7 @@ __global__ __launch_bounds__(kBlock) void k_rotate(RotArgs a) {
   float sn[PV], cs[PV];
 #pragma unroll
   for (int i = 0; i < PV; ++i) {
-    sincos_turns(uint64_t(pos) * (SHARED ? steps[p0 + i] : turn_step(a.freqs[p0 + i])), sn[i], cs[i]);
+    sincos_turns(turns_at(pos, SHARED ? steps[p0 + i] : turn_step(a.freqs[p0 + i])), sn[i], cs[i]);
     sn[i] *= a.gain * a.way;
     cs[i] *= a.gain;
   }
@@ -163,7 +196,7 @@ constexpr int kStretch = 16384 / int(sizeof(T));   // elements of a workgroup's 
 template <typename T, bool INTER>
 __global__ __launch_bounds__(kBlock) void k_rotate_odd(RotArgs a, int tile_rows) {
   __shared__ __align__(16) T tile[kStretch<T>];
-  __shared__ uint64_t steps[kSteps];
+  __shared__ Step steps[kSteps];
   __shared__ int64_t pos[kStretchRows];
   const int sd = int64_t(blockIdx.x) >= a.side[1].first ? 1 : 0, tid = threadIdx.x;
   const Side &s = a.side[sd];
@@ -190,7 +223,7 @@ __global__ __launch_bounds__(kBlock) void k_rotate_odd(RotArgs a, int tile_rows)
   for (int i = tid; i < rows * half; i += kBlock) {
     const int r = i / half, p = i - r * half;
     float sn, cs;
-    sincos_turns(uint64_t(pos[r]) * steps[p], sn, cs);
+    sincos_turns(turns_at(pos[r], steps[p]), sn, cs);
     sn *= a.gain * a.way;
     cs *= a.gain;
     T *v = tile + r * width + (INTER ? 2 * p : p);
