@@ -1026,9 +1026,10 @@ typedef struct sgl_rotary_side {
 } sgl_rotary_side;
 
 /* Pairs of the first `rot` of dh channels turned by pos * freqs[i] (freqs:
- * double [rot / 2]) and scaled by gain, the other channels copied: pairs (i, i +
- * rot / 2), or interleaved != 0 (2 i, 2 i + 1). inverse != 0: by the negative
- * angles (the gradient). k may be NULL. The structs are HOST memory. */
+ * double [rot / 2], under 2^128: another makes its pair NaN) and scaled by
+ * gain, the other channels copied: pairs (i, i + rot / 2), or interleaved != 0
+ * (2 i, 2 i + 1). inverse != 0: by the negative angles (the gradient). k may be
+ * NULL. The structs are HOST memory. */
 int sgl_rotary(int32_t dtype, int64_t n, int32_t dh, int32_t rot,
                const sgl_rotary_side *q, const sgl_rotary_side *k,
                const double *freqs, int32_t interleaved, float gain,

@@ -54,6 +54,7 @@ __device__ __forceinline__ void sincos_turns(uint64_t turns, float &s, float &c)
 }
 
 // A frequency (angle a unit of position) in turns, modulo 1: (hi 2^64 + lo) / 2^128.
+// The last bit marks one that has no angle (not finite, or 2^128 and more).
 struct Step {
   uint64_t hi, lo;
 };
@@ -92,11 +93,19 @@ __device__ __forceinline__ Step turn_step(double f) {
     s.lo = 0 - s.lo;
     s.hi = 0 - s.hi - (s.lo != 0 ? 1 : 0);
   }
+  s.lo = (s.lo & ~1ull) | (fabs(f) < 0x1p128 ? 0ull : 1ull);
   return s;
 }
 // The position's turns, modulo 1, as a 64-bit fraction (within two of its units).
 __device__ __forceinline__ uint64_t turns_at(int64_t pos, const Step &s) {
   return uint64_t(pos) * s.hi + __umul64hi(uint64_t(pos), s.lo) - (pos < 0 ? s.lo : 0);
+}
+// gain times the angle's sine (way -1: the other way round) and cosine.
+__device__ __forceinline__ void sincos_at(int64_t pos, const Step &step, float gain, float way, float &sn, float &cs) {
+  sincos_turns(turns_at(pos, step), sn, cs);
+  const float by = (step.lo & 1) != 0 ? NAN : gain;
+  sn *= by * way;
+  cs *= by;
 }
 
 // a cos - b sin and a sin + b cos, rounded to 32 bits before the type's (one
@@ -158,11 +167,8 @@ __global__ __launch_bounds__(kBlock) void k_rotate(RotArgs a) {
   const int64_t pos = s.pos[n * s.pn + t * s.pt];
   float sn[PV], cs[PV];
 #pragma unroll
-  for (int i = 0; i < PV; ++i) {
-    sincos_turns(turns_at(pos, SHARED ? steps[p0 + i] : turn_step(a.freqs[p0 + i])), sn[i], cs[i]);
-    sn[i] *= a.gain * a.way;
-    cs[i] *= a.gain;
-  }
+  for (int i = 0; i < PV; ++i)
+    sincos_at(pos, SHARED ? steps[p0 + i] : turn_step(a.freqs[p0 + i]), a.gain, a.way, sn[i], cs[i]);
   for (int h = 0; h < s.H; ++h, x += s.sh, y += a.dh) {
     if constexpr (INTER) {
       T v[VEC];
@@ -223,9 +229,7 @@ __global__ __launch_bounds__(kBlock) void k_rotate_odd(RotArgs a, int tile_rows)
   for (int i = tid; i < rows * half; i += kBlock) {
     const int r = i / half, p = i - r * half;
     float sn, cs;
-    sincos_turns(turns_at(pos[r], steps[p]), sn, cs);
-    sn *= a.gain * a.way;
-    cs *= a.gain;
+    sincos_at(pos[r], steps[p], a.gain, a.way, sn, cs);
     T *v = tile + r * width + (INTER ? 2 * p : p);
     constexpr int one = INTER ? 1 : 0;
     const int other = one != 0 ? 1 : half;
