@@ -57,7 +57,7 @@ __global__ __launch_bounds__(kBlock) void k_teacher(TeacherArgs a) {
     const int64_t id = a.ids[n * a.K + k];
     const float z = a.logits[n * a.K + k] / a.temperature;
     const bool live = id >= 0 && !(z == -INFINITY);
-    past |= id >= a.V;
+    past |= live && id >= a.V;
     ids[k] = live ? int(min(id, a.V)) : -1;
     q[k] = z;
     if (live) most = fmaxf(most, z);

@@ -1,0 +1,34 @@
+"""A teacher's entries that are none, with anything beside the mark that makes
+them so."""
+import math
+
+import pytest
+import torch
+
+import candidates_oracle as co
+from test_gpu_candidates import BF16, FP32, _check, _inputs, _rand, ops  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+def test_entries_that_are_none(ops, gpu, dtype):  # noqa: F811
+    """A logit of -inf is no entry whatever its id (past the table too), a negative id whatever its logit."""
+    N, V, D, K = 40, 90, 32, 6
+    g, h, w, b, go = _inputs(3, N, V, D, dtype, True)
+    ids, z = torch.randint(0, V, (N, K), generator=g), _rand(g, N, K)
+    clean, live = ids.clone(), z.clone()
+    clean[::2, 1], live[1::3, 4], clean[2, :], clean[::5, 0] = -1, -math.inf, -1, -1
+    want, bound = co.loss(h, w, *co.teacher(clean, live, 1.0), go, b)
+    ids, z = clean.clone(), live.clone()
+    for at, i in (((1, 4), V), ((4, 4), V + 5), ((7, 4), 1 << 40), ((10, 4), (1 << 63) - 1)):
+        ids[at] = i                       # (their logits are -inf)
+    ids[2, :3], z[2, :3] = V, -math.inf
+    z[::5, 0] = torch.tensor([math.nan, math.inf, -math.inf, 3e38, 0.0, -3e38, math.nan, math.inf])
+    leaves = [x.to(gpu).requires_grad_() for x in (h, w, b)]
+    loss = ops.distillation(leaves[0], leaves[1], ids.to(gpu), z.to(gpu), bias=leaves[2])
+    _check(loss, leaves, go, want, bound)
+    ids[1, 0], z[1, 0] = V, 0.0           # an entry past the table
+    loss = ops.distillation(leaves[0], leaves[1], ids.to(gpu), z.to(gpu), bias=leaves[2])
+    assert torch.isnan(loss).nonzero().tolist() == [[1]]
+    assert not torch.autograd.grad(loss.sum(), leaves[0])[0][1].any()
