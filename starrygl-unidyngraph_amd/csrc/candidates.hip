@@ -30,7 +30,8 @@ __device__ __forceinline__ float wave_max(float v) {
 }
 
 // ------------------------------------------------------------------ a teacher's distribution
-// q = softmax(z / T) over a row's live entries, one wave a row. Entries of the
+// q = softmax(z / T) over a row's live entries, one wave a row (the maximum is
+// taken off before the division, which may pass float32's range). Entries of the
 // same candidate are put together in the first of them (the sums over entries
 // are the same), so that a candidate is wanted once. A row without a live
 // entry has the constant 0 and no targets, one with an index past the table
@@ -55,7 +56,7 @@ __global__ __launch_bounds__(kBlock) void k_teacher(TeacherArgs a) {
   bool past = false;
   for (int k = lane; k < a.K; k += kWave) {
     const int64_t id = a.ids[n * a.K + k];
-    const float z = a.logits[n * a.K + k] / a.temperature;
+    const float z = a.logits[n * a.K + k];
     const bool live = id >= 0 && !(z == -INFINITY);
     past |= live && id >= a.V;
     ids[k] = live ? int(min(id, a.V)) : -1;
@@ -69,7 +70,7 @@ __global__ __launch_bounds__(kBlock) void k_teacher(TeacherArgs a) {
   for (int k = lane; k < a.K; k += kWave) {
     if (ids[k] < 0) continue;
     any = true;
-    total += expf(q[k] - most);
+    total += expf((q[k] - most) / a.temperature);
   }
   total = wave_sum(total);
   const bool live_row = __any(any) && !bad;
@@ -77,7 +78,7 @@ __global__ __launch_bounds__(kBlock) void k_teacher(TeacherArgs a) {
   float konst = 0.f;
   for (int k = lane; k < a.K; k += kWave) {
     if (ids[k] < 0) continue;
-    const float z = q[k] - most, w = expf(z) / total;
+    const float z = (q[k] - most) / a.temperature, w = expf(z) / total;
     if (!(w == 0.f)) konst += w * (z - log_total);
     else ids[k] = -1;   // (nothing wanted of it)
     q[k] = w;

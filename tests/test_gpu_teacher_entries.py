@@ -32,3 +32,16 @@ def test_entries_that_are_none(ops, gpu, dtype):  # noqa: F811
     loss = ops.distillation(leaves[0], leaves[1], ids.to(gpu), z.to(gpu), bias=leaves[2])
     assert torch.isnan(loss).nonzero().tolist() == [[1]]
     assert not torch.autograd.grad(loss.sum(), leaves[0])[0][1].any()
+
+
+@pytest.mark.parametrize("T", [0.01, 0.5, 1.0])
+def test_logits_at_the_ends_of_float32(ops, gpu, T):  # noqa: F811
+    """Logits whose quotient by the temperature is beyond float32: their distribution is not."""
+    N, V, D = 5, 70, 32
+    g, h, w, b, go = _inputs(7, N, V, D, FP32, False)
+    ids = torch.arange(4).repeat(N, 1) + 3
+    z = torch.tensor([[3e38, 3e38, -3e38, 0.0], [3e38, 1.0, 2.0, -3e38], [-3e38, -3e38, -3.4e38, -math.inf],
+                      [2e38, 2e38, 2e38, 2e38], [1e38, 1e38, 0.0, 0.0]])
+    want, bound = co.loss(h, w, *co.teacher(ids, z, T), go, temperature=T)
+    leaves = [x.to(gpu).requires_grad_() for x in (h, w)]
+    _check(ops.distillation(leaves[0], leaves[1], ids.to(gpu), z.to(gpu), temperature=T), leaves, go, want, bound)
