@@ -45,3 +45,16 @@ def test_logits_at_the_ends_of_float32(ops, gpu, T):  # noqa: F811
     want, bound = co.loss(h, w, *co.teacher(ids, z, T), go, temperature=T)
     leaves = [x.to(gpu).requires_grad_() for x in (h, w)]
     _check(ops.distillation(leaves[0], leaves[1], ids.to(gpu), z.to(gpu), temperature=T), leaves, go, want, bound)
+
+
+@pytest.mark.parametrize("T", [1e-10, 1e-25, 1e-30])
+def test_loss_at_temperatures_whose_square_is_lost(ops, gpu, T):  # noqa: F811
+    """T^2 times a divergence of the order of 1 / T is of the order of T."""
+    N, V, D = 5, 70, 32
+    g, h, w, _, go = _inputs(8, N, V, D, FP32, False)
+    ids, z = torch.arange(2).repeat(N, 1) + 3, torch.zeros(N, 2)
+    want, bound = co.loss(h, w, *co.teacher(ids, z, T), go, temperature=T)
+    with torch.no_grad():
+        got = ops.distillation(h.to(gpu), w.to(gpu), ids.to(gpu), z.to(gpu), temperature=T).cpu().double()
+    assert bool((want["loss"] > 100 * bound["loss"]).all())
+    assert bool(((got - want["loss"]).abs() <= bound["loss"]).all())
