@@ -105,7 +105,8 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) 
     const int D = fresh(p.D);
     const int64_t x = int64_t(xt) * XT + wave * 32 + col, xr = min(x, p.V - 1);
     const float b2 = p.bias != nullptr ? bias2(p, xr) : 0.f;
-    load_outer<T>(xf, static_cast<const T *>(p.table) + xr * p.ts, b2 == -INFINITY, D);
+    const bool out = b2 == -INFINITY;
+    load_outer<T>(xf, static_cast<const T *>(p.table) + xr * p.ts, out, D);
     float db = 0.f, sc = kFirstScale;
     f32x16 o[OB];
 #pragma unroll
@@ -205,7 +206,8 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) 
 
     const int width = fresh(p.D);
     const bool whole = first == 0 && end == line.inner;
-    const float sum = pair_sum(db), by = HALF ? p.scale / sc : p.scale;
+    const float sum = out ? 0.f : pair_sum(db), by = HALF ? p.scale / sc : p.scale;
+    // (a row that is not finite makes NaN of every candidate that is in, and of those only)
     if (x < p.V) {
       if (!whole) {
         float *row = a.part + (int64_t(w + xt) * XT + wave * 32 + col) * (DP + 4);
@@ -215,7 +217,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) 
           for (int i = 0; i < 4; ++i) {
             float y[4];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) y[v] = o[d][4 * i + v] * by;
+            for (int v = 0; v < 4; ++v) y[v] = out ? 0.f : o[d][4 * i + v] * by;
             store_n(row + 32 * d + 8 * i + 4 * h, y);
           }
         if (h == 0) row[DP] = sum;
@@ -227,7 +229,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) 
           for (int i = 0; i < 4; ++i) {
             f32x4 y;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) y[v] = o[d][4 * i + v] * by;
+            for (int v = 0; v < 4; ++v) y[v] = out ? 0.f : o[d][4 * i + v] * by;
             attn::store4<T>(row, 32 * d + 8 * i + 4 * h, width, y);
           }
         if (a.dbias != nullptr && h == 0) a.dbias[x] = sum;
