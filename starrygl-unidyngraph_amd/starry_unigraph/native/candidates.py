@@ -23,8 +23,8 @@ import math
 import torch
 
 from starry_unigraph.lib import _capi
-from starry_unigraph.native.history import (_as_rows, _first, _first_order, _guard, _no_grad, _no_tangents, _rows,
-                                            _tensor, _tracked)
+from starry_unigraph.native.history import (_as_rows, _first, _first_order, _guard, _no_grad, _no_tangents, _number,
+                                            _rows, _tensor, _tracked)
 
 MAX_DIM = 256       # channels of a row
 MAX_TARGETS = 1024  # a teacher's entries of a row
@@ -44,12 +44,13 @@ def cross_entropy(h: torch.Tensor, table: torch.Tensor, target: torch.Tensor, *,
     the table may hold anything and have gradients of 0 (a target that is left
     out: the loss is inf and the row has no gradient; if all are, 0).
     Differentiable in h, table and bias. One new event is one row."""
+    scale = _number("scale", scale)
     rows = _check(h, table, bias, scale)
     if target.dtype != torch.int64 or target.shape != h.shape[:-1] or target.device != h.device:
         raise ValueError(f"target: {target.dtype} {tuple(target.shape)} on {target.device}, expected int64 "
                          f"{tuple(h.shape[:-1])} on {h.device}")
     _no_tangents(h, table, bias)
-    return _shaped(_call(rows, table, bias, target.reshape(-1).contiguous(), None, float(scale), 1.0), h)
+    return _shaped(_call(rows, table, bias, target.reshape(-1).contiguous(), None, scale, 1.0), h)
 
 
 def distillation(h: torch.Tensor, table: torch.Tensor, ids: torch.Tensor, logits: torch.Tensor, *,
@@ -66,8 +67,8 @@ def distillation(h: torch.Tensor, table: torch.Tensor, ids: torch.Tensor, logits
     loss 0 and no gradient; one with an id of V or more NaN and none; one that
     wants a candidate that is left out inf and none. Differentiable in h, table and
     bias."""
+    scale, temperature = _number("scale", scale), _number("temperature", temperature)
     rows = _check(h, table, bias, scale)
-    temperature = float(temperature)
     if not (0.0 < temperature < math.inf):
         raise ValueError(f"temperature: {temperature}, expected a positive number")
     if not max(abs(scale), 1.0) / temperature < 2e38 or not temperature < 1e19:
@@ -82,7 +83,7 @@ def distillation(h: torch.Tensor, table: torch.Tensor, ids: torch.Tensor, logits
     _no_grad("logits", logits)
     _no_tangents(h, table, bias, logits)
     entries = (ids.reshape(-1, K).contiguous(), logits.reshape(-1, K).contiguous())
-    return _shaped(_call(rows, table, bias, None, entries, float(scale), temperature), h)
+    return _shaped(_call(rows, table, bias, None, entries, scale, temperature), h)
 
 
 def _check(h, table, bias, scale) -> torch.Tensor:

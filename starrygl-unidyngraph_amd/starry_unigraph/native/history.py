@@ -107,6 +107,14 @@ def _no_grad(name: str, t) -> None:
         raise ValueError(f"{name}: has no gradient here (detach it)")
 
 
+def _number(name: str, value) -> float:
+    """A factor as a number; one that asks for a gradient is refused (it would be dropped)."""
+    if isinstance(value, torch.Tensor):
+        _no_grad(name, value)
+        _no_tangents(value)
+    return float(value)
+
+
 # ------------------------------------------------------------------ gated scan
 def gated_scan(gate: torch.Tensor, value: torch.Tensor, *, lens: torch.Tensor | None = None,
                state: torch.Tensor | None = None, gaps: torch.Tensor | None = None,

@@ -17,7 +17,8 @@ import math
 import torch
 
 from starry_unigraph.lib import _capi
-from starry_unigraph.native.history import _first, _first_order, _guard, _no_tangents, _rows, _tensor, _tracked
+from starry_unigraph.native.history import (_first, _first_order, _guard, _no_tangents, _number, _rows, _tensor,
+                                            _tracked)
 
 
 def frequencies(dims: int, *, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
@@ -82,7 +83,7 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, q_pos: torch.Tensor, k_pos: 
     _tensor("freqs", freqs, q, freqs.shape, torch.float64)
     if freqs.requires_grad:
         raise ValueError("freqs: has no gradient here (detach it)")
-    gain = float(gain)
+    gain = _number("gain", gain)
     if not math.isfinite(gain):
         raise ValueError(f"gain: {gain}")
     _no_tangents(q, k)

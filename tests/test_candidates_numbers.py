@@ -1,0 +1,25 @@
+"""Factors of the losses over all candidates and of the rotation are numbers: a
+tensor that asks for a gradient is refused, not read and dropped."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from starry_unigraph.native import candidates, rotary
+from test_candidates_refusals import _f, _i, anywhere  # noqa: F401
+
+
+def _calls():
+    return {"scale": [lambda x: candidates.cross_entropy(_f(2, 8), _f(5, 8), _i(2), scale=x),
+                      lambda x: candidates.distillation(_f(2, 8), _f(5, 8), _i(2, 3), _f(2, 3), scale=x)],
+            "temperature": [lambda x: candidates.distillation(_f(2, 8), _f(5, 8), _i(2, 3), _f(2, 3), temperature=x)],
+            "gain": [lambda x: rotary.rotate(_f(1, 2, 1, 8), None, _i(1, 2), None, _f(4, dtype=torch.float64), gain=x)]}
+
+
+@pytest.mark.parametrize("name", ["scale", "temperature", "gain"])
+def test_gradients_are_refused(anywhere, name):  # noqa: F811
+    for call in _calls()[name]:
+        for x in (torch.ones(()).requires_grad_(), torch.nn.Parameter(torch.ones(1))):
+            with pytest.raises(ValueError, match=f"{name}: has no gradient"):
+                call(x)
+        with fwd.dual_level(), pytest.raises(NotImplementedError):
+            call(fwd.make_dual(torch.ones(()), torch.ones(())))
