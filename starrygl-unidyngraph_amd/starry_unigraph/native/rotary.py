@@ -84,8 +84,8 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, q_pos: torch.Tensor, k_pos: 
     if freqs.requires_grad:
         raise ValueError("freqs: has no gradient here (detach it)")
     gain = _number("gain", gain)
-    if not math.isfinite(gain):
-        raise ValueError(f"gain: {gain}")
+    if not abs(gain) <= torch.finfo(torch.float32).max:
+        raise ValueError(f"gain: {gain}, expected a number in float32's range")
     _no_tangents(q, k)
     args = (q, k, q_pos, k_pos, freqs.contiguous(), bool(interleaved), gain)
     if _tracked(q, k):

@@ -23,3 +23,9 @@ def test_gradients_are_refused(anywhere, name):  # noqa: F811
                 call(x)
         with fwd.dual_level(), pytest.raises(NotImplementedError):
             call(fwd.make_dual(torch.ones(()), torch.ones(())))
+
+
+@pytest.mark.parametrize("gain", [1e39, -1e300, float("nan"), float("-inf")])
+def test_gains_beyond_float32_are_refused(anywhere, gain):  # noqa: F811
+    with pytest.raises(ValueError, match="gain"):
+        _calls()["gain"][0](gain)
