@@ -47,13 +47,23 @@ class HistoryEncoder(nn.Module):
         if positions == "bias":
             self.age_bias = nn.Parameter(torch.zeros(heads, buckets))
         else:
-            self.register_buffer("freqs", rotary.frequencies(dim // heads // 2 * 2, scaling="linear",
-                                                             factor=1.0 / self.per_gap, device="cpu"), persistent=False)
+            freqs = rotary.frequencies(dim // heads // 2 * 2, scaling="linear", factor=1.0 / self.per_gap, device="cpu")
+            # (as integers: a module's casts leave their 64 bits alone)
+            self.register_buffer("freq_bits", freqs.view(torch.int64), persistent=False)
         self.out = nn.Linear(dim, 2 * dim)
         self.norms = nn.ParameterDict({
             **{f"{at}_{w}_{k}": nn.Parameter((torch.ones if k == "w" else torch.zeros)(dim))
                for at in ("event", "root") for w in ("post", "pre") for k in ("w", "b")},
             **{f"{at}_scale": nn.Parameter(torch.ones(dim)) for at in ("event", "root")}})
+
+    @property
+    def freqs(self) -> torch.Tensor:
+        """The rotary frequencies, float64 [pairs]."""
+        return self.freq_bits.view(torch.float64)
+
+    @freqs.setter
+    def freqs(self, value: torch.Tensor) -> None:
+        self.freq_bits = value.to(torch.float64).view(torch.int64)
 
     def _norm(self, at: str, x, z, gate):
         n = self.norms
