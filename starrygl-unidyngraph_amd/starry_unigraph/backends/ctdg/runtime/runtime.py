@@ -28,6 +28,7 @@ import torch
 import torch.nn.functional as F
 
 from starry_unigraph.lib import _capi
+from starry_unigraph.native.candidates import MAX_TARGETS
 from starry_unigraph.native.step import Bf16Shadow, ConvDims, DeviceStep, FusedAdam, StepParamUpdate
 
 from .data import CTDGDataBatch, TGTemporalDataset
@@ -172,10 +173,8 @@ class CTDGOnlineRuntime:
         # its products in bf16 (the fused update keeps them current; dirty:
         # rebuild from the parameters before the next step)
         self._bf16: Bf16Shadow | None = None
-        # a larger model's answers that the next-node objective learns from as
-        # well (set_teacher), and those of the step at hand
+        # a larger model that the next-node objective learns from as well (set_teacher)
         self._teacher: tuple | None = None
-        self._taught: tuple | None = None
         self._bf16_dirty = True
         self._bf16_ver: tuple = ()
         self._back_metrics = False
@@ -431,6 +430,8 @@ class CTDGOnlineRuntime:
 
     def _forward(self, batch: CTDGDataBatch, split: str, train: bool) -> StepTensors:
         n = batch.size
+        # (first: what it raises leaves the negatives, the memory and the parameters as they were)
+        taught = self._answers(batch) if train and self._teacher is not None else None
         if n > self.steps[0].buf.max_batch or self._dropout_passes() != self._passes:
             self._make_steps(max(n, self.steps[0].buf.max_batch))
             self.reset_plans()
@@ -456,8 +457,7 @@ class CTDGOnlineRuntime:
             neg = buf[off:off + n] if off >= 0 else buf
             self._front_body(step, split, n, src, dst, neg, ts, ef, None)
             self._commit_body(step, train)
-            self._taught = self._teacher[0](batch) if train and self._teacher is not None else None
-            self._back_body(step, train, n, dst, neg)
+            self._back_body(step, train, n, (dst, neg, taught))
             self.fence()
         else:
             # the negatives must sit at the batch's place in the stream-wide array
@@ -582,15 +582,15 @@ class CTDGOnlineRuntime:
         if train and not self._hist:
             self._param_update(step).advance()
 
-    def _back_body(self, step: DeviceStep, train: bool, n: int, dst=None, neg=None) -> None:
+    def _back_body(self, step: DeviceStep, train: bool, n: int, nodes: tuple | None = None) -> None:
         """Attention forward, edge predictor + BCE and, in training, the
-        backward and the fused weight-gradient + Adam update. ``dst``, ``neg``:
-        the batch's destinations and negatives (the history embedding alone:
-        its steps are not planned)."""
+        backward and the fused weight-gradient + Adam update. ``nodes``: the
+        batch's destinations, negatives and teacher's answers (the history
+        embedding alone: its steps are not planned)."""
         core = self._core()
         conv = core.conv
         if self._hist:
-            self._history_back(step, train, n, dst, neg)
+            self._history_back(step, train, n, nodes)
             self._metrics_op(step, n)
             return
         efeat_all = self._dev["edge_feat"]
@@ -626,7 +626,7 @@ class CTDGOnlineRuntime:
             upd.run()
         self._metrics_op(step, n)
 
-    def _history_back(self, step: DeviceStep, train: bool, n: int, dst: torch.Tensor, neg: torch.Tensor) -> None:
+    def _history_back(self, step: DeviceStep, train: bool, n: int, nodes: tuple) -> None:
         """The back part of the history embedding: embeddings, edge predictor
         and BCE (runtime.py:197-199), or the next-node objective, and, in training, autograd's backward
         into the optimizer's flat gradients and its step."""
@@ -635,7 +635,7 @@ class CTDGOnlineRuntime:
         with torch.set_grad_enabled(train):
             y = core.roots(step, self.dims)
             if self._next_node:
-                out, loss = self._next_node_loss(core, y[b.ridx_src[:n]], dst, neg)
+                out, loss = self._next_node_loss(core, y[b.ridx_src[:n]], *nodes)
             else:
                 out = core(y[b.ridx_src[:n]], y[b.ridx_dst[:n]], y[b.ridx_neg[:n]])
                 # BCE of 1 and 0 on the logits
@@ -648,18 +648,19 @@ class CTDGOnlineRuntime:
         b.neg[:n].copy_(out.neg_logits.detach())
         b.loss.copy_(loss.detach())
 
-    def _next_node_loss(self, core, src: torch.Tensor, dst: torch.Tensor, neg: torch.Tensor) -> tuple:
+    def _next_node_loss(self, core, src: torch.Tensor, dst: torch.Tensor, neg: torch.Tensor,
+                        taught: tuple | None) -> tuple:
         """(logits, loss) of the next-node objective: the mean cross entropy of
         the destinations over all candidates, and with a teacher its
         divergence. ``src``: the sources' embeddings; ``dst``, ``neg``: node
-        ids (a drawn negative is seldom one of the batch's roots)."""
+        ids (a drawn negative is seldom one of the batch's roots); ``taught``:
+        the teacher's (ids, logits, weight, temperature) or None."""
         with torch.no_grad():
             out = core(src, dst, neg)
         h = core.src_fc(src)
         loss = core.head.loss(h, dst).mean()
-        if self._taught is not None:
-            (ids, logits), self._taught = self._taught, None
-            _, weight, temperature = self._teacher
+        if taught is not None:
+            ids, logits, weight, temperature = taught
             loss = (1.0 - weight) * loss + weight * core.head.distill(h, ids, logits, temperature).mean()
         return out, loss
 
@@ -669,8 +670,9 @@ class CTDGOnlineRuntime:
         (node ids int64 [n, K], logits float32 [n, K]) on the runtime's device
         (a negative id, one that is no candidate, or a logit of -inf: no
         entry). The step's loss is then ``(1 - weight) * cross entropy + weight *
-        divergence`` at ``temperature``. None: no teacher. The reference has no
-        counterpart."""
+        divergence`` at ``temperature``. It is asked before the step: an error
+        of its own, or an answer of another form (ValueError), leaves the
+        runtime as it was. None: no teacher. The reference has no counterpart."""
         if not self._next_node:
             raise ValueError("set_teacher: needs ctdg.embedding = history and ctdg.objective = next_node")
         if not 0.0 <= weight <= 1.0:
@@ -678,6 +680,23 @@ class CTDGOnlineRuntime:
         if not 0.0 < temperature < float("inf"):
             raise ValueError(f"set_teacher: temperature {temperature}, expected a positive number")
         self._teacher = None if teacher is None else (teacher, float(weight), float(temperature))
+
+    def _answers(self, batch: CTDGDataBatch) -> tuple:
+        """The teacher's (ids, logits, weight, temperature) of a batch, checked."""
+        teacher, weight, temperature = self._teacher
+        ids, logits = teacher(batch)
+        if ids.dtype not in (torch.int64, torch.int32) or logits.dtype != torch.float32:
+            raise ValueError(f"teacher: ids of {ids.dtype} and logits of {logits.dtype}, expected int64 and float32")
+        if ids.dim() != 2 or ids.shape[0] != batch.size or not 1 <= ids.shape[1] <= MAX_TARGETS or \
+                logits.shape != ids.shape:
+            raise ValueError(f"teacher: ids {tuple(ids.shape)} and logits {tuple(logits.shape)}, expected both "
+                             f"[{batch.size}, K], K from 1 to {MAX_TARGETS}")
+        on = self._dev["src"].device
+        if ids.device != on or logits.device != on:
+            raise ValueError(f"teacher: ids on {ids.device} and logits on {logits.device}, expected {on}")
+        if logits.requires_grad:
+            raise ValueError("teacher: logits: has no gradient here (detach it)")
+        return ids, logits, weight, temperature
 
     def _metrics_op(self, step: DeviceStep, n: int) -> None:
         """The step's metrics into the next ring slot as the last op of its
