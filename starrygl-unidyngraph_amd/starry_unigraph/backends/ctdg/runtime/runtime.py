@@ -28,7 +28,7 @@ import torch
 import torch.nn.functional as F
 
 from starry_unigraph.lib import _capi
-from starry_unigraph.native.candidates import MAX_TARGETS
+from starry_unigraph.native.candidates import MAX_TARGETS, check_temperature
 from starry_unigraph.native.step import Bf16Shadow, ConvDims, DeviceStep, FusedAdam, StepParamUpdate
 
 from .data import CTDGDataBatch, TGTemporalDataset
@@ -675,11 +675,17 @@ class CTDGOnlineRuntime:
         runtime as it was. None: no teacher. The reference has no counterpart."""
         if not self._next_node:
             raise ValueError("set_teacher: needs ctdg.embedding = history and ctdg.objective = next_node")
+        for name, x in (("weight", weight), ("temperature", temperature)):
+            if getattr(x, "requires_grad", False):
+                raise ValueError(f"set_teacher: {name} has no gradient here (detach it)")
+        weight, temperature = float(weight), float(temperature)
         if not 0.0 <= weight <= 1.0:
             raise ValueError(f"set_teacher: weight {weight}, expected 0 to 1")
-        if not 0.0 < temperature < float("inf"):
-            raise ValueError(f"set_teacher: temperature {temperature}, expected a positive number")
-        self._teacher = None if teacher is None else (teacher, float(weight), float(temperature))
+        try:
+            check_temperature(temperature)
+        except ValueError as e:
+            raise ValueError(f"set_teacher: {e}") from None
+        self._teacher = None if teacher is None else (teacher, weight, temperature)
 
     def _answers(self, batch: CTDGDataBatch) -> tuple:
         """The teacher's (ids, logits, weight, temperature) of a batch, checked."""

@@ -69,10 +69,7 @@ def distillation(h: torch.Tensor, table: torch.Tensor, ids: torch.Tensor, logits
     bias."""
     scale, temperature = _number("scale", scale), _number("temperature", temperature)
     rows = _check(h, table, bias, scale)
-    if not (0.0 < temperature < math.inf):
-        raise ValueError(f"temperature: {temperature}, expected a positive number")
-    if not max(abs(scale), 1.0) / temperature < 2e38 or not temperature < 1e19:
-        raise ValueError(f"temperature: {temperature} with a scale of {scale} is out of float32's range")
+    check_temperature(temperature, scale)
     if ids.dtype != torch.int64 or ids.dim() != h.dim() or ids.shape[:-1] != h.shape[:-1] or ids.device != h.device:
         raise ValueError(f"ids: {ids.dtype} {tuple(ids.shape)} on {ids.device}, expected int64 "
                          f"[{', '.join(str(n) for n in h.shape[:-1])}, K] on {h.device}")
@@ -84,6 +81,14 @@ def distillation(h: torch.Tensor, table: torch.Tensor, ids: torch.Tensor, logits
     _no_tangents(h, table, bias, logits)
     entries = (ids.reshape(-1, K).contiguous(), logits.reshape(-1, K).contiguous())
     return _shaped(_call(rows, table, bias, None, entries, scale, temperature), h)
+
+
+def check_temperature(temperature: float, scale: float = 1.0) -> None:
+    """Refuses a temperature that :func:`distillation` does not take."""
+    if not (0.0 < temperature < math.inf):
+        raise ValueError(f"temperature: {temperature}, expected a positive number")
+    if not max(abs(scale), 1.0) / temperature < 2e38 or not temperature < 1e19:
+        raise ValueError(f"temperature: {temperature} with a scale of {scale} is out of float32's range")
 
 
 def _check(h, table, bias, scale) -> torch.Tensor:

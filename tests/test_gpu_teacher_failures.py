@@ -59,3 +59,15 @@ def test_a_failed_step_leaves_nothing(gpu, plain, what):
     assert got[0] == plain[0]
     assert got[1]["loss"] == plain[1]["loss"] and got[1]["predictions"] == plain[1]["predictions"]
     assert torch.equal(got[2], plain[2])
+
+
+def test_temperatures_that_the_step_refuses(gpu):
+    rt = _runtime()
+    for kw in (dict(temperature=1e-39), dict(temperature=1e20), dict(temperature=-1.0), dict(temperature=float("nan")),
+               dict(temperature=torch.ones(()).requires_grad_()), dict(weight=torch.ones(()).requires_grad_())):
+        with pytest.raises(ValueError, match="set_teacher"):
+            rt.set_teacher(_teacher(rt), **kw)
+    batch = list(rt.iter_batches("train", 50))[200]
+    for T in (1e-30, 1e18):   # the ends of what is taken: the step takes them too
+        rt.set_teacher(_teacher(rt), weight=0.0, temperature=T)
+        rt.train_step(batch)
