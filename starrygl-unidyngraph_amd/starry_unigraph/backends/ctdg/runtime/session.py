@@ -2,11 +2,12 @@
 from __future__ import annotations
 
 from pathlib import Path
-from typing import Any
+from typing import Any, Iterable
 
 import torch
 
 from starry_unigraph.backends.ctdg.preprocess import CTDGPreprocessor
+from starry_unigraph.runtime.modules import CandidateHead
 from starry_unigraph.types import PreparedArtifacts, RuntimeBundle, SessionContext
 
 from .factory import build_ctdg_runtime
@@ -74,10 +75,12 @@ class CTDGSession:
         ckpt = torch.load(str(path), map_location="cpu", weights_only=True)
         model = rt.model
         core = model.module if hasattr(model, "module") else model
-        _check_state_keys(type(core).__name__, core.state_dict(), ckpt["model"])
+        loaded = dict(ckpt["model"])
+        wrong = [m.match_nodes(loaded, f"{name}.") for name, m in core.named_modules() if isinstance(m, CandidateHead)]
+        _check_state_keys(type(core).__name__, core.state_dict(), loaded, [w for w in wrong if w is not None])
         with torch.no_grad():
             own = core.state_dict()
-            for name, t in ckpt["model"].items():
+            for name, t in loaded.items():
                 own[name].copy_(t)
             if rt.memory_updater is not None and "memory_updater" in ckpt:
                 rt.memory_updater.load_state_dict(ckpt["memory_updater"])
@@ -86,12 +89,13 @@ class CTDGSession:
         rt.fence()
 
 
-def _check_state_keys(owner: str, own: dict, loaded: dict) -> None:
+def _check_state_keys(owner: str, own: dict, loaded: dict, wrong: Iterable[str] = ()) -> None:
     """The strict checks of nn.Module.load_state_dict (same message form):
-    missing and unexpected keys and shape mismatches raise RuntimeError."""
+    missing and unexpected keys, shape mismatches and what modules found
+    ``wrong`` raise RuntimeError."""
     missing = [k for k in own if k not in loaded]
     unexpected = [k for k in loaded if k not in own]
-    errs = []
+    errs = list(wrong)
     if unexpected:
         errs.append("Unexpected key(s) in state_dict: " + ", ".join(f'"{k}"' for k in unexpected) + ". ")
     if missing:

@@ -12,7 +12,9 @@ from starry_unigraph.native import candidates
 
 class CandidateHead(nn.Module):
     """Scores ``<h, table_v> + bias_v`` of rows ``h`` [N, dim] over ``nodes``,
-    the node ids (distinct, each in [0, num_nodes)) that may come next."""
+    the node ids (distinct, each in [0, num_nodes)) that may come next. Row i of
+    the table is of ``nodes[i]``: the ids are kept in the state, and a state of
+    other ids is refused (one of before they were kept is taken as of these)."""
 
     def __init__(self, nodes: torch.Tensor, num_nodes: int, dim: int) -> None:
         super().__init__()
@@ -27,7 +29,25 @@ class CandidateHead(nn.Module):
             raise ValueError("candidate head: a node id given twice")
         self.table = nn.Parameter(torch.randn(nodes.numel(), dim) * dim ** -0.5)
         self.bias = nn.Parameter(torch.zeros(nodes.numel()))
+        self.register_buffer("nodes", nodes.clone())
         self.register_buffer("row_of", rows, persistent=False)
+
+    def match_nodes(self, state: dict, prefix: str) -> str | None:
+        """What is wrong with the node ids in a state that is to be loaded
+        (None: nothing; ids that it lacks are added to it)."""
+        ids = state.setdefault(prefix + "nodes", self.nodes)
+        if ids.shape == self.nodes.shape and not torch.equal(ids.to(self.nodes.device), self.nodes):
+            return f"{prefix}nodes: the table's rows are of other nodes."
+        return None
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                              error_msgs):
+        wrong = self.match_nodes(state_dict, prefix)
+        if wrong is not None:
+            error_msgs.append(wrong)
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                                      error_msgs)
 
     def rows(self, ids: torch.Tensor) -> torch.Tensor:
         """The table's rows of node ids; -1 for those that are no candidate."""
