@@ -421,7 +421,7 @@ struct RowCoef {
 void route_targets(int32_t dtype, const Problem &p, int K, const int32_t *ids, const float *weight, int32_t *index,
                    int2 *entries, hipStream_t stream);
 constexpr int kGradBlock = 32;   // candidates of a wave
-// fp32 elements of `part` at most (those of tiles that are not shared out are never touched).
+// fp32 elements of `part`: whatever the table's size, two pieces a workgroup.
 int64_t table_grad_part(int32_t dtype, const Problem &p);
 void table_grad(int32_t dtype, const Problem &p, const RowCoef &r, void *dtable, float *dbias, float *part,
                 hipStream_t stream);

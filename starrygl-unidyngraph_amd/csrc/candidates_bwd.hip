@@ -19,6 +19,10 @@ struct BwdArgs {
   void *dtable;
   float *dbias, *part;   // part: [pieces][candidates of a workgroup][dp + 4]
 };
+// Pieces of tiles that are shared out, the only ones that are kept apart: a
+// workgroup has two at most, one of a tile begun earlier (2 w) and one of a tile
+// that it begins and leaves (2 w + 1).
+__device__ __forceinline__ int64_t shared_piece(int64_t w, bool begins) { return 2 * w + (begins ? 1 : 0); }
 
 // fp16: a coefficient goes into the product times a power of two a candidate
 // that follows its largest magnitude so far (from a start that any value
@@ -210,7 +214,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void k_table_grad(BwdArgs a) 
     // (a row that is not finite makes NaN of every candidate that is in, and of those only)
     if (x < p.V) {
       if (!whole) {
-        float *row = a.part + (int64_t(w + xt) * XT + wave * 32 + col) * (DP + 4);
+        float *row = a.part + (shared_piece(w, first == 0) * XT + wave * 32 + col) * (DP + 4);
 #pragma unroll
         for (int d = 0; d < OB; ++d)
 #pragma unroll
@@ -253,18 +257,19 @@ __global__ __launch_bounds__(kBlock) void k_join_grad(BwdArgs a, int xtile, int 
   const int64_t u = line.begin(w), xt = u / line.inner;
   if (u == xt * line.inner || line.begin(w - 1) > xt * line.inner) return;
   const int64_t w0 = w - 1, w1 = line.group_of((xt + 1) * line.inner - 1);
-  const int ld = dp + 4, n = int(w1 - w0) + 1, units = (p.D + 3) / 4 + 1;   // four columns a thread, and the bias
+  const int ld = dp + 4, n = int(w1 - w0), units = (p.D + 3) / 4 + 1;   // four columns a thread, and the bias
   const int64_t step = int64_t(xtile) * ld;
-  const float *first = a.part + (w0 + xt) * step;
+  // (the tile's first piece begins it, the others are of tiles begun earlier)
+  const float *first = a.part + shared_piece(w0, true) * step, *rest = a.part + shared_piece(w, false) * step;
   const int rows = int(min(int64_t(xtile), p.V - xt * xtile));
   const int r0 = rows * part / kJoin, r1 = rows * (part + 1) / kJoin;
   for (int i = threadIdx.x; i < (r1 - r0) * units; i += kBlock) {
     const int r = r0 + i / units, c = i % units, d = c == units - 1 ? dp : 4 * c;
     const int64_t v = xt * xtile + r;
-    const float *src = first + int64_t(r) * ld + d;
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    const int64_t at = int64_t(r) * ld + d;
+    f32x4 x = *reinterpret_cast<const f32x4 *>(first + at);
 #pragma unroll 4
-    for (int s = 0; s < n; ++s) x += *reinterpret_cast<const f32x4 *>(src + s * step);
+    for (int s = 0; s < n; ++s) x += *reinterpret_cast<const f32x4 *>(rest + 2 * s * step + at);
     if (d == dp) {
       if (a.dbias != nullptr) a.dbias[v] = x[0];
     } else {
@@ -362,8 +367,9 @@ Image grad_image(int32_t dtype, int D) {
 int64_t table_grad_part(int32_t dtype, const Problem &p) {
   return pick_dim(dtype, p.D, [&](auto t, auto db, auto) {
     using P = Plan<decltype(t), db.value>;
-    constexpr int64_t xtile = 32 * P::WAVES;
-    return ((p.V + xtile - 1) / xtile + P::GROUPS) * xtile * (32 * db.value + 4);
+    constexpr int64_t xtile = 32 * P::WAVES, ytile = Tiles<decltype(t), db.value>::YT;
+    const Line line((p.V + xtile - 1) / xtile, (p.N + ytile - 1) / ytile, P::GROUPS);
+    return 2 * int64_t(line.groups) * xtile * (32 * db.value + 4);
   });
 }
 
