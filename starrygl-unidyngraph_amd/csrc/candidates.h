@@ -249,12 +249,26 @@ __device__ __forceinline__ float max16(const V &p) {
     for (int i = 0; i < d; ++i) a[i] = fmaxf(a[i], a[i + d]);
   return a[0];
 }
+// Every block an operand of what stands between: no product of theirs is moved
+// across it in either direction.
+template <int NB>
+__device__ __forceinline__ void settle_blocks(f32x16 (&o)[NB]) {
+  static_assert(NB <= 8, "operands of one statement");
+  if constexpr (NB == 8)
+    asm volatile("s_nop 15\n\ts_nop 15" : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]), "+a"(o[4]), "+a"(o[5]),
+                 "+a"(o[6]), "+a"(o[7]));
+  else if constexpr (NB == 6)
+    asm volatile("s_nop 15\n\ts_nop 15" : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]), "+a"(o[4]), "+a"(o[5]));
+  else static_assert(NB == 6, "blocks of rows of 192 and 256 channels");
+}
 // Accumulator blocks times a factor. With one wave a SIMD (ALONE) they lie in
 // the matrix unit's own registers, and the factor is applied in place by hand:
 // behind a branch that is seldom taken the compiler otherwise keeps the blocks
 // in two places and moves all of them on the path that does nothing (128 moves
-// a step of 256 channels). The waits are a matrix product's before its
-// result is read and a write's before the next one.
+// a step of 256 channels). The waits before and behind it are a matrix product's
+// before its result is read (19 of the 32 wait states after one of 16 passes) and a
+// write's before the next one; the blocks pass through them, so that no product
+// stands between a wait and what it is for.
 template <bool ALONE, int NB>
 __device__ __forceinline__ void scale_blocks(f32x16 (&o)[NB], float by) {
   if constexpr (!ALONE) {
@@ -262,28 +276,29 @@ __device__ __forceinline__ void scale_blocks(f32x16 (&o)[NB], float by) {
     for (int d = 0; d < NB; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] *= by;
-    return;
+  } else {
+    settle_blocks(o);
+#pragma unroll
+    for (int d = 0; d < NB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        float x[4], t[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = o[d][r + i];
+        asm volatile("v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\t"
+                     "v_accvgpr_read_b32 %6, %2\n\tv_accvgpr_read_b32 %7, %3\n\t"
+                     "v_mul_f32 %4, %4, %8\n\tv_mul_f32 %5, %5, %8\n\t"
+                     "v_mul_f32 %6, %6, %8\n\tv_mul_f32 %7, %7, %8\n\t"
+                     "v_accvgpr_write_b32 %0, %4\n\tv_accvgpr_write_b32 %1, %5\n\t"
+                     "v_accvgpr_write_b32 %2, %6\n\tv_accvgpr_write_b32 %3, %7"
+                     : "+a"(x[0]), "+a"(x[1]), "+a"(x[2]), "+a"(x[3]), "=&v"(t[0]), "=&v"(t[1]), "=&v"(t[2]),
+                       "=&v"(t[3])
+                     : "v"(by));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d][r + i] = x[i];
+      }
+    settle_blocks(o);
   }
-  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-#pragma unroll
-  for (int d = 0; d < NB; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      float x[4], t[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = o[d][r + i];
-      asm volatile("v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\t"
-                   "v_accvgpr_read_b32 %6, %2\n\tv_accvgpr_read_b32 %7, %3\n\t"
-                   "v_mul_f32 %4, %4, %8\n\tv_mul_f32 %5, %5, %8\n\t"
-                   "v_mul_f32 %6, %6, %8\n\tv_mul_f32 %7, %7, %8\n\t"
-                   "v_accvgpr_write_b32 %0, %4\n\tv_accvgpr_write_b32 %1, %5\n\t"
-                   "v_accvgpr_write_b32 %2, %6\n\tv_accvgpr_write_b32 %3, %7"
-                   : "+a"(x[0]), "+a"(x[1]), "+a"(x[2]), "+a"(x[3]), "=&v"(t[0]), "=&v"(t[1]), "=&v"(t[2]), "=&v"(t[3])
-                   : "v"(by));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[d][r + i] = x[i];
-    }
-  asm volatile("s_nop 15" ::: "memory");
 }
 template <typename V>
 __device__ __forceinline__ float abs_max16(const V &p) {   // (three operands an instruction)
