@@ -410,7 +410,6 @@ struct Partials {
   int64_t ytiles;
   int rows, wy, dp, groups, ones;
 };
-int padded_dim(int D);
 Partials forward_shape(int32_t dtype, const Problem &p);   // (without its arrays)
 void forward_partials(int32_t dtype, const Problem &p, const Order &order, const Partials &out, hipStream_t stream);
 

@@ -257,8 +257,6 @@ void pick(const FwdArgs &a, hipStream_t stream) {
 namespace sgl {
 namespace cand {
 
-int padded_dim(int D) { return (D + 63) / 64 * 64; }
-
 Partials forward_shape(int32_t dtype, const Problem &p) {
   return pick_dim(dtype, p.D, [&](auto t, auto db, auto cut) {
     return shape_of<decltype(t), db.value, kForwardCut<db.value, cut.value>>(p);
