@@ -86,7 +86,7 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, q_pos: torch.Tensor, k_pos: 
     gain = _number("gain", gain)
     if not abs(gain) <= torch.finfo(torch.float32).max:
         raise ValueError(f"gain: {gain}, expected a number in float32's range")
-    _no_tangents(q, k)
+    _no_tangents(q, k, freqs)
     args = (q, k, q_pos, k_pos, freqs.contiguous(), bool(interleaved), gain)
     if _tracked(q, k):
         return _Rotate.apply(*args)

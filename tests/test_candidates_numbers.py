@@ -29,3 +29,9 @@ def test_gradients_are_refused(anywhere, name):  # noqa: F811
 def test_gains_beyond_float32_are_refused(anywhere, gain):  # noqa: F811
     with pytest.raises(ValueError, match="gain"):
         _calls()["gain"][0](gain)
+
+
+def test_a_tangent_of_the_frequencies_is_refused(anywhere):  # noqa: F811
+    f = _f(4, dtype=torch.float64)
+    with fwd.dual_level(), pytest.raises(NotImplementedError):
+        rotary.rotate(_f(1, 2, 1, 8), None, _i(1, 2), None, fwd.make_dual(f, f))
