@@ -39,12 +39,15 @@ def frequencies(dims: int, *, base: float = 10000.0, scaling: str = "none", fact
     if not (base > 0 and math.isfinite(base)) or not (factor > 0 and math.isfinite(factor)):
         raise ValueError(f"base {base}, factor {factor}: expected positive numbers")
     if scaling == "base" and dims > 2:
+        log = math.log(base) + math.log(factor) * (dims / (dims - 2))
+        if not abs(log) < 708.0:   # (float64's range)
+            raise ValueError(f"base {base} raised for a factor of {factor} is out of range")
         base = base * factor ** (dims / (dims - 2))
     f = base ** (torch.arange(0, dims, 2, dtype=torch.float64) * (-1.0 / max(dims, 1)))
     if scaling == "linear":
         f = f / factor
     elif scaling == "wavelength":
-        if trained is None or trained < 1 or not low < high:
+        if trained is None or not 1 <= trained < math.inf or not -math.inf < low < high:
             raise ValueError(f"wavelength scaling: trained {trained}, low {low}, high {high}")
         keep = ((f * (trained / (2.0 * math.pi)) - low) / (high - low)).clamp(0.0, 1.0)
         f = f * keep + f / factor * (1.0 - keep)

@@ -35,3 +35,14 @@ def test_a_tangent_of_the_frequencies_is_refused(anywhere):  # noqa: F811
     f = _f(4, dtype=torch.float64)
     with fwd.dual_level(), pytest.raises(NotImplementedError):
         rotary.rotate(_f(1, 2, 1, 8), None, _i(1, 2), None, fwd.make_dual(f, f))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(scaling="base", factor=1e300), dict(scaling="base", base=1e-300, factor=1e-10),
+    dict(scaling="wavelength", trained=float("nan")), dict(scaling="wavelength", trained=float("inf")),
+    dict(scaling="wavelength", trained=8192, low=float("-inf")),
+    dict(scaling="wavelength", trained=8192, low=float("nan")),
+    dict(scaling="wavelength", trained=8192, high=float("nan"))])
+def test_frequencies_without_angles_are_refused(kw):
+    with pytest.raises(ValueError):
+        rotary.frequencies(8, device="cpu", **kw)
