@@ -3,10 +3,11 @@
 //
 // (a, b) -> gain (a cos t - b sin t, a sin t + b cos t), t = position * f_i.
 // The angle is kept in turns, as a 64-bit fraction: position times f_i / 2 pi
-// modulo 1 is an integer product, and with f_i / 2 pi to 128 bits it is within
-// 2^-63 of a turn at every int64 position (a float angle of a position of 1e9 has
-// no digits left of the turn, a 64-bit f_i / 2 pi is 0.6 rad off at nanosecond
-// stamps of 1.7e18). The gradient is the same rotation the other way round.
+// modulo 1 is an integer product, and with f_i / 2 pi to 96 bits it is within
+// 2^-32 of a turn (1.5e-9 rad) at every int64 position (a float angle of a position
+// of 1e9 has no digits left of the turn, a 64-bit f_i / 2 pi is 0.6 rad off at
+// nanosecond stamps of 1.7e18). The gradient is the same rotation the other way
+// round.
 //
 // Memory bounds it, every element read and written once: 16 sequences of 8,191
 // x (8 + 2) heads of 128 in fp16 120 us, 5.6 TB/s (a large copy: 5.1); 4,000 x
@@ -53,14 +54,24 @@ __device__ __forceinline__ void sincos_turns(uint64_t turns, float &s, float &c)
   c = ((quarter + 1) & 2) != 0 ? -v : v;
 }
 
-// A frequency (angle a unit of position) in turns, modulo 1: (hi 2^64 + lo) / 2^128.
-// The last bit marks one that has no angle (not finite, or 2^128 and more).
+// A frequency (angle a unit of position) in turns, modulo 1: (hi 2^32 + lo) / 2^96.
+// The last bit marks one that has no angle (not finite, or 2^128 and more). (128 bits
+// take two products more a pair: 4,000 x 52 x 4 heads of 43 in bf16 38.5 us for 37.3.)
 struct Step {
-  uint64_t hi, lo;
+  uint64_t hi;
+  uint32_t lo;
 };
-// m 2^e / 2 pi of a double m 2^e, with 1 / 2 pi to 320 bits: as many behind a
-// turn's point as a position has in front of it, and 64 more, for any
-// frequency under 2^128.
+struct Steps {   // a workgroup's, in LDS of kStepBytes for each
+  uint64_t *hi;
+  uint32_t *lo;
+  __device__ __forceinline__ Steps(char *lds, int n)
+      : hi(reinterpret_cast<uint64_t *>(lds)), lo(reinterpret_cast<uint32_t *>(hi + n)) {}
+  __device__ __forceinline__ void put(int i, const Step &s) const { hi[i] = s.hi, lo[i] = s.lo; }
+  __device__ __forceinline__ Step at(int i) const { return Step{hi[i], lo[i]}; }
+};
+constexpr size_t kStepBytes = sizeof(uint64_t) + sizeof(uint32_t);
+// m 2^e / 2 pi of a double m 2^e, with 1 / 2 pi to 320 bits: enough behind the
+// point of a turn for any frequency under 2^128.
 __device__ __forceinline__ Step turn_step(double f) {
   constexpr uint64_t kInv[5] = {0x28be60db9391054aull, 0x7f09d5f47d4d3770ull, 0x36d8a5664f10e410ull,
                                 0x7f9458eaf7aef158ull, 0x6dc91b8e909374b8ull};
@@ -81,24 +92,25 @@ __device__ __forceinline__ Step turn_step(double f) {
   const uint64_t p1 = m * w1 + __umul64hi(m, w2), c1 = p1 < m * w1 ? 1 : 0;
   const uint64_t t = m * w0 + __umul64hi(m, w1), p2 = t + c1;
   const uint64_t p3 = __umul64hi(m, w0) + (t < m * w0 ? 1 : 0) + (p2 < t ? 1 : 0);
-  Step s{p2, p1};
+  uint64_t hi = p2, lo = p1;
   if (e < 0) {   // 2^e of it
     const int r = -e, by = r & 63;
     const uint64_t x0 = r < 64 ? p2 : r < 128 ? p3 : 0, up = r < 64 ? p3 : 0;
     const uint64_t x1 = r < 64 ? p1 : r < 128 ? p2 : r < 192 ? p3 : 0;
-    s.hi = by != 0 ? x0 >> by | up << (64 - by) : x0;
-    s.lo = by != 0 ? x1 >> by | x0 << (64 - by) : x1;
+    hi = by != 0 ? x0 >> by | up << (64 - by) : x0;
+    lo = by != 0 ? x1 >> by | x0 << (64 - by) : x1;
   }
   if (f < 0.0) {
-    s.lo = 0 - s.lo;
-    s.hi = 0 - s.hi - (s.lo != 0 ? 1 : 0);
+    lo = 0 - lo;
+    hi = 0 - hi - (lo != 0 ? 1 : 0);
   }
-  s.lo = (s.lo & ~1ull) | (fabs(f) < 0x1p128 ? 0ull : 1ull);
-  return s;
+  return Step{hi, (uint32_t(lo >> 32) & ~1u) | (fabs(f) < 0x1p128 ? 0u : 1u)};
 }
-// The position's turns, modulo 1, as a 64-bit fraction (within two of its units).
+// The position's turns, modulo 1, as a 64-bit fraction, within 2^-32 of a turn.
 __device__ __forceinline__ uint64_t turns_at(int64_t pos, const Step &s) {
-  return uint64_t(pos) * s.hi + __umul64hi(uint64_t(pos), s.lo) - (pos < 0 ? s.lo : 0);
+  const uint64_t u = uint64_t(pos);
+  const uint64_t low = (u >> 32) * s.lo + __umulhi(uint32_t(u), s.lo);   // u lo / 2^32
+  return u * s.hi + low - (pos < 0 ? uint64_t(s.lo) << 32 : 0);
 }
 // gain times the angle's sine (way -1: the other way round) and cosine.
 __device__ __forceinline__ void sincos_at(int64_t pos, const Step &step, float gain, float way, float &sn, float &cs) {
@@ -138,9 +150,10 @@ __global__ __launch_bounds__(kBlock) void k_rotate(RotArgs a) {
   const int ru = (half + PV - 1) / PV, cu = (a.dh - a.rot + VEC - 1) / VEC, units = ru + cu;
   const int64_t at = (int64_t(blockIdx.x) - s.first) * kBlock + threadIdx.x;
   const int64_t row = at / units;
-  __shared__ Step steps[SHARED ? kSteps : 1];
+  extern __shared__ __align__(16) char lds[];
+  const Steps steps(lds, half);
   if constexpr (SHARED) {
-    for (int i = threadIdx.x; i < half; i += kBlock) steps[i] = turn_step(a.freqs[i]);
+    for (int i = threadIdx.x; i < half; i += kBlock) steps.put(i, turn_step(a.freqs[i]));
     __syncthreads();
   }
   if (row >= s.rows) return;
@@ -168,7 +181,7 @@ __global__ __launch_bounds__(kBlock) void k_rotate(RotArgs a) {
   float sn[PV], cs[PV];
 #pragma unroll
   for (int i = 0; i < PV; ++i)
-    sincos_at(pos, SHARED ? steps[p0 + i] : turn_step(a.freqs[p0 + i]), a.gain, a.way, sn[i], cs[i]);
+    sincos_at(pos, SHARED ? steps.at(p0 + i) : turn_step(a.freqs[p0 + i]), a.gain, a.way, sn[i], cs[i]);
   for (int h = 0; h < s.H; ++h, x += s.sh, y += a.dh) {
     if constexpr (INTER) {
       T v[VEC];
@@ -202,12 +215,13 @@ constexpr int kStretch = 16384 / int(sizeof(T));   // elements of a workgroup's 
 template <typename T, bool INTER>
 __global__ __launch_bounds__(kBlock) void k_rotate_odd(RotArgs a, int tile_rows) {
   __shared__ __align__(16) T tile[kStretch<T>];
-  __shared__ Step steps[kSteps];
+  extern __shared__ __align__(16) char lds[];   // (as much as the pairs take: eight workgroups a CU mostly)
   __shared__ int64_t pos[kStretchRows];
   const int sd = int64_t(blockIdx.x) >= a.side[1].first ? 1 : 0, tid = threadIdx.x;
   const Side &s = a.side[sd];
   const int64_t row0 = (int64_t(blockIdx.x) - s.first) * tile_rows;
   const int rows = int(min(int64_t(tile_rows), s.rows - row0)), width = s.H * a.dh, n = rows * width, half = a.rot / 2;
+  const Steps steps(lds, half);
   const T *x = static_cast<const T *>(s.x) + row0 * width;
   T *y = static_cast<T *>(s.y) + row0 * width;
   constexpr int E = 16 / int(sizeof(T));
@@ -219,8 +233,10 @@ __global__ __launch_bounds__(kBlock) void k_rotate_odd(RotArgs a, int tile_rows)
     }
     for (int i = n / E * E + tid; i < n; i += kBlock) to[i] = from[i];
   };
+  const double f = tid < half ? a.freqs[tid] : 0.0;   // (on its way beside the rows)
   copy(tile, x);
-  for (int i = tid; i < half; i += kBlock) steps[i] = turn_step(a.freqs[i]);
+  if (tid < half) steps.put(tid, turn_step(f));
+  for (int i = tid + kBlock; i < half; i += kBlock) steps.put(i, turn_step(a.freqs[i]));
   for (int i = tid; i < rows; i += kBlock) {
     const int64_t seq = (row0 + i) / s.L, t = row0 + i - seq * s.L;
     pos[i] = s.pos[seq * s.pn + t * s.pt];
@@ -229,7 +245,7 @@ __global__ __launch_bounds__(kBlock) void k_rotate_odd(RotArgs a, int tile_rows)
   for (int i = tid; i < rows * half; i += kBlock) {
     const int r = i / half, p = i - r * half;
     float sn, cs;
-    sincos_at(pos[r], steps[p], a.gain, a.way, sn, cs);
+    sincos_at(pos[r], steps.at(p), a.gain, a.way, sn, cs);
     T *v = tile + r * width + (INTER ? 2 * p : p);
     constexpr int one = INTER ? 1 : 0;
     const int other = one != 0 ? 1 : half;
@@ -256,7 +272,7 @@ int odd_rows(const RotArgs &a) {
 
 template <typename T, int VEC, bool INTER>
 void go(RotArgs a, dim3 grid, hipStream_t stream) {
-  if (a.rot / 2 <= kSteps) launch(&k_rotate<T, VEC, INTER, true>, grid, dim3(kBlock), 0, stream, a);
+  if (a.rot / 2 <= kSteps) launch(&k_rotate<T, VEC, INTER, true>, grid, dim3(kBlock), size_t(a.rot / 2) * kStepBytes, stream, a);
   else launch(&k_rotate<T, VEC, INTER, false>, grid, dim3(kBlock), 0, stream, a);
 }
 template <typename T, bool INTER>
@@ -271,7 +287,7 @@ int run(RotArgs a, hipStream_t stream) {
     }
     if (a.side[1].rows == 0) a.side[1].first = INT64_MAX;
     SGL_REQUIRE(grid < (1 << 24), "rotary: too many rows");
-    launch(&k_rotate_odd<T, INTER>, dim3(unsigned(grid)), dim3(kBlock), 0, stream, a, rows);
+    launch(&k_rotate_odd<T, INTER>, dim3(unsigned(grid)), dim3(kBlock), size_t(half) * kStepBytes, stream, a, rows);
     SGL_CHECK_LAUNCH();
     return SGL_OK;
   }

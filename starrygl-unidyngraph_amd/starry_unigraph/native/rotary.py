@@ -64,7 +64,7 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, q_pos: torch.Tensor, k_pos: 
     other channels as they are. ``k`` and ``k_pos`` may both be None.
 
     ``q_pos``, ``k_pos``: int64 [N, Lq], [N, Lk] (any values: an angle is within
-    2^-63 of a turn at every one). ``freqs``: float64 [P], 2 P <= dh, the angle a
+    2^-32 of a turn at every one). ``freqs``: float64 [P], 2 P <= dh, the angle a
     unit of position of each pair (``frequencies``), under 2^128 (another, as one
     that is not finite, makes its pair NaN); no gradient. Pairs are channels
     (i, i + P), or with ``interleaved`` (2 i, 2 i + 1). Differentiable in q and

@@ -1,10 +1,10 @@
 """Rotary positions far from zero: stamps in seconds to nanoseconds and the ends
 of int64, each channel against the definition with exact angles.
 
-An angle is within 2^-63 of a turn (nothing beside what follows); as a float
-within an eighth of a turn it is off by 3 roundings of 0.79, 2.4 x 2^-24, and by as much
-its sine and cosine, which add 1 x 2^-24; the gain and its product 2, the products
-and sum of a pair 1 and 1.4: 8 x 2^-24 = 2^-21 of gain (|a| + |b|)."""
+An angle is within 2^-32 of a turn (0.03 x 2^-24); as a float within an eighth of a
+turn it is off by 3 roundings of 0.79, 2.4 x 2^-24, and by as much its sine and cosine,
+which add 1 x 2^-24 (0.03 of it their series'); the gain and its product 2, the
+products and sum of a pair 1 and 1.4: 8 x 2^-24 = 2^-21 of gain (|a| + |b|)."""
 import math
 from fractions import Fraction
 
