@@ -344,12 +344,14 @@ struct Line {
 // How the work is cut: waves of a workgroup (32 outer rows each), steps of 32
 // inner rows a tile, workgroups of a launch (all resident) and waves a SIMD.
 // Two waves a SIMD: one's vector work and LDS reads run beside the other's
-// matrix instructions (one wave of 64 rows reads half as much from LDS and
-// took 5 to 12 % longer: 404 us and 360 for 768 x 570,074 x 172 bf16). 16-bit
+// matrix instructions (one wave of 64 rows reads half as much from LDS and took
+// longer: forward and gradient 357 + 502 us for 310 + 402, 768 x 570,074 x 172 bf16). 16-bit
 // types have them in one workgroup, so that a tile is read once for 256 rows;
 // fp32, whose matrix instructions take 16 times as long, in two of 128 rows,
 // which fill up ragged numbers of rows better. fp32 rows of more than 128
-// channels would spill in half the registers (450 us for 412). A step a tile in fp32:
+// channels have one wave a SIMD: 172 channels in half the registers take 419 + 382 us
+// for 400 + 380 at 600 x 100,000 and 514 + 465 for 508 + 478 at 4,000 x 20,000, and 256
+// channels' tiles of two workgroups do not fit a CU's LDS. A step a tile in fp32:
 // more even shares of small problems (200 x 1,000 x 100 16 us for 20 with two, 600 x
 // 20,000 71 for 75, 4,000 x 100,000 1,473 for 1,454).
 template <typename T, int DB>

@@ -322,7 +322,8 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
       loss = INFINITY;
     } else {
       const float konst = a.target != nullptr ? 0.f : a.konst[row];
-      loss = p.temperature * (p.temperature * (konst + kLn2 * (far + want * __builtin_amdgcn_logf(l))));   // (T^2 may be 0)
+      loss = konst + kLn2 * (far + want * __builtin_amdgcn_logf(l));
+      loss = p.temperature * (p.temperature * loss);   // (T^2 may be 0)
       loss = loss < 0.f ? 0.f : loss;   // (rounding: it is not negative)
     }
     a.loss[row] = loss;

@@ -1,9 +1,9 @@
 // The gradient of the table (and of a bias): dw_v = scale sum_n (gl_n e_nv -
 // gq_n q_nv) h_n over the rows, e the forward's exponentials, formed again.
 //
-// 4 N V D operations, bound as the forward is: 4,096 x 570,074 x 172 in bf16 1,575
-// us, 1,020 TFLOP/s; 600 x 100,000 x 172 in fp32 385 us, 107. Few rows: reading the
-// candidates and writing their gradients, 128 x 570,074 x 172 176 us for 392 MB, which
+// 4 N V D operations, bound as the forward is: 4,096 x 570,074 x 172 in bf16 1,600
+// us, 1,000 TFLOP/s; 600 x 100,000 x 172 in fp32 380 us, 109. Few rows: reading the
+// candidates and writing their gradients, 128 x 570,074 x 172 177 us for 392 MB, which
 // the products of a workgroup's next candidates do not cover (two workgroups of
 // half the size a CU: 3 to 7 % less up to 600 rows, 3 to 5 % more from 1,200).
 #include "candidates.h"

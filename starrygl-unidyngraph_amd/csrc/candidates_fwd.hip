@@ -4,11 +4,13 @@
 // One pass over the table: a tile of it gives scores, the running maximum and
 // sum (what was summed is rescaled when the maximum has grown), and the tile's
 // share of sum p w. 2 N V D operations, 4 with sum p w: the matrix unit
-// bounds it, at the rate that the card's power leaves (a large library product
-// 1,099 TFLOP/s in bf16): 4,096 x 570,074 x 172 in bf16 1,557 us, 1,032; rows of
-// 100 channels 786 (7 and 8 steps of 16 are run for 6.25); 600 x 100,000 x 172 in
-// fp32 400 us, 103 of 152. A few rows: the table's bytes, 1 x 1,140,149 x 172 in 72
-// us, 5.4 TB/s.
+// and the vector unit (exponentials, maxima) bound it together, at the clock that
+// the card's power leaves: 4,096 x 570,074 x 172 in bf16 1,558 us, 1,031 TFLOP/s, the
+// matrix unit busy for half and the vector unit for 0.44 of the cycles, at 1.95 GHz of
+// 2.4 (a large library product 1,099 TFLOP/s, 0.7 of the cycles at 1.5 to 1.9 GHz);
+// rows of 100 channels 786 TFLOP/s (7 and 8 steps of 16 are run for 6.25); 600 x 100,000
+// x 172 in fp32 400 us, 103 of 152. A few rows: the table's bytes, 1 x 1,140,149 x 172
+// in 72 us, 5.4 TB/s.
 #include "candidates.h"
 
 namespace {
@@ -109,7 +111,8 @@ __global__ __launch_bounds__(64 * WX * WY, PER_SIMD) void k_forward(FwdArgs a) {
       if (t + 1 < end || u < u1) fetch(t + 1 < end ? t + 1 : 0);   // (the next outer tile's first)
       if (NBUF == 2) buf ^= 1;
       // The loss alone, bound by vector work: in whole tiles without a bias scores get their factor as their
-      // exponentials are taken (4,096 x 570,074 x 172 in bf16 913 us for 1,004; beside sum p w it gains nothing).
+      // exponentials are taken (4,096 x 570,074 in bf16, 172 channels 950 us for 1,085, 64 635 for 650; 4,000 x 50,001
+      // x 100 in fp32 369 for 385; beside sum p w it gains nothing).
       const bool plain = !DIR && !biased && rows >= YT && p.c > 0.f;
       const float by_c = plain ? p.c : 1.f;
 #pragma unroll 1

@@ -10,8 +10,8 @@
 // round.
 //
 // Memory bounds it, every element read and written once: 16 sequences of 8,191
-// x (8 + 2) heads of 128 in fp16 120 us, 5.6 TB/s (a large copy: 5.1); 4,000 x
-// (20 + 32) x 4 heads of 43 in bf16 30 us, 4.7 TB/s; 400 x 1 x 2 heads of 50, one
+// x (8 + 2) heads of 128 in fp16 123 us, 5.5 TB/s (a large copy: 5.1); 4,000 x
+// (20 + 32) x 4 heads of 43 in bf16 34 us, 4.2 TB/s; 400 x 1 x 2 heads of 50, one
 // new event each, 4 us, the launch.
 #include "history.h"
 
@@ -272,7 +272,8 @@ int odd_rows(const RotArgs &a) {
 
 template <typename T, int VEC, bool INTER>
 void go(RotArgs a, dim3 grid, hipStream_t stream) {
-  if (a.rot / 2 <= kSteps) launch(&k_rotate<T, VEC, INTER, true>, grid, dim3(kBlock), size_t(a.rot / 2) * kStepBytes, stream, a);
+  const size_t steps = size_t(a.rot / 2) * kStepBytes;
+  if (a.rot / 2 <= kSteps) launch(&k_rotate<T, VEC, INTER, true>, grid, dim3(kBlock), steps, stream, a);
   else launch(&k_rotate<T, VEC, INTER, false>, grid, dim3(kBlock), 0, stream, a);
 }
 template <typename T, bool INTER>

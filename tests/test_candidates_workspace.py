@@ -11,8 +11,8 @@ from starry_unigraph.lib import _capi
 def _bytes(dtype, dim, n, v, k=1, teacher=0):
     a = ctypes.byref(_capi.Candidates(dtype, dim, n, v, 16, 16, dim, dim, None, 1.0, 1.0))
     lib = _capi.lib()
-    return (lib.sgl_candidates_workspace_bytes(a, k, teacher, 3, 0), lib.sgl_candidates_workspace_bytes(a, k, teacher, 3, 1),
-            lib.sgl_candidates_keep_bytes(a, k, teacher, 3))
+    return (lib.sgl_candidates_workspace_bytes(a, k, teacher, 3, 0),
+            lib.sgl_candidates_workspace_bytes(a, k, teacher, 3, 1), lib.sgl_candidates_keep_bytes(a, k, teacher, 3))
 
 
 @pytest.mark.parametrize("dtype", [0, 1, 2], ids=["fp32", "bf16", "fp16"])

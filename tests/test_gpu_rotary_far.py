@@ -84,7 +84,8 @@ def test_scores_of_stamps_depend_on_distances(ops, gpu):  # noqa: F811
     q, k = (torch.randn(1, 1, 2, 64, generator=g).to(gpu) for _ in range(2))
     scores = []
     for at in (0, 1_700_000_000_123_456_789, -(1 << 62)):
-        a, b = ops.rotate(q, k, torch.tensor([[at + 40_000_000_000]], device=gpu), torch.tensor([[at]], device=gpu), freqs)
+        pos = [torch.tensor([[t]], device=gpu) for t in (at + 40_000_000_000, at)]
+        a, b = ops.rotate(q, k, *pos, freqs)
         scores.append((a.double() * b.double()).sum(-1))
     # each rotated value within 2^-21 of its pair's sizes, 64 products of two of them
     most = float((2.0 ** -20 * 2 * q.norm(dim=-1).double() * k.norm(dim=-1).double()).max())
