@@ -311,13 +311,13 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
   }
   const bool wanted = !(want == 0.f);   // (NaN: a row that its teacher spoils)
   const bool spoilt = mx == -INFINITY && !(l == 0.f);   // (no score but NaN)
-  const bool grad = wanted && out == 0.f && (mx > -INFINITY || spoilt);
+  const bool grad = wanted && out == 0.f;
   if (here && w == 0 && lane == 0) {
     float loss;
     if (!wanted) {
       loss = a.target != nullptr ? (target >= p.V ? NAN : 0.f) : a.konst[row];
-    } else if (mx == -INFINITY) {
-      loss = spoilt ? NAN : 0.f;   // (no live candidate)
+    } else if (mx == -INFINITY) {   // no live candidate, or one is wanted whose score is -inf as every other's is
+      loss = spoilt || out == 0.f ? NAN : 0.f;
     } else if (out != 0.f) {
       loss = INFINITY;
     } else {
