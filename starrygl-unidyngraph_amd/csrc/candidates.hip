@@ -165,7 +165,7 @@ struct Cols {
 template <typename T, int W, int BATCH, bool DIR>
 __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
   __shared__ float parts[kWaves][DIR && W > 1 ? kMaxDim : 1];
-  __shared__ float sums[2][kWaves][3];
+  __shared__ float sums[2][kWaves][4];
   const Problem &p = a.p;
   const int lane = threadIdx.x & 63, wave = attn::wave_index(), w = wave % W;
   const int64_t at = int64_t(blockIdx.x) * (kWaves / W) + wave / W;
@@ -270,8 +270,9 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
   }
   if constexpr (!ROUNDED) lr = l;
 
-  // the targets: sum of q (mx - s), of q, of q w
-  float x[4], tw[4], far = 0.f;
+  // the targets: sum of q (mx - s), of q, of q w; a bias that base 2 takes past float32's range (a mask of its
+  // lowest value) goes into a sum of its own, as it is
+  float x[4], tw[4], far = 0.f, low = 0.f;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     x[j] = c.own[j] ? float(raw[j]) : 0.f;
@@ -294,20 +295,26 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
     for (int i = 0; i < BATCH; ++i) dot[i] = wave_sum(dot[i]);
 #pragma unroll
     for (int i = 0; i < BATCH; ++i)
-      if (lane == i && id >= 0) far += q * (mx - fmaf(dot[i], p.c, b));
+      if (lane == i && id >= 0) {
+        const bool past = b == -FLT_MAX && mx > -0.99f * FLT_MAX;   // (of rows where it is not every candidate's)
+        far += q * (mx - fmaf(dot[i], p.c, past ? 0.f : b));
+        if (past) low -= q * p.bias[id];
+      }
     k0 += W * BATCH;
     if (k0 >= a.K) break;
     ask(k0);
   }
   far = wave_sum(far);
+  low = wave_sum(low);
   want = wave_sum(want);
   out = wave_max(out);
   if constexpr (W > 1) {
-    if (lane == 0) sums[1][wave][0] = far, sums[1][wave][1] = want, sums[1][wave][2] = out;
+    if (lane == 0) sums[1][wave][0] = far, sums[1][wave][1] = want, sums[1][wave][2] = out, sums[1][wave][3] = low;
     __syncthreads();
-    far = want = out = 0.f;
+    far = want = out = low = 0.f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) far += sums[1][i][0], want += sums[1][i][1], out = fmaxf(out, sums[1][i][2]);
+    for (int i = 0; i < W; ++i)
+      far += sums[1][i][0], want += sums[1][i][1], out = fmaxf(out, sums[1][i][2]), low += sums[1][i][3];
   }
   const bool wanted = !(want == 0.f);   // (NaN: a row that its teacher spoils)
   const bool spoilt = mx == -INFINITY && !(l == 0.f);   // (no score but NaN)
@@ -323,7 +330,7 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
     } else {
       const float konst = a.target != nullptr ? 0.f : a.konst[row];
       loss = konst + kLn2 * (far + want * __builtin_amdgcn_logf(l));
-      loss = p.temperature * (p.temperature * loss);   // (T^2 may be 0)
+      loss = p.temperature * (p.temperature * loss + low);   // (T^2 may be 0)
       loss = loss < 0.f ? 0.f : loss;   // (rounding: it is not negative)
     }
     a.loss[row] = loss;
