@@ -33,7 +33,9 @@ __device__ __forceinline__ float wave_max(float v) {
 // q = softmax(z / T) over a row's live entries, one wave a row (the maximum is
 // taken off before the division, which may pass float32's range). Entries of the
 // same candidate are put together in the first of them (the sums over entries
-// are the same), so that a candidate is wanted once. A row without a live
+// are the same), so that a candidate is wanted once; the loss of such a row may be
+// negative, down to `least`: sum q log q over the entries less that over the
+// candidates. A row without a live
 // entry has the constant 0 and no targets, one with an index past the table
 // NaN and none.
 struct TeacherArgs {
@@ -43,7 +45,7 @@ struct TeacherArgs {
   int K;
   float temperature;
   int32_t *ids_out;
-  float *weight, *konst;
+  float *weight, *konst, *least;
 };
 __global__ __launch_bounds__(kBlock) void k_teacher(TeacherArgs a) {
   extern __shared__ __align__(16) char lds[];
@@ -85,6 +87,8 @@ __global__ __launch_bounds__(kBlock) void k_teacher(TeacherArgs a) {
   }
   konst = wave_sum(konst);
   attn::wave_sync();
+  float together = 0.f;   // sum q log q over the candidates
+  bool twice = false;
   for (int k = lane; k < a.K; k += kWave) {
     int id = live_row ? ids[k] : -1;
     float w = 0.f;
@@ -93,10 +97,17 @@ __global__ __launch_bounds__(kBlock) void k_teacher(TeacherArgs a) {
       if (i < k) id = -2;   // put together in an earlier entry (no index is -2)
       else w += q[i];
     }
+    twice |= id == -2 && ids[k] >= 0;
+    if (id >= 0) together += w * logf(w);
     a.ids_out[n * a.K + k] = id < 0 ? -1 : id;
     a.weight[n * a.K + k] = id < 0 ? 0.f : w;
   }
-  if (lane == 0) a.konst[n] = bad ? NAN : live_row ? konst : 0.f;
+  together = wave_sum(together);
+  twice = __any(twice);
+  if (lane == 0) {
+    a.konst[n] = bad ? NAN : live_row ? konst : 0.f;
+    a.least[n] = twice ? konst - together : 0.f;
+  }
 }
 
 // ------------------------------------------------------------------ the rows with a target first
@@ -135,7 +146,7 @@ struct FinishArgs {
   Partials in;
   const int64_t *target;   // [N], or NULL:
   const int32_t *ids;      // [N][K]
-  const float *weight, *konst;
+  const float *weight, *konst, *least;
   int K;
   float *loss, *stat, *dir;   // stat: [2][N] the maximum and 1 / sum (0: no gradient)
   int32_t *ids_out;           // of `target`
@@ -328,10 +339,11 @@ __global__ __launch_bounds__(kBlock) void k_finish(FinishArgs a) {
     } else if (out != 0.f) {
       loss = INFINITY;
     } else {
-      const float konst = a.target != nullptr ? 0.f : a.konst[row];
+      const float konst = a.target != nullptr ? 0.f : a.konst[row], least = a.target != nullptr ? 0.f : a.least[row];
       loss = konst + kLn2 * (far + want * __builtin_amdgcn_logf(l));
       loss = p.temperature * (p.temperature * loss + low);   // (T^2 may be 0)
-      loss = loss < 0.f ? 0.f : loss;   // (rounding: it is not negative)
+      const float bound = p.temperature * (p.temperature * least);
+      loss = loss < bound ? bound : loss;   // (rounding: it is not under it)
     }
     a.loss[row] = loss;
     if (a.stat != nullptr) {
@@ -474,7 +486,7 @@ bool orders(int64_t N) { return N >= kOrderLeast && N <= kOrderMost; }
 
 // What the backward reads of the forward (and the forward's own steps of each other).
 struct Keep {
-  float *stat, *dir, *weight, *konst;
+  float *stat, *dir, *weight, *konst, *least;
   int32_t *ids, *order;
 };
 constexpr int32_t kNeedRows = 1, kNeedTable = 2;
@@ -488,6 +500,7 @@ Keep carve_keep(void *keep, const Problem &p, int K, bool teacher, int32_t need,
   if (teacher) {
     k.weight = c.take<float>(e);
     k.konst = c.take<float>(n);
+    k.least = c.take<float>(n);
   } else if (orders(p.N)) {
     k.order = c.take<int32_t>(n + 1);
   }
@@ -574,7 +587,8 @@ extern "C" int sgl_candidates_forward(const sgl_candidates *problem, const int64
   const Partials part = carve_forward(workspace, problem->dtype, p, (need & kNeedRows) != 0, &room);
   if (const int rc = check_room("workspace", workspace, workspace_bytes, room)) return rc;
   if (teacher) {
-    const TeacherArgs a{ids, logits, p.N, p.V, k, p.temperature, kept.ids, kept.weight, kept.konst};
+    const TeacherArgs a{ids, logits, p.N, p.V, k, p.temperature, kept.ids, kept.weight, kept.konst,
+                        kept.least};
     sgl::launch(&k_teacher, dim3(unsigned((p.N + kWaves - 1) / kWaves)), dim3(kBlock), size_t(kWaves) * 8 * size_t(k),
                 stream, a);
   } else if (kept.order != nullptr) {
@@ -583,8 +597,8 @@ extern "C" int sgl_candidates_forward(const sgl_candidates *problem, const int64
   }
   const Order o{kept.order, kept.order != nullptr ? kept.order + p.N : nullptr};
   forward_partials(problem->dtype, p, o, part, stream);
-  const FinishArgs a{p,           o, part, target,    teacher ? kept.ids : nullptr, kept.weight, kept.konst, k, loss,
-                     kept.stat, kept.dir, teacher ? nullptr : kept.ids};
+  const FinishArgs a{p,           o, part, target,    teacher ? kept.ids : nullptr, kept.weight, kept.konst, kept.least, k,
+                     loss, kept.stat, kept.dir, teacher ? nullptr : kept.ids};
   if (problem->dtype == SGL_FP32) finish<float>(a, stream);
   else if (problem->dtype == SGL_BF16) finish<bf16_t>(a, stream);
   else finish<fp16_t>(a, stream);

@@ -62,8 +62,9 @@ def distillation(h: torch.Tensor, table: torch.Tensor, ids: torch.Tensor, logits
 
     ``h``, ``table``, ``bias`` and ``scale`` as in :func:`cross_entropy`.
     ``ids``: int64 [..., K], K up to 1024, the teacher's candidates in any order
-    (negative: no entry; the same one twice: two entries); ``logits``: float32
-    [..., K], without gradient (-inf: no entry). A row without an entry has
+    (negative: no entry; the same one twice: two entries, with which the sum may
+    be negative); ``logits``: float32 [..., K], without gradient (-inf: no entry,
+    whatever its id). A row without an entry has
     loss 0 and no gradient; one with an id of V or more NaN and none; one that
     wants a candidate that is left out inf and none. Differentiable in h, table and
     bias."""

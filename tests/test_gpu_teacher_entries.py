@@ -58,3 +58,28 @@ def test_loss_at_temperatures_whose_square_is_lost(ops, gpu, T):  # noqa: F811
         got = ops.distillation(h.to(gpu), w.to(gpu), ids.to(gpu), z.to(gpu), temperature=T).cpu().double()
     assert bool((want["loss"] > 100 * bound["loss"]).all())
     assert bool(((got - want["loss"]).abs() <= bound["loss"]).all())
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("N,V,K,T", [(3, 1, 2, 1.0), (40, 1, 20, 2.0), (300, 2, 7, 0.5), (40, 2, 33, 1.0), (5000, 3, 4, 1.0)])
+def test_entries_of_one_candidate_where_it_has_nearly_all(ops, gpu, N, V, K, T, dtype):  # noqa: F811
+    """Each entry counts by itself: sum q (log q - log p) is negative where p exceeds its parts of q."""
+    g, h, w, b, go = _inputs(N + K, N, V, 32, dtype, True)
+    b *= 6.0
+    ids, z = torch.randint(0, V, (N, K), generator=g), _rand(g, N, K, std=2.0)
+    ids[0] = 0
+    want, bound = co.loss(h, w, *co.teacher(ids, z, T), go, b, temperature=T)
+    leaves = [x.to(gpu).requires_grad_() for x in (h, w, b)]
+    loss = ops.distillation(leaves[0], leaves[1], ids.to(gpu), z.to(gpu), bias=leaves[2], temperature=T)
+    assert bool((want["loss"] < -0.05).any())
+    _check(loss, leaves, go, want, bound)
+
+
+def test_a_matched_teacher_of_one_entry_each_is_not_under_zero(ops, gpu):  # noqa: F811
+    """Without an entry given twice the divergence is 0 or more, rounding or not."""
+    g, h, w, b, go = _inputs(1, 400, 6, 32, FP32, False)
+    z = (h.double() @ w.double().t()).float()
+    ids = torch.arange(6).expand(400, 6)
+    with torch.no_grad():
+        loss = ops.distillation(h.to(gpu), w.to(gpu), ids.to(gpu), z.to(gpu))
+    assert bool((loss >= 0).all()) and float(loss.max()) < 1e-5
