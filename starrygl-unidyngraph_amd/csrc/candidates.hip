@@ -597,8 +597,9 @@ extern "C" int sgl_candidates_forward(const sgl_candidates *problem, const int64
   }
   const Order o{kept.order, kept.order != nullptr ? kept.order + p.N : nullptr};
   forward_partials(problem->dtype, p, o, part, stream);
-  const FinishArgs a{p,           o, part, target,    teacher ? kept.ids : nullptr, kept.weight, kept.konst, kept.least, k,
-                     loss, kept.stat, kept.dir, teacher ? nullptr : kept.ids};
+  const FinishArgs a{p,          o,          part,       target, teacher ? kept.ids : nullptr,
+                     kept.weight, kept.konst, kept.least, k,      loss,
+                     kept.stat,   kept.dir,   teacher ? nullptr : kept.ids};
   if (problem->dtype == SGL_FP32) finish<float>(a, stream);
   else if (problem->dtype == SGL_BF16) finish<bf16_t>(a, stream);
   else finish<fp16_t>(a, stream);

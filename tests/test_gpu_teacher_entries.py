@@ -61,7 +61,8 @@ def test_loss_at_temperatures_whose_square_is_lost(ops, gpu, T):  # noqa: F811
 
 
 @pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
-@pytest.mark.parametrize("N,V,K,T", [(3, 1, 2, 1.0), (40, 1, 20, 2.0), (300, 2, 7, 0.5), (40, 2, 33, 1.0), (5000, 3, 4, 1.0)])
+@pytest.mark.parametrize("N,V,K,T", [(3, 1, 2, 1.0), (40, 1, 20, 2.0), (300, 2, 7, 0.5), (40, 2, 33, 1.0),
+                                     (5000, 3, 4, 1.0)])
 def test_entries_of_one_candidate_where_it_has_nearly_all(ops, gpu, N, V, K, T, dtype):  # noqa: F811
     """Each entry counts by itself: sum q (log q - log p) is negative where p exceeds its parts of q."""
     g, h, w, b, go = _inputs(N + K, N, V, 32, dtype, True)
